@@ -20,6 +20,8 @@ DS_CHAIN_ONE_LAUNCH = 0x200
 DS_CHAIN_LAUNCH_PER_LAYER = 0x400
 DS_CHAIN_CONTROL_BYTES = 12288
 DS_CHAIN_STATUS_AT = 1536
+DS_F32, DS_BF16, DS_F16 = 0, 1, 2
+DS_NONE, DS_SUM, DS_MEAN = 0, 1, 2
 
 _c_int = ctypes.c_int
 _c_i64 = ctypes.c_int64
@@ -43,6 +45,16 @@ class ChainLayer(ctypes.Structure):
 
 
 _clp = ctypes.POINTER(ChainLayer)
+
+
+class Tensor(ctypes.Structure):
+    """``ds_tensor`` of the header: one tensor of a clipping call."""
+    _fields_ = [("src", _ptr), ("dst", _ptr), ("n", _c_i64), ("src_type", _c_int), ("dst_type", _c_int)]
+
+
+_tp = ctypes.POINTER(Tensor)
+_float = ctypes.c_float
+_matrix = [_ptr, _c_i64]   # an operand and the distance of its rows
 
 # name -> (restype, argtypes); mirrors include/deepshift_hip.h one to one
 SIGNATURES = {
@@ -107,6 +119,15 @@ SIGNATURES = {
     "ds_mul_tile_weights_f32": (_c_int, [_ptr, _ptr] + [_c_int] * 4 + [_ptr]),
     "ds_mul_conv2d_f32": (_c_int, [_ptr] * 4 + [_c_int] * 9 + [_ptr]),
     "ds_mul_linear_f32": (_c_int, [_ptr, _c_int, _ptr, _ptr, _ptr] + [_c_int] * 3 + [_ptr]),
+    "ds_embed": (_c_int, [_ptr, _c_int] + _matrix + [_ptr, _c_i64, _c_i64, _c_i64, _float, _c_int, _ptr]),
+    "ds_embed_grad_workspace_bytes": (_size, [_c_i64, _c_i64]),
+    "ds_embed_grad": (_c_int, [_ptr, _c_int] + _matrix + [_ptr] + [_c_i64] * 4 + [_float, _c_int, _ptr, _size, _ptr]),
+    "ds_vocab_workspace_bytes": (_size, _matrix * 2 + [_c_i64] * 3 + [_c_int, _c_int]),
+    "ds_vocab_loss": (_c_int, _matrix * 2 + [_ptr, _ptr, _c_int] + [_c_i64] * 4 + [_c_int, _c_int, _ptr, _ptr, _ptr, _ptr,
+                                                                                   _size, _ptr]),
+    "ds_vocab_loss_grad": (_c_int, _matrix * 2 + [_ptr, _ptr, _c_int] + [_c_i64] * 4 + [_c_int] + [_ptr] * 8 + [_size, _ptr]),
+    "ds_clip_workspace_bytes": (_size, [_c_int]),
+    "ds_clip": (_c_int, [_tp, _c_int, _float, _c_int, _ptr, _ptr, _size, _ptr]),
     "ds_valu_calibrate": (_c_int, [_ptr, _c_int, _c_int, _ptr]),
     "ds_copy_i32": (_c_int, [_ptr, _ptr, _c_i64, _ptr]),
     "ds_test_tune": (_c_int, [ctypes.c_char_p, _c_int]),

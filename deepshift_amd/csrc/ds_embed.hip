@@ -1,0 +1,469 @@
+// Embedding lookup with scaling, and its gradient by sorted tokens.
+//
+//   out[t][:] = scale * W[id_t][:]             dW[v][:] = scale * sum over { t : id_t = v, v != padding } of g[t][:]
+//
+// Both only move data.  The sum of a word's gradients runs over its tokens in ascending order, in 32 bits, and is rounded
+// once: the tokens are sorted by word (stably), so no atomics touch the sums and a call repeats bit for bit.
+#include "ds_train.h"
+
+namespace ds {
+
+// ---- lookup ------------------------------------------------------------------------------------------------
+
+constexpr int kLookupUnits = 4;  // accesses a thread has in flight
+
+// A workgroup takes 256 * kLookupUnits consecutive accesses of the result; row and column of its first one are the only
+// 64-bit division.
+template <typename E, int N>
+__global__ __launch_bounds__(256) void embed_kernel(const void *__restrict__ ids, int wide, const E *__restrict__ w,
+                                                    E *__restrict__ out, int64_t T, int64_t V, int64_t ldw, float scale,
+                                                    uint32_t per_row, FastDiv by_row)
+{
+    const uint64_t first = (uint64_t)blockIdx.x * (256 * kLookupUnits);
+    const uint64_t row0 = first / per_row;
+    const uint32_t rem0 = (uint32_t)(first - row0 * per_row);
+    Vec<E, N> got[kLookupUnits];
+    int id[kLookupUnits];
+#pragma unroll
+    for (int j = 0; j < kLookupUnits; ++j) {
+        const uint32_t local = rem0 + j * 256 + threadIdx.x;
+        const uint32_t r = div_by(local, by_row);
+        const int64_t t = (int64_t)row0 + r;
+        id[j] = t < T ? token_at(ids, wide, t, V) : -1;
+        if (id[j] >= 0)
+            got[j] = ((const Vec<E, N> *)(w + (int64_t)id[j] * ldw))[local - r * per_row];
+    }
+#pragma unroll
+    for (int j = 0; j < kLookupUnits; ++j) {
+        const uint64_t at = first + j * 256 + threadIdx.x;
+        if (at >= (uint64_t)T * per_row) continue;
+        Vec<E, N> o;
+#pragma unroll
+        for (int e = 0; e < N; ++e) o.v[e] = from_float<E>(id[j] >= 0 ? to_float(got[j].v[e]) * scale : NAN);
+        ((Vec<E, N> *)out)[at] = o;
+    }
+}
+
+template <typename E>
+int launch_embed(const void *ids, int wide, const void *w, void *out, int64_t T, int64_t V, int64_t D, int64_t ldw,
+                 float scale, hipStream_t st)
+{
+    const int n = vector_elements(sizeof(E), {D, ldw}, {w, out});
+    const uint64_t per_row = (uint64_t)(D / n), blocks = ((uint64_t)T * per_row + 256 * kLookupUnits - 1) / (256 * kLookupUnits);
+    if (per_row > 0x7fffffffull - 256 * kLookupUnits || blocks > 0x7fffffffull) return DS_ETOOLARGE;
+    const FastDiv by_row = fast_div((uint32_t)per_row);
+#define DS_LAUNCH(N)                                                                                                    \
+    hipLaunchKernelGGL((embed_kernel<E, N>), dim3((unsigned)blocks), dim3(256), 0, st, ids, wide, (const E *)w, (E *)out, \
+                       T, V, ldw, scale, (uint32_t)per_row, by_row)
+    if (n == 8) { if constexpr (sizeof(E) == 2) DS_LAUNCH(8); }
+    else if (n == 4) DS_LAUNCH(4);
+    else if (n == 2) DS_LAUNCH(2);
+    else DS_LAUNCH(1);
+#undef DS_LAUNCH
+    return launch_status();
+}
+
+// ---- tokens sorted by word ------------------------------------------------------------------------------------
+
+constexpr uint32_t kNoWord = 0xffffffffu;  // sorts behind every word: padding, and what is no word at all
+
+__device__ __forceinline__ uint32_t key_at(const void *ids, int wide, int64_t i, int64_t V, int64_t padding)
+{
+    const int id = token_at(ids, wide, i, V);
+    return id < 0 || id == padding ? kNoWord : (uint32_t)id;
+}
+
+// Up to kRankMost tokens: the place of a token is the number of tokens with a smaller word, or the same word and an earlier
+// position.  Every workgroup holds all words in LDS and places 64 tokens, its 16 waves each compare them with a sixteenth:
+// T * T comparisons, two instructions each.
+constexpr int kRankMost = 16384;
+
+__global__ __launch_bounds__(1024) void embed_rank_kernel(const void *__restrict__ ids, int wide, int T, int64_t V,
+                                                          int64_t padding, uint32_t *__restrict__ keys,
+                                                          uint32_t *__restrict__ pos)
+{
+    __shared__ uint32_t word[kRankMost + 64];
+    __shared__ uint32_t before[16][64];
+    const int padded = (T + 63) & ~63;
+    for (int i = threadIdx.x; i < padded; i += 1024) word[i] = i < T ? key_at(ids, wide, i, V, padding) : kNoWord;
+    __syncthreads();
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, t0 = blockIdx.x * 64;
+    const uint32_t mine = word[t0 + lane];
+    uint32_t n = 0;
+    for (int g = wave * 64; g < padded; g += 16 * 64) {
+        if (g == t0) {
+            for (int i = 0; i < 64; ++i) n += word[g + i] < mine || (word[g + i] == mine && i < lane);
+        } else if (g < t0) {
+            // earlier positions come first among equals
+#pragma unroll 16
+            for (int i = 0; i < 64; ++i) n += word[g + i] <= mine;
+        } else {
+#pragma unroll 16
+            for (int i = 0; i < 64; ++i) n += word[g + i] < mine;
+        }
+    }
+    before[wave][lane] = n;
+    __syncthreads();
+    if (wave == 0 && t0 + lane < T) {
+        uint32_t place = 0;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) place += before[i][lane];
+        keys[place] = mine;
+        pos[place] = t0 + lane;
+    }
+}
+
+// More tokens: a radix sort, least significant digit first, 9 bits a pass.  At most kSortBlocks workgroups, each with one
+// stretch of the tokens; the counts of all of them (512 digits x 64) are few enough that every workgroup adds up its own
+// offsets, so a pass is two launches.
+constexpr int kDigitBits = 9, kDigits = 1 << kDigitBits, kSortBlocks = 64, kSortTile = 2048;
+
+struct SortPass {
+    const void *ids;  // first pass: the token numbers themselves; NULL later
+    int wide;
+    int64_t V, padding;
+    const uint32_t *keys, *pos;
+    uint32_t *out_keys, *out_pos;
+    uint32_t *counts;  // [kDigits][blocks]
+    int64_t T, stretch;
+    int shift;
+};
+
+__device__ __forceinline__ uint32_t sort_key(const SortPass &p, int64_t i)
+{
+    return p.ids ? key_at(p.ids, p.wide, i, p.V, p.padding) : p.keys[i];
+}
+
+__global__ __launch_bounds__(256) void embed_count_kernel(SortPass p)
+{
+    __shared__ uint32_t count[kDigits];
+    for (int d = threadIdx.x; d < kDigits; d += 256) count[d] = 0;
+    __syncthreads();
+    const int64_t from = blockIdx.x * p.stretch, to = min(p.T, from + p.stretch);
+    for (int64_t i = from + threadIdx.x; i < to; i += 256)
+        atomicAdd(&count[(sort_key(p, i) >> p.shift) & (kDigits - 1)], 1u);  // whole numbers: any order gives the same
+    __syncthreads();
+    for (int d = threadIdx.x; d < kDigits; d += 256) p.counts[d * gridDim.x + blockIdx.x] = count[d];
+}
+
+__global__ __launch_bounds__(256) void embed_scatter_kernel(SortPass p)
+{
+    constexpr int kItems = kSortTile / 256;
+    __shared__ uint32_t base[kDigits];      // where the next key of each digit goes
+    __shared__ uint32_t seen[4][kDigits];   // keys of each digit that each wave has had in this tile
+    __shared__ uint32_t wave_sum[4];
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    {
+        // two neighbouring digits a thread: totals, then an exclusive scan over the 512 digits
+        uint32_t total[2], mine[2];
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+            const uint32_t *c = p.counts + (threadIdx.x * 2 + k) * gridDim.x;
+            total[k] = mine[k] = 0;
+            for (unsigned b = 0; b < gridDim.x; ++b) {
+                const uint32_t v = c[b];
+                total[k] += v;
+                mine[k] += b < blockIdx.x ? v : 0;
+            }
+        }
+        const uint32_t own = total[0] + total[1];
+        uint32_t run = own;
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) {
+            const uint32_t up = __shfl_up(run, o);
+            run += lane >= o ? up : 0;
+        }
+        if (lane == 63) wave_sum[wave] = run;
+        __syncthreads();
+        uint32_t front = run - own;
+        for (int w = 0; w < wave; ++w) front += wave_sum[w];
+        base[threadIdx.x * 2] = front + mine[0];
+        base[threadIdx.x * 2 + 1] = front + total[0] + mine[1];
+    }
+    const int64_t from = blockIdx.x * p.stretch, to = min(p.T, from + p.stretch);
+    for (int64_t tile = from; tile < to; tile += kSortTile) {
+        for (int i = threadIdx.x; i < 4 * kDigits; i += 256) (&seen[0][0])[i] = 0;
+        __syncthreads();
+        // a wave has a contiguous quarter of the tile, 64 keys at a time
+        uint32_t key[kItems], at[kItems], rank[kItems];
+#pragma unroll
+        for (int j = 0; j < kItems; ++j) {
+            const int64_t i = tile + wave * (kSortTile / 4) + j * 64 + lane;
+            const bool valid = i < to;
+            key[j] = valid ? sort_key(p, i) : kNoWord;
+            at[j] = valid ? (p.ids ? (uint32_t)i : p.pos[i]) : 0;
+            const uint32_t digit = (key[j] >> p.shift) & (kDigits - 1);
+            // the lanes that hold the same digit, counting only real keys
+            uint64_t same = __ballot(valid);
+#pragma unroll
+            for (int b = 0; b < kDigitBits; ++b) {
+                const uint64_t set = __ballot((digit >> b) & 1);
+                same &= (digit >> b) & 1 ? set : ~set;
+            }
+            const uint32_t earlier = seen[wave][digit];  // one wave, program order: read by all before the first lane adds
+            __builtin_amdgcn_wave_barrier();
+            const uint32_t lower = __popcll(same & ((1ull << lane) - 1));
+            rank[j] = earlier + lower;
+            if (valid && lower == 0) seen[wave][digit] = earlier + (uint32_t)__popcll(same);
+            __builtin_amdgcn_wave_barrier();
+        }
+        __syncthreads();
+#pragma unroll
+        for (int j = 0; j < kItems; ++j) {
+            const int64_t i = tile + wave * (kSortTile / 4) + j * 64 + lane;
+            if (i >= to) continue;
+            const uint32_t digit = (key[j] >> p.shift) & (kDigits - 1);
+            uint32_t place = base[digit] + rank[j];
+            for (int w = 0; w < wave; ++w) place += seen[w][digit];
+            p.out_keys[place] = key[j];
+            p.out_pos[place] = at[j];
+        }
+        __syncthreads();
+        for (int d = threadIdx.x; d < kDigits; d += 256) base[d] += seen[0][d] + seen[1][d] + seen[2][d] + seen[3][d];
+        __syncthreads();
+    }
+}
+
+// ---- sums ------------------------------------------------------------------------------------------------------
+
+// The sorted tokens are cut into chunks; a wave adds up one chunk for 64 * N columns.  A word whose tokens lie in one chunk
+// is finished there.  One that runs on leaves a partial sum: in slot 1 of the chunk that it begins in, in slot 0 of the
+// others; embed_finish_kernel joins them in order.
+template <typename E, int N>
+__global__ __launch_bounds__(64) void embed_sum_kernel(const E *__restrict__ g, int64_t ldg, const uint32_t *__restrict__ keys,
+                                                       const uint32_t *__restrict__ pos, E *__restrict__ dw,
+                                                       float *__restrict__ part, int64_t T, int64_t D, int chunk, float scale)
+{
+    const int64_t from = (int64_t)blockIdx.x * chunk, to = min(T, from + chunk);
+    const int64_t col = ((int64_t)blockIdx.y * 64 + threadIdx.x) * N;
+    const bool in = col < D;
+    const uint32_t before = from > 0 ? keys[from - 1] : kNoWord;
+    const uint32_t behind = to < T ? keys[to] : kNoWord;
+    float acc[N];
+#pragma unroll
+    for (int e = 0; e < N; ++e) acc[e] = 0.f;
+    uint32_t run = keys[from];
+    bool first = true;
+    constexpr int kAhead = 8;  // rows on their way
+    for (int64_t i = from; i < to; i += kAhead) {
+        Vec<E, N> got[kAhead];
+        uint32_t key[kAhead];
+#pragma unroll
+        for (int j = 0; j < kAhead; ++j) {
+            const bool real = i + j < to;
+            key[j] = real ? keys[i + j] : kNoWord;
+            if (real && key[j] != kNoWord && in) got[j] = *(const Vec<E, N> *)(g + (int64_t)pos[i + j] * ldg + col);
+        }
+#pragma unroll
+        for (int j = 0; j < kAhead; ++j) {
+            if (i + j >= to) break;
+            if (key[j] != run) {
+                // the run ends inside this chunk
+                if (run != kNoWord && in) {
+                    if (first && run == before) {
+#pragma unroll
+                        for (int e = 0; e < N; ++e) part[(int64_t)blockIdx.x * 2 * D + col + e] = acc[e];
+                    } else {
+                        Vec<E, N> o;
+#pragma unroll
+                        for (int e = 0; e < N; ++e) o.v[e] = from_float<E>(acc[e] * scale);
+                        *(Vec<E, N> *)(dw + (int64_t)run * D + col) = o;
+                    }
+                }
+                first = false;
+                run = key[j];
+#pragma unroll
+                for (int e = 0; e < N; ++e) acc[e] = 0.f;
+            }
+            if (run == kNoWord || !in) continue;
+#pragma unroll
+            for (int e = 0; e < N; ++e) acc[e] += to_float(got[j].v[e]);
+        }
+    }
+    if (run == kNoWord || !in) return;
+    const bool came = first && run == before, goes = run == behind;
+    if (came || goes) {
+#pragma unroll
+        for (int e = 0; e < N; ++e) part[((int64_t)blockIdx.x * 2 + (came ? 0 : 1)) * D + col + e] = acc[e];
+    } else {
+        Vec<E, N> o;
+#pragma unroll
+        for (int e = 0; e < N; ++e) o.v[e] = from_float<E>(acc[e] * scale);
+        *(Vec<E, N> *)(dw + (int64_t)run * D + col) = o;
+    }
+}
+
+// Every row that embed_sum_kernel has not finished: words without tokens get zeros, words in several chunks their joined
+// sums.  A workgroup owns `rows` rows (at most 256) and finds where their tokens begin by bisection, a thread per row.
+template <typename E, int N>
+__global__ __launch_bounds__(256) void embed_finish_kernel(const uint32_t *__restrict__ keys, const float *__restrict__ part,
+                                                           E *__restrict__ dw, int64_t T, int64_t V, int64_t D, int chunk,
+                                                           int rows, float scale)
+{
+    __shared__ uint32_t begin[257];
+    const int64_t v0 = (int64_t)blockIdx.x * rows;
+    const int mine = (int)min((int64_t)rows, V - v0);
+    for (int i = threadIdx.x; i <= mine; i += 256) {
+        const uint32_t v = (uint32_t)(v0 + i);
+        uint32_t lo = 0, hi = (uint32_t)T;
+        while (lo < hi) {
+            const uint32_t mid = (lo + hi) >> 1;
+            if (keys[mid] < v) lo = mid + 1;
+            else hi = mid;
+        }
+        begin[i] = lo;
+    }
+    __syncthreads();
+    const int64_t per_row = D / N;
+    for (int r = 0; r < mine; ++r) {
+        const uint32_t from = begin[r], to = begin[r + 1];
+        const uint32_t c0 = from / chunk, c1 = to > from ? (to - 1) / chunk : c0;
+        if (to > from && c0 == c1) continue;
+        E *row = dw + (v0 + r) * D;
+        for (int64_t u = threadIdx.x; u < per_row; u += 256) {
+            float acc[N];
+#pragma unroll
+            for (int e = 0; e < N; ++e) acc[e] = 0.f;
+            if (to > from) {
+                const float *p = part + u * N;
+#pragma unroll
+                for (int e = 0; e < N; ++e) acc[e] = p[((int64_t)c0 * 2 + 1) * D + e];
+#pragma unroll 8
+                for (uint32_t c = c0 + 1; c <= c1; ++c)
+#pragma unroll
+                    for (int e = 0; e < N; ++e) acc[e] += p[(int64_t)c * 2 * D + e];
+            }
+            Vec<E, N> o;
+#pragma unroll
+            for (int e = 0; e < N; ++e) o.v[e] = from_float<E>(acc[e] * scale);
+            ((Vec<E, N> *)row)[u] = o;
+        }
+    }
+}
+
+// Tokens a chunk: long ones leave hot words fewer partial sums to join, short ones more waves.
+inline int embed_chunk(int64_t T) { return T <= 4096 ? 16 : T <= 32768 ? 32 : T <= 131072 ? 64 : 128; }
+
+struct EmbedSpace {
+    size_t keys[2], pos[2], counts, part, bytes;
+};
+inline EmbedSpace embed_space(int64_t T, int64_t D)
+{
+    EmbedSpace s;
+    const size_t list = align_up((size_t)T * 4, 256);
+    size_t at = 0;
+    for (int i = 0; i < 2; ++i) {
+        s.keys[i] = at, at += list;
+        s.pos[i] = at, at += list;
+    }
+    s.counts = at, at += (size_t)kDigits * kSortBlocks * 4;
+    const int64_t chunks = (T + embed_chunk(T) - 1) / embed_chunk(T);
+    s.part = at, at += align_up((size_t)chunks * 2 * (size_t)D * 4, 256);
+    s.bytes = at;
+    return s;
+}
+
+template <typename E>
+int launch_embed_grad(const uint32_t *keys, const uint32_t *pos, const void *g, int64_t ldg, void *dw, float *part, int64_t T,
+                      int64_t V, int64_t D, float scale, hipStream_t st)
+{
+    const int n = vector_elements(sizeof(E), {D, ldg}, {g, dw});
+    const int chunk = embed_chunk(T);
+    const int64_t chunks = (T + chunk - 1) / chunk, slices = (D / n + 63) / 64;
+    // about 16 KB of the result a workgroup
+    const int64_t row_bytes = D * (int64_t)sizeof(E);
+    const int rows = (int)min((int64_t)256, max((int64_t)1, (int64_t)16384 / row_bytes));
+    const int64_t finish = (V + rows - 1) / rows;
+    if (chunks > 0x7fffffff || slices > 65535 || finish > 0x7fffffff) return DS_ETOOLARGE;
+#define DS_LAUNCH(N)                                                                                                    \
+    do {                                                                                                                \
+        if (T > 0)                                                                                                      \
+            hipLaunchKernelGGL((embed_sum_kernel<E, N>), dim3((unsigned)chunks, (unsigned)slices), dim3(64), 0, st,     \
+                               (const E *)g, ldg, keys, pos, (E *)dw, part, T, D, chunk, scale);                        \
+        hipLaunchKernelGGL((embed_finish_kernel<E, N>), dim3((unsigned)finish), dim3(256), 0, st, keys, part, (E *)dw, T, V, \
+                           D, chunk, rows, scale);                                                                      \
+    } while (0)
+    if (n == 8) { if constexpr (sizeof(E) == 2) DS_LAUNCH(8); }
+    else if (n == 4) DS_LAUNCH(4);
+    else if (n == 2) DS_LAUNCH(2);
+    else DS_LAUNCH(1);
+#undef DS_LAUNCH
+    return launch_status();
+}
+
+int sort_tokens(const void *ids, int wide, int64_t T, int64_t V, int64_t padding, char *ws, const EmbedSpace &s,
+                hipStream_t st, const uint32_t **keys, const uint32_t **pos)
+{
+    uint32_t *k[2] = {(uint32_t *)(ws + s.keys[0]), (uint32_t *)(ws + s.keys[1])};
+    uint32_t *p[2] = {(uint32_t *)(ws + s.pos[0]), (uint32_t *)(ws + s.pos[1])};
+    int at = 0;
+    if (T <= kRankMost && g_tune.embed_radix != 1) {
+        if (T > 0)
+            hipLaunchKernelGGL(embed_rank_kernel, dim3((unsigned)((T + 63) / 64)), dim3(1024), 0, st, ids, wide, (int)T, V,
+                               padding, k[0], p[0]);
+    } else if (T > 0) {
+        // kNoWord has every bit set: one value more than the words need
+        int bits = 1;
+        while (((int64_t)1 << bits) <= V) ++bits;
+        int64_t blocks = min((int64_t)kSortBlocks, (T + kSortTile - 1) / kSortTile);
+        const int64_t stretch = ((T + blocks - 1) / blocks + kSortTile - 1) / kSortTile * kSortTile;
+        blocks = (T + stretch - 1) / stretch;
+        SortPass pass{ids, wide, V, padding, nullptr, nullptr, k[0], p[0], (uint32_t *)(ws + s.counts), T, stretch, 0};
+        for (int shift = 0; shift < bits; shift += kDigitBits) {
+            pass.shift = shift;
+            if (shift > 0) {
+                pass.ids = nullptr;
+                pass.keys = k[at], pass.pos = p[at];
+                at ^= 1;
+                pass.out_keys = k[at], pass.out_pos = p[at];
+            }
+            hipLaunchKernelGGL(embed_count_kernel, dim3((unsigned)blocks), dim3(256), 0, st, pass);
+            hipLaunchKernelGGL(embed_scatter_kernel, dim3((unsigned)blocks), dim3(256), 0, st, pass);
+        }
+    }
+    *keys = k[at], *pos = p[at];
+    return launch_status();
+}
+
+}  // namespace ds
+
+using namespace ds;
+
+DS_EXPORT int ds_embed(const void *ids, int id_bytes, const void *weight, int64_t ldw, void *out, int64_t T, int64_t V,
+                       int64_t D, float scale, int type, ds_stream_t stream)
+{
+    if (T < 0 || V < 0 || D < 0 || !element_bytes(type) || (id_bytes != 4 && id_bytes != 8)) return DS_EINVAL;
+    if (T == 0 || D == 0) return DS_OK;
+    if (!ids || !out || (V > 0 && (!weight || ldw < D))) return DS_EINVAL;
+    if (V > 0x7fffffff || T > 0x7fffffff) return DS_ETOOLARGE;
+    const int wide = id_bytes == 8;
+    hipStream_t st = (hipStream_t)stream;
+    if (type == DS_F32) return launch_embed<float>(ids, wide, weight, out, T, V, D, ldw, scale, st);
+    if (type == DS_BF16) return launch_embed<bf16_t>(ids, wide, weight, out, T, V, D, ldw, scale, st);
+    return launch_embed<f16_t>(ids, wide, weight, out, T, V, D, ldw, scale, st);
+}
+
+DS_EXPORT size_t ds_embed_grad_workspace_bytes(int64_t T, int64_t D)
+{
+    return T < 0 || D < 0 ? 0 : embed_space(T, D).bytes;
+}
+
+DS_EXPORT int ds_embed_grad(const void *ids, int id_bytes, const void *grad, int64_t ldg, void *dweight, int64_t T, int64_t V,
+                            int64_t D, int64_t padding, float scale, int type, void *workspace, size_t workspace_bytes,
+                            ds_stream_t stream)
+{
+    if (T < 0 || V < 0 || D < 0 || !element_bytes(type) || (id_bytes != 4 && id_bytes != 8)) return DS_EINVAL;
+    if (V == 0 || D == 0) return DS_OK;
+    if (!dweight || (T > 0 && (!ids || !grad || ldg < D))) return DS_EINVAL;
+    if (V > 0x7fffffff || T > 0x7fffffff) return DS_ETOOLARGE;
+    const EmbedSpace s = embed_space(T, D);
+    if (workspace_bytes < s.bytes || !workspace || (uintptr_t)workspace % 16) return DS_EWORKSPACE;
+    hipStream_t st = (hipStream_t)stream;
+    const uint32_t *keys, *pos;
+    const int status = sort_tokens(ids, id_bytes == 8, T, V, padding, (char *)workspace, s, st, &keys, &pos);
+    if (status != DS_OK) return status;
+    float *part = (float *)((char *)workspace + s.part);
+    if (type == DS_F32) return launch_embed_grad<float>(keys, pos, grad, ldg, dweight, part, T, V, D, scale, st);
+    if (type == DS_BF16) return launch_embed_grad<bf16_t>(keys, pos, grad, ldg, dweight, part, T, V, D, scale, st);
+    return launch_embed_grad<f16_t>(keys, pos, grad, ldg, dweight, part, T, V, D, scale, st);
+}

@@ -1,0 +1,538 @@
+// Matrix products of the cross entropy of a linear head (ds_vocab*.hip): one tiled kernel, whose operands may lie either way
+// and whose results go through the epilogue of the step that they belong to.
+//
+//   logits     s[t][v] = sum_d W[v][d] h[t][d] + b[v]        both operands contiguous along the reduction
+//   dhidden    dh[t][d] = sum_v W[v][d] P[t][v]              W contiguous across it
+//   dweight    dW[v][d] = sum_t h[t][d] P[t][v]              both contiguous across it
+//
+// Every product is C[n][m] = sum_k A(m, k) B(n, k): a lane of the matrix instruction holds four neighbouring m of one n, so
+// results are written along m, and what is summed over the vocabulary (m of the logits) is summed inside a lane first.
+//
+// float32 operands come as three bfloat16 planes, x = x0 + 2^-8 x1 + 2^-16 x2, and a product is the sum of the six plane
+// products above 2^-24 of it (x0 y0, x0 y1, x1 y0, x1 y1, x0 y2, x2 y0): six times the bf16 work at a rate of bf16, where the
+// float32 matrix instructions take sixteen times the time of bf16.  The planes' factors keep all 24 bits of the smallest
+// values, which planes without them would lose below 2^-110.
+#pragma once
+#include "ds_train.h"
+
+namespace ds {
+namespace vocab {
+
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef int i32x4 __attribute__((ext_vector_type(4)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef short s16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+
+// The 16-bit type that the matrix instructions take, and how many planes of it make a value.
+struct Bf16 { static constexpr int planes = 1; static constexpr bool half = false; };
+struct F16 { static constexpr int planes = 1; static constexpr bool half = true; };
+struct Split { static constexpr int planes = 3; static constexpr bool half = false; };  // float32
+
+template <typename P>
+__device__ __forceinline__ f32x4 mfma(s16x8 a, s16x8 b, f32x4 c)
+{
+    if constexpr (P::half)
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+    else
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
+
+// Planes of a float32 value, each what is left of it times 2^8, rounded to nearest, so that what a product leaves out has no
+// sign of its own; where that would round to infinity it is cut instead.
+__device__ __forceinline__ void split_planes(float f, bf16_t *p)
+{
+#pragma unroll
+    for (int q = 0; q < 3; ++q) {
+        bf16_t a = from_float<bf16_t>(f);
+        if ((a.bits & 0x7fff) == 0x7f80 && fabsf(f) < INFINITY) a.bits = (uint16_t)(__float_as_uint(f) >> 16);
+        p[q] = a;
+        f = (a.bits & 0x7f80) == 0x7f80 ? 0.f : (f - to_float(a)) * 256.f;
+    }
+}
+
+// An operand: `rows` x `k` elements, 16 bits each, planes `plane` elements apart.  Contiguous along k (element (r, k) at
+// r * ld + k) or across it (at k * ld + r).  ld and the address allow 16-byte accesses; past `rows` or `k` everything up to
+// the next multiple of 8 along the contiguous axis may be read and is zero, nothing beyond is touched.
+struct Operand {
+    const void *at;
+    int64_t ld, plane;
+};
+
+// What a launch computes with its tiles.
+enum { kStats = 0, kProb = 1, kOut = 2 };
+
+struct Args {
+    Operand a, b;
+    int M, N, K;          // of the whole product
+    int tiles_m, tiles_n;
+    int splits, k_split;  // kOut: the reduction is cut into `splits` stretches of k_split (a multiple of the step)
+    // logits: bias, targets, which stretch of the vocabulary this is
+    const void *bias;
+    int bias_type;
+    const void *target;
+    int target_wide;
+    int64_t V, ignore;
+    int v0;
+    float *stats;         // kStats: [tiles_m] [T][2] maximum and sum of exponentials, base 2
+    float *picked;        // kStats: [T] the target's logit
+    // kProb
+    const float *lse;     // [T], base 2
+    const float *row_scale;  // [T], or NULL: 1 for every counted row
+    void *prob;           // [planes][T][ldp]
+    int64_t ldp, prob_plane;
+    float *bias_part;     // [tiles_n][ld of the piece]: sums over the rows of a tile, or NULL
+    int ld_bias_part;
+    // kOut
+    float *slice;         // [splits][N][M] float, or NULL: final
+    void *out;            // [N] rows of type out_type, ldo apart
+    int64_t ldo;
+    int out_type;
+    const float *factor[2];  // final: what to multiply with, 1 value each, or NULL
+    int n_store;          // rows of C that exist (N may be rounded up for the loads)
+};
+
+constexpr float kLog2e = 1.4426950408889634f;
+// float16 holds probabilities times 2^15: the smallest that keeps all its bits is 2^-29 instead of 2^-14.  bfloat16 has the
+// exponents of float32 and needs none.
+constexpr float kProbScale = 32768.f;
+
+// A launch's tile: the workgroups of one XCD (they are dealt out in turn) get neighbouring tiles, in strips of kStrip along m,
+// so that what they read at the same time fits its L2.
+__device__ __forceinline__ void tile_of(int id, int tiles_m, int tiles_n, int *tm, int *tn)
+{
+    constexpr int kXcds = 8, kStrip = 8;
+    const int total = tiles_m * tiles_n, even = total / kXcds * kXcds;
+    if (id < even) id = (id % kXcds) * (even / kXcds) + id / kXcds;
+    const int per_strip = kStrip * tiles_n;
+    const int strip = id / per_strip, in = id - strip * per_strip;
+    const int first = strip * kStrip, width = min(kStrip, tiles_m - first);
+    *tn = in / width;
+    *tm = first + in - *tn * width;
+}
+
+// 16 bytes per lane from a buffer to LDS: lane l's go to `lds` + 16 l.  An offset past 2^31 fetches zeros.  No register is
+// written; whoever reads the LDS waits for the wave's own loads (vmcnt) and then for the workgroup's barrier.
+__device__ __forceinline__ void fetch(uint32_t offset, i32x4 buffer, uint32_t lds)
+{
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds"
+                 :: "v"(offset), "s"(buffer), "s"(lds) : "memory");
+}
+constexpr uint32_t kNothing = 0x80000000u;
+
+__device__ __forceinline__ i32x4 buffer_at(uint64_t address)
+{
+    i32x4 r;
+    r.x = __builtin_amdgcn_readfirstlane((int)(uint32_t)address);
+    r.y = __builtin_amdgcn_readfirstlane((int)((uint32_t)(address >> 32) & 0xffffu));
+    r.z = 0x7fffffff;
+    r.w = 0x00020000;
+    return r;
+}
+
+constexpr int kStep = 32;  // reduction per stage: one matrix instruction deep
+
+// A stage of one operand in LDS, ROWS x kStep.
+//   along k:  [row][32 k], 64 bytes a row, its four 16-byte pieces exchanged by row (piece ^ (row >> 1 & 3)), so that eight
+//             lanes reading the same piece of eight rows meet all banks;
+//   across:   [k][ROWS], its 32-byte pieces exchanged by k (piece ^ (k & 3)), for the transposing reads of 4 k x 16 rows.
+template <int ROWS, bool ACROSS, int WAVES>
+struct Tile {
+    static constexpr int bytes = ROWS * kStep * 2;
+    static constexpr int fetches = bytes / 1024;             // 1 KB each
+    static constexpr int mine = (fetches + WAVES - 1) / WAVES;  // of one wave
+    static_assert(fetches % WAVES == 0, "every wave fetches the same number");
+
+    uint32_t offset[mine];  // of this lane within the tile's first stage, or kNothing
+    int k_at[mine];         // along: first k of this lane's piece; across: its k
+
+    __device__ void init(const Operand &o, int rows_left, int wave)
+    {
+        const int lane = threadIdx.x & 63;
+#pragma unroll
+        for (int i = 0; i < mine; ++i) {
+            const int p = (wave * mine + i) * 64 + lane;  // 16-byte piece of the stage
+            if constexpr (!ACROSS) {
+                const int row = p >> 2, piece = (p & 3) ^ (row >> 1 & 3);
+                k_at[i] = piece * 8;
+                offset[i] = row < rows_left ? (uint32_t)(row * o.ld * 2 + piece * 16) : kNothing;
+            } else {
+                constexpr int per_k = ROWS / 8;
+                const int k = p / per_k, piece = (p % per_k) ^ ((k & 3) << 1);
+                k_at[i] = k;
+                offset[i] = piece * 8 < rows_left ? (uint32_t)(k * o.ld * 2 + piece * 16) : kNothing;
+            }
+        }
+    }
+    // `k_left` of the reduction remain at this stage; `base` is the address of its element (0, 0)
+    __device__ __forceinline__ void stage(uint64_t base, int k_left, uint32_t lds, int wave) const
+    {
+        const i32x4 buffer = buffer_at(base);
+#pragma unroll
+        for (int i = 0; i < mine; ++i)
+            fetch(k_at[i] < k_left ? offset[i] : kNothing, buffer, lds + (wave * mine + i) * 1024);
+    }
+    __device__ static __forceinline__ int64_t step_bytes(const Operand &o) { return ACROSS ? o.ld * kStep * 2 : kStep * 2; }
+    __device__ static __forceinline__ int64_t row_bytes(const Operand &o) { return ACROSS ? 2 : o.ld * 2; }
+
+    // Fragments: rows r0 .. r0+15 (a multiple of 16), lane l gets row l & 15 and k = 8 (l >> 4) .. + 7.
+    __device__ static __forceinline__ s16x8 fragment(const char *lds, int r0)
+    {
+        const int lane = threadIdx.x & 63, i = lane & 15, g = lane >> 4;
+        if constexpr (!ACROSS) {
+            const int row = r0 + i;
+            return *(const s16x8 *)(lds + row * 64 + ((g ^ (row >> 1 & 3)) << 4));
+        } else {
+            // 16 lanes read 4 k x 16 rows, 8 bytes each, and get them transposed
+            typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+            const int k = 8 * g + (i >> 2);
+            const int piece = (r0 >> 4) ^ (k & 3);  // the same for k and k + 4
+            const char *p = lds + k * ROWS * 2 + piece * 32 + (i & 3) * 8;
+            const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)p);
+            const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)(p + 4 * ROWS * 2));
+            s16x8 r;
+            r.lo = lo;
+            r.hi = hi;
+            return r;
+        }
+    }
+};
+
+__device__ __forceinline__ float bias_at(const Args &a, int v)
+{
+    if (!a.bias) return 0.f;
+    if (a.bias_type == DS_F32) return ((const float *)a.bias)[v];
+    if (a.bias_type == DS_BF16) return to_float(((const bf16_t *)a.bias)[v]);
+    return to_float(((const f16_t *)a.bias)[v]);
+}
+
+__device__ __forceinline__ int64_t target_at(const Args &a, int t)
+{
+    return a.target_wide ? ((const int64_t *)a.target)[t] : (int64_t)((const int32_t *)a.target)[t];
+}
+
+// What sums of probabilities are multiplied with on their way out.
+template <typename P>
+__device__ __forceinline__ float out_factor(const float *const *f)
+{
+    return (f[0] ? *f[0] : 1.f) * (f[1] ? *f[1] : 1.f) * (P::half ? 1.f / kProbScale : 1.f);
+}
+
+template <typename P, int BM, int BN, int WM, int WN, bool A_ACROSS, bool B_ACROSS, int KIND, int STAGES>
+__global__ __launch_bounds__(WM * WN * 64) void product_kernel(Args g)
+{
+    constexpr int WAVES = WM * WN, MT = BM / WM / 16, NT = BN / WN / 16, NP = P::planes;
+    using TA = Tile<BM, A_ACROSS, WAVES>;
+    using TB = Tile<BN, B_ACROSS, WAVES>;
+    constexpr int kStageBytes = NP * (TA::bytes + TB::bytes);
+    constexpr int kInFlight = NP * (TA::mine + TB::mine);  // loads of one stage and wave
+    __shared__ __attribute__((aligned(1024))) char lds[STAGES * kStageBytes];
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+    const int wm = wave % WM, wn = wave / WM;
+
+    int tm, tn;
+    const int tiles = g.tiles_m * g.tiles_n;
+    const int split = blockIdx.x / tiles;
+    tile_of(blockIdx.x - split * tiles, g.tiles_m, g.tiles_n, &tm, &tn);
+    const int m0 = tm * BM, n0 = tn * BN;
+    const int k_from = split * g.k_split, k_to = min(g.K, k_from + g.k_split);
+    const int steps = (k_to - k_from + kStep - 1) / kStep;
+
+    TA ta;
+    TB tb;
+    ta.init(g.a, g.M - m0, wave);
+    tb.init(g.b, g.N - n0, wave);
+    const int64_t a_step = TA::step_bytes(g.a), b_step = TB::step_bytes(g.b);
+    uint64_t a_at = (uint64_t)g.a.at + m0 * TA::row_bytes(g.a) + k_from / kStep * a_step;
+    uint64_t b_at = (uint64_t)g.b.at + n0 * TB::row_bytes(g.b) + k_from / kStep * b_step;
+    const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char *)lds;
+
+    int k_left = k_to - k_from;  // of the next stage to fetch
+    auto fetch_stage = [&](int slot) {
+        const uint32_t to = lds0 + slot * kStageBytes;
+#pragma unroll
+        for (int p = 0; p < NP; ++p) {
+            ta.stage(a_at + p * g.a.plane * 2, k_left, to + p * TA::bytes, wave);
+            tb.stage(b_at + p * g.b.plane * 2, k_left, to + NP * TA::bytes + p * TB::bytes, wave);
+        }
+        a_at += a_step, b_at += b_step, k_left -= kStep;
+    };
+
+    f32x4 acc[MT][NT];
+#pragma unroll
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+        for (int j = 0; j < NT; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+
+    // Stages past the end are fetched too, as zeros (k_left <= 0 fetches nothing): the number of loads in flight is the same
+    // in every step, and nothing past the operands is read.
+#pragma unroll
+    for (int s = 0; s < STAGES - 1; ++s) fetch_stage(s);
+    int slot = 0;
+    for (int s = 0; s < steps; ++s) {
+        // this wave's part of the stage has arrived, and it has read the slot that is filled next; then everyone's
+        asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" :: "i"((STAGES - 2) * kInFlight) : "memory");
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+        fetch_stage(slot == 0 ? STAGES - 1 : slot - 1);
+        const char *at = lds + slot * kStageBytes;
+        if constexpr (NP == 1) {
+            s16x8 fa[MT], fb[NT];
+#pragma unroll
+            for (int j = 0; j < NT; ++j) fb[j] = TB::fragment(at + TA::bytes, wn * NT * 16 + j * 16);
+#pragma unroll
+            for (int i = 0; i < MT; ++i) fa[i] = TA::fragment(at, wm * MT * 16 + i * 16);
+#pragma unroll
+            for (int i = 0; i < MT; ++i)
+#pragma unroll
+                for (int j = 0; j < NT; ++j) acc[i][j] = mfma<P>(fa[i], fb[j], acc[i][j]);
+        } else {
+            s16x8 fb[NP][NT];
+#pragma unroll
+            for (int p = 0; p < NP; ++p)
+#pragma unroll
+                for (int j = 0; j < NT; ++j)
+                    fb[p][j] = TB::fragment(at + NP * TA::bytes + p * TB::bytes, wn * NT * 16 + j * 16);
+#pragma unroll
+            for (int i = 0; i < MT; ++i) {
+                s16x8 fa[NP];
+#pragma unroll
+                for (int p = 0; p < NP; ++p) fa[p] = TA::fragment(at + p * TA::bytes, wm * MT * 16 + i * 16);
+                // the products of 2^-16, then those of 2^-8, then the largest
+                f32x4 low[NT];
+#pragma unroll
+                for (int j = 0; j < NT; ++j) low[j] = mfma<P>(fa[1], fb[1][j], f32x4{0.f, 0.f, 0.f, 0.f});
+#pragma unroll
+                for (int j = 0; j < NT; ++j) low[j] = mfma<P>(fa[0], fb[2][j], low[j]);
+#pragma unroll
+                for (int j = 0; j < NT; ++j) low[j] = mfma<P>(fa[2], fb[0][j], low[j]) * (1.f / 256);
+#pragma unroll
+                for (int j = 0; j < NT; ++j) low[j] = mfma<P>(fa[0], fb[1][j], low[j]);
+#pragma unroll
+                for (int j = 0; j < NT; ++j) low[j] = mfma<P>(fa[1], fb[0][j], low[j]);
+#pragma unroll
+                for (int j = 0; j < NT; ++j) acc[i][j] = mfma<P>(fa[0], fb[0][j], acc[i][j]);
+#pragma unroll
+                for (int j = 0; j < NT; ++j)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) acc[i][j][r] = fmaf(low[j][r], 1.f / 256, acc[i][j][r]);
+            }
+        }
+        slot = slot + 1 == STAGES ? 0 : slot + 1;
+    }
+    // nothing of this wave is on its way to LDS any more, and nobody reads it
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+    __syncthreads();
+
+    const int m_lane = m0 + wm * MT * 16 + (lane >> 4) * 4, n_lane = n0 + wn * NT * 16 + (lane & 15);
+    float *fl = (float *)lds;
+    if constexpr (KIND != kOut) {
+        // acc becomes the logits in base 2
+#pragma unroll
+        for (int i = 0; i < MT; ++i)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const int m = m_lane + i * 16 + r;
+                const bool real = m < g.M;
+                const float b = real ? bias_at(g, g.v0 + m) : 0.f;
+#pragma unroll
+                for (int j = 0; j < NT; ++j) acc[i][j][r] = real ? (acc[i][j][r] + b) * kLog2e : -INFINITY;
+            }
+    }
+    if constexpr (KIND == kStats) {
+#pragma unroll
+        for (int j = 0; j < NT; ++j) {
+            const int t = n_lane + j * 16;
+            const int64_t from_here = t < g.N ? target_at(g, t) - g.v0 - m_lane : -1;
+            const int want = from_here >= 0 && from_here < BM ? (int)from_here : -1;
+            float top = -INFINITY;
+#pragma unroll
+            for (int i = 0; i < MT; ++i)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    // a maximum that a value which is no number does not slip through
+                    top = acc[i][j][r] > top || acc[i][j][r] != acc[i][j][r] ? acc[i][j][r] : top;
+                    if (want == i * 16 + r && m_lane + i * 16 + r < g.M) g.picked[t] = acc[i][j][r];
+                }
+            float sum = 0.f;
+            // a column of nothing but -inf keeps a sum of 0
+            const float base = top == -INFINITY ? 0.f : top;
+#pragma unroll
+            for (int i = 0; i < MT; ++i)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) sum += exp2f(acc[i][j][r] - base);
+#pragma unroll
+            for (int o = 16; o <= 32; o <<= 1) {
+                const float top2 = __shfl_xor(top, o), sum2 = __shfl_xor(sum, o);
+                const float both = fmaxf(top, top2);
+                sum = both == -INFINITY ? sum + sum2 : sum * exp2f(top - both) + sum2 * exp2f(top2 - both);
+                top = both;
+            }
+            if (lane < 16) {
+                const int c = wn * NT * 16 + j * 16 + lane;
+                fl[(wm * BN + c) * 2] = top;
+                fl[(wm * BN + c) * 2 + 1] = sum;
+            }
+        }
+        __syncthreads();
+        for (int c = threadIdx.x; c < BN; c += WAVES * 64) {
+            if (n0 + c >= g.N) continue;
+            float top = fl[c * 2], sum = fl[c * 2 + 1];
+#pragma unroll
+            for (int w = 1; w < WM; ++w) {
+                const float top2 = fl[(w * BN + c) * 2], sum2 = fl[(w * BN + c) * 2 + 1];
+                const float both = fmaxf(top, top2);
+                sum = both == -INFINITY ? sum + sum2 : sum * exp2f(top - both) + sum2 * exp2f(top2 - both);
+                top = both;
+            }
+            float2 *to = (float2 *)g.stats + (int64_t)tm * g.N + n0 + c;
+            *to = float2{top, sum};
+        }
+    }
+    if constexpr (KIND == kProb) {
+        float over_n[MT][4];  // sums over this lane's rows, for the bias
+#pragma unroll
+        for (int i = 0; i < MT; ++i)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) over_n[i][r] = 0.f;
+#pragma unroll
+        for (int j = 0; j < NT; ++j) {
+            const int t = n_lane + j * 16;
+            const bool real = t < g.N;
+            const int64_t y = real ? target_at(g, t) : 0;
+            const float lse = real ? g.lse[t] : 0.f;
+            const float scale = !real || y == g.ignore ? 0.f : y < 0 || y >= g.V ? NAN : g.row_scale ? g.row_scale[t] : 1.f;
+            const int64_t from_here = y - g.v0 - m_lane;
+            const int want = from_here >= 0 && from_here < BM ? (int)from_here : -1;
+#pragma unroll
+            for (int i = 0; i < MT; ++i) {
+                float p[4];
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const float e = exp2f(acc[i][j][r] - lse) - (want == i * 16 + r ? 1.f : 0.f);
+                    // rows that do not count leave nothing, whatever their logits are; neither do words past the end
+                    p[r] = scale == 0.f || m_lane + i * 16 + r >= g.M ? 0.f : e * scale;
+                    over_n[i][r] += p[r];
+                    if constexpr (P::half) p[r] *= kProbScale;
+                }
+                const int m = m_lane + i * 16;
+                if (!real || m >= g.ldp) continue;
+                Vec<bf16_t, 4> *to = (Vec<bf16_t, 4> *)((bf16_t *)g.prob + (int64_t)t * g.ldp + m);
+                if constexpr (NP == 1) {
+                    Vec<bf16_t, 4> o;
+#pragma unroll
+                    for (int r = 0; r < 4; ++r)
+                        o.v[r].bits = P::half ? from_float<f16_t>(p[r]).bits : from_float<bf16_t>(p[r]).bits;
+                    *to = o;
+                } else {
+                    bf16_t planes[4][3];
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) split_planes(p[r], planes[r]);
+#pragma unroll
+                    for (int q = 0; q < NP; ++q) {
+                        const Vec<bf16_t, 4> o{{planes[0][q], planes[1][q], planes[2][q], planes[3][q]}};
+                        *(Vec<bf16_t, 4> *)((bf16_t *)to + q * g.prob_plane) = o;
+                    }
+                }
+            }
+        }
+        if (g.bias_part) {
+#pragma unroll
+            for (int i = 0; i < MT; ++i)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+#pragma unroll
+                    for (int o = 1; o < 16; o <<= 1) over_n[i][r] += __shfl_xor(over_n[i][r], o);
+                    if ((lane & 15) == 0) fl[wn * BM + wm * MT * 16 + i * 16 + (lane >> 4) * 4 + r] = over_n[i][r];
+                }
+            __syncthreads();
+            for (int c = threadIdx.x; c < BM; c += WAVES * 64) {
+                if (m0 + c >= g.M) continue;
+                float s = fl[c];
+#pragma unroll
+                for (int w = 1; w < WN; ++w) s += fl[w * BM + c];
+                g.bias_part[(int64_t)tn * g.ld_bias_part + m0 + c] = s;
+            }
+        }
+    }
+    if constexpr (KIND == kOut) {
+        const float factor = g.slice ? 1.f : out_factor<P>(g.factor);
+#pragma unroll
+        for (int j = 0; j < NT; ++j) {
+            const int n = n_lane + j * 16;
+            if (n >= g.n_store) continue;
+#pragma unroll
+            for (int i = 0; i < MT; ++i) {
+                const int m = m_lane + i * 16;
+                if (m >= g.M) continue;
+                const int many = min(4, g.M - m);
+                if (g.slice) {
+                    float *to = g.slice + ((int64_t)split * g.n_store + n) * g.M + m;
+                    if (many == 4 && g.M % 4 == 0) *(f32x4 *)to = acc[i][j];
+                    else
+#pragma unroll
+                        for (int r = 0; r < 4; ++r)
+                            if (r < many) to[r] = acc[i][j][r];
+                    continue;
+                }
+                float v[4];
+#pragma unroll
+                for (int r = 0; r < 4; ++r) v[r] = acc[i][j][r] * factor;
+                const bool whole = many == 4 && g.ldo % 4 == 0 && (uintptr_t)g.out % 16 == 0;
+                if (g.out_type == DS_F32) {
+                    float *to = (float *)g.out + (int64_t)n * g.ldo + m;
+                    if (whole) *(f32x4 *)to = f32x4{v[0], v[1], v[2], v[3]};
+                    else
+#pragma unroll
+                        for (int r = 0; r < 4; ++r)
+                            if (r < many) to[r] = v[r];
+                } else {
+                    uint16_t *to = (uint16_t *)g.out + (int64_t)n * g.ldo + m;
+                    Vec<bf16_t, 4> o;
+#pragma unroll
+                    for (int r = 0; r < 4; ++r)
+                        o.v[r].bits = P::half ? from_float<f16_t>(v[r]).bits : from_float<bf16_t>(v[r]).bits;
+                    if (whole) *(Vec<bf16_t, 4> *)to = o;
+                    else
+#pragma unroll
+                        for (int r = 0; r < 4; ++r)
+                            if (r < many) to[r] = o.v[r].bits;
+                }
+            }
+        }
+    }
+}
+
+// Which product a launch is.
+enum { kLogitStats = 0, kLogitProb = 1, kHidden = 2, kWeight = 3 };
+
+// Tile shapes, m x n, by their number in a launch.
+template <typename P> struct Shapes;
+template <> struct Shapes<Bf16> { static constexpr int m[3] = {256, 128, 128}, n[3] = {256, 128, 64}; };
+template <> struct Shapes<F16> : Shapes<Bf16> {};
+template <> struct Shapes<Split> { static constexpr int m[3] = {256, 128, 64}, n[3] = {128, 128, 64}; };
+
+// Launches one product with tiles of shape `tile`; fills in the tile counts.  A translation unit per P.
+template <typename P> int launch_product(int kind, int tile, Args &g, hipStream_t st);
+
+template <typename P, int BM, int BN, int WM, int WN, int STAGES>
+int launch_tiled(int kind, Args &g, hipStream_t st)
+{
+    g.tiles_m = ceil_div(g.M, BM), g.tiles_n = ceil_div(g.N, BN);
+    const int64_t blocks = (int64_t)g.tiles_m * g.tiles_n * g.splits;
+    if (blocks > 0x7fffffff) return DS_ETOOLARGE;
+    const dim3 grid((unsigned)blocks), threads(WM * WN * 64);
+    if (kind == kLogitStats)
+        hipLaunchKernelGGL((product_kernel<P, BM, BN, WM, WN, false, false, kStats, STAGES>), grid, threads, 0, st, g);
+    else if (kind == kLogitProb)
+        hipLaunchKernelGGL((product_kernel<P, BM, BN, WM, WN, false, false, kProb, STAGES>), grid, threads, 0, st, g);
+    else if (kind == kHidden)
+        hipLaunchKernelGGL((product_kernel<P, BM, BN, WM, WN, true, false, kOut, STAGES>), grid, threads, 0, st, g);
+    else
+        hipLaunchKernelGGL((product_kernel<P, BM, BN, WM, WN, true, true, kOut, STAGES>), grid, threads, 0, st, g);
+    return launch_status();
+}
+
+}  // namespace vocab
+}  // namespace ds

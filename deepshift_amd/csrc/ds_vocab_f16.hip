@@ -1,0 +1,15 @@
+// The products of the vocabulary's cross entropy on float16 operands.
+#include "ds_vocab.h"
+
+namespace ds {
+namespace vocab {
+
+template <> int launch_product<F16>(int kind, int tile, Args &g, hipStream_t st)
+{
+    if (tile == 0) return launch_tiled<F16, 256, 256, 2, 4, 4>(kind, g, st);
+    if (tile == 1) return launch_tiled<F16, 128, 128, 2, 2, 4>(kind, g, st);
+    return launch_tiled<F16, 128, 64, 4, 1, 4>(kind, g, st);
+}
+
+}  // namespace vocab
+}  // namespace ds

@@ -1,0 +1,15 @@
+// The products of the vocabulary's cross entropy on float32 operands, as three bfloat16 planes each.
+#include "ds_vocab.h"
+
+namespace ds {
+namespace vocab {
+
+template <> int launch_product<Split>(int kind, int tile, Args &g, hipStream_t st)
+{
+    if (tile == 0) return launch_tiled<Split, 256, 128, 4, 2, 2>(kind, g, st);
+    if (tile == 1) return launch_tiled<Split, 128, 128, 2, 2, 3>(kind, g, st);
+    return launch_tiled<Split, 64, 64, 2, 2, 3>(kind, g, st);
+}
+
+}  // namespace vocab
+}  // namespace ds

@@ -1,0 +1,397 @@
+"""Operators of a token model's training step around shift layers: the scaled embedding lookup at its entrance, the cross
+entropy of a linear head over a large vocabulary at its exit, and the clipping of gradients by their global norm.
+
+The layers between are ``LinearShift`` / ``LinearShiftQ`` on their float path, whose straight-through gradients
+(``ste.py``) reach shifts and signs unscaled -- the reason to clip them.  Everything here runs in the gfx950 library, on the
+current stream of the tensors' device, on float32, bfloat16 and float16; sums are held in 32 bits or more and rounded once,
+and a call repeats bit for bit.  There is no CPU path: a CPU tensor raises.
+
+Functions whose names end in ``_grad`` return gradients directly; ``embedding`` and ``linear_cross_entropy`` also take part
+in autograd.
+"""
+import ctypes
+import math
+
+import torch
+import torch.nn as nn
+from torch.autograd import Function
+
+from . import _lib, kernels
+
+__all__ = ["embedding", "embedding_grad", "linear_cross_entropy", "linear_cross_entropy_grad", "gradient_norm",
+           "clip_gradients_", "clip_grad_norm_", "ScaledEmbedding", "LinearCrossEntropy"]
+
+_TYPES = {torch.float32: _lib.DS_F32, torch.bfloat16: _lib.DS_BF16, torch.float16: _lib.DS_F16}
+_REDUCTIONS = {"none": _lib.DS_NONE, "sum": _lib.DS_SUM, "mean": _lib.DS_MEAN}
+
+
+def _type_of(name, t):
+    code = _TYPES.get(t.dtype)
+    if code is None:
+        raise TypeError("%s must be float32, bfloat16 or float16, got %s" % (name, t.dtype))
+    if not t.is_cuda:
+        raise ValueError("%s must be a GPU tensor" % name)
+    return code
+
+
+def _tokens_of(name, t, device):
+    if t.dtype != torch.int64 and t.dtype != torch.int32:
+        raise TypeError("%s must be int64 or int32, got %s" % (name, t.dtype))
+    if t.device != device:
+        raise ValueError("%s must be on %s, is on %s" % (name, device, t.device))
+    return t if t.is_contiguous() else t.contiguous()
+
+
+def _rows_of(t):
+    """A matrix whose rows lie contiguously, and the distance between them."""
+    if t.stride(1) != 1 and t.size(1) > 1 or t.size(0) > 1 and t.stride(0) < t.size(1):
+        t = t.contiguous()
+    return t, t.stride(0) if t.size(0) > 1 else t.size(1)
+
+
+class _On:
+    """Makes a tensor's device the current one for the launches of a call."""
+
+    def __init__(self, device):
+        self.device = device if device.index is not None and device.index != torch.cuda.current_device() else None
+
+    def __enter__(self):
+        if self.device is not None:
+            self.guard = torch.cuda.device(self.device)
+            self.guard.__enter__()
+
+    def __exit__(self, *exc):
+        if self.device is not None:
+            self.guard.__exit__(*exc)
+
+
+# ---------------------------------------------------------------------------------------------
+# embedding
+# ---------------------------------------------------------------------------------------------
+
+def _embed(ids, weight, scale):
+    code = _type_of("weight", weight)
+    if weight.dim() != 2:
+        raise ValueError("weight must be [V, D]")
+    ids = _tokens_of("ids", ids, weight.device)
+    weight, ld = _rows_of(weight)
+    V, D = weight.shape
+    out = torch.empty(ids.shape + (D,), dtype=weight.dtype, device=weight.device)
+    with _On(weight.device):
+        _lib.call("ds_embed", ids.data_ptr(), ids.element_size(), weight.data_ptr(), ld, out.data_ptr(), ids.numel(), V, D,
+                  scale, code, _lib.stream_handle(weight.device))
+    return out
+
+
+def embedding_grad(ids, grad, num_embeddings, scale=1.0, padding_idx=None):
+    """Gradient of :func:`embedding` with respect to its weight, ``[num_embeddings, D]`` in ``grad``'s type: row ``v`` is
+    ``scale`` times the sum of ``grad`` over the tokens ``v``, in ascending order and 32 bits.  Tokens equal to
+    ``padding_idx`` add nothing, and neither do numbers outside ``[0, num_embeddings)``."""
+    code = _type_of("grad", grad)
+    ids = _tokens_of("ids", ids, grad.device)
+    if grad.dim() < 1 or grad.shape[:-1] != ids.shape:
+        raise ValueError("grad must be %s + [D], is %s" % (list(ids.shape), list(grad.shape)))
+    V, D = int(num_embeddings), grad.shape[-1]
+    if V < 0:
+        raise ValueError("num_embeddings must not be negative")
+    padding = _padding(padding_idx, V)
+    T = ids.numel()
+    grad, ld = _rows_of(grad.reshape(T, D))
+    out = torch.empty((V, D), dtype=grad.dtype, device=grad.device)
+    with _On(grad.device):
+        nbytes = _lib.lib().ds_embed_grad_workspace_bytes(T, D)
+        ws = kernels._workspace(nbytes, grad.device)
+        _lib.call("ds_embed_grad", ids.data_ptr(), ids.element_size(), grad.data_ptr(), ld, out.data_ptr(), T, V, D, padding,
+                  float(scale), code, ws.data_ptr(), nbytes, _lib.stream_handle(grad.device))
+    return out
+
+
+def _padding(padding_idx, V):
+    if padding_idx is None:
+        return -1
+    if not -V <= padding_idx < V:
+        raise ValueError("padding_idx must be in [-%d, %d), is %d" % (V, V, padding_idx))
+    return padding_idx % V
+
+
+class _Embedding(Function):
+    @staticmethod
+    def forward(ctx, ids, weight, scale, padding_idx):
+        ctx.save_for_backward(ids)
+        ctx.of = (weight.shape[0], scale, padding_idx)
+        return _embed(ids, weight, scale)
+
+    @staticmethod
+    def backward(ctx, grad):
+        ids, = ctx.saved_tensors
+        V, scale, padding_idx = ctx.of
+        return None, embedding_grad(ids, grad, V, scale, padding_idx), None, None
+
+
+def embedding(ids, weight, scale=1.0, padding_idx=None):
+    """``scale * weight[ids]`` for ``ids`` of any shape (int64 or int32) and ``weight`` ``[V, D]``, multiplied in 32 bits and
+    rounded once.  A number outside ``[0, V)`` gives a row of NaN (the GPU cannot raise).  ``padding_idx`` names the word
+    whose row gets no gradient."""
+    scale = float(scale)
+    if not math.isfinite(scale):
+        raise ValueError("scale must be finite")
+    if weight.requires_grad and torch.is_grad_enabled():
+        if weight.dim() == 2:
+            _padding(padding_idx, weight.shape[0])
+        return _Embedding.apply(ids, weight, scale, padding_idx)
+    return _embed(ids, weight, scale)
+
+
+# ---------------------------------------------------------------------------------------------
+# cross entropy of a linear head
+# ---------------------------------------------------------------------------------------------
+
+class _Head:
+    """The checked operands of one call, as the library takes them."""
+
+    def __init__(self, hidden, weight, target, bias, ignore_index, reduction):
+        self.type = _type_of("hidden", hidden)
+        device = hidden.device
+        if reduction not in _REDUCTIONS:
+            raise ValueError("reduction must be 'none', 'sum' or 'mean', is %r" % (reduction,))
+        self.reduction = _REDUCTIONS[reduction]
+        if hidden.dim() < 1 or weight.dim() != 2 or weight.shape[1] != hidden.shape[-1]:
+            raise ValueError("weight must be [V, %s], is %s" % (hidden.shape[-1] if hidden.dim() else "D", list(weight.shape)))
+        if weight.shape[0] < 1:
+            raise ValueError("weight must have at least one row")
+        for name, t in (("weight", weight), ("bias", bias)):
+            if t is not None and (t.dtype != hidden.dtype or t.device != device):
+                raise TypeError("%s must be %s on %s like hidden, is %s on %s" % (name, hidden.dtype, device, t.dtype, t.device))
+        if bias is not None and bias.shape != weight.shape[:1]:
+            raise ValueError("bias must be [%d], is %s" % (weight.shape[0], list(bias.shape)))
+        if target.shape != hidden.shape[:-1]:
+            raise ValueError("target must be %s, is %s" % (list(hidden.shape[:-1]), list(target.shape)))
+        self.shape = target.shape
+        self.target = _tokens_of("target", target, device)
+        self.V, self.D = weight.shape
+        self.T = self.target.numel()
+        self.hidden_shape = hidden.shape
+        self.hidden, self.ldh = _rows_of(hidden.reshape(self.T, self.D))
+        self.weight, self.ldw = _rows_of(weight)
+        self.bias = None if bias is None else bias.contiguous()
+        self.ignore = int(ignore_index)
+        if not -2 ** 63 <= self.ignore < 2 ** 63:
+            raise ValueError("ignore_index must fit 64 bits")
+
+    def _matrices(self):
+        return self.hidden.data_ptr(), self.ldh, self.weight.data_ptr(), self.ldw
+
+    def _problem(self):
+        return self._matrices() + (_lib.ptr(self.bias), self.target.data_ptr(), self.target.element_size(), self.ignore, self.T,
+                                   self.D, self.V, self.type)
+
+    def workspace(self, grad):
+        nbytes = _lib.lib().ds_vocab_workspace_bytes(*(self._matrices() + (self.T, self.D, self.V, self.type, grad)))
+        return kernels._workspace(nbytes, self.hidden.device), nbytes
+
+    def loss(self):
+        """``(loss, lse, share)``: the reduced loss (or one per token), and what the gradients need of it."""
+        device = self.hidden.device
+        rows = torch.empty(2, self.T, dtype=torch.float32, device=device)
+        total = torch.empty(2, dtype=torch.float32, device=device) if self.reduction else None
+        ws, nbytes = self.workspace(0)
+        row = rows.data_ptr()
+        _lib.call("ds_vocab_loss", *(self._problem() + (self.reduction, row, row + 4 * self.T, _lib.ptr(total), ws.data_ptr(),
+                                                        nbytes, _lib.stream_handle(device))))
+        if total is None:
+            return rows[0].view(self.shape), rows[1], None
+        return total[0], rows[1], total[1]
+
+    def gradients(self, lse, share, row_grad, grad, wanted):
+        """Gradients of hidden, weight and bias, ``None`` for those that are not ``wanted``."""
+        device = self.hidden.device
+        dtype = self.hidden.dtype
+        dhidden = torch.empty(self.hidden_shape, dtype=dtype, device=device) if wanted[0] else None
+        dweight = torch.empty((self.V, self.D), dtype=dtype, device=device) if wanted[1] else None
+        dbias = torch.empty(self.V, dtype=dtype, device=device) if wanted[2] and self.bias is not None else None
+        ws, nbytes = self.workspace(1)
+        ptr = _lib.ptr
+        _lib.call("ds_vocab_loss_grad", *(self._problem() + (ptr(lse), ptr(row_grad), ptr(grad), ptr(share), ptr(dhidden),
+                                                             ptr(dweight), ptr(dbias), ws.data_ptr(), nbytes,
+                                                             _lib.stream_handle(device))))
+        return dhidden, dweight, dbias
+
+
+class _LinearCrossEntropy(Function):
+    @staticmethod
+    def forward(ctx, hidden, weight, target, bias, ignore_index, reduction):
+        with _On(hidden.device):
+            head = _Head(hidden, weight, target, bias, ignore_index, reduction)
+            loss, lse, share = head.loss()
+        ctx.save_for_backward(hidden, weight, target, bias, lse, share)
+        ctx.of = (ignore_index, reduction)
+        return loss
+
+    @staticmethod
+    def backward(ctx, grad):
+        hidden, weight, target, bias, lse, share = ctx.saved_tensors
+        with _On(hidden.device):
+            head = _Head(hidden, weight, target, bias, *ctx.of)
+            grad = grad.float().contiguous()
+            needed = ctx.needs_input_grad
+            got = head.gradients(lse, share, grad if share is None else None, None if share is None else grad,
+                                 (needed[0], needed[1], needed[3]))
+        return got[0], got[1], None, got[2], None, None
+
+
+def linear_cross_entropy(hidden, weight, target, bias=None, ignore_index=-100, reduction="mean"):
+    """Cross entropy of ``softmax(hidden @ weight.T + bias)`` against ``target``, without ever storing the logits.
+
+    ``hidden`` ``[..., D]``, ``weight`` ``[V, D]`` and ``bias`` ``[V]`` are of one type, ``target`` ``[...]`` int64 or int32.
+    The loss is float32: per token with ``reduction='none'``, else their sum, or their mean over the tokens that count.
+    Tokens whose target is ``ignore_index`` have loss 0 and leave nothing in any gradient, whatever ``hidden`` holds there; if
+    no token counts, the loss and its gradients are 0.  A target that is neither ``ignore_index`` nor in ``[0, V)`` gives NaN.
+    A bias of ``-inf`` takes a word out."""
+    if torch.is_grad_enabled() and (hidden.requires_grad or weight.requires_grad or (bias is not None and bias.requires_grad)):
+        return _LinearCrossEntropy.apply(hidden, weight, target, bias, ignore_index, reduction)
+    with _On(hidden.device):
+        return _Head(hidden, weight, target, bias, ignore_index, reduction).loss()[0]
+
+
+def linear_cross_entropy_grad(hidden, weight, target, bias=None, ignore_index=-100, reduction="mean"):
+    """``(loss, dhidden, dweight, dbias)`` of :func:`linear_cross_entropy` for a gradient of 1 (of ones, with
+    ``reduction='none'``), without autograd; ``dbias`` is ``None`` where there is no bias."""
+    with torch.no_grad(), _On(hidden.device):
+        head = _Head(hidden, weight, target, bias, ignore_index, reduction)
+        loss, lse, share = head.loss()
+        return (loss,) + head.gradients(lse, share, None, None, (True, True, True))
+
+
+# ---------------------------------------------------------------------------------------------
+# clipping
+# ---------------------------------------------------------------------------------------------
+
+def _flat(t):
+    """Whether the tensor's elements fill one stretch of memory in some order."""
+    return t.is_contiguous() or torch.ops.aten.is_non_overlapping_and_dense(t)
+
+
+def _clip(grads, max_norm, out, scale):
+    grads = [grads] if isinstance(grads, torch.Tensor) else list(grads)
+    if not grads:
+        raise ValueError("no gradients given")
+    device = grads[0].device
+    outs = grads if out is None else ([out] if isinstance(out, torch.Tensor) else list(out))
+    if len(outs) != len(grads):
+        raise ValueError("%d tensors in out for %d gradients" % (len(outs), len(grads)))
+    table = (_lib.Tensor * len(grads))()
+    kept, back = [], []   # copies that have to live until the launches are issued, and those that go back
+    for i, (t, o) in enumerate(zip(grads, outs)):
+        code = _type_of("gradient %d" % i, t)
+        to = _type_of("out %d" % i, o)
+        if t.device != device or o.device != device:
+            raise ValueError("all gradients must be on %s" % device)
+        if o.shape != t.shape:
+            raise ValueError("out %d must be %s, is %s" % (i, list(t.shape), list(o.shape)))
+        src, dst = t, o
+        if t is o:
+            if not _flat(t):
+                src = dst = t.contiguous()
+        elif not (t.is_contiguous() and o.is_contiguous()) and not (t.stride() == o.stride() and _flat(t)):
+            src = t.contiguous()
+            dst = o if o.is_contiguous() else torch.empty_like(src, dtype=o.dtype)
+        if src is not t or dst is not o:
+            kept.append((src, dst))
+            if dst is not o:
+                back.append((o, dst))
+        table[i] = (src.data_ptr(), dst.data_ptr(), t.numel(), code, to)
+    if scale and len({e.dst for e in table if e.n}) != sum(e.n > 0 for e in table):
+        raise ValueError("a tensor is given twice")
+    norm = torch.empty((), dtype=torch.float32, device=device)
+    with _On(device):
+        nbytes = _lib.lib().ds_clip_workspace_bytes(len(grads))
+        ws = kernels._workspace(nbytes, device)
+        _lib.call("ds_clip", table, len(grads), max_norm, int(scale), norm.data_ptr(), ws.data_ptr(), nbytes,
+                  _lib.stream_handle(device))
+        if scale:
+            for o, dst in back:
+                o.copy_(dst)
+    return norm
+
+
+def gradient_norm(grads):
+    """The global 2-norm of all tensors in ``grads``, a float32 scalar on their device."""
+    with torch.no_grad():
+        return _clip(grads, 0.0, None, False)
+
+
+def clip_gradients_(grads, max_norm, out=None):
+    """Scales ``grads`` by ``min(1, max_norm / (norm + 1e-6))`` and returns ``norm``, their global 2-norm before it (a float32
+    scalar on the device; nothing waits for it).  The results go to ``out``, a tensor for each gradient, of any of the three
+    types, or in place.  Types may differ from tensor to tensor.  A norm that is infinite or NaN scales by 0 or NaN."""
+    max_norm = float(max_norm)
+    if not max_norm >= 0:
+        raise ValueError("max_norm must not be negative")
+    with torch.no_grad():
+        return _clip(grads, max_norm, out, True)
+
+
+def clip_grad_norm_(parameters, max_norm, error_if_nonfinite=False):
+    """Clips the ``.grad`` of ``parameters`` (those that have one) in place by their global 2-norm, which is returned: the
+    counterpart of ``torch.nn.utils.clip_grad_norm_``.  ``error_if_nonfinite`` raises before anything is scaled, and waits
+    for the GPU to know."""
+    parameters = [parameters] if isinstance(parameters, torch.Tensor) else parameters
+    grads = [p.grad for p in parameters if p.grad is not None]
+    if not grads:
+        return torch.zeros(())
+    if error_if_nonfinite:
+        norm = gradient_norm(grads)
+        if not torch.isfinite(norm):
+            raise RuntimeError("the gradients' norm is %s" % norm.item())
+    return clip_gradients_(grads, max_norm)
+
+
+# ---------------------------------------------------------------------------------------------
+# modules
+# ---------------------------------------------------------------------------------------------
+
+class ScaledEmbedding(nn.Module):
+    """``scale * weight[ids]``; the row of ``padding_idx`` starts at zero and gets no gradient."""
+
+    def __init__(self, num_embeddings, embedding_dim, scale=1.0, padding_idx=None):
+        super().__init__()
+        self.num_embeddings, self.embedding_dim, self.scale = num_embeddings, embedding_dim, scale
+        self.padding_idx = None if padding_idx is None else _padding(padding_idx, num_embeddings)
+        self.weight = nn.Parameter(torch.empty(num_embeddings, embedding_dim))
+        self.reset_parameters()
+
+    def reset_parameters(self):
+        nn.init.normal_(self.weight, std=1.0 / self.scale if self.scale else 1.0)
+        if self.padding_idx is not None:
+            with torch.no_grad():
+                self.weight[self.padding_idx].zero_()
+
+    def forward(self, ids):
+        return embedding(ids, self.weight, self.scale, self.padding_idx)
+
+    def extra_repr(self):
+        return "{num_embeddings}, {embedding_dim}, scale={scale}, padding_idx={padding_idx}".format(**self.__dict__)
+
+
+class LinearCrossEntropy(nn.Module):
+    """A linear head and its cross entropy in one module: ``forward(hidden, target)`` is the loss, :meth:`logits` what an
+    ``nn.Linear`` of the same weight would give."""
+
+    def __init__(self, in_features, num_classes, bias=True, ignore_index=-100, reduction="mean"):
+        super().__init__()
+        if reduction not in _REDUCTIONS:
+            raise ValueError("reduction must be 'none', 'sum' or 'mean', is %r" % (reduction,))
+        self.in_features, self.num_classes = in_features, num_classes
+        self.ignore_index, self.reduction = ignore_index, reduction
+        head = nn.Linear(in_features, num_classes, bias=bias)
+        self.weight, self.bias = head.weight, head.bias
+
+    def forward(self, hidden, target):
+        return linear_cross_entropy(hidden, self.weight, target, self.bias, self.ignore_index, self.reduction)
+
+    def logits(self, hidden):
+        return nn.functional.linear(hidden, self.weight, self.bias)
+
+    def extra_repr(self):
+        return "{}, {}, bias={}, ignore_index={}, reduction={}".format(
+            self.in_features, self.num_classes, self.bias is not None, self.ignore_index, self.reduction)

@@ -521,6 +521,59 @@ int ds_mul_conv2d_f32(const float *x_padded, const void *tiled, const float *bia
 int ds_mul_linear_f32(const float *xT, int ldx, const void *tiled, const float *bias, float *y, int M,
                       int K, int N, ds_stream_t stream);
 
+/* ---- operators of a training step -------------------------------------------------------------
+ * The two ends of a token model around shift layers, and the clipping of its gradients.  Elements are float32, bfloat16 or
+ * float16 (DS_F32, DS_BF16, DS_F16); sums are held in 32 bits or more and rounded once.  Rows may be `ld*` elements apart.
+ * Token numbers are int32 or int64 (id_bytes 4 or 8).  No counterpart in the reference's kernels. */
+
+enum { DS_F32 = 0, DS_BF16 = 1, DS_F16 = 2 };
+
+/* out[t][:] = scale * weight[ids[t]][:], out [T][D], weight [V][D].  A token number outside [0, V) gives a row of NaN. */
+int ds_embed(const void *ids, int id_bytes, const void *weight, int64_t ldw, void *out, int64_t T, int64_t V, int64_t D,
+             float scale, int type, ds_stream_t stream);
+
+/* dweight[v][:] = scale * sum of grad[t][:] over the tokens t of word v in ascending order; every row of dweight [V][D] is
+ * written.  Tokens equal to `padding`, or outside [0, V), add nothing (padding < 0: none is).  Bit-reproducible. */
+size_t ds_embed_grad_workspace_bytes(int64_t T, int64_t D);
+int ds_embed_grad(const void *ids, int id_bytes, const void *grad, int64_t ldg, void *dweight, int64_t T, int64_t V, int64_t D,
+                  int64_t padding, float scale, int type, void *workspace, size_t workspace_bytes, ds_stream_t stream);
+
+/* Reductions of ds_vocab_loss. */
+enum { DS_NONE = 0, DS_SUM = 1, DS_MEAN = 2 };
+
+/* Cross entropy of softmax(hidden weight^T + bias), hidden [T][D], weight [V][D], bias [V] or NULL of the same type.
+ * rows[t] is the loss of token t, 0 where target[t] == ignore and NaN where target[t] is neither that nor in [0, V); lse[t]
+ * the logarithm, base 2, of the sum of its exponentials; total[0] (DS_SUM, DS_MEAN) the sum of the rows or their mean over the
+ * counted ones (0 where none is), total[1] the share of one row in it.  The logits are not stored.
+ * workspace: 256-byte aligned, ds_vocab_workspace_bytes(..., grad) bytes, for grad 0 (loss) or 1 (gradients). */
+size_t ds_vocab_workspace_bytes(const void *hidden, int64_t ldh, const void *weight, int64_t ldw, int64_t T, int64_t D, int64_t V,
+                                int type, int grad);
+int ds_vocab_loss(const void *hidden, int64_t ldh, const void *weight, int64_t ldw, const void *bias, const void *target,
+                  int target_bytes, int64_t ignore, int64_t T, int64_t D, int64_t V, int type, int reduction, float *rows,
+                  float *lse, float *total, void *workspace, size_t workspace_bytes, ds_stream_t stream);
+
+/* Its gradients: dhidden [T][D], dweight [V][D], dbias [V], each of the operands' type, or NULL where it is not asked for.
+ * lse is ds_vocab_loss's.  Either row_grad [T] holds the gradient of each row's loss, or every counted row has
+ * grad[0] * share[0] (1 for a pointer that is NULL; share = total + 1 after DS_SUM or DS_MEAN). */
+int ds_vocab_loss_grad(const void *hidden, int64_t ldh, const void *weight, int64_t ldw, const void *bias, const void *target,
+                       int target_bytes, int64_t ignore, int64_t T, int64_t D, int64_t V, int type, const float *lse,
+                       const float *row_grad, const float *grad, const float *share, void *dhidden, void *dweight, void *dbias,
+                       void *workspace, size_t workspace_bytes, ds_stream_t stream);
+
+/* One tensor of ds_clip: n elements at src, and where their clipped values go (src itself for a clip in place). */
+typedef struct {
+    const void *src;
+    void *dst;
+    int64_t n;
+    int src_type, dst_type;
+} ds_tensor;
+
+/* The global norm of `count` tensors (an array on the host), norm[0] = sqrt(sum of squares) on the device (NULL: not wanted);
+ * with scale != 0 also dst = src * min(1, max_norm / (norm + 1e-6)).  Squares are summed in 64 bits.  Bit-reproducible. */
+size_t ds_clip_workspace_bytes(int count);
+int ds_clip(const ds_tensor *tensors, int count, float max_norm, int scale, float *norm, void *workspace,
+            size_t workspace_bytes, ds_stream_t stream);
+
 /* ---- measurement ----------------------------------------------------------------------- */
 
 /* VALU calibration: every lane of `blocks` x 256 threads runs `iters` x 64 independent
