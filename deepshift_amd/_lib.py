@@ -126,6 +126,8 @@ SIGNATURES = {
     "ds_vocab_loss": (_c_int, _matrix * 2 + [_ptr, _ptr, _c_int] + [_c_i64] * 4 + [_c_int, _c_int, _ptr, _ptr, _ptr, _ptr,
                                                                                    _size, _ptr]),
     "ds_vocab_loss_grad": (_c_int, _matrix * 2 + [_ptr, _ptr, _c_int] + [_c_i64] * 4 + [_c_int] + [_ptr] * 8 + [_size, _ptr]),
+    "ds_vocab_loss_step": (_c_int, _matrix * 2 + [_ptr, _ptr, _c_int] + [_c_i64] * 4 + [_c_int, _c_int] + [_ptr] * 7 +
+                           [_size, _ptr]),
     "ds_clip_workspace_bytes": (_size, [_c_int]),
     "ds_clip": (_c_int, [_tp, _c_int, _float, _c_int, _ptr, _ptr, _size, _ptr]),
     "ds_valu_calibrate": (_c_int, [_ptr, _c_int, _c_int, _ptr]),

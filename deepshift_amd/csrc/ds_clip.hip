@@ -8,31 +8,36 @@
 
 namespace ds {
 
-constexpr int kSpans = 128;        // per launch: 4 KB of arguments
-constexpr int kClipChunk = 16384;  // elements that a workgroup takes at a time
 constexpr int kClipBlocks = 2048;  // partial sums of one launch at most
 
+// The tensors of a launch: 3.9 KB of kernel arguments, 192 tensors where nothing is written elsewhere, else 136.
+template <bool ELSEWHERE>
 struct SpanTable {
+    static constexpr int kSpans = ELSEWHERE ? 136 : 192;
     const void *src[kSpans];
-    void *dst[kSpans];
-    int64_t n[kSpans];
+    int64_t n[kSpans];      // elements | type of src << 56 | type of dst << 60
     int32_t first[kSpans];  // chunks before this tensor
-    uint8_t src_type[kSpans], dst_type[kSpans];
-    int count, chunks;
-};
+    int count, chunks, chunk;
+    void *dst[ELSEWHERE ? kSpans : 1];
 
-// Which tensor holds chunk c: the last one that begins at or before it.  Every lane looks at two.
-__device__ __forceinline__ int span_of(const SpanTable &t, int c)
-{
-    const int lane = threadIdx.x & 63;
-    int n = 0;
+    __device__ int64_t elements(int i) const { return n[i] & 0xffffffffffffffll; }
+    __device__ int src_type(int i) const { return (int)(n[i] >> 56) & 15; }
+    __device__ int dst_type(int i) const { return (int)(n[i] >> 60) & 7; }
+    __device__ void *to(int i) const { return ELSEWHERE ? dst[i] : const_cast<void *>(src[i]); }
+
+    // Which tensor holds chunk c: the last one that begins at or before it.  Every lane looks at some.
+    __device__ int span_of(int c) const
+    {
+        const int lane = threadIdx.x & 63;
+        int found = 0;
 #pragma unroll
-    for (int j = 0; j < kSpans; j += 64) {
-        const int i = j + lane;
-        n += __popcll(__ballot(i < t.count && t.first[i] <= c));
+        for (int j = 0; j < kSpans; j += 64) {
+            const int i = j + lane;
+            found += __popcll(__ballot(i < count && i < kSpans && first[i < kSpans ? i : 0] <= c));
+        }
+        return __builtin_amdgcn_readfirstlane(found - 1);
     }
-    return __builtin_amdgcn_readfirstlane(n - 1);
-}
+};
 
 // Squares are added up in 64 bits: values of float32 up to its largest have a norm, and the order of the additions, which
 // is fixed all the same, would not show.
@@ -87,16 +92,16 @@ __device__ __forceinline__ double block_sum(double v, double *lds)
     return (lds[0] + lds[1]) + (lds[2] + lds[3]);
 }
 
-__global__ __launch_bounds__(256) void clip_norm_kernel(SpanTable t, double *__restrict__ part)
+__global__ __launch_bounds__(256) void clip_norm_kernel(SpanTable<false> t, double *__restrict__ part)
 {
     __shared__ double lds[4];
     double s = 0;
     for (int c = blockIdx.x; c < t.chunks; c += gridDim.x) {
-        const int i = span_of(t, c);
-        const int64_t at = (int64_t)(c - t.first[i]) * kClipChunk;
-        const int n = (int)min((int64_t)kClipChunk, t.n[i] - at);
-        if (t.src_type[i] == DS_F32) s += square_sum((const float *)t.src[i] + at, n);
-        else if (t.src_type[i] == DS_BF16) s += square_sum((const bf16_t *)t.src[i] + at, n);
+        const int i = t.span_of(c);
+        const int64_t at = (int64_t)(c - t.first[i]) * t.chunk;
+        const int n = (int)min((int64_t)t.chunk, t.elements(i) - at);
+        if (t.src_type(i) == DS_F32) s += square_sum((const float *)t.src[i] + at, n);
+        else if (t.src_type(i) == DS_BF16) s += square_sum((const bf16_t *)t.src[i] + at, n);
         else s += square_sum((const f16_t *)t.src[i] + at, n);
     }
     s = block_sum(s, lds);
@@ -118,10 +123,10 @@ __global__ __launch_bounds__(256) void clip_join_kernel(const double *__restrict
     if (threadIdx.x == 0) *norm = (float)n;
 }
 
-template <typename E, typename O>
+template <bool STREAM, typename E, typename O>
 __device__ __forceinline__ void scale_span(const E *x, O *y, int n, float pre, float f)
 {
-    constexpr int N = sizeof(E) == 4 && sizeof(O) == 4 ? 4 : 8;
+    constexpr int N = sizeof(O) == 4 ? 4 : 8;
     int i = 0;
     if (((uintptr_t)x % (sizeof(E) * N < 16 ? sizeof(E) * N : 16)) == 0 && ((uintptr_t)y % (sizeof(O) * N < 16 ? sizeof(O) * N : 16)) == 0) {
         const int units = n / N;
@@ -137,7 +142,8 @@ __device__ __forceinline__ void scale_span(const E *x, O *y, int n, float pre, f
                 Vec<O, N> o;
 #pragma unroll
                 for (int e = 0; e < N; ++e) o.v[e] = from_float<O>(to_float(got[j].v[e]) * pre * f);
-                ((Vec<O, N> *)y)[u + j * 256] = o;
+                if constexpr (STREAM && sizeof(O) * N == 16) store_streaming((Vec<O, N> *)y + u + j * 256, o);
+                else ((Vec<O, N> *)y)[u + j * 256] = o;
             }
         }
         i = units * N;
@@ -145,16 +151,18 @@ __device__ __forceinline__ void scale_span(const E *x, O *y, int n, float pre, f
     for (i += threadIdx.x; i < n; i += 256) y[i] = from_float<O>(to_float(x[i]) * pre * f);
 }
 
-template <typename E>
-__device__ __forceinline__ void scale_any(const SpanTable &t, int i, int64_t at, int n, float pre, float f)
+template <bool STREAM, typename E, typename TABLE>
+__device__ __forceinline__ void scale_any(const TABLE &t, int i, int64_t at, int n, float pre, float f)
 {
     const E *x = (const E *)t.src[i] + at;
-    if (t.dst_type[i] == DS_F32) scale_span(x, (float *)t.dst[i] + at, n, pre, f);
-    else if (t.dst_type[i] == DS_BF16) scale_span(x, (bf16_t *)t.dst[i] + at, n, pre, f);
-    else scale_span(x, (f16_t *)t.dst[i] + at, n, pre, f);
+    if (t.dst_type(i) == DS_F32) scale_span<STREAM>(x, (float *)t.to(i) + at, n, pre, f);
+    else if (t.dst_type(i) == DS_BF16) scale_span<STREAM>(x, (bf16_t *)t.to(i) + at, n, pre, f);
+    else scale_span<STREAM>(x, (f16_t *)t.to(i) + at, n, pre, f);
 }
 
-__global__ __launch_bounds__(256) void clip_scale_kernel(SpanTable t, const double *__restrict__ part, int parts,
+// Chunks are taken from the last one down: what the norm read last is the likeliest to be in cache still.
+template <bool ELSEWHERE>
+__global__ __launch_bounds__(256) void clip_scale_kernel(SpanTable<ELSEWHERE> t, const double *__restrict__ part, int parts,
                                                          float max_norm, float *__restrict__ norm)
 {
     __shared__ double lds[4];
@@ -164,45 +172,55 @@ __global__ __launch_bounds__(256) void clip_scale_kernel(SpanTable t, const doub
     // a factor that float32 would hold with fewer bits is applied in two steps; a norm that is no number stays one
     const float pre = ratio < 0x1p-64 ? 0x1p-64f : 1.f;
     const float f = ratio >= 1.0 ? 1.f : (float)(ratio / pre);
-    for (int c = blockIdx.x; c < t.chunks; c += gridDim.x) {
-        const int i = span_of(t, c);
-        // a factor of one leaves a tensor in place as it is
-        if (f == 1.f && t.src[i] == t.dst[i] && t.src_type[i] == t.dst_type[i]) continue;
-        const int64_t at = (int64_t)(c - t.first[i]) * kClipChunk;
-        const int m = (int)min((int64_t)kClipChunk, t.n[i] - at);
-        if (t.src_type[i] == DS_F32) scale_any<float>(t, i, at, m, pre, f);
-        else if (t.src_type[i] == DS_BF16) scale_any<bf16_t>(t, i, at, m, pre, f);
-        else scale_any<f16_t>(t, i, at, m, pre, f);
+    // a factor of one leaves tensors in place as they are
+    if (!ELSEWHERE && f == 1.f && pre == 1.f) return;
+    for (int c = t.chunks - 1 - (int)blockIdx.x; c >= 0; c -= gridDim.x) {
+        const int i = t.span_of(c);
+        const int64_t at = (int64_t)(c - t.first[i]) * t.chunk;
+        const int m = (int)min((int64_t)t.chunk, t.elements(i) - at);
+        if (t.src_type(i) == DS_F32) scale_any<ELSEWHERE, float>(t, i, at, m, pre, f);
+        else if (t.src_type(i) == DS_BF16) scale_any<ELSEWHERE, bf16_t>(t, i, at, m, pre, f);
+        else scale_any<ELSEWHERE, f16_t>(t, i, at, m, pre, f);
     }
 }
 
 // The tensors from `from` on that one launch takes; returns the first one that it does not.
-int fill_table(const ds_tensor *tensors, int count, int from, SpanTable &t, int64_t *too_many)
+template <bool ELSEWHERE>
+int fill_table(const ds_tensor *tensors, int count, int from, int chunk, SpanTable<ELSEWHERE> &t)
 {
     t.count = 0;
+    t.chunk = chunk;
     int64_t chunks = 0;
     int i = from;
-    for (; i < count && t.count < kSpans; ++i) {
+    for (; i < count && t.count < t.kSpans; ++i) {
         const ds_tensor &x = tensors[i];
         if (x.n == 0) continue;
-        const int64_t more = (x.n + kClipChunk - 1) / kClipChunk;
-        if (chunks + more > 0x7fffffff - kClipBlocks) {
-            if (t.count == 0) *too_many = 1;
-            break;
-        }
         t.src[t.count] = x.src;
-        t.dst[t.count] = x.dst;
-        t.n[t.count] = x.n;
-        t.src_type[t.count] = (uint8_t)x.src_type;
-        t.dst_type[t.count] = (uint8_t)x.dst_type;
+        t.n[t.count] = x.n | (int64_t)x.src_type << 56 | (int64_t)x.dst_type << 60;
+        if (ELSEWHERE) t.dst[t.count] = x.dst;
         t.first[t.count++] = (int32_t)chunks;
-        chunks += more;
+        chunks += (x.n + chunk - 1) / chunk;
     }
     t.chunks = (int)chunks;
     return i;
 }
 
-inline size_t clip_bytes(int count) { return (size_t)(count / kSpans + 1) * kClipBlocks * sizeof(double); }
+template <bool ELSEWHERE>
+int scale_tensors(const ds_tensor *tensors, int count, int chunk, const double *part, int parts, float max_norm, float *norm,
+                  hipStream_t st)
+{
+    SpanTable<ELSEWHERE> t;
+    for (int i = 0; i < count;) {
+        i = fill_table(tensors, count, i, chunk, t);
+        if (t.chunks == 0) continue;
+        const int blocks = t.chunks < kClipBlocks ? t.chunks : kClipBlocks;
+        hipLaunchKernelGGL((clip_scale_kernel<ELSEWHERE>), dim3(blocks), dim3(256), 0, st, t, part, parts, max_norm, norm);
+        norm = nullptr;
+    }
+    return launch_status();
+}
+
+inline size_t clip_bytes(int count) { return (size_t)(count / SpanTable<false>::kSpans + 1) * kClipBlocks * sizeof(double); }
 
 }  // namespace ds
 
@@ -214,37 +232,35 @@ DS_EXPORT int ds_clip(const ds_tensor *tensors, int count, float max_norm, int s
                       size_t workspace_bytes, ds_stream_t stream)
 {
     if (count < 0 || (count > 0 && !tensors) || (!norm && !scale) || !(max_norm >= 0.f || !scale)) return DS_EINVAL;
+    int64_t total = 0;
+    bool elsewhere = false;
     for (int i = 0; i < count; ++i) {
         const ds_tensor &x = tensors[i];
-        if (x.n < 0 || !element_bytes(x.src_type) || (x.n > 0 && !x.src)) return DS_EINVAL;
-        if (scale && (!element_bytes(x.dst_type) || (x.n > 0 && !x.dst))) return DS_EINVAL;
-        if ((uintptr_t)x.src % element_bytes(x.src_type) || (scale && (uintptr_t)x.dst % element_bytes(x.dst_type))) return DS_EINVAL;
+        const int from = element_bytes(x.src_type), to = scale ? element_bytes(x.dst_type) : from;
+        if (x.n < 0 || !from || !to || (x.n > 0 && (!x.src || (scale && !x.dst)))) return DS_EINVAL;
+        if ((uintptr_t)x.src % from || (scale && (uintptr_t)x.dst % to)) return DS_EINVAL;
+        if (x.n >= (int64_t)1 << 40 || (total += x.n) >= (int64_t)1 << 40) return DS_ETOOLARGE;
+        if (scale && x.n > 0 && (x.src != x.dst || x.src_type != x.dst_type)) elsewhere = true;
     }
     if (!workspace || workspace_bytes < clip_bytes(count) || (uintptr_t)workspace % 8) return DS_EWORKSPACE;
+    // Chunks of 64 KB and more keep a workgroup's loads together; few elements are cut smaller, to reach every CU.
+    int chunk = 16384;
+    while (chunk > 2048 && total / chunk < 2 * device_cus()) chunk >>= 1;
     hipStream_t st = (hipStream_t)stream;
     double *part = (double *)workspace;
-    SpanTable t;
-    int64_t too_many = 0;
-    int parts = 0, launches = 0;
+    SpanTable<false> t;
+    int parts = 0;
     for (int i = 0; i < count;) {
-        i = fill_table(tensors, count, i, t, &too_many);
-        if (too_many || (size_t)(parts + kClipBlocks) * sizeof(double) > clip_bytes(count)) return DS_ETOOLARGE;
+        i = fill_table(tensors, count, i, chunk, t);
         if (t.chunks == 0) continue;
         const int blocks = t.chunks < kClipBlocks ? t.chunks : kClipBlocks;
         hipLaunchKernelGGL(clip_norm_kernel, dim3(blocks), dim3(256), 0, st, t, part + parts);
         parts += blocks;
-        ++launches;
     }
-    if (!scale || launches == 0) {
-        if (!norm) return DS_OK;
-        hipLaunchKernelGGL(clip_join_kernel, dim3(1), dim3(256), 0, st, part, parts, norm);
+    if (!scale || parts == 0) {
+        if (norm) hipLaunchKernelGGL(clip_join_kernel, dim3(1), dim3(256), 0, st, part, parts, norm);
         return launch_status();
     }
-    for (int i = 0, done = 0; i < count; ) {
-        i = fill_table(tensors, count, i, t, &too_many);
-        if (t.chunks == 0) continue;
-        const int blocks = t.chunks < kClipBlocks ? t.chunks : kClipBlocks;
-        hipLaunchKernelGGL(clip_scale_kernel, dim3(blocks), dim3(256), 0, st, t, part, parts, max_norm, done++ == 0 ? norm : nullptr);
-    }
-    return launch_status();
+    if (elsewhere) return scale_tensors<true>(tensors, count, chunk, part, parts, max_norm, norm, st);
+    return scale_tensors<false>(tensors, count, chunk, part, parts, max_norm, norm, st);
 }

@@ -40,7 +40,7 @@ __global__ __launch_bounds__(256) void embed_kernel(const void *__restrict__ ids
         Vec<E, N> o;
 #pragma unroll
         for (int e = 0; e < N; ++e) o.v[e] = from_float<E>(id[j] >= 0 ? to_float(got[j].v[e]) * scale : NAN);
-        ((Vec<E, N> *)out)[at] = o;
+        store_streaming((Vec<E, N> *)out + at, o);
     }
 }
 
@@ -65,7 +65,7 @@ int launch_embed(const void *ids, int wide, const void *w, void *out, int64_t T,
 
 // ---- tokens sorted by word ------------------------------------------------------------------------------------
 
-constexpr uint32_t kNoWord = 0xffffffffu;  // sorts behind every word: padding, and what is no word at all
+constexpr uint32_t kNoWord = 0xfffffffeu;  // sorts behind every word: padding, and what is no word at all
 
 __device__ __forceinline__ uint32_t key_at(const void *ids, int wide, int64_t i, int64_t V, int64_t padding)
 {
@@ -76,13 +76,13 @@ __device__ __forceinline__ uint32_t key_at(const void *ids, int wide, int64_t i,
 // Up to kRankMost tokens: the place of a token is the number of tokens with a smaller word, or the same word and an earlier
 // position.  Every workgroup holds all words in LDS and places 64 tokens, its 16 waves each compare them with a sixteenth:
 // T * T comparisons, two instructions each.
-constexpr int kRankMost = 16384;
+constexpr int kRankMost = 16384;  // a multiple of 64
 
 __global__ __launch_bounds__(1024) void embed_rank_kernel(const void *__restrict__ ids, int wide, int T, int64_t V,
                                                           int64_t padding, uint32_t *__restrict__ keys,
                                                           uint32_t *__restrict__ pos)
 {
-    __shared__ uint32_t word[kRankMost + 64];
+    __shared__ __attribute__((aligned(16))) uint32_t word[kRankMost];
     __shared__ uint32_t before[16][64];
     const int padded = (T + 63) & ~63;
     for (int i = threadIdx.x; i < padded; i += 1024) word[i] = i < T ? key_at(ids, wide, i, V, padding) : kNoWord;
@@ -93,13 +93,15 @@ __global__ __launch_bounds__(1024) void embed_rank_kernel(const void *__restrict
     for (int g = wave * 64; g < padded; g += 16 * 64) {
         if (g == t0) {
             for (int i = 0; i < 64; ++i) n += word[g + i] < mine || (word[g + i] == mine && i < lane);
-        } else if (g < t0) {
-            // earlier positions come first among equals
-#pragma unroll 16
-            for (int i = 0; i < 64; ++i) n += word[g + i] <= mine;
         } else {
-#pragma unroll 16
-            for (int i = 0; i < 64; ++i) n += word[g + i] < mine;
+            // of two equal words the earlier one comes first
+            const uint32_t below = mine + (g < t0);
+            const uint4 *four = (const uint4 *)(word + g);
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                const uint4 w = four[i];
+                n += (w.x < below) + (w.y < below) + (w.z < below) + (w.w < below);
+            }
         }
     }
     before[wave][lane] = n;
@@ -116,7 +118,7 @@ __global__ __launch_bounds__(1024) void embed_rank_kernel(const void *__restrict
 // More tokens: a radix sort, least significant digit first, 9 bits a pass.  At most kSortBlocks workgroups, each with one
 // stretch of the tokens; the counts of all of them (512 digits x 64) are few enough that every workgroup adds up its own
 // offsets, so a pass is two launches.
-constexpr int kDigitBits = 9, kDigits = 1 << kDigitBits, kSortBlocks = 64, kSortTile = 2048;
+constexpr int kDigitBits = 9, kDigits = 1 << kDigitBits, kSortBlocks = 64, kSortTile = 1024;
 
 struct SortPass {
     const void *ids;  // first pass: the token numbers themselves; NULL later
@@ -124,7 +126,7 @@ struct SortPass {
     int64_t V, padding;
     const uint32_t *keys, *pos;
     uint32_t *out_keys, *out_pos;
-    uint32_t *counts;  // [kDigits][blocks]
+    uint32_t *counts;  // [blocks][kDigits]
     int64_t T, stretch;
     int shift;
 };
@@ -143,7 +145,7 @@ __global__ __launch_bounds__(256) void embed_count_kernel(SortPass p)
     for (int64_t i = from + threadIdx.x; i < to; i += 256)
         atomicAdd(&count[(sort_key(p, i) >> p.shift) & (kDigits - 1)], 1u);  // whole numbers: any order gives the same
     __syncthreads();
-    for (int d = threadIdx.x; d < kDigits; d += 256) p.counts[d * gridDim.x + blockIdx.x] = count[d];
+    for (int d = threadIdx.x; d < kDigits; d += 256) p.counts[blockIdx.x * kDigits + d] = count[d];
 }
 
 __global__ __launch_bounds__(256) void embed_scatter_kernel(SortPass p)
@@ -155,16 +157,13 @@ __global__ __launch_bounds__(256) void embed_scatter_kernel(SortPass p)
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
     {
         // two neighbouring digits a thread: totals, then an exclusive scan over the 512 digits
-        uint32_t total[2], mine[2];
-#pragma unroll
-        for (int k = 0; k < 2; ++k) {
-            const uint32_t *c = p.counts + (threadIdx.x * 2 + k) * gridDim.x;
-            total[k] = mine[k] = 0;
-            for (unsigned b = 0; b < gridDim.x; ++b) {
-                const uint32_t v = c[b];
-                total[k] += v;
-                mine[k] += b < blockIdx.x ? v : 0;
-            }
+        uint32_t total[2] = {0, 0}, mine[2] = {0, 0};
+        const uint2 *c = (const uint2 *)p.counts + threadIdx.x;
+#pragma unroll 16
+        for (unsigned b = 0; b < gridDim.x; ++b) {
+            const uint2 v = c[b * (kDigits / 2)];
+            total[0] += v.x, total[1] += v.y;
+            if (b < blockIdx.x) mine[0] += v.x, mine[1] += v.y;
         }
         const uint32_t own = total[0] + total[1];
         uint32_t run = own;
@@ -293,50 +292,106 @@ __global__ __launch_bounds__(64) void embed_sum_kernel(const E *__restrict__ g, 
     }
 }
 
+// The first of `n` sorted keys that is not below v, found by a whole wave: 64 probes a round.
+__device__ __forceinline__ uint32_t wave_lower_bound(const uint32_t *__restrict__ keys, uint32_t n, uint32_t v)
+{
+    uint32_t lo = 0, left = n;  // the answer is in [lo, lo + left]
+    while (left > 0) {
+        const uint32_t stride = (left + 63) / 64, at = (threadIdx.x & 63) * stride;
+        const bool below = at < left && keys[lo + at] < v;
+        const uint32_t passed = (uint32_t)__popcll(__ballot(below));
+        if (passed == 0) break;
+        // keys[lo + (passed - 1) * stride] is below v, the next probe is not
+        const uint32_t skip = (passed - 1) * stride + 1;
+        const uint32_t end = passed * stride < left ? passed * stride : left;
+        lo += skip, left = end - skip;
+    }
+    return lo;
+}
+
 // Every row that embed_sum_kernel has not finished: words without tokens get zeros, words in several chunks their joined
-// sums.  A workgroup owns `rows` rows (at most 256) and finds where their tokens begin by bisection, a thread per row.
+// sums.  A workgroup owns `rows` rows (at most 256, together a multiple of 16 bytes): two waves find the stretch of tokens
+// that belongs to them; inside it the rows' own stretches are marked by its tokens, or bisected where it is long.
 template <typename E, int N>
 __global__ __launch_bounds__(256) void embed_finish_kernel(const uint32_t *__restrict__ keys, const float *__restrict__ part,
                                                            E *__restrict__ dw, int64_t T, int64_t V, int64_t D, int chunk,
-                                                           int rows, float scale)
+                                                           int rows, float scale, FastDiv by_row)
 {
-    __shared__ uint32_t begin[257];
+    __shared__ uint32_t bound[2], begin[257];
+    __shared__ uint8_t empty[256];
     const int64_t v0 = (int64_t)blockIdx.x * rows;
     const int mine = (int)min((int64_t)rows, V - v0);
-    for (int i = threadIdx.x; i <= mine; i += 256) {
-        const uint32_t v = (uint32_t)(v0 + i);
-        uint32_t lo = 0, hi = (uint32_t)T;
-        while (lo < hi) {
-            const uint32_t mid = (lo + hi) >> 1;
-            if (keys[mid] < v) lo = mid + 1;
-            else hi = mid;
-        }
-        begin[i] = lo;
+    const int wave = threadIdx.x >> 6;
+    if (wave < 2) {
+        const uint32_t found = wave_lower_bound(keys, (uint32_t)T, (uint32_t)(v0 + (wave ? mine : 0)));
+        if ((threadIdx.x & 63) == 0) bound[wave] = found;
     }
     __syncthreads();
+    const uint32_t first = bound[0], end = bound[1];
+    if (end - first <= 1024) {
+        // every token whose word differs from the one before begins the rows in between
+        for (uint32_t i = first + threadIdx.x; i <= end; i += 256) {
+            const int row = i < end ? (int)(keys[i] - (uint32_t)v0) : mine;
+            for (int r = i > first ? (int)(keys[i - 1] - (uint32_t)v0) + 1 : 0; r <= row; ++r) begin[r] = i;
+        }
+    } else {
+        for (int i = threadIdx.x; i <= mine; i += 256) {
+            const uint32_t v = (uint32_t)(v0 + i);
+            uint32_t lo = first, hi = end;
+            while (lo < hi) {
+                const uint32_t mid = (lo + hi) >> 1;
+                if (keys[mid] < v) lo = mid + 1;
+                else hi = mid;
+            }
+            begin[i] = lo;
+        }
+    }
+    __syncthreads();
+    if ((int)threadIdx.x < mine) empty[threadIdx.x] = begin[threadIdx.x] == begin[threadIdx.x + 1];
+    __syncthreads();
+    // zeros, 16 bytes at a time where the whole of it lies in empty rows
+    constexpr int kUnit = 16 / sizeof(E);
+    E *const block = dw + v0 * D;
+    const int64_t total = mine * D;
+    const bool aligned = ((uintptr_t)block & 15) == 0;
+    for (int64_t u = (int64_t)threadIdx.x * kUnit; u < total; u += 256 * kUnit) {
+        const uint32_t r0 = div_by((uint32_t)u, by_row);
+        const int64_t last = min(u + kUnit, total) - 1;
+        const uint32_t r1 = div_by((uint32_t)last, by_row);
+        if (aligned && u + kUnit <= total && empty[r0] && (r1 == r0 || (r1 == r0 + 1 && empty[r1]))) {
+            *(uint4 *)(block + u) = uint4{0, 0, 0, 0};
+        } else {
+            for (int64_t i = u; i <= last; ++i)
+                if (empty[div_by((uint32_t)i, by_row)]) block[i] = from_float<E>(0.f);
+        }
+    }
+    if (first == end) return;
     const int64_t per_row = D / N;
     for (int r = 0; r < mine; ++r) {
         const uint32_t from = begin[r], to = begin[r + 1];
-        const uint32_t c0 = from / chunk, c1 = to > from ? (to - 1) / chunk : c0;
-        if (to > from && c0 == c1) continue;
-        E *row = dw + (v0 + r) * D;
+        if (to == from) continue;
+        const uint32_t c0 = from / chunk, c1 = (to - 1) / chunk;
+        if (c0 == c1) continue;
         for (int64_t u = threadIdx.x; u < per_row; u += 256) {
             float acc[N];
+            const float *p = part + u * N;
 #pragma unroll
-            for (int e = 0; e < N; ++e) acc[e] = 0.f;
-            if (to > from) {
-                const float *p = part + u * N;
+            for (int e = 0; e < N; ++e) acc[e] = p[((int64_t)c0 * 2 + 1) * D + e];
+            constexpr int kAhead = N <= 2 ? 24 : 8;  // partial sums on their way
+            for (uint32_t c = c0 + 1; c <= c1; c += kAhead) {
+                Vec<float, N> got[kAhead];
 #pragma unroll
-                for (int e = 0; e < N; ++e) acc[e] = p[((int64_t)c0 * 2 + 1) * D + e];
-#pragma unroll 8
-                for (uint32_t c = c0 + 1; c <= c1; ++c)
+                for (int j = 0; j < kAhead; ++j)
+                    if (c + j <= c1) got[j] = *(const Vec<float, N> *)(p + (int64_t)(c + j) * 2 * D);
 #pragma unroll
-                    for (int e = 0; e < N; ++e) acc[e] += p[(int64_t)c * 2 * D + e];
+                for (int j = 0; j < kAhead; ++j)
+#pragma unroll
+                    for (int e = 0; e < N; ++e) acc[e] += c + j <= c1 ? got[j].v[e] : 0.f;
             }
             Vec<E, N> o;
 #pragma unroll
             for (int e = 0; e < N; ++e) o.v[e] = from_float<E>(acc[e] * scale);
-            ((Vec<E, N> *)row)[u] = o;
+            ((Vec<E, N> *)(block + r * D))[u] = o;
         }
     }
 }
@@ -370,9 +425,13 @@ int launch_embed_grad(const uint32_t *keys, const uint32_t *pos, const void *g, 
     const int n = vector_elements(sizeof(E), {D, ldg}, {g, dw});
     const int chunk = embed_chunk(T);
     const int64_t chunks = (T + chunk - 1) / chunk, slices = (D / n + 63) / 64;
-    // about 16 KB of the result a workgroup
+    // 16 to 64 KB of the result a workgroup, in whole 16-byte units: the search for its tokens is paid for by larger ones,
+    // enough workgroups for every CU by smaller ones
+    constexpr int64_t kUnit = 16 / sizeof(E);
     const int64_t row_bytes = D * (int64_t)sizeof(E);
-    const int rows = (int)min((int64_t)256, max((int64_t)1, (int64_t)16384 / row_bytes));
+    const int64_t region = min((int64_t)65536, max((int64_t)16384, V * row_bytes / (8 * device_cus())));
+    const int rows = (int)min((int64_t)256, max(kUnit, region / row_bytes / kUnit * kUnit));
+    if (rows * D > 0x7fffffff) return DS_ETOOLARGE;
     const int64_t finish = (V + rows - 1) / rows;
     if (chunks > 0x7fffffff || slices > 65535 || finish > 0x7fffffff) return DS_ETOOLARGE;
 #define DS_LAUNCH(N)                                                                                                    \
@@ -381,7 +440,7 @@ int launch_embed_grad(const uint32_t *keys, const uint32_t *pos, const void *g, 
             hipLaunchKernelGGL((embed_sum_kernel<E, N>), dim3((unsigned)chunks, (unsigned)slices), dim3(64), 0, st,     \
                                (const E *)g, ldg, keys, pos, (E *)dw, part, T, D, chunk, scale);                        \
         hipLaunchKernelGGL((embed_finish_kernel<E, N>), dim3((unsigned)finish), dim3(256), 0, st, keys, part, (E *)dw, T, V, \
-                           D, chunk, rows, scale);                                                                      \
+                           D, chunk, rows, scale, fast_div((uint32_t)D));                                                                      \
     } while (0)
     if (n == 8) { if constexpr (sizeof(E) == 2) DS_LAUNCH(8); }
     else if (n == 4) DS_LAUNCH(4);
@@ -402,9 +461,9 @@ int sort_tokens(const void *ids, int wide, int64_t T, int64_t V, int64_t padding
             hipLaunchKernelGGL(embed_rank_kernel, dim3((unsigned)((T + 63) / 64)), dim3(1024), 0, st, ids, wide, (int)T, V,
                                padding, k[0], p[0]);
     } else if (T > 0) {
-        // kNoWord has every bit set: one value more than the words need
+        // the low bits of kNoWord, all set but the last, have to stay above every word
         int bits = 1;
-        while (((int64_t)1 << bits) <= V) ++bits;
+        while (((int64_t)1 << bits) <= V + 1) ++bits;
         int64_t blocks = min((int64_t)kSortBlocks, (T + kSortTile - 1) / kSortTile);
         const int64_t stretch = ((T + blocks - 1) / blocks + kSortTile - 1) / kSortTile * kSortTile;
         blocks = (T + stretch - 1) / stretch;

@@ -28,6 +28,23 @@ template <> __device__ __forceinline__ f16_t from_float<f16_t>(float v)
 // N elements that travel as one access.
 template <typename E, int N> struct alignas(sizeof(E) * N) Vec { E v[N]; };
 
+// A result that nobody reads soon.
+template <typename E, int N>
+__device__ __forceinline__ void store_streaming(Vec<E, N> *to, const Vec<E, N> &v)
+{
+    constexpr int kBytes = sizeof(E) * N;
+    if constexpr (kBytes == 16) {
+        typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+        __builtin_nontemporal_store(__builtin_bit_cast(u32x4, v), (u32x4 *)to);
+    } else if constexpr (kBytes == 8) {
+        __builtin_nontemporal_store(__builtin_bit_cast(uint64_t, v), (uint64_t *)to);
+    } else if constexpr (kBytes == 4) {
+        __builtin_nontemporal_store(__builtin_bit_cast(uint32_t, v), (uint32_t *)to);
+    } else {
+        __builtin_nontemporal_store(__builtin_bit_cast(uint16_t, v), (uint16_t *)to);
+    }
+}
+
 inline int element_bytes(int type) { return type == DS_F32 ? 4 : type == DS_BF16 || type == DS_F16 ? 2 : 0; }
 
 // The widest access, in elements of `bytes`, that every one of the sizes (in elements) and addresses allows.

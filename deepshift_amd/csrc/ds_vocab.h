@@ -84,12 +84,14 @@ struct Args {
     int64_t ldp, prob_plane;
     float *bias_part;     // [tiles_n][ld of the piece]: sums over the rows of a tile, or NULL
     int ld_bias_part;
+    void *bias_out;       // one tile holds all rows: the bias's gradient itself (times factor), or NULL
+    uint32_t *arrived;    // kStats: set to 0, for row_kernel
     // kOut
     float *slice;         // [splits][N][M] float, or NULL: final
     void *out;            // [N] rows of type out_type, ldo apart
     int64_t ldo;
     int out_type;
-    const float *factor[2];  // final: what to multiply with, 1 value each, or NULL
+    const float *factor[2];  // what results are multiplied with, 1 value each, or NULL
     int n_store;          // rows of C that exist (N may be rounded up for the loads)
 };
 
@@ -213,28 +215,45 @@ __device__ __forceinline__ int64_t target_at(const Args &a, int t)
 }
 
 // What sums of probabilities are multiplied with on their way out.
+__device__ __forceinline__ float factor_of(const float *const *f) { return (f[0] ? *f[0] : 1.f) * (f[1] ? *f[1] : 1.f); }
 template <typename P>
 __device__ __forceinline__ float out_factor(const float *const *f)
 {
-    return (f[0] ? *f[0] : 1.f) * (f[1] ? *f[1] : 1.f) * (P::half ? 1.f / kProbScale : 1.f);
+    return factor_of(f) * (P::half ? 1.f / kProbScale : 1.f);
 }
+template <typename P> struct ElementOf { typedef bf16_t type; };
+template <> struct ElementOf<F16> { typedef f16_t type; };
+template <> struct ElementOf<Split> { typedef float type; };
 
+// LDS of a workgroup: the stages, and what the epilogue of the logits needs to know of its words and tokens, fetched before
+// the products start (one load after another behind them took half of a short reduction's time).
+template <typename P, int BM, int BN, int STAGES>
+constexpr int kStagesBytes = STAGES * P::planes * (BM + BN) * kStep * 2;
+template <int BM, int BN>
+struct Known {
+    float bias[BM];
+    int want[BN];     // the target, counted from the tile's first word, where it lies in the tile; else -1
+    float lse[BN], scale[BN];
+};
+template <typename P, int BM, int BN, int STAGES, bool LOGITS>
+constexpr int kLdsBytes = kStagesBytes<P, BM, BN, STAGES> + (LOGITS ? (int)sizeof(Known<BM, BN>) : 0);
+
+// One tile of a product, by a whole workgroup; `block` counts the product's workgroups.
 template <typename P, int BM, int BN, int WM, int WN, bool A_ACROSS, bool B_ACROSS, int KIND, int STAGES>
-__global__ __launch_bounds__(WM * WN * 64) void product_kernel(Args g)
+__device__ __forceinline__ void product_tile(const Args &g, const int block, char *lds)
 {
     constexpr int WAVES = WM * WN, MT = BM / WM / 16, NT = BN / WN / 16, NP = P::planes;
     using TA = Tile<BM, A_ACROSS, WAVES>;
     using TB = Tile<BN, B_ACROSS, WAVES>;
     constexpr int kStageBytes = NP * (TA::bytes + TB::bytes);
     constexpr int kInFlight = NP * (TA::mine + TB::mine);  // loads of one stage and wave
-    __shared__ __attribute__((aligned(1024))) char lds[STAGES * kStageBytes];
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
     const int wm = wave % WM, wn = wave / WM;
 
     int tm, tn;
     const int tiles = g.tiles_m * g.tiles_n;
-    const int split = blockIdx.x / tiles;
-    tile_of(blockIdx.x - split * tiles, g.tiles_m, g.tiles_n, &tm, &tn);
+    const int split = block / tiles;
+    tile_of(block - split * tiles, g.tiles_m, g.tiles_n, &tm, &tn);
     const int m0 = tm * BM, n0 = tn * BN;
     const int k_from = split * g.k_split, k_to = min(g.K, k_from + g.k_split);
     const int steps = (k_to - k_from + kStep - 1) / kStep;
@@ -265,10 +284,31 @@ __global__ __launch_bounds__(WM * WN * 64) void product_kernel(Args g)
 #pragma unroll
         for (int j = 0; j < NT; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
 
+    Known<BM, BN> &known = *(Known<BM, BN> *)(lds + kStagesBytes<P, BM, BN, STAGES>);
+    static_assert(BM <= WAVES * 64 && BN <= WAVES * 64, "a thread per word and token");
+    float bias = 0.f, lse = 0.f, scale = 0.f;
+    int want = -1;
+    if constexpr (KIND != kOut) {
+        const int m = m0 + threadIdx.x, n = n0 + threadIdx.x;
+        if (threadIdx.x < BM && m < g.M) bias = bias_at(g, g.v0 + m);
+        if (threadIdx.x < BN && n < g.N) {
+            const int64_t y = target_at(g, n), here = y - g.v0 - m0;
+            if (here >= 0 && here < BM && m0 + here < g.M) want = (int)here;
+            if constexpr (KIND == kProb) {
+                lse = g.lse[n];
+                scale = y == g.ignore ? 0.f : y < 0 || y >= g.V ? NAN : g.row_scale ? g.row_scale[n] : 1.f;
+            }
+        }
+    }
+
     // Stages past the end are fetched too, as zeros (k_left <= 0 fetches nothing): the number of loads in flight is the same
     // in every step, and nothing past the operands is read.
 #pragma unroll
     for (int s = 0; s < STAGES - 1; ++s) fetch_stage(s);
+    if constexpr (KIND != kOut) {
+        if (threadIdx.x < BM) known.bias[threadIdx.x] = bias;
+        if (threadIdx.x < BN) known.want[threadIdx.x] = want, known.lse[threadIdx.x] = lse, known.scale[threadIdx.x] = scale;
+    }
     int slot = 0;
     for (int s = 0; s < steps; ++s) {
         // this wave's part of the stage has arrived, and it has read the slot that is filled next; then everyone's
@@ -325,7 +365,8 @@ __global__ __launch_bounds__(WM * WN * 64) void product_kernel(Args g)
     asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
     __syncthreads();
 
-    const int m_lane = m0 + wm * MT * 16 + (lane >> 4) * 4, n_lane = n0 + wn * NT * 16 + (lane & 15);
+    const int m_in = wm * MT * 16 + (lane >> 4) * 4, n_in = wn * NT * 16 + (lane & 15);  // of this lane, in the tile
+    const int m_lane = m0 + m_in, n_lane = n0 + n_in;
     float *fl = (float *)lds;
     if constexpr (KIND != kOut) {
         // acc becomes the logits in base 2
@@ -333,19 +374,18 @@ __global__ __launch_bounds__(WM * WN * 64) void product_kernel(Args g)
         for (int i = 0; i < MT; ++i)
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-                const int m = m_lane + i * 16 + r;
-                const bool real = m < g.M;
-                const float b = real ? bias_at(g, g.v0 + m) : 0.f;
+                const bool real = m_lane + i * 16 + r < g.M;
+                const float b = known.bias[m_in + i * 16 + r];
 #pragma unroll
                 for (int j = 0; j < NT; ++j) acc[i][j][r] = real ? (acc[i][j][r] + b) * kLog2e : -INFINITY;
             }
     }
     if constexpr (KIND == kStats) {
+        if (block == 0 && threadIdx.x == 0) *g.arrived = 0;
 #pragma unroll
         for (int j = 0; j < NT; ++j) {
             const int t = n_lane + j * 16;
-            const int64_t from_here = t < g.N ? target_at(g, t) - g.v0 - m_lane : -1;
-            const int want = from_here >= 0 && from_here < BM ? (int)from_here : -1;
+            const int at = known.want[n_in + j * 16] - m_in;  // below 0 or past this lane's words: not here
             float top = -INFINITY;
 #pragma unroll
             for (int i = 0; i < MT; ++i)
@@ -353,7 +393,7 @@ __global__ __launch_bounds__(WM * WN * 64) void product_kernel(Args g)
                 for (int r = 0; r < 4; ++r) {
                     // a maximum that a value which is no number does not slip through
                     top = acc[i][j][r] > top || acc[i][j][r] != acc[i][j][r] ? acc[i][j][r] : top;
-                    if (want == i * 16 + r && m_lane + i * 16 + r < g.M) g.picked[t] = acc[i][j][r];
+                    if (at == i * 16 + r) g.picked[t] = acc[i][j][r];
                 }
             float sum = 0.f;
             // a column of nothing but -inf keeps a sum of 0
@@ -400,17 +440,14 @@ __global__ __launch_bounds__(WM * WN * 64) void product_kernel(Args g)
         for (int j = 0; j < NT; ++j) {
             const int t = n_lane + j * 16;
             const bool real = t < g.N;
-            const int64_t y = real ? target_at(g, t) : 0;
-            const float lse = real ? g.lse[t] : 0.f;
-            const float scale = !real || y == g.ignore ? 0.f : y < 0 || y >= g.V ? NAN : g.row_scale ? g.row_scale[t] : 1.f;
-            const int64_t from_here = y - g.v0 - m_lane;
-            const int want = from_here >= 0 && from_here < BM ? (int)from_here : -1;
+            const float lse = known.lse[n_in + j * 16], scale = known.scale[n_in + j * 16];
+            const int at = known.want[n_in + j * 16] - m_in;
 #pragma unroll
             for (int i = 0; i < MT; ++i) {
                 float p[4];
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
-                    const float e = exp2f(acc[i][j][r] - lse) - (want == i * 16 + r ? 1.f : 0.f);
+                    const float e = exp2f(acc[i][j][r] - lse) - (at == i * 16 + r ? 1.f : 0.f);
                     // rows that do not count leave nothing, whatever their logits are; neither do words past the end
                     p[r] = scale == 0.f || m_lane + i * 16 + r >= g.M ? 0.f : e * scale;
                     over_n[i][r] += p[r];
@@ -437,7 +474,9 @@ __global__ __launch_bounds__(WM * WN * 64) void product_kernel(Args g)
                 }
             }
         }
-        if (g.bias_part) {
+        if (g.bias_part || g.bias_out) {
+            typedef typename ElementOf<P>::type E;
+            const float factor = g.bias_out ? factor_of(g.factor) : 1.f;
 #pragma unroll
             for (int i = 0; i < MT; ++i)
 #pragma unroll
@@ -452,7 +491,8 @@ __global__ __launch_bounds__(WM * WN * 64) void product_kernel(Args g)
                 float s = fl[c];
 #pragma unroll
                 for (int w = 1; w < WN; ++w) s += fl[w * BM + c];
-                g.bias_part[(int64_t)tn * g.ld_bias_part + m0 + c] = s;
+                if (g.bias_out) ((E *)g.bias_out)[m0 + c] = from_float<E>(s * factor);
+                else g.bias_part[(int64_t)tn * g.ld_bias_part + m0 + c] = s;
             }
         }
     }
@@ -504,6 +544,24 @@ __global__ __launch_bounds__(WM * WN * 64) void product_kernel(Args g)
     }
 }
 
+template <typename P, int BM, int BN, int WM, int WN, bool A_ACROSS, bool B_ACROSS, int KIND, int STAGES>
+__global__ __launch_bounds__(WM * WN * 64) void product_kernel(Args g)
+{
+    __shared__ __attribute__((aligned(1024))) char lds[kLdsBytes<P, BM, BN, STAGES, KIND != kOut>];
+    product_tile<P, BM, BN, WM, WN, A_ACROSS, B_ACROSS, KIND, STAGES>(g, blockIdx.x, lds);
+}
+
+// Both gradients' products in one launch, `first` workgroups for the first.
+template <typename P, int BM, int BN, int WM, int WN, int STAGES>
+__global__ __launch_bounds__(WM * WN * 64) void both_kernel(Args hidden, Args weight, int first)
+{
+    __shared__ __attribute__((aligned(1024))) char lds[kLdsBytes<P, BM, BN, STAGES, false>];
+    if ((int)blockIdx.x < first)
+        product_tile<P, BM, BN, WM, WN, true, false, kOut, STAGES>(hidden, blockIdx.x, lds);
+    else
+        product_tile<P, BM, BN, WM, WN, true, true, kOut, STAGES>(weight, blockIdx.x - first, lds);
+}
+
 // Which product a launch is.
 enum { kLogitStats = 0, kLogitProb = 1, kHidden = 2, kWeight = 3 };
 
@@ -513,17 +571,23 @@ template <> struct Shapes<Bf16> { static constexpr int m[3] = {256, 128, 128}, n
 template <> struct Shapes<F16> : Shapes<Bf16> {};
 template <> struct Shapes<Split> { static constexpr int m[3] = {256, 128, 64}, n[3] = {128, 128, 64}; };
 
-// Launches one product with tiles of shape `tile`; fills in the tile counts.  A translation unit per P.
-template <typename P> int launch_product(int kind, int tile, Args &g, hipStream_t st);
+// Launches one product with tiles of shape `tile`; fills in the tile counts.  With `other` the two gradients' products run in
+// one launch, both with that shape (g is kHidden, *other kWeight).  A translation unit per P.
+template <typename P> int launch_product(int kind, int tile, Args &g, Args *other, hipStream_t st);
 
 template <typename P, int BM, int BN, int WM, int WN, int STAGES>
-int launch_tiled(int kind, Args &g, hipStream_t st)
+int launch_tiled(int kind, Args &g, Args *other, hipStream_t st)
 {
-    g.tiles_m = ceil_div(g.M, BM), g.tiles_n = ceil_div(g.N, BN);
-    const int64_t blocks = (int64_t)g.tiles_m * g.tiles_n * g.splits;
-    if (blocks > 0x7fffffff) return DS_ETOOLARGE;
-    const dim3 grid((unsigned)blocks), threads(WM * WN * 64);
-    if (kind == kLogitStats)
+    auto count = [](Args &x) {
+        x.tiles_m = ceil_div(x.M, BM), x.tiles_n = ceil_div(x.N, BN);
+        return (int64_t)x.tiles_m * x.tiles_n * x.splits;
+    };
+    const int64_t blocks = count(g), more = other ? count(*other) : 0;
+    if (blocks + more > 0x7fffffff) return DS_ETOOLARGE;
+    const dim3 grid((unsigned)(blocks + more)), threads(WM * WN * 64);
+    if (other)
+        hipLaunchKernelGGL((both_kernel<P, BM, BN, WM, WN, STAGES>), grid, threads, 0, st, g, *other, (int)blocks);
+    else if (kind == kLogitStats)
         hipLaunchKernelGGL((product_kernel<P, BM, BN, WM, WN, false, false, kStats, STAGES>), grid, threads, 0, st, g);
     else if (kind == kLogitProb)
         hipLaunchKernelGGL((product_kernel<P, BM, BN, WM, WN, false, false, kProb, STAGES>), grid, threads, 0, st, g);

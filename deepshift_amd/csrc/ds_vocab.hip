@@ -16,52 +16,66 @@ namespace vocab {
 // Rows of D elements to rows of Dp (a multiple of 8, zeros behind D): 16-bit elements as they are, float32 as three planes.
 // Rows whose target is `ignore` (where targets are given) become zeros: tokens that do
 // not count leave nothing in the weights' gradient, not even a value that is no number.
+struct Pack {
+    const void *x;
+    int64_t ld, rows;
+    int D, Dp;
+    uint16_t *out;
+    int64_t plane;
+    const void *target;
+    int wide;
+    int64_t ignore;
+};
+
+// One operand, or two in one launch, the first by `first` workgroups.
 template <typename E, int N>
-__global__ __launch_bounds__(256) void pack_kernel(const E *__restrict__ x, int64_t ld, int64_t rows, int D, int Dp,
-                                                   uint16_t *__restrict__ out, int64_t plane, const void *__restrict__ target,
-                                                   int wide, int64_t ignore)
+__global__ __launch_bounds__(256) void pack_kernel(Pack one, Pack two, int first)
 {
-    const int units = Dp / N;
-    const int64_t total = rows * units;
-    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
+    const bool is_one = (int)blockIdx.x < first;
+    const Pack &p = is_one ? one : two;
+    const int block = is_one ? blockIdx.x : blockIdx.x - first, blocks = is_one ? first : gridDim.x - first;
+    const int units = p.Dp / N;
+    const int64_t total = p.rows * units;
+    for (int64_t i = (int64_t)block * 256 + threadIdx.x; i < total; i += (int64_t)blocks * 256) {
         const int64_t r = i / units;
         const int c = (int)(i - r * units) * N;
+        const E *x = (const E *)p.x + r * p.ld;
         Vec<E, N> v{};
-        if (target && (wide ? ((const int64_t *)target)[r] : (int64_t)((const int32_t *)target)[r]) == ignore) {
-        } else if (c + N <= D) v = *(const Vec<E, N> *)(x + r * ld + c);
+        if (p.target && (p.wide ? ((const int64_t *)p.target)[r] : (int64_t)((const int32_t *)p.target)[r]) == p.ignore) {
+        } else if (c + N <= p.D) v = *(const Vec<E, N> *)(x + c);
         else
 #pragma unroll
             for (int e = 0; e < N; ++e)
-                if (c + e < D) v.v[e] = x[r * ld + c + e];
-        uint16_t *to = out + r * Dp + c;
+                if (c + e < p.D) v.v[e] = x[c + e];
+        uint16_t *to = p.out + r * p.Dp + c;
         if constexpr (sizeof(E) == 2) {
             *(Vec<E, N> *)to = v;
         } else {
-            Vec<bf16_t, N> p[3];
+            Vec<bf16_t, N> q[3];
 #pragma unroll
             for (int e = 0; e < N; ++e) {
                 bf16_t planes[3];
                 split_planes(to_float(v.v[e]), planes);
 #pragma unroll
-                for (int q = 0; q < 3; ++q) p[q].v[e] = planes[q];
+                for (int k = 0; k < 3; ++k) q[k].v[e] = planes[k];
             }
 #pragma unroll
-            for (int q = 0; q < 3; ++q) *(Vec<bf16_t, N> *)(to + q * plane) = p[q];
+            for (int k = 0; k < 3; ++k) *(Vec<bf16_t, N> *)(to + k * p.plane) = q[k];
         }
     }
 }
 
 template <typename E>
-int launch_pack(const void *x, int64_t ld, int64_t rows, int D, int Dp, void *out, int64_t plane, const void *target, int wide,
-                int64_t ignore, hipStream_t st)
+int launch_pack(const Pack &one, const Pack &two, hipStream_t st)
 {
-    if (rows == 0 || Dp == 0) return DS_OK;
-    const int n = vector_elements(sizeof(E), {ld, 8}, {x});
-    const int64_t blocks = (rows * (Dp / n) + 255) / 256;
-    const dim3 grid((unsigned)(blocks < 8192 ? blocks : 8192));
-#define DS_LAUNCH(N)                                                                                                   \
-    hipLaunchKernelGGL((pack_kernel<E, N>), grid, dim3(256), 0, st, (const E *)x, ld, rows, D, Dp, (uint16_t *)out, plane, target,  \
-                       wide, ignore)
+    const int n = vector_elements(sizeof(E), {one.ld, two.ld, 8}, {one.x, two.x});
+    auto blocks = [&](const Pack &p) {
+        const int64_t b = (p.rows * (p.Dp / n) + 255) / 256;
+        return (int)(b < 8192 ? b : 8192);
+    };
+    const int first = blocks(one), all = first + blocks(two);
+    if (all == 0) return DS_OK;
+#define DS_LAUNCH(N) hipLaunchKernelGGL((pack_kernel<E, N>), dim3(all), dim3(256), 0, st, one, two, first)
     if (n == 8) { if constexpr (sizeof(E) == 2) DS_LAUNCH(8); }
     else if (n == 4) DS_LAUNCH(4);
     else if (n == 2) DS_LAUNCH(2);
@@ -74,72 +88,88 @@ int launch_pack(const void *x, int64_t ld, int64_t rows, int D, int Dp, void *ou
 
 constexpr float kLn2 = 0.6931471805599453f;
 
-// Joins the tiles' maxima and sums: a workgroup has 64 rows, each wave a quarter of the tiles.
-__global__ __launch_bounds__(256) void row_kernel(const float2 *__restrict__ stats, const float *__restrict__ picked, int tiles,
-                                                  int T, const void *__restrict__ target, int wide, int64_t V, int64_t ignore,
-                                                  float *__restrict__ lse, float *__restrict__ loss)
+__device__ __forceinline__ int64_t target_of(const void *target, int wide, int64_t t)
 {
-    __shared__ float tops[4][64], sums[4][64];
+    return wide ? ((const int64_t *)target)[t] : (int64_t)((const int32_t *)target)[t];
+}
+
+// The sums of every workgroup's rows, and how many of them count.
+struct Share { double loss, rows; };
+
+// total[0]: the sum or the mean of the counted rows' losses, total[1]: one row's share in it.  Without a counted row both the
+// loss and the gradients are 0.
+__device__ __forceinline__ void write_total(double loss, double rows, int mean, float *total)
+{
+    const double share = mean && rows > 0 ? 1.0 / rows : 1.0;
+    total[0] = (float)(loss * share);
+    total[1] = (float)share;
+}
+
+// Joins the tiles' maxima and sums: a workgroup has 64 rows, each of its 16 waves a sixteenth of the tiles.  The workgroup that
+// ends last adds up all of them, in order.
+__global__ __launch_bounds__(1024) void row_kernel(const float2 *__restrict__ stats, const float *__restrict__ picked, int tiles,
+                                                   int T, const void *__restrict__ target, int wide, int64_t V, int64_t ignore,
+                                                   float *__restrict__ lse, float *__restrict__ loss, int reduction, Share *shares,
+                                                   uint32_t *arrived, float *__restrict__ total)
+{
+    __shared__ float tops[16][64], sums[16][64];
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, t = blockIdx.x * 64 + lane;
     float top = -INFINITY, sum = 0.f;
     if (t < T) {
-#pragma unroll 4
-        for (int i = wave; i < tiles; i += 4) {
-            const float2 s = stats[(int64_t)i * T + t];
-            const float both = fmaxf(top, s.x);
-            sum = both == -INFINITY ? sum + s.y : sum * exp2f(top - both) + s.y * exp2f(s.x - both);
-            top = both;
+        constexpr int kAhead = 4;
+        for (int i = wave; i < tiles; i += 16 * kAhead) {
+            float2 s[kAhead];
+#pragma unroll
+            for (int j = 0; j < kAhead; ++j)
+                s[j] = i + j * 16 < tiles ? stats[(int64_t)(i + j * 16) * T + t] : float2{-INFINITY, 0.f};
+#pragma unroll
+            for (int j = 0; j < kAhead; ++j) {
+                const float both = fmaxf(top, s[j].x);
+                sum = both == -INFINITY ? sum + s[j].y : sum * exp2f(top - both) + s[j].y * exp2f(s[j].x - both);
+                top = both;
+            }
         }
     }
     tops[wave][lane] = top, sums[wave][lane] = sum;
     __syncthreads();
-    if (wave != 0 || t >= T) return;
+    if (wave != 0) return;
+    double mine = 0, counts = 0;
+    if (t < T) {
 #pragma unroll
-    for (int w = 1; w < 4; ++w) {
-        const float both = fmaxf(top, tops[w][lane]);
-        sum = both == -INFINITY ? sum + sums[w][lane] : sum * exp2f(top - both) + sums[w][lane] * exp2f(tops[w][lane] - both);
-        top = both;
+        for (int w = 1; w < 16; ++w) {
+            const float both = fmaxf(top, tops[w][lane]);
+            sum = both == -INFINITY ? sum + sums[w][lane] : sum * exp2f(top - both) + sums[w][lane] * exp2f(tops[w][lane] - both);
+            top = both;
+        }
+        const float all = sum == 0.f ? -INFINITY : top + log2f(sum);
+        lse[t] = all;
+        const int64_t y = target_of(target, wide, t);
+        const float l = y == ignore ? 0.f : y < 0 || y >= V ? NAN : (all - picked[t]) * kLn2;
+        loss[t] = l;
+        mine = l, counts = y != ignore;
     }
-    const float total = sum == 0.f ? -INFINITY : top + log2f(sum);
-    lse[t] = total;
-    const int64_t y = wide ? ((const int64_t *)target)[t] : (int64_t)((const int32_t *)target)[t];
-    loss[t] = y == ignore ? 0.f : y < 0 || y >= V ? NAN : (total - picked[t]) * kLn2;
+    if (!reduction) return;
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) mine += __shfl_xor(mine, o), counts += __shfl_xor(counts, o);
+    if (gridDim.x == 1) {
+        if (lane == 0) write_total(mine, counts, reduction == DS_MEAN, total);
+        return;
+    }
+    uint32_t before = 0;
+    if (lane == 0) {
+        shares[blockIdx.x] = Share{mine, counts};
+        before = __hip_atomic_fetch_add(arrived, 1u, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT);
+    }
+    if (__builtin_amdgcn_readfirstlane(before) != gridDim.x - 1) return;
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "agent");
+    mine = counts = 0;
+    for (unsigned i = lane; i < gridDim.x; i += 64) mine += shares[i].loss, counts += shares[i].rows;
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) mine += __shfl_xor(mine, o), counts += __shfl_xor(counts, o);
+    if (lane == 0) write_total(mine, counts, reduction == DS_MEAN, total);
 }
 
-// Sum of a workgroup's values in a fixed order, in every thread.
-template <typename S>
-__device__ __forceinline__ S sum_of_block(S v, S *lds)
-{
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o);
-    __syncthreads();
-    if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = v;
-    __syncthreads();
-    S s = 0;
-    for (int w = 0; w < (int)blockDim.x / 64; ++w) s += lds[w];
-    return s;
-}
-
-// total[0]: the sum or the mean of the counted rows' losses, total[1]: one row's share in it.  Without a counted row both the
-// loss and the gradients are 0.
-__global__ __launch_bounds__(1024) void total_kernel(const float *__restrict__ loss, const void *__restrict__ target, int wide,
-                                                     int T, int64_t ignore, int mean, float *__restrict__ total)
-{
-    __shared__ double lds[16];
-    double sum = 0, n = 0;
-    for (int t = threadIdx.x; t < T; t += 1024) {
-        const int64_t y = wide ? ((const int64_t *)target)[t] : (int64_t)((const int32_t *)target)[t];
-        sum += loss[t];
-        n += y != ignore;
-    }
-    sum = sum_of_block(sum, lds);
-    n = sum_of_block(n, lds);
-    if (threadIdx.x == 0) {
-        const double share = mean && n > 0 ? 1.0 / n : 1.0;
-        total[0] = (float)(sum * share);
-        total[1] = (float)share;
-    }
-}
+__global__ void no_rows_kernel(int mean, float *total) { write_total(0, 0, mean, total); }
 
 // Gradients of single losses: the largest of them in `factor`, each one's share of that in `scale`, so that what the products
 // take lies in [-1, 1] whatever the gradients' size.
@@ -231,18 +261,21 @@ struct Plan {
     bool pack_h, pack_w;
     int tile_logits, tile_hidden, tile_weight, split_hidden, split_weight;
     int64_t ldp;
-    size_t h, w, stats, picked, prob, bias, slices, acc, scale, factor, bytes;
+    size_t h, w, stats, picked, shares, arrived, prob, bias, slices, acc, scale, factor, bytes;
 };
 
 inline bool in_place(const void *p, int64_t ld, int64_t D) { return (uintptr_t)p % 16 == 0 && ld % 8 == 0 && D % 8 == 0; }
 
+// What a call does: the loss, the gradients, or both.
+enum { kLoss = 1, kGrad = 2 };
+
 template <typename P>
-Plan plan_of(const void *hidden, int64_t ldh, const void *weight, int64_t ldw, int64_t T, int64_t D, int64_t V, bool grad)
+Plan plan_of(const void *hidden, int64_t ldh, const void *weight, int64_t ldw, int64_t T, int64_t D, int64_t V, int what)
 {
     constexpr size_t NP = P::planes;
     Plan p{};
     p.Dp = (int)((D + 7) / 8 * 8);
-    p.pack_h = NP > 1 || grad || !in_place(hidden, ldh, D);  // grad: without the rows that do not count
+    p.pack_h = NP > 1 || what & kGrad || !in_place(hidden, ldh, D);  // for gradients: without the rows that do not count
     p.pack_w = NP > 1 || !in_place(weight, ldw, D);
     const int kb = g_tune.vocab_piece_kb;
     const size_t piece_bytes = kb == kTuneUnset ? kPieceBytes : (size_t)kb << 10;
@@ -252,7 +285,7 @@ Plan plan_of(const void *hidden, int64_t ldh, const void *weight, int64_t ldw, i
         most = n < 256 ? (most < 256 ? most : 256) : n < most ? n : most;
     };
     if (p.pack_w) at_most(NP * (size_t)p.Dp * 2);
-    if (grad) at_most(NP * (size_t)T * 2);
+    if (what & kGrad) at_most(NP * (size_t)T * 2);
     // equal pieces, of whole tiles
     p.pieces = (V + most - 1) / most;
     p.piece = ((V + p.pieces - 1) / p.pieces + 255) / 256 * 256;
@@ -267,11 +300,14 @@ Plan plan_of(const void *hidden, int64_t ldh, const void *weight, int64_t ldw, i
     };
     if (p.pack_h) p.h = take(NP * (size_t)T * p.Dp * 2);
     if (p.pack_w) p.w = take(NP * (size_t)p.piece * p.Dp * 2);
-    if (!grad) {
+    if (what & kLoss) {
         const int64_t tiles = (p.piece + Shapes<P>::m[p.tile_logits] - 1) / Shapes<P>::m[p.tile_logits];
         p.stats = take((size_t)(tiles * p.pieces) * T * 8);
         p.picked = take((size_t)T * 4);
-    } else {
+        p.shares = take((size_t)((T + 63) / 64) * sizeof(Share));
+        p.arrived = take(4);
+    }
+    if (what & kGrad) {
         p.ldp = (p.piece + 31) / 32 * 32;
         p.tile_hidden = pick_tile<P>(D, T);
         p.tile_weight = pick_tile<P>(D, p.piece);
@@ -299,6 +335,7 @@ struct Call {
     int64_t ldh, ldw, T, D, V, ignore;
     int wide, type;
     char *ws;
+    size_t ws_bytes;
     hipStream_t st;
 };
 
@@ -311,40 +348,45 @@ inline int check(const Call &c)
     return DS_OK;
 }
 
-template <typename P> struct ElementOf { typedef bf16_t type; };
-template <> struct ElementOf<F16> { typedef f16_t type; };
-template <> struct ElementOf<Split> { typedef float type; };
+#define DS_TRY(what)                    \
+    do {                                \
+        const int s_ = (what);          \
+        if (s_ != DS_OK) return s_;     \
+    } while (0)
 
+// The operands as the products take them: hidden states once, weights piece by piece.
 template <typename P>
-int hidden_operand(const Call &c, const Plan &p, bool counted_only, Operand *o)
-{
-    if (!p.pack_h) {
-        *o = Operand{c.hidden, c.ldh, 0};
-        return DS_OK;
+struct Operands {
+    Operand h, w;
+    int64_t w_at = -1;
+    bool h_there = false;
+
+    int prepare(const Call &c, const Plan &p, bool counted_only, int64_t v0, int64_t n)
+    {
+        typedef typename ElementOf<P>::type E;
+        const E *from = (const E *)c.weight + v0 * c.ldw;
+        Pack ph{}, pw{};
+        if (!h_there) {
+            h = p.pack_h ? Operand{c.ws + p.h, p.Dp, c.T * p.Dp} : Operand{c.hidden, c.ldh, 0};
+            if (p.pack_h)
+                ph = Pack{c.hidden, c.ldh, c.T, (int)c.D, p.Dp, (uint16_t *)(c.ws + p.h), h.plane,
+                          counted_only ? c.target : nullptr, c.wide, c.ignore};
+            h_there = true;
+        }
+        if (w_at != v0) {
+            w = p.pack_w ? Operand{c.ws + p.w, p.Dp, p.piece * p.Dp} : Operand{from, c.ldw, 0};
+            if (p.pack_w) pw = Pack{from, c.ldw, n, (int)c.D, p.Dp, (uint16_t *)(c.ws + p.w), w.plane, nullptr, 0, 0};
+            w_at = v0;
+        }
+        return launch_pack<E>(ph, pw, c.st);
     }
-    *o = Operand{c.ws + p.h, p.Dp, c.T * p.Dp};
-    return launch_pack<typename ElementOf<P>::type>(c.hidden, c.ldh, c.T, (int)c.D, p.Dp, c.ws + p.h, c.T * p.Dp,
-                                                    counted_only ? c.target : nullptr, c.wide, c.ignore, c.st);
-}
+};
 
 template <typename P>
-int weight_operand(const Call &c, const Plan &p, int64_t v0, int64_t n, Operand *o)
-{
-    typedef typename ElementOf<P>::type E;
-    const E *from = (const E *)c.weight + v0 * c.ldw;
-    if (!p.pack_w) {
-        *o = Operand{from, c.ldw, 0};
-        return DS_OK;
-    }
-    *o = Operand{c.ws + p.w, p.Dp, p.piece * p.Dp};
-    return launch_pack<E>(from, c.ldw, n, (int)c.D, p.Dp, c.ws + p.w, p.piece * p.Dp, nullptr, 0, 0, c.st);
-}
-
-template <typename P>
-Args logit_args(const Call &c, const Plan &p, int64_t v0, int64_t n, const Operand &h, const Operand &w)
+Args logit_args(const Call &c, const Plan &p, int64_t v0, int64_t n, const Operands<P> &o)
 {
     Args g{};
-    g.a = w, g.b = h;
+    g.a = o.w, g.b = o.h;
     g.M = (int)n, g.N = (int)c.T, g.K = p.Dp;
     g.splits = 1, g.k_split = (p.Dp + kStep - 1) / kStep * kStep;
     g.bias = c.bias, g.bias_type = c.type;
@@ -353,53 +395,45 @@ Args logit_args(const Call &c, const Plan &p, int64_t v0, int64_t n, const Opera
     return g;
 }
 
-#define DS_TRY(what)                    \
-    do {                                \
-        const int s_ = (what);          \
-        if (s_ != DS_OK) return s_;     \
-    } while (0)
-
 template <typename P>
-int loss(const Call &c, int reduction, float *rows, float *lse, float *total, size_t ws_bytes)
+int loss(const Call &c, const Plan &p, bool counted_only, Operands<P> &o, int reduction, float *rows, float *lse, float *total)
 {
-    const Plan p = plan_of<P>(c.hidden, c.ldh, c.weight, c.ldw, c.T, c.D, c.V, false);
-    if (!c.ws || ws_bytes < p.bytes || (uintptr_t)c.ws % 256) return DS_EWORKSPACE;
-    Operand h, w;
-    if (c.T > 0) {
-        DS_TRY(hidden_operand<P>(c, p, false, &h));
-        int tiles = 0;
-        for (int64_t v0 = 0; v0 < c.V; v0 += p.piece) {
-            const int64_t n = c.V - v0 < p.piece ? c.V - v0 : p.piece;
-            DS_TRY(weight_operand<P>(c, p, v0, n, &w));
-            Args g = logit_args<P>(c, p, v0, n, h, w);
-            g.stats = (float *)(c.ws + p.stats) + (int64_t)tiles * c.T * 2;
-            g.picked = (float *)(c.ws + p.picked);
-            DS_TRY(launch_product<P>(kLogitStats, p.tile_logits, g, c.st));
-            tiles += g.tiles_m;
-        }
-        hipLaunchKernelGGL(row_kernel, dim3((unsigned)((c.T + 63) / 64)), dim3(256), 0, c.st, (const float2 *)(c.ws + p.stats),
-                           (const float *)(c.ws + p.picked), tiles, (int)c.T, c.target, c.wide, c.V, c.ignore, lse, rows);
+    if (c.T == 0) {
+        if (reduction) hipLaunchKernelGGL(no_rows_kernel, dim3(1), dim3(1), 0, c.st, reduction == DS_MEAN, total);
+        return launch_status();
     }
-    if (reduction)
-        hipLaunchKernelGGL(total_kernel, dim3(1), dim3(1024), 0, c.st, rows, c.target, c.wide, (int)c.T, c.ignore,
-                           reduction == DS_MEAN, total);
+    int tiles = 0;
+    for (int64_t v0 = 0; v0 < c.V; v0 += p.piece) {
+        const int64_t n = c.V - v0 < p.piece ? c.V - v0 : p.piece;
+        DS_TRY(o.prepare(c, p, counted_only, v0, n));
+        Args g = logit_args<P>(c, p, v0, n, o);
+        g.stats = (float *)(c.ws + p.stats) + (int64_t)tiles * c.T * 2;
+        g.picked = (float *)(c.ws + p.picked);
+        g.arrived = (uint32_t *)(c.ws + p.arrived);
+        DS_TRY(launch_product<P>(kLogitStats, p.tile_logits, g, nullptr, c.st));
+        tiles += g.tiles_m;
+    }
+    hipLaunchKernelGGL(row_kernel, dim3((unsigned)((c.T + 63) / 64)), dim3(1024), 0, c.st, (const float2 *)(c.ws + p.stats),
+                       (const float *)(c.ws + p.picked), tiles, (int)c.T, c.target, c.wide, c.V, c.ignore, lse, rows, reduction,
+                       (Share *)(c.ws + p.shares), (uint32_t *)(c.ws + p.arrived), total);
     return launch_status();
 }
 
+// What the gradients are asked for with, and where they go.
+struct Grads {
+    const float *lse, *row_grad, *grad, *share;
+    void *dhidden, *dweight, *dbias;
+};
+
 template <typename P>
-int loss_grad(const Call &c, const float *lse, const float *row_grad, const float *grad, const float *share, void *dhidden,
-              void *dweight, void *dbias, size_t ws_bytes)
+int loss_grad(const Call &c, const Plan &p, Operands<P> &o, Grads r)
 {
     typedef typename ElementOf<P>::type E;
-    const Plan p = plan_of<P>(c.hidden, c.ldh, c.weight, c.ldw, c.T, c.D, c.V, true);
-    if (!c.ws || ws_bytes < p.bytes || (uintptr_t)c.ws % 256) return DS_EWORKSPACE;
-    if (c.T > 0 && row_grad) {
-        hipLaunchKernelGGL(row_scale_kernel, dim3(1), dim3(1024), 0, c.st, row_grad, c.target, c.wide, (int)c.T, c.ignore,
+    if (c.T > 0 && r.row_grad) {
+        hipLaunchKernelGGL(row_scale_kernel, dim3(1), dim3(1024), 0, c.st, r.row_grad, c.target, c.wide, (int)c.T, c.ignore,
                            (float *)(c.ws + p.scale), (float *)(c.ws + p.factor));
-        grad = (const float *)(c.ws + p.factor);
+        r.grad = (const float *)(c.ws + p.factor);
     }
-    Operand h{}, w{};
-    if (c.T > 0) DS_TRY(hidden_operand<P>(c, p, true, &h));
     float *const slices = (float *)(c.ws + p.slices);
     for (int64_t v0 = 0; v0 < c.V; v0 += p.piece) {
         const int64_t n = c.V - v0 < p.piece ? c.V - v0 : p.piece;
@@ -407,47 +441,86 @@ int loss_grad(const Call &c, const float *lse, const float *row_grad, const floa
         int bias_tiles = 0;
         const Operand prob{c.ws + p.prob, p.ldp, c.T * p.ldp};
         if (c.T > 0) {
-            DS_TRY(weight_operand<P>(c, p, v0, n, &w));
-            Args g = logit_args<P>(c, p, v0, n, h, w);
-            g.lse = lse;
-            g.row_scale = row_grad ? (const float *)(c.ws + p.scale) : nullptr;
+            DS_TRY(o.prepare(c, p, true, v0, n));
+            Args g = logit_args<P>(c, p, v0, n, o);
+            g.lse = r.lse;
+            g.row_scale = r.row_grad ? (const float *)(c.ws + p.scale) : nullptr;
             g.prob = c.ws + p.prob, g.ldp = p.ldp, g.prob_plane = prob.plane;
-            g.bias_part = dbias ? (float *)(c.ws + p.bias) : nullptr;
+            g.factor[0] = r.grad, g.factor[1] = r.share;
+            if (r.dbias && c.T <= Shapes<P>::n[p.tile_logits]) g.bias_out = (E *)r.dbias + v0;
+            else if (r.dbias) g.bias_part = (float *)(c.ws + p.bias);
             g.ld_bias_part = (int)p.ldp;
-            DS_TRY(launch_product<P>(kLogitProb, p.tile_logits, g, c.st));
+            DS_TRY(launch_product<P>(kLogitProb, p.tile_logits, g, nullptr, c.st));
             bias_tiles = g.tiles_n;
         }
-        if (dbias)
+        if (r.dbias && bias_tiles != 1)
             hipLaunchKernelGGL((bias_join_kernel<E>), dim3((unsigned)((n + 255) / 256)), dim3(256), 0, c.st,
-                               (const float *)(c.ws + p.bias), (int)p.ldp, bias_tiles, (int)n, grad, share, (E *)dbias + v0);
+                               (const float *)(c.ws + p.bias), (int)p.ldp, bias_tiles, (int)n, r.grad, r.share, (E *)r.dbias + v0);
         if (c.D == 0) continue;
+        Args g[2] = {};
+        bool wanted[2], joined[2];
         for (int which = 0; which < 2; ++which) {
-            void *out = which ? dweight : dhidden;
-            if (!out || (!which && c.T == 0)) continue;
-            Args g{};
-            g.a = which ? h : w;
-            g.b = prob;
-            g.M = (int)c.D;
-            g.N = which ? (int)((n + 7) / 8 * 8) : (int)c.T;
-            g.n_store = which ? (int)n : (int)c.T;
-            g.K = which ? (int)c.T : (int)n;
-            g.factor[0] = grad, g.factor[1] = share;
-            g.out = which ? (void *)((E *)dweight + v0 * c.D) : dhidden;
-            g.ldo = c.D, g.out_type = c.type;
-            g.splits = which ? p.split_weight : p.split_hidden;
-            g.k_split = ((g.K + g.splits - 1) / g.splits + kStep - 1) / kStep * kStep;
-            const bool joined = g.splits > 1 || (!which && p.pieces > 1);
-            g.slice = joined ? slices : nullptr;
-            DS_TRY(launch_product<P>(which ? kWeight : kHidden, which ? p.tile_weight : p.tile_hidden, g, c.st));
-            if (!joined) continue;
-            const int64_t count = (int64_t)g.n_store * c.D;
-            const int64_t blocks = (count + 255) / 256;
-            hipLaunchKernelGGL((join_kernel<P, E>), dim3((unsigned)(blocks < 16384 ? blocks : 16384)), dim3(256), 0, c.st, slices,
-                               g.splits, count, (int)c.D, which ? nullptr : (float *)(c.ws + p.acc), which || first, which || last,
-                               grad, share, (E *)g.out, c.D);
+            Args &x = g[which];
+            wanted[which] = which ? r.dweight != nullptr : r.dhidden && c.T > 0;
+            x.a = which ? o.h : o.w;
+            x.b = prob;
+            x.M = (int)c.D;
+            x.N = which ? (int)((n + 7) / 8 * 8) : (int)c.T;
+            x.n_store = which ? (int)n : (int)c.T;
+            x.K = which ? (int)c.T : (int)n;
+            x.factor[0] = r.grad, x.factor[1] = r.share;
+            x.out = which ? (void *)((E *)r.dweight + v0 * c.D) : r.dhidden;
+            x.ldo = c.D, x.out_type = c.type;
+            x.splits = which ? p.split_weight : p.split_hidden;
+            x.k_split = ((x.K + x.splits - 1) / x.splits + kStep - 1) / kStep * kStep;
+            joined[which] = x.splits > 1 || (!which && p.pieces > 1);
+            x.slice = joined[which] ? slices : nullptr;
+        }
+        // few workgroups each, and no slices to share: both in one launch
+        const int64_t blocks = (int64_t)ceil_div((int)c.D, Shapes<P>::m[p.tile_weight]) *
+                               (ceil_div((int)c.T, Shapes<P>::n[p.tile_weight]) + ceil_div((int)n, Shapes<P>::n[p.tile_weight]));
+        if (wanted[0] && wanted[1] && !joined[0] && !joined[1] && p.tile_hidden == p.tile_weight && blocks <= 2 * device_cus()) {
+            DS_TRY(launch_product<P>(kHidden, p.tile_weight, g[0], &g[1], c.st));
+            continue;
+        }
+        for (int which = 0; which < 2; ++which) {
+            Args &x = g[which];
+            if (!wanted[which]) continue;
+            DS_TRY(launch_product<P>(which ? kWeight : kHidden, which ? p.tile_weight : p.tile_hidden, x, nullptr, c.st));
+            if (!joined[which]) continue;
+            const int64_t count = (int64_t)x.n_store * c.D;
+            const int64_t join = (count + 255) / 256;
+            hipLaunchKernelGGL((join_kernel<P, E>), dim3((unsigned)(join < 16384 ? join : 16384)), dim3(256), 0, c.st, slices,
+                               x.splits, count, (int)c.D, which ? nullptr : (float *)(c.ws + p.acc), which || first, which || last,
+                               r.grad, r.share, (E *)x.out, c.D);
         }
     }
     return launch_status();
+}
+
+struct Outputs {
+    int reduction;
+    float *rows, *lse, *total;
+    Grads grads;
+};
+
+template <typename P>
+int run(const Call &c, int what, const Outputs &out)
+{
+    const Plan p = plan_of<P>(c.hidden, c.ldh, c.weight, c.ldw, c.T, c.D, c.V, what);
+    if (!c.ws || c.ws_bytes < p.bytes || (uintptr_t)c.ws % 256) return DS_EWORKSPACE;
+    Operands<P> o;
+    if (what & kLoss) DS_TRY(loss<P>(c, p, what & kGrad, o, out.reduction, out.rows, out.lse, out.total));
+    if (what & kGrad) DS_TRY(loss_grad<P>(c, p, o, out.grads));
+    return DS_OK;
+}
+
+int run(const Call &c, int what, const Outputs &out)
+{
+    DS_TRY(check(c));
+    if (c.type == DS_F32) return run<Split>(c, what, out);
+    if (c.type == DS_BF16) return run<Bf16>(c, what, out);
+    return run<F16>(c, what, out);
 }
 
 }  // namespace vocab
@@ -457,12 +530,12 @@ using namespace ds;
 using namespace ds::vocab;
 
 DS_EXPORT size_t ds_vocab_workspace_bytes(const void *hidden, int64_t ldh, const void *weight, int64_t ldw, int64_t T, int64_t D,
-                                          int64_t V, int type, int grad)
+                                          int64_t V, int type, int what)
 {
-    if (T < 0 || D < 0 || V < 1 || !element_bytes(type)) return 0;
-    if (type == DS_F32) return plan_of<Split>(hidden, ldh, weight, ldw, T, D, V, grad).bytes;
-    if (type == DS_BF16) return plan_of<Bf16>(hidden, ldh, weight, ldw, T, D, V, grad).bytes;
-    return plan_of<F16>(hidden, ldh, weight, ldw, T, D, V, grad).bytes;
+    if (T < 0 || D < 0 || V < 1 || !element_bytes(type) || what < kLoss || what > (kLoss | kGrad)) return 0;
+    if (type == DS_F32) return plan_of<Split>(hidden, ldh, weight, ldw, T, D, V, what).bytes;
+    if (type == DS_BF16) return plan_of<Bf16>(hidden, ldh, weight, ldw, T, D, V, what).bytes;
+    return plan_of<F16>(hidden, ldh, weight, ldw, T, D, V, what).bytes;
 }
 
 DS_EXPORT int ds_vocab_loss(const void *hidden, int64_t ldh, const void *weight, int64_t ldw, const void *bias,
@@ -472,12 +545,9 @@ DS_EXPORT int ds_vocab_loss(const void *hidden, int64_t ldh, const void *weight,
 {
     if ((target_bytes != 4 && target_bytes != 8) || reduction < 0 || reduction > DS_MEAN) return DS_EINVAL;
     if ((T > 0 && (!rows || !lse)) || (reduction && !total)) return DS_EINVAL;
-    const Call c{hidden, weight, bias, target, ldh, ldw, T, D, V, ignore, target_bytes == 8, type, (char *)workspace,
-                 (hipStream_t)stream};
-    DS_TRY(check(c));
-    if (type == DS_F32) return loss<Split>(c, reduction, rows, lse, total, workspace_bytes);
-    if (type == DS_BF16) return loss<Bf16>(c, reduction, rows, lse, total, workspace_bytes);
-    return loss<F16>(c, reduction, rows, lse, total, workspace_bytes);
+    return run(Call{hidden, weight, bias, target, ldh, ldw, T, D, V, ignore, target_bytes == 8, type, (char *)workspace,
+                    workspace_bytes, (hipStream_t)stream},
+               kLoss, Outputs{reduction, rows, lse, total, Grads{}});
 }
 
 DS_EXPORT int ds_vocab_loss_grad(const void *hidden, int64_t ldh, const void *weight, int64_t ldw, const void *bias,
@@ -486,10 +556,20 @@ DS_EXPORT int ds_vocab_loss_grad(const void *hidden, int64_t ldh, const void *we
                                  void *dweight, void *dbias, void *workspace, size_t workspace_bytes, ds_stream_t stream)
 {
     if ((target_bytes != 4 && target_bytes != 8) || (row_grad && (grad || share)) || (T > 0 && !lse)) return DS_EINVAL;
-    const Call c{hidden, weight, bias, target, ldh, ldw, T, D, V, ignore, target_bytes == 8, type, (char *)workspace,
-                 (hipStream_t)stream};
-    DS_TRY(check(c));
-    if (type == DS_F32) return loss_grad<Split>(c, lse, row_grad, grad, share, dhidden, dweight, dbias, workspace_bytes);
-    if (type == DS_BF16) return loss_grad<Bf16>(c, lse, row_grad, grad, share, dhidden, dweight, dbias, workspace_bytes);
-    return loss_grad<F16>(c, lse, row_grad, grad, share, dhidden, dweight, dbias, workspace_bytes);
+    return run(Call{hidden, weight, bias, target, ldh, ldw, T, D, V, ignore, target_bytes == 8, type, (char *)workspace,
+                    workspace_bytes, (hipStream_t)stream},
+               kGrad, Outputs{0, nullptr, nullptr, nullptr, Grads{lse, row_grad, grad, share, dhidden, dweight, dbias}});
+}
+
+DS_EXPORT int ds_vocab_loss_step(const void *hidden, int64_t ldh, const void *weight, int64_t ldw, const void *bias,
+                                 const void *target, int target_bytes, int64_t ignore, int64_t T, int64_t D, int64_t V, int type,
+                                 int reduction, float *rows, float *lse, float *total, void *dhidden, void *dweight, void *dbias,
+                                 void *workspace, size_t workspace_bytes, ds_stream_t stream)
+{
+    if ((target_bytes != 4 && target_bytes != 8) || reduction < 0 || reduction > DS_MEAN) return DS_EINVAL;
+    if ((T > 0 && (!rows || !lse)) || (reduction && !total)) return DS_EINVAL;
+    return run(Call{hidden, weight, bias, target, ldh, ldw, T, D, V, ignore, target_bytes == 8, type, (char *)workspace,
+                    workspace_bytes, (hipStream_t)stream},
+               kLoss | kGrad, Outputs{reduction, rows, lse, total,
+                                      Grads{lse, nullptr, nullptr, reduction ? total + 1 : nullptr, dhidden, dweight, dbias}});
 }

@@ -4,11 +4,11 @@
 namespace ds {
 namespace vocab {
 
-template <> int launch_product<F16>(int kind, int tile, Args &g, hipStream_t st)
+template <> int launch_product<F16>(int kind, int tile, Args &g, Args *other, hipStream_t st)
 {
-    if (tile == 0) return launch_tiled<F16, 256, 256, 2, 4, 4>(kind, g, st);
-    if (tile == 1) return launch_tiled<F16, 128, 128, 2, 2, 4>(kind, g, st);
-    return launch_tiled<F16, 128, 64, 4, 1, 4>(kind, g, st);
+    if (tile == 0) return launch_tiled<F16, 256, 256, 2, 4, 4>(kind, g, other, st);
+    if (tile == 1) return launch_tiled<F16, 128, 128, 2, 2, 4>(kind, g, other, st);
+    return launch_tiled<F16, 128, 64, 4, 1, 6>(kind, g, other, st);
 }
 
 }  // namespace vocab

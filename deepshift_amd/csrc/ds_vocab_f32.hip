@@ -4,11 +4,11 @@
 namespace ds {
 namespace vocab {
 
-template <> int launch_product<Split>(int kind, int tile, Args &g, hipStream_t st)
+template <> int launch_product<Split>(int kind, int tile, Args &g, Args *other, hipStream_t st)
 {
-    if (tile == 0) return launch_tiled<Split, 256, 128, 4, 2, 2>(kind, g, st);
-    if (tile == 1) return launch_tiled<Split, 128, 128, 2, 2, 3>(kind, g, st);
-    return launch_tiled<Split, 64, 64, 2, 2, 3>(kind, g, st);
+    if (tile == 0) return launch_tiled<Split, 256, 128, 4, 2, 2>(kind, g, other, st);
+    if (tile == 1) return launch_tiled<Split, 128, 128, 2, 2, 3>(kind, g, other, st);
+    return launch_tiled<Split, 64, 64, 2, 2, 6>(kind, g, other, st);
 }
 
 }  // namespace vocab

@@ -9,6 +9,7 @@ and a call repeats bit for bit.  There is no CPU path: a CPU tensor raises.
 Functions whose names end in ``_grad`` return gradients directly; ``embedding`` and ``linear_cross_entropy`` also take part
 in autograd.
 """
+import array
 import ctypes
 import math
 
@@ -185,36 +186,49 @@ class _Head:
         return self._matrices() + (_lib.ptr(self.bias), self.target.data_ptr(), self.target.element_size(), self.ignore, self.T,
                                    self.D, self.V, self.type)
 
-    def workspace(self, grad):
-        nbytes = _lib.lib().ds_vocab_workspace_bytes(*(self._matrices() + (self.T, self.D, self.V, self.type, grad)))
-        return kernels._workspace(nbytes, self.hidden.device), nbytes
+    def _workspace(self, what):
+        """Workspace, its size and the stream, as the calls end."""
+        nbytes = _lib.lib().ds_vocab_workspace_bytes(*(self._matrices() + (self.T, self.D, self.V, self.type, what)))
+        device = self.hidden.device
+        # the tensor has to live until the launches are issued
+        self.ws = kernels._workspace(nbytes, device)
+        return self.ws.data_ptr(), nbytes, _lib.stream_handle(device)
+
+    def _losses(self):
+        """Losses and logarithms of the rows, and the total and a row's share in it where there is one."""
+        rows = torch.empty((2, self.T), dtype=torch.float32, device=self.hidden.device)
+        total = torch.empty(2, dtype=torch.float32, device=self.hidden.device) if self.reduction else None
+        at = rows.data_ptr()
+        return rows, total, (self.reduction, at, at + 4 * self.T, _lib.ptr(total))
+
+    def _gradients(self, wanted=(True, True, True)):
+        like = dict(dtype=self.hidden.dtype, device=self.hidden.device)
+        return (torch.empty(self.hidden_shape, **like) if wanted[0] else None,
+                torch.empty((self.V, self.D), **like) if wanted[1] else None,
+                torch.empty(self.V, **like) if wanted[2] and self.bias is not None else None)
+
+    def _result(self, rows, total):
+        return rows[0].view(self.shape) if total is None else total[0]
 
     def loss(self):
         """``(loss, lse, share)``: the reduced loss (or one per token), and what the gradients need of it."""
-        device = self.hidden.device
-        rows = torch.empty(2, self.T, dtype=torch.float32, device=device)
-        total = torch.empty(2, dtype=torch.float32, device=device) if self.reduction else None
-        ws, nbytes = self.workspace(0)
-        row = rows.data_ptr()
-        _lib.call("ds_vocab_loss", *(self._problem() + (self.reduction, row, row + 4 * self.T, _lib.ptr(total), ws.data_ptr(),
-                                                        nbytes, _lib.stream_handle(device))))
-        if total is None:
-            return rows[0].view(self.shape), rows[1], None
-        return total[0], rows[1], total[1]
+        rows, total, args = self._losses()
+        _lib.call("ds_vocab_loss", *(self._problem() + args + self._workspace(1)))
+        return self._result(rows, total), rows[1], None if total is None else total[1]
 
     def gradients(self, lse, share, row_grad, grad, wanted):
         """Gradients of hidden, weight and bias, ``None`` for those that are not ``wanted``."""
-        device = self.hidden.device
-        dtype = self.hidden.dtype
-        dhidden = torch.empty(self.hidden_shape, dtype=dtype, device=device) if wanted[0] else None
-        dweight = torch.empty((self.V, self.D), dtype=dtype, device=device) if wanted[1] else None
-        dbias = torch.empty(self.V, dtype=dtype, device=device) if wanted[2] and self.bias is not None else None
-        ws, nbytes = self.workspace(1)
-        ptr = _lib.ptr
-        _lib.call("ds_vocab_loss_grad", *(self._problem() + (ptr(lse), ptr(row_grad), ptr(grad), ptr(share), ptr(dhidden),
-                                                             ptr(dweight), ptr(dbias), ws.data_ptr(), nbytes,
-                                                             _lib.stream_handle(device))))
-        return dhidden, dweight, dbias
+        got = self._gradients(wanted)
+        _lib.call("ds_vocab_loss_grad", *(self._problem() + tuple(map(_lib.ptr, (lse, row_grad, grad, share) + got)) +
+                                          self._workspace(2)))
+        return got
+
+    def step(self):
+        """The loss and all gradients, for a gradient of 1."""
+        rows, total, args = self._losses()
+        got = self._gradients()
+        _lib.call("ds_vocab_loss_step", *(self._problem() + args + tuple(map(_lib.ptr, got)) + self._workspace(3)))
+        return (self._result(rows, total),) + got
 
 
 class _LinearCrossEntropy(Function):
@@ -257,9 +271,7 @@ def linear_cross_entropy_grad(hidden, weight, target, bias=None, ignore_index=-1
     """``(loss, dhidden, dweight, dbias)`` of :func:`linear_cross_entropy` for a gradient of 1 (of ones, with
     ``reduction='none'``), without autograd; ``dbias`` is ``None`` where there is no bias."""
     with torch.no_grad(), _On(hidden.device):
-        head = _Head(hidden, weight, target, bias, ignore_index, reduction)
-        loss, lse, share = head.loss()
-        return (loss,) + head.gradients(lse, share, None, None, (True, True, True))
+        return _Head(hidden, weight, target, bias, ignore_index, reduction).step()
 
 
 # ---------------------------------------------------------------------------------------------
@@ -275,19 +287,60 @@ def _clip(grads, max_norm, out, scale):
     grads = [grads] if isinstance(grads, torch.Tensor) else list(grads)
     if not grads:
         raise ValueError("no gradients given")
-    device = grads[0].device
     outs = grads if out is None else ([out] if isinstance(out, torch.Tensor) else list(out))
     if len(outs) != len(grads):
         raise ValueError("%d tensors in out for %d gradients" % (len(outs), len(grads)))
-    table = (_lib.Tensor * len(grads))()
-    kept, back = [], []   # copies that have to live until the launches are issued, and those that go back
-    for i, (t, o) in enumerate(zip(grads, outs)):
-        code = _type_of("gradient %d" % i, t)
-        to = _type_of("out %d" % i, o)
-        if t.device != device or o.device != device:
-            raise ValueError("all gradients must be on %s" % device)
-        if o.shape != t.shape:
-            raise ValueError("out %d must be %s, is %s" % (i, list(t.shape), list(o.shape)))
+    device = grads[0].device
+    codes = to = _types_of("gradient", grads, device)
+    back = ()
+    if out is not None:
+        to = _types_of("out", outs, device)
+        for i, (t, o) in enumerate(zip(grads, outs)):
+            if o.shape != t.shape:
+                raise ValueError("out %d must be %s, is %s" % (i, list(t.shape), list(o.shape)))
+    if not (all([t.is_contiguous() for t in grads]) and (out is None or all([t.is_contiguous() for t in outs]))):
+        grads, outs, back = _stretches(grads, outs)
+    # one ds_tensor each: two addresses, the number of elements, two types
+    sources = [t.data_ptr() for t in grads]
+    targets = sources if outs is grads else [t.data_ptr() for t in outs]
+    sizes = [t.numel() for t in grads]
+    if scale and len(set(targets)) != len(targets):
+        if len({p for p, n in zip(targets, sizes) if n}) != sum([n > 0 for n in sizes]):
+            raise ValueError("a tensor is given twice")
+    table = array.array("q", [0]) * (4 * len(grads))
+    table[0::4], table[1::4], table[2::4] = array.array("q", sources), array.array("q", targets), array.array("q", sizes)
+    if len(set(codes)) == len(set(to)) == 1:
+        table[3::4] = array.array("q", [codes[0] | to[0] << 32]) * len(grads)
+    else:
+        table[3::4] = array.array("q", [a | b << 32 for a, b in zip(codes, to)])
+    norm = torch.empty((), dtype=torch.float32, device=device)
+    with _On(device):
+        nbytes = _lib.lib().ds_clip_workspace_bytes(len(grads))
+        ws = kernels._workspace(nbytes, device)
+        _lib.call("ds_clip", ctypes.cast(table.buffer_info()[0], _lib._tp), len(grads), max_norm, int(scale), norm.data_ptr(),
+                  ws.data_ptr(), nbytes, _lib.stream_handle(device))
+        if scale:
+            for o, copy in back:
+                o.copy_(copy)
+    return norm
+
+
+def _types_of(name, tensors, device):
+    try:
+        codes = [_TYPES[t.dtype] for t in tensors]
+    except KeyError as e:
+        raise TypeError("%ss must be float32, bfloat16 or float16, one is %s" % (name, e.args[0])) from None
+    index = device.index if device.type == "cuda" else None
+    for at in {t.get_device() for t in tensors}:
+        if index is None or at != index:
+            raise ValueError("every %s must be a GPU tensor, all on one device" % name)
+    return codes
+
+
+def _stretches(grads, outs):
+    """The same calls on tensors whose elements fill stretches of memory in one order, and the results to copy back."""
+    sources, targets, back = [], [], []
+    for t, o in zip(grads, outs):
         src, dst = t, o
         if t is o:
             if not _flat(t):
@@ -295,23 +348,11 @@ def _clip(grads, max_norm, out, scale):
         elif not (t.is_contiguous() and o.is_contiguous()) and not (t.stride() == o.stride() and _flat(t)):
             src = t.contiguous()
             dst = o if o.is_contiguous() else torch.empty_like(src, dtype=o.dtype)
-        if src is not t or dst is not o:
-            kept.append((src, dst))
-            if dst is not o:
-                back.append((o, dst))
-        table[i] = (src.data_ptr(), dst.data_ptr(), t.numel(), code, to)
-    if scale and len({e.dst for e in table if e.n}) != sum(e.n > 0 for e in table):
-        raise ValueError("a tensor is given twice")
-    norm = torch.empty((), dtype=torch.float32, device=device)
-    with _On(device):
-        nbytes = _lib.lib().ds_clip_workspace_bytes(len(grads))
-        ws = kernels._workspace(nbytes, device)
-        _lib.call("ds_clip", table, len(grads), max_norm, int(scale), norm.data_ptr(), ws.data_ptr(), nbytes,
-                  _lib.stream_handle(device))
-        if scale:
-            for o, dst in back:
-                o.copy_(dst)
-    return norm
+        if dst is not o:
+            back.append((o, dst))
+        sources.append(src)
+        targets.append(dst)
+    return sources, (sources if all([a is b for a, b in zip(sources, targets)]) else targets), back
 
 
 def gradient_norm(grads):

@@ -545,9 +545,10 @@ enum { DS_NONE = 0, DS_SUM = 1, DS_MEAN = 2 };
  * rows[t] is the loss of token t, 0 where target[t] == ignore and NaN where target[t] is neither that nor in [0, V); lse[t]
  * the logarithm, base 2, of the sum of its exponentials; total[0] (DS_SUM, DS_MEAN) the sum of the rows or their mean over the
  * counted ones (0 where none is), total[1] the share of one row in it.  The logits are not stored.
- * workspace: 256-byte aligned, ds_vocab_workspace_bytes(..., grad) bytes, for grad 0 (loss) or 1 (gradients). */
+ * workspace: 256-byte aligned, ds_vocab_workspace_bytes(..., what) bytes with what = 1 here, 2 for ds_vocab_loss_grad and 3 for
+ * ds_vocab_loss_step. */
 size_t ds_vocab_workspace_bytes(const void *hidden, int64_t ldh, const void *weight, int64_t ldw, int64_t T, int64_t D, int64_t V,
-                                int type, int grad);
+                                int type, int what);
 int ds_vocab_loss(const void *hidden, int64_t ldh, const void *weight, int64_t ldw, const void *bias, const void *target,
                   int target_bytes, int64_t ignore, int64_t T, int64_t D, int64_t V, int type, int reduction, float *rows,
                   float *lse, float *total, void *workspace, size_t workspace_bytes, ds_stream_t stream);
@@ -559,6 +560,12 @@ int ds_vocab_loss_grad(const void *hidden, int64_t ldh, const void *weight, int6
                        int target_bytes, int64_t ignore, int64_t T, int64_t D, int64_t V, int type, const float *lse,
                        const float *row_grad, const float *grad, const float *share, void *dhidden, void *dweight, void *dbias,
                        void *workspace, size_t workspace_bytes, ds_stream_t stream);
+
+/* Both in one call: the loss, and its gradients for a gradient of 1 (of every row's loss with DS_NONE). */
+int ds_vocab_loss_step(const void *hidden, int64_t ldh, const void *weight, int64_t ldw, const void *bias, const void *target,
+                       int target_bytes, int64_t ignore, int64_t T, int64_t D, int64_t V, int type, int reduction, float *rows,
+                       float *lse, float *total, void *dhidden, void *dweight, void *dbias, void *workspace,
+                       size_t workspace_bytes, ds_stream_t stream);
 
 /* One tensor of ds_clip: n elements at src, and where their clipped values go (src itself for a clip in place). */
 typedef struct {

@@ -42,11 +42,11 @@ def test_workspaces_grow_with_what_they_hold():
     assert L.ds_embed_grad_workspace_bytes(-1, 4) == 0
     assert L.ds_embed_grad_workspace_bytes(1000, 512) >= 1000 * 16
     args = (4096, 64, 4096, 64, 100, 64, 1000)
-    assert L.ds_vocab_workspace_bytes(*args, 9, 0) == 0
-    assert L.ds_vocab_workspace_bytes(*args, _lib.DS_BF16, 1) >= 100 * 1000 * 2     # the probabilities of one piece
-    assert L.ds_vocab_workspace_bytes(*args, _lib.DS_F32, 1) >= 100 * 1000 * 6
+    assert L.ds_vocab_workspace_bytes(*args, 9, 1) == 0
+    assert L.ds_vocab_workspace_bytes(*args, _lib.DS_BF16, 2) >= 100 * 1000 * 2     # the probabilities of one piece
+    assert L.ds_vocab_workspace_bytes(*args, _lib.DS_F32, 2) >= 100 * 1000 * 6
     # a piece is bounded: the logits of a large batch over a large vocabulary are never all there
-    large = L.ds_vocab_workspace_bytes(4096, 64, 4096, 64, 1 << 20, 64, 1 << 18, _lib.DS_BF16, 1)
+    large = L.ds_vocab_workspace_bytes(4096, 64, 4096, 64, 1 << 20, 64, 1 << 18, _lib.DS_BF16, 2)
     assert large < (1 << 20) * (1 << 18) * 2 // 64
 
 
