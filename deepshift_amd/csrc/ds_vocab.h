@@ -26,9 +26,11 @@ typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 
 // The 16-bit type that the matrix instructions take, and how many planes of it make a value.
-struct Bf16 { static constexpr int planes = 1; static constexpr bool half = false; };
-struct F16 { static constexpr int planes = 1; static constexpr bool half = true; };
-struct Split { static constexpr int planes = 3; static constexpr bool half = false; };  // float32
+// `step` is the reduction of a stage: rows of 128 bytes, a cache line, for operands along k.  (Half of it, with twice the
+// stages, fetched every line twice.)  float32's planes lie 64 bytes of each after the other, and make up 192.
+struct Bf16 { static constexpr int planes = 1, step = 64; static constexpr bool half = false; };
+struct F16 { static constexpr int planes = 1, step = 64; static constexpr bool half = true; };
+struct Split { static constexpr int planes = 3, step = 32; static constexpr bool half = false; };  // float32
 
 template <typename P>
 __device__ __forceinline__ f32x4 mfma(s16x8 a, s16x8 b, f32x4 c)
@@ -52,13 +54,19 @@ __device__ __forceinline__ void split_planes(float f, bf16_t *p)
     }
 }
 
-// An operand: `rows` x `k` elements, 16 bits each, planes `plane` elements apart.  Contiguous along k (element (r, k) at
-// r * ld + k) or across it (at k * ld + r).  ld and the address allow 16-byte accesses; past `rows` or `k` everything up to
-// the next multiple of 8 along the contiguous axis may be read and is zero, nothing beyond is touched.
+// An operand: `rows` x `k` elements, 16 bits each.  Contiguous along k (element (r, k) at r * ld + k) or across it (at
+// k * ld + r).  ld and the address allow 16-byte accesses; past `rows` or `k` everything up to the next multiple of 8 along the
+// contiguous axis may be read and is zero, nothing beyond is touched.  Three planes lie in turns of 32 elements along the
+// contiguous axis: element c of plane q at c / 32 * 96 + q * 32 + c % 32, and ld counts all three.
 struct Operand {
     const void *at;
-    int64_t ld, plane;
+    int64_t ld;
 };
+// Elements of a row of n, all planes.
+template <typename P> __host__ __device__ constexpr int64_t row_elements(int64_t n)
+{
+    return P::planes == 1 ? (n + 7) / 8 * 8 : (n + 31) / 32 * 96;
+}
 
 // What a launch computes with its tiles.
 enum { kStats = 0, kProb = 1, kOut = 2 };
@@ -80,8 +88,9 @@ struct Args {
     // kProb
     const float *lse;     // [T], base 2
     const float *row_scale;  // [T], or NULL: 1 for every counted row
-    void *prob;           // [planes][T][ldp]
-    int64_t ldp, prob_plane;
+    void *prob;           // [T] rows of ldp
+    int64_t ldp;
+    int prob_words;       // words of a row, a multiple of 32; zeros from M on
     float *bias_part;     // [tiles_n][ld of the piece]: sums over the rows of a tile, or NULL
     int ld_bias_part;
     void *bias_out;       // one tile holds all rows: the bias's gradient itself (times factor), or NULL
@@ -133,21 +142,23 @@ __device__ __forceinline__ i32x4 buffer_at(uint64_t address)
     return r;
 }
 
-constexpr int kStep = 32;  // reduction per stage: one matrix instruction deep
-
-// A stage of one operand in LDS, ROWS x kStep.
-//   along k:  [row][32 k], 64 bytes a row, its four 16-byte pieces exchanged by row (piece ^ (row >> 1 & 3)), so that eight
-//             lanes reading the same piece of eight rows meet all banks;
-//   across:   [k][ROWS], its 32-byte pieces exchanged by k (piece ^ (k & 3)), for the transposing reads of 4 k x 16 rows.
-template <int ROWS, bool ACROSS, int WAVES>
+// A stage of one operand in LDS, ROWS x P::step, one plane after the other.
+//   along k:  [row][k], rows of 128 (64) bytes, whose 16-byte pieces are exchanged by row (piece ^ row & 7, or ^ row >> 1 & 3),
+//             so that eight lanes reading the same piece of eight rows meet all banks;
+//   across:   [k][ROWS], its 32-byte pieces exchanged by k (piece ^ k & 3), for the transposing reads of 4 k x 16 rows.
+template <typename P, int ROWS, bool ACROSS, int WAVES>
 struct Tile {
-    static constexpr int bytes = ROWS * kStep * 2;
+    static constexpr int kStep = P::step, kPlanes = P::planes;
+    static constexpr int bytes = ROWS * kStep * 2;           // of a plane
     static constexpr int fetches = bytes / 1024;             // 1 KB each
     static constexpr int mine = (fetches + WAVES - 1) / WAVES;  // of one wave
     static_assert(fetches % WAVES == 0, "every wave fetches the same number");
+    static constexpr int kPieces = kStep / 8;                // of a row, along k
 
     uint32_t offset[mine];  // of this lane within the tile's first stage, or kNothing
     int k_at[mine];         // along: first k of this lane's piece; across: its k
+
+    __device__ static __forceinline__ int swapped(int row) { return kPieces == 8 ? row & 7 : row >> 1 & 3; }
 
     __device__ void init(const Operand &o, int rows_left, int wave)
     {
@@ -156,39 +167,50 @@ struct Tile {
         for (int i = 0; i < mine; ++i) {
             const int p = (wave * mine + i) * 64 + lane;  // 16-byte piece of the stage
             if constexpr (!ACROSS) {
-                const int row = p >> 2, piece = (p & 3) ^ (row >> 1 & 3);
+                const int row = p / kPieces, piece = (p % kPieces) ^ swapped(row);
                 k_at[i] = piece * 8;
                 offset[i] = row < rows_left ? (uint32_t)(row * o.ld * 2 + piece * 16) : kNothing;
             } else {
                 constexpr int per_k = ROWS / 8;
                 const int k = p / per_k, piece = (p % per_k) ^ ((k & 3) << 1);
                 k_at[i] = k;
-                offset[i] = piece * 8 < rows_left ? (uint32_t)(k * o.ld * 2 + piece * 16) : kNothing;
+                const int at = kPlanes == 1 ? piece * 16 : (piece >> 2) * 192 + (piece & 3) * 16;
+                offset[i] = piece * 8 < rows_left ? (uint32_t)(k * o.ld * 2 + at) : kNothing;
             }
         }
     }
     // `k_left` of the reduction remain at this stage; `base` is the address of its element (0, 0)
     __device__ __forceinline__ void stage(uint64_t base, int k_left, uint32_t lds, int wave) const
     {
-        const i32x4 buffer = buffer_at(base);
 #pragma unroll
-        for (int i = 0; i < mine; ++i)
-            fetch(k_at[i] < k_left ? offset[i] : kNothing, buffer, lds + (wave * mine + i) * 1024);
+        for (int q = 0; q < kPlanes; ++q) {
+            const i32x4 buffer = buffer_at(base + q * 64);
+#pragma unroll
+            for (int i = 0; i < mine; ++i)
+                fetch(k_at[i] < k_left ? offset[i] : kNothing, buffer, lds + q * bytes + (wave * mine + i) * 1024);
+        }
     }
-    __device__ static __forceinline__ int64_t step_bytes(const Operand &o) { return ACROSS ? o.ld * kStep * 2 : kStep * 2; }
-    __device__ static __forceinline__ int64_t row_bytes(const Operand &o) { return ACROSS ? 2 : o.ld * 2; }
+    __device__ static __forceinline__ int64_t step_bytes(const Operand &o)
+    {
+        return ACROSS ? o.ld * kStep * 2 : kStep * kPlanes * 2;
+    }
+    // of rows before a tile: a multiple of 32 of them
+    __device__ static __forceinline__ int64_t rows_bytes(const Operand &o, int rows)
+    {
+        return ACROSS ? (int64_t)rows * kPlanes * 2 : rows * o.ld * 2;
+    }
 
-    // Fragments: rows r0 .. r0+15 (a multiple of 16), lane l gets row l & 15 and k = 8 (l >> 4) .. + 7.
-    __device__ static __forceinline__ s16x8 fragment(const char *lds, int r0)
+    // Fragments: rows r0 .. r0+15 (a multiple of 16), lane l gets row l & 15 and k = 32 part + 8 (l >> 4) .. + 7.
+    __device__ static __forceinline__ s16x8 fragment(const char *lds, int r0, int part)
     {
         const int lane = threadIdx.x & 63, i = lane & 15, g = lane >> 4;
         if constexpr (!ACROSS) {
             const int row = r0 + i;
-            return *(const s16x8 *)(lds + row * 64 + ((g ^ (row >> 1 & 3)) << 4));
+            return *(const s16x8 *)(lds + row * (kStep * 2) + (((part * 4 + g) ^ swapped(row)) << 4));
         } else {
             // 16 lanes read 4 k x 16 rows, 8 bytes each, and get them transposed
             typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
-            const int k = 8 * g + (i >> 2);
+            const int k = part * 32 + 8 * g + (i >> 2);
             const int piece = (r0 >> 4) ^ (k & 3);  // the same for k and k + 4
             const char *p = lds + k * ROWS * 2 + piece * 32 + (i & 3) * 8;
             const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)p);
@@ -228,7 +250,7 @@ template <> struct ElementOf<Split> { typedef float type; };
 // LDS of a workgroup: the stages, and what the epilogue of the logits needs to know of its words and tokens, fetched before
 // the products start (one load after another behind them took half of a short reduction's time).
 template <typename P, int BM, int BN, int STAGES>
-constexpr int kStagesBytes = STAGES * P::planes * (BM + BN) * kStep * 2;
+constexpr int kStagesBytes = STAGES * P::planes * (BM + BN) * P::step * 2;
 template <int BM, int BN>
 struct Known {
     float bias[BM];
@@ -243,8 +265,9 @@ template <typename P, int BM, int BN, int WM, int WN, bool A_ACROSS, bool B_ACRO
 __device__ __forceinline__ void product_tile(const Args &g, const int block, char *lds)
 {
     constexpr int WAVES = WM * WN, MT = BM / WM / 16, NT = BN / WN / 16, NP = P::planes;
-    using TA = Tile<BM, A_ACROSS, WAVES>;
-    using TB = Tile<BN, B_ACROSS, WAVES>;
+    constexpr int kStep = P::step;
+    using TA = Tile<P, BM, A_ACROSS, WAVES>;
+    using TB = Tile<P, BN, B_ACROSS, WAVES>;
     constexpr int kStageBytes = NP * (TA::bytes + TB::bytes);
     constexpr int kInFlight = NP * (TA::mine + TB::mine);  // loads of one stage and wave
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
@@ -263,18 +286,15 @@ __device__ __forceinline__ void product_tile(const Args &g, const int block, cha
     ta.init(g.a, g.M - m0, wave);
     tb.init(g.b, g.N - n0, wave);
     const int64_t a_step = TA::step_bytes(g.a), b_step = TB::step_bytes(g.b);
-    uint64_t a_at = (uint64_t)g.a.at + m0 * TA::row_bytes(g.a) + k_from / kStep * a_step;
-    uint64_t b_at = (uint64_t)g.b.at + n0 * TB::row_bytes(g.b) + k_from / kStep * b_step;
+    uint64_t a_at = (uint64_t)g.a.at + TA::rows_bytes(g.a, m0) + k_from / kStep * a_step;
+    uint64_t b_at = (uint64_t)g.b.at + TB::rows_bytes(g.b, n0) + k_from / kStep * b_step;
     const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char *)lds;
 
     int k_left = k_to - k_from;  // of the next stage to fetch
     auto fetch_stage = [&](int slot) {
         const uint32_t to = lds0 + slot * kStageBytes;
-#pragma unroll
-        for (int p = 0; p < NP; ++p) {
-            ta.stage(a_at + p * g.a.plane * 2, k_left, to + p * TA::bytes, wave);
-            tb.stage(b_at + p * g.b.plane * 2, k_left, to + NP * TA::bytes + p * TB::bytes, wave);
-        }
+        ta.stage(a_at, k_left, to, wave);
+        tb.stage(b_at, k_left, to + NP * TA::bytes, wave);
         a_at += a_step, b_at += b_step, k_left -= kStep;
     };
 
@@ -318,27 +338,30 @@ __device__ __forceinline__ void product_tile(const Args &g, const int block, cha
         fetch_stage(slot == 0 ? STAGES - 1 : slot - 1);
         const char *at = lds + slot * kStageBytes;
         if constexpr (NP == 1) {
-            s16x8 fa[MT], fb[NT];
 #pragma unroll
-            for (int j = 0; j < NT; ++j) fb[j] = TB::fragment(at + TA::bytes, wn * NT * 16 + j * 16);
+            for (int part = 0; part < kStep / 32; ++part) {
+                s16x8 fa[MT], fb[NT];
 #pragma unroll
-            for (int i = 0; i < MT; ++i) fa[i] = TA::fragment(at, wm * MT * 16 + i * 16);
+                for (int j = 0; j < NT; ++j) fb[j] = TB::fragment(at + TA::bytes, wn * NT * 16 + j * 16, part);
 #pragma unroll
-            for (int i = 0; i < MT; ++i)
+                for (int i = 0; i < MT; ++i) fa[i] = TA::fragment(at, wm * MT * 16 + i * 16, part);
 #pragma unroll
-                for (int j = 0; j < NT; ++j) acc[i][j] = mfma<P>(fa[i], fb[j], acc[i][j]);
+                for (int i = 0; i < MT; ++i)
+#pragma unroll
+                    for (int j = 0; j < NT; ++j) acc[i][j] = mfma<P>(fa[i], fb[j], acc[i][j]);
+            }
         } else {
             s16x8 fb[NP][NT];
 #pragma unroll
             for (int p = 0; p < NP; ++p)
 #pragma unroll
                 for (int j = 0; j < NT; ++j)
-                    fb[p][j] = TB::fragment(at + NP * TA::bytes + p * TB::bytes, wn * NT * 16 + j * 16);
+                    fb[p][j] = TB::fragment(at + NP * TA::bytes + p * TB::bytes, wn * NT * 16 + j * 16, 0);
 #pragma unroll
             for (int i = 0; i < MT; ++i) {
                 s16x8 fa[NP];
 #pragma unroll
-                for (int p = 0; p < NP; ++p) fa[p] = TA::fragment(at + p * TA::bytes, wm * MT * 16 + i * 16);
+                for (int p = 0; p < NP; ++p) fa[p] = TA::fragment(at + p * TA::bytes, wm * MT * 16 + i * 16, 0);
                 // the products of 2^-16, then those of 2^-8, then the largest
                 f32x4 low[NT];
 #pragma unroll
@@ -454,14 +477,14 @@ __device__ __forceinline__ void product_tile(const Args &g, const int block, cha
                     if constexpr (P::half) p[r] *= kProbScale;
                 }
                 const int m = m_lane + i * 16;
-                if (!real || m >= g.ldp) continue;
-                Vec<bf16_t, 4> *to = (Vec<bf16_t, 4> *)((bf16_t *)g.prob + (int64_t)t * g.ldp + m);
+                if (!real || m >= g.prob_words) continue;
+                uint16_t *row = (uint16_t *)g.prob + (int64_t)t * g.ldp;
                 if constexpr (NP == 1) {
                     Vec<bf16_t, 4> o;
 #pragma unroll
                     for (int r = 0; r < 4; ++r)
                         o.v[r].bits = P::half ? from_float<f16_t>(p[r]).bits : from_float<bf16_t>(p[r]).bits;
-                    *to = o;
+                    *(Vec<bf16_t, 4> *)(row + m) = o;
                 } else {
                     bf16_t planes[4][3];
 #pragma unroll
@@ -469,7 +492,7 @@ __device__ __forceinline__ void product_tile(const Args &g, const int block, cha
 #pragma unroll
                     for (int q = 0; q < NP; ++q) {
                         const Vec<bf16_t, 4> o{{planes[0][q], planes[1][q], planes[2][q], planes[3][q]}};
-                        *(Vec<bf16_t, 4> *)((bf16_t *)to + q * g.prob_plane) = o;
+                        *(Vec<bf16_t, 4> *)(row + (m >> 5) * 96 + q * 32 + (m & 31)) = o;
                     }
                 }
             }

@@ -13,7 +13,7 @@ namespace vocab {
 
 // ---- operands as the products take them --------------------------------------------------------------------------
 
-// Rows of D elements to rows of Dp (a multiple of 8, zeros behind D): 16-bit elements as they are, float32 as three planes.
+// Rows of D elements to rows of Dp (a multiple of 8 or 32, zeros behind D): 16-bit elements as they are, float32 as three planes.
 // Rows whose target is `ignore` (where targets are given) become zeros: tokens that do
 // not count leave nothing in the weights' gradient, not even a value that is no number.
 struct Pack {
@@ -21,7 +21,7 @@ struct Pack {
     int64_t ld, rows;
     int D, Dp;
     uint16_t *out;
-    int64_t plane;
+    int64_t ldo;
     const void *target;
     int wide;
     int64_t ignore;
@@ -47,9 +47,9 @@ __global__ __launch_bounds__(256) void pack_kernel(Pack one, Pack two, int first
 #pragma unroll
             for (int e = 0; e < N; ++e)
                 if (c + e < p.D) v.v[e] = x[c + e];
-        uint16_t *to = p.out + r * p.Dp + c;
+        uint16_t *row = p.out + r * p.ldo;
         if constexpr (sizeof(E) == 2) {
-            *(Vec<E, N> *)to = v;
+            *(Vec<E, N> *)(row + c) = v;
         } else {
             Vec<bf16_t, N> q[3];
 #pragma unroll
@@ -60,7 +60,7 @@ __global__ __launch_bounds__(256) void pack_kernel(Pack one, Pack two, int first
                 for (int k = 0; k < 3; ++k) q[k].v[e] = planes[k];
             }
 #pragma unroll
-            for (int k = 0; k < 3; ++k) *(Vec<bf16_t, N> *)(to + k * p.plane) = q[k];
+            for (int k = 0; k < 3; ++k) *(Vec<bf16_t, N> *)(row + (c >> 5) * 96 + k * 32 + (c & 31)) = q[k];
         }
     }
 }
@@ -250,17 +250,19 @@ int pick_splits(int tile, int64_t m, int64_t n, int64_t k)
     const int64_t tiles = ((m + Shapes<P>::m[tile] - 1) / Shapes<P>::m[tile]) * ((n + Shapes<P>::n[tile] - 1) / Shapes<P>::n[tile]);
     if (tiles < 1) return 1;
     const int64_t want = g_tune.vocab_split != kTuneUnset ? (int64_t)g_tune.vocab_split : device_cus() / tiles;
-    const int64_t most = (k + kStep - 1) / kStep / 8;
+    const int64_t most = (k + P::step - 1) / P::step / (256 / P::step);
     const int64_t s = want < most ? want : most;
     return (int)(s < 1 ? 1 : s > 64 ? 64 : s);
 }
 
 struct Plan {
-    int Dp;               // row length of repacked operands
+    int Dp;               // features of repacked operands,
+    int64_t ldd;          // and what their rows take
     int64_t piece, pieces;
     bool pack_h, pack_w;
     int tile_logits, tile_hidden, tile_weight, split_hidden, split_weight;
-    int64_t ldp;
+    int words;            // of a piece's probabilities, a multiple of 32,
+    int64_t ldp;          // and what a row of them takes
     size_t h, w, stats, picked, shares, arrived, prob, bias, slices, acc, scale, factor, bytes;
 };
 
@@ -274,7 +276,8 @@ Plan plan_of(const void *hidden, int64_t ldh, const void *weight, int64_t ldw, i
 {
     constexpr size_t NP = P::planes;
     Plan p{};
-    p.Dp = (int)((D + 7) / 8 * 8);
+    p.Dp = (int)(NP > 1 ? (D + 31) / 32 * 32 : (D + 7) / 8 * 8);
+    p.ldd = row_elements<P>(D);
     p.pack_h = NP > 1 || what & kGrad || !in_place(hidden, ldh, D);  // for gradients: without the rows that do not count
     p.pack_w = NP > 1 || !in_place(weight, ldw, D);
     const int kb = g_tune.vocab_piece_kb;
@@ -284,7 +287,7 @@ Plan plan_of(const void *hidden, int64_t ldh, const void *weight, int64_t ldw, i
         const int64_t n = (int64_t)(piece_bytes / (per_word ? per_word : 1)) / 256 * 256;
         most = n < 256 ? (most < 256 ? most : 256) : n < most ? n : most;
     };
-    if (p.pack_w) at_most(NP * (size_t)p.Dp * 2);
+    if (p.pack_w) at_most((size_t)p.ldd * 2);
     if (what & kGrad) at_most(NP * (size_t)T * 2);
     // equal pieces, of whole tiles
     p.pieces = (V + most - 1) / most;
@@ -298,8 +301,8 @@ Plan plan_of(const void *hidden, int64_t ldh, const void *weight, int64_t ldw, i
         at = align_up(at + n, 256);
         return was;
     };
-    if (p.pack_h) p.h = take(NP * (size_t)T * p.Dp * 2);
-    if (p.pack_w) p.w = take(NP * (size_t)p.piece * p.Dp * 2);
+    if (p.pack_h) p.h = take((size_t)T * p.ldd * 2);
+    if (p.pack_w) p.w = take((size_t)p.piece * p.ldd * 2);
     if (what & kLoss) {
         const int64_t tiles = (p.piece + Shapes<P>::m[p.tile_logits] - 1) / Shapes<P>::m[p.tile_logits];
         p.stats = take((size_t)(tiles * p.pieces) * T * 8);
@@ -308,13 +311,14 @@ Plan plan_of(const void *hidden, int64_t ldh, const void *weight, int64_t ldw, i
         p.arrived = take(4);
     }
     if (what & kGrad) {
-        p.ldp = (p.piece + 31) / 32 * 32;
+        p.words = (int)((p.piece + 31) / 32 * 32);
+        p.ldp = p.words * (int64_t)NP;
         p.tile_hidden = pick_tile<P>(D, T);
         p.tile_weight = pick_tile<P>(D, p.piece);
         p.split_hidden = pick_splits<P>(p.tile_hidden, D, T, p.piece);
         p.split_weight = pick_splits<P>(p.tile_weight, D, p.piece, T);
-        p.prob = take(NP * (size_t)T * p.ldp * 2);
-        p.bias = take((size_t)((T + Shapes<P>::n[p.tile_logits] - 1) / Shapes<P>::n[p.tile_logits]) * p.ldp * 4);
+        p.prob = take((size_t)T * p.ldp * 2);
+        p.bias = take((size_t)((T + Shapes<P>::n[p.tile_logits] - 1) / Shapes<P>::n[p.tile_logits]) * p.words * 4);
         size_t slices = 0;
         if (p.split_hidden > 1 || p.pieces > 1) slices = (size_t)p.split_hidden * T * D * 4;
         if (p.split_weight > 1) {
@@ -344,7 +348,7 @@ inline int check(const Call &c)
     if (c.T < 0 || c.D < 0 || c.V < 1 || !element_bytes(c.type)) return DS_EINVAL;
     if (c.T > 0 && (!c.target || (c.D > 0 && (!c.hidden || !c.weight || c.ldh < c.D || c.ldw < c.D)))) return DS_EINVAL;
     const int64_t most = 0x7fffffff - 512;
-    if (c.T > most || c.V > most || c.D > 4000000 || c.ldh > 4000000 || c.ldw > 4000000) return DS_ETOOLARGE;
+    if (c.T > most || c.V > most || c.D > 1000000 || c.ldh > 2000000 || c.ldw > 2000000) return DS_ETOOLARGE;
     return DS_OK;
 }
 
@@ -367,15 +371,15 @@ struct Operands {
         const E *from = (const E *)c.weight + v0 * c.ldw;
         Pack ph{}, pw{};
         if (!h_there) {
-            h = p.pack_h ? Operand{c.ws + p.h, p.Dp, c.T * p.Dp} : Operand{c.hidden, c.ldh, 0};
+            h = p.pack_h ? Operand{c.ws + p.h, p.ldd} : Operand{c.hidden, c.ldh};
             if (p.pack_h)
-                ph = Pack{c.hidden, c.ldh, c.T, (int)c.D, p.Dp, (uint16_t *)(c.ws + p.h), h.plane,
+                ph = Pack{c.hidden, c.ldh, c.T, (int)c.D, p.Dp, (uint16_t *)(c.ws + p.h), p.ldd,
                           counted_only ? c.target : nullptr, c.wide, c.ignore};
             h_there = true;
         }
         if (w_at != v0) {
-            w = p.pack_w ? Operand{c.ws + p.w, p.Dp, p.piece * p.Dp} : Operand{from, c.ldw, 0};
-            if (p.pack_w) pw = Pack{from, c.ldw, n, (int)c.D, p.Dp, (uint16_t *)(c.ws + p.w), w.plane, nullptr, 0, 0};
+            w = p.pack_w ? Operand{c.ws + p.w, p.ldd} : Operand{from, c.ldw};
+            if (p.pack_w) pw = Pack{from, c.ldw, n, (int)c.D, p.Dp, (uint16_t *)(c.ws + p.w), p.ldd, nullptr, 0, 0};
             w_at = v0;
         }
         return launch_pack<E>(ph, pw, c.st);
@@ -388,7 +392,7 @@ Args logit_args(const Call &c, const Plan &p, int64_t v0, int64_t n, const Opera
     Args g{};
     g.a = o.w, g.b = o.h;
     g.M = (int)n, g.N = (int)c.T, g.K = p.Dp;
-    g.splits = 1, g.k_split = (p.Dp + kStep - 1) / kStep * kStep;
+    g.splits = 1, g.k_split = (p.Dp + P::step - 1) / P::step * P::step;
     g.bias = c.bias, g.bias_type = c.type;
     g.target = c.target, g.target_wide = c.wide;
     g.V = c.V, g.ignore = c.ignore, g.v0 = (int)v0;
@@ -439,23 +443,23 @@ int loss_grad(const Call &c, const Plan &p, Operands<P> &o, Grads r)
         const int64_t n = c.V - v0 < p.piece ? c.V - v0 : p.piece;
         const bool first = v0 == 0, last = v0 + n == c.V;
         int bias_tiles = 0;
-        const Operand prob{c.ws + p.prob, p.ldp, c.T * p.ldp};
+        const Operand prob{c.ws + p.prob, p.ldp};
         if (c.T > 0) {
             DS_TRY(o.prepare(c, p, true, v0, n));
             Args g = logit_args<P>(c, p, v0, n, o);
             g.lse = r.lse;
             g.row_scale = r.row_grad ? (const float *)(c.ws + p.scale) : nullptr;
-            g.prob = c.ws + p.prob, g.ldp = p.ldp, g.prob_plane = prob.plane;
+            g.prob = c.ws + p.prob, g.ldp = p.ldp, g.prob_words = p.words;
             g.factor[0] = r.grad, g.factor[1] = r.share;
             if (r.dbias && c.T <= Shapes<P>::n[p.tile_logits]) g.bias_out = (E *)r.dbias + v0;
             else if (r.dbias) g.bias_part = (float *)(c.ws + p.bias);
-            g.ld_bias_part = (int)p.ldp;
+            g.ld_bias_part = p.words;
             DS_TRY(launch_product<P>(kLogitProb, p.tile_logits, g, nullptr, c.st));
             bias_tiles = g.tiles_n;
         }
         if (r.dbias && bias_tiles != 1)
             hipLaunchKernelGGL((bias_join_kernel<E>), dim3((unsigned)((n + 255) / 256)), dim3(256), 0, c.st,
-                               (const float *)(c.ws + p.bias), (int)p.ldp, bias_tiles, (int)n, r.grad, r.share, (E *)r.dbias + v0);
+                               (const float *)(c.ws + p.bias), p.words, bias_tiles, (int)n, r.grad, r.share, (E *)r.dbias + v0);
         if (c.D == 0) continue;
         Args g[2] = {};
         bool wanted[2], joined[2];
@@ -472,7 +476,7 @@ int loss_grad(const Call &c, const Plan &p, Operands<P> &o, Grads r)
             x.out = which ? (void *)((E *)r.dweight + v0 * c.D) : r.dhidden;
             x.ldo = c.D, x.out_type = c.type;
             x.splits = which ? p.split_weight : p.split_hidden;
-            x.k_split = ((x.K + x.splits - 1) / x.splits + kStep - 1) / kStep * kStep;
+            x.k_split = ((x.K + x.splits - 1) / x.splits + P::step - 1) / P::step * P::step;
             joined[which] = x.splits > 1 || (!which && p.pieces > 1);
             x.slice = joined[which] ? slices : nullptr;
         }
