@@ -14,11 +14,13 @@
 // values, which planes without them would lose below 2^-110.
 #pragma once
 #include "ds_train.h"
+#include <type_traits>
 
 namespace ds {
 namespace vocab {
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef int i32x4 __attribute__((ext_vector_type(4)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef short s16x8 __attribute__((ext_vector_type(8)));
@@ -28,18 +30,36 @@ typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 // The 16-bit type that the matrix instructions take, and how many planes of it make a value.
 // `step` is the reduction of a stage: rows of 128 bytes, a cache line, for operands along k.  (Half of it, with twice the
 // stages, fetched every line twice.)  float32's planes lie 64 bytes of each after the other, and make up 192.
-struct Bf16 { static constexpr int planes = 1, step = 64; static constexpr bool half = false; };
-struct F16 { static constexpr int planes = 1, step = 64; static constexpr bool half = true; };
-struct Split { static constexpr int planes = 3, step = 32; static constexpr bool half = false; };  // float32
+struct Bf16 { static constexpr int planes = 1, step = 64, unit = 32; static constexpr bool half = false; };
+struct F16 { static constexpr int planes = 1, step = 64, unit = 32; static constexpr bool half = true; };
+struct Split { static constexpr int planes = 3, step = 32, unit = 16; static constexpr bool half = false; };  // float32
 
+// A matrix instruction: unit x unit results, 16 x 16 from 32 of the reduction or 32 x 32 from 16.  Lane l has one n,
+// l % unit, and `groups` times four neighbouring m.
 template <typename P>
-__device__ __forceinline__ f32x4 mfma(s16x8 a, s16x8 b, f32x4 c)
-{
-    if constexpr (P::half)
-        return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
-    else
-        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
-}
+struct Unit {
+    static constexpr int size = P::unit, groups = size == 32 ? 4 : 1, depth = size == 32 ? 16 : 32;
+    typedef typename std::conditional<size == 32, f32x16, f32x4>::type Result;
+
+    // first m of a lane, and of its groups behind that
+    __device__ static __forceinline__ int lane_m(int lane) { return lane / size * 4; }
+    static constexpr int group_m(int q) { return q * 8; }
+
+    __device__ static __forceinline__ Result multiply(s16x8 a, s16x8 b, Result c)
+    {
+        if constexpr (size == 32) {
+            if constexpr (P::half)
+                return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+            else
+                return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+        } else {
+            if constexpr (P::half)
+                return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+            else
+                return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+        }
+    }
+};
 
 // Planes of a float32 value, each what is left of it times 2^8, rounded to nearest, so that what a product leaves out has no
 // sign of its own; where that would round to infinity it is cut instead.
@@ -109,6 +129,9 @@ constexpr float kLog2e = 1.4426950408889634f;
 // exponents of float32 and needs none.
 constexpr float kProbScale = 32768.f;
 
+// For terms of a sum whose largest is 1: one instruction, good to a unit in the last place; what is below 2^-126 becomes 0.
+__device__ __forceinline__ float exp2_of(float x) { return __builtin_amdgcn_exp2f(x); }
+
 // A launch's tile: the workgroups of one XCD (they are dealt out in turn) get neighbouring tiles, in strips of kStrip along m,
 // so that what they read at the same time fits its L2.
 __device__ __forceinline__ void tile_of(int id, int tiles_m, int tiles_n, int *tm, int *tn)
@@ -143,22 +166,28 @@ __device__ __forceinline__ i32x4 buffer_at(uint64_t address)
 }
 
 // A stage of one operand in LDS, ROWS x P::step, one plane after the other.
-//   along k:  [row][k], rows of 128 (64) bytes, whose 16-byte pieces are exchanged by row (piece ^ row & 7, or ^ row >> 1 & 3),
-//             so that eight lanes reading the same piece of eight rows meet all banks;
-//   across:   [k][ROWS], its 32-byte pieces exchanged by k (piece ^ k & 3), for the transposing reads of 4 k x 16 rows.
+//   along k:  [row][k], rows of 128 (64) bytes, whose 16-byte pieces are exchanged by row, so that 16 lanes that read together
+//             (0-3, 12-15, 20-23 and 24-27, and so on) meet all banks;
+//   across:   [k][ROWS], its 32-byte pieces exchanged by k, so that the transposing reads that 32 lanes make together, of
+//             k .. k + 3 and k + 8 .. k + 11 or of two neighbouring pieces of k .. k + 3, meet all banks.
 template <typename P, int ROWS, bool ACROSS, int WAVES>
 struct Tile {
     static constexpr int kStep = P::step, kPlanes = P::planes;
     static constexpr int bytes = ROWS * kStep * 2;           // of a plane
     static constexpr int fetches = bytes / 1024;             // 1 KB each
     static constexpr int mine = (fetches + WAVES - 1) / WAVES;  // of one wave
-    static_assert(fetches % WAVES == 0, "every wave fetches the same number");
+    static_assert(ROWS >= 64 && fetches % WAVES == 0, "every wave fetches the same number");
     static constexpr int kPieces = kStep / 8;                // of a row, along k
 
     uint32_t offset[mine];  // of this lane within the tile's first stage, or kNothing
     int k_at[mine];         // along: first k of this lane's piece; across: its k
 
-    __device__ static __forceinline__ int swapped(int row) { return kPieces == 8 ? row & 7 : row >> 1 & 3; }
+    __device__ static __forceinline__ int swapped(int row) { return kPieces == 8 ? (row & 7) ^ (row >> 4 & 1) : row >> 1 & 3; }
+    __device__ static __forceinline__ int swapped_across(int k)
+    {
+        if (Unit<P>::size == 32) return ROWS >= 128 ? (k & 3) << 1 : k & 2;
+        return ROWS >= 128 ? (k & 3) | (k >> 1 & 4) : (k >> 1 & 1) | (k >> 2 & 2);
+    }
 
     __device__ void init(const Operand &o, int rows_left, int wave)
     {
@@ -172,23 +201,25 @@ struct Tile {
                 offset[i] = row < rows_left ? (uint32_t)(row * o.ld * 2 + piece * 16) : kNothing;
             } else {
                 constexpr int per_k = ROWS / 8;
-                const int k = p / per_k, piece = (p % per_k) ^ ((k & 3) << 1);
+                const int k = p / per_k, piece = (p % per_k) ^ (swapped_across(k) << 1);
                 k_at[i] = k;
                 const int at = kPlanes == 1 ? piece * 16 : (piece >> 2) * 192 + (piece & 3) * 16;
                 offset[i] = piece * 8 < rows_left ? (uint32_t)(k * o.ld * 2 + at) : kNothing;
             }
         }
     }
-    // `k_left` of the reduction remain at this stage; `base` is the address of its element (0, 0)
+    // The wave's fetch `i` of a stage, of plane q; `k_left` of the reduction remain at this stage, whose element (0, 0) is at
+    // `base`.
+    __device__ __forceinline__ void one(uint64_t base, int k_left, uint32_t lds, int wave, int q, int i) const
+    {
+        fetch(k_at[i] < k_left ? offset[i] : kNothing, buffer_at(base + q * 64), lds + q * bytes + (wave * mine + i) * 1024);
+    }
     __device__ __forceinline__ void stage(uint64_t base, int k_left, uint32_t lds, int wave) const
     {
 #pragma unroll
-        for (int q = 0; q < kPlanes; ++q) {
-            const i32x4 buffer = buffer_at(base + q * 64);
+        for (int q = 0; q < kPlanes; ++q)
 #pragma unroll
-            for (int i = 0; i < mine; ++i)
-                fetch(k_at[i] < k_left ? offset[i] : kNothing, buffer, lds + q * bytes + (wave * mine + i) * 1024);
-        }
+            for (int i = 0; i < mine; ++i) one(base, k_left, lds, wave, q, i);
     }
     __device__ static __forceinline__ int64_t step_bytes(const Operand &o)
     {
@@ -200,18 +231,20 @@ struct Tile {
         return ACROSS ? (int64_t)rows * kPlanes * 2 : rows * o.ld * 2;
     }
 
-    // Fragments: rows r0 .. r0+15 (a multiple of 16), lane l gets row l & 15 and k = 32 part + 8 (l >> 4) .. + 7.
+    // Fragments of instruction `part` of the stage: unit rows from r0 (a multiple of unit), lane l gets row l % unit and eight k,
+    // those from 8 (l / unit) on.
     __device__ static __forceinline__ s16x8 fragment(const char *lds, int r0, int part)
     {
-        const int lane = threadIdx.x & 63, i = lane & 15, g = lane >> 4;
+        constexpr int U = Unit<P>::size, kDepth = Unit<P>::depth;
+        const int lane = threadIdx.x & 63, g = lane / U;
         if constexpr (!ACROSS) {
-            const int row = r0 + i;
-            return *(const s16x8 *)(lds + row * (kStep * 2) + (((part * 4 + g) ^ swapped(row)) << 4));
+            const int row = r0 + lane % U;
+            return *(const s16x8 *)(lds + row * (kStep * 2) + (((part * (kDepth / 8) + g) ^ swapped(row)) << 4));
         } else {
             // 16 lanes read 4 k x 16 rows, 8 bytes each, and get them transposed
             typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
-            const int k = part * 32 + 8 * g + (i >> 2);
-            const int piece = (r0 >> 4) ^ (k & 3);  // the same for k and k + 4
+            const int i = lane & 15, k = part * kDepth + 8 * g + (i >> 2);
+            const int piece = (r0 + lane % U) >> 4 ^ swapped_across(k);  // bit 2 of k, clear here, makes no difference
             const char *p = lds + k * ROWS * 2 + piece * 32 + (i & 3) * 8;
             const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)p);
             const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)(p + 4 * ROWS * 2));
@@ -247,6 +280,15 @@ template <typename P> struct ElementOf { typedef bf16_t type; };
 template <> struct ElementOf<F16> { typedef f16_t type; };
 template <> struct ElementOf<Split> { typedef float type; };
 
+// Until all but `in_flight` of this wave's fetches have arrived and all its reads of LDS, and then until every wave's have.
+template <int in_flight>
+__device__ __forceinline__ void wait_for_stage()
+{
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" :: "i"(in_flight) : "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+}
+
 // LDS of a workgroup: the stages, and what the epilogue of the logits needs to know of its words and tokens, fetched before
 // the products start (one load after another behind them took half of a short reduction's time).
 template <typename P, int BM, int BN, int STAGES>
@@ -264,7 +306,8 @@ constexpr int kLdsBytes = kStagesBytes<P, BM, BN, STAGES> + (LOGITS ? (int)sizeo
 template <typename P, int BM, int BN, int WM, int WN, bool A_ACROSS, bool B_ACROSS, int KIND, int STAGES>
 __device__ __forceinline__ void product_tile(const Args &g, const int block, char *lds)
 {
-    constexpr int WAVES = WM * WN, MT = BM / WM / 16, NT = BN / WN / 16, NP = P::planes;
+    using U = Unit<P>;
+    constexpr int WAVES = WM * WN, MT = BM / WM / U::size, NT = BN / WN / U::size, NP = P::planes;
     constexpr int kStep = P::step;
     using TA = Tile<P, BM, A_ACROSS, WAVES>;
     using TB = Tile<P, BN, B_ACROSS, WAVES>;
@@ -298,11 +341,13 @@ __device__ __forceinline__ void product_tile(const Args &g, const int block, cha
         a_at += a_step, b_at += b_step, k_left -= kStep;
     };
 
-    f32x4 acc[MT][NT];
+    typename U::Result acc[MT][NT];
 #pragma unroll
     for (int i = 0; i < MT; ++i)
 #pragma unroll
-        for (int j = 0; j < NT; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+        for (int j = 0; j < NT; ++j)
+#pragma unroll
+            for (int r = 0; r < 4 * U::groups; ++r) acc[i][j][r] = 0.f;
 
     Known<BM, BN> &known = *(Known<BM, BN> *)(lds + kStagesBytes<P, BM, BN, STAGES>);
     static_assert(BM <= WAVES * 64 && BN <= WAVES * 64, "a thread per word and token");
@@ -321,119 +366,180 @@ __device__ __forceinline__ void product_tile(const Args &g, const int block, cha
         }
     }
 
+    auto keep_known = [&] {
+        if constexpr (KIND != kOut) {
+            if (threadIdx.x < BM) known.bias[threadIdx.x] = bias;
+            if (threadIdx.x < BN)
+                known.want[threadIdx.x] = want, known.lse[threadIdx.x] = lse, known.scale[threadIdx.x] = scale;
+        }
+    };
+
     // Stages past the end are fetched too, as zeros (k_left <= 0 fetches nothing): the number of loads in flight is the same
     // in every step, and nothing past the operands is read.
-#pragma unroll
-    for (int s = 0; s < STAGES - 1; ++s) fetch_stage(s);
-    if constexpr (KIND != kOut) {
-        if (threadIdx.x < BM) known.bias[threadIdx.x] = bias;
-        if (threadIdx.x < BN) known.want[threadIdx.x] = want, known.lse[threadIdx.x] = lse, known.scale[threadIdx.x] = scale;
-    }
     int slot = 0;
-    for (int s = 0; s < steps; ++s) {
-        // this wave's part of the stage has arrived, and it has read the slot that is filled next; then everyone's
-        asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" :: "i"((STAGES - 2) * kInFlight) : "memory");
-        __builtin_amdgcn_s_barrier();
-        asm volatile("" ::: "memory");
-        fetch_stage(slot == 0 ? STAGES - 1 : slot - 1);
-        const char *at = lds + slot * kStageBytes;
-        if constexpr (NP == 1) {
+    if constexpr (NP == 1) {
+        // While the products of one half of a stage run, the fragments of the next half are read: the second half's between
+        // the first's products, the next stage's first half between the second's.  In the middle, where every wave has read
+        // the whole stage, its slot is fetched anew, one fetch after each row of products.
+        constexpr int kParts = kStep / U::depth / 2, kRows = kParts * MT, kFragments = kParts * (MT + NT);
+        constexpr int kPerRow = (kFragments * 4 + kRows * 3 - 1) / (kRows * 3);  // read in the first three quarters of the rows
+        constexpr int kFetches = TA::mine + TB::mine, kFetchesPerRow = (kFetches + kRows - 1) / kRows;
+        s16x8 a0[kParts][MT], b0[kParts][NT], a1[kParts][MT], b1[kParts][NT];
+        auto read = [&](int from, int half, int n, s16x8 (&fa)[kParts][MT], s16x8 (&fb)[kParts][NT]) {
+            const char *at = lds + from * kStageBytes;
+            const int p = n / (MT + NT), k = n % (MT + NT);
+            if (n >= kFragments) return;
+            if (k < NT) fb[p][k] = TB::fragment(at + TA::bytes, (wn * NT + k) * U::size, half * kParts + p);
+            else fa[p][k - NT] = TA::fragment(at, (wm * MT + k - NT) * U::size, half * kParts + p);
+        };
+        auto multiply = [&](int row, const s16x8 (&fa)[kParts][MT], const s16x8 (&fb)[kParts][NT]) {
+            const int p = row / MT, i = row % MT;
 #pragma unroll
-            for (int part = 0; part < kStep / 32; ++part) {
-                s16x8 fa[MT], fb[NT];
+            for (int j = 0; j < NT; ++j) acc[i][j] = U::multiply(fa[p][i], fb[p][j], acc[i][j]);
+        };
 #pragma unroll
-                for (int j = 0; j < NT; ++j) fb[j] = TB::fragment(at + TA::bytes, wn * NT * 16 + j * 16, part);
+        for (int s = 0; s < STAGES; ++s) fetch_stage(s);
+        keep_known();
+        wait_for_stage<(STAGES - 1) * kInFlight>();
 #pragma unroll
-                for (int i = 0; i < MT; ++i) fa[i] = TA::fragment(at, wm * MT * 16 + i * 16, part);
+        for (int n = 0; n < kFragments; ++n) read(0, 0, n, a0, b0);
+        for (int s = 0; s < steps; ++s) {
 #pragma unroll
-                for (int i = 0; i < MT; ++i)
+            for (int row = 0; row < kRows; ++row) {
+                multiply(row, a0, b0);
 #pragma unroll
-                    for (int j = 0; j < NT; ++j) acc[i][j] = mfma<P>(fa[i], fb[j], acc[i][j]);
+                for (int n = 0; n < kPerRow; ++n) read(slot, 1, row * kPerRow + n, a1, b1);
+                __builtin_amdgcn_sched_barrier(0);
             }
-        } else {
+            wait_for_stage<(STAGES - 2) * kInFlight>();
+            const uint32_t to = lds0 + slot * kStageBytes;
+            slot = slot + 1 == STAGES ? 0 : slot + 1;
+#pragma unroll
+            for (int row = 0; row < kRows; ++row) {
+                multiply(row, a1, b1);
+#pragma unroll
+                for (int f = row * kFetchesPerRow; f < (row + 1) * kFetchesPerRow && f < kFetches; ++f) {
+                    if (f < TA::mine) ta.one(a_at, k_left, to, wave, 0, f);
+                    else tb.one(b_at, k_left, to + TA::bytes, wave, 0, f - TA::mine);
+                }
+#pragma unroll
+                for (int n = 0; n < kPerRow; ++n) read(slot, 0, row * kPerRow + n, a0, b0);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            a_at += a_step, b_at += b_step, k_left -= kStep;
+        }
+    } else {
+#pragma unroll
+        for (int s = 0; s < STAGES - 1; ++s) fetch_stage(s);
+        keep_known();
+        // rows of tiles that are multiplied together: the six products of a tile follow each other, so four tiles at least
+        // have to take turns
+        constexpr int G = NT >= 4 || MT == 1 ? 1 : 2;
+        static_assert(MT % G == 0, "");
+        for (int s = 0; s < steps; ++s) {
+            wait_for_stage<(STAGES - 2) * kInFlight>();
+            fetch_stage(slot == 0 ? STAGES - 1 : slot - 1);
+            const char *at = lds + slot * kStageBytes;
             s16x8 fb[NP][NT];
 #pragma unroll
             for (int p = 0; p < NP; ++p)
 #pragma unroll
                 for (int j = 0; j < NT; ++j)
-                    fb[p][j] = TB::fragment(at + NP * TA::bytes + p * TB::bytes, wn * NT * 16 + j * 16, 0);
+                    fb[p][j] = TB::fragment(at + NP * TA::bytes + p * TB::bytes, (wn * NT + j) * U::size, 0);
 #pragma unroll
-            for (int i = 0; i < MT; ++i) {
-                s16x8 fa[NP];
+            for (int i0 = 0; i0 < MT; i0 += G) {
+                s16x8 fa[G][NP];
+                f32x4 low[G][NT];
 #pragma unroll
-                for (int p = 0; p < NP; ++p) fa[p] = TA::fragment(at + p * TA::bytes, wm * MT * 16 + i * 16, 0);
+                for (int i = 0; i < G; ++i)
+#pragma unroll
+                    for (int p = 0; p < NP; ++p)
+                        fa[i][p] = TA::fragment(at + p * TA::bytes, (wm * MT + i0 + i) * U::size, 0);
                 // the products of 2^-16, then those of 2^-8, then the largest
-                f32x4 low[NT];
+                auto add = [&](int p, int q) {
 #pragma unroll
-                for (int j = 0; j < NT; ++j) low[j] = mfma<P>(fa[1], fb[1][j], f32x4{0.f, 0.f, 0.f, 0.f});
+                    for (int i = 0; i < G; ++i)
 #pragma unroll
-                for (int j = 0; j < NT; ++j) low[j] = mfma<P>(fa[0], fb[2][j], low[j]);
+                        for (int j = 0; j < NT; ++j) low[i][j] = U::multiply(fa[i][p], fb[q][j], low[i][j]);
+                };
 #pragma unroll
-                for (int j = 0; j < NT; ++j) low[j] = mfma<P>(fa[2], fb[0][j], low[j]) * (1.f / 256);
+                for (int i = 0; i < G; ++i)
 #pragma unroll
-                for (int j = 0; j < NT; ++j) low[j] = mfma<P>(fa[0], fb[1][j], low[j]);
+                    for (int j = 0; j < NT; ++j) low[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+                add(1, 1), add(0, 2), add(2, 0);
 #pragma unroll
-                for (int j = 0; j < NT; ++j) low[j] = mfma<P>(fa[1], fb[0][j], low[j]);
+                for (int i = 0; i < G; ++i)
 #pragma unroll
-                for (int j = 0; j < NT; ++j) acc[i][j] = mfma<P>(fa[0], fb[0][j], acc[i][j]);
+                    for (int j = 0; j < NT; ++j) low[i][j] *= 1.f / 256;
+                add(0, 1), add(1, 0);
 #pragma unroll
-                for (int j = 0; j < NT; ++j)
+                for (int i = 0; i < G; ++i)
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) acc[i][j][r] = fmaf(low[j][r], 1.f / 256, acc[i][j][r]);
+                    for (int j = 0; j < NT; ++j) {
+                        f32x4 &c = acc[i0 + i][j];
+                        c = U::multiply(fa[i][0], fb[0][j], c);
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) c[r] = fmaf(low[i][j][r], 1.f / 256, c[r]);
+                    }
             }
+            slot = slot + 1 == STAGES ? 0 : slot + 1;
         }
-        slot = slot + 1 == STAGES ? 0 : slot + 1;
     }
     // nothing of this wave is on its way to LDS any more, and nobody reads it
     asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
     __syncthreads();
 
-    const int m_in = wm * MT * 16 + (lane >> 4) * 4, n_in = wn * NT * 16 + (lane & 15);  // of this lane, in the tile
+    // This lane's results: I counts its groups of four neighbouring m, j its n.
+    constexpr int MG = MT * U::groups;
+    const int m_in = wm * MT * U::size + U::lane_m(lane), n_in = wn * NT * U::size + lane % U::size;  // in the tile
     const int m_lane = m0 + m_in, n_lane = n0 + n_in;
+    auto m_of = [](int I) constexpr { return I / U::groups * U::size + U::group_m(I % U::groups); };
+    auto value = [&](int I, int j, int r) -> float { return acc[I / U::groups][j][I % U::groups * 4 + r]; };
     float *fl = (float *)lds;
     if constexpr (KIND != kOut) {
         // acc becomes the logits in base 2
 #pragma unroll
-        for (int i = 0; i < MT; ++i)
+        for (int I = 0; I < MG; ++I)
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-                const bool real = m_lane + i * 16 + r < g.M;
-                const float b = known.bias[m_in + i * 16 + r];
+                const bool real = m_lane + m_of(I) + r < g.M;
+                const float b = known.bias[m_in + m_of(I) + r];
 #pragma unroll
-                for (int j = 0; j < NT; ++j) acc[i][j][r] = real ? (acc[i][j][r] + b) * kLog2e : -INFINITY;
+                for (int j = 0; j < NT; ++j) acc[I / U::groups][j][I % U::groups * 4 + r] = real ? (value(I, j, r) + b) * kLog2e : -INFINITY;
             }
     }
     if constexpr (KIND == kStats) {
         if (block == 0 && threadIdx.x == 0) *g.arrived = 0;
 #pragma unroll
         for (int j = 0; j < NT; ++j) {
-            const int t = n_lane + j * 16;
-            const int at = known.want[n_in + j * 16] - m_in;  // below 0 or past this lane's words: not here
+            const int t = n_lane + j * U::size;
+            const int at = known.want[n_in + j * U::size] - m_in;  // below 0 or past this lane's words: not here
             float top = -INFINITY;
 #pragma unroll
-            for (int i = 0; i < MT; ++i)
+            for (int I = 0; I < MG; ++I)
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
                     // a maximum that a value which is no number does not slip through
-                    top = acc[i][j][r] > top || acc[i][j][r] != acc[i][j][r] ? acc[i][j][r] : top;
-                    if (at == i * 16 + r) g.picked[t] = acc[i][j][r];
+                    const float v = value(I, j, r);
+                    top = v > top || v != v ? v : top;
+                    if (at == m_of(I) + r) g.picked[t] = v;
                 }
             float sum = 0.f;
             // a column of nothing but -inf keeps a sum of 0
             const float base = top == -INFINITY ? 0.f : top;
 #pragma unroll
-            for (int i = 0; i < MT; ++i)
+            for (int I = 0; I < MG; ++I)
 #pragma unroll
-                for (int r = 0; r < 4; ++r) sum += exp2f(acc[i][j][r] - base);
+                for (int r = 0; r < 4; ++r) sum += exp2_of(value(I, j, r) - base);
 #pragma unroll
-            for (int o = 16; o <= 32; o <<= 1) {
+            for (int o = U::size; o < 64; o <<= 1) {
                 const float top2 = __shfl_xor(top, o), sum2 = __shfl_xor(sum, o);
                 const float both = fmaxf(top, top2);
-                sum = both == -INFINITY ? sum + sum2 : sum * exp2f(top - both) + sum2 * exp2f(top2 - both);
+                sum = both == -INFINITY ? sum + sum2 : sum * exp2_of(top - both) + sum2 * exp2_of(top2 - both);
                 top = both;
             }
-            if (lane < 16) {
-                const int c = wn * NT * 16 + j * 16 + lane;
+            if (lane < U::size) {
+                const int c = (wn * NT + j) * U::size + lane;
                 fl[(wm * BN + c) * 2] = top;
                 fl[(wm * BN + c) * 2 + 1] = sum;
             }
@@ -446,7 +552,7 @@ __device__ __forceinline__ void product_tile(const Args &g, const int block, cha
             for (int w = 1; w < WM; ++w) {
                 const float top2 = fl[(w * BN + c) * 2], sum2 = fl[(w * BN + c) * 2 + 1];
                 const float both = fmaxf(top, top2);
-                sum = both == -INFINITY ? sum + sum2 : sum * exp2f(top - both) + sum2 * exp2f(top2 - both);
+                sum = both == -INFINITY ? sum + sum2 : sum * exp2_of(top - both) + sum2 * exp2_of(top2 - both);
                 top = both;
             }
             float2 *to = (float2 *)g.stats + (int64_t)tm * g.N + n0 + c;
@@ -454,29 +560,29 @@ __device__ __forceinline__ void product_tile(const Args &g, const int block, cha
         }
     }
     if constexpr (KIND == kProb) {
-        float over_n[MT][4];  // sums over this lane's rows, for the bias
+        float over_n[MG][4];  // sums over this lane's rows, for the bias
 #pragma unroll
-        for (int i = 0; i < MT; ++i)
+        for (int I = 0; I < MG; ++I)
 #pragma unroll
-            for (int r = 0; r < 4; ++r) over_n[i][r] = 0.f;
+            for (int r = 0; r < 4; ++r) over_n[I][r] = 0.f;
 #pragma unroll
         for (int j = 0; j < NT; ++j) {
-            const int t = n_lane + j * 16;
+            const int t = n_lane + j * U::size;
             const bool real = t < g.N;
-            const float lse = known.lse[n_in + j * 16], scale = known.scale[n_in + j * 16];
-            const int at = known.want[n_in + j * 16] - m_in;
+            const float lse = known.lse[n_in + j * U::size], scale = known.scale[n_in + j * U::size];
+            const int at = known.want[n_in + j * U::size] - m_in;
 #pragma unroll
-            for (int i = 0; i < MT; ++i) {
+            for (int I = 0; I < MG; ++I) {
                 float p[4];
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
-                    const float e = exp2f(acc[i][j][r] - lse) - (at == i * 16 + r ? 1.f : 0.f);
+                    const float e = exp2f(value(I, j, r) - lse) - (at == m_of(I) + r ? 1.f : 0.f);
                     // rows that do not count leave nothing, whatever their logits are; neither do words past the end
-                    p[r] = scale == 0.f || m_lane + i * 16 + r >= g.M ? 0.f : e * scale;
-                    over_n[i][r] += p[r];
+                    p[r] = scale == 0.f || m_lane + m_of(I) + r >= g.M ? 0.f : e * scale;
+                    over_n[I][r] += p[r];
                     if constexpr (P::half) p[r] *= kProbScale;
                 }
-                const int m = m_lane + i * 16;
+                const int m = m_lane + m_of(I);
                 if (!real || m >= g.prob_words) continue;
                 uint16_t *row = (uint16_t *)g.prob + (int64_t)t * g.ldp;
                 if constexpr (NP == 1) {
@@ -501,12 +607,12 @@ __device__ __forceinline__ void product_tile(const Args &g, const int block, cha
             typedef typename ElementOf<P>::type E;
             const float factor = g.bias_out ? factor_of(g.factor) : 1.f;
 #pragma unroll
-            for (int i = 0; i < MT; ++i)
+            for (int I = 0; I < MG; ++I)
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
 #pragma unroll
-                    for (int o = 1; o < 16; o <<= 1) over_n[i][r] += __shfl_xor(over_n[i][r], o);
-                    if ((lane & 15) == 0) fl[wn * BM + wm * MT * 16 + i * 16 + (lane >> 4) * 4 + r] = over_n[i][r];
+                    for (int o = 1; o < U::size; o <<= 1) over_n[I][r] += __shfl_xor(over_n[I][r], o);
+                    if (lane % U::size == 0) fl[wn * BM + m_in + m_of(I) + r] = over_n[I][r];
                 }
             __syncthreads();
             for (int c = threadIdx.x; c < BM; c += WAVES * 64) {
@@ -523,25 +629,25 @@ __device__ __forceinline__ void product_tile(const Args &g, const int block, cha
         const float factor = g.slice ? 1.f : out_factor<P>(g.factor);
 #pragma unroll
         for (int j = 0; j < NT; ++j) {
-            const int n = n_lane + j * 16;
+            const int n = n_lane + j * U::size;
             if (n >= g.n_store) continue;
 #pragma unroll
-            for (int i = 0; i < MT; ++i) {
-                const int m = m_lane + i * 16;
+            for (int I = 0; I < MG; ++I) {
+                const int m = m_lane + m_of(I);
                 if (m >= g.M) continue;
                 const int many = min(4, g.M - m);
                 if (g.slice) {
                     float *to = g.slice + ((int64_t)split * g.n_store + n) * g.M + m;
-                    if (many == 4 && g.M % 4 == 0) *(f32x4 *)to = acc[i][j];
+                    if (many == 4 && g.M % 4 == 0) *(f32x4 *)to = f32x4{value(I, j, 0), value(I, j, 1), value(I, j, 2), value(I, j, 3)};
                     else
 #pragma unroll
                         for (int r = 0; r < 4; ++r)
-                            if (r < many) to[r] = acc[i][j][r];
+                            if (r < many) to[r] = value(I, j, r);
                     continue;
                 }
                 float v[4];
 #pragma unroll
-                for (int r = 0; r < 4; ++r) v[r] = acc[i][j][r] * factor;
+                for (int r = 0; r < 4; ++r) v[r] = value(I, j, r) * factor;
                 const bool whole = many == 4 && g.ldo % 4 == 0 && (uintptr_t)g.out % 16 == 0;
                 if (g.out_type == DS_F32) {
                     float *to = (float *)g.out + (int64_t)n * g.ldo + m;

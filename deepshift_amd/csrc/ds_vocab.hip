@@ -125,7 +125,7 @@ __global__ __launch_bounds__(1024) void row_kernel(const float2 *__restrict__ st
 #pragma unroll
             for (int j = 0; j < kAhead; ++j) {
                 const float both = fmaxf(top, s[j].x);
-                sum = both == -INFINITY ? sum + s[j].y : sum * exp2f(top - both) + s[j].y * exp2f(s[j].x - both);
+                sum = both == -INFINITY ? sum + s[j].y : sum * exp2_of(top - both) + s[j].y * exp2_of(s[j].x - both);
                 top = both;
             }
         }
@@ -138,7 +138,7 @@ __global__ __launch_bounds__(1024) void row_kernel(const float2 *__restrict__ st
 #pragma unroll
         for (int w = 1; w < 16; ++w) {
             const float both = fmaxf(top, tops[w][lane]);
-            sum = both == -INFINITY ? sum + sums[w][lane] : sum * exp2f(top - both) + sums[w][lane] * exp2f(tops[w][lane] - both);
+            sum = both == -INFINITY ? sum + sums[w][lane] : sum * exp2_of(top - both) + sums[w][lane] * exp2_of(tops[w][lane] - both);
             top = both;
         }
         const float all = sum == 0.f ? -INFINITY : top + log2f(sum);
