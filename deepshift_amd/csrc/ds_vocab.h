@@ -176,7 +176,7 @@ struct Tile {
     static constexpr int bytes = ROWS * kStep * 2;           // of a plane
     static constexpr int fetches = bytes / 1024;             // 1 KB each
     static constexpr int mine = (fetches + WAVES - 1) / WAVES;  // of one wave
-    static_assert(ROWS >= 64 && fetches % WAVES == 0, "every wave fetches the same number");
+    static_assert((ROWS >= 64 || !ACROSS) && fetches % WAVES == 0, "every wave fetches the same number");
     static constexpr int kPieces = kStep / 8;                // of a row, along k
 
     uint32_t offset[mine];  // of this lane within the tile's first stage, or kNothing
@@ -694,17 +694,25 @@ __global__ __launch_bounds__(WM * WN * 64) void both_kernel(Args hidden, Args we
 // Which product a launch is.
 enum { kLogitStats = 0, kLogitProb = 1, kHidden = 2, kWeight = 3 };
 
-// Tile shapes, m x n, by their number in a launch.
-template <typename P> struct Shapes;
-template <> struct Shapes<Bf16> { static constexpr int m[3] = {256, 128, 128}, n[3] = {256, 128, 64}; };
-template <> struct Shapes<F16> : Shapes<Bf16> {};
-template <> struct Shapes<Split> { static constexpr int m[3] = {256, 128, 64}, n[3] = {128, 128, 64}; };
+// Tile shapes, m x n, by their number in a launch.  For choosing among them: workgroups that a CU holds, and the measured
+// microseconds of a step of the reduction while every CU has its fill, and while none has more than one.
+constexpr int kShapes = 4;
+template <typename P> struct Shapes {
+    static constexpr int m[kShapes] = {256, 128, 128, 64}, n[kShapes] = {256, 128, 64, 64}, resident[kShapes] = {1, 2, 2, 3};
+    static constexpr float step_us[kShapes] = {1.8f, 1.2f, 0.85f, 0.7f}, alone_us[kShapes] = {1.2f, 0.78f, 0.5f, 0.35f};
+};
+template <> struct Shapes<Split> {
+    // the last for logits only
+    static constexpr int m[kShapes] = {256, 128, 64, 32}, n[kShapes] = {128, 128, 64, 32}, resident[kShapes] = {1, 1, 1, 2};
+    static constexpr float step_us[kShapes] = {2.7f, 1.7f, 0.6f, 0.5f}, alone_us[kShapes] = {2.5f, 1.5f, 0.55f, 0.27f};
+};
+template <typename P> constexpr int kGradShapes = P::planes == 1 ? 4 : 3;
 
 // Launches one product with tiles of shape `tile`; fills in the tile counts.  With `other` the two gradients' products run in
 // one launch, both with that shape (g is kHidden, *other kWeight).  A translation unit per P.
 template <typename P> int launch_product(int kind, int tile, Args &g, Args *other, hipStream_t st);
 
-template <typename P, int BM, int BN, int WM, int WN, int STAGES>
+template <typename P, int BM, int BN, int WM, int WN, int STAGES, bool GRADS = true>
 int launch_tiled(int kind, Args &g, Args *other, hipStream_t st)
 {
     auto count = [](Args &x) {
@@ -714,16 +722,20 @@ int launch_tiled(int kind, Args &g, Args *other, hipStream_t st)
     const int64_t blocks = count(g), more = other ? count(*other) : 0;
     if (blocks + more > 0x7fffffff) return DS_ETOOLARGE;
     const dim3 grid((unsigned)(blocks + more)), threads(WM * WN * 64);
-    if (other)
-        hipLaunchKernelGGL((both_kernel<P, BM, BN, WM, WN, STAGES>), grid, threads, 0, st, g, *other, (int)blocks);
-    else if (kind == kLogitStats)
+    if (kind == kLogitStats) {
         hipLaunchKernelGGL((product_kernel<P, BM, BN, WM, WN, false, false, kStats, STAGES>), grid, threads, 0, st, g);
-    else if (kind == kLogitProb)
+    } else if (kind == kLogitProb) {
         hipLaunchKernelGGL((product_kernel<P, BM, BN, WM, WN, false, false, kProb, STAGES>), grid, threads, 0, st, g);
-    else if (kind == kHidden)
-        hipLaunchKernelGGL((product_kernel<P, BM, BN, WM, WN, true, false, kOut, STAGES>), grid, threads, 0, st, g);
-    else
-        hipLaunchKernelGGL((product_kernel<P, BM, BN, WM, WN, true, true, kOut, STAGES>), grid, threads, 0, st, g);
+    } else if constexpr (GRADS) {
+        if (other)
+            hipLaunchKernelGGL((both_kernel<P, BM, BN, WM, WN, STAGES>), grid, threads, 0, st, g, *other, (int)blocks);
+        else if (kind == kHidden)
+            hipLaunchKernelGGL((product_kernel<P, BM, BN, WM, WN, true, false, kOut, STAGES>), grid, threads, 0, st, g);
+        else
+            hipLaunchKernelGGL((product_kernel<P, BM, BN, WM, WN, true, true, kOut, STAGES>), grid, threads, 0, st, g);
+    } else {
+        return DS_EINVAL;
+    }
     return launch_status();
 }
 

@@ -116,7 +116,7 @@ __global__ __launch_bounds__(1024) void row_kernel(const float2 *__restrict__ st
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, t = blockIdx.x * 64 + lane;
     float top = -INFINITY, sum = 0.f;
     if (t < T) {
-        constexpr int kAhead = 4;
+        constexpr int kAhead = 8;
         for (int i = wave; i < tiles; i += 16 * kAhead) {
             float2 s[kAhead];
 #pragma unroll
@@ -232,27 +232,40 @@ __global__ __launch_bounds__(256) void bias_join_kernel(const float *__restrict_
 
 constexpr size_t kPieceBytes = (size_t)1 << 30;  // of P, and of repacked weights
 
+// The tile shape of a product, and how many stretches its reduction of k is cut into (1 of `most_splits`): the pair with the
+// shortest estimate.  A round of workgroups takes its steps and some four more to begin and end; slices are written and read
+// once more by a launch of their own.  What decides it, measured: 1543 x 1000 results from 20011 words, float16, 157 us on
+// 128 x 128 tiles in two stretches, 89 us on 256 x 256 in nine; 2048 x 1024 from 32768 words, float32, 1113 and 768 us;
+// 64 x 512 from 1000 words, float32, 25 us in one stretch, 13 in four.
+struct Choice { int tile, splits; };
 template <typename P>
-int pick_tile(int64_t m, int64_t n)
+Choice choose(int64_t m, int64_t n, int64_t k, int shapes, int most_splits)
 {
-    const int64_t cus = device_cus();
-    const int forced = g_tune.vocab_tile;
-    if (forced >= 0 && forced < 3) return forced;
-    for (int i = 0; i < 2; ++i)
-        if (n > Shapes<P>::n[i] / 2 && m > Shapes<P>::m[i] / 2 &&
-            ((m + Shapes<P>::m[i] - 1) / Shapes<P>::m[i]) * ((n + Shapes<P>::n[i] - 1) / Shapes<P>::n[i]) >= cus) return i;
-    return n > 64 ? 1 : 2;
-}
-
-template <typename P>
-int pick_splits(int tile, int64_t m, int64_t n, int64_t k)
-{
-    const int64_t tiles = ((m + Shapes<P>::m[tile] - 1) / Shapes<P>::m[tile]) * ((n + Shapes<P>::n[tile] - 1) / Shapes<P>::n[tile]);
-    if (tiles < 1) return 1;
-    const int64_t want = g_tune.vocab_split != kTuneUnset ? (int64_t)g_tune.vocab_split : device_cus() / tiles;
-    const int64_t most = (k + P::step - 1) / P::step / (256 / P::step);
-    const int64_t s = want < most ? want : most;
-    return (int)(s < 1 ? 1 : s > 64 ? 64 : s);
+    typedef Shapes<P> S;
+    const int cus = device_cus(), tile_knob = g_tune.vocab_tile, split_knob = g_tune.vocab_split;
+    const int64_t steps = (k + P::step - 1) / P::step;
+    Choice best{0, 1};
+    if (m < 1 || n < 1) return best;
+    double shortest = 1e300;
+    for (int i = 0; i < shapes; ++i) {
+        if (tile_knob >= 0 && tile_knob < shapes && i != tile_knob) continue;
+        const int64_t tiles = ((m + S::m[i] - 1) / S::m[i]) * ((n + S::n[i] - 1) / S::n[i]);
+        const int64_t fill = (int64_t)cus * S::resident[i];
+        // stretches of 256 at least, and no more workgroups than two rounds of them
+        int most = most_splits;
+        if (most > steps * P::step / 256) most = (int)(steps * P::step / 256);
+        if (split_knob >= 1) most = most < split_knob ? most : split_knob;
+        else if (most > 2 * fill / tiles) most = (int)(2 * fill / tiles);
+        if (most < 1) most = 1;
+        for (int s = split_knob >= 1 ? most : 1; s <= most; s += 1 + s / 4) {
+            const int64_t blocks = tiles * s;
+            const double step = blocks <= cus ? S::alone_us[i] : S::step_us[i];
+            const double us = (double)((blocks + fill - 1) / fill) * ((double)((steps + s - 1) / s) + 4) * step +
+                              (s > 1 ? 4 + (double)s * m * n * 4 / 3e6 : 0);
+            if (us < shortest) shortest = us, best = Choice{i, s};
+        }
+    }
+    return best;
 }
 
 struct Plan {
@@ -260,7 +273,8 @@ struct Plan {
     int64_t ldd;          // and what their rows take
     int64_t piece, pieces;
     bool pack_h, pack_w;
-    int tile_logits, tile_hidden, tile_weight, split_hidden, split_weight;
+    int tile_logits;
+    Choice hidden, weight;
     int words;            // of a piece's probabilities, a multiple of 32,
     int64_t ldp;          // and what a row of them takes
     size_t h, w, stats, picked, shares, arrived, prob, bias, slices, acc, scale, factor, bytes;
@@ -294,7 +308,7 @@ Plan plan_of(const void *hidden, int64_t ldh, const void *weight, int64_t ldw, i
     p.piece = ((V + p.pieces - 1) / p.pieces + 255) / 256 * 256;
     if (p.piece > V) p.piece = V;
     p.pieces = (V + p.piece - 1) / p.piece;
-    p.tile_logits = pick_tile<P>(p.piece, T);
+    p.tile_logits = choose<P>(p.piece, T, D, kShapes, 1).tile;
     size_t at = 0;
     auto take = [&](size_t n) {
         const size_t was = at;
@@ -313,16 +327,14 @@ Plan plan_of(const void *hidden, int64_t ldh, const void *weight, int64_t ldw, i
     if (what & kGrad) {
         p.words = (int)((p.piece + 31) / 32 * 32);
         p.ldp = p.words * (int64_t)NP;
-        p.tile_hidden = pick_tile<P>(D, T);
-        p.tile_weight = pick_tile<P>(D, p.piece);
-        p.split_hidden = pick_splits<P>(p.tile_hidden, D, T, p.piece);
-        p.split_weight = pick_splits<P>(p.tile_weight, D, p.piece, T);
+        p.hidden = choose<P>(D, T, p.piece, kGradShapes<P>, 64);
+        p.weight = choose<P>(D, p.piece, T, kGradShapes<P>, 64);
         p.prob = take((size_t)T * p.ldp * 2);
         p.bias = take((size_t)((T + Shapes<P>::n[p.tile_logits] - 1) / Shapes<P>::n[p.tile_logits]) * p.words * 4);
         size_t slices = 0;
-        if (p.split_hidden > 1 || p.pieces > 1) slices = (size_t)p.split_hidden * T * D * 4;
-        if (p.split_weight > 1) {
-            const size_t n = (size_t)p.split_weight * p.piece * D * 4;
+        if (p.hidden.splits > 1 || p.pieces > 1) slices = (size_t)p.hidden.splits * T * D * 4;
+        if (p.weight.splits > 1) {
+            const size_t n = (size_t)p.weight.splits * p.piece * D * 4;
             slices = n > slices ? n : slices;
         }
         p.slices = take(slices);
@@ -475,22 +487,22 @@ int loss_grad(const Call &c, const Plan &p, Operands<P> &o, Grads r)
             x.factor[0] = r.grad, x.factor[1] = r.share;
             x.out = which ? (void *)((E *)r.dweight + v0 * c.D) : r.dhidden;
             x.ldo = c.D, x.out_type = c.type;
-            x.splits = which ? p.split_weight : p.split_hidden;
+            x.splits = which ? p.weight.splits : p.hidden.splits;
             x.k_split = ((x.K + x.splits - 1) / x.splits + P::step - 1) / P::step * P::step;
             joined[which] = x.splits > 1 || (!which && p.pieces > 1);
             x.slice = joined[which] ? slices : nullptr;
         }
         // few workgroups each, and no slices to share: both in one launch
-        const int64_t blocks = (int64_t)ceil_div((int)c.D, Shapes<P>::m[p.tile_weight]) *
-                               (ceil_div((int)c.T, Shapes<P>::n[p.tile_weight]) + ceil_div((int)n, Shapes<P>::n[p.tile_weight]));
-        if (wanted[0] && wanted[1] && !joined[0] && !joined[1] && p.tile_hidden == p.tile_weight && blocks <= 2 * device_cus()) {
-            DS_TRY(launch_product<P>(kHidden, p.tile_weight, g[0], &g[1], c.st));
+        const int64_t blocks = (int64_t)ceil_div((int)c.D, Shapes<P>::m[p.weight.tile]) *
+                               (ceil_div((int)c.T, Shapes<P>::n[p.weight.tile]) + ceil_div((int)n, Shapes<P>::n[p.weight.tile]));
+        if (wanted[0] && wanted[1] && !joined[0] && !joined[1] && p.hidden.tile == p.weight.tile && blocks <= 2 * device_cus()) {
+            DS_TRY(launch_product<P>(kHidden, p.weight.tile, g[0], &g[1], c.st));
             continue;
         }
         for (int which = 0; which < 2; ++which) {
             Args &x = g[which];
             if (!wanted[which]) continue;
-            DS_TRY(launch_product<P>(which ? kWeight : kHidden, which ? p.tile_weight : p.tile_hidden, x, nullptr, c.st));
+            DS_TRY(launch_product<P>(which ? kWeight : kHidden, which ? p.weight.tile : p.hidden.tile, x, nullptr, c.st));
             if (!joined[which]) continue;
             const int64_t count = (int64_t)x.n_store * c.D;
             const int64_t join = (count + 255) / 256;

@@ -18,7 +18,7 @@ extern "C" {
  * tiles in image order); "chain_spin_us" (bound of a barrier wait of ds_linear_chain_f32 in
  * microseconds) and "chain_extra" (arrivals its barriers wait for beyond the grid, which never come: with
  * a small bound every workgroup gives up and exits, which is how the tests reach that path without
- * hanging anything); "vocab_tile" (0, 1, 2: tile shape of the products of ds_vocab_*), "vocab_piece_kb"
+ * hanging anything); "vocab_tile" (0 to 3: tile shape of the products of ds_vocab_*), "vocab_piece_kb"
  * (workspace of a piece of the vocabulary there, in KiB), "vocab_split" (stretches that its gradients'
  * reductions are cut into, at most) and "embed_radix" (1: ds_embed_grad sorts any number of tokens as it
  * sorts many).  knob == NULL clears every override.  Each knob is an atomic integer that an

@@ -208,7 +208,7 @@ HEAD_SHAPES = [(1, 1, 1), (1, 8, 2), (3, 5, 7), (64, 512, 10), (2, 64, 1000), (6
 
 
 @pytest.mark.parametrize("dtype", TYPES, ids=str)
-@pytest.mark.parametrize("tile", [0, 1, 2])
+@pytest.mark.parametrize("tile", [0, 1, 2, 3])
 def test_cross_entropy_and_gradients(dtype, tile):
     for i, (T, D, V) in enumerate(HEAD_SHAPES):
         print(T, D, V, flush=True)
@@ -236,7 +236,7 @@ def test_cross_entropy_in_pieces_and_stretches(dtype):
         h, w, b, y = _head(T, D, V, dtype, True, g)
         ones = torch.ones(T, device=DEV)
         for tune in (dict(vocab_piece_kb=1), dict(vocab_piece_kb=1, vocab_split=3), dict(vocab_split=5), dict(vocab_split=1)):
-            for tile in (0, 1, 2):
+            for tile in (0, 1, 2, 3):
                 print(T, D, V, tune, tile, flush=True)
                 with Tune(vocab_tile=tile, **tune):
                     rows = training.linear_cross_entropy(h, w, y, b, reduction="none")
