@@ -366,33 +366,32 @@ __global__ __launch_bounds__(256) void embed_finish_kernel(const uint32_t *__res
         }
     }
     if (first == end) return;
-    const int64_t per_row = D / N;
-    for (int r = 0; r < mine; ++r) {
+    const uint32_t per_row = (uint32_t)(D / N);
+    for (uint32_t i = threadIdx.x; i < mine * per_row; i += 256) {
+        const uint32_t r = div_by(i * N, by_row), u = i - r * per_row;
         const uint32_t from = begin[r], to = begin[r + 1];
         if (to == from) continue;
         const uint32_t c0 = from / chunk, c1 = (to - 1) / chunk;
         if (c0 == c1) continue;
-        for (int64_t u = threadIdx.x; u < per_row; u += 256) {
-            float acc[N];
-            const float *p = part + u * N;
+        float acc[N];
+        const float *p = part + (int64_t)u * N;
 #pragma unroll
-            for (int e = 0; e < N; ++e) acc[e] = p[((int64_t)c0 * 2 + 1) * D + e];
-            constexpr int kAhead = N <= 2 ? 24 : 8;  // partial sums on their way
-            for (uint32_t c = c0 + 1; c <= c1; c += kAhead) {
-                Vec<float, N> got[kAhead];
+        for (int e = 0; e < N; ++e) acc[e] = p[((int64_t)c0 * 2 + 1) * D + e];
+        constexpr int kAhead = N <= 2 ? 24 : 8;  // partial sums on their way
+        for (uint32_t c = c0 + 1; c <= c1; c += kAhead) {
+            Vec<float, N> got[kAhead];
 #pragma unroll
-                for (int j = 0; j < kAhead; ++j)
-                    if (c + j <= c1) got[j] = *(const Vec<float, N> *)(p + (int64_t)(c + j) * 2 * D);
+            for (int j = 0; j < kAhead; ++j)
+                if (c + j <= c1) got[j] = *(const Vec<float, N> *)(p + (int64_t)(c + j) * 2 * D);
 #pragma unroll
-                for (int j = 0; j < kAhead; ++j)
+            for (int j = 0; j < kAhead; ++j)
 #pragma unroll
-                    for (int e = 0; e < N; ++e) acc[e] += c + j <= c1 ? got[j].v[e] : 0.f;
-            }
-            Vec<E, N> o;
-#pragma unroll
-            for (int e = 0; e < N; ++e) o.v[e] = from_float<E>(acc[e] * scale);
-            ((Vec<E, N> *)(block + r * D))[u] = o;
+                for (int e = 0; e < N; ++e) acc[e] += c + j <= c1 ? got[j].v[e] : 0.f;
         }
+        Vec<E, N> o;
+#pragma unroll
+        for (int e = 0; e < N; ++e) o.v[e] = from_float<E>(acc[e] * scale);
+        ((Vec<E, N> *)(block + (int64_t)r * D))[u] = o;
     }
 }
 
@@ -425,11 +424,11 @@ int launch_embed_grad(const uint32_t *keys, const uint32_t *pos, const void *g, 
     const int n = vector_elements(sizeof(E), {D, ldg}, {g, dw});
     const int chunk = embed_chunk(T);
     const int64_t chunks = (T + chunk - 1) / chunk, slices = (D / n + 63) / 64;
-    // 16 to 64 KB of the result a workgroup, in whole 16-byte units: the search for its tokens is paid for by larger ones,
+    // 2 to 64 KB of the result a workgroup, in whole 16-byte units: the search for its tokens is paid for by larger ones,
     // enough workgroups for every CU by smaller ones
     constexpr int64_t kUnit = 16 / sizeof(E);
     const int64_t row_bytes = D * (int64_t)sizeof(E);
-    const int64_t region = min((int64_t)65536, max((int64_t)16384, V * row_bytes / (8 * device_cus())));
+    const int64_t region = min((int64_t)65536, max((int64_t)2048, V * row_bytes / (8 * device_cus())));
     const int rows = (int)min((int64_t)256, max(kUnit, region / row_bytes / kUnit * kUnit));
     if (rows * D > 0x7fffffff) return DS_ETOOLARGE;
     const int64_t finish = (V + rows - 1) / rows;

@@ -117,9 +117,8 @@ struct Args {
     uint32_t *arrived;    // kStats: set to 0, for row_kernel
     // kOut
     float *slice;         // [splits][N][M] float, or NULL: final
-    void *out;            // [N] rows of type out_type, ldo apart
+    void *out;            // [N] rows of the operands' type, ldo apart
     int64_t ldo;
-    int out_type;
     const float *factor[2];  // what results are multiplied with, 1 value each, or NULL
     int n_store;          // rows of C that exist (N may be rounded up for the loads)
 };
@@ -301,6 +300,45 @@ struct Known {
 };
 template <typename P, int BM, int BN, int STAGES, bool LOGITS>
 constexpr int kLdsBytes = kStagesBytes<P, BM, BN, STAGES> + (LOGITS ? (int)sizeof(Known<BM, BN>) : 0);
+
+// Results on their way out: rows of COLS elements gathered in LDS, whose 16-byte pieces are exchanged by row, so that lanes
+// that each hold a few neighbours of another row do not meet in a bank; from there every row leaves as one stretch.  (Stored
+// from the registers, eight bytes here and there, a tile of 256 x 256 took some 25 us.)
+template <typename S, int COLS>
+struct Gather {
+    static constexpr int kPer = 16 / sizeof(S), kPieces = COLS / kPer;
+    static constexpr int kMask = (kPieces & -kPieces) < 32 ? (kPieces & -kPieces) - 1 : 31;
+
+    __device__ static __forceinline__ char *at(char *lds, int row, int col)
+    {
+        const int piece = col / kPer ^ (row & kMask);
+        return lds + (row * kPieces + piece) * 16 + col % kPer * (int)sizeof(S);
+    }
+    // `row_at(r)` is where row r goes, or NULL; `cols` of it exist
+    template <int THREADS, typename ROW>
+    __device__ static __forceinline__ void leave(char *lds, int rows, int cols, ROW row_at)
+    {
+        for (int i = threadIdx.x; i < rows * kPieces; i += THREADS) {
+            const int row = i / kPieces, col = i % kPieces * kPer;
+            S *to = row_at(row);
+            if (!to || col >= cols) continue;
+            to += col;
+            const Vec<S, kPer> v = *(const Vec<S, kPer> *)at(lds, row, col);
+            if (col + kPer <= cols && (uintptr_t)to % 16 == 0) {
+                *(Vec<S, kPer> *)to = v;
+            } else if (col + kPer <= cols && (uintptr_t)to % 4 == 0) {
+                typedef Vec<S, 4 / sizeof(S)> Word;
+                const Word *w = (const Word *)&v;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) ((Word *)to)[e] = w[e];
+            } else {
+#pragma unroll
+                for (int e = 0; e < kPer; ++e)
+                    if (col + e < cols) to[e] = v.v[e];
+            }
+        }
+    }
+};
 
 // One tile of a product, by a whole workgroup; `block` counts the product's workgroups.
 template <typename P, int BM, int BN, int WM, int WN, bool A_ACROSS, bool B_ACROSS, int KIND, int STAGES>
@@ -559,7 +597,12 @@ __device__ __forceinline__ void product_tile(const Args &g, const int block, cha
             *to = float2{top, sum};
         }
     }
+    constexpr int kRowsOut = WN * U::size, kThreads = WAVES * 64;  // rows that leave together: one j of every wave
+    auto n_of = [](int row, int j) { return (row / U::size * NT + j) * U::size + row % U::size; };
+    const int row_out = wn * U::size + lane % U::size;
     if constexpr (KIND == kProb) {
+        typedef Gather<uint16_t, BM * NP> Out;
+        static_assert(kRowsOut * BM * NP * 2 <= kStagesBytes<P, BM, BN, STAGES>, "");
         float over_n[MG][4];  // sums over this lane's rows, for the bias
 #pragma unroll
         for (int I = 0; I < MG; ++I)
@@ -567,8 +610,6 @@ __device__ __forceinline__ void product_tile(const Args &g, const int block, cha
             for (int r = 0; r < 4; ++r) over_n[I][r] = 0.f;
 #pragma unroll
         for (int j = 0; j < NT; ++j) {
-            const int t = n_lane + j * U::size;
-            const bool real = t < g.N;
             const float lse = known.lse[n_in + j * U::size], scale = known.scale[n_in + j * U::size];
             const int at = known.want[n_in + j * U::size] - m_in;
 #pragma unroll
@@ -582,15 +623,13 @@ __device__ __forceinline__ void product_tile(const Args &g, const int block, cha
                     over_n[I][r] += p[r];
                     if constexpr (P::half) p[r] *= kProbScale;
                 }
-                const int m = m_lane + m_of(I);
-                if (!real || m >= g.prob_words) continue;
-                uint16_t *row = (uint16_t *)g.prob + (int64_t)t * g.ldp;
+                const int m = m_in + m_of(I);
                 if constexpr (NP == 1) {
                     Vec<bf16_t, 4> o;
 #pragma unroll
                     for (int r = 0; r < 4; ++r)
                         o.v[r].bits = P::half ? from_float<f16_t>(p[r]).bits : from_float<bf16_t>(p[r]).bits;
-                    *(Vec<bf16_t, 4> *)(row + m) = o;
+                    *(Vec<bf16_t, 4> *)Out::at(lds, row_out, m) = o;
                 } else {
                     bf16_t planes[4][3];
 #pragma unroll
@@ -598,10 +637,16 @@ __device__ __forceinline__ void product_tile(const Args &g, const int block, cha
 #pragma unroll
                     for (int q = 0; q < NP; ++q) {
                         const Vec<bf16_t, 4> o{{planes[0][q], planes[1][q], planes[2][q], planes[3][q]}};
-                        *(Vec<bf16_t, 4> *)(row + (m >> 5) * 96 + q * 32 + (m & 31)) = o;
+                        *(Vec<bf16_t, 4> *)Out::at(lds, row_out, (m >> 5) * 96 + q * 32 + (m & 31)) = o;
                     }
                 }
             }
+            __syncthreads();
+            Out::template leave<kThreads>(lds, kRowsOut, (g.prob_words - m0) * NP, [&](int row) -> uint16_t * {
+                const int t = n0 + n_of(row, j);
+                return t < g.N ? (uint16_t *)g.prob + t * g.ldp + m0 * NP : nullptr;
+            });
+            __syncthreads();
         }
         if (g.bias_part || g.bias_out) {
             typedef typename ElementOf<P>::type E;
@@ -626,49 +671,30 @@ __device__ __forceinline__ void product_tile(const Args &g, const int block, cha
         }
     }
     if constexpr (KIND == kOut) {
+        typedef typename ElementOf<P>::type E;
+        static_assert(kRowsOut * BM * 4 <= kStagesBytes<P, BM, BN, STAGES>, "");
         const float factor = g.slice ? 1.f : out_factor<P>(g.factor);
 #pragma unroll
         for (int j = 0; j < NT; ++j) {
-            const int n = n_lane + j * U::size;
-            if (n >= g.n_store) continue;
+            auto leave = [&](auto kind, int64_t ld, void *base) {
+                typedef decltype(kind) S;
+                typedef Gather<S, BM> Out;
 #pragma unroll
-            for (int I = 0; I < MG; ++I) {
-                const int m = m_lane + m_of(I);
-                if (m >= g.M) continue;
-                const int many = min(4, g.M - m);
-                if (g.slice) {
-                    float *to = g.slice + ((int64_t)split * g.n_store + n) * g.M + m;
-                    if (many == 4 && g.M % 4 == 0) *(f32x4 *)to = f32x4{value(I, j, 0), value(I, j, 1), value(I, j, 2), value(I, j, 3)};
-                    else
+                for (int I = 0; I < MG; ++I) {
+                    Vec<S, 4> o;
 #pragma unroll
-                        for (int r = 0; r < 4; ++r)
-                            if (r < many) to[r] = value(I, j, r);
-                    continue;
+                    for (int r = 0; r < 4; ++r) o.v[r] = from_float<S>(value(I, j, r) * factor);
+                    *(Vec<S, 4> *)Out::at(lds, row_out, m_in + m_of(I)) = o;
                 }
-                float v[4];
-#pragma unroll
-                for (int r = 0; r < 4; ++r) v[r] = value(I, j, r) * factor;
-                const bool whole = many == 4 && g.ldo % 4 == 0 && (uintptr_t)g.out % 16 == 0;
-                if (g.out_type == DS_F32) {
-                    float *to = (float *)g.out + (int64_t)n * g.ldo + m;
-                    if (whole) *(f32x4 *)to = f32x4{v[0], v[1], v[2], v[3]};
-                    else
-#pragma unroll
-                        for (int r = 0; r < 4; ++r)
-                            if (r < many) to[r] = v[r];
-                } else {
-                    uint16_t *to = (uint16_t *)g.out + (int64_t)n * g.ldo + m;
-                    Vec<bf16_t, 4> o;
-#pragma unroll
-                    for (int r = 0; r < 4; ++r)
-                        o.v[r].bits = P::half ? from_float<f16_t>(v[r]).bits : from_float<bf16_t>(v[r]).bits;
-                    if (whole) *(Vec<bf16_t, 4> *)to = o;
-                    else
-#pragma unroll
-                        for (int r = 0; r < 4; ++r)
-                            if (r < many) to[r] = o.v[r].bits;
-                }
-            }
+                __syncthreads();
+                Out::template leave<kThreads>(lds, kRowsOut, g.M - m0, [&](int row) -> S * {
+                    const int n = n0 + n_of(row, j);
+                    return n < g.n_store ? (S *)base + n * ld + m0 : nullptr;
+                });
+                __syncthreads();
+            };
+            if (g.slice) leave(float{}, g.M, g.slice + (int64_t)split * g.n_store * g.M);
+            else leave(E{}, g.ldo, g.out);
         }
     }
 }

@@ -105,42 +105,43 @@ __device__ __forceinline__ void write_total(double loss, double rows, int mean, 
     total[1] = (float)share;
 }
 
-// Joins the tiles' maxima and sums: a workgroup has 64 rows, each of its 16 waves a sixteenth of the tiles.  The workgroup that
-// ends last adds up all of them, in order.
+// Joins the tiles' maxima and sums: a workgroup has kRowsJoined rows, each of its waves a sixteenth of the tiles and each
+// quarter of a wave a quarter of those.  The workgroup that ends last adds up all of them, in order.
+constexpr int kRowsJoined = 16;
+
 __global__ __launch_bounds__(1024) void row_kernel(const float2 *__restrict__ stats, const float *__restrict__ picked, int tiles,
                                                    int T, const void *__restrict__ target, int wide, int64_t V, int64_t ignore,
                                                    float *__restrict__ lse, float *__restrict__ loss, int reduction, Share *shares,
                                                    uint32_t *arrived, float *__restrict__ total)
 {
-    __shared__ float tops[16][64], sums[16][64];
-    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, t = blockIdx.x * 64 + lane;
+    __shared__ float tops[64][kRowsJoined], sums[64][kRowsJoined];
+    const int row = threadIdx.x % kRowsJoined, part = threadIdx.x / kRowsJoined, t = blockIdx.x * kRowsJoined + row;
     float top = -INFINITY, sum = 0.f;
+    auto join = [&](float top2, float sum2) {
+        const float both = fmaxf(top, top2);
+        sum = both == -INFINITY ? sum + sum2 : sum * exp2_of(top - both) + sum2 * exp2_of(top2 - both);
+        top = both;
+    };
     if (t < T) {
-        constexpr int kAhead = 8;
-        for (int i = wave; i < tiles; i += 16 * kAhead) {
+        constexpr int kAhead = 4;
+        for (int i = part; i < tiles; i += 64 * kAhead) {
             float2 s[kAhead];
 #pragma unroll
             for (int j = 0; j < kAhead; ++j)
-                s[j] = i + j * 16 < tiles ? stats[(int64_t)(i + j * 16) * T + t] : float2{-INFINITY, 0.f};
+                s[j] = i + j * 64 < tiles ? stats[(int64_t)(i + j * 64) * T + t] : float2{-INFINITY, 0.f};
 #pragma unroll
-            for (int j = 0; j < kAhead; ++j) {
-                const float both = fmaxf(top, s[j].x);
-                sum = both == -INFINITY ? sum + s[j].y : sum * exp2_of(top - both) + s[j].y * exp2_of(s[j].x - both);
-                top = both;
-            }
+            for (int j = 0; j < kAhead; ++j) join(s[j].x, s[j].y);
         }
     }
-    tops[wave][lane] = top, sums[wave][lane] = sum;
+    tops[part][row] = top, sums[part][row] = sum;
     __syncthreads();
-    if (wave != 0) return;
-    double mine = 0, counts = 0;
-    if (t < T) {
+    if (threadIdx.x >= 64) return;
+    // the quarters of a wave join 16 parts each, then each other
+    for (int i = part + 4; i < 64; i += 4) join(tops[i][row], sums[i][row]);
 #pragma unroll
-        for (int w = 1; w < 16; ++w) {
-            const float both = fmaxf(top, tops[w][lane]);
-            sum = both == -INFINITY ? sum + sums[w][lane] : sum * exp2_of(top - both) + sums[w][lane] * exp2_of(tops[w][lane] - both);
-            top = both;
-        }
+    for (int o = 16; o < 64; o <<= 1) join(__shfl_xor(top, o), __shfl_xor(sum, o));
+    double mine = 0, counts = 0;
+    if (t < T && part == 0) {
         const float all = sum == 0.f ? -INFINITY : top + log2f(sum);
         lse[t] = all;
         const int64_t y = target_of(target, wide, t);
@@ -151,6 +152,7 @@ __global__ __launch_bounds__(1024) void row_kernel(const float2 *__restrict__ st
     if (!reduction) return;
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) mine += __shfl_xor(mine, o), counts += __shfl_xor(counts, o);
+    const int lane = threadIdx.x;
     if (gridDim.x == 1) {
         if (lane == 0) write_total(mine, counts, reduction == DS_MEAN, total);
         return;
@@ -210,7 +212,14 @@ __global__ __launch_bounds__(256) void join_kernel(const float *__restrict__ sli
     const float factor = last ? out_factor<P>(f) : 1.f;
     for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
         float s = first ? 0.f : acc[i];
-        for (int k = 0; k < splits; ++k) s += slices[k * n + i];
+        constexpr int kAhead = 8;
+        for (int k = 0; k < splits; k += kAhead) {
+            float got[kAhead];
+#pragma unroll
+            for (int j = 0; j < kAhead; ++j) got[j] = k + j < splits ? slices[(k + j) * n + i] : 0.f;
+#pragma unroll
+            for (int j = 0; j < kAhead; ++j) s += got[j];
+        }
         if (last) out[i / M * ldo + i % M] = from_float<E>(s * factor);
         else acc[i] = s;
     }
@@ -321,7 +330,7 @@ Plan plan_of(const void *hidden, int64_t ldh, const void *weight, int64_t ldw, i
         const int64_t tiles = (p.piece + Shapes<P>::m[p.tile_logits] - 1) / Shapes<P>::m[p.tile_logits];
         p.stats = take((size_t)(tiles * p.pieces) * T * 8);
         p.picked = take((size_t)T * 4);
-        p.shares = take((size_t)((T + 63) / 64) * sizeof(Share));
+        p.shares = take((size_t)((T + kRowsJoined - 1) / kRowsJoined) * sizeof(Share));
         p.arrived = take(4);
     }
     if (what & kGrad) {
@@ -429,7 +438,7 @@ int loss(const Call &c, const Plan &p, bool counted_only, Operands<P> &o, int re
         DS_TRY(launch_product<P>(kLogitStats, p.tile_logits, g, nullptr, c.st));
         tiles += g.tiles_m;
     }
-    hipLaunchKernelGGL(row_kernel, dim3((unsigned)((c.T + 63) / 64)), dim3(1024), 0, c.st, (const float2 *)(c.ws + p.stats),
+    hipLaunchKernelGGL(row_kernel, dim3((unsigned)((c.T + kRowsJoined - 1) / kRowsJoined)), dim3(1024), 0, c.st, (const float2 *)(c.ws + p.stats),
                        (const float *)(c.ws + p.picked), tiles, (int)c.T, c.target, c.wide, c.V, c.ignore, lse, rows, reduction,
                        (Share *)(c.ws + p.shares), (uint32_t *)(c.ws + p.arrived), total);
     return launch_status();
@@ -486,7 +495,7 @@ int loss_grad(const Call &c, const Plan &p, Operands<P> &o, Grads r)
             x.K = which ? (int)c.T : (int)n;
             x.factor[0] = r.grad, x.factor[1] = r.share;
             x.out = which ? (void *)((E *)r.dweight + v0 * c.D) : r.dhidden;
-            x.ldo = c.D, x.out_type = c.type;
+            x.ldo = c.D;
             x.splits = which ? p.weight.splits : p.hidden.splits;
             x.k_split = ((x.K + x.splits - 1) / x.splits + P::step - 1) / P::step * P::step;
             joined[which] = x.splits > 1 || (!which && p.pieces > 1);

@@ -10,6 +10,7 @@ Functions whose names end in ``_grad`` return gradients directly; ``embedding`` 
 in autograd.
 """
 import array
+import contextlib
 import ctypes
 import math
 
@@ -50,20 +51,14 @@ def _rows_of(t):
     return t, t.stride(0) if t.size(0) > 1 else t.size(1)
 
 
-class _On:
+_HERE = contextlib.nullcontext()
+
+
+def _on(device):
     """Makes a tensor's device the current one for the launches of a call."""
-
-    def __init__(self, device):
-        self.device = device if device.index is not None and device.index != torch.cuda.current_device() else None
-
-    def __enter__(self):
-        if self.device is not None:
-            self.guard = torch.cuda.device(self.device)
-            self.guard.__enter__()
-
-    def __exit__(self, *exc):
-        if self.device is not None:
-            self.guard.__exit__(*exc)
+    if device.type != "cuda" or device.index == torch._C._cuda_getDevice():
+        return _HERE
+    return torch.cuda.device(device)
 
 
 # ---------------------------------------------------------------------------------------------
@@ -74,13 +69,14 @@ def _embed(ids, weight, scale):
     code = _type_of("weight", weight)
     if weight.dim() != 2:
         raise ValueError("weight must be [V, D]")
-    ids = _tokens_of("ids", ids, weight.device)
+    device = weight.device
+    ids = _tokens_of("ids", ids, device)
     weight, ld = _rows_of(weight)
     V, D = weight.shape
-    out = torch.empty(ids.shape + (D,), dtype=weight.dtype, device=weight.device)
-    with _On(weight.device):
+    out = torch.empty(ids.shape + (D,), dtype=weight.dtype, device=device)
+    with _on(device):
         _lib.call("ds_embed", ids.data_ptr(), ids.element_size(), weight.data_ptr(), ld, out.data_ptr(), ids.numel(), V, D,
-                  scale, code, _lib.stream_handle(weight.device))
+                  scale, code, _lib.stream_handle(device))
     return out
 
 
@@ -99,7 +95,7 @@ def embedding_grad(ids, grad, num_embeddings, scale=1.0, padding_idx=None):
     T = ids.numel()
     grad, ld = _rows_of(grad.reshape(T, D))
     out = torch.empty((V, D), dtype=grad.dtype, device=grad.device)
-    with _On(grad.device):
+    with _on(grad.device):
         nbytes = _lib.lib().ds_embed_grad_workspace_bytes(T, D)
         ws = kernels._workspace(nbytes, grad.device)
         _lib.call("ds_embed_grad", ids.data_ptr(), ids.element_size(), grad.data_ptr(), ld, out.data_ptr(), T, V, D, padding,
@@ -234,7 +230,7 @@ class _Head:
 class _LinearCrossEntropy(Function):
     @staticmethod
     def forward(ctx, hidden, weight, target, bias, ignore_index, reduction):
-        with _On(hidden.device):
+        with _on(hidden.device):
             head = _Head(hidden, weight, target, bias, ignore_index, reduction)
             loss, lse, share = head.loss()
         ctx.save_for_backward(hidden, weight, target, bias, lse, share)
@@ -244,7 +240,7 @@ class _LinearCrossEntropy(Function):
     @staticmethod
     def backward(ctx, grad):
         hidden, weight, target, bias, lse, share = ctx.saved_tensors
-        with _On(hidden.device):
+        with _on(hidden.device):
             head = _Head(hidden, weight, target, bias, *ctx.of)
             grad = grad.float().contiguous()
             needed = ctx.needs_input_grad
@@ -263,14 +259,14 @@ def linear_cross_entropy(hidden, weight, target, bias=None, ignore_index=-100, r
     A bias of ``-inf`` takes a word out."""
     if torch.is_grad_enabled() and (hidden.requires_grad or weight.requires_grad or (bias is not None and bias.requires_grad)):
         return _LinearCrossEntropy.apply(hidden, weight, target, bias, ignore_index, reduction)
-    with _On(hidden.device):
+    with _on(hidden.device):
         return _Head(hidden, weight, target, bias, ignore_index, reduction).loss()[0]
 
 
 def linear_cross_entropy_grad(hidden, weight, target, bias=None, ignore_index=-100, reduction="mean"):
     """``(loss, dhidden, dweight, dbias)`` of :func:`linear_cross_entropy` for a gradient of 1 (of ones, with
     ``reduction='none'``), without autograd; ``dbias`` is ``None`` where there is no bias."""
-    with torch.no_grad(), _On(hidden.device):
+    with torch.no_grad(), _on(hidden.device):
         return _Head(hidden, weight, target, bias, ignore_index, reduction).step()
 
 
@@ -314,7 +310,7 @@ def _clip(grads, max_norm, out, scale):
     else:
         table[3::4] = array.array("q", [a | b << 32 for a, b in zip(codes, to)])
     norm = torch.empty((), dtype=torch.float32, device=device)
-    with _On(device):
+    with _on(device):
         nbytes = _lib.lib().ds_clip_workspace_bytes(len(grads))
         ws = kernels._workspace(nbytes, device)
         _lib.call("ds_clip", ctypes.cast(table.buffer_info()[0], _lib._tp), len(grads), max_norm, int(scale), norm.data_ptr(),
