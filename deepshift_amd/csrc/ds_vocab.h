@@ -74,6 +74,16 @@ __device__ __forceinline__ void split_planes(float f, bf16_t *p)
     }
 }
 
+// Four values rounded to the 16-bit type of P, to nearest even.
+template <typename P>
+__device__ __forceinline__ s16x4 round4(f32x4 v)
+{
+    typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
+    typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
+    if constexpr (P::half) return __builtin_bit_cast(s16x4, __builtin_convertvector(v, f16x4));
+    else return __builtin_bit_cast(s16x4, __builtin_convertvector(v, bf16x4));
+}
+
 // An operand: `rows` x `k` elements, 16 bits each.  Contiguous along k (element (r, k) at r * ld + k) or across it (at
 // k * ld + r).  ld and the address allow 16-byte accesses; past `rows` or `k` everything up to the next multiple of 8 along the
 // contiguous axis may be read and is zero, nothing beyond is touched.  Three planes lie in turns of 32 elements along the
@@ -294,9 +304,10 @@ template <typename P, int BM, int BN, int STAGES>
 constexpr int kStagesBytes = STAGES * P::planes * (BM + BN) * P::step * 2;
 template <int BM, int BN>
 struct Known {
-    float bias[BM];
-    int want[BN];     // the target, counted from the tile's first word, where it lies in the tile; else -1
-    float lse[BN], scale[BN];
+    float bias[BM];   // times log2 e; -inf for words past the end, which leave nothing that way
+    int want[BN];     // the target, counted from the tile's first word, where it lies in the tile; else far below 0
+    float lse[BN];    // +inf for rows that do not count: theirs are probabilities of 0
+    float scale[BN];
 };
 template <typename P, int BM, int BN, int STAGES, bool LOGITS>
 constexpr int kLdsBytes = kStagesBytes<P, BM, BN, STAGES> + (LOGITS ? (int)sizeof(Known<BM, BN>) : 0);
@@ -389,17 +400,22 @@ __device__ __forceinline__ void product_tile(const Args &g, const int block, cha
 
     Known<BM, BN> &known = *(Known<BM, BN> *)(lds + kStagesBytes<P, BM, BN, STAGES>);
     static_assert(BM <= WAVES * 64 && BN <= WAVES * 64, "a thread per word and token");
-    float bias = 0.f, lse = 0.f, scale = 0.f;
-    int want = -1;
+    constexpr int kNowhere = -(1 << 20);
+    float bias = -INFINITY, lse = INFINITY, scale = 0.f;
+    int want = kNowhere;
     if constexpr (KIND != kOut) {
         const int m = m0 + threadIdx.x, n = n0 + threadIdx.x;
-        if (threadIdx.x < BM && m < g.M) bias = bias_at(g, g.v0 + m);
+        if (threadIdx.x < BM && m < g.M) bias = bias_at(g, g.v0 + m) * kLog2e;
         if (threadIdx.x < BN && n < g.N) {
             const int64_t y = target_at(g, n), here = y - g.v0 - m0;
             if (here >= 0 && here < BM && m0 + here < g.M) want = (int)here;
             if constexpr (KIND == kProb) {
-                lse = g.lse[n];
-                scale = y == g.ignore ? 0.f : y < 0 || y >= g.V ? NAN : g.row_scale ? g.row_scale[n] : 1.f;
+                if (y != g.ignore) {
+                    lse = g.lse[n];
+                    scale = y < 0 || y >= g.V ? NAN : g.row_scale ? g.row_scale[n] : 1.f;
+                } else {
+                    want = kNowhere;
+                }
             }
         }
     }
@@ -530,45 +546,36 @@ __device__ __forceinline__ void product_tile(const Args &g, const int block, cha
     // This lane's results: I counts its groups of four neighbouring m, j its n.
     constexpr int MG = MT * U::groups;
     const int m_in = wm * MT * U::size + U::lane_m(lane), n_in = wn * NT * U::size + lane % U::size;  // in the tile
-    const int m_lane = m0 + m_in, n_lane = n0 + n_in;
     auto m_of = [](int I) constexpr { return I / U::groups * U::size + U::group_m(I % U::groups); };
     auto value = [&](int I, int j, int r) -> float { return acc[I / U::groups][j][I % U::groups * 4 + r]; };
     float *fl = (float *)lds;
-    if constexpr (KIND != kOut) {
-        // acc becomes the logits in base 2
-#pragma unroll
-        for (int I = 0; I < MG; ++I)
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const bool real = m_lane + m_of(I) + r < g.M;
-                const float b = known.bias[m_in + m_of(I) + r];
-#pragma unroll
-                for (int j = 0; j < NT; ++j) acc[I / U::groups][j][I % U::groups * 4 + r] = real ? (value(I, j, r) + b) * kLog2e : -INFINITY;
-            }
-    }
+    // a logit, base 2
+    auto logit = [&](int I, int j, int r) -> float { return fmaf(value(I, j, r), kLog2e, known.bias[m_in + m_of(I) + r]); };
     if constexpr (KIND == kStats) {
         if (block == 0 && threadIdx.x == 0) *g.arrived = 0;
 #pragma unroll
         for (int j = 0; j < NT; ++j) {
-            const int t = n_lane + j * U::size;
-            const int at = known.want[n_in + j * U::size] - m_in;  // below 0 or past this lane's words: not here
-            float top = -INFINITY;
+            const int at = known.want[n_in + j * U::size] - m_in;  // where the target lies behind this lane's first word
+            float s[MG][4], top = -INFINITY;
 #pragma unroll
-            for (int I = 0; I < MG; ++I)
+            for (int I = 0; I < MG; ++I) {
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
-                    // a maximum that a value which is no number does not slip through
-                    const float v = value(I, j, r);
-                    top = v > top || v != v ? v : top;
-                    if (at == m_of(I) + r) g.picked[t] = v;
+                    s[I][r] = logit(I, j, r);
+                    top = fmaxf(top, s[I][r]);  // what is no number shows in the sum
                 }
+                if ((unsigned)(at - m_of(I)) < 4u)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r)
+                        if (at == m_of(I) + r) g.picked[n0 + n_in + j * U::size] = s[I][r];
+            }
             float sum = 0.f;
             // a column of nothing but -inf keeps a sum of 0
             const float base = top == -INFINITY ? 0.f : top;
 #pragma unroll
             for (int I = 0; I < MG; ++I)
 #pragma unroll
-                for (int r = 0; r < 4; ++r) sum += exp2_of(value(I, j, r) - base);
+                for (int r = 0; r < 4; ++r) sum += exp2_of(s[I][r] - base);
 #pragma unroll
             for (int o = U::size; o < 64; o <<= 1) {
                 const float top2 = __shfl_xor(top, o), sum2 = __shfl_xor(sum, o);
@@ -614,22 +621,32 @@ __device__ __forceinline__ void product_tile(const Args &g, const int block, cha
             const int at = known.want[n_in + j * U::size] - m_in;
 #pragma unroll
             for (int I = 0; I < MG; ++I) {
-                float p[4];
+                float x[4], p[4], least = INFINITY;
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
-                    const float e = exp2f(value(I, j, r) - lse) - (at == m_of(I) + r ? 1.f : 0.f);
-                    // rows that do not count leave nothing, whatever their logits are; neither do words past the end
-                    p[r] = scale == 0.f || m_lane + m_of(I) + r >= g.M ? 0.f : e * scale;
+                    x[r] = logit(I, j, r) - lse;
+                    least = fminf(least, x[r]);
+                }
+                // below 2^-126 the instruction by itself gives 0
+                if (__any(least < -126.f)) {
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) p[r] = exp2f(x[r]);
+                } else {
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) p[r] = exp2_of(x[r]);
+                }
+                if ((unsigned)(at - m_of(I)) < 4u)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) p[r] -= at == m_of(I) + r ? 1.f : 0.f;
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    p[r] *= scale;
                     over_n[I][r] += p[r];
                     if constexpr (P::half) p[r] *= kProbScale;
                 }
                 const int m = m_in + m_of(I);
                 if constexpr (NP == 1) {
-                    Vec<bf16_t, 4> o;
-#pragma unroll
-                    for (int r = 0; r < 4; ++r)
-                        o.v[r].bits = P::half ? from_float<f16_t>(p[r]).bits : from_float<bf16_t>(p[r]).bits;
-                    *(Vec<bf16_t, 4> *)Out::at(lds, row_out, m) = o;
+                    *(s16x4 *)Out::at(lds, row_out, m) = round4<P>(f32x4{p[0], p[1], p[2], p[3]});
                 } else {
                     bf16_t planes[4][3];
 #pragma unroll
@@ -681,10 +698,10 @@ __device__ __forceinline__ void product_tile(const Args &g, const int block, cha
                 typedef Gather<S, BM> Out;
 #pragma unroll
                 for (int I = 0; I < MG; ++I) {
-                    Vec<S, 4> o;
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) o.v[r] = from_float<S>(value(I, j, r) * factor);
-                    *(Vec<S, 4> *)Out::at(lds, row_out, m_in + m_of(I)) = o;
+                    const f32x4 v = f32x4{value(I, j, 0), value(I, j, 1), value(I, j, 2), value(I, j, 3)} * factor;
+                    char *to = Out::at(lds, row_out, m_in + m_of(I));
+                    if constexpr (sizeof(S) == 4) *(f32x4 *)to = v;
+                    else *(s16x4 *)to = round4<P>(v);
                 }
                 __syncthreads();
                 Out::template leave<kThreads>(lds, kRowsOut, g.M - m0, [&](int row) -> S * {
