@@ -737,17 +737,20 @@ __global__ __launch_bounds__(WM * WN * 64) void both_kernel(Args hidden, Args we
 // Which product a launch is.
 enum { kLogitStats = 0, kLogitProb = 1, kHidden = 2, kWeight = 3 };
 
-// Tile shapes, m x n, by their number in a launch.  For choosing among them: workgroups that a CU holds, and the measured
-// microseconds of a step of the reduction while every CU has its fill, and while none has more than one.
+// Tile shapes, m x n, by their number in a launch.  For choosing among them: workgroups that a CU holds, and measured, in
+// microseconds, a step of the reduction while every CU has its fill, a step while none has more than one workgroup, and what a
+// workgroup takes to begin and end.
 constexpr int kShapes = 4;
 template <typename P> struct Shapes {
     static constexpr int m[kShapes] = {256, 128, 128, 64}, n[kShapes] = {256, 128, 64, 64}, resident[kShapes] = {1, 2, 2, 3};
-    static constexpr float step_us[kShapes] = {1.8f, 1.2f, 0.85f, 0.7f}, alone_us[kShapes] = {1.2f, 0.78f, 0.5f, 0.35f};
+    static constexpr float step_us[kShapes] = {1.6f, 1.05f, 0.8f, 0.5f}, alone_us[kShapes] = {1.0f, 0.6f, 0.5f, 0.3f};
+    static constexpr float ends_us[kShapes] = {7.f, 5.f, 4.f, 3.f};
 };
 template <> struct Shapes<Split> {
     // the last for logits only
     static constexpr int m[kShapes] = {256, 128, 64, 32}, n[kShapes] = {128, 128, 64, 32}, resident[kShapes] = {1, 1, 1, 2};
-    static constexpr float step_us[kShapes] = {2.7f, 1.7f, 0.6f, 0.5f}, alone_us[kShapes] = {2.5f, 1.5f, 0.55f, 0.27f};
+    static constexpr float step_us[kShapes] = {2.5f, 1.6f, 0.75f, 0.5f}, alone_us[kShapes] = {2.0f, 1.1f, 0.57f, 0.38f};
+    static constexpr float ends_us[kShapes] = {9.f, 5.f, 3.f, 3.f};
 };
 template <typename P> constexpr int kGradShapes = P::planes == 1 ? 4 : 3;
 

@@ -201,16 +201,43 @@ __global__ __launch_bounds__(1024) void row_scale_kernel(const float *__restrict
 
 // ---- joins -------------------------------------------------------------------------------------------------------
 
+// The sums of a bias's tiles, to the gradient of 256 words.
+struct BiasJoin {
+    const float *part;
+    int ld, tiles, n;
+    void *out;
+};
+template <typename E>
+__device__ __forceinline__ void join_bias(const BiasJoin &b, int block, float factor)
+{
+    const int v = block * 256 + threadIdx.x;
+    if (v >= b.n) return;
+    float s = 0.f;
+#pragma unroll 4
+    for (int i = 0; i < b.tiles; ++i) s += b.part[(int64_t)i * b.ld + v];
+    ((E *)b.out)[v] = from_float<E>(s * factor);
+}
+template <typename E>
+__global__ __launch_bounds__(256) void bias_join_kernel(BiasJoin b, const float *f0, const float *f1)
+{
+    const float *const f[2] = {f0, f1};
+    join_bias<E>(b, blockIdx.x, factor_of(f));
+}
+
 // The slices of a product in order, behind what earlier pieces of the vocabulary left in `acc`; the last piece's result is
-// multiplied and rounded.
+// multiplied and rounded.  Workgroups from `blocks` on join a bias.
 template <typename P, typename E>
 __global__ __launch_bounds__(256) void join_kernel(const float *__restrict__ slices, int splits, int64_t n, int M, float *acc,
                                                    int first, int last, const float *f0, const float *f1, E *__restrict__ out,
-                                                   int64_t ldo)
+                                                   int64_t ldo, int blocks, BiasJoin bias)
 {
     const float *const f[2] = {f0, f1};
+    if ((int)blockIdx.x >= blocks) {
+        join_bias<E>(bias, blockIdx.x - blocks, factor_of(f));
+        return;
+    }
     const float factor = last ? out_factor<P>(f) : 1.f;
-    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)blocks * 256) {
         float s = first ? 0.f : acc[i];
         constexpr int kAhead = 8;
         for (int k = 0; k < splits; k += kAhead) {
@@ -225,27 +252,16 @@ __global__ __launch_bounds__(256) void join_kernel(const float *__restrict__ sli
     }
 }
 
-template <typename E>
-__global__ __launch_bounds__(256) void bias_join_kernel(const float *__restrict__ part, int ld, int tiles, int n, const float *f0,
-                                                        const float *f1, E *__restrict__ out)
-{
-    const int v = blockIdx.x * 256 + threadIdx.x;
-    if (v >= n) return;
-    float s = 0.f;
-#pragma unroll 4
-    for (int i = 0; i < tiles; ++i) s += part[(int64_t)i * ld + v];
-    out[v] = from_float<E>(s * (f0 ? *f0 : 1.f) * (f1 ? *f1 : 1.f));
-}
-
 // ---- plan --------------------------------------------------------------------------------------------------------
 
 constexpr size_t kPieceBytes = (size_t)1 << 30;  // of P, and of repacked weights
 
 // The tile shape of a product, and how many stretches its reduction of k is cut into (1 of `most_splits`): the pair with the
-// shortest estimate.  A round of workgroups takes its steps and some four more to begin and end; slices are written and read
-// once more by a launch of their own.  What decides it, measured: 1543 x 1000 results from 20011 words, float16, 157 us on
-// 128 x 128 tiles in two stretches, 89 us on 256 x 256 in nine; 2048 x 1024 from 32768 words, float32, 1113 and 768 us;
-// 64 x 512 from 1000 words, float32, 25 us in one stretch, 13 in four.
+// shortest estimate, rounds of workgroups times their steps and ends; slices are written and read once more by a launch of
+// their own.  What decides it, measured: hidden gradients of 1543 x 1000 from 20011 words, float16, 157 us on 128 x 128 tiles
+// in two stretches, 76 us on 256 x 256 in eight; 2048 x 1024 from 32768 words, float32, 1113 us (128 x 128, two) and 707 us
+// (256 x 128, four); 64 x 512 from 1000 words, float32, 25 us in one stretch, 13 in four; scores of 512 tokens of 1024 features
+// over 8000 words, bfloat16, 25, 16, 16 and 19 us from the largest tiles to the smallest.
 struct Choice { int tile, splits; };
 template <typename P>
 Choice choose(int64_t m, int64_t n, int64_t k, int shapes, int most_splits)
@@ -269,7 +285,7 @@ Choice choose(int64_t m, int64_t n, int64_t k, int shapes, int most_splits)
         for (int s = split_knob >= 1 ? most : 1; s <= most; s += 1 + s / 4) {
             const int64_t blocks = tiles * s;
             const double step = blocks <= cus ? S::alone_us[i] : S::step_us[i];
-            const double us = (double)((blocks + fill - 1) / fill) * ((double)((steps + s - 1) / s) + 4) * step +
+            const double us = (double)((blocks + fill - 1) / fill) * ((double)((steps + s - 1) / s) * step + S::ends_us[i]) +
                               (s > 1 ? 4 + (double)s * m * n * 4 / 3e6 : 0);
             if (us < shortest) shortest = us, best = Choice{i, s};
         }
@@ -478,9 +494,16 @@ int loss_grad(const Call &c, const Plan &p, Operands<P> &o, Grads r)
             DS_TRY(launch_product<P>(kLogitProb, p.tile_logits, g, nullptr, c.st));
             bias_tiles = g.tiles_n;
         }
-        if (r.dbias && bias_tiles != 1)
-            hipLaunchKernelGGL((bias_join_kernel<E>), dim3((unsigned)((n + 255) / 256)), dim3(256), 0, c.st,
-                               (const float *)(c.ws + p.bias), p.words, bias_tiles, (int)n, r.grad, r.share, (E *)r.dbias + v0);
+        BiasJoin bias{(const float *)(c.ws + p.bias), p.words, bias_tiles, (int)n, r.dbias ? (E *)r.dbias + v0 : nullptr};
+        bool bias_left = r.dbias && bias_tiles != 1;
+        // by itself, or along with the join of a product
+        auto join_bias_alone = [&] {
+            if (bias_left)
+                hipLaunchKernelGGL((bias_join_kernel<E>), dim3((unsigned)((n + 255) / 256)), dim3(256), 0, c.st, bias, r.grad,
+                                   r.share);
+            bias_left = false;
+        };
+        if (c.D == 0) join_bias_alone();
         if (c.D == 0) continue;
         Args g[2] = {};
         bool wanted[2], joined[2];
@@ -506,6 +529,7 @@ int loss_grad(const Call &c, const Plan &p, Operands<P> &o, Grads r)
                                (ceil_div((int)c.T, Shapes<P>::n[p.weight.tile]) + ceil_div((int)n, Shapes<P>::n[p.weight.tile]));
         if (wanted[0] && wanted[1] && !joined[0] && !joined[1] && p.hidden.tile == p.weight.tile && blocks <= 2 * device_cus()) {
             DS_TRY(launch_product<P>(kHidden, p.weight.tile, g[0], &g[1], c.st));
+            join_bias_alone();
             continue;
         }
         for (int which = 0; which < 2; ++which) {
@@ -514,11 +538,14 @@ int loss_grad(const Call &c, const Plan &p, Operands<P> &o, Grads r)
             DS_TRY(launch_product<P>(which ? kWeight : kHidden, which ? p.weight.tile : p.hidden.tile, x, nullptr, c.st));
             if (!joined[which]) continue;
             const int64_t count = (int64_t)x.n_store * c.D;
-            const int64_t join = (count + 255) / 256;
-            hipLaunchKernelGGL((join_kernel<P, E>), dim3((unsigned)(join < 16384 ? join : 16384)), dim3(256), 0, c.st, slices,
-                               x.splits, count, (int)c.D, which ? nullptr : (float *)(c.ws + p.acc), which || first, which || last,
-                               r.grad, r.share, (E *)x.out, c.D);
+            const int64_t all = (count + 255) / 256;
+            const int join = (int)(all < 16384 ? all : 16384), more = bias_left ? ceil_div((int)n, 256) : 0;
+            hipLaunchKernelGGL((join_kernel<P, E>), dim3(join + more), dim3(256), 0, c.st, slices, x.splits, count, (int)c.D,
+                               which ? nullptr : (float *)(c.ws + p.acc), which || first, which || last, r.grad, r.share,
+                               (E *)x.out, c.D, join, bias);
+            bias_left = false;
         }
+        join_bias_alone();
     }
     return launch_status();
 }
