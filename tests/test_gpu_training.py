@@ -614,3 +614,35 @@ def test_refusals():
     assert L.ds_embed(ids.data_ptr(), 8, w.data_ptr(), 7, f.data_ptr(), 4, 5, 8, 1.0, 0, None) == -1
     assert L.ds_embed_grad(ids.data_ptr(), 8, f.data_ptr(), 8, w.data_ptr(), 4, 5, 8, -1, 1.0, 0, ws.data_ptr(), 16, None) == -4
     assert L.ds_embed_grad(ids.data_ptr(), 8, f.data_ptr(), 8, w.data_ptr(), 4, 5, 8, -1, 1.0, 7, ws.data_ptr(), 1 << 20, None) == -1
+
+
+# ---- together -----------------------------------------------------------------------------------------------------
+
+def test_a_step_of_the_token_model_against_plain_torch():
+    from deepshift_amd import train_tokens
+    torch.manual_seed(5)
+    with torch.device(DEV):
+        model = train_tokens.TokenModel(300, 32, 2)
+    generator = torch.Generator(device=DEV).manual_seed(1)
+    pair, target = train_tokens.batch(200, 300, torch.device(DEV), generator, ignored=0.2)
+    loss = model(pair, target)
+    loss.backward()
+    got = {n: p.grad.clone() for n, p in model.named_parameters()}
+    model.zero_grad()
+    x = torch.nn.functional.embedding(pair, model.embedding.weight).mul(model.embedding.scale).flatten(1)
+    for norm, layer in zip(model.norms, model.layers):
+        x = x + torch.relu(layer(norm(x)))
+    want = torch.nn.functional.cross_entropy(model.head.logits(x), target)
+    want.backward()
+    torch.testing.assert_close(loss, want, rtol=1e-5, atol=0)
+    for n, p in model.named_parameters():
+        # the same float32 layers between: what differs is the order of sums
+        assert (got[n] - p.grad).norm() <= 1e-4 * p.grad.norm(), n
+
+
+@pytest.mark.parametrize("shift_type", ["PS", "Q"])
+def test_the_token_model_learns(shift_type):
+    from deepshift_amd import train_tokens
+    first, last = train_tokens.main(["--steps", "60", "--tokens", "2048", "--vocabulary", "64", "--width", "128", "--depth", "1",
+                                     "--shift-type", shift_type, "--lr", "0.01"])
+    assert last < 0.8 * first
