@@ -525,17 +525,14 @@ int loss_grad(const Call &c, const Plan &p, Operands<P> &o, Grads r)
             x.slice = joined[which] ? slices : nullptr;
         }
         // few workgroups each, and no slices to share: both in one launch
-        const int64_t blocks = (int64_t)ceil_div((int)c.D, Shapes<P>::m[p.weight.tile]) *
-                               (ceil_div((int)c.T, Shapes<P>::n[p.weight.tile]) + ceil_div((int)n, Shapes<P>::n[p.weight.tile]));
-        if (wanted[0] && wanted[1] && !joined[0] && !joined[1] && p.hidden.tile == p.weight.tile && blocks <= 2 * device_cus()) {
-            DS_TRY(launch_product<P>(kHidden, p.weight.tile, g[0], &g[1], c.st));
-            join_bias_alone();
-            continue;
-        }
+        const int tm = Shapes<P>::m[p.weight.tile], tn = Shapes<P>::n[p.weight.tile];
+        const int64_t blocks = (int64_t)ceil_div((int)c.D, tm) * ((int64_t)ceil_div((int)c.T, tn) * p.hidden.splits + ceil_div((int)n, tn));
+        const bool both = wanted[0] && wanted[1] && !joined[1] && p.hidden.tile == p.weight.tile && blocks <= 2 * device_cus();
+        if (both) DS_TRY(launch_product<P>(kHidden, p.weight.tile, g[0], &g[1], c.st));
         for (int which = 0; which < 2; ++which) {
             Args &x = g[which];
             if (!wanted[which]) continue;
-            DS_TRY(launch_product<P>(which ? kWeight : kHidden, which ? p.weight.tile : p.hidden.tile, x, nullptr, c.st));
+            if (!both) DS_TRY(launch_product<P>(which ? kWeight : kHidden, which ? p.weight.tile : p.hidden.tile, x, nullptr, c.st));
             if (!joined[which]) continue;
             const int64_t count = (int64_t)x.n_store * c.D;
             const int64_t all = (count + 255) / 256;
