@@ -483,60 +483,101 @@ __device__ __forceinline__ void product_tile(const Args &g, const int block, cha
             a_at += a_step, b_at += b_step, k_left -= kStep;
         }
     } else {
+        // Rows of tiles that are multiplied together: the six products of a tile follow each other, so four tiles at least have
+        // to take turns.  While one such group is multiplied the next one's fragments of A are read; during the last group of a
+        // stage, whose fragments are all there by then, the next stage's first ones, and its own slot is fetched anew.
+        constexpr int G = NT >= 4 || MT == 1 ? 1 : 2, kGroups = MT / G;
+        static_assert(MT % G == 0 && (kGroups == 1 || kGroups % 2 == 0), "");
+        constexpr int kTurns = 6, kFetches = NP * (TA::mine + TB::mine), kReads = NP * (NT + G);
+        s16x8 b0[NP][NT], b1[NP][NT], a0[G][NP], a1[G][NP], turn[G][NP];
+        auto read_a = [&](int from, int group, int n, s16x8 (&fa)[G][NP]) {
+            const int i = n / NP, p = n % NP;
+            fa[i][p] = TA::fragment(lds + from * kStageBytes + p * TA::bytes, (wm * MT + group * G + i) * U::size, 0);
+        };
+        auto read_b = [&](int from, int n, s16x8 (&fb)[NP][NT]) {
+            const int p = n / NT, j = n % NT;
+            fb[p][j] = TB::fragment(lds + from * kStageBytes + NP * TA::bytes + p * TB::bytes, (wn * NT + j) * U::size, 0);
+        };
+        // the products of 2^-16, then those of 2^-8, then the largest; between(0) .. between(kTurns - 1) in between
+        auto multiply = [&](int group, const s16x8 (&fa)[G][NP], const s16x8 (&fb)[NP][NT], auto between) {
+            f32x4 low[G][NT];
+            auto add = [&](int p, int q) {
 #pragma unroll
-        for (int s = 0; s < STAGES - 1; ++s) fetch_stage(s);
-        keep_known();
-        // rows of tiles that are multiplied together: the six products of a tile follow each other, so four tiles at least
-        // have to take turns
-        constexpr int G = NT >= 4 || MT == 1 ? 1 : 2;
-        static_assert(MT % G == 0, "");
-        for (int s = 0; s < steps; ++s) {
+                for (int i = 0; i < G; ++i)
+#pragma unroll
+                    for (int j = 0; j < NT; ++j) low[i][j] = U::multiply(fa[i][p], fb[q][j], low[i][j]);
+            };
+#pragma unroll
+            for (int i = 0; i < G; ++i)
+#pragma unroll
+                for (int j = 0; j < NT; ++j) low[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+            add(1, 1), between(0);
+            add(0, 2), between(1);
+            add(2, 0), between(2);
+#pragma unroll
+            for (int i = 0; i < G; ++i)
+#pragma unroll
+                for (int j = 0; j < NT; ++j) low[i][j] *= 1.f / 256;
+            add(0, 1), between(3);
+            add(1, 0), between(4);
+#pragma unroll
+            for (int i = 0; i < G; ++i)
+#pragma unroll
+                for (int j = 0; j < NT; ++j) {
+                    f32x4 &c = acc[group * G + i][j];
+                    c = U::multiply(fa[i][0], fb[0][j], c);
+                }
+            between(5);
+#pragma unroll
+            for (int i = 0; i < G; ++i)
+#pragma unroll
+                for (int j = 0; j < NT; ++j) {
+                    f32x4 &c = acc[group * G + i][j];
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) c[r] = fmaf(low[i][j][r], 1.f / 256, c[r]);
+                }
+        };
+        auto step = [&](s16x8 (&fb)[NP][NT], s16x8 (&fa)[G][NP], s16x8 (&next_b)[NP][NT], s16x8 (&next_a)[G][NP]) {
+#pragma unroll
+            for (int k = 0; k + 1 < kGroups; ++k)
+                multiply(k, k % 2 ? turn : fa, fb, [&](int t) {
+                    if (t == 0)
+#pragma unroll
+                        for (int n = 0; n < G * NP; ++n) read_a(slot, k + 1, n, k % 2 ? fa : turn);
+                    __builtin_amdgcn_sched_barrier(0);
+                });
             wait_for_stage<(STAGES - 2) * kInFlight>();
-            fetch_stage(slot == 0 ? STAGES - 1 : slot - 1);
-            const char *at = lds + slot * kStageBytes;
-            s16x8 fb[NP][NT];
-#pragma unroll
-            for (int p = 0; p < NP; ++p)
-#pragma unroll
-                for (int j = 0; j < NT; ++j)
-                    fb[p][j] = TB::fragment(at + NP * TA::bytes + p * TB::bytes, (wn * NT + j) * U::size, 0);
-#pragma unroll
-            for (int i0 = 0; i0 < MT; i0 += G) {
-                s16x8 fa[G][NP];
-                f32x4 low[G][NT];
-#pragma unroll
-                for (int i = 0; i < G; ++i)
-#pragma unroll
-                    for (int p = 0; p < NP; ++p)
-                        fa[i][p] = TA::fragment(at + p * TA::bytes, (wm * MT + i0 + i) * U::size, 0);
-                // the products of 2^-16, then those of 2^-8, then the largest
-                auto add = [&](int p, int q) {
-#pragma unroll
-                    for (int i = 0; i < G; ++i)
-#pragma unroll
-                        for (int j = 0; j < NT; ++j) low[i][j] = U::multiply(fa[i][p], fb[q][j], low[i][j]);
-                };
-#pragma unroll
-                for (int i = 0; i < G; ++i)
-#pragma unroll
-                    for (int j = 0; j < NT; ++j) low[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-                add(1, 1), add(0, 2), add(2, 0);
-#pragma unroll
-                for (int i = 0; i < G; ++i)
-#pragma unroll
-                    for (int j = 0; j < NT; ++j) low[i][j] *= 1.f / 256;
-                add(0, 1), add(1, 0);
-#pragma unroll
-                for (int i = 0; i < G; ++i)
-#pragma unroll
-                    for (int j = 0; j < NT; ++j) {
-                        f32x4 &c = acc[i0 + i][j];
-                        c = U::multiply(fa[i][0], fb[0][j], c);
-#pragma unroll
-                        for (int r = 0; r < 4; ++r) c[r] = fmaf(low[i][j][r], 1.f / 256, c[r]);
-                    }
-            }
+            const uint32_t to = lds0 + slot * kStageBytes;
             slot = slot + 1 == STAGES ? 0 : slot + 1;
+            multiply(kGroups - 1, kGroups > 1 ? turn : fa, fb, [&](int t) {
+                // a share of the fetches and of the reads, the latter in the first five turns
+#pragma unroll
+                for (int f = 0; f < kFetches; ++f) {
+                    if (f * kTurns / kFetches != t) continue;
+                    if (f < NP * TA::mine) ta.one(a_at, k_left, to, wave, f / TA::mine, f % TA::mine);
+                    else tb.one(b_at, k_left, to + NP * TA::bytes, wave, (f - NP * TA::mine) / TB::mine, (f - NP * TA::mine) % TB::mine);
+                }
+#pragma unroll
+                for (int n = 0; n < kReads; ++n) {
+                    if (n * (kTurns - 1) / kReads != t) continue;
+                    if (n < G * NP) read_a(slot, 0, n, next_a);
+                    else read_b(slot, n - G * NP, next_b);
+                }
+                __builtin_amdgcn_sched_barrier(0);
+            });
+            a_at += a_step, b_at += b_step, k_left -= kStep;
+        };
+#pragma unroll
+        for (int s = 0; s < STAGES; ++s) fetch_stage(s);
+        keep_known();
+        wait_for_stage<(STAGES - 1) * kInFlight>();
+#pragma unroll
+        for (int n = 0; n < G * NP; ++n) read_a(0, 0, n, a0);
+#pragma unroll
+        for (int n = 0; n < NP * NT; ++n) read_b(0, n, b0);
+        for (int s = 0; s < steps; s += 2) {
+            step(b0, a0, b1, a1);
+            if (s + 1 < steps) step(b1, a1, b0, a0);
         }
     }
     // nothing of this wave is on its way to LDS any more, and nobody reads it
