@@ -99,7 +99,12 @@ template <typename P> __host__ __device__ constexpr int64_t row_elements(int64_t
 }
 
 // What a launch computes with its tiles.
-enum { kStats = 0, kProb = 1, kOut = 2 };
+enum {
+    kStats = 0,  // maxima and sums of the logits' exponentials
+    kKeep = 1,   // the same, and the exponentials themselves, relative to their tile's maximum, where P will be
+    kProb = 2,   // P, from finished sums
+    kOut = 3     // a gradient
+};
 
 struct Args {
     Operand a, b;
@@ -113,9 +118,9 @@ struct Args {
     int target_wide;
     int64_t V, ignore;
     int v0;
-    float *stats;         // kStats: [tiles_m] [T][2] maximum and sum of exponentials, base 2
-    float *picked;        // kStats: [T] the target's logit
-    // kProb
+    float *stats;         // kStats, kKeep: [tiles_m] [T][2] maximum and sum of exponentials, base 2
+    float *picked;        // kStats, kKeep: [T] the target's logit
+    // kProb (prob also kKeep)
     const float *lse;     // [T], base 2
     const float *row_scale;  // [T], or NULL: 1 for every counted row
     void *prob;           // [T] rows of ldp
@@ -124,7 +129,7 @@ struct Args {
     float *bias_part;     // [tiles_n][ld of the piece]: sums over the rows of a tile, or NULL
     int ld_bias_part;
     void *bias_out;       // one tile holds all rows: the bias's gradient itself (times factor), or NULL
-    uint32_t *arrived;    // kStats: set to 0, for row_kernel
+    uint32_t *arrived;    // kStats, kKeep: set to 0, for row_kernel
     // kOut
     float *slice;         // [splits][N][M] float, or NULL: final
     void *out;            // [N] rows of the operands' type, ldo apart
@@ -140,6 +145,18 @@ constexpr float kProbScale = 32768.f;
 
 // For terms of a sum whose largest is 1: one instruction, good to a unit in the last place; what is below 2^-126 becomes 0.
 __device__ __forceinline__ float exp2_of(float x) { return __builtin_amdgcn_exp2f(x); }
+
+// All of 2^x's range; the few more instructions that takes only where a lane needs them.
+__device__ __forceinline__ void exp2_of_four(const float (&x)[4], float (&e)[4])
+{
+    if (__any(fminf(fminf(x[0], x[1]), fminf(x[2], x[3])) < -126.f)) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) e[r] = exp2f(x[r]);
+    } else {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) e[r] = exp2_of(x[r]);
+    }
+}
 
 // A launch's tile: the workgroups of one XCD (they are dealt out in turn) get neighbouring tiles, in strips of kStrip along m,
 // so that what they read at the same time fits its L2.
@@ -592,31 +609,99 @@ __device__ __forceinline__ void product_tile(const Args &g, const int block, cha
     float *fl = (float *)lds;
     // a logit, base 2
     auto logit = [&](int I, int j, int r) -> float { return fmaf(value(I, j, r), kLog2e, known.bias[m_in + m_of(I) + r]); };
-    if constexpr (KIND == kStats) {
-        if (block == 0 && threadIdx.x == 0) *g.arrived = 0;
+    constexpr int kRowsOut = WN * U::size, kThreads = WAVES * 64;  // rows that leave together: one j of every wave
+    auto n_of = [](int row, int j) { return (row / U::size * NT + j) * U::size + row % U::size; };
+    const int row_out = wn * U::size + lane % U::size;
+    // four neighbouring probabilities to their place among the rows that leave
+    auto put_prob = [&](int I, float (&p)[4]) {
+        typedef Gather<uint16_t, BM * NP> Out;
+        static_assert(KIND == kOut || kRowsOut * BM * NP * 2 <= kStagesBytes<P, BM, BN, STAGES>, "");
+        const int m = m_in + m_of(I);
+        if constexpr (NP == 1) {
+            *(s16x4 *)Out::at(lds, row_out, m) = round4<P>(f32x4{p[0], p[1], p[2], p[3]} * (P::half ? kProbScale : 1.f));
+        } else {
+            bf16_t planes[4][3];
 #pragma unroll
-        for (int j = 0; j < NT; ++j) {
+            for (int r = 0; r < 4; ++r) split_planes(p[r], planes[r]);
+#pragma unroll
+            for (int q = 0; q < NP; ++q) {
+                const Vec<bf16_t, 4> o{{planes[0][q], planes[1][q], planes[2][q], planes[3][q]}};
+                *(Vec<bf16_t, 4> *)Out::at(lds, row_out, (m >> 5) * 96 + q * 32 + (m & 31)) = o;
+            }
+        }
+    };
+    auto leave_prob = [&](int j) {
+        __syncthreads();
+        Gather<uint16_t, BM * NP>::template leave<kThreads>(lds, kRowsOut, (g.prob_words - m0) * NP, [&](int row) -> uint16_t * {
+            const int t = n0 + n_of(row, j);
+            return t < g.N ? (uint16_t *)g.prob + t * g.ldp + m0 * NP : nullptr;
+        });
+        __syncthreads();
+    };
+    if constexpr (KIND == kStats || KIND == kKeep) {
+        if (block == 0 && threadIdx.x == 0) *g.arrived = 0;
+        float tops[NT];
+        auto tops_of = [&](int j) {
             const int at = known.want[n_in + j * U::size] - m_in;  // where the target lies behind this lane's first word
-            float s[MG][4], top = -INFINITY;
+            float top = -INFINITY;
 #pragma unroll
             for (int I = 0; I < MG; ++I) {
+                float s[4];
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
-                    s[I][r] = logit(I, j, r);
-                    top = fmaxf(top, s[I][r]);  // what is no number shows in the sum
+                    s[r] = logit(I, j, r);
+                    top = fmaxf(top, s[r]);  // what is no number shows in the sum
                 }
                 if ((unsigned)(at - m_of(I)) < 4u)
 #pragma unroll
                     for (int r = 0; r < 4; ++r)
-                        if (at == m_of(I) + r) g.picked[n0 + n_in + j * U::size] = s[I][r];
+                        if (at == m_of(I) + r) g.picked[n0 + n_in + j * U::size] = s[r];
             }
-            float sum = 0.f;
-            // a column of nothing but -inf keeps a sum of 0
+            return top;
+        };
+        // exponentials relative to `top`, and their sum over this lane's words; a column of nothing but -inf keeps a sum of 0
+        auto sum_of = [&](int j, float top) {
             const float base = top == -INFINITY ? 0.f : top;
+            float sum = 0.f;
 #pragma unroll
-            for (int I = 0; I < MG; ++I)
+            for (int I = 0; I < MG; ++I) {
+                float x[4], e[4];
 #pragma unroll
-                for (int r = 0; r < 4; ++r) sum += exp2_of(s[I][r] - base);
+                for (int r = 0; r < 4; ++r) x[r] = logit(I, j, r) - base;
+                // a sum does not notice what the instruction by itself leaves out, what is kept has it
+                if constexpr (KIND == kKeep) exp2_of_four(x, e);
+                else
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) e[r] = exp2_of(x[r]);
+#pragma unroll
+                for (int r = 0; r < 4; ++r) sum += e[r];
+                if constexpr (KIND == kKeep) put_prob(I, e);
+            }
+            return sum;
+        };
+        // a place behind the rows on their way out, where other waves' results wait
+        float2 *const others = (float2 *)(lds + kStagesBytes<P, BM, BN, STAGES>) - WM * BN;
+        static_assert(KIND == kStats || kRowsOut * BM * NP * 2 + WM * BN * 8 <= kStagesBytes<P, BM, BN, STAGES>, "");
+        if constexpr (KIND == kKeep) {
+            // the tile's maximum first: what is kept is relative to it
+#pragma unroll
+            for (int j = 0; j < NT; ++j) {
+                tops[j] = tops_of(j);
+#pragma unroll
+                for (int o = U::size; o < 64; o <<= 1) tops[j] = fmaxf(tops[j], __shfl_xor(tops[j], o));
+                if (lane < U::size) others[wm * BN + (wn * NT + j) * U::size + lane].x = tops[j];
+            }
+            __syncthreads();
+#pragma unroll
+            for (int j = 0; j < NT; ++j)
+#pragma unroll
+                for (int w = 0; w < WM; ++w) tops[j] = fmaxf(tops[j], others[w * BN + n_in + j * U::size].x);
+            __syncthreads();
+        }
+#pragma unroll
+        for (int j = 0; j < NT; ++j) {
+            float top = KIND == kKeep ? tops[j] : tops_of(j);
+            float sum = sum_of(j, top);
 #pragma unroll
             for (int o = U::size; o < 64; o <<= 1) {
                 const float top2 = __shfl_xor(top, o), sum2 = __shfl_xor(sum, o);
@@ -624,33 +709,24 @@ __device__ __forceinline__ void product_tile(const Args &g, const int block, cha
                 sum = both == -INFINITY ? sum + sum2 : sum * exp2_of(top - both) + sum2 * exp2_of(top2 - both);
                 top = both;
             }
-            if (lane < U::size) {
-                const int c = (wn * NT + j) * U::size + lane;
-                fl[(wm * BN + c) * 2] = top;
-                fl[(wm * BN + c) * 2 + 1] = sum;
-            }
+            if (lane < U::size) others[wm * BN + (wn * NT + j) * U::size + lane] = float2{top, sum};
+            if constexpr (KIND == kKeep) leave_prob(j);
         }
         __syncthreads();
         for (int c = threadIdx.x; c < BN; c += WAVES * 64) {
             if (n0 + c >= g.N) continue;
-            float top = fl[c * 2], sum = fl[c * 2 + 1];
+            float top = others[c].x, sum = others[c].y;
 #pragma unroll
             for (int w = 1; w < WM; ++w) {
-                const float top2 = fl[(w * BN + c) * 2], sum2 = fl[(w * BN + c) * 2 + 1];
+                const float top2 = others[w * BN + c].x, sum2 = others[w * BN + c].y;
                 const float both = fmaxf(top, top2);
                 sum = both == -INFINITY ? sum + sum2 : sum * exp2_of(top - both) + sum2 * exp2_of(top2 - both);
                 top = both;
             }
-            float2 *to = (float2 *)g.stats + (int64_t)tm * g.N + n0 + c;
-            *to = float2{top, sum};
+            ((float2 *)g.stats)[(int64_t)tm * g.N + n0 + c] = float2{top, sum};
         }
     }
-    constexpr int kRowsOut = WN * U::size, kThreads = WAVES * 64;  // rows that leave together: one j of every wave
-    auto n_of = [](int row, int j) { return (row / U::size * NT + j) * U::size + row % U::size; };
-    const int row_out = wn * U::size + lane % U::size;
     if constexpr (KIND == kProb) {
-        typedef Gather<uint16_t, BM * NP> Out;
-        static_assert(kRowsOut * BM * NP * 2 <= kStagesBytes<P, BM, BN, STAGES>, "");
         float over_n[MG][4];  // sums over this lane's rows, for the bias
 #pragma unroll
         for (int I = 0; I < MG; ++I)
@@ -662,20 +738,10 @@ __device__ __forceinline__ void product_tile(const Args &g, const int block, cha
             const int at = known.want[n_in + j * U::size] - m_in;
 #pragma unroll
             for (int I = 0; I < MG; ++I) {
-                float x[4], p[4], least = INFINITY;
+                float x[4], p[4];
 #pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    x[r] = logit(I, j, r) - lse;
-                    least = fminf(least, x[r]);
-                }
-                // below 2^-126 the instruction by itself gives 0
-                if (__any(least < -126.f)) {
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) p[r] = exp2f(x[r]);
-                } else {
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) p[r] = exp2_of(x[r]);
-                }
+                for (int r = 0; r < 4; ++r) x[r] = logit(I, j, r) - lse;
+                exp2_of_four(x, p);
                 if ((unsigned)(at - m_of(I)) < 4u)
 #pragma unroll
                     for (int r = 0; r < 4; ++r) p[r] -= at == m_of(I) + r ? 1.f : 0.f;
@@ -683,28 +749,10 @@ __device__ __forceinline__ void product_tile(const Args &g, const int block, cha
                 for (int r = 0; r < 4; ++r) {
                     p[r] *= scale;
                     over_n[I][r] += p[r];
-                    if constexpr (P::half) p[r] *= kProbScale;
                 }
-                const int m = m_in + m_of(I);
-                if constexpr (NP == 1) {
-                    *(s16x4 *)Out::at(lds, row_out, m) = round4<P>(f32x4{p[0], p[1], p[2], p[3]});
-                } else {
-                    bf16_t planes[4][3];
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) split_planes(p[r], planes[r]);
-#pragma unroll
-                    for (int q = 0; q < NP; ++q) {
-                        const Vec<bf16_t, 4> o{{planes[0][q], planes[1][q], planes[2][q], planes[3][q]}};
-                        *(Vec<bf16_t, 4> *)Out::at(lds, row_out, (m >> 5) * 96 + q * 32 + (m & 31)) = o;
-                    }
-                }
+                put_prob(I, p);
             }
-            __syncthreads();
-            Out::template leave<kThreads>(lds, kRowsOut, (g.prob_words - m0) * NP, [&](int row) -> uint16_t * {
-                const int t = n0 + n_of(row, j);
-                return t < g.N ? (uint16_t *)g.prob + t * g.ldp + m0 * NP : nullptr;
-            });
-            __syncthreads();
+            leave_prob(j);
         }
         if (g.bias_part || g.bias_out) {
             typedef typename ElementOf<P>::type E;
@@ -776,7 +824,7 @@ __global__ __launch_bounds__(WM * WN * 64) void both_kernel(Args hidden, Args we
 }
 
 // Which product a launch is.
-enum { kLogitStats = 0, kLogitProb = 1, kHidden = 2, kWeight = 3 };
+enum { kLogitStats = 0, kLogitKeep = 1, kLogitProb = 2, kHidden = 3, kWeight = 4 };
 
 // Tile shapes, m x n, by their number in a launch.  For choosing among them: workgroups that a CU holds, and measured, in
 // microseconds, a step of the reduction while every CU has its fill, a step while none has more than one workgroup, and what a
@@ -811,6 +859,8 @@ int launch_tiled(int kind, Args &g, Args *other, hipStream_t st)
     const dim3 grid((unsigned)(blocks + more)), threads(WM * WN * 64);
     if (kind == kLogitStats) {
         hipLaunchKernelGGL((product_kernel<P, BM, BN, WM, WN, false, false, kStats, STAGES>), grid, threads, 0, st, g);
+    } else if (kind == kLogitKeep) {
+        hipLaunchKernelGGL((product_kernel<P, BM, BN, WM, WN, false, false, kKeep, STAGES>), grid, threads, 0, st, g);
     } else if (kind == kLogitProb) {
         hipLaunchKernelGGL((product_kernel<P, BM, BN, WM, WN, false, false, kProb, STAGES>), grid, threads, 0, st, g);
     } else if constexpr (GRADS) {

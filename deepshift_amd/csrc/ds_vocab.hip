@@ -3,9 +3,12 @@
 //   s[t][v] = h[t] . W[v] + b[v]      lse[t] = log sum_v exp s[t][v]      loss[t] = lse[t] - s[t][y_t]
 //   P[t][v] = g_t (exp(s[t][v] - lse[t]) - [v = y_t])      dh = P W      dW = P^T h      db = sum_t P[t]
 //
-// The logits are never stored: the forward pass keeps a maximum and a sum of exponentials per tile (T x V / 128 pairs), the
-// backward pass computes the logits of a piece of the vocabulary again, leaves that piece's P in a workspace, and forms both
-// gradients from it.  Four products of 2 T D V operations for a step, of which three are the formula's own.
+// The logits are never stored: the forward pass keeps a maximum and a sum of exponentials per tile (a pair for every 32 to 256
+// of them), the backward pass computes the logits of a piece of the vocabulary again, leaves that piece's P in a workspace of
+// a bounded size, and forms both gradients from it: four products of 2 T D V operations for a step, of which three are the
+// formula's own.  Where one piece is the whole vocabulary and loss and gradients are asked for in one call, the forward pass
+// leaves the exponentials, relative to their tiles' maxima, in that workspace, and a pass over them makes them P: three
+// products.
 #include "ds_vocab.h"
 
 namespace ds {
@@ -199,6 +202,102 @@ __global__ __launch_bounds__(1024) void row_scale_kernel(const float *__restrict
     if (threadIdx.x == 0) *factor = top;
 }
 
+// ---- exponentials to probabilities -----------------------------------------------------------------------------------
+
+// P[t][v] = scale_t (e[t][v] 2^(top[tile of v][t] - lse[t]) - [v = y_t]), in place; the target's own from its logit, in 32 bits.
+// A workgroup has 256 words of 64 rows, a thread 8 words of every eighth row; its rows' sums are the bias's gradient.
+struct Finish {
+    void *prob;
+    int64_t ldp;
+    int words, T, tile;    // words of a row, a multiple of 32; words a tile of the logits had
+    int64_t V, ignore;
+    const float2 *stats;   // [tiles][T]
+    const float *picked, *lse;
+    const void *target;
+    int wide;
+    float *bias_part;      // [workgroups along T][words], or NULL
+    void *bias_out;        // one workgroup has all rows: the gradient itself, of V words, or NULL
+    const float *factor[2];
+};
+constexpr int kFinishRows = 64;
+
+template <typename P>
+__global__ __launch_bounds__(256) void finish_kernel(Finish f)
+{
+    typedef typename ElementOf<P>::type E;
+    constexpr int NP = P::planes;
+    __shared__ float sums[8][256];
+    const int word = blockIdx.x * 256 + threadIdx.x % 32 * 8, part = threadIdx.x / 32;
+    float over_t[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) over_t[e] = 0.f;
+    if (word < f.words) {
+        const float2 *tops = f.stats + (int64_t)(word / f.tile) * f.T;
+        uint16_t *const column = (uint16_t *)f.prob + (NP == 1 ? word : (word >> 5) * 96 + (word & 31));
+#pragma unroll 4
+        for (int i = 0; i < kFinishRows / 8; ++i) {
+            const int t = blockIdx.y * kFinishRows + i * 8 + part;
+            if (t >= f.T) break;
+            const int64_t y = target_of(f.target, f.wide, t);
+            const float lse = f.lse[t], top = tops[t].x;
+            Vec<uint16_t, 8> *const at = (Vec<uint16_t, 8> *)(column + t * f.ldp);
+            Vec<uint16_t, 8> v[NP];
+#pragma unroll
+            for (int q = 0; q < NP; ++q) v[q] = at[q * 4];
+            // rows that do not count leave nothing; a target that is no word leaves no number
+            const float factor = y == f.ignore ? 0.f : y < 0 || y >= f.V ? NAN : exp2f(top - lse);
+            float p[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                if constexpr (NP == 3)
+                    p[e] = to_float(bf16_t{v[0].v[e]}) + (to_float(bf16_t{v[1].v[e]}) + to_float(bf16_t{v[2].v[e]}) * (1.f / 256)) * (1.f / 256);
+                else if constexpr (P::half)
+                    p[e] = to_float(f16_t{v[0].v[e]}) * (1.f / kProbScale);
+                else
+                    p[e] = to_float(bf16_t{v[0].v[e]});
+                p[e] = y == f.ignore ? 0.f : p[e] * factor;
+            }
+            if (y >= word && y < word + 8 && y != f.ignore) {
+                const float hot = exp2f(f.picked[t] - lse) - 1.f;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) p[e] = y == word + e ? hot : p[e];
+            }
+#pragma unroll
+            for (int e = 0; e < 8; ++e) over_t[e] += p[e];
+            if constexpr (NP == 3) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    bf16_t planes[3];
+                    split_planes(p[e], planes);
+#pragma unroll
+                    for (int q = 0; q < 3; ++q) v[q].v[e] = planes[q].bits;
+                }
+            } else {
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const f32x4 four = f32x4{p[h * 4], p[h * 4 + 1], p[h * 4 + 2], p[h * 4 + 3]} * (P::half ? kProbScale : 1.f);
+                    const s16x4 r = round4<P>(four);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) v[0].v[h * 4 + e] = (uint16_t)r[e];
+                }
+            }
+#pragma unroll
+            for (int q = 0; q < NP; ++q) at[q * 4] = v[q];
+        }
+    }
+    if (!f.bias_part && !f.bias_out) return;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) sums[part][threadIdx.x % 32 * 8 + e] = over_t[e];
+    __syncthreads();
+    const int v = blockIdx.x * 256 + threadIdx.x;
+    if (v >= f.V) return;
+    float s = 0.f;
+#pragma unroll
+    for (int w = 0; w < 8; ++w) s += sums[w][threadIdx.x];
+    if (f.bias_out) ((E *)f.bias_out)[v] = from_float<E>(s * factor_of(f.factor));
+    else f.bias_part[(int64_t)blockIdx.y * f.words + v] = s;
+}
+
 // ---- joins -------------------------------------------------------------------------------------------------------
 
 // The sums of a bias's tiles, to the gradient of 256 words.
@@ -298,6 +397,7 @@ struct Plan {
     int64_t ldd;          // and what their rows take
     int64_t piece, pieces;
     bool pack_h, pack_w;
+    bool keep;            // the loss's exponentials become the gradients' probabilities (run may decide against it)
     int tile_logits;
     Choice hidden, weight;
     int words;            // of a piece's probabilities, a multiple of 32,
@@ -333,6 +433,7 @@ Plan plan_of(const void *hidden, int64_t ldh, const void *weight, int64_t ldw, i
     p.piece = ((V + p.pieces - 1) / p.pieces + 255) / 256 * 256;
     if (p.piece > V) p.piece = V;
     p.pieces = (V + p.piece - 1) / p.piece;
+    p.keep = what == (kLoss | kGrad) && p.pieces == 1 && (T + kFinishRows - 1) / kFinishRows <= 65535;
     p.tile_logits = choose<P>(p.piece, T, D, kShapes, 1).tile;
     size_t at = 0;
     auto take = [&](size_t n) {
@@ -355,7 +456,9 @@ Plan plan_of(const void *hidden, int64_t ldh, const void *weight, int64_t ldw, i
         p.hidden = choose<P>(D, T, p.piece, kGradShapes<P>, 64);
         p.weight = choose<P>(D, p.piece, T, kGradShapes<P>, 64);
         p.prob = take((size_t)T * p.ldp * 2);
-        p.bias = take((size_t)((T + Shapes<P>::n[p.tile_logits] - 1) / Shapes<P>::n[p.tile_logits]) * p.words * 4);
+        // what a workgroup of either pass leaves of its rows
+        const int rows = p.keep && kFinishRows < Shapes<P>::n[p.tile_logits] ? kFinishRows : Shapes<P>::n[p.tile_logits];
+        p.bias = take((size_t)((T + rows - 1) / rows) * p.words * 4);
         size_t slices = 0;
         if (p.hidden.splits > 1 || p.pieces > 1) slices = (size_t)p.hidden.splits * T * D * 4;
         if (p.weight.splits > 1) {
@@ -451,7 +554,8 @@ int loss(const Call &c, const Plan &p, bool counted_only, Operands<P> &o, int re
         g.stats = (float *)(c.ws + p.stats) + (int64_t)tiles * c.T * 2;
         g.picked = (float *)(c.ws + p.picked);
         g.arrived = (uint32_t *)(c.ws + p.arrived);
-        DS_TRY(launch_product<P>(kLogitStats, p.tile_logits, g, nullptr, c.st));
+        g.prob = c.ws + p.prob, g.ldp = p.ldp, g.prob_words = p.words;
+        DS_TRY(launch_product<P>(p.keep ? kLogitKeep : kLogitStats, p.tile_logits, g, nullptr, c.st));
         tiles += g.tiles_m;
     }
     hipLaunchKernelGGL(row_kernel, dim3((unsigned)((c.T + kRowsJoined - 1) / kRowsJoined)), dim3(1024), 0, c.st, (const float2 *)(c.ws + p.stats),
@@ -482,17 +586,27 @@ int loss_grad(const Call &c, const Plan &p, Operands<P> &o, Grads r)
         int bias_tiles = 0;
         const Operand prob{c.ws + p.prob, p.ldp};
         if (c.T > 0) {
-            DS_TRY(o.prepare(c, p, true, v0, n));
-            Args g = logit_args<P>(c, p, v0, n, o);
-            g.lse = r.lse;
-            g.row_scale = r.row_grad ? (const float *)(c.ws + p.scale) : nullptr;
-            g.prob = c.ws + p.prob, g.ldp = p.ldp, g.prob_words = p.words;
-            g.factor[0] = r.grad, g.factor[1] = r.share;
-            if (r.dbias && c.T <= Shapes<P>::n[p.tile_logits]) g.bias_out = (E *)r.dbias + v0;
-            else if (r.dbias) g.bias_part = (float *)(c.ws + p.bias);
-            g.ld_bias_part = p.words;
-            DS_TRY(launch_product<P>(kLogitProb, p.tile_logits, g, nullptr, c.st));
-            bias_tiles = g.tiles_n;
+            const int rows = p.keep ? kFinishRows : Shapes<P>::n[p.tile_logits];
+            bias_tiles = (int)((c.T + rows - 1) / rows);
+            float *const bias_part = r.dbias && bias_tiles > 1 ? (float *)(c.ws + p.bias) : nullptr;
+            void *const bias_out = r.dbias && bias_tiles == 1 ? (E *)r.dbias + v0 : nullptr;
+            if (p.keep) {
+                const Finish f{c.ws + p.prob, p.ldp, p.words, (int)c.T, Shapes<P>::m[p.tile_logits], c.V, c.ignore,
+                               (const float2 *)(c.ws + p.stats), (const float *)(c.ws + p.picked), r.lse, c.target, c.wide,
+                               bias_part, bias_out, {r.grad, r.share}};
+                hipLaunchKernelGGL(finish_kernel<P>, dim3(ceil_div(p.words, 256), ceil_div((int)c.T, kFinishRows)), dim3(256), 0,
+                                   c.st, f);
+            } else {
+                DS_TRY(o.prepare(c, p, true, v0, n));
+                Args g = logit_args<P>(c, p, v0, n, o);
+                g.lse = r.lse;
+                g.row_scale = r.row_grad ? (const float *)(c.ws + p.scale) : nullptr;
+                g.prob = c.ws + p.prob, g.ldp = p.ldp, g.prob_words = p.words;
+                g.factor[0] = r.grad, g.factor[1] = r.share;
+                g.bias_out = bias_out, g.bias_part = bias_part;
+                g.ld_bias_part = p.words;
+                DS_TRY(launch_product<P>(kLogitProb, p.tile_logits, g, nullptr, c.st));
+            }
         }
         BiasJoin bias{(const float *)(c.ws + p.bias), p.words, bias_tiles, (int)n, r.dbias ? (E *)r.dbias + v0 : nullptr};
         bool bias_left = r.dbias && bias_tiles != 1;
@@ -556,7 +670,9 @@ struct Outputs {
 template <typename P>
 int run(const Call &c, int what, const Outputs &out)
 {
-    const Plan p = plan_of<P>(c.hidden, c.ldh, c.weight, c.ldw, c.T, c.D, c.V, what);
+    Plan p = plan_of<P>(c.hidden, c.ldh, c.weight, c.ldw, c.T, c.D, c.V, what);
+    // a bias's gradient sums what has not been rounded to 16 bits
+    p.keep = p.keep && (P::planes == 3 || !out.grads.dbias);
     if (!c.ws || c.ws_bytes < p.bytes || (uintptr_t)c.ws % 256) return DS_EWORKSPACE;
     Operands<P> o;
     if (what & kLoss) DS_TRY(loss<P>(c, p, what & kGrad, o, out.reduction, out.rows, out.lse, out.total));
