@@ -827,19 +827,19 @@ __global__ __launch_bounds__(WM * WN * 64) void both_kernel(Args hidden, Args we
 enum { kLogitStats = 0, kLogitKeep = 1, kLogitProb = 2, kHidden = 3, kWeight = 4 };
 
 // Tile shapes, m x n, by their number in a launch.  For choosing among them: workgroups that a CU holds, and measured, in
-// microseconds, a step of the reduction while every CU has its fill, a step while none has more than one workgroup, and what a
-// workgroup takes to begin and end.
+// microseconds, a step of the reduction while every CU has its fill, a step while none has more than one workgroup, what a
+// workgroup takes to begin and end, and what it takes besides where it leaves probabilities.
 constexpr int kShapes = 4;
 template <typename P> struct Shapes {
     static constexpr int m[kShapes] = {256, 128, 128, 64}, n[kShapes] = {256, 128, 64, 64}, resident[kShapes] = {1, 2, 2, 3};
     static constexpr float step_us[kShapes] = {1.6f, 1.05f, 0.8f, 0.5f}, alone_us[kShapes] = {1.0f, 0.6f, 0.5f, 0.3f};
-    static constexpr float ends_us[kShapes] = {7.f, 5.f, 4.f, 3.f};
+    static constexpr float ends_us[kShapes] = {6.f, 8.f, 6.f, 4.f}, prob_us[kShapes] = {5.f, 10.f, 6.f, 3.f};
 };
 template <> struct Shapes<Split> {
     // the last for logits only
     static constexpr int m[kShapes] = {256, 128, 64, 32}, n[kShapes] = {128, 128, 64, 32}, resident[kShapes] = {1, 1, 1, 2};
     static constexpr float step_us[kShapes] = {2.5f, 1.6f, 0.75f, 0.5f}, alone_us[kShapes] = {2.0f, 1.1f, 0.57f, 0.38f};
-    static constexpr float ends_us[kShapes] = {9.f, 5.f, 3.f, 3.f};
+    static constexpr float ends_us[kShapes] = {6.f, 5.f, 3.f, 3.f}, prob_us[kShapes] = {16.f, 8.f, 4.f, 3.f};
 };
 template <typename P> constexpr int kGradShapes = P::planes == 1 ? 4 : 3;
 

@@ -205,11 +205,12 @@ __global__ __launch_bounds__(1024) void row_scale_kernel(const float *__restrict
 // ---- exponentials to probabilities -----------------------------------------------------------------------------------
 
 // P[t][v] = scale_t (e[t][v] 2^(top[tile of v][t] - lse[t]) - [v = y_t]), in place; the target's own from its logit, in 32 bits.
-// A workgroup has 256 words of 64 rows, a thread 8 words of every eighth row; its rows' sums are the bias's gradient.
+// A workgroup has 256 words of some rows, a thread 8 words of every eighth of them; its rows' sums are the bias's gradient.
 struct Finish {
     void *prob;
     int64_t ldp;
     int words, T, tile;    // words of a row, a multiple of 32; words a tile of the logits had
+    int rows;              // of a workgroup, a multiple of 8
     int64_t V, ignore;
     const float2 *stats;   // [tiles][T]
     const float *picked, *lse;
@@ -219,7 +220,8 @@ struct Finish {
     void *bias_out;        // one workgroup has all rows: the gradient itself, of V words, or NULL
     const float *factor[2];
 };
-constexpr int kFinishRows = 64;
+// 64 rows, or 8 where that would leave CUs without work.
+inline int finish_rows(int64_t T, int64_t words) { return (T + 63) / 64 * ((words + 255) / 256) >= 2 * device_cus() ? 64 : 8; }
 
 template <typename P>
 __global__ __launch_bounds__(256) void finish_kernel(Finish f)
@@ -235,8 +237,8 @@ __global__ __launch_bounds__(256) void finish_kernel(Finish f)
         const float2 *tops = f.stats + (int64_t)(word / f.tile) * f.T;
         uint16_t *const column = (uint16_t *)f.prob + (NP == 1 ? word : (word >> 5) * 96 + (word & 31));
 #pragma unroll 4
-        for (int i = 0; i < kFinishRows / 8; ++i) {
-            const int t = blockIdx.y * kFinishRows + i * 8 + part;
+        for (int i = 0; i < f.rows; i += 8) {
+            const int t = blockIdx.y * f.rows + i + part;
             if (t >= f.T) break;
             const int64_t y = target_of(f.target, f.wide, t);
             const float lse = f.lse[t], top = tops[t].x;
@@ -363,7 +365,7 @@ constexpr size_t kPieceBytes = (size_t)1 << 30;  // of P, and of repacked weight
 // over 8000 words, bfloat16, 25, 16, 16 and 19 us from the largest tiles to the smallest.
 struct Choice { int tile, splits; };
 template <typename P>
-Choice choose(int64_t m, int64_t n, int64_t k, int shapes, int most_splits)
+Choice choose(int64_t m, int64_t n, int64_t k, int shapes, int most_splits, bool prob)
 {
     typedef Shapes<P> S;
     const int cus = device_cus(), tile_knob = g_tune.vocab_tile, split_knob = g_tune.vocab_split;
@@ -384,7 +386,7 @@ Choice choose(int64_t m, int64_t n, int64_t k, int shapes, int most_splits)
         for (int s = split_knob >= 1 ? most : 1; s <= most; s += 1 + s / 4) {
             const int64_t blocks = tiles * s;
             const double step = blocks <= cus ? S::alone_us[i] : S::step_us[i];
-            const double us = (double)((blocks + fill - 1) / fill) * ((double)((steps + s - 1) / s) * step + S::ends_us[i]) +
+            const double us = (double)((blocks + fill - 1) / fill) * ((double)((steps + s - 1) / s) * step + S::ends_us[i] + (prob ? S::prob_us[i] : 0)) +
                               (s > 1 ? 4 + (double)s * m * n * 4 / 3e6 : 0);
             if (us < shortest) shortest = us, best = Choice{i, s};
         }
@@ -433,8 +435,8 @@ Plan plan_of(const void *hidden, int64_t ldh, const void *weight, int64_t ldw, i
     p.piece = ((V + p.pieces - 1) / p.pieces + 255) / 256 * 256;
     if (p.piece > V) p.piece = V;
     p.pieces = (V + p.piece - 1) / p.piece;
-    p.keep = what == (kLoss | kGrad) && p.pieces == 1 && (T + kFinishRows - 1) / kFinishRows <= 65535;
-    p.tile_logits = choose<P>(p.piece, T, D, kShapes, 1).tile;
+    p.keep = what == (kLoss | kGrad) && p.pieces == 1 && T <= 65535 * 8;
+    p.tile_logits = choose<P>(p.piece, T, D, kShapes, 1, what & kGrad).tile;
     size_t at = 0;
     auto take = [&](size_t n) {
         const size_t was = at;
@@ -453,11 +455,12 @@ Plan plan_of(const void *hidden, int64_t ldh, const void *weight, int64_t ldw, i
     if (what & kGrad) {
         p.words = (int)((p.piece + 31) / 32 * 32);
         p.ldp = p.words * (int64_t)NP;
-        p.hidden = choose<P>(D, T, p.piece, kGradShapes<P>, 64);
-        p.weight = choose<P>(D, p.piece, T, kGradShapes<P>, 64);
+        p.hidden = choose<P>(D, T, p.piece, kGradShapes<P>, 64, false);
+        p.weight = choose<P>(D, p.piece, T, kGradShapes<P>, 64, false);
         p.prob = take((size_t)T * p.ldp * 2);
         // what a workgroup of either pass leaves of its rows
-        const int rows = p.keep && kFinishRows < Shapes<P>::n[p.tile_logits] ? kFinishRows : Shapes<P>::n[p.tile_logits];
+        const int tile_rows = Shapes<P>::n[p.tile_logits], kept_rows = finish_rows(T, p.words);
+        const int rows = p.keep && kept_rows < tile_rows ? kept_rows : tile_rows;
         p.bias = take((size_t)((T + rows - 1) / rows) * p.words * 4);
         size_t slices = 0;
         if (p.hidden.splits > 1 || p.pieces > 1) slices = (size_t)p.hidden.splits * T * D * 4;
@@ -586,15 +589,15 @@ int loss_grad(const Call &c, const Plan &p, Operands<P> &o, Grads r)
         int bias_tiles = 0;
         const Operand prob{c.ws + p.prob, p.ldp};
         if (c.T > 0) {
-            const int rows = p.keep ? kFinishRows : Shapes<P>::n[p.tile_logits];
+            const int rows = p.keep ? finish_rows(c.T, p.words) : Shapes<P>::n[p.tile_logits];
             bias_tiles = (int)((c.T + rows - 1) / rows);
             float *const bias_part = r.dbias && bias_tiles > 1 ? (float *)(c.ws + p.bias) : nullptr;
             void *const bias_out = r.dbias && bias_tiles == 1 ? (E *)r.dbias + v0 : nullptr;
             if (p.keep) {
-                const Finish f{c.ws + p.prob, p.ldp, p.words, (int)c.T, Shapes<P>::m[p.tile_logits], c.V, c.ignore,
+                const Finish f{c.ws + p.prob, p.ldp, p.words, (int)c.T, Shapes<P>::m[p.tile_logits], rows, c.V, c.ignore,
                                (const float2 *)(c.ws + p.stats), (const float *)(c.ws + p.picked), r.lse, c.target, c.wide,
                                bias_part, bias_out, {r.grad, r.share}};
-                hipLaunchKernelGGL(finish_kernel<P>, dim3(ceil_div(p.words, 256), ceil_div((int)c.T, kFinishRows)), dim3(256), 0,
+                hipLaunchKernelGGL(finish_kernel<P>, dim3(ceil_div(p.words, 256), ceil_div((int)c.T, rows)), dim3(256), 0,
                                    c.st, f);
             } else {
                 DS_TRY(o.prepare(c, p, true, v0, n));
