@@ -266,7 +266,7 @@ __global__ __launch_bounds__(64) void embed_sum_kernel(const E *__restrict__ g, 
                         Vec<E, N> o;
 #pragma unroll
                         for (int e = 0; e < N; ++e) o.v[e] = from_float<E>(acc[e] * scale);
-                        *(Vec<E, N> *)(dw + (int64_t)run * D + col) = o;
+                        store_streaming((Vec<E, N> *)(dw + (int64_t)run * D + col), o);
                     }
                 }
                 first = false;
@@ -288,7 +288,7 @@ __global__ __launch_bounds__(64) void embed_sum_kernel(const E *__restrict__ g, 
         Vec<E, N> o;
 #pragma unroll
         for (int e = 0; e < N; ++e) o.v[e] = from_float<E>(acc[e] * scale);
-        *(Vec<E, N> *)(dw + (int64_t)run * D + col) = o;
+        store_streaming((Vec<E, N> *)(dw + (int64_t)run * D + col), o);
     }
 }
 
@@ -359,7 +359,7 @@ __global__ __launch_bounds__(256) void embed_finish_kernel(const uint32_t *__res
         const int64_t last = min(u + kUnit, total) - 1;
         const uint32_t r1 = div_by((uint32_t)last, by_row);
         if (aligned && u + kUnit <= total && empty[r0] && (r1 == r0 || (r1 == r0 + 1 && empty[r1]))) {
-            *(uint4 *)(block + u) = uint4{0, 0, 0, 0};
+            store_streaming((Vec<uint32_t, 4> *)(block + u), Vec<uint32_t, 4>{});
         } else {
             for (int64_t i = u; i <= last; ++i)
                 if (empty[div_by((uint32_t)i, by_row)]) block[i] = from_float<E>(0.f);

@@ -173,10 +173,11 @@ __device__ __forceinline__ void tile_of(int id, int tiles_m, int tiles_n, int *t
 }
 
 // 16 bytes per lane from a buffer to LDS: lane l's go to `lds` + 16 l.  An offset past 2^31 fetches zeros.  No register is
-// written; whoever reads the LDS waits for the wave's own loads (vmcnt) and then for the workgroup's barrier.
+// written; whoever reads the LDS waits for the wave's own loads (vmcnt) and then for the workgroup's barrier.  The five wait
+// states cover M0, which needs one, and a descriptor that a vector instruction might have written just before.
 __device__ __forceinline__ void fetch(uint32_t offset, i32x4 buffer, uint32_t lds)
 {
-    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds"
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 3\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds"
                  :: "v"(offset), "s"(buffer), "s"(lds) : "memory");
 }
 constexpr uint32_t kNothing = 0x80000000u;

@@ -17,6 +17,7 @@ import math
 import torch
 import torch.nn as nn
 from torch.autograd import Function
+from torch.autograd.function import once_differentiable
 
 from . import _lib, kernels
 
@@ -24,6 +25,7 @@ __all__ = ["embedding", "embedding_grad", "linear_cross_entropy", "linear_cross_
            "clip_gradients_", "clip_grad_norm_", "ScaledEmbedding", "LinearCrossEntropy"]
 
 _TYPES = {torch.float32: _lib.DS_F32, torch.bfloat16: _lib.DS_BF16, torch.float16: _lib.DS_F16}
+_LONGEST_ROW = 2000000    # elements between rows that the products' 32-bit offsets reach
 _REDUCTIONS = {"none": _lib.DS_NONE, "sum": _lib.DS_SUM, "mean": _lib.DS_MEAN}
 
 
@@ -46,7 +48,7 @@ def _tokens_of(name, t, device):
 
 def _rows_of(t):
     """A matrix whose rows lie contiguously, and the distance between them."""
-    if t.stride(1) != 1 and t.size(1) > 1 or t.size(0) > 1 and t.stride(0) < t.size(1):
+    if t.stride(1) != 1 and t.size(1) > 1 or t.size(0) > 1 and not t.size(1) <= t.stride(0) <= _LONGEST_ROW:
         t = t.contiguous()
     return t, t.stride(0) if t.size(0) > 1 else t.size(1)
 
@@ -119,6 +121,7 @@ class _Embedding(Function):
         return _embed(ids, weight, scale)
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, grad):
         ids, = ctx.saved_tensors
         V, scale, padding_idx = ctx.of
@@ -238,6 +241,7 @@ class _LinearCrossEntropy(Function):
         return loss
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, grad):
         hidden, weight, target, bias, lse, share = ctx.saved_tensors
         with _on(hidden.device):
@@ -287,6 +291,7 @@ def _clip(grads, max_norm, out, scale):
     if len(outs) != len(grads):
         raise ValueError("%d tensors in out for %d gradients" % (len(outs), len(grads)))
     device = grads[0].device
+    targets_of = outs
     codes = to = _types_of("gradient", grads, device)
     back = ()
     if out is not None:
@@ -318,6 +323,12 @@ def _clip(grads, max_norm, out, scale):
         if scale:
             for o, copy in back:
                 o.copy_(copy)
+    if scale:
+        # autograd hears of what was written behind its back
+        try:
+            torch.autograd.graph.increment_version(targets_of)
+        except RuntimeError:   # inference tensors keep no count
+            torch.autograd.graph.increment_version([t for t in targets_of if not t.is_inference()])
     return norm
 
 

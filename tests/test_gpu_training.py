@@ -503,6 +503,36 @@ def test_clipping_layouts():
     torch.testing.assert_close(a, b, rtol=2.0 ** -21, atol=0)
 
 
+def test_autograd_hears_of_clipped_tensors_and_refuses_second_derivatives():
+    g = _gen(53)
+    a, b = _rand(g, 30), _rand(g, 30)
+    before = a._version, b._version
+    training.clip_gradients_([a], 0.1)
+    training.clip_gradients_([a], 0.1, out=[b])
+    training.gradient_norm([a, b])
+    assert a._version == before[0] + 1 and b._version == before[1] + 1
+    with torch.inference_mode():
+        c = torch.ones(4, device=DEV)
+        assert training.clip_gradients_([c], 1.0).item() == 2.0 and c[0] < 0.6
+    h, w = _rand(g, 5, 8).requires_grad_(), _rand(g, 6, 8).requires_grad_()
+    y = torch.arange(5, device=DEV)
+    for loss, of in ((training.linear_cross_entropy(h, w, y), h), (training.embedding(y, w).square().sum(), w)):
+        first, = torch.autograd.grad(loss, of, create_graph=True)
+        with pytest.raises(RuntimeError):
+            torch.autograd.grad(first.sum(), of)
+
+
+def test_rows_far_apart():
+    g = _gen(54)
+    h, w, b, y = _head(3, 16, 20, torch.bfloat16, True, g)
+    far = torch.zeros(3 * 2100000, dtype=torch.bfloat16, device=DEV).view(3, 2100000)
+    far[:, 8:24] = h
+    want = training.linear_cross_entropy_grad(h, w, y, b)
+    got = training.linear_cross_entropy_grad(far[:, 8:24], w, y, b)
+    assert all(torch.equal(x, z) for x, z in zip(got, want))
+    assert torch.equal(training.embedding(torch.tensor([2, 0], device=DEV), far[:, 8:24]), h[[2, 0]])
+
+
 def test_clip_grad_norm_of_parameters():
     torch.manual_seed(1)
     m = torch.nn.Sequential(modules.LinearShift(20, 30), torch.nn.ReLU(), modules.LinearShift(30, 5)).to(DEV)
