@@ -108,70 +108,98 @@ __device__ __forceinline__ void write_total(double loss, double rows, int mean, 
     total[1] = (float)share;
 }
 
+// A maximum and a sum of exponentials relative to it, joined with another such pair.
+__device__ __forceinline__ void join_pair(float &top, float &sum, float top2, float sum2)
+{
+    const float both = fmaxf(top, top2);
+    sum = both == -INFINITY ? sum + sum2 : sum * exp2_of(top - both) + sum2 * exp2_of(top2 - both);
+    top = both;
+}
+
+// Where the losses of rows go, and what they come from.
+struct Rows {
+    const float2 *stats;   // [tiles][T]
+    const float *picked;
+    int tiles, T;
+    const void *target;
+    int wide;
+    int64_t V, ignore;
+    float *lse, *loss;
+    int reduction;
+    Share *shares;
+    uint32_t *arrived;
+    float *total;
+};
+
+__device__ __forceinline__ float log_of_sum(float top, float sum) { return sum == 0.f ? -INFINITY : top + log2f(sum); }
+
+__device__ __forceinline__ float loss_of(const Rows &r, int t, int64_t y, float lse)
+{
+    return y == r.ignore ? 0.f : y < 0 || y >= r.V ? NAN : (lse - r.picked[t]) * kLn2;
+}
+
+// A workgroup's part in the total: its wave's sums of losses and of counted rows, `group` of `groups`.  The one that ends last
+// adds up all of them, in order.
+__device__ __forceinline__ void add_to_total(const Rows &r, double loss, double counted, int group, int groups)
+{
+    const int lane = threadIdx.x & 63;
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) loss += __shfl_xor(loss, o), counted += __shfl_xor(counted, o);
+    if (groups == 1) {
+        if (lane == 0) write_total(loss, counted, r.reduction == DS_MEAN, r.total);
+        return;
+    }
+    uint32_t before = 0;
+    if (lane == 0) {
+        r.shares[group] = Share{loss, counted};
+        before = __hip_atomic_fetch_add(r.arrived, 1u, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT);
+    }
+    if ((int)__builtin_amdgcn_readfirstlane(before) != groups - 1) return;
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "agent");
+    loss = counted = 0;
+    for (int i = lane; i < groups; i += 64) loss += r.shares[i].loss, counted += r.shares[i].rows;
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) loss += __shfl_xor(loss, o), counted += __shfl_xor(counted, o);
+    if (lane == 0) write_total(loss, counted, r.reduction == DS_MEAN, r.total);
+}
+
 // Joins the tiles' maxima and sums: a workgroup has kRowsJoined rows, each of its waves a sixteenth of the tiles and each
-// quarter of a wave a quarter of those.  The workgroup that ends last adds up all of them, in order.
+// quarter of a wave a quarter of those.
 constexpr int kRowsJoined = 16;
 
-__global__ __launch_bounds__(1024) void row_kernel(const float2 *__restrict__ stats, const float *__restrict__ picked, int tiles,
-                                                   int T, const void *__restrict__ target, int wide, int64_t V, int64_t ignore,
-                                                   float *__restrict__ lse, float *__restrict__ loss, int reduction, Share *shares,
-                                                   uint32_t *arrived, float *__restrict__ total)
+__global__ __launch_bounds__(1024) void row_kernel(Rows r)
 {
     __shared__ float tops[64][kRowsJoined], sums[64][kRowsJoined];
     const int row = threadIdx.x % kRowsJoined, part = threadIdx.x / kRowsJoined, t = blockIdx.x * kRowsJoined + row;
     float top = -INFINITY, sum = 0.f;
-    auto join = [&](float top2, float sum2) {
-        const float both = fmaxf(top, top2);
-        sum = both == -INFINITY ? sum + sum2 : sum * exp2_of(top - both) + sum2 * exp2_of(top2 - both);
-        top = both;
-    };
-    if (t < T) {
+    if (t < r.T) {
         constexpr int kAhead = 4;
-        for (int i = part; i < tiles; i += 64 * kAhead) {
+        for (int i = part; i < r.tiles; i += 64 * kAhead) {
             float2 s[kAhead];
 #pragma unroll
             for (int j = 0; j < kAhead; ++j)
-                s[j] = i + j * 64 < tiles ? stats[(int64_t)(i + j * 64) * T + t] : float2{-INFINITY, 0.f};
+                s[j] = i + j * 64 < r.tiles ? r.stats[(int64_t)(i + j * 64) * r.T + t] : float2{-INFINITY, 0.f};
 #pragma unroll
-            for (int j = 0; j < kAhead; ++j) join(s[j].x, s[j].y);
+            for (int j = 0; j < kAhead; ++j) join_pair(top, sum, s[j].x, s[j].y);
         }
     }
     tops[part][row] = top, sums[part][row] = sum;
     __syncthreads();
     if (threadIdx.x >= 64) return;
     // the quarters of a wave join 16 parts each, then each other
-    for (int i = part + 4; i < 64; i += 4) join(tops[i][row], sums[i][row]);
+    for (int i = part + 4; i < 64; i += 4) join_pair(top, sum, tops[i][row], sums[i][row]);
 #pragma unroll
-    for (int o = 16; o < 64; o <<= 1) join(__shfl_xor(top, o), __shfl_xor(sum, o));
+    for (int o = 16; o < 64; o <<= 1) join_pair(top, sum, __shfl_xor(top, o), __shfl_xor(sum, o));
     double mine = 0, counts = 0;
-    if (t < T && part == 0) {
-        const float all = sum == 0.f ? -INFINITY : top + log2f(sum);
-        lse[t] = all;
-        const int64_t y = target_of(target, wide, t);
-        const float l = y == ignore ? 0.f : y < 0 || y >= V ? NAN : (all - picked[t]) * kLn2;
-        loss[t] = l;
-        mine = l, counts = y != ignore;
+    if (t < r.T && part == 0) {
+        const float lse = log_of_sum(top, sum);
+        const int64_t y = target_of(r.target, r.wide, t);
+        r.lse[t] = lse;
+        const float l = loss_of(r, t, y, lse);
+        r.loss[t] = l;
+        mine = l, counts = y != r.ignore;
     }
-    if (!reduction) return;
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) mine += __shfl_xor(mine, o), counts += __shfl_xor(counts, o);
-    const int lane = threadIdx.x;
-    if (gridDim.x == 1) {
-        if (lane == 0) write_total(mine, counts, reduction == DS_MEAN, total);
-        return;
-    }
-    uint32_t before = 0;
-    if (lane == 0) {
-        shares[blockIdx.x] = Share{mine, counts};
-        before = __hip_atomic_fetch_add(arrived, 1u, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT);
-    }
-    if (__builtin_amdgcn_readfirstlane(before) != gridDim.x - 1) return;
-    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "agent");
-    mine = counts = 0;
-    for (unsigned i = lane; i < gridDim.x; i += 64) mine += shares[i].loss, counts += shares[i].rows;
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) mine += __shfl_xor(mine, o), counts += __shfl_xor(counts, o);
-    if (lane == 0) write_total(mine, counts, reduction == DS_MEAN, total);
+    if (r.reduction) add_to_total(r, mine, counts, blockIdx.x, gridDim.x);
 }
 
 __global__ void no_rows_kernel(int mean, float *total) { write_total(0, 0, mean, total); }
@@ -209,13 +237,9 @@ __global__ __launch_bounds__(1024) void row_scale_kernel(const float *__restrict
 struct Finish {
     void *prob;
     int64_t ldp;
-    int words, T, tile;    // words of a row, a multiple of 32; words a tile of the logits had
+    int words, tile;       // words of a row, a multiple of 32; words a tile of the logits had
     int rows;              // of a workgroup, a multiple of 8
-    int64_t V, ignore;
-    const float2 *stats;   // [tiles][T]
-    const float *picked, *lse;
-    const void *target;
-    int wide;
+    Rows of;
     float *bias_part;      // [workgroups along T][words], or NULL
     void *bias_out;        // one workgroup has all rows: the gradient itself, of V words, or NULL
     const float *factor[2];
@@ -223,76 +247,125 @@ struct Finish {
 // 64 rows, or 8 where that would leave CUs without work.
 inline int finish_rows(int64_t T, int64_t words) { return (T + 63) / 64 * ((words + 255) / 256) >= 2 * device_cus() ? 64 : 8; }
 
-template <typename P>
+// A row's sum, joined by half a wave, a lane every 32nd tile.
+__device__ __forceinline__ float lse_of_row(const Rows &r, int t, int lane)
+{
+    float top = -INFINITY, sum = 0.f;
+    for (int k = lane; k < r.tiles; k += 32) {
+        const float2 s = r.stats[(int64_t)k * r.T + t];
+        join_pair(top, sum, s.x, s.y);
+    }
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) join_pair(top, sum, __shfl_xor(top, o), __shfl_xor(sum, o));
+    return log_of_sum(top, sum);
+}
+
+// JOIN: every workgroup joins its rows' sums for itself, and one more (the last along the rows) all of them, for the losses;
+// else they are in of.lse.
+template <typename P, bool JOIN>
 __global__ __launch_bounds__(256) void finish_kernel(Finish f)
 {
     typedef typename ElementOf<P>::type E;
     constexpr int NP = P::planes;
     __shared__ float sums[8][256];
-    const int word = blockIdx.x * 256 + threadIdx.x % 32 * 8, part = threadIdx.x / 32;
+    const Rows &r = f.of;
+    const int lane = threadIdx.x % 32, part = threadIdx.x / 32, word = blockIdx.x * 256 + lane * 8;
+    if (JOIN && blockIdx.y == gridDim.y - 1) {
+        if (blockIdx.x > 0) return;
+        // a wave has 64 rows at a time, a quarter of the tiles
+        double loss = 0, counted = 0;
+        const int wave = threadIdx.x / 64, row = threadIdx.x % 64;
+        float2 *const parts = (float2 *)sums;  // [4][64]
+        for (int t0 = 0; t0 < r.T; t0 += 64) {
+            const int t = t0 + row;
+            float top = -INFINITY, sum = 0.f;
+            constexpr int kAhead = 8;
+            for (int k = wave; k < r.tiles; k += 4 * kAhead) {
+                float2 s[kAhead];
+#pragma unroll
+                for (int j = 0; j < kAhead; ++j)
+                    s[j] = t < r.T && k + j * 4 < r.tiles ? r.stats[(int64_t)(k + j * 4) * r.T + t] : float2{-INFINITY, 0.f};
+#pragma unroll
+                for (int j = 0; j < kAhead; ++j) join_pair(top, sum, s[j].x, s[j].y);
+            }
+            parts[wave * 64 + row] = float2{top, sum};
+            __syncthreads();
+            if (wave == 0 && t < r.T) {
+#pragma unroll
+                for (int w = 1; w < 4; ++w) join_pair(top, sum, parts[w * 64 + row].x, parts[w * 64 + row].y);
+                const float lse = log_of_sum(top, sum);
+                const int64_t y = target_of(r.target, r.wide, t);
+                const float l = loss_of(r, t, y, lse);
+                r.lse[t] = lse, r.loss[t] = l;
+                loss += l, counted += y != r.ignore;
+            }
+            __syncthreads();
+        }
+        if (wave == 0 && r.reduction) add_to_total(r, loss, counted, 0, 1);
+        return;
+    }
     float over_t[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) over_t[e] = 0.f;
-    if (word < f.words) {
-        const float2 *tops = f.stats + (int64_t)(word / f.tile) * f.T;
-        uint16_t *const column = (uint16_t *)f.prob + (NP == 1 ? word : (word >> 5) * 96 + (word & 31));
-#pragma unroll 4
-        for (int i = 0; i < f.rows; i += 8) {
-            const int t = blockIdx.y * f.rows + i + part;
-            if (t >= f.T) break;
-            const int64_t y = target_of(f.target, f.wide, t);
-            const float lse = f.lse[t], top = tops[t].x;
-            Vec<uint16_t, 8> *const at = (Vec<uint16_t, 8> *)(column + t * f.ldp);
-            Vec<uint16_t, 8> v[NP];
+    const float2 *tops = r.stats + (int64_t)(word < f.words ? word / f.tile : 0) * r.T;
+    uint16_t *const column = (uint16_t *)f.prob + (NP == 1 ? word : (word >> 5) * 96 + (word & 31));
+#pragma unroll JOIN ? 1 : 4
+    for (int i = 0; i < f.rows; i += 8) {
+        const int t = blockIdx.y * f.rows + i + part;
+        if (t >= r.T) break;
+        const int64_t y = target_of(r.target, r.wide, t);
+        const float lse = JOIN ? lse_of_row(r, t, lane) : r.lse[t];
+        if (word >= f.words) continue;
+        Vec<uint16_t, 8> *const at = (Vec<uint16_t, 8> *)(column + t * f.ldp);
+        Vec<uint16_t, 8> v[NP];
 #pragma unroll
-            for (int q = 0; q < NP; ++q) v[q] = at[q * 4];
-            // rows that do not count leave nothing; a target that is no word leaves no number
-            const float factor = y == f.ignore ? 0.f : y < 0 || y >= f.V ? NAN : exp2f(top - lse);
-            float p[8];
+        for (int q = 0; q < NP; ++q) v[q] = at[q * 4];
+        // rows that do not count leave nothing; a target that is no word leaves no number
+        const float factor = y == r.ignore ? 0.f : y < 0 || y >= r.V ? NAN : exp2f(tops[t].x - lse);
+        float p[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            if constexpr (NP == 3)
+                p[e] = to_float(bf16_t{v[0].v[e]}) + (to_float(bf16_t{v[1].v[e]}) + to_float(bf16_t{v[2].v[e]}) * (1.f / 256)) * (1.f / 256);
+            else if constexpr (P::half)
+                p[e] = to_float(f16_t{v[0].v[e]}) * (1.f / kProbScale);
+            else
+                p[e] = to_float(bf16_t{v[0].v[e]});
+            p[e] = y == r.ignore ? 0.f : p[e] * factor;
+        }
+        if (y >= word && y < word + 8 && y != r.ignore) {
+            const float hot = exp2f(r.picked[t] - lse) - 1.f;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) p[e] = y == word + e ? hot : p[e];
+        }
+#pragma unroll
+        for (int e = 0; e < 8; ++e) over_t[e] += p[e];
+        if constexpr (NP == 3) {
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
-                if constexpr (NP == 3)
-                    p[e] = to_float(bf16_t{v[0].v[e]}) + (to_float(bf16_t{v[1].v[e]}) + to_float(bf16_t{v[2].v[e]}) * (1.f / 256)) * (1.f / 256);
-                else if constexpr (P::half)
-                    p[e] = to_float(f16_t{v[0].v[e]}) * (1.f / kProbScale);
-                else
-                    p[e] = to_float(bf16_t{v[0].v[e]});
-                p[e] = y == f.ignore ? 0.f : p[e] * factor;
+                bf16_t planes[3];
+                split_planes(p[e], planes);
+#pragma unroll
+                for (int q = 0; q < 3; ++q) v[q].v[e] = planes[q].bits;
             }
-            if (y >= word && y < word + 8 && y != f.ignore) {
-                const float hot = exp2f(f.picked[t] - lse) - 1.f;
+        } else {
 #pragma unroll
-                for (int e = 0; e < 8; ++e) p[e] = y == word + e ? hot : p[e];
+            for (int h = 0; h < 2; ++h) {
+                const f32x4 four = f32x4{p[h * 4], p[h * 4 + 1], p[h * 4 + 2], p[h * 4 + 3]} * (P::half ? kProbScale : 1.f);
+                const s16x4 rounded = round4<P>(four);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) v[0].v[h * 4 + e] = (uint16_t)rounded[e];
             }
-#pragma unroll
-            for (int e = 0; e < 8; ++e) over_t[e] += p[e];
-            if constexpr (NP == 3) {
-#pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    bf16_t planes[3];
-                    split_planes(p[e], planes);
-#pragma unroll
-                    for (int q = 0; q < 3; ++q) v[q].v[e] = planes[q].bits;
-                }
-            } else {
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    const f32x4 four = f32x4{p[h * 4], p[h * 4 + 1], p[h * 4 + 2], p[h * 4 + 3]} * (P::half ? kProbScale : 1.f);
-                    const s16x4 r = round4<P>(four);
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) v[0].v[h * 4 + e] = (uint16_t)r[e];
-                }
-            }
-#pragma unroll
-            for (int q = 0; q < NP; ++q) at[q * 4] = v[q];
         }
+#pragma unroll
+        for (int q = 0; q < NP; ++q) at[q * 4] = v[q];
     }
     if (!f.bias_part && !f.bias_out) return;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) sums[part][threadIdx.x % 32 * 8 + e] = over_t[e];
+    for (int e = 0; e < 8; ++e) sums[part][lane * 8 + e] = over_t[e];
     __syncthreads();
     const int v = blockIdx.x * 256 + threadIdx.x;
-    if (v >= f.V) return;
+    if (v >= r.V) return;
     float s = 0.f;
 #pragma unroll
     for (int w = 0; w < 8; ++w) s += sums[w][threadIdx.x];
@@ -542,8 +615,13 @@ Args logit_args(const Call &c, const Plan &p, int64_t v0, int64_t n, const Opera
     return g;
 }
 
+// Whether finish_kernel joins the rows' sums: each of its workgroups does it for its own rows, and one for all, which pays
+// while there are few of both (64 tokens, 1000 words, float32: 41 us a step instead of 44).
+inline bool joined_later(const Plan &p, int64_t T, int tiles) { return p.keep && T <= 128 && tiles <= 64; }
+
 template <typename P>
-int loss(const Call &c, const Plan &p, bool counted_only, Operands<P> &o, int reduction, float *rows, float *lse, float *total)
+int loss(const Call &c, const Plan &p, bool counted_only, Operands<P> &o, int reduction, float *rows, float *lse, float *total,
+         Rows *of)
 {
     if (c.T == 0) {
         if (reduction) hipLaunchKernelGGL(no_rows_kernel, dim3(1), dim3(1), 0, c.st, reduction == DS_MEAN, total);
@@ -561,9 +639,10 @@ int loss(const Call &c, const Plan &p, bool counted_only, Operands<P> &o, int re
         DS_TRY(launch_product<P>(p.keep ? kLogitKeep : kLogitStats, p.tile_logits, g, nullptr, c.st));
         tiles += g.tiles_m;
     }
-    hipLaunchKernelGGL(row_kernel, dim3((unsigned)((c.T + kRowsJoined - 1) / kRowsJoined)), dim3(1024), 0, c.st, (const float2 *)(c.ws + p.stats),
-                       (const float *)(c.ws + p.picked), tiles, (int)c.T, c.target, c.wide, c.V, c.ignore, lse, rows, reduction,
-                       (Share *)(c.ws + p.shares), (uint32_t *)(c.ws + p.arrived), total);
+    *of = Rows{(const float2 *)(c.ws + p.stats), (const float *)(c.ws + p.picked), tiles, (int)c.T, c.target, c.wide, c.V, c.ignore,
+               lse, rows, reduction, (Share *)(c.ws + p.shares), (uint32_t *)(c.ws + p.arrived), total};
+    if (!joined_later(p, c.T, tiles))
+        hipLaunchKernelGGL(row_kernel, dim3((unsigned)((c.T + kRowsJoined - 1) / kRowsJoined)), dim3(1024), 0, c.st, *of);
     return launch_status();
 }
 
@@ -574,7 +653,7 @@ struct Grads {
 };
 
 template <typename P>
-int loss_grad(const Call &c, const Plan &p, Operands<P> &o, Grads r)
+int loss_grad(const Call &c, const Plan &p, Operands<P> &o, const Rows &of, Grads r)
 {
     typedef typename ElementOf<P>::type E;
     if (c.T > 0 && r.row_grad) {
@@ -587,18 +666,23 @@ int loss_grad(const Call &c, const Plan &p, Operands<P> &o, Grads r)
         const int64_t n = c.V - v0 < p.piece ? c.V - v0 : p.piece;
         const bool first = v0 == 0, last = v0 + n == c.V;
         int bias_tiles = 0;
+        bool bias_left = r.dbias != nullptr;
         const Operand prob{c.ws + p.prob, p.ldp};
         if (c.T > 0) {
             const int rows = p.keep ? finish_rows(c.T, p.words) : Shapes<P>::n[p.tile_logits];
             bias_tiles = (int)((c.T + rows - 1) / rows);
-            float *const bias_part = r.dbias && bias_tiles > 1 ? (float *)(c.ws + p.bias) : nullptr;
-            void *const bias_out = r.dbias && bias_tiles == 1 ? (E *)r.dbias + v0 : nullptr;
+            // the sums of one workgroup are the gradient, but for the share that a launch which joins the rows only finds
+            bias_left = r.dbias && (bias_tiles > 1 || joined_later(p, c.T, of.tiles));
+            float *const bias_part = bias_left ? (float *)(c.ws + p.bias) : nullptr;
+            void *const bias_out = r.dbias && !bias_left ? (E *)r.dbias + v0 : nullptr;
             if (p.keep) {
-                const Finish f{c.ws + p.prob, p.ldp, p.words, (int)c.T, Shapes<P>::m[p.tile_logits], rows, c.V, c.ignore,
-                               (const float2 *)(c.ws + p.stats), (const float *)(c.ws + p.picked), r.lse, c.target, c.wide,
+                const Finish f{c.ws + p.prob, p.ldp, p.words, Shapes<P>::m[p.tile_logits], rows, of,
                                bias_part, bias_out, {r.grad, r.share}};
-                hipLaunchKernelGGL(finish_kernel<P>, dim3(ceil_div(p.words, 256), ceil_div((int)c.T, rows)), dim3(256), 0,
-                                   c.st, f);
+                const unsigned along = ceil_div(p.words, 256), down = ceil_div((int)c.T, rows);
+                if (joined_later(p, c.T, of.tiles))
+                    hipLaunchKernelGGL((finish_kernel<P, true>), dim3(along, down + 1), dim3(256), 0, c.st, f);
+                else
+                    hipLaunchKernelGGL((finish_kernel<P, false>), dim3(along, down), dim3(256), 0, c.st, f);
             } else {
                 DS_TRY(o.prepare(c, p, true, v0, n));
                 Args g = logit_args<P>(c, p, v0, n, o);
@@ -612,7 +696,6 @@ int loss_grad(const Call &c, const Plan &p, Operands<P> &o, Grads r)
             }
         }
         BiasJoin bias{(const float *)(c.ws + p.bias), p.words, bias_tiles, (int)n, r.dbias ? (E *)r.dbias + v0 : nullptr};
-        bool bias_left = r.dbias && bias_tiles != 1;
         // by itself, or along with the join of a product
         auto join_bias_alone = [&] {
             if (bias_left)
@@ -678,8 +761,9 @@ int run(const Call &c, int what, const Outputs &out)
     p.keep = p.keep && (P::planes == 3 || !out.grads.dbias);
     if (!c.ws || c.ws_bytes < p.bytes || (uintptr_t)c.ws % 256) return DS_EWORKSPACE;
     Operands<P> o;
-    if (what & kLoss) DS_TRY(loss<P>(c, p, what & kGrad, o, out.reduction, out.rows, out.lse, out.total));
-    if (what & kGrad) DS_TRY(loss_grad<P>(c, p, o, out.grads));
+    Rows of{};
+    if (what & kLoss) DS_TRY(loss<P>(c, p, what & kGrad, o, out.reduction, out.rows, out.lse, out.total, &of));
+    if (what & kGrad) DS_TRY(loss_grad<P>(c, p, o, of, out.grads));
     return DS_OK;
 }
 
