@@ -76,7 +76,7 @@ __device__ __forceinline__ uint32_t key_at(const void *ids, int wide, int64_t i,
 // Up to kRankMost tokens: the place of a token is the number of tokens with a smaller word, or the same word and an earlier
 // position.  Every workgroup holds all words in LDS and places 64 tokens, its 16 waves each compare them with a sixteenth:
 // T * T comparisons, two instructions each.
-constexpr int kRankMost = 16384;  // a multiple of 64
+constexpr int kRankMost = 8192;  // a multiple of 64
 
 __global__ __launch_bounds__(1024) void embed_rank_kernel(const void *__restrict__ ids, int wide, int T, int64_t V,
                                                           int64_t padding, uint32_t *__restrict__ keys,
