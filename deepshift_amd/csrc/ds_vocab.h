@@ -12,6 +12,14 @@
 // products above 2^-24 of it (x0 y0, x0 y1, x1 y0, x1 y1, x0 y2, x2 y0): six times the bf16 work at a rate of bf16, where the
 // float32 matrix instructions take sixteen times the time of bf16.  The planes' factors keep all 24 bits of the smallest
 // values, which planes without them would lose below 2^-110.
+//
+// What bounds them: large ones the power of the chip, which holds the clock at 1.5 to 1.6 GHz while the matrix cores are busy 70
+// to 85 % of the cycles (a library's products of the same sizes run at the same rate).  A piece of 8192 tokens x 65536 words x
+// 4096 features, bfloat16, 4.4 TFLOP each: scores 3.2 ms, probabilities 3.5 ms, hidden gradients 3.15 ms, weight gradients 3.2 ms,
+// 1.25 to 1.4 PFLOP/s; plain library products of these operands take 3.24, 3.43 and 3.92 ms.  float32, 2048 tokens x 32768 words x
+// 1024 features, 137 GFLOP each: 0.68 to 0.85 ms, 1.0 to 1.2 PFLOP/s of plane products, 160 to 200 TFLOP/s of float32, where the
+// library reaches 154.  Few tokens are bound by reading the weights (37 tokens, 50021 words x 2048, bfloat16: 205 MB in 41 us),
+// small problems by what one CU can fetch at a time, some 50 bytes per ns from other XCDs' results: hence the small tiles.
 #pragma once
 #include "ds_train.h"
 #include <type_traits>
@@ -41,6 +49,8 @@ struct Unit {
     static constexpr int size = P::unit, groups = size == 32 ? 4 : 1, depth = size == 32 ? 16 : 32;
     typedef typename std::conditional<size == 32, f32x16, f32x4>::type Result;
 
+    template <typename V> __device__ static __forceinline__ V as(s16x8 v) { return __builtin_bit_cast(V, v); }
+
     // first m of a lane, and of its groups behind that
     __device__ static __forceinline__ int lane_m(int lane) { return lane / size * 4; }
     static constexpr int group_m(int q) { return q * 8; }
@@ -49,14 +59,14 @@ struct Unit {
     {
         if constexpr (size == 32) {
             if constexpr (P::half)
-                return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+                return __builtin_amdgcn_mfma_f32_32x32x16_f16(as<f16x8>(a), as<f16x8>(b), c, 0, 0, 0);
             else
-                return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+                return __builtin_amdgcn_mfma_f32_32x32x16_bf16(as<bf16x8>(a), as<bf16x8>(b), c, 0, 0, 0);
         } else {
             if constexpr (P::half)
-                return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+                return __builtin_amdgcn_mfma_f32_16x16x32_f16(as<f16x8>(a), as<f16x8>(b), c, 0, 0, 0);
             else
-                return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+                return __builtin_amdgcn_mfma_f32_16x16x32_bf16(as<bf16x8>(a), as<bf16x8>(b), c, 0, 0, 0);
         }
     }
 };
@@ -391,6 +401,11 @@ __device__ __forceinline__ int spread_sums(float (&v)[ALL], int lane)
 }
 
 // One tile of a product, by a whole workgroup; `block` counts the product's workgroups.
+//
+// Operands go from memory to LDS without registers, two stages and more ahead; a wave holds up to 128 x 64 results.  Fragments
+// are read and stages fetched between rows of products, a few each: with all of them behind the barrier the matrix cores were
+// busy 55 % of the cycles instead of 70 to 85 (4.0 instead of 3.2 ms for the scores above).  32 x 32 instructions take half as
+// many issues as 16 x 16 ones at the same rate; float32 keeps the smaller ones, whose partial sums of the planes fit.
 template <typename P, int BM, int BN, int WM, int WN, bool A_ACROSS, bool B_ACROSS, int KIND, int STAGES>
 __device__ __forceinline__ void product_tile(const Args &g, const int block, char *lds)
 {
@@ -594,7 +609,9 @@ __device__ __forceinline__ void product_tile(const Args &g, const int block, cha
                 for (int f = 0; f < kFetches; ++f) {
                     if (f * kTurns / kFetches != t) continue;
                     if (f < NP * TA::mine) ta.one(a_at, k_left, to, wave, f / TA::mine, f % TA::mine);
-                    else tb.one(b_at, k_left, to + NP * TA::bytes, wave, (f - NP * TA::mine) / TB::mine, (f - NP * TA::mine) % TB::mine);
+                    else
+                        tb.one(b_at, k_left, to + NP * TA::bytes, wave, (f - NP * TA::mine) / TB::mine,
+                               (f - NP * TA::mine) % TB::mine);
                 }
 #pragma unroll
                 for (int n = 0; n < kReads; ++n) {
@@ -634,7 +651,10 @@ __device__ __forceinline__ void product_tile(const Args &g, const int block, cha
     constexpr int kRowsOut = WN * U::size, kThreads = WAVES * 64;  // rows that leave together: one j of every wave
     auto n_of = [](int row, int j) { return (row / U::size * NT + j) * U::size + row % U::size; };
     const int row_out = wn * U::size + lane % U::size;
-    // four neighbouring probabilities to their place among the rows that leave
+    // Four neighbouring probabilities to their place among the rows that leave.  Here they are rounded to the operands' type (of
+    // float32 nothing is lost in three planes): the second product's other operand has no more bits either, each rounding is
+    // independent of the others, and against 64 bits the gradients are as far off, 0.0017 of their norm in bfloat16, as a
+    // float32 computation rounded once at its end.
     auto put_prob = [&](int I, float (&p)[4]) {
         typedef Gather<uint16_t, BM * NP> Out;
         static_assert(KIND == kOut || kRowsOut * BM * NP * 2 <= kStagesBytes<P, BM, BN, STAGES>, "");
