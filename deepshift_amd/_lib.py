@@ -4,10 +4,13 @@ The library is the only compute path of this package: if it is missing, loading 
 there is no CPU or eager-PyTorch fallback.
 """
 import ctypes
+import importlib.machinery
+import importlib.util
 import os
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "lib", "libdeepshift_hip.so")
+NATIVE_PATH = os.path.join(_HERE, "lib", "ds_torch.so")
 
 DS_Q_ROUND_TO_FIXED = 0
 DS_Q_CAST = 1
@@ -137,6 +140,7 @@ SIGNATURES = {
 }
 
 _LIB = None
+_NATIVE = None
 
 
 class DeepShiftError(RuntimeError):
@@ -162,6 +166,22 @@ def lib():
             fn.argtypes = argtypes
         _LIB = handle
     return _LIB
+
+
+def native():
+    """``lib/ds_torch.so``: entry points that take torch's tensors themselves, for calls that the interpreter would hold up."""
+    global _NATIVE
+    if _NATIVE is None:
+        import torch  # noqa: F401  (the module is linked with it and with the library)
+        lib()
+        if not os.path.exists(NATIVE_PATH):
+            raise RuntimeError("%s is missing: build it with `python -m deepshift_amd.build` (there is no fallback path)"
+                               % NATIVE_PATH)
+        loader = importlib.machinery.ExtensionFileLoader("ds_torch", NATIVE_PATH)
+        module = importlib.util.module_from_spec(importlib.util.spec_from_loader("ds_torch", loader))
+        loader.exec_module(module)
+        _NATIVE = module
+    return _NATIVE
 
 
 def call(name, *args):

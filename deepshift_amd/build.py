@@ -1,4 +1,5 @@
-"""Builds ``lib/libdeepshift_hip.so`` (gfx950) from ``csrc/*.hip`` with hipcc.
+"""Builds ``lib/libdeepshift_hip.so`` (gfx950) from ``csrc/*.hip`` with hipcc, and ``lib/ds_torch.so``, the module that hands it
+torch's tensors, from ``csrc/host/*.cpp``.
 
     python -m deepshift_amd.build            # rebuild unconditionally
     python -m deepshift_amd.build --if-stale # only when a source is newer than the library
@@ -8,11 +9,14 @@ import glob
 import os
 import subprocess
 import sys
+import sysconfig
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(_HERE, "csrc")
 LIB_DIR = os.path.join(_HERE, "lib")
 LIB_PATH = os.path.join(LIB_DIR, "libdeepshift_hip.so")
+NATIVE_PATH = os.path.join(LIB_DIR, "ds_torch.so")
+INCLUDE = os.path.join(_HERE, "..", "include")
 ARCH = "gfx950"
 
 # -packed-fp32-ops is switched off: this library has no business with packed fp32 and the
@@ -35,11 +39,21 @@ def sources():
     return sorted(glob.glob(os.path.join(CSRC, "*.hip")) + glob.glob(os.path.join(CSRC, "*.cpp")))
 
 
+def native_sources():
+    """Units that are built against torch, on the host only."""
+    return sorted(glob.glob(os.path.join(CSRC, "host", "*.cpp")))
+
+
+def _torch_dir():
+    import torch
+    return os.path.dirname(torch.__file__)
+
+
 def is_stale():
-    if not os.path.exists(LIB_PATH):
+    if not os.path.exists(LIB_PATH) or not os.path.exists(NATIVE_PATH):
         return True
-    built = os.path.getmtime(LIB_PATH)
-    deps = sources() + glob.glob(os.path.join(CSRC, "*.h")) + glob.glob(os.path.join(CSRC, "*.py")) + \
+    built = min(os.path.getmtime(LIB_PATH), os.path.getmtime(NATIVE_PATH))
+    deps = sources() + native_sources() + glob.glob(os.path.join(CSRC, "*.h")) + glob.glob(os.path.join(CSRC, "*.py")) + \
         glob.glob(os.path.join(_HERE, "..", "include", "*.h"))
     return any(os.path.getmtime(p) > built for p in deps)
 
@@ -59,13 +73,18 @@ def build(verbose=True, incremental=False):
     os.makedirs(obj_dir, exist_ok=True)
     procs = []
     objs = []
-    for src in sources():
+    native = native_sources()
+    native_objs = []
+    for src in sources() + native:
         obj = os.path.join(obj_dir, os.path.splitext(os.path.basename(src))[0] + ".o")
-        objs.append(obj)
+        (native_objs if src in native else objs).append(obj)
         if incremental and os.path.exists(obj) and \
                 all(os.path.getmtime(d) <= os.path.getmtime(obj) for d in _deps(src)):
             continue
-        if src.endswith(".cpp"):
+        if src in native:
+            cmd = [hipcc(), "-O2", "-std=c++17", "-fPIC", "-fvisibility=hidden", "-Wall", "-I", INCLUDE, "-I",
+                   os.path.join(_torch_dir(), "include"), "-I", sysconfig.get_paths()["include"], "-c", src, "-o", obj]
+        elif src.endswith(".cpp"):
             cmd = [hipcc(), "-O3", "-std=c++17", "-fPIC", "-fvisibility=hidden", "-pthread", "-Wall",
                    "-c", src, "-o", obj]
         else:
@@ -85,10 +104,13 @@ def build(verbose=True, incremental=False):
             failed = True
     if failed:
         raise RuntimeError("hipcc failed")
-    cmd = [hipcc(), "--offload-arch=" + ARCH, "-shared", "-fPIC", "-pthread", "-o", LIB_PATH] + objs
-    if verbose:
-        print(" ".join(cmd), flush=True)
-    subprocess.check_call(cmd)
+    link = [hipcc(), "--offload-arch=" + ARCH, "-shared", "-fPIC", "-pthread", "-o"]
+    against = ["-L", LIB_DIR, "-ldeepshift_hip", "-L", os.path.join(_torch_dir(), "lib"), "-ltorch_python", "-ltorch_cpu", "-lc10",
+               "-Wl,-rpath,$ORIGIN"]
+    for cmd in (link + [LIB_PATH] + objs, link + [NATIVE_PATH] + native_objs + against):
+        if verbose:
+            print(" ".join(cmd), flush=True)
+        subprocess.check_call(cmd)
     return LIB_PATH
 
 

@@ -1,0 +1,219 @@
+// The host's side of calls whose kernels are over sooner than a few dozen steps of the Python interpreter: the lookup of an
+// embedding and the clipping of gradients.  Checks, allocations and the call of the library, on torch's tensors as they are.
+//
+// Bound by the launches themselves (2.7 us each) and torch's allocations (0.8 us).
+#include <Python.h>
+#include <torch/csrc/autograd/python_variable.h>
+#include <ATen/core/Tensor.h>
+#include <ATen/ops/empty.h>
+#include <algorithm>
+#include <string>
+#include <vector>
+#include "deepshift_hip.h"
+
+namespace {
+
+// What a caller hears: the type of a Python exception and its text.
+struct Refusal {
+    PyObject *type;
+    std::string text;
+};
+
+struct Failure {
+    const char *entry;
+    int status;
+};
+
+int type_code(const at::Tensor &t)
+{
+    switch (t.scalar_type()) {
+    case at::kFloat: return DS_F32;
+    case at::kBFloat16: return DS_BF16;
+    case at::kHalf: return DS_F16;
+    default: return -1;
+    }
+}
+
+std::string text_of(const char *what) { return what; }
+std::string text_of(const std::string &what) { return what; }
+std::string text_of(at::IntArrayRef sizes)
+{
+    std::string s = "[";
+    for (size_t i = 0; i < sizes.size(); ++i) s += (i ? ", " : "") + std::to_string(sizes[i]);
+    return s + "]";
+}
+template <typename... T> [[noreturn]] void refuse(PyObject *type, const T &...parts) { throw Refusal{type, (text_of(parts) + ...)}; }
+
+const at::Tensor &tensor(const char *name, PyObject *o)
+{
+    if (!THPVariable_Check(o)) refuse(PyExc_TypeError, name, " must be a tensor, is ", Py_TYPE(o)->tp_name);
+    return THPVariable_Unpack(o);
+}
+
+int checked_type(const char *name, const at::Tensor &t)
+{
+    const int code = type_code(t);
+    if (code < 0) refuse(PyExc_TypeError, name, " must be float32, bfloat16 or float16, is ", c10::toString(t.scalar_type()));
+    if (!t.is_cuda()) refuse(PyExc_ValueError, name, " must be a GPU tensor");
+    return code;
+}
+
+int64_t integer(PyObject *o)
+{
+    const long long v = PyLong_AsLongLong(o);
+    if (v == -1 && PyErr_Occurred()) throw Refusal{nullptr, ""};
+    return v;
+}
+double number(PyObject *o)
+{
+    const double v = PyFloat_AsDouble(o);
+    if (v == -1.0 && PyErr_Occurred()) throw Refusal{nullptr, ""};
+    return v;
+}
+void *stream(PyObject *o)
+{
+    void *p = PyLong_AsVoidPtr(o);
+    if (!p && PyErr_Occurred()) throw Refusal{nullptr, ""};
+    return p;
+}
+
+void expect(const char *entry, int status)
+{
+    if (status != DS_OK) throw Failure{entry, status};
+}
+
+// Runs an entry point; whatever is thrown in it becomes a Python exception.
+template <typename F> PyObject *guarded(Py_ssize_t got, Py_ssize_t wanted, F &&body)
+{
+    try {
+        if (got != wanted) refuse(PyExc_TypeError, std::to_string(wanted), " arguments expected");
+        return body();
+    } catch (const Refusal &r) {
+        if (r.type) PyErr_SetString(r.type, r.text.c_str());
+    } catch (const Failure &f) {
+        PyObject *module = PyImport_ImportModule("deepshift_amd._lib");
+        PyObject *type = module ? PyObject_GetAttrString(module, "DeepShiftError") : nullptr;
+        PyObject *args = type ? Py_BuildValue("(sis)", f.entry, f.status, ds_status_string(f.status)) : nullptr;
+        if (args) PyErr_SetObject(type, args);
+        Py_XDECREF(args);
+        Py_XDECREF(type);
+        Py_XDECREF(module);
+    } catch (const std::exception &e) {
+        PyErr_SetString(PyExc_RuntimeError, e.what());
+    }
+    return nullptr;
+}
+
+// embed(ids, weight, scale, stream): scale * weight[ids]
+PyObject *embed(PyObject *, PyObject *const *args, Py_ssize_t count)
+{
+    return guarded(count, 4, [&] {
+        at::Tensor ids = tensor("ids", args[0]), weight = tensor("weight", args[1]);
+        const int code = checked_type("weight", weight);
+        if (weight.dim() != 2) refuse(PyExc_ValueError, "weight must be [V, D], is ", weight.sizes());
+        if (ids.scalar_type() != at::kLong && ids.scalar_type() != at::kInt)
+            refuse(PyExc_TypeError, "ids must be int64 or int32, is ", c10::toString(ids.scalar_type()));
+        if (ids.device() != weight.device())
+            refuse(PyExc_ValueError, "ids must be on ", weight.device().str(), ", is on ", ids.device().str());
+        if (!ids.is_contiguous()) ids = ids.contiguous();
+        // rows that lie contiguously, any distance apart
+        const int64_t V = weight.size(0), D = weight.size(1);
+        if ((D > 1 && weight.stride(1) != 1) || (V > 1 && weight.stride(0) < D)) weight = weight.contiguous();
+        c10::SmallVector<int64_t, 6> shape(ids.sizes().begin(), ids.sizes().end());
+        shape.push_back(D);
+        at::Tensor out = at::empty(shape, weight.options().requires_grad(false));
+        expect("ds_embed", ds_embed(ids.const_data_ptr(), (int)ids.element_size(), weight.const_data_ptr(),
+                                    V > 1 ? weight.stride(0) : D, out.mutable_data_ptr(), ids.numel(), V, D,
+                                    (float)number(args[2]), code, stream(args[3])));
+        return THPVariable_Wrap(std::move(out));
+    });
+}
+
+// The tensors of a list: types, one device; false where one is not contiguous.
+bool look_at(const char *name, PyObject *list, c10::Device device, std::vector<const at::Tensor *> &tensors, std::vector<int> &types)
+{
+    bool contiguous = true;
+    const Py_ssize_t n = PyList_GET_SIZE(list);
+    tensors.reserve(n), types.reserve(n);
+    for (Py_ssize_t i = 0; i < n; ++i) {
+        const at::Tensor &t = tensor(name, PyList_GET_ITEM(list, i));
+        types.push_back(checked_type(name, t));
+        if (t.device() != device) refuse(PyExc_ValueError, "every ", name, " must be on one device, the first gradient's");
+        contiguous = t.is_contiguous() && contiguous;
+        tensors.push_back(&t);
+    }
+    return contiguous;
+}
+
+// clip(grads, outs or None, max_norm, scale, any_order, stream): the norm; None, with nothing done, where a tensor is not
+// contiguous and the caller has not said by `any_order` that all elements fill stretches of memory in the same order.
+PyObject *clip(PyObject *, PyObject *const *args, Py_ssize_t count)
+{
+    return guarded(count, 6, [&]() -> PyObject * {
+        PyObject *const grads = args[0], *const outs = args[1];
+        if (!PyList_Check(grads) || (outs != Py_None && !PyList_Check(outs))) refuse(PyExc_TypeError, "lists of tensors expected");
+        const Py_ssize_t n = PyList_GET_SIZE(grads);
+        if (n == 0 || n > 0x7fffffff) refuse(PyExc_ValueError, n ? "too many gradients" : "no gradients given");
+        const bool elsewhere = outs != Py_None, scale = integer(args[3]) != 0, any_order = integer(args[4]) != 0;
+        if (elsewhere && PyList_GET_SIZE(outs) != n)
+            refuse(PyExc_ValueError, std::to_string(PyList_GET_SIZE(outs)), " tensors in out for ", std::to_string(n), " gradients");
+        std::vector<const at::Tensor *> from, to_elsewhere;
+        std::vector<int> from_types, to_types;
+        const c10::Device device = tensor("gradient", PyList_GET_ITEM(grads, 0)).device();
+        bool contiguous = look_at("gradient", grads, device, from, from_types);
+        if (elsewhere) {
+            contiguous = look_at("out", outs, device, to_elsewhere, to_types) && contiguous;
+            for (Py_ssize_t i = 0; i < n; ++i)
+                if (from[i]->sizes() != to_elsewhere[i]->sizes())
+                    refuse(PyExc_ValueError, "out ", std::to_string(i), " must be ", from[i]->sizes(), ", is ",
+                           to_elsewhere[i]->sizes());
+        }
+        if (!contiguous && !any_order) Py_RETURN_NONE;
+        const std::vector<const at::Tensor *> &to = elsewhere ? to_elsewhere : from;
+
+        std::vector<ds_tensor> table(n);
+        for (Py_ssize_t i = 0; i < n; ++i) {
+            ds_tensor &x = table[i];
+            x.src = from[i]->const_data_ptr();
+            x.dst = scale ? to[i]->mutable_data_ptr() : const_cast<void *>(x.src);
+            // (a tensor that shares its memory until it is written to has moved)
+            if (scale && !elsewhere) x.src = x.dst;
+            x.n = from[i]->numel();
+            x.src_type = from_types[i], x.dst_type = elsewhere ? to_types[i] : from_types[i];
+        }
+        if (scale) {
+            // nothing may be written twice
+            std::vector<std::pair<uintptr_t, uintptr_t>> written;
+            written.reserve(n);
+            for (Py_ssize_t i = 0; i < n; ++i)
+                if (table[i].n) written.emplace_back((uintptr_t)table[i].dst, (uintptr_t)table[i].dst + to[i]->nbytes());
+            if (!std::is_sorted(written.begin(), written.end())) std::sort(written.begin(), written.end());
+            for (size_t i = 1; i < written.size(); ++i)
+                if (written[i].first < written[i - 1].second)
+                    refuse(PyExc_ValueError, "a tensor is given twice, or shares memory with another one that is written");
+        }
+        const auto options = at::TensorOptions().device(device);
+        at::Tensor norm = at::empty({}, options.dtype(at::kFloat));
+        const size_t bytes = ds_clip_workspace_bytes((int)n);
+        at::Tensor workspace = at::empty({(int64_t)bytes}, options.dtype(at::kByte));
+        expect("ds_clip", ds_clip(table.data(), (int)n, (float)number(args[2]), scale, (float *)norm.mutable_data_ptr(),
+                                  workspace.mutable_data_ptr(), bytes, stream(args[5])));
+        // autograd hears of what was written behind its back; inference tensors keep no count
+        if (scale)
+            for (const at::Tensor *t : to)
+                if (!t->is_inference()) t->unsafeGetTensorImpl()->bump_version();
+        return THPVariable_Wrap(std::move(norm));
+    });
+}
+
+PyMethodDef methods[] = {
+    {"embed", (PyCFunction)(void (*)(void))embed, METH_FASTCALL, "embed(ids, weight, scale, stream) -> scale * weight[ids]"},
+    {"clip", (PyCFunction)(void (*)(void))clip, METH_FASTCALL,
+     "clip(grads, outs or None, max_norm, scale, any_order, stream) -> norm, or None"},
+    {nullptr, nullptr, 0, nullptr},
+};
+PyModuleDef module = {PyModuleDef_HEAD_INIT, "ds_torch", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
+
+}  // namespace
+
+PyMODINIT_FUNC PyInit_ds_torch(void) { return PyModule_Create(&module); }

@@ -9,9 +9,7 @@ and a call repeats bit for bit.  There is no CPU path: a CPU tensor raises.
 Functions whose names end in ``_grad`` return gradients directly; ``embedding`` and ``linear_cross_entropy`` also take part
 in autograd.
 """
-import array
 import contextlib
-import ctypes
 import math
 
 import torch
@@ -63,23 +61,18 @@ def _on(device):
     return torch.cuda.device(device)
 
 
+def _stream_of(device):
+    return _lib.stream_handle(device) if device.type == "cuda" else 0   # a CPU tensor is refused further down
+
+
 # ---------------------------------------------------------------------------------------------
 # embedding
 # ---------------------------------------------------------------------------------------------
 
 def _embed(ids, weight, scale):
-    code = _type_of("weight", weight)
-    if weight.dim() != 2:
-        raise ValueError("weight must be [V, D]")
     device = weight.device
-    ids = _tokens_of("ids", ids, device)
-    weight, ld = _rows_of(weight)
-    V, D = weight.shape
-    out = torch.empty(ids.shape + (D,), dtype=weight.dtype, device=device)
     with _on(device):
-        _lib.call("ds_embed", ids.data_ptr(), ids.element_size(), weight.data_ptr(), ld, out.data_ptr(), ids.numel(), V, D,
-                  scale, code, _lib.stream_handle(device))
-    return out
+        return _lib.native().embed(ids, weight, scale, _stream_of(device))
 
 
 def embedding_grad(ids, grad, num_embeddings, scale=1.0, padding_idx=None):
@@ -285,63 +278,19 @@ def _flat(t):
 
 def _clip(grads, max_norm, out, scale):
     grads = [grads] if isinstance(grads, torch.Tensor) else list(grads)
-    if not grads:
-        raise ValueError("no gradients given")
-    outs = grads if out is None else ([out] if isinstance(out, torch.Tensor) else list(out))
-    if len(outs) != len(grads):
-        raise ValueError("%d tensors in out for %d gradients" % (len(outs), len(grads)))
-    device = grads[0].device
-    targets_of = outs
-    codes = to = _types_of("gradient", grads, device)
-    back = ()
-    if out is not None:
-        to = _types_of("out", outs, device)
-        for i, (t, o) in enumerate(zip(grads, outs)):
-            if o.shape != t.shape:
-                raise ValueError("out %d must be %s, is %s" % (i, list(t.shape), list(o.shape)))
-    if not (all([t.is_contiguous() for t in grads]) and (out is None or all([t.is_contiguous() for t in outs]))):
-        grads, outs, back = _stretches(grads, outs)
-    # one ds_tensor each: two addresses, the number of elements, two types
-    sources = [t.data_ptr() for t in grads]
-    targets = sources if outs is grads else [t.data_ptr() for t in outs]
-    sizes = [t.numel() for t in grads]
-    if scale and len(set(targets)) != len(targets):
-        if len({p for p, n in zip(targets, sizes) if n}) != sum([n > 0 for n in sizes]):
-            raise ValueError("a tensor is given twice")
-    table = array.array("q", [0]) * (4 * len(grads))
-    table[0::4], table[1::4], table[2::4] = array.array("q", sources), array.array("q", targets), array.array("q", sizes)
-    if len(set(codes)) == len(set(to)) == 1:
-        table[3::4] = array.array("q", [codes[0] | to[0] << 32]) * len(grads)
-    else:
-        table[3::4] = array.array("q", [a | b << 32 for a, b in zip(codes, to)])
-    norm = torch.empty((), dtype=torch.float32, device=device)
+    outs = None if out is None else [out] if isinstance(out, torch.Tensor) else list(out)
+    device = grads[0].device if grads and isinstance(grads[0], torch.Tensor) else torch.device("cpu")
     with _on(device):
-        nbytes = _lib.lib().ds_clip_workspace_bytes(len(grads))
-        ws = kernels._workspace(nbytes, device)
-        _lib.call("ds_clip", ctypes.cast(table.buffer_info()[0], _lib._tp), len(grads), max_norm, int(scale), norm.data_ptr(),
-                  ws.data_ptr(), nbytes, _lib.stream_handle(device))
-        if scale:
-            for o, copy in back:
-                o.copy_(copy)
-    if scale:
-        # autograd hears of what was written behind its back
-        try:
-            torch.autograd.graph.increment_version(targets_of)
-        except RuntimeError:   # inference tensors keep no count
-            torch.autograd.graph.increment_version([t for t in targets_of if not t.is_inference()])
+        clip = _lib.native().clip
+        norm = clip(grads, outs, max_norm, scale, False, _stream_of(device))
+        if norm is None:
+            # not all contiguous; what is written to copies is copied back, on the same stream
+            sources, targets, back = _stretches(grads, grads if outs is None else outs)
+            norm = clip(sources, None if targets is sources else targets, max_norm, scale, True, _stream_of(device))
+            if scale:
+                for o, copy in back:
+                    o.copy_(copy)
     return norm
-
-
-def _types_of(name, tensors, device):
-    try:
-        codes = [_TYPES[t.dtype] for t in tensors]
-    except KeyError as e:
-        raise TypeError("%ss must be float32, bfloat16 or float16, one is %s" % (name, e.args[0])) from None
-    index = device.index if device.type == "cuda" else None
-    for at in {t.get_device() for t in tensors}:
-        if index is None or at != index:
-            raise ValueError("every %s must be a GPU tensor, all on one device" % name)
-    return codes
 
 
 def _stretches(grads, outs):
@@ -371,7 +320,8 @@ def gradient_norm(grads):
 def clip_gradients_(grads, max_norm, out=None):
     """Scales ``grads`` by ``min(1, max_norm / (norm + 1e-6))`` and returns ``norm``, their global 2-norm before it (a float32
     scalar on the device; nothing waits for it).  The results go to ``out``, a tensor for each gradient, of any of the three
-    types, or in place.  Types may differ from tensor to tensor.  A norm that is infinite or NaN scales by 0 or NaN."""
+    types, or in place.  Types may differ from tensor to tensor.  A norm that is infinite or NaN scales by 0 or NaN.  Tensors
+    that are written may not overlap."""
     max_norm = float(max_norm)
     if not max_norm >= 0:
         raise ValueError("max_norm must not be negative")

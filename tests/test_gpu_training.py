@@ -638,6 +638,13 @@ def test_refusals():
         training.clip_gradients_([f.double()], 1.0)
     with pytest.raises(ValueError):
         training.clip_gradients_([f.cpu()], 1.0)
+    # what is written may not overlap, what is only read may
+    run = torch.ones(10, device=DEV)
+    for grads, out in (([run[:6], run[4:]], None), ([run[:4], run[4:8]], [run[:4], run[3:7]]), ([f, None], None)):
+        with pytest.raises((ValueError, TypeError)):
+            training.clip_gradients_(grads, 1.0, out=out)
+    assert training.gradient_norm([run[:6], run[4:]]).item() == pytest.approx(12 ** 0.5, rel=2.0 ** -22)
+    training.clip_gradients_([run[4:8], run[:0], run[:4], run[8:]], 1.0)
     L = _lib.lib()
     ws = torch.empty(1 << 20, dtype=torch.uint8, device=DEV)
     assert L.ds_embed(ids.data_ptr(), 3, w.data_ptr(), 8, f.data_ptr(), 4, 5, 8, 1.0, 0, None) == -1

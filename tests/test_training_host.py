@@ -24,6 +24,21 @@ def test_cpu_tensors_are_refused():
         training.ScaledEmbedding(5, 4, padding_idx=5)
 
 
+def test_native_entry_points_refuse():
+    native = _lib.native()
+    x = torch.zeros(3)
+    for args in ((), (1, 2, 3), (x, x, 1.0, 0, 0)):
+        with pytest.raises(TypeError):
+            native.embed(*args)
+    for args in ((), (x, None, 1.0, 1, 0, 0), ([x, 1], None, 1.0, 1, 0, 0), ([1], None, 1.0, 1, 0, 0), ([x], x, 1.0, 1, 0, 0)):
+        with pytest.raises((TypeError, ValueError)):
+            native.clip(*args)
+    with pytest.raises(ValueError, match="no gradients"):
+        native.clip([], None, 1.0, 1, 0, 0)
+    with pytest.raises(ValueError, match="1 tensors in out for 2"):
+        native.clip([x, x], [x], 1.0, 1, 0, 0)
+
+
 def test_modules_hold_what_their_counterparts_hold():
     e = training.ScaledEmbedding(7, 3, scale=4.0, padding_idx=-1)
     assert e.weight.shape == (7, 3) and e.padding_idx == 6 and (e.weight[6] == 0).all()
