@@ -68,6 +68,44 @@ int launch_embed(const void *ids, int wide, const void *w, void *out, int64_t T,
 
 // ---- tokens sorted by word ------------------------------------------------------------------------------------
 
+// The gradient begins as zeros, which words without tokens keep: most of a large table's.  Sorting takes a few CUs, so the
+// launches that sort fill it besides, and rows with tokens are written once more.  (Filling empty rows alone, which took a
+// launch that searches for them behind the sums: 8192 tokens of 2048 bfloat16 features, 131072 words, 139 us instead of 125; 500
+// of 4096 float32 features 424, now 373; 131072 of 4096, 32768 words, most rows written twice, 425, now 389; 2065 of 385, 10007
+// words, 24, now 20.)  They pass the caches by, which leaves those to the gradients.
+
+// Zeros to a stretch of `bytes`, an even number, `units` times 16 bytes a thread.
+struct Zeros {
+    char *to;
+    int64_t bytes;
+    int units;
+};
+template <int THREADS>
+__device__ __forceinline__ void fill_zeros(const Zeros &z, int block)
+{
+    const int64_t head = min(z.bytes, (int64_t)(-(uintptr_t)z.to & 15)), all = (z.bytes - head) >> 4, tail = head + (all << 4);
+    Vec<uint32_t, 4> *const to = (Vec<uint32_t, 4> *)(z.to + head);
+#pragma unroll 4
+    for (int j = 0; j < z.units; ++j) {
+        const int64_t u = ((int64_t)block * z.units + j) * THREADS + threadIdx.x;
+        if (u < all) store_streaming(to + u, Vec<uint32_t, 4>{});
+    }
+    if (block > 0) return;
+    if ((int)threadIdx.x * 2 < head) ((uint16_t *)z.to)[threadIdx.x] = 0;
+    if ((int)threadIdx.x * 2 < z.bytes - tail) ((uint16_t *)(z.to + tail))[threadIdx.x] = 0;
+}
+// 16 KB a workgroup, up to 256 where all CUs have eight of them (2.1 GB: 438 us with 64 KB each, 386 with 128, 373 with 256).
+inline Zeros zeros_of(void *to, int64_t bytes, int threads)
+{
+    const int64_t share = max((int64_t)16384, min((int64_t)262144, bytes / (8 * device_cus())));
+    return Zeros{(char *)to, bytes, (int)(share / (threads * 16))};
+}
+inline int zero_blocks(const Zeros &z, int threads)
+{
+    const int64_t share = (int64_t)z.units * threads * 16;
+    return (int)((z.bytes + share - 1) / share);
+}
+
 constexpr uint32_t kNoWord = 0xfffffffeu;  // sorts behind every word: padding, and what is no word at all
 
 __device__ __forceinline__ uint32_t key_at(const void *ids, int wide, int64_t i, int64_t V, int64_t padding)
@@ -82,12 +120,18 @@ __device__ __forceinline__ uint32_t key_at(const void *ids, int wide, int64_t i,
 // take 22 (20 against 26 for 16384).
 constexpr int kRankMost = 8192;  // a multiple of 64
 
+// Workgroups behind those that sort fill `zeros` with zeros.
 __global__ __launch_bounds__(1024) void embed_rank_kernel(const void *__restrict__ ids, int wide, int T, int64_t V,
                                                           int64_t padding, uint32_t *__restrict__ keys,
-                                                          uint32_t *__restrict__ pos)
+                                                          uint32_t *__restrict__ pos, Zeros zeros)
 {
     __shared__ __attribute__((aligned(16))) uint32_t word[kRankMost];
     __shared__ uint32_t before[16][64];
+    const int sorting = (T + 63) / 64;
+    if ((int)blockIdx.x >= sorting) {
+        fill_zeros<1024>(zeros, blockIdx.x - sorting);
+        return;
+    }
     const int padded = (T + 63) & ~63;
     for (int i = threadIdx.x; i < padded; i += 1024) word[i] = i < T ? key_at(ids, wide, i, V, padding) : kNoWord;
     __syncthreads();
@@ -132,7 +176,8 @@ struct SortPass {
     uint32_t *out_keys, *out_pos;
     uint32_t *counts;  // [blocks][kDigits]
     int64_t T, stretch;
-    int shift;
+    int shift, blocks;  // workgroups from `blocks` on fill
+    Zeros zeros;
 };
 
 __device__ __forceinline__ uint32_t sort_key(const SortPass &p, int64_t i)
@@ -143,6 +188,10 @@ __device__ __forceinline__ uint32_t sort_key(const SortPass &p, int64_t i)
 __global__ __launch_bounds__(256) void embed_count_kernel(SortPass p)
 {
     __shared__ uint32_t count[kDigits];
+    if ((int)blockIdx.x >= p.blocks) {
+        fill_zeros<256>(p.zeros, blockIdx.x - p.blocks);
+        return;
+    }
     for (int d = threadIdx.x; d < kDigits; d += 256) count[d] = 0;
     __syncthreads();
     const int64_t from = blockIdx.x * p.stretch, to = min(p.T, from + p.stretch);
@@ -159,15 +208,19 @@ __global__ __launch_bounds__(256) void embed_scatter_kernel(SortPass p)
     __shared__ uint32_t seen[4][kDigits];   // keys of each digit that each wave has had in this tile
     __shared__ uint32_t wave_sum[4];
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    if ((int)blockIdx.x >= p.blocks) {
+        fill_zeros<256>(p.zeros, blockIdx.x - p.blocks);
+        return;
+    }
     {
         // two neighbouring digits a thread: totals, then an exclusive scan over the 512 digits
         uint32_t total[2] = {0, 0}, mine[2] = {0, 0};
         const uint2 *c = (const uint2 *)p.counts + threadIdx.x;
 #pragma unroll 16
-        for (unsigned b = 0; b < gridDim.x; ++b) {
+        for (int b = 0; b < p.blocks; ++b) {
             const uint2 v = c[b * (kDigits / 2)];
             total[0] += v.x, total[1] += v.y;
-            if (b < blockIdx.x) mine[0] += v.x, mine[1] += v.y;
+            if (b < (int)blockIdx.x) mine[0] += v.x, mine[1] += v.y;
         }
         const uint32_t own = total[0] + total[1];
         uint32_t run = own;
@@ -231,8 +284,8 @@ __global__ __launch_bounds__(256) void embed_scatter_kernel(SortPass p)
 
 // The sorted tokens are cut into chunks; a wave adds up one chunk for 64 * N columns.  A word whose tokens lie in one chunk
 // is finished there.  One that runs on leaves a partial sum: in slot 1 of the chunk that it begins in, in slot 0 of the
-// others; embed_finish_kernel joins them in order, so that a word with most of the tokens does not wait for one wave.  Bound by
-// memory: 65536 x 2048 bfloat16 gradients in, 0.27 GB, and some 0.14 GB of finished rows out in 68 us.  Eight rows are on their
+// others; embed_join_kernel joins them in order, so that a word with most of the tokens does not wait for one wave.  Bound by
+// memory: 65536 x 2048 bfloat16 gradients in, 0.27 GB, and 0.21 GB of finished rows out in 90 us.  Eight rows are on their
 // way at a time; sixteen take more registers than they hide (151 us where eight took 114).
 template <typename E, int N>
 __global__ __launch_bounds__(64) void embed_sum_kernel(const E *__restrict__ g, int64_t ldg, const uint32_t *__restrict__ keys,
@@ -315,92 +368,43 @@ __device__ __forceinline__ uint32_t wave_lower_bound(const uint32_t *__restrict_
     return lo;
 }
 
-// Every row that embed_sum_kernel has not finished: words without tokens get zeros, words in several chunks their joined
-// sums.  The zeros are most of a large table's gradient (0.4 GB of 131072 x 2048 in 92 us; stored past the caches, which keeps
-// the gradients that embed_sum_kernel reads in them: 203 instead of 224 us for the whole).  A workgroup owns `rows` rows (at most
-// 256, together a multiple of 16 bytes): two waves find the stretch of tokens that belongs to them; inside it the rows' own
-// stretches are marked by its tokens, or bisected where it is long.
+// The partial sums of a word that begins in chunk c0 and ends in c1, in order; `p` is chunk 0's slot 0, at the columns wanted.
 template <typename E, int N>
-__global__ __launch_bounds__(256) void embed_finish_kernel(const uint32_t *__restrict__ keys, const float *__restrict__ part,
-                                                           E *__restrict__ dw, int64_t T, int64_t V, int64_t D, int chunk,
-                                                           int rows, float scale, FastDiv by_row)
+__device__ __forceinline__ Vec<E, N> joined(const float *__restrict__ p, uint32_t c0, uint32_t c1, int64_t D, float scale)
 {
-    __shared__ uint32_t bound[2], begin[257];
-    __shared__ uint8_t empty[256];
-    const int64_t v0 = (int64_t)blockIdx.x * rows;
-    const int mine = (int)min((int64_t)rows, V - v0);
-    const int wave = threadIdx.x >> 6;
-    if (wave < 2) {
-        const uint32_t found = wave_lower_bound(keys, (uint32_t)T, (uint32_t)(v0 + (wave ? mine : 0)));
-        if ((threadIdx.x & 63) == 0) bound[wave] = found;
+    float acc[N];
+#pragma unroll
+    for (int e = 0; e < N; ++e) acc[e] = p[((int64_t)c0 * 2 + 1) * D + e];
+    constexpr int kAhead = N <= 2 ? 24 : 8;  // partial sums on their way
+    for (uint32_t c = c0 + 1; c <= c1; c += kAhead) {
+        Vec<float, N> got[kAhead];
+#pragma unroll
+        for (int j = 0; j < kAhead; ++j)
+            if (c + j <= c1) got[j] = *(const Vec<float, N> *)(p + (int64_t)(c + j) * 2 * D);
+#pragma unroll
+        for (int j = 0; j < kAhead; ++j)
+#pragma unroll
+            for (int e = 0; e < N; ++e) acc[e] += c + j <= c1 ? got[j].v[e] : 0.f;
     }
-    __syncthreads();
-    const uint32_t first = bound[0], end = bound[1];
-    if (end - first <= 1024) {
-        // every token whose word differs from the one before begins the rows in between
-        for (uint32_t i = first + threadIdx.x; i <= end; i += 256) {
-            const int row = i < end ? (int)(keys[i] - (uint32_t)v0) : mine;
-            for (int r = i > first ? (int)(keys[i - 1] - (uint32_t)v0) + 1 : 0; r <= row; ++r) begin[r] = i;
-        }
-    } else {
-        for (int i = threadIdx.x; i <= mine; i += 256) {
-            const uint32_t v = (uint32_t)(v0 + i);
-            uint32_t lo = first, hi = end;
-            while (lo < hi) {
-                const uint32_t mid = (lo + hi) >> 1;
-                if (keys[mid] < v) lo = mid + 1;
-                else hi = mid;
-            }
-            begin[i] = lo;
-        }
-    }
-    __syncthreads();
-    if ((int)threadIdx.x < mine) empty[threadIdx.x] = begin[threadIdx.x] == begin[threadIdx.x + 1];
-    __syncthreads();
-    // zeros, 16 bytes at a time where the whole of it lies in empty rows
-    constexpr int kUnit = 16 / sizeof(E);
-    E *const block = dw + v0 * D;
-    const int64_t total = mine * D;
-    const bool aligned = ((uintptr_t)block & 15) == 0;
-    for (int64_t u = (int64_t)threadIdx.x * kUnit; u < total; u += 256 * kUnit) {
-        const uint32_t r0 = div_by((uint32_t)u, by_row);
-        const int64_t last = min(u + kUnit, total) - 1;
-        const uint32_t r1 = div_by((uint32_t)last, by_row);
-        if (aligned && u + kUnit <= total && empty[r0] && (r1 == r0 || (r1 == r0 + 1 && empty[r1]))) {
-            store_streaming((Vec<uint32_t, 4> *)(block + u), Vec<uint32_t, 4>{});
-        } else {
-            for (int64_t i = u; i <= last; ++i)
-                if (empty[div_by((uint32_t)i, by_row)]) block[i] = from_float<E>(0.f);
-        }
-    }
-    if (first == end) return;
-    const uint32_t per_row = (uint32_t)(D / N);
-    for (uint32_t i = threadIdx.x; i < mine * per_row; i += 256) {
-        const uint32_t r = div_by(i * N, by_row), u = i - r * per_row;
-        const uint32_t from = begin[r], to = begin[r + 1];
-        if (to == from) continue;
-        const uint32_t c0 = from / chunk, c1 = (to - 1) / chunk;
-        if (c0 == c1) continue;
-        float acc[N];
-        const float *p = part + (int64_t)u * N;
+    Vec<E, N> o;
 #pragma unroll
-        for (int e = 0; e < N; ++e) acc[e] = p[((int64_t)c0 * 2 + 1) * D + e];
-        constexpr int kAhead = N <= 2 ? 24 : 8;  // partial sums on their way
-        for (uint32_t c = c0 + 1; c <= c1; c += kAhead) {
-            Vec<float, N> got[kAhead];
-#pragma unroll
-            for (int j = 0; j < kAhead; ++j)
-                if (c + j <= c1) got[j] = *(const Vec<float, N> *)(p + (int64_t)(c + j) * 2 * D);
-#pragma unroll
-            for (int j = 0; j < kAhead; ++j)
-#pragma unroll
-                for (int e = 0; e < N; ++e) acc[e] += c + j <= c1 ? got[j].v[e] : 0.f;
-        }
-        Vec<E, N> o;
-#pragma unroll
-        for (int e = 0; e < N; ++e) o.v[e] = from_float<E>(acc[e] * scale);
-        ((Vec<E, N> *)(block + (int64_t)r * D))[u] = o;
-    }
+    for (int e = 0; e < N; ++e) o.v[e] = from_float<E>(acc[e] * scale);
+    return o;
+}
+
+// Words in several chunks: their joined sums, by the workgroup of the chunk that such a word begins in.  Bound by latency: 44
+// partial sums of the most frequent of 2065 tokens in 4.4 us.
+template <typename E, int N>
+__global__ __launch_bounds__(64) void embed_join_kernel(const uint32_t *__restrict__ keys, const float *__restrict__ part,
+                                                        E *__restrict__ dw, int64_t T, int64_t D, int chunk, float scale)
+{
+    const int64_t from = (int64_t)blockIdx.x * chunk, to = min(T, from + chunk);
+    if (to >= T) return;
+    const uint32_t run = keys[to - 1];
+    if (run == kNoWord || keys[to] != run || (from > 0 && keys[from - 1] == run)) return;
+    const uint32_t end = (uint32_t)to + wave_lower_bound(keys + to, (uint32_t)(T - to), run + 1);
+    const int64_t col = ((int64_t)blockIdx.y * 64 + threadIdx.x) * N;
+    if (col < D) *(Vec<E, N> *)(dw + (int64_t)run * D + col) = joined<E, N>(part + col, blockIdx.x, (end - 1) / chunk, D, scale);
 }
 
 // Tokens a chunk: long ones leave hot words fewer partial sums to join, short ones more waves (2065 tokens, 700 of them one word:
@@ -428,27 +432,18 @@ inline EmbedSpace embed_space(int64_t T, int64_t D)
 
 template <typename E>
 int launch_embed_grad(const uint32_t *keys, const uint32_t *pos, const void *g, int64_t ldg, void *dw, float *part, int64_t T,
-                      int64_t V, int64_t D, float scale, hipStream_t st)
+                      int64_t D, float scale, hipStream_t st)
 {
     const int n = vector_elements(sizeof(E), {D, ldg}, {g, dw});
     const int chunk = embed_chunk(T);
     const int64_t chunks = (T + chunk - 1) / chunk, slices = (D / n + 63) / 64;
-    // 2 to 64 KB of the result a workgroup, in whole 16-byte units: the search for its tokens is paid for by larger ones,
-    // enough workgroups for every CU by smaller ones
-    constexpr int64_t kUnit = 16 / sizeof(E);
-    const int64_t row_bytes = D * (int64_t)sizeof(E);
-    const int64_t region = min((int64_t)65536, max((int64_t)2048, V * row_bytes / (8 * device_cus())));
-    const int rows = (int)min((int64_t)256, max(kUnit, region / row_bytes / kUnit * kUnit));
-    if (rows * D > 0x7fffffff) return DS_ETOOLARGE;
-    const int64_t finish = (V + rows - 1) / rows;
-    if (chunks > 0x7fffffff || slices > 65535 || finish > 0x7fffffff) return DS_ETOOLARGE;
+    if (chunks > 0x7fffffff || slices > 65535) return DS_ETOOLARGE;
 #define DS_LAUNCH(N)                                                                                                    \
     do {                                                                                                                \
-        if (T > 0)                                                                                                      \
-            hipLaunchKernelGGL((embed_sum_kernel<E, N>), dim3((unsigned)chunks, (unsigned)slices), dim3(64), 0, st,     \
-                               (const E *)g, ldg, keys, pos, (E *)dw, part, T, D, chunk, scale);                        \
-        hipLaunchKernelGGL((embed_finish_kernel<E, N>), dim3((unsigned)finish), dim3(256), 0, st, keys, part, (E *)dw, T, V, \
-                           D, chunk, rows, scale, fast_div((uint32_t)D));                                               \
+        hipLaunchKernelGGL((embed_sum_kernel<E, N>), dim3((unsigned)chunks, (unsigned)slices), dim3(64), 0, st,         \
+                           (const E *)g, ldg, keys, pos, (E *)dw, part, T, D, chunk, scale);                            \
+        hipLaunchKernelGGL((embed_join_kernel<E, N>), dim3((unsigned)chunks, (unsigned)slices), dim3(64), 0, st, keys,  \
+                           part, (E *)dw, T, D, chunk, scale);                                                          \
     } while (0)
     if (n == 8) { if constexpr (sizeof(E) == 2) DS_LAUNCH(8); }
     else if (n == 4) DS_LAUNCH(4);
@@ -458,24 +453,29 @@ int launch_embed_grad(const uint32_t *keys, const uint32_t *pos, const void *g, 
     return launch_status();
 }
 
-int sort_tokens(const void *ids, int wide, int64_t T, int64_t V, int64_t padding, char *ws, const EmbedSpace &s,
-                hipStream_t st, const uint32_t **keys, const uint32_t **pos)
+// The tokens in order of their words; the launches on the way also fill `bytes` at `zeros` with zeros.
+int sort_tokens(const void *ids, int wide, int64_t T, int64_t V, int64_t padding, char *ws, const EmbedSpace &s, void *zeros,
+                int64_t bytes, hipStream_t st, const uint32_t **keys, const uint32_t **pos)
 {
     uint32_t *k[2] = {(uint32_t *)(ws + s.keys[0]), (uint32_t *)(ws + s.keys[1])};
     uint32_t *p[2] = {(uint32_t *)(ws + s.pos[0]), (uint32_t *)(ws + s.pos[1])};
     int at = 0;
-    if (T <= kRankMost && g_tune.embed_radix != 1) {
-        if (T > 0)
-            hipLaunchKernelGGL(embed_rank_kernel, dim3((unsigned)((T + 63) / 64)), dim3(1024), 0, st, ids, wide, (int)T, V,
-                               padding, k[0], p[0]);
-    } else if (T > 0) {
+    if (T == 0 || (T <= kRankMost && g_tune.embed_radix != 1)) {
+        const Zeros z = zeros_of(zeros, bytes, 1024);
+        hipLaunchKernelGGL(embed_rank_kernel, dim3((unsigned)((T + 63) / 64 + zero_blocks(z, 1024))), dim3(1024), 0, st, ids, wide,
+                           (int)T, V, padding, k[0], p[0], z);
+    } else {
         // the low bits of kNoWord, all set but the last, have to stay above every word
         int bits = 1;
         while (((int64_t)1 << bits) <= V + 1) ++bits;
         int64_t blocks = min((int64_t)kSortBlocks, (T + kSortTile - 1) / kSortTile);
         const int64_t stretch = ((T + blocks - 1) / blocks + kSortTile - 1) / kSortTile * kSortTile;
         blocks = (T + stretch - 1) / stretch;
-        SortPass pass{ids, wide, V, padding, nullptr, nullptr, k[0], p[0], (uint32_t *)(ws + s.counts), T, stretch, 0};
+        // every launch fills its share
+        const int launches = (bits + kDigitBits - 1) / kDigitBits * 2;
+        const int64_t share = (bytes / launches / 65536 + 1) * 65536;
+        int64_t filled = 0;
+        SortPass pass{ids, wide, V, padding, nullptr, nullptr, k[0], p[0], (uint32_t *)(ws + s.counts), T, stretch, 0, (int)blocks, {}};
         for (int shift = 0; shift < bits; shift += kDigitBits) {
             pass.shift = shift;
             if (shift > 0) {
@@ -484,8 +484,12 @@ int sort_tokens(const void *ids, int wide, int64_t T, int64_t V, int64_t padding
                 at ^= 1;
                 pass.out_keys = k[at], pass.out_pos = p[at];
             }
-            hipLaunchKernelGGL(embed_count_kernel, dim3((unsigned)blocks), dim3(256), 0, st, pass);
-            hipLaunchKernelGGL(embed_scatter_kernel, dim3((unsigned)blocks), dim3(256), 0, st, pass);
+            for (auto kernel : {embed_count_kernel, embed_scatter_kernel}) {
+                const int64_t now = min(share, bytes - filled);
+                pass.zeros = zeros_of((char *)zeros + filled, now, 256);
+                filled += now;
+                hipLaunchKernelGGL(kernel, dim3((unsigned)(blocks + zero_blocks(pass.zeros, 256))), dim3(256), 0, st, pass);
+            }
         }
     }
     *keys = k[at], *pos = p[at];
@@ -527,10 +531,12 @@ DS_EXPORT int ds_embed_grad(const void *ids, int id_bytes, const void *grad, int
     if (workspace_bytes < s.bytes || !workspace || (uintptr_t)workspace % 16) return DS_EWORKSPACE;
     hipStream_t st = (hipStream_t)stream;
     const uint32_t *keys, *pos;
-    const int status = sort_tokens(ids, id_bytes == 8, T, V, padding, (char *)workspace, s, st, &keys, &pos);
-    if (status != DS_OK) return status;
+    const int64_t bytes = V * D * (int64_t)element_bytes(type);
+    const int status = sort_tokens(ids, id_bytes == 8, T, V, padding, (char *)workspace, s, dweight, bytes, st, &keys,
+                                   &pos);
+    if (status != DS_OK || T == 0) return status;
     float *part = (float *)((char *)workspace + s.part);
-    if (type == DS_F32) return launch_embed_grad<float>(keys, pos, grad, ldg, dweight, part, T, V, D, scale, st);
-    if (type == DS_BF16) return launch_embed_grad<bf16_t>(keys, pos, grad, ldg, dweight, part, T, V, D, scale, st);
-    return launch_embed_grad<f16_t>(keys, pos, grad, ldg, dweight, part, T, V, D, scale, st);
+    if (type == DS_F32) return launch_embed_grad<float>(keys, pos, grad, ldg, dweight, part, T, D, scale, st);
+    if (type == DS_BF16) return launch_embed_grad<bf16_t>(keys, pos, grad, ldg, dweight, part, T, D, scale, st);
+    return launch_embed_grad<f16_t>(keys, pos, grad, ldg, dweight, part, T, D, scale, st);
 }

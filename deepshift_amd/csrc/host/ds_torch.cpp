@@ -1,5 +1,5 @@
 // The host's side of calls whose kernels are over sooner than a few dozen steps of the Python interpreter: the lookup of an
-// embedding and the clipping of gradients.  Checks, allocations and the call of the library, on torch's tensors as they are.
+// embedding, its gradient, and the clipping of gradients.  Checks, allocations and the call of the library, on torch's tensors as they are.
 //
 // Bound by the launches themselves (2.7 us each) and torch's allocations (0.8 us).
 #include <Python.h>
@@ -104,27 +104,62 @@ template <typename F> PyObject *guarded(Py_ssize_t got, Py_ssize_t wanted, F &&b
     return nullptr;
 }
 
+// Token numbers on a device, contiguous.
+at::Tensor tokens(PyObject *o, c10::Device device)
+{
+    const at::Tensor &ids = tensor("ids", o);
+    if (ids.scalar_type() != at::kLong && ids.scalar_type() != at::kInt)
+        refuse(PyExc_TypeError, "ids must be int64 or int32, is ", c10::toString(ids.scalar_type()));
+    if (ids.device() != device) refuse(PyExc_ValueError, "ids must be on ", device.str(), ", is on ", ids.device().str());
+    return ids.is_contiguous() ? ids : ids.contiguous();
+}
+
+// A matrix whose rows lie contiguously, any distance apart, and that distance.
+int64_t rows(at::Tensor &t)
+{
+    const int64_t n = t.size(0), D = t.size(1);
+    if ((D > 1 && t.stride(1) != 1) || (n > 1 && t.stride(0) < D)) t = t.contiguous();
+    return n > 1 ? t.stride(0) : D;
+}
+
 // embed(ids, weight, scale, stream): scale * weight[ids]
 PyObject *embed(PyObject *, PyObject *const *args, Py_ssize_t count)
 {
     return guarded(count, 4, [&] {
-        at::Tensor ids = tensor("ids", args[0]), weight = tensor("weight", args[1]);
+        at::Tensor weight = tensor("weight", args[1]);
         const int code = checked_type("weight", weight);
         if (weight.dim() != 2) refuse(PyExc_ValueError, "weight must be [V, D], is ", weight.sizes());
-        if (ids.scalar_type() != at::kLong && ids.scalar_type() != at::kInt)
-            refuse(PyExc_TypeError, "ids must be int64 or int32, is ", c10::toString(ids.scalar_type()));
-        if (ids.device() != weight.device())
-            refuse(PyExc_ValueError, "ids must be on ", weight.device().str(), ", is on ", ids.device().str());
-        if (!ids.is_contiguous()) ids = ids.contiguous();
-        // rows that lie contiguously, any distance apart
-        const int64_t V = weight.size(0), D = weight.size(1);
-        if ((D > 1 && weight.stride(1) != 1) || (V > 1 && weight.stride(0) < D)) weight = weight.contiguous();
+        const at::Tensor ids = tokens(args[0], weight.device());
+        const int64_t V = weight.size(0), D = weight.size(1), ld = rows(weight);
         c10::SmallVector<int64_t, 6> shape(ids.sizes().begin(), ids.sizes().end());
         shape.push_back(D);
         at::Tensor out = at::empty(shape, weight.options().requires_grad(false));
-        expect("ds_embed", ds_embed(ids.const_data_ptr(), (int)ids.element_size(), weight.const_data_ptr(),
-                                    V > 1 ? weight.stride(0) : D, out.mutable_data_ptr(), ids.numel(), V, D,
-                                    (float)number(args[2]), code, stream(args[3])));
+        expect("ds_embed", ds_embed(ids.const_data_ptr(), (int)ids.element_size(), weight.const_data_ptr(), ld,
+                                    out.mutable_data_ptr(), ids.numel(), V, D, (float)number(args[2]), code, stream(args[3])));
+        return THPVariable_Wrap(std::move(out));
+    });
+}
+
+// embed_grad(ids, grad, V, scale, padding, stream): the gradient of embed with respect to a weight of V rows
+PyObject *embed_grad(PyObject *, PyObject *const *args, Py_ssize_t count)
+{
+    return guarded(count, 6, [&] {
+        const at::Tensor &given = tensor("grad", args[1]);
+        const int code = checked_type("grad", given);
+        const at::Tensor ids = tokens(args[0], given.device());
+        if (given.dim() < 1 || given.sizes().slice(0, given.dim() - 1) != ids.sizes())
+            refuse(PyExc_ValueError, "grad must have the shape of ids, ", ids.sizes(), ", and one more axis, is ", given.sizes());
+        const int64_t T = ids.numel(), D = given.size(-1), V = integer(args[2]);
+        if (V < 0) refuse(PyExc_ValueError, "num_embeddings must not be negative");
+        at::Tensor grad = given.reshape({T, D});
+        const int64_t ld = rows(grad);
+        const at::TensorOptions options = grad.options().requires_grad(false);
+        at::Tensor out = at::empty({V, D}, options);
+        const size_t bytes = ds_embed_grad_workspace_bytes(T, D);
+        at::Tensor workspace = at::empty({(int64_t)bytes}, options.dtype(at::kByte));
+        expect("ds_embed_grad", ds_embed_grad(ids.const_data_ptr(), (int)ids.element_size(), grad.const_data_ptr(), ld,
+                                              out.mutable_data_ptr(), T, V, D, integer(args[4]), (float)number(args[3]), code,
+                                              workspace.mutable_data_ptr(), bytes, stream(args[5])));
         return THPVariable_Wrap(std::move(out));
     });
 }
@@ -208,6 +243,8 @@ PyObject *clip(PyObject *, PyObject *const *args, Py_ssize_t count)
 
 PyMethodDef methods[] = {
     {"embed", (PyCFunction)(void (*)(void))embed, METH_FASTCALL, "embed(ids, weight, scale, stream) -> scale * weight[ids]"},
+    {"embed_grad", (PyCFunction)(void (*)(void))embed_grad, METH_FASTCALL,
+     "embed_grad(ids, grad, V, scale, padding, stream) -> gradient of a weight of V rows"},
     {"clip", (PyCFunction)(void (*)(void))clip, METH_FASTCALL,
      "clip(grads, outs or None, max_norm, scale, any_order, stream) -> norm, or None"},
     {nullptr, nullptr, 0, nullptr},

@@ -79,23 +79,11 @@ def embedding_grad(ids, grad, num_embeddings, scale=1.0, padding_idx=None):
     """Gradient of :func:`embedding` with respect to its weight, ``[num_embeddings, D]`` in ``grad``'s type: row ``v`` is
     ``scale`` times the sum of ``grad`` over the tokens ``v``, in ascending order and 32 bits.  Tokens equal to
     ``padding_idx`` add nothing, and neither do numbers outside ``[0, num_embeddings)``."""
-    code = _type_of("grad", grad)
-    ids = _tokens_of("ids", ids, grad.device)
-    if grad.dim() < 1 or grad.shape[:-1] != ids.shape:
-        raise ValueError("grad must be %s + [D], is %s" % (list(ids.shape), list(grad.shape)))
-    V, D = int(num_embeddings), grad.shape[-1]
-    if V < 0:
-        raise ValueError("num_embeddings must not be negative")
+    V = int(num_embeddings)
     padding = _padding(padding_idx, V)
-    T = ids.numel()
-    grad, ld = _rows_of(grad.reshape(T, D))
-    out = torch.empty((V, D), dtype=grad.dtype, device=grad.device)
-    with _on(grad.device):
-        nbytes = _lib.lib().ds_embed_grad_workspace_bytes(T, D)
-        ws = kernels._workspace(nbytes, grad.device)
-        _lib.call("ds_embed_grad", ids.data_ptr(), ids.element_size(), grad.data_ptr(), ld, out.data_ptr(), T, V, D, padding,
-                  float(scale), code, ws.data_ptr(), nbytes, _lib.stream_handle(grad.device))
-    return out
+    device = grad.device
+    with _on(device):
+        return _lib.native().embed_grad(ids, grad, V, float(scale), padding, _stream_of(device))
 
 
 def _padding(padding_idx, V):
