@@ -526,7 +526,7 @@ DS_EXPORT int ds_embed_grad(const void *ids, int id_bytes, const void *grad, int
     if (T < 0 || V < 0 || D < 0 || !element_bytes(type) || (id_bytes != 4 && id_bytes != 8)) return DS_EINVAL;
     if (V == 0 || D == 0) return DS_OK;
     if (!dweight || (T > 0 && (!ids || !grad || ldg < D))) return DS_EINVAL;
-    if (V > 0x7fffffff || T > 0x7fffffff) return DS_ETOOLARGE;
+    if (V > 0x7fffffff || T > 0x7fffffff || D > 0x7fffffff || V * D > (int64_t)1 << 44) return DS_ETOOLARGE;
     const EmbedSpace s = embed_space(T, D);
     if (workspace_bytes < s.bytes || !workspace || (uintptr_t)workspace % 16) return DS_EWORKSPACE;
     hipStream_t st = (hipStream_t)stream;

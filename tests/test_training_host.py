@@ -88,6 +88,11 @@ def test_status_codes_of_the_loss(fault):
     assert L.ds_vocab_loss(p, ld, p, ld, None, p, tb, -100, T, D, V, kind, red, rows, p, p, ws, nbytes, None) == want
 
 
+@pytest.mark.parametrize("T, V, D", [(4, 1 << 31, 8), (1 << 31, 4, 8), (4, 1 << 20, 1 << 40), (4, 1 << 30, 1 << 30)])
+def test_an_embeddings_gradient_has_to_fit(T, V, D):
+    assert _lib.lib().ds_embed_grad(4096, 8, 4096, D, 4096, T, V, D, -1, 1.0, 0, 4096, 1 << 62, None) == -5
+
+
 def test_status_codes_of_clipping():
     L = _lib.lib()
     t = (_lib.Tensor * 1)((4096, 4096, 10, 0, 0))
