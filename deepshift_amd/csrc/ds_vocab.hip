@@ -236,6 +236,9 @@ __global__ __launch_bounds__(1024) void row_scale_kernel(const float *__restrict
 
 // P[t][v] = scale_t (e[t][v] 2^(top[tile of v][t] - lse[t]) - [v = y_t]), in place; the target's own from its logit, in 32 bits.
 // A workgroup has 256 words of some rows, a thread 8 words of every eighth of them; its rows' sums are the bias's gradient.
+// 16-bit exponentials have been rounded once, and their probabilities are once more: bfloat16 gradients are 0.0021 of their norm
+// off instead of 0.0017, float16 ones 0.00022 instead of 0.00021, for one product less of four (float16 in place of bfloat16 would
+// hold nothing below 2^-39 of a tile's largest).
 // Bound by memory: 2048 x 32768 in three planes in 161 us, 0.8 GB at 5 TB/s, where forming the logits again takes 830.
 struct Finish {
     void *prob;
@@ -622,7 +625,7 @@ Args logit_args(const Call &c, const Plan &p, int64_t v0, int64_t n, const Opera
 }
 
 // Whether finish_kernel joins the rows' sums: each of its workgroups does it for its own rows, and one for all, which pays
-// while there are few of both (64 tokens, 1000 words, float32: 41 us a step instead of 44).
+// while there are few of both (64 tokens, 1000 words, float32: 3 us of a step).
 inline bool joined_later(const Plan &p, int64_t T, int tiles) { return p.keep && T <= 128 && tiles <= 64; }
 
 template <typename P>

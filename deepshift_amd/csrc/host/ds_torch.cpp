@@ -1,5 +1,5 @@
-// The host's side of calls whose kernels are over sooner than a few dozen steps of the Python interpreter: the lookup of an
-// embedding, its gradient, and the clipping of gradients.  Checks, allocations and the call of the library, on torch's tensors as they are.
+// The host's side of a training step's operators, whose kernels may be over sooner than a few dozen steps of the Python
+// interpreter: checks, allocations and the call of the library, on torch's tensors as they are.
 //
 // Bound by the launches themselves (2.7 us each) and torch's allocations (0.8 us).
 #include <Python.h>
@@ -105,20 +105,20 @@ template <typename F> PyObject *guarded(Py_ssize_t got, Py_ssize_t wanted, F &&b
 }
 
 // Token numbers on a device, contiguous.
-at::Tensor tokens(PyObject *o, c10::Device device)
+at::Tensor tokens(const char *name, PyObject *o, c10::Device device)
 {
-    const at::Tensor &ids = tensor("ids", o);
+    const at::Tensor &ids = tensor(name, o);
     if (ids.scalar_type() != at::kLong && ids.scalar_type() != at::kInt)
-        refuse(PyExc_TypeError, "ids must be int64 or int32, is ", c10::toString(ids.scalar_type()));
-    if (ids.device() != device) refuse(PyExc_ValueError, "ids must be on ", device.str(), ", is on ", ids.device().str());
+        refuse(PyExc_TypeError, name, " must be int64 or int32, is ", c10::toString(ids.scalar_type()));
+    if (ids.device() != device) refuse(PyExc_ValueError, name, " must be on ", device.str(), ", is on ", ids.device().str());
     return ids.is_contiguous() ? ids : ids.contiguous();
 }
 
-// A matrix whose rows lie contiguously, any distance apart, and that distance.
-int64_t rows(at::Tensor &t)
+// A matrix whose rows lie contiguously, up to `most` elements apart, and their distance.
+int64_t rows(at::Tensor &t, int64_t most = INT64_MAX)
 {
     const int64_t n = t.size(0), D = t.size(1);
-    if ((D > 1 && t.stride(1) != 1) || (n > 1 && t.stride(0) < D)) t = t.contiguous();
+    if ((D > 1 && t.stride(1) != 1) || (n > 1 && (t.stride(0) < D || t.stride(0) > most))) t = t.contiguous();
     return n > 1 ? t.stride(0) : D;
 }
 
@@ -129,7 +129,7 @@ PyObject *embed(PyObject *, PyObject *const *args, Py_ssize_t count)
         at::Tensor weight = tensor("weight", args[1]);
         const int code = checked_type("weight", weight);
         if (weight.dim() != 2) refuse(PyExc_ValueError, "weight must be [V, D], is ", weight.sizes());
-        const at::Tensor ids = tokens(args[0], weight.device());
+        const at::Tensor ids = tokens("ids", args[0], weight.device());
         const int64_t V = weight.size(0), D = weight.size(1), ld = rows(weight);
         c10::SmallVector<int64_t, 6> shape(ids.sizes().begin(), ids.sizes().end());
         shape.push_back(D);
@@ -146,7 +146,7 @@ PyObject *embed_grad(PyObject *, PyObject *const *args, Py_ssize_t count)
     return guarded(count, 6, [&] {
         const at::Tensor &given = tensor("grad", args[1]);
         const int code = checked_type("grad", given);
-        const at::Tensor ids = tokens(args[0], given.device());
+        const at::Tensor ids = tokens("ids", args[0], given.device());
         if (given.dim() < 1 || given.sizes().slice(0, given.dim() - 1) != ids.sizes())
             refuse(PyExc_ValueError, "grad must have the shape of ids, ", ids.sizes(), ", and one more axis, is ", given.sizes());
         const int64_t T = ids.numel(), D = given.size(-1), V = integer(args[2]);
@@ -161,6 +161,157 @@ PyObject *embed_grad(PyObject *, PyObject *const *args, Py_ssize_t count)
                                               out.mutable_data_ptr(), T, V, D, integer(args[4]), (float)number(args[3]), code,
                                               workspace.mutable_data_ptr(), bytes, stream(args[5])));
         return THPVariable_Wrap(std::move(out));
+    });
+}
+
+// The operands of a head's cross entropy: hidden [..., D], weight [V, D], target [...], bias [V] or None.
+struct Head {
+    at::Tensor hidden, weight, target, bias;
+    std::vector<int64_t> shape;  // of hidden
+    int64_t ldh, ldw, T, D, V, ignore;
+    int type;
+
+    explicit Head(PyObject *const *args) : hidden(tensor("hidden", args[0])), weight(tensor("weight", args[1]))
+    {
+        constexpr int64_t kLongestRow = 2000000;  // elements between rows that the products' 32-bit offsets reach
+        type = checked_type("hidden", hidden);
+        if (hidden.dim() < 1) refuse(PyExc_ValueError, "hidden must have the features as its last axis, is ", hidden.sizes());
+        shape = hidden.sizes().vec();
+        D = shape.back();
+        if (weight.dim() != 2 || weight.size(1) != D)
+            refuse(PyExc_ValueError, "weight must be [V, ", std::to_string(D), "], is ", weight.sizes());
+        V = weight.size(0);
+        if (V < 1) refuse(PyExc_ValueError, "weight must have at least one row");
+        alike("weight", weight);
+        target = tokens("target", args[2], hidden.device());
+        if (target.sizes() != hidden.sizes().slice(0, shape.size() - 1))
+            refuse(PyExc_ValueError, "target must be ", hidden.sizes().slice(0, shape.size() - 1), ", is ", target.sizes());
+        if (args[3] != Py_None) {
+            bias = tensor("bias", args[3]);
+            alike("bias", bias);
+            if (bias.dim() != 1 || bias.size(0) != V)
+                refuse(PyExc_ValueError, "bias must be [", std::to_string(V), "], is ", bias.sizes());
+            bias = bias.contiguous();
+        }
+        ignore = integer(args[4]);
+        T = target.numel();
+        if (hidden.dim() != 2) hidden = hidden.reshape({T, D});
+        ldh = rows(hidden, kLongestRow);
+        ldw = rows(weight, kLongestRow);
+    }
+
+    void alike(const char *name, const at::Tensor &t) const
+    {
+        if (t.scalar_type() != hidden.scalar_type() || t.device() != hidden.device())
+            refuse(PyExc_TypeError, name, " must be ", c10::toString(hidden.scalar_type()), " on ", hidden.device().str(),
+                   " like hidden, is ", c10::toString(t.scalar_type()), " on ", t.device().str());
+    }
+
+    at::Tensor empty(at::IntArrayRef sizes, at::ScalarType as) const
+    {
+        return at::empty(sizes, at::TensorOptions().device(hidden.device()).dtype(as));
+    }
+    at::Tensor empty(at::IntArrayRef sizes) const { return empty(sizes, hidden.scalar_type()); }
+
+    // loss 1, gradients 2, both 3
+    at::Tensor workspace(int what) const
+    {
+        const size_t bytes =
+            ds_vocab_workspace_bytes(hidden.const_data_ptr(), ldh, weight.const_data_ptr(), ldw, T, D, V, type, what);
+        return empty({(int64_t)bytes}, at::kByte);
+    }
+    const void *bias_at() const { return bias.defined() ? bias.const_data_ptr() : nullptr; }
+};
+
+template <typename E = void> E *at_or_null(const at::Tensor &t) { return t.defined() ? (E *)t.mutable_data_ptr() : nullptr; }
+
+// New references to tensors, None for those that are not defined.
+PyObject *tuple_of(std::initializer_list<at::Tensor> tensors)
+{
+    PyObject *t = PyTuple_New((Py_ssize_t)tensors.size());
+    if (!t) return nullptr;
+    Py_ssize_t i = 0;
+    for (const at::Tensor &x : tensors) PyTuple_SET_ITEM(t, i++, THPVariable_Wrap(x));
+    return t;
+}
+
+// What a call finds out about the losses of rows.
+struct Losses {
+    int reduction;
+    at::Tensor rows, lse, total;
+
+    Losses(const Head &h, PyObject *red) : reduction((int)integer(red))
+    {
+        rows = h.empty(h.target.sizes(), at::kFloat);
+        lse = h.empty({h.T}, at::kFloat);
+        if (reduction) total = h.empty({2}, at::kFloat);
+    }
+    at::Tensor result() const { return reduction ? total.select(0, 0) : rows; }
+};
+
+// cross_entropy(hidden, weight, target, bias or None, ignore, reduction, stream): the loss, and what its gradients need: the
+// rows' logarithms, and a row's share in the loss where it is reduced
+PyObject *cross_entropy(PyObject *, PyObject *const *args, Py_ssize_t count)
+{
+    return guarded(count, 7, [&] {
+        const Head h(args);
+        const Losses l(h, args[5]);
+        const at::Tensor ws = h.workspace(1);
+        expect("ds_vocab_loss",
+               ds_vocab_loss(h.hidden.const_data_ptr(), h.ldh, h.weight.const_data_ptr(), h.ldw, h.bias_at(),
+                             h.target.const_data_ptr(), (int)h.target.element_size(), h.ignore, h.T, h.D, h.V, h.type, l.reduction,
+                             at_or_null<float>(l.rows), at_or_null<float>(l.lse), at_or_null<float>(l.total),
+                             ws.mutable_data_ptr(), ws.nbytes(), stream(args[6])));
+        return tuple_of({l.result(), l.lse, l.reduction ? l.total.select(0, 1) : at::Tensor()});
+    });
+}
+
+// cross_entropy_grad(hidden, weight, target, bias or None, ignore, lse, share or None, grad, wanted, stream): gradients of
+// hidden, weight and bias for `grad`, of the loss or (where there is no share) of the rows; bits 0 to 2 of `wanted` say which
+PyObject *cross_entropy_grad(PyObject *, PyObject *const *args, Py_ssize_t count)
+{
+    return guarded(count, 10, [&] {
+        const Head h(args);
+        const at::Tensor &lse = tensor("lse", args[5]), &grad = tensor("grad", args[7]);
+        const at::Tensor share = args[6] == Py_None ? at::Tensor() : tensor("share", args[6]);
+        for (const at::Tensor *t : {&lse, &grad, &share})
+            if (t->defined() && (t->scalar_type() != at::kFloat || !t->is_contiguous() || t->device() != h.hidden.device() ||
+                                 t->numel() != (t == &lse || (t == &grad && !share.defined()) ? h.T : 1)))
+                refuse(PyExc_ValueError, "lse, share and grad must be float32 and fit the tokens");
+        const int64_t wanted = integer(args[8]);
+        at::Tensor dhidden, dweight, dbias;
+        if (wanted & 1) dhidden = h.empty(h.shape);
+        if (wanted & 2) dweight = h.empty({h.V, h.D});
+        if (wanted & 4 && h.bias.defined()) dbias = h.empty({h.V});
+        const at::Tensor ws = h.workspace(2);
+        const float *g = (const float *)grad.const_data_ptr();
+        expect("ds_vocab_loss_grad",
+               ds_vocab_loss_grad(h.hidden.const_data_ptr(), h.ldh, h.weight.const_data_ptr(), h.ldw, h.bias_at(),
+                                  h.target.const_data_ptr(), (int)h.target.element_size(), h.ignore, h.T, h.D, h.V, h.type,
+                                  (const float *)lse.const_data_ptr(), share.defined() ? nullptr : g, share.defined() ? g : nullptr,
+                                  share.defined() ? (const float *)share.const_data_ptr() : nullptr, at_or_null(dhidden),
+                                  at_or_null(dweight), at_or_null(dbias), ws.mutable_data_ptr(), ws.nbytes(), stream(args[9])));
+        return tuple_of({dhidden, dweight, dbias});
+    });
+}
+
+// cross_entropy_step(hidden, weight, target, bias or None, ignore, reduction, stream): the loss and its gradients, for a
+// gradient of 1
+PyObject *cross_entropy_step(PyObject *, PyObject *const *args, Py_ssize_t count)
+{
+    return guarded(count, 7, [&] {
+        const Head h(args);
+        const Losses l(h, args[5]);
+        const at::Tensor dhidden = h.empty(h.shape), dweight = h.empty({h.V, h.D});
+        const at::Tensor dbias = h.bias.defined() ? h.empty({h.V}) : at::Tensor();
+        const at::Tensor ws = h.workspace(3);
+        expect("ds_vocab_loss_step",
+               ds_vocab_loss_step(h.hidden.const_data_ptr(), h.ldh, h.weight.const_data_ptr(), h.ldw, h.bias_at(),
+                                  h.target.const_data_ptr(), (int)h.target.element_size(), h.ignore, h.T, h.D, h.V, h.type,
+                                  l.reduction, at_or_null<float>(l.rows), at_or_null<float>(l.lse), at_or_null<float>(l.total),
+                                  at_or_null(dhidden), at_or_null(dweight), at_or_null(dbias), ws.mutable_data_ptr(), ws.nbytes(),
+                                  stream(args[6])));
+        return tuple_of({l.result(), dhidden, dweight, dbias});
     });
 }
 
@@ -245,6 +396,12 @@ PyMethodDef methods[] = {
     {"embed", (PyCFunction)(void (*)(void))embed, METH_FASTCALL, "embed(ids, weight, scale, stream) -> scale * weight[ids]"},
     {"embed_grad", (PyCFunction)(void (*)(void))embed_grad, METH_FASTCALL,
      "embed_grad(ids, grad, V, scale, padding, stream) -> gradient of a weight of V rows"},
+    {"cross_entropy", (PyCFunction)(void (*)(void))cross_entropy, METH_FASTCALL,
+     "cross_entropy(hidden, weight, target, bias or None, ignore, reduction, stream) -> loss, lse, share or None"},
+    {"cross_entropy_grad", (PyCFunction)(void (*)(void))cross_entropy_grad, METH_FASTCALL,
+     "cross_entropy_grad(hidden, weight, target, bias or None, ignore, lse, share or None, grad, wanted, stream) -> gradients"},
+    {"cross_entropy_step", (PyCFunction)(void (*)(void))cross_entropy_step, METH_FASTCALL,
+     "cross_entropy_step(hidden, weight, target, bias or None, ignore, reduction, stream) -> loss, gradients"},
     {"clip", (PyCFunction)(void (*)(void))clip, METH_FASTCALL,
      "clip(grads, outs or None, max_norm, scale, any_order, stream) -> norm, or None"},
     {nullptr, nullptr, 0, nullptr},

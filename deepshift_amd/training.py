@@ -17,38 +17,12 @@ import torch.nn as nn
 from torch.autograd import Function
 from torch.autograd.function import once_differentiable
 
-from . import _lib, kernels
+from . import _lib
 
 __all__ = ["embedding", "embedding_grad", "linear_cross_entropy", "linear_cross_entropy_grad", "gradient_norm",
            "clip_gradients_", "clip_grad_norm_", "ScaledEmbedding", "LinearCrossEntropy"]
 
-_TYPES = {torch.float32: _lib.DS_F32, torch.bfloat16: _lib.DS_BF16, torch.float16: _lib.DS_F16}
-_LONGEST_ROW = 2000000    # elements between rows that the products' 32-bit offsets reach
 _REDUCTIONS = {"none": _lib.DS_NONE, "sum": _lib.DS_SUM, "mean": _lib.DS_MEAN}
-
-
-def _type_of(name, t):
-    code = _TYPES.get(t.dtype)
-    if code is None:
-        raise TypeError("%s must be float32, bfloat16 or float16, got %s" % (name, t.dtype))
-    if not t.is_cuda:
-        raise ValueError("%s must be a GPU tensor" % name)
-    return code
-
-
-def _tokens_of(name, t, device):
-    if t.dtype != torch.int64 and t.dtype != torch.int32:
-        raise TypeError("%s must be int64 or int32, got %s" % (name, t.dtype))
-    if t.device != device:
-        raise ValueError("%s must be on %s, is on %s" % (name, device, t.device))
-    return t if t.is_contiguous() else t.contiguous()
-
-
-def _rows_of(t):
-    """A matrix whose rows lie contiguously, and the distance between them."""
-    if t.stride(1) != 1 and t.size(1) > 1 or t.size(0) > 1 and not t.size(1) <= t.stride(0) <= _LONGEST_ROW:
-        t = t.contiguous()
-    return t, t.stride(0) if t.size(0) > 1 else t.size(1)
 
 
 _HERE = contextlib.nullcontext()
@@ -127,111 +101,37 @@ def embedding(ids, weight, scale=1.0, padding_idx=None):
 # cross entropy of a linear head
 # ---------------------------------------------------------------------------------------------
 
-class _Head:
-    """The checked operands of one call, as the library takes them."""
-
-    def __init__(self, hidden, weight, target, bias, ignore_index, reduction):
-        self.type = _type_of("hidden", hidden)
-        device = hidden.device
-        if reduction not in _REDUCTIONS:
-            raise ValueError("reduction must be 'none', 'sum' or 'mean', is %r" % (reduction,))
-        self.reduction = _REDUCTIONS[reduction]
-        if hidden.dim() < 1 or weight.dim() != 2 or weight.shape[1] != hidden.shape[-1]:
-            raise ValueError("weight must be [V, %s], is %s" % (hidden.shape[-1] if hidden.dim() else "D", list(weight.shape)))
-        if weight.shape[0] < 1:
-            raise ValueError("weight must have at least one row")
-        for name, t in (("weight", weight), ("bias", bias)):
-            if t is not None and (t.dtype != hidden.dtype or t.device != device):
-                raise TypeError("%s must be %s on %s like hidden, is %s on %s" % (name, hidden.dtype, device, t.dtype, t.device))
-        if bias is not None and bias.shape != weight.shape[:1]:
-            raise ValueError("bias must be [%d], is %s" % (weight.shape[0], list(bias.shape)))
-        if target.shape != hidden.shape[:-1]:
-            raise ValueError("target must be %s, is %s" % (list(hidden.shape[:-1]), list(target.shape)))
-        self.shape = target.shape
-        self.target = _tokens_of("target", target, device)
-        self.V, self.D = weight.shape
-        self.T = self.target.numel()
-        self.hidden_shape = hidden.shape
-        self.hidden, self.ldh = _rows_of(hidden.reshape(self.T, self.D))
-        self.weight, self.ldw = _rows_of(weight)
-        self.bias = None if bias is None else bias.contiguous()
-        self.ignore = int(ignore_index)
-        if not -2 ** 63 <= self.ignore < 2 ** 63:
-            raise ValueError("ignore_index must fit 64 bits")
-
-    def _matrices(self):
-        return self.hidden.data_ptr(), self.ldh, self.weight.data_ptr(), self.ldw
-
-    def _problem(self):
-        return self._matrices() + (_lib.ptr(self.bias), self.target.data_ptr(), self.target.element_size(), self.ignore, self.T,
-                                   self.D, self.V, self.type)
-
-    def _workspace(self, what):
-        """Workspace, its size and the stream, as the calls end."""
-        nbytes = _lib.lib().ds_vocab_workspace_bytes(*(self._matrices() + (self.T, self.D, self.V, self.type, what)))
-        device = self.hidden.device
-        # the tensor has to live until the launches are issued
-        self.ws = kernels._workspace(nbytes, device)
-        return self.ws.data_ptr(), nbytes, _lib.stream_handle(device)
-
-    def _losses(self):
-        """Losses and logarithms of the rows, and the total and a row's share in it where there is one."""
-        rows = torch.empty((2, self.T), dtype=torch.float32, device=self.hidden.device)
-        total = torch.empty(2, dtype=torch.float32, device=self.hidden.device) if self.reduction else None
-        at = rows.data_ptr()
-        return rows, total, (self.reduction, at, at + 4 * self.T, _lib.ptr(total))
-
-    def _gradients(self, wanted=(True, True, True)):
-        like = dict(dtype=self.hidden.dtype, device=self.hidden.device)
-        return (torch.empty(self.hidden_shape, **like) if wanted[0] else None,
-                torch.empty((self.V, self.D), **like) if wanted[1] else None,
-                torch.empty(self.V, **like) if wanted[2] and self.bias is not None else None)
-
-    def _result(self, rows, total):
-        return rows[0].view(self.shape) if total is None else total[0]
-
-    def loss(self):
-        """``(loss, lse, share)``: the reduced loss (or one per token), and what the gradients need of it."""
-        rows, total, args = self._losses()
-        _lib.call("ds_vocab_loss", *(self._problem() + args + self._workspace(1)))
-        return self._result(rows, total), rows[1], None if total is None else total[1]
-
-    def gradients(self, lse, share, row_grad, grad, wanted):
-        """Gradients of hidden, weight and bias, ``None`` for those that are not ``wanted``."""
-        got = self._gradients(wanted)
-        _lib.call("ds_vocab_loss_grad", *(self._problem() + tuple(map(_lib.ptr, (lse, row_grad, grad, share) + got)) +
-                                          self._workspace(2)))
-        return got
-
-    def step(self):
-        """The loss and all gradients, for a gradient of 1."""
-        rows, total, args = self._losses()
-        got = self._gradients()
-        _lib.call("ds_vocab_loss_step", *(self._problem() + args + tuple(map(_lib.ptr, got)) + self._workspace(3)))
-        return (self._result(rows, total),) + got
+def _decided(ignore_index, reduction):
+    """``ignore_index`` and ``reduction`` as the library takes them."""
+    if reduction not in _REDUCTIONS:
+        raise ValueError("reduction must be 'none', 'sum' or 'mean', is %r" % (reduction,))
+    ignore_index = int(ignore_index)
+    if not -2 ** 63 <= ignore_index < 2 ** 63:
+        raise ValueError("ignore_index must fit 64 bits")
+    return ignore_index, _REDUCTIONS[reduction]
 
 
 class _LinearCrossEntropy(Function):
     @staticmethod
     def forward(ctx, hidden, weight, target, bias, ignore_index, reduction):
-        with _on(hidden.device):
-            head = _Head(hidden, weight, target, bias, ignore_index, reduction)
-            loss, lse, share = head.loss()
+        device = hidden.device
+        with _on(device):
+            loss, lse, share = _lib.native().cross_entropy(hidden, weight, target, bias, ignore_index, reduction,
+                                                           _stream_of(device))
         ctx.save_for_backward(hidden, weight, target, bias, lse, share)
-        ctx.of = (ignore_index, reduction)
+        ctx.ignore_index = ignore_index
         return loss
 
     @staticmethod
     @once_differentiable
     def backward(ctx, grad):
         hidden, weight, target, bias, lse, share = ctx.saved_tensors
-        with _on(hidden.device):
-            head = _Head(hidden, weight, target, bias, *ctx.of)
-            grad = grad.float().contiguous()
-            needed = ctx.needs_input_grad
-            got = head.gradients(lse, share, grad if share is None else None, None if share is None else grad,
-                                 (needed[0], needed[1], needed[3]))
-        return got[0], got[1], None, got[2], None, None
+        device, needed = hidden.device, ctx.needs_input_grad
+        with _on(device):
+            dhidden, dweight, dbias = _lib.native().cross_entropy_grad(
+                hidden, weight, target, bias, ctx.ignore_index, lse, share, grad.float().contiguous(),
+                needed[0] | needed[1] << 1 | needed[3] << 2, _stream_of(device))
+        return dhidden, dweight, None, dbias, None, None
 
 
 def linear_cross_entropy(hidden, weight, target, bias=None, ignore_index=-100, reduction="mean"):
@@ -242,17 +142,21 @@ def linear_cross_entropy(hidden, weight, target, bias=None, ignore_index=-100, r
     Tokens whose target is ``ignore_index`` have loss 0 and leave nothing in any gradient, whatever ``hidden`` holds there; if
     no token counts, the loss and its gradients are 0.  A target that is neither ``ignore_index`` nor in ``[0, V)`` gives NaN.
     A bias of ``-inf`` takes a word out."""
+    ignore_index, reduction = _decided(ignore_index, reduction)
     if torch.is_grad_enabled() and (hidden.requires_grad or weight.requires_grad or (bias is not None and bias.requires_grad)):
         return _LinearCrossEntropy.apply(hidden, weight, target, bias, ignore_index, reduction)
-    with _on(hidden.device):
-        return _Head(hidden, weight, target, bias, ignore_index, reduction).loss()[0]
+    device = hidden.device
+    with _on(device):
+        return _lib.native().cross_entropy(hidden, weight, target, bias, ignore_index, reduction, _stream_of(device))[0]
 
 
 def linear_cross_entropy_grad(hidden, weight, target, bias=None, ignore_index=-100, reduction="mean"):
     """``(loss, dhidden, dweight, dbias)`` of :func:`linear_cross_entropy` for a gradient of 1 (of ones, with
     ``reduction='none'``), without autograd; ``dbias`` is ``None`` where there is no bias."""
-    with torch.no_grad(), _on(hidden.device):
-        return _Head(hidden, weight, target, bias, ignore_index, reduction).step()
+    ignore_index, reduction = _decided(ignore_index, reduction)
+    device = hidden.device
+    with _on(device):
+        return _lib.native().cross_entropy_step(hidden, weight, target, bias, ignore_index, reduction, _stream_of(device))
 
 
 # ---------------------------------------------------------------------------------------------
