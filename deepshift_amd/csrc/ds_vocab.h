@@ -171,11 +171,13 @@ __device__ __forceinline__ void exp2_of_four(const float (&x)[4], float (&e)[4],
 
 // A launch's tile: the workgroups of one XCD (they are dealt out in turn) get neighbouring tiles, in strips of kStrip along m,
 // so that what they read at the same time fits its L2.
-__device__ __forceinline__ void tile_of(int id, int tiles_m, int tiles_n, int *tm, int *tn)
+__device__ __forceinline__ void tile_of(int id, int tiles_m, int tiles_n, int splits, int *tm, int *tn, int *split)
 {
     constexpr int kXcds = 8, kStrip = 8;
-    const int total = tiles_m * tiles_n, even = total / kXcds * kXcds;
+    const int tiles = tiles_m * tiles_n, even = tiles * splits / kXcds * kXcds;
     if (id < even) id = (id % kXcds) * (even / kXcds) + id / kXcds;
+    *split = id / tiles;
+    id -= *split * tiles;
     const int per_strip = kStrip * tiles_n;
     const int strip = id / per_strip, in = id - strip * per_strip;
     const int first = strip * kStrip, width = min(kStrip, tiles_m - first);
@@ -419,10 +421,8 @@ __device__ __forceinline__ void product_tile(const Args &g, const int block, cha
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
     const int wm = wave % WM, wn = wave / WM;
 
-    int tm, tn;
-    const int tiles = g.tiles_m * g.tiles_n;
-    const int split = block / tiles;
-    tile_of(block - split * tiles, g.tiles_m, g.tiles_n, &tm, &tn);
+    int tm, tn, split;
+    tile_of(block, g.tiles_m, g.tiles_n, g.splits, &tm, &tn, &split);
     const int m0 = tm * BM, n0 = tn * BN;
     const int k_from = split * g.k_split, k_to = min(g.K, k_from + g.k_split);
     const int steps = (k_to - k_from + kStep - 1) / kStep;
@@ -552,44 +552,54 @@ __device__ __forceinline__ void product_tile(const Args &g, const int block, cha
             const int p = n / NT, j = n % NT;
             fb[p][j] = TB::fragment(lds + from * kStageBytes + NP * TA::bytes + p * TB::bytes, (wn * NT + j) * U::size, 0);
         };
-        // the products of 2^-16, then those of 2^-8, then the largest; between(0) .. between(kTurns - 1) in between
+        // The products of 2^-16, the largest ones while those are made 2^-8, then the products of 2^-8; between(0) ..
+        // between(kTurns - 1) in between.  What they amount to joins the result during the first turns of the next group (of
+        // this one, where it is the only one): the matrix cores do not wait for either.
+        f32x4 low[2][G][NT];
+        auto join = [&](int group, int i, int j) {
+            f32x4 &c = acc[group * G + i][j];
+#pragma unroll
+            for (int r = 0; r < 4; ++r) c[r] = fmaf(low[group % 2][i][j][r], 1.f / 256, c[r]);
+        };
         auto multiply = [&](int group, const s16x8 (&fa)[G][NP], const s16x8 (&fb)[NP][NT], auto between) {
-            f32x4 low[G][NT];
-            auto add = [&](int p, int q) {
+            f32x4(&mine)[G][NT] = low[group % 2];
+            const int last = (group + kGroups - 1) % kGroups;
+            auto add = [&](int p, int q, auto besides) {
 #pragma unroll
                 for (int i = 0; i < G; ++i)
 #pragma unroll
-                    for (int j = 0; j < NT; ++j) low[i][j] = U::multiply(fa[i][p], fb[q][j], low[i][j]);
+                    for (int j = 0; j < NT; ++j) {
+                        mine[i][j] = U::multiply(fa[i][p], fb[q][j], mine[i][j]);
+                        besides(i, j);
+                    }
             };
+            auto nothing = [](int, int) {};
 #pragma unroll
             for (int i = 0; i < G; ++i)
 #pragma unroll
-                for (int j = 0; j < NT; ++j) low[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-            add(1, 1), between(0);
-            add(0, 2), between(1);
-            add(2, 0), between(2);
-#pragma unroll
-            for (int i = 0; i < G; ++i)
-#pragma unroll
-                for (int j = 0; j < NT; ++j) low[i][j] *= 1.f / 256;
-            add(0, 1), between(3);
-            add(1, 0), between(4);
+                for (int j = 0; j < NT; ++j) mine[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+            add(1, 1, [&](int i, int j) {
+                if (kGroups > 1) join(last, i, j);
+            });
+            between(0);
+            add(0, 2, nothing), between(1);
+            add(2, 0, nothing), between(2);
 #pragma unroll
             for (int i = 0; i < G; ++i)
 #pragma unroll
                 for (int j = 0; j < NT; ++j) {
                     f32x4 &c = acc[group * G + i][j];
                     c = U::multiply(fa[i][0], fb[0][j], c);
+                    mine[i][j] *= 1.f / 256;
                 }
-            between(5);
+            between(3);
+            add(0, 1, nothing), between(4);
+            add(1, 0, nothing), between(5);
+            if (kGroups == 1)
 #pragma unroll
-            for (int i = 0; i < G; ++i)
+                for (int i = 0; i < G; ++i)
 #pragma unroll
-                for (int j = 0; j < NT; ++j) {
-                    f32x4 &c = acc[group * G + i][j];
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) c[r] = fmaf(low[i][j][r], 1.f / 256, c[r]);
-                }
+                    for (int j = 0; j < NT; ++j) join(group, i, j);
         };
         auto step = [&](s16x8 (&fb)[NP][NT], s16x8 (&fa)[G][NP], s16x8 (&next_b)[NP][NT], s16x8 (&next_a)[G][NP]) {
 #pragma unroll
@@ -631,10 +641,20 @@ __device__ __forceinline__ void product_tile(const Args &g, const int block, cha
         for (int n = 0; n < G * NP; ++n) read_a(0, 0, n, a0);
 #pragma unroll
         for (int n = 0; n < NP * NT; ++n) read_b(0, n, b0);
+        if (kGroups > 1)
+#pragma unroll
+            for (int i = 0; i < G; ++i)
+#pragma unroll
+                for (int j = 0; j < NT; ++j) low[(kGroups - 1) % 2][i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
         for (int s = 0; s < steps; s += 2) {
             step(b0, a0, b1, a1);
             if (s + 1 < steps) step(b1, a1, b0, a0);
         }
+        if (kGroups > 1)
+#pragma unroll
+            for (int i = 0; i < G; ++i)
+#pragma unroll
+                for (int j = 0; j < NT; ++j) join(kGroups - 1, i, j);
     }
     // nothing of this wave is on its way to LDS any more, and nobody reads it
     asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
