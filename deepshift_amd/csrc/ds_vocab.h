@@ -72,15 +72,16 @@ struct Unit {
 };
 
 // Planes of a float32 value, each what is left of it times 2^8, rounded to nearest, so that what a product leaves out has no
-// sign of its own; where that would round to infinity it is cut instead.
+// sign of its own; where that would round to infinity it is cut instead.  SMALL: values in [-1, 1], or no number.
+template <bool SMALL = false>
 __device__ __forceinline__ void split_planes(float f, bf16_t *p)
 {
 #pragma unroll
     for (int q = 0; q < 3; ++q) {
         bf16_t a = from_float<bf16_t>(f);
-        if ((a.bits & 0x7fff) == 0x7f80 && fabsf(f) < INFINITY) a.bits = (uint16_t)(__float_as_uint(f) >> 16);
+        if (!SMALL && (a.bits & 0x7fff) == 0x7f80 && fabsf(f) < INFINITY) a.bits = (uint16_t)(__float_as_uint(f) >> 16);
         p[q] = a;
-        f = (a.bits & 0x7f80) == 0x7f80 ? 0.f : (f - to_float(a)) * 256.f;
+        f = !SMALL && (a.bits & 0x7f80) == 0x7f80 ? 0.f : (f - to_float(a)) * 256.f;
     }
 }
 
@@ -111,7 +112,8 @@ template <typename P> __host__ __device__ constexpr int64_t row_elements(int64_t
 // What a launch computes with its tiles.
 enum {
     kStats = 0,  // maxima and sums of the logits' exponentials
-    kKeep = 1,   // the same, and the exponentials themselves, relative to their tile's maximum, where P will be
+    kKeep = 1,   // the same, and the exponentials themselves, relative to their tile's maximum, where P will be (of float32 as
+                 // they are, 32 of them in the first 128 of the 192 bytes that their planes will take)
     kProb = 2,   // P, from finished sums
     kOut = 3     // a gradient
 };
@@ -356,14 +358,14 @@ struct Gather {
         const int piece = col / kPer ^ (row & kMask);
         return lds + (row * kPieces + piece) * 16 + col % kPer * (int)sizeof(S);
     }
-    // `row_at(r)` is where row r goes, or NULL; `cols` of it exist
-    template <int THREADS, typename ROW>
+    // `row_at(r)` is where row r goes, or NULL; `cols` of it exist, and of every TURN only the first FILLED
+    template <int THREADS, int FILLED = 1, int TURN = 1, typename ROW>
     __device__ static __forceinline__ void leave(char *lds, int rows, int cols, ROW row_at)
     {
         for (int i = threadIdx.x; i < rows * kPieces; i += THREADS) {
             const int row = i / kPieces, col = i % kPieces * kPer;
             S *to = row_at(row);
-            if (!to || col >= cols) continue;
+            if (!to || col >= cols || col % TURN >= FILLED) continue;
             to += col;
             const Vec<S, kPer> v = *(const Vec<S, kPer> *)at(lds, row, col);
             if (col + kPer <= cols && (uintptr_t)to % 16 == 0) {
@@ -679,12 +681,14 @@ __device__ __forceinline__ void product_tile(const Args &g, const int block, cha
         typedef Gather<uint16_t, BM * NP> Out;
         static_assert(KIND == kOut || kRowsOut * BM * NP * 2 <= kStagesBytes<P, BM, BN, STAGES>, "");
         const int m = m_in + m_of(I);
-        if constexpr (NP == 1) {
+        if constexpr (NP > 1 && KIND == kKeep) {
+            *(f32x4 *)Out::at(lds, row_out, (m >> 5) * 96 + (m & 31) * 2) = f32x4{p[0], p[1], p[2], p[3]};
+        } else if constexpr (NP == 1) {
             *(s16x4 *)Out::at(lds, row_out, m) = round4<P>(f32x4{p[0], p[1], p[2], p[3]} * (P::half ? kProbScale : 1.f));
         } else {
             bf16_t planes[4][3];
 #pragma unroll
-            for (int r = 0; r < 4; ++r) split_planes(p[r], planes[r]);
+            for (int r = 0; r < 4; ++r) split_planes<true>(p[r], planes[r]);
 #pragma unroll
             for (int q = 0; q < NP; ++q) {
                 const Vec<bf16_t, 4> o{{planes[0][q], planes[1][q], planes[2][q], planes[3][q]}};
@@ -694,7 +698,8 @@ __device__ __forceinline__ void product_tile(const Args &g, const int block, cha
     };
     auto leave_prob = [&](int j) {
         __syncthreads();
-        Gather<uint16_t, BM * NP>::template leave<kThreads>(lds, kRowsOut, (g.prob_words - m0) * NP, [&](int row) -> uint16_t * {
+        constexpr int kFilled = NP > 1 && KIND == kKeep ? 64 : 96;  // of three planes' place
+        Gather<uint16_t, BM * NP>::template leave<kThreads, kFilled, 96>(lds, kRowsOut, (g.prob_words - m0) * NP, [&](int row) -> uint16_t * {
             const int t = n0 + n_of(row, j);
             return t < g.N ? (uint16_t *)g.prob + t * g.ldp + m0 * NP : nullptr;
         });

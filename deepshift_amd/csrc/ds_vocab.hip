@@ -239,7 +239,8 @@ __global__ __launch_bounds__(1024) void row_scale_kernel(const float *__restrict
 // 16-bit exponentials have been rounded once, and their probabilities are once more: bfloat16 gradients are 0.0021 of their norm
 // off instead of 0.0017, float16 ones 0.00022 instead of 0.00021, for one product less of four (float16 in place of bfloat16 would
 // hold nothing below 2^-39 of a tile's largest).
-// Bound by memory: 2048 x 32768 in three planes in 161 us, 0.8 GB at 5 TB/s, where forming the logits again takes 830.
+// Bound by memory: 2048 x 32768 float32 exponentials to three planes in 155 us, 0.67 GB at 4.3 TB/s, where forming the logits
+// again takes 830.
 struct Finish {
     void *prob;
     int64_t ldp;
@@ -315,6 +316,7 @@ __global__ __launch_bounds__(256) void finish_kernel(Finish f)
     for (int e = 0; e < 8; ++e) over_t[e] = 0.f;
     const float2 *tops = r.stats + (int64_t)(word < f.words ? word / f.tile : 0) * r.T;
     uint16_t *const column = (uint16_t *)f.prob + (NP == 1 ? word : (word >> 5) * 96 + (word & 31));
+    const float *const kept = (const float *)((uint16_t *)f.prob + (word >> 5) * 96) + (word & 31);  // of float32
 #pragma unroll JOIN ? 1 : 4
     for (int i = 0; i < f.rows; i += 8) {
         const int t = blockIdx.y * f.rows + i + part;
@@ -324,16 +326,18 @@ __global__ __launch_bounds__(256) void finish_kernel(Finish f)
         if (word >= f.words) continue;
         Vec<uint16_t, 8> *const at = (Vec<uint16_t, 8> *)(column + t * f.ldp);
         Vec<uint16_t, 8> v[NP];
-#pragma unroll
-        for (int q = 0; q < NP; ++q) v[q] = at[q * 4];
+        f32x4 e32[2];
+        // four neighbouring lanes' planes take the place of all their exponentials: each lane needs both of its loads for
+        // any store, and a wave's loads are one instruction
+        if constexpr (NP == 3) e32[0] = *(const f32x4 *)(kept + t * (f.ldp / 2)), e32[1] = *(const f32x4 *)(kept + t * (f.ldp / 2) + 4);
+        else v[0] = at[0];
         // rows that do not count leave nothing; a target that is no word leaves no number
         const float factor = y == r.ignore ? 0.f : y < 0 || y >= r.V ? NAN : exp2f(tops[t].x - lse);
         float p[8];
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
             if constexpr (NP == 3)
-                p[e] = to_float(bf16_t{v[0].v[e]}) +
-                       (to_float(bf16_t{v[1].v[e]}) + to_float(bf16_t{v[2].v[e]}) * (1.f / 256)) * (1.f / 256);
+                p[e] = e32[e / 4][e % 4];
             else if constexpr (P::half)
                 p[e] = to_float(f16_t{v[0].v[e]}) * (1.f / kProbScale);
             else
@@ -351,7 +355,7 @@ __global__ __launch_bounds__(256) void finish_kernel(Finish f)
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
                 bf16_t planes[3];
-                split_planes(p[e], planes);
+                split_planes<true>(p[e], planes);
 #pragma unroll
                 for (int q = 0; q < 3; ++q) v[q].v[e] = planes[q].bits;
             }
