@@ -6,9 +6,9 @@
 // The logits are never stored: the forward pass keeps a maximum and a sum of exponentials per tile (a pair for every 32 to 256
 // of them), the backward pass computes the logits of a piece of the vocabulary again, leaves that piece's P in a workspace of
 // a bounded size, and forms both gradients from it: four products of 2 T D V operations for a step, of which three are the
-// formula's own.  Where one piece is the whole vocabulary and loss and gradients are asked for in one call, the forward pass
-// leaves the exponentials, relative to their tiles' maxima, in that workspace, and a pass over them makes them P: three
-// products.
+// formula's own.  Where loss and gradients are asked for in one call, the forward pass leaves the last piece's exponentials,
+// relative to their tiles' maxima, in that workspace, and a pass over them makes them P: three products for that piece, which
+// may be the whole vocabulary.
 #include "ds_vocab.h"
 
 namespace ds {
@@ -246,8 +246,11 @@ struct Finish {
     int64_t ldp;
     int words, tile;       // words of a row, a multiple of 32; words a tile of the logits had
     int rows;              // of a workgroup, a multiple of 8
+    int64_t v0, n;         // the piece: its first word, and how many there are
+    int tile0;             // and its first tile
+    int ld_bias_part;
     Rows of;
-    float *bias_part;      // [workgroups along T][words], or NULL
+    float *bias_part;      // [workgroups along T][ld_bias_part], or NULL
     void *bias_out;        // one workgroup has all rows: the gradient itself, of V words, or NULL
     const float *factor[2];
 };
@@ -314,7 +317,7 @@ __global__ __launch_bounds__(256) void finish_kernel(Finish f)
     float over_t[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) over_t[e] = 0.f;
-    const float2 *tops = r.stats + (int64_t)(word < f.words ? word / f.tile : 0) * r.T;
+    const float2 *tops = r.stats + (int64_t)(f.tile0 + (word < f.words ? word / f.tile : 0)) * r.T;
     uint16_t *const column = (uint16_t *)f.prob + (NP == 1 ? word : (word >> 5) * 96 + (word & 31));
     const float *const kept = (const float *)((uint16_t *)f.prob + (word >> 5) * 96) + (word & 31);  // of float32
 #pragma unroll JOIN ? 1 : 4
@@ -344,10 +347,11 @@ __global__ __launch_bounds__(256) void finish_kernel(Finish f)
                 p[e] = to_float(bf16_t{v[0].v[e]});
             p[e] = y == r.ignore ? 0.f : p[e] * factor;
         }
-        if (y >= word && y < word + 8 && y != r.ignore) {
+        const int64_t here = y - f.v0 - word;
+        if (here >= 0 && here < 8 && word + here < f.n && y != r.ignore) {
             const float hot = exp2f(r.picked[t] - lse) - 1.f;
 #pragma unroll
-            for (int e = 0; e < 8; ++e) p[e] = y == word + e ? hot : p[e];
+            for (int e = 0; e < 8; ++e) p[e] = here == e ? hot : p[e];
         }
 #pragma unroll
         for (int e = 0; e < 8; ++e) over_t[e] += p[e];
@@ -376,12 +380,12 @@ __global__ __launch_bounds__(256) void finish_kernel(Finish f)
     for (int e = 0; e < 8; ++e) sums[part][lane * 8 + e] = over_t[e];
     __syncthreads();
     const int v = blockIdx.x * 256 + threadIdx.x;
-    if (v >= r.V) return;
+    if (v >= f.n) return;
     float s = 0.f;
 #pragma unroll
     for (int w = 0; w < 8; ++w) s += sums[w][threadIdx.x];
     if (f.bias_out) ((E *)f.bias_out)[v] = from_float<E>(s * factor_of(f.factor));
-    else f.bias_part[(int64_t)blockIdx.y * f.words + v] = s;
+    else f.bias_part[(int64_t)blockIdx.y * f.ld_bias_part + v] = s;
 }
 
 // ---- joins -------------------------------------------------------------------------------------------------------
@@ -485,7 +489,7 @@ struct Plan {
     int64_t ldd;          // and what their rows take
     int64_t piece, pieces;
     bool pack_h, pack_w;
-    bool keep;            // the loss's exponentials become the gradients' probabilities (run may decide against it)
+    bool keep;            // the last piece's exponentials become its probabilities (run may decide against it)
     int tile_logits;
     Choice hidden, weight;
     int words;            // of a piece's probabilities, a multiple of 32,
@@ -521,7 +525,7 @@ Plan plan_of(const void *hidden, int64_t ldh, const void *weight, int64_t ldw, i
     p.piece = ((V + p.pieces - 1) / p.pieces + 255) / 256 * 256;
     if (p.piece > V) p.piece = V;
     p.pieces = (V + p.piece - 1) / p.piece;
-    p.keep = what == (kLoss | kGrad) && p.pieces == 1 && T <= 65535 * 8;
+    p.keep = what == (kLoss | kGrad) && T <= 65535 * 8;
     p.tile_logits = choose<P>(p.piece, T, D, kShapes, 1, what & kGrad).tile;
     size_t at = 0;
     auto take = [&](size_t n) {
@@ -630,7 +634,7 @@ Args logit_args(const Call &c, const Plan &p, int64_t v0, int64_t n, const Opera
 
 // Whether finish_kernel joins the rows' sums: each of its workgroups does it for its own rows, and one for all, which pays
 // while there are few of both (64 tokens, 1000 words, float32: 3 us of a step).
-inline bool joined_later(const Plan &p, int64_t T, int tiles) { return p.keep && T <= 128 && tiles <= 64; }
+inline bool joined_later(const Plan &p, int64_t T, int tiles) { return p.keep && p.pieces == 1 && T <= 128 && tiles <= 64; }
 
 template <typename P>
 int loss(const Call &c, const Plan &p, bool counted_only, Operands<P> &o, int reduction, float *rows, float *lse, float *total,
@@ -649,7 +653,7 @@ int loss(const Call &c, const Plan &p, bool counted_only, Operands<P> &o, int re
         g.picked = (float *)(c.ws + p.picked);
         g.arrived = (uint32_t *)(c.ws + p.arrived);
         g.prob = c.ws + p.prob, g.ldp = p.ldp, g.prob_words = p.words;
-        DS_TRY(launch_product<P>(p.keep ? kLogitKeep : kLogitStats, p.tile_logits, g, nullptr, c.st));
+        DS_TRY(launch_product<P>(p.keep && v0 + n == c.V ? kLogitKeep : kLogitStats, p.tile_logits, g, nullptr, c.st));
         tiles += g.tiles_m;
     }
     *of = Rows{(const float2 *)(c.ws + p.stats), (const float *)(c.ws + p.picked), tiles, (int)c.T, c.target, c.wide, c.V, c.ignore,
@@ -675,23 +679,26 @@ int loss_grad(const Call &c, const Plan &p, Operands<P> &o, const Rows &of, Grad
         r.grad = (const float *)(c.ws + p.factor);
     }
     float *const slices = (float *)(c.ws + p.slices);
-    for (int64_t v0 = 0; v0 < c.V; v0 += p.piece) {
+    // the last piece first: its exponentials may be there, and its weights are
+    for (int64_t i = 0; i < p.pieces; ++i) {
+        const int64_t v0 = (i == 0 ? p.pieces - 1 : i - 1) * p.piece;
         const int64_t n = c.V - v0 < p.piece ? c.V - v0 : p.piece;
-        const bool first = v0 == 0, last = v0 + n == c.V;
+        const bool first = i == 0, last = i == p.pieces - 1, kept = p.keep && i == 0;
         int bias_tiles = 0;
         bool bias_left = r.dbias != nullptr;
         const Operand prob{c.ws + p.prob, p.ldp};
         if (c.T > 0) {
-            const int rows = p.keep ? finish_rows(c.T, p.words) : Shapes<P>::n[p.tile_logits];
+            const int rows = kept ? finish_rows(c.T, p.words) : Shapes<P>::n[p.tile_logits];
             bias_tiles = (int)((c.T + rows - 1) / rows);
             // the sums of one workgroup are the gradient, but for the share that a launch which joins the rows only finds
             bias_left = r.dbias && (bias_tiles > 1 || joined_later(p, c.T, of.tiles));
             float *const bias_part = bias_left ? (float *)(c.ws + p.bias) : nullptr;
             void *const bias_out = r.dbias && !bias_left ? (E *)r.dbias + v0 : nullptr;
-            if (p.keep) {
-                const Finish f{c.ws + p.prob, p.ldp, p.words, Shapes<P>::m[p.tile_logits], rows, of,
+            if (kept) {
+                const int tile = Shapes<P>::m[p.tile_logits], words = ceil_div((int)n, 32) * 32;
+                const Finish f{c.ws + p.prob, p.ldp, words, tile, rows, v0, n, of.tiles - ceil_div((int)n, tile), p.words, of,
                                bias_part, bias_out, {r.grad, r.share}};
-                const unsigned along = ceil_div(p.words, 256), down = ceil_div((int)c.T, rows);
+                const unsigned along = ceil_div(words, 256), down = ceil_div((int)c.T, rows);
                 if (joined_later(p, c.T, of.tiles))
                     hipLaunchKernelGGL((finish_kernel<P, true>), dim3(along, down + 1), dim3(256), 0, c.st, f);
                 else

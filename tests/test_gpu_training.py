@@ -245,6 +245,26 @@ def test_cross_entropy_in_pieces_and_stretches(dtype):
 
 
 @pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("bias", [False, True])
+def test_cross_entropy_keeps_the_last_piece(dtype, bias):
+    # targets in every piece, the last piece shorter than the others, or of a single word, or of a whole tile
+    for T, D, V in [(70, 40, 517), (129, 64, 1025), (8, 24, 768), (300, 33, 900)]:
+        g = _gen(T, D, V, 7)
+        h, w, b, y = _head(T, D, V, dtype, bias, g)
+        y[0], y[1], y[T // 2] = V - 1, 0, 256
+        y[2::7] = -100
+        kept = int((y != -100).sum())
+        for tile in (0, 1, 2, 3):
+            print(T, D, V, tile, flush=True)
+            with Tune(vocab_tile=tile, vocab_piece_kb=1):
+                rows = training.linear_cross_entropy(h, w, y, b, reduction="none")
+                loss, dh, dw, db = training.linear_cross_entropy_grad(h, w, y, b)
+                again = training.linear_cross_entropy_grad(h, w, y, b)
+            _head_check(h, w, b, y, -100, torch.full((T,), 1.0 / kept, device=DEV), rows, dh, dw, db)
+            assert all(x is z or torch.equal(x, z) for x, z in zip((loss, dh, dw, db), again))
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
 def test_cross_entropy_layouts(dtype):
     g = _gen(11)
     h, w, b, y = _head(60, 64, 301, dtype, True, g)
