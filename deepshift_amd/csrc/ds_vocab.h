@@ -912,6 +912,11 @@ template <typename P> constexpr int kGradShapes = P::planes == 1 ? 4 : 3;
 // one launch, both with that shape (g is kHidden, *other kWeight).  A translation unit per P.
 template <typename P> int launch_product(int kind, int tile, Args &g, Args *other, hipStream_t st);
 
+// The same for up to kFewTokens tokens of float32, with operands that lie as the caller's do (P excepted); the logits' tiles are
+// kFewWords words of all tokens, hidden gradients always go to slices.
+constexpr int kFewTokens = 16, kFewWords = 32;
+int launch_few(int kind, int tokens, Args &g, hipStream_t st);
+
 template <typename P, int BM, int BN, int WM, int WN, int STAGES, bool GRADS = true>
 int launch_tiled(int kind, Args &g, Args *other, hipStream_t st)
 {

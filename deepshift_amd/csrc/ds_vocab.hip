@@ -10,6 +10,7 @@
 // relative to their tiles' maxima, in that workspace, and a pass over them makes them P: three products for that piece, which
 // may be the whole vocabulary.
 #include "ds_vocab.h"
+#include <algorithm>
 
 namespace ds {
 namespace vocab {
@@ -490,7 +491,8 @@ struct Plan {
     int64_t piece, pieces;
     bool pack_h, pack_w;
     bool keep;            // the last piece's exponentials become its probabilities (run may decide against it)
-    int tile_logits;
+    bool few;             // ds_vocab_few.hip's kernels
+    int tile_logits, tile_words, tile_tokens;
     Choice hidden, weight;
     int words;            // of a piece's probabilities, a multiple of 32,
     int64_t ldp;          // and what a row of them takes
@@ -498,6 +500,10 @@ struct Plan {
 };
 
 inline bool in_place(const void *p, int64_t ld, int64_t D) { return (uintptr_t)p % 16 == 0 && ld % 8 == 0 && D % 8 == 0; }
+
+// Up to how many tokens of float32 read the weights as they are.  Small heads give each workgroup too little to read: 16 tokens of
+// 512 features, 1000 words, 44 us a step where planes take 33 (8 tokens: 31 and 34), 16 of 1024, 8000 words, 74 and 78.
+inline int64_t few_tokens(int64_t weights) { return weights < 1 << 23 ? kFewTokens / 2 : kFewTokens; }
 
 // What a call does: the loss, the gradients, or both.
 enum { kLoss = 1, kGrad = 2 };
@@ -509,8 +515,9 @@ Plan plan_of(const void *hidden, int64_t ldh, const void *weight, int64_t ldw, i
     Plan p{};
     p.Dp = (int)(NP > 1 ? (D + 31) / 32 * 32 : (D + 7) / 8 * 8);
     p.ldd = row_elements<P>(D);
-    p.pack_h = NP > 1 || what & kGrad || !in_place(hidden, ldh, D);  // for gradients: without the rows that do not count
-    p.pack_w = NP > 1 || !in_place(weight, ldw, D);
+    p.few = NP > 1 && T > 0 && T <= few_tokens(V * D) && g_tune.vocab_tile == kTuneUnset;
+    p.pack_h = !p.few && (NP > 1 || what & kGrad || !in_place(hidden, ldh, D));  // for gradients: without the rows that do not count
+    p.pack_w = !p.few && (NP > 1 || !in_place(weight, ldw, D));
     const int kb = g_tune.vocab_piece_kb;
     const size_t piece_bytes = kb == kTuneUnset ? kPieceBytes : (size_t)kb << 10;
     int64_t most = V;
@@ -526,7 +533,9 @@ Plan plan_of(const void *hidden, int64_t ldh, const void *weight, int64_t ldw, i
     if (p.piece > V) p.piece = V;
     p.pieces = (V + p.piece - 1) / p.piece;
     p.keep = what == (kLoss | kGrad) && T <= 65535 * 8;
-    p.tile_logits = choose<P>(p.piece, T, D, kShapes, 1, what & kGrad).tile;
+    p.tile_logits = p.few ? 0 : choose<P>(p.piece, T, D, kShapes, 1, what & kGrad).tile;
+    p.tile_words = p.few ? kFewWords : Shapes<P>::m[p.tile_logits];
+    p.tile_tokens = p.few ? kFewTokens : Shapes<P>::n[p.tile_logits];
     size_t at = 0;
     auto take = [&](size_t n) {
         const size_t was = at;
@@ -536,7 +545,7 @@ Plan plan_of(const void *hidden, int64_t ldh, const void *weight, int64_t ldw, i
     if (p.pack_h) p.h = take((size_t)T * p.ldd * 2);
     if (p.pack_w) p.w = take((size_t)p.piece * p.ldd * 2);
     if (what & kLoss) {
-        const int64_t tiles = (p.piece + Shapes<P>::m[p.tile_logits] - 1) / Shapes<P>::m[p.tile_logits];
+        const int64_t tiles = (p.piece + p.tile_words - 1) / p.tile_words;
         p.stats = take((size_t)(tiles * p.pieces) * T * 8);
         p.picked = take((size_t)T * 4);
         p.shares = take((size_t)((T + kRowsJoined - 1) / kRowsJoined) * sizeof(Share));
@@ -545,15 +554,21 @@ Plan plan_of(const void *hidden, int64_t ldh, const void *weight, int64_t ldw, i
     if (what & kGrad) {
         p.words = (int)((p.piece + 31) / 32 * 32);
         p.ldp = p.words * (int64_t)NP;
-        p.hidden = choose<P>(D, T, p.piece, kGradShapes<P>, 64, false);
-        p.weight = choose<P>(D, p.piece, T, kGradShapes<P>, 64, false);
+        if (p.few) {
+            // four workgroups a CU, with 16 words at least
+            const int64_t across = D > 0 ? (D + 255) / 256 : 1;
+            p.hidden.splits = (int)std::min({(int64_t)64, (4 * device_cus() + across - 1) / across, (p.piece + 15) / 16});
+            p.weight.splits = 1;
+        } else {
+            p.hidden = choose<P>(D, T, p.piece, kGradShapes<P>, 64, false);
+            p.weight = choose<P>(D, p.piece, T, kGradShapes<P>, 64, false);
+        }
         p.prob = take((size_t)T * p.ldp * 2);
         // what a workgroup of either pass leaves of its rows
-        const int tile_rows = Shapes<P>::n[p.tile_logits], kept_rows = finish_rows(T, p.words);
-        const int rows = p.keep && kept_rows < tile_rows ? kept_rows : tile_rows;
+        const int kept_rows = finish_rows(T, p.words), rows = p.keep && kept_rows < p.tile_tokens ? kept_rows : p.tile_tokens;
         p.bias = take((size_t)((T + rows - 1) / rows) * p.words * 4);
         size_t slices = 0;
-        if (p.hidden.splits > 1 || p.pieces > 1) slices = (size_t)p.hidden.splits * T * D * 4;
+        if (p.few || p.hidden.splits > 1 || p.pieces > 1) slices = (size_t)p.hidden.splits * T * D * 4;
         if (p.weight.splits > 1) {
             const size_t n = (size_t)p.weight.splits * p.piece * D * 4;
             slices = n > slices ? n : slices;
@@ -624,7 +639,7 @@ Args logit_args(const Call &c, const Plan &p, int64_t v0, int64_t n, const Opera
 {
     Args g{};
     g.a = o.w, g.b = o.h;
-    g.M = (int)n, g.N = (int)c.T, g.K = p.Dp;
+    g.M = (int)n, g.N = (int)c.T, g.K = p.few ? (int)c.D : p.Dp;
     g.splits = 1, g.k_split = (p.Dp + P::step - 1) / P::step * P::step;
     g.bias = c.bias, g.bias_type = c.type;
     g.target = c.target, g.target_wide = c.wide;
@@ -635,6 +650,13 @@ Args logit_args(const Call &c, const Plan &p, int64_t v0, int64_t n, const Opera
 // Whether finish_kernel joins the rows' sums: each of its workgroups does it for its own rows, and one for all, which pays
 // while there are few of both (64 tokens, 1000 words, float32: 3 us of a step).
 inline bool joined_later(const Plan &p, int64_t T, int tiles) { return p.keep && p.pieces == 1 && T <= 128 && tiles <= 64; }
+
+// One product, of `kind`, by the kernels of the plan; fills in the tile counts.
+template <typename P>
+int product(const Plan &p, int kind, int tile, Args &g, int64_t T, hipStream_t st)
+{
+    return p.few ? launch_few(kind, (int)T, g, st) : launch_product<P>(kind, tile, g, nullptr, st);
+}
 
 template <typename P>
 int loss(const Call &c, const Plan &p, bool counted_only, Operands<P> &o, int reduction, float *rows, float *lse, float *total,
@@ -653,7 +675,7 @@ int loss(const Call &c, const Plan &p, bool counted_only, Operands<P> &o, int re
         g.picked = (float *)(c.ws + p.picked);
         g.arrived = (uint32_t *)(c.ws + p.arrived);
         g.prob = c.ws + p.prob, g.ldp = p.ldp, g.prob_words = p.words;
-        DS_TRY(launch_product<P>(p.keep && v0 + n == c.V ? kLogitKeep : kLogitStats, p.tile_logits, g, nullptr, c.st));
+        DS_TRY(product<P>(p, p.keep && v0 + n == c.V ? kLogitKeep : kLogitStats, p.tile_logits, g, c.T, c.st));
         tiles += g.tiles_m;
     }
     *of = Rows{(const float2 *)(c.ws + p.stats), (const float *)(c.ws + p.picked), tiles, (int)c.T, c.target, c.wide, c.V, c.ignore,
@@ -688,16 +710,16 @@ int loss_grad(const Call &c, const Plan &p, Operands<P> &o, const Rows &of, Grad
         bool bias_left = r.dbias != nullptr;
         const Operand prob{c.ws + p.prob, p.ldp};
         if (c.T > 0) {
-            const int rows = kept ? finish_rows(c.T, p.words) : Shapes<P>::n[p.tile_logits];
+            const int rows = kept ? finish_rows(c.T, p.words) : p.tile_tokens;
             bias_tiles = (int)((c.T + rows - 1) / rows);
             // the sums of one workgroup are the gradient, but for the share that a launch which joins the rows only finds
             bias_left = r.dbias && (bias_tiles > 1 || joined_later(p, c.T, of.tiles));
             float *const bias_part = bias_left ? (float *)(c.ws + p.bias) : nullptr;
             void *const bias_out = r.dbias && !bias_left ? (E *)r.dbias + v0 : nullptr;
             if (kept) {
-                const int tile = Shapes<P>::m[p.tile_logits], words = ceil_div((int)n, 32) * 32;
-                const Finish f{c.ws + p.prob, p.ldp, words, tile, rows, v0, n, of.tiles - ceil_div((int)n, tile), p.words, of,
-                               bias_part, bias_out, {r.grad, r.share}};
+                const int words = ceil_div((int)n, 32) * 32;
+                const Finish f{c.ws + p.prob, p.ldp, words, p.tile_words, rows, v0, n, of.tiles - ceil_div((int)n, p.tile_words),
+                               p.words, of, bias_part, bias_out, {r.grad, r.share}};
                 const unsigned along = ceil_div(words, 256), down = ceil_div((int)c.T, rows);
                 if (joined_later(p, c.T, of.tiles))
                     hipLaunchKernelGGL((finish_kernel<P, true>), dim3(along, down + 1), dim3(256), 0, c.st, f);
@@ -712,7 +734,7 @@ int loss_grad(const Call &c, const Plan &p, Operands<P> &o, const Rows &of, Grad
                 g.factor[0] = r.grad, g.factor[1] = r.share;
                 g.bias_out = bias_out, g.bias_part = bias_part;
                 g.ld_bias_part = p.words;
-                DS_TRY(launch_product<P>(kLogitProb, p.tile_logits, g, nullptr, c.st));
+                DS_TRY(product<P>(p, kLogitProb, p.tile_logits, g, c.T, c.st));
             }
         }
         BiasJoin bias{(const float *)(c.ws + p.bias), p.words, bias_tiles, (int)n, r.dbias ? (E *)r.dbias + v0 : nullptr};
@@ -741,20 +763,22 @@ int loss_grad(const Call &c, const Plan &p, Operands<P> &o, const Rows &of, Grad
             x.ldo = c.D;
             x.splits = which ? p.weight.splits : p.hidden.splits;
             x.k_split = ((x.K + x.splits - 1) / x.splits + P::step - 1) / P::step * P::step;
-            joined[which] = x.splits > 1 || (!which && p.pieces > 1);
+            if (p.few) x.k_split = ceil_div(x.K, x.splits);
+            x.target = c.target, x.target_wide = c.wide, x.ignore = c.ignore;
+            joined[which] = x.splits > 1 || (!which && (p.pieces > 1 || p.few));
             x.slice = joined[which] ? slices : nullptr;
         }
         // few workgroups each, and no slices to share: both in one launch
         const int tm = Shapes<P>::m[p.weight.tile], tn = Shapes<P>::n[p.weight.tile];
         const int64_t across = (int64_t)ceil_div((int)c.T, tn) * p.hidden.splits + ceil_div((int)n, tn);
         const int64_t blocks = ceil_div((int)c.D, tm) * across;
-        const bool both = wanted[0] && wanted[1] && !joined[1] && p.hidden.tile == p.weight.tile && blocks <= 2 * device_cus();
+        const bool both = !p.few && wanted[0] && wanted[1] && !joined[1] && p.hidden.tile == p.weight.tile && blocks <= 2 * device_cus();
         if (both) DS_TRY(launch_product<P>(kHidden, p.weight.tile, g[0], &g[1], c.st));
         for (int which = 0; which < 2; ++which) {
             Args &x = g[which];
             if (!wanted[which]) continue;
             const int tile = which ? p.weight.tile : p.hidden.tile;
-            if (!both) DS_TRY(launch_product<P>(which ? kWeight : kHidden, tile, x, nullptr, c.st));
+            if (!both) DS_TRY(product<P>(p, which ? kWeight : kHidden, tile, x, c.T, c.st));
             if (!joined[which]) continue;
             const int64_t count = (int64_t)x.n_store * c.D;
             const int64_t all = (count + 255) / 256;

@@ -264,6 +264,57 @@ def test_cross_entropy_keeps_the_last_piece(dtype, bias):
             assert all(x is z or torch.equal(x, z) for x, z in zip((loss, dh, dw, db), again))
 
 
+@pytest.mark.parametrize("T", [1, 2, 3, 4, 5, 8, 9, 15, 16, 17])
+def test_cross_entropy_of_a_few_tokens(T):
+    # features around a wave's 256, words around a workgroup's 32, rows at every alignment
+    for i, (D, V) in enumerate([(1, 1), (3, 2), (4, 31), (5, 33), (255, 64), (256, 65), (257, 1000), (700, 300), (1030, 2085),
+                               (1030, 8201)]):
+        print(T, D, V, flush=True)
+        g = _gen(T, D, V, 5)
+        h, w, b, y = _head(T, D, V, torch.float32, i % 2 == 0, g)
+        y[0] = V - 1
+        if T > 2:
+            y[1::4] = -100
+            h[1::4] = float("nan")
+        kept = int((y != -100).sum())
+        clean = torch.where((y != -100)[:, None], h, torch.zeros_like(h))
+        wide_h, wide_w = torch.full((T, D + 3), float("nan"), device=DEV), torch.full((V, D + 1), float("inf"), device=DEV)
+        wide_h[:, 2:D + 2], wide_w[:, 1:] = h, w
+        share = torch.full((T,), 1.0 / kept, device=DEV)
+        for hh, ww, tune in ((h, w, {}), (wide_h[:, 2:D + 2], wide_w[:, 1:], {}), (h, w, dict(vocab_piece_kb=1))):
+            with Tune(**tune):
+                rows = training.linear_cross_entropy(hh, ww, y, b, reduction="none")
+                loss, dh, dw, db = training.linear_cross_entropy_grad(hh, ww, y, b)
+                again = training.linear_cross_entropy_grad(hh, ww, y, b)
+            _head_check(clean, w, b, y, -100, share, rows, dh, dw, db)
+            assert (dh[y == -100] == 0).all()
+            assert all(x is z or torch.equal(x, z) for x, z in zip((loss, dh, dw, db), again))
+        # the gradients by themselves, of rows with gradients of their own
+        grads = _rand(g, T)
+        leaves = [x.detach().requires_grad_() for x in (h, w) + ((b,) if b is not None else ())]
+        training.linear_cross_entropy(leaves[0], leaves[1], y, *leaves[2:], reduction="none").backward(grads)
+        _head_check(clean, w, b, y, -100, grads, rows, leaves[0].grad, leaves[1].grad, leaves[2].grad if b is not None else None)
+
+
+def test_cross_entropy_of_a_few_tokens_with_words_taken_out():
+    g = _gen(8, 8)
+    h, w, b, y = _head(6, 20, 200, torch.float32, True, g)
+    b[30:170] = float("-inf")
+    y = y % 30
+    rows = training.linear_cross_entropy(h, w, y, b, reduction="none")
+    loss, dh, dw, db = training.linear_cross_entropy_grad(h, w, y, b, reduction="sum")
+    _head_check(h, w, b, y, -100, torch.ones(6, device=DEV), rows, dh, dw, db)
+    assert (dw[30:170] == 0).all() and (db[30:170] == 0).all()
+    assert training.linear_cross_entropy(h, w, torch.full_like(y, 100), b, reduction="none").isposinf().all()
+    assert training.linear_cross_entropy(h, w, y, torch.full_like(b, float("-inf")), reduction="none").isnan().all()
+    # logits far apart
+    h, w = h * 2.0 ** 30, w * 2.0 ** 40
+    rows = training.linear_cross_entropy(h, w, y, b, reduction="none")
+    s = h.double() @ w.double().t() + b.double()
+    size = (h.abs().double() @ w.abs().double().t())[:, :30].amax(1) + (h.abs().double() @ w.abs().double().t())[:, 170:].amax(1)
+    _within(rows, s.logsumexp(1) - s.gather(1, y[:, None])[:, 0], 2 * 28 * E * size + 8 * E * size, "loss")
+
+
 @pytest.mark.parametrize("dtype", TYPES, ids=str)
 def test_cross_entropy_layouts(dtype):
     g = _gen(11)
