@@ -109,6 +109,9 @@ template <typename P> __host__ __device__ constexpr int64_t row_elements(int64_t
     return P::planes == 1 ? (n + 7) / 8 * 8 : (n + 31) / 32 * 96;
 }
 
+// Tiles of products that take float32 weights as they are.
+constexpr int kRawWords = 128, kRawTokens = 64;
+
 // What a launch computes with its tiles.
 enum {
     kStats = 0,  // maxima and sums of the logits' exponentials
@@ -298,6 +301,98 @@ struct Tile {
     }
 };
 
+// A stage of float32 weights as they are, whose fragments are split into planes on their way out of LDS: for few tokens, where
+// weights in planes would be written and read for little use.  Like a Tile, but for
+//   along k:  [row][32], rows of 128 bytes, whose 16-byte pieces are exchanged by row;
+//   across:   [k][ROWS], whose 64-byte pieces are exchanged by k / 8, so that the four groups of 16 lanes that read together
+//             meet other banks.
+// Rows and reductions are multiples of four.
+template <int ROWS, bool ACROSS, int WAVES>
+struct RawTile {
+    static constexpr int kStep = Split::step, kPlanes = 1;
+    static constexpr int bytes = ROWS * kStep * 4, fetches = bytes / 1024, mine = fetches / WAVES;
+    static_assert(fetches % WAVES == 0 && ROWS >= 64, "");
+
+    uint32_t offset[mine];
+    int k_at[mine];
+
+    __device__ static __forceinline__ int swapped(int row) { return row & 7; }
+    __device__ static __forceinline__ int swapped_across(int k) { return (k >> 3 & 3) << 2; }
+
+    __device__ void init(const Operand &o, int rows_left, int wave)
+    {
+        const int lane = threadIdx.x & 63;
+#pragma unroll
+        for (int i = 0; i < mine; ++i) {
+            const int p = (wave * mine + i) * 64 + lane;
+            if constexpr (!ACROSS) {
+                const int row = p / 8, piece = p % 8 ^ swapped(row);
+                k_at[i] = piece * 4;
+                offset[i] = row < rows_left ? (uint32_t)(row * o.ld * 4 + piece * 16) : kNothing;
+            } else {
+                const int k = p / (ROWS / 4), piece = p % (ROWS / 4) ^ swapped_across(k);
+                k_at[i] = k;
+                offset[i] = piece * 4 < rows_left ? (uint32_t)(k * o.ld * 4 + piece * 16) : kNothing;
+            }
+        }
+    }
+    __device__ __forceinline__ void one(uint64_t base, int k_left, uint32_t lds, int wave, int, int i) const
+    {
+        fetch(k_at[i] < k_left ? offset[i] : kNothing, buffer_at(base), lds + (wave * mine + i) * 1024);
+    }
+    __device__ __forceinline__ void stage(uint64_t base, int k_left, uint32_t lds, int wave) const
+    {
+#pragma unroll
+        for (int i = 0; i < mine; ++i) one(base, k_left, lds, wave, 0, i);
+    }
+    __device__ static __forceinline__ int64_t step_bytes(const Operand &o) { return ACROSS ? o.ld * kStep * 4 : kStep * 4; }
+    __device__ static __forceinline__ int64_t rows_bytes(const Operand &o, int rows)
+    {
+        return ACROSS ? (int64_t)rows * 4 : rows * o.ld * 4;
+    }
+
+    // 16 rows from r0 on, lane l's being row l % 16 and the eight k from 8 (l / 16) on
+    __device__ static __forceinline__ void load(const char *lds, int r0, float (&x)[8])
+    {
+        const int lane = threadIdx.x & 63, g = lane / 16, row = r0 + lane % 16;
+        if constexpr (!ACROSS) {
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+                const f32x4 v = *(const f32x4 *)(lds + row * 128 + (((2 * g + half) ^ swapped(row)) << 4));
+#pragma unroll
+                for (int e = 0; e < 4; ++e) x[half * 4 + e] = v[e];
+            }
+        } else {
+            const char *p = lds + g * 8 * ROWS * 4 + ((row / 4 ^ swapped_across(g * 8)) * 16 + row % 4 * 4);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) x[e] = *(const float *)(p + e * ROWS * 4);
+        }
+    }
+    // Planes of two of them.  EXACT: of all values; else of those below kLimit, and `top` becomes the largest.
+    static constexpr float kLimit = 0x1.fep127f;  // what rounds to infinity, and infinities
+    template <bool EXACT>
+    __device__ static __forceinline__ void split(const float (&x)[8], int e, s16x8 (&planes)[3], float &top)
+    {
+        float a = x[e], b = x[e + 1];
+        if constexpr (EXACT) {
+            bf16_t p[3], q[3];
+            split_planes(a, p), split_planes(b, q);
+#pragma unroll
+            for (int k = 0; k < 3; ++k) planes[k][e] = (short)p[k].bits, planes[k][e + 1] = (short)q[k].bits;
+            return;
+        }
+        typedef float f32x2 __attribute__((ext_vector_type(2)));
+        typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+        top = fmaxf(top, fmaxf(fabsf(a), fabsf(b)));
+#pragma unroll
+        for (int k = 0; k < 3; ++k) {
+            const uint32_t two = __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2{a, b}), bf16x2));
+            planes[k][e] = (short)two, planes[k][e + 1] = (short)(two >> 16);
+            a = (a - __uint_as_float(two << 16)) * 256.f, b = (b - __uint_as_float(two & 0xffff0000u)) * 256.f;
+        }
+    }
+};
+
 __device__ __forceinline__ float bias_at(const Args &a, int v)
 {
     if (!a.bias) return 0.f;
@@ -333,8 +428,8 @@ __device__ __forceinline__ void wait_for_stage()
 
 // LDS of a workgroup: the stages, and what the epilogue of the logits needs to know of its words and tokens, fetched before
 // the products start (one load after another behind them took half of a short reduction's time).
-template <typename P, int BM, int BN, int STAGES>
-constexpr int kStagesBytes = STAGES * P::planes * (BM + BN) * P::step * 2;
+template <typename P, int BM, int BN, int STAGES, bool RAW = false>
+constexpr int kStagesBytes = STAGES * P::step * (RAW ? BM * 4 + P::planes * BN * 2 : P::planes * (BM + BN) * 2);
 template <int BM, int BN>
 struct Known {
     float bias[BM];   // times log2 e; -inf for words past the end, which leave nothing that way
@@ -342,8 +437,8 @@ struct Known {
     float lse[BN];    // +inf for rows that do not count: theirs are probabilities of 0
     float scale[BN];
 };
-template <typename P, int BM, int BN, int STAGES, bool LOGITS>
-constexpr int kLdsBytes = kStagesBytes<P, BM, BN, STAGES> + (LOGITS ? (int)sizeof(Known<BM, BN>) : 0);
+template <typename P, int BM, int BN, int STAGES, bool LOGITS, bool RAW = false>
+constexpr int kLdsBytes = kStagesBytes<P, BM, BN, STAGES, RAW> + (LOGITS ? (int)sizeof(Known<BM, BN>) : 0);
 
 // Results on their way out: rows of COLS elements gathered in LDS, whose 16-byte pieces are exchanged by row, so that lanes
 // that each hold a few neighbours of another row do not meet in a bank; from there every row leaves as one stretch.  (Stored
@@ -413,16 +508,18 @@ __device__ __forceinline__ int spread_sums(float (&v)[ALL], int lane)
 // are read and stages fetched between rows of products, a few each: with all of them behind the barrier the matrix cores were
 // busy 55 % of the cycles instead of 70 to 85 (4.0 instead of 3.2 ms for the scores above).  32 x 32 instructions take half as
 // many issues as 16 x 16 ones at the same rate; float32 keeps the smaller ones, whose partial sums of the planes fit.
-template <typename P, int BM, int BN, int WM, int WN, bool A_ACROSS, bool B_ACROSS, int KIND, int STAGES>
+template <typename P, int BM, int BN, int WM, int WN, bool A_ACROSS, bool B_ACROSS, int KIND, int STAGES, bool RAW = false>
 __device__ __forceinline__ void product_tile(const Args &g, const int block, char *lds)
 {
     using U = Unit<P>;
     constexpr int WAVES = WM * WN, MT = BM / WM / U::size, NT = BN / WN / U::size, NP = P::planes;
     constexpr int kStep = P::step;
-    using TA = Tile<P, BM, A_ACROSS, WAVES>;
+    static_assert(!RAW || NP == 3, "");
+    using TA = typename std::conditional<RAW, RawTile<BM, A_ACROSS, WAVES>, Tile<P, BM, A_ACROSS, WAVES>>::type;
     using TB = Tile<P, BN, B_ACROSS, WAVES>;
-    constexpr int kStageBytes = NP * (TA::bytes + TB::bytes);
-    constexpr int kInFlight = NP * (TA::mine + TB::mine);  // loads of one stage and wave
+    constexpr int kBytesA = TA::kPlanes * TA::bytes, kStageBytes = kBytesA + NP * TB::bytes;
+    constexpr int kFetchesA = TA::kPlanes * TA::mine, kInFlight = kFetchesA + NP * TB::mine;  // loads of one stage and wave
+    static_assert(STAGES * kStageBytes == kStagesBytes<P, BM, BN, STAGES, RAW>, "");
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
     const int wm = wave % WM, wn = wave / WM;
 
@@ -445,7 +542,7 @@ __device__ __forceinline__ void product_tile(const Args &g, const int block, cha
     auto fetch_stage = [&](int slot) {
         const uint32_t to = lds0 + slot * kStageBytes;
         ta.stage(a_at, k_left, to, wave);
-        tb.stage(b_at, k_left, to + NP * TA::bytes, wave);
+        tb.stage(b_at, k_left, to + kBytesA, wave);
         a_at += a_step, b_at += b_step, k_left -= kStep;
     };
 
@@ -457,7 +554,7 @@ __device__ __forceinline__ void product_tile(const Args &g, const int block, cha
 #pragma unroll
             for (int r = 0; r < 4 * U::groups; ++r) acc[i][j][r] = 0.f;
 
-    Known<BM, BN> &known = *(Known<BM, BN> *)(lds + kStagesBytes<P, BM, BN, STAGES>);
+    Known<BM, BN> &known = *(Known<BM, BN> *)(lds + kStagesBytes<P, BM, BN, STAGES, RAW>);
     static_assert(BM <= WAVES * 64 && BN <= WAVES * 64, "a thread per word and token");
     constexpr int kNowhere = -(1 << 20);
     float bias = -INFINITY, lse = INFINITY, scale = 0.f;
@@ -542,124 +639,157 @@ __device__ __forceinline__ void product_tile(const Args &g, const int block, cha
             a_at += a_step, b_at += b_step, k_left -= kStep;
         }
     } else {
-        // Rows of tiles that are multiplied together: the six products of a tile follow each other, so four tiles at least have
-        // to take turns.  While one such group is multiplied the next one's fragments of A are read; during the last group of a
-        // stage, whose fragments are all there by then, the next stage's first ones, and its own slot is fetched anew.
-        constexpr int G = NT >= 4 || MT == 1 ? 1 : 2, kGroups = MT / G;
-        static_assert(MT % G == 0 && (kGroups == 1 || kGroups % 2 == 0), "");
-        constexpr int kTurns = 6, kFetches = NP * (TA::mine + TB::mine), kReads = NP * (NT + G);
-        s16x8 b0[NP][NT], b1[NP][NT], a0[G][NP], a1[G][NP], turn[G][NP];
-        auto read_a = [&](int from, int group, int n, s16x8 (&fa)[G][NP]) {
-            const int i = n / NP, p = n % NP;
-            fa[i][p] = TA::fragment(lds + from * kStageBytes + p * TA::bytes, (wm * MT + group * G + i) * U::size, 0);
-        };
-        auto read_b = [&](int from, int n, s16x8 (&fb)[NP][NT]) {
-            const int p = n / NT, j = n % NT;
-            fb[p][j] = TB::fragment(lds + from * kStageBytes + NP * TA::bytes + p * TB::bytes, (wn * NT + j) * U::size, 0);
-        };
-        // The products of 2^-16, the largest ones while those are made 2^-8, then the products of 2^-8; between(0) ..
-        // between(kTurns - 1) in between.  What they amount to joins the result during the first turns of the next group (of
-        // this one, where it is the only one): the matrix cores do not wait for either.
-        f32x4 low[2][G][NT];
-        auto join = [&](int group, int i, int j) {
-            f32x4 &c = acc[group * G + i][j];
+        float top = 0.f;  // of weights that are split here
+        // from the beginning again, for weights that the quick split does not do
+        auto restart = [&] {
+            asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+            __syncthreads();
+            const int64_t done = (int64_t)(steps + STAGES);
+            a_at -= done * a_step, b_at -= done * b_step, k_left = k_to - k_from, slot = 0;
 #pragma unroll
-            for (int r = 0; r < 4; ++r) c[r] = fmaf(low[group % 2][i][j][r], 1.f / 256, c[r]);
+            for (int i = 0; i < MT; ++i)
+#pragma unroll
+                for (int j = 0; j < NT; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
         };
-        auto multiply = [&](int group, const s16x8 (&fa)[G][NP], const s16x8 (&fb)[NP][NT], auto between) {
-            f32x4(&mine)[G][NT] = low[group % 2];
-            const int last = (group + kGroups - 1) % kGroups;
-            auto add = [&](int p, int q, auto besides) {
+        auto products = [&](auto exact) {
+            // Rows of tiles that are multiplied together: the six products of a tile follow each other, so four tiles at least have
+            // to take turns.  While one such group is multiplied the next one's fragments of A are read; during the last group of a
+            // stage, whose fragments are all there by then, the next stage's first ones, and its own slot is fetched anew.
+            constexpr int G = NT >= 4 || MT == 1 ? 1 : 2, kGroups = MT / G;
+            static_assert(MT % G == 0 && (kGroups == 1 || kGroups % 2 == 0), "");
+            constexpr int kTurns = 6, kFetches = kInFlight, kReads = NP * (NT + G);
+            s16x8 b0[NP][NT], b1[NP][NT], a0[G][NP], a1[G][NP], turn[G][NP];
+            float whole[G][8];  // of weights that are split here
+            auto read_a = [&](int from, int group, int n, s16x8 (&fa)[G][NP]) {
+                const int i = n / NP, p = n % NP;
+                const char *at = lds + from * kStageBytes;
+                if constexpr (RAW) {
+                    if (p == 0) TA::load(at, (wm * MT + group * G + i) * U::size, whole[i]);
+                } else {
+                    fa[i][p] = TA::fragment(at + p * TA::bytes, (wm * MT + group * G + i) * U::size, 0);
+                }
+            };
+            // two of the eight in turn t, 1 to 4
+            auto split_a = [&](int t, s16x8 (&fa)[G][NP]) {
+                if constexpr (RAW)
+                    if (t >= 1 && t <= 4)
+#pragma unroll
+                        for (int i = 0; i < G; ++i) TA::template split<decltype(exact)::value>(whole[i], (t - 1) * 2, fa[i], top);
+            };
+            auto read_b = [&](int from, int n, s16x8 (&fb)[NP][NT]) {
+                const int p = n / NT, j = n % NT;
+                fb[p][j] = TB::fragment(lds + from * kStageBytes + kBytesA + p * TB::bytes, (wn * NT + j) * U::size, 0);
+            };
+            // The products of 2^-16, the largest ones while those are made 2^-8, then the products of 2^-8; between(0) ..
+            // between(kTurns - 1) in between.  What they amount to joins the result during the first turns of the next group (of
+            // this one, where it is the only one): the matrix cores do not wait for either.
+            f32x4 low[2][G][NT];
+            auto join = [&](int group, int i, int j) {
+                f32x4 &c = acc[group * G + i][j];
+#pragma unroll
+                for (int r = 0; r < 4; ++r) c[r] = fmaf(low[group % 2][i][j][r], 1.f / 256, c[r]);
+            };
+            auto multiply = [&](int group, const s16x8 (&fa)[G][NP], const s16x8 (&fb)[NP][NT], auto between) {
+                f32x4(&mine)[G][NT] = low[group % 2];
+                const int last = (group + kGroups - 1) % kGroups;
+                auto add = [&](int p, int q, auto besides) {
+#pragma unroll
+                    for (int i = 0; i < G; ++i)
+#pragma unroll
+                        for (int j = 0; j < NT; ++j) {
+                            mine[i][j] = U::multiply(fa[i][p], fb[q][j], mine[i][j]);
+                            besides(i, j);
+                        }
+                };
+                auto nothing = [](int, int) {};
+#pragma unroll
+                for (int i = 0; i < G; ++i)
+#pragma unroll
+                    for (int j = 0; j < NT; ++j) mine[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+                add(1, 1, [&](int i, int j) {
+                    if (kGroups > 1) join(last, i, j);
+                });
+                between(0);
+                add(0, 2, nothing), between(1);
+                add(2, 0, nothing), between(2);
 #pragma unroll
                 for (int i = 0; i < G; ++i)
 #pragma unroll
                     for (int j = 0; j < NT; ++j) {
-                        mine[i][j] = U::multiply(fa[i][p], fb[q][j], mine[i][j]);
-                        besides(i, j);
+                        f32x4 &c = acc[group * G + i][j];
+                        c = U::multiply(fa[i][0], fb[0][j], c);
+                        mine[i][j] *= 1.f / 256;
                     }
+                between(3);
+                add(0, 1, nothing), between(4);
+                add(1, 0, nothing), between(5);
+                if (kGroups == 1)
+#pragma unroll
+                    for (int i = 0; i < G; ++i)
+#pragma unroll
+                        for (int j = 0; j < NT; ++j) join(group, i, j);
             };
-            auto nothing = [](int, int) {};
+            auto step = [&](s16x8 (&fb)[NP][NT], s16x8 (&fa)[G][NP], s16x8 (&next_b)[NP][NT], s16x8 (&next_a)[G][NP]) {
 #pragma unroll
-            for (int i = 0; i < G; ++i)
+                for (int k = 0; k + 1 < kGroups; ++k)
+                    multiply(k, k % 2 ? turn : fa, fb, [&](int t) {
+                        if (t == 0)
 #pragma unroll
-                for (int j = 0; j < NT; ++j) mine[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-            add(1, 1, [&](int i, int j) {
-                if (kGroups > 1) join(last, i, j);
-            });
-            between(0);
-            add(0, 2, nothing), between(1);
-            add(2, 0, nothing), between(2);
+                            for (int n = 0; n < G * NP; ++n) read_a(slot, k + 1, n, k % 2 ? fa : turn);
+                        split_a(t, k % 2 ? fa : turn);
+                        __builtin_amdgcn_sched_barrier(0);
+                    });
+                wait_for_stage<(STAGES - 2) * kInFlight>();
+                const uint32_t to = lds0 + slot * kStageBytes;
+                slot = slot + 1 == STAGES ? 0 : slot + 1;
+                multiply(kGroups - 1, kGroups > 1 ? turn : fa, fb, [&](int t) {
+                    // a share of the fetches and of the reads, the latter in the first five turns
 #pragma unroll
-            for (int i = 0; i < G; ++i)
+                    for (int f = 0; f < kFetches; ++f) {
+                        if (f * kTurns / kFetches != t) continue;
+                        if (f < kFetchesA) ta.one(a_at, k_left, to, wave, f / TA::mine, f % TA::mine);
+                        else tb.one(b_at, k_left, to + kBytesA, wave, (f - kFetchesA) / TB::mine, (f - kFetchesA) % TB::mine);
+                    }
 #pragma unroll
-                for (int j = 0; j < NT; ++j) {
-                    f32x4 &c = acc[group * G + i][j];
-                    c = U::multiply(fa[i][0], fb[0][j], c);
-                    mine[i][j] *= 1.f / 256;
-                }
-            between(3);
-            add(0, 1, nothing), between(4);
-            add(1, 0, nothing), between(5);
-            if (kGroups == 1)
+                    for (int n = 0; n < kReads; ++n) {
+                        if (n * (kTurns - 1) / kReads != t) continue;
+                        if (n < G * NP) read_a(slot, 0, n, next_a);
+                        else read_b(slot, n - G * NP, next_b);
+                    }
+                    split_a(t, next_a);
+                    __builtin_amdgcn_sched_barrier(0);
+                });
+                a_at += a_step, b_at += b_step, k_left -= kStep;
+            };
+            if constexpr (decltype(exact)::value) restart();
+#pragma unroll
+            for (int s = 0; s < STAGES; ++s) fetch_stage(s);
+            keep_known();
+            wait_for_stage<(STAGES - 1) * kInFlight>();
+#pragma unroll
+            for (int n = 0; n < G * NP; ++n) read_a(0, 0, n, a0);
+#pragma unroll
+            for (int t = 1; t <= 4; ++t) split_a(t, a0);
+#pragma unroll
+            for (int n = 0; n < NP * NT; ++n) read_b(0, n, b0);
+            if (kGroups > 1)
 #pragma unroll
                 for (int i = 0; i < G; ++i)
 #pragma unroll
-                    for (int j = 0; j < NT; ++j) join(group, i, j);
+                    for (int j = 0; j < NT; ++j) low[(kGroups - 1) % 2][i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+            for (int s = 0; s < steps; s += 2) {
+                step(b0, a0, b1, a1);
+                if (s + 1 < steps) step(b1, a1, b0, a0);
+            }
+            if (kGroups > 1)
+#pragma unroll
+                for (int i = 0; i < G; ++i)
+#pragma unroll
+                    for (int j = 0; j < NT; ++j) join(kGroups - 1, i, j);
         };
-        auto step = [&](s16x8 (&fb)[NP][NT], s16x8 (&fa)[G][NP], s16x8 (&next_b)[NP][NT], s16x8 (&next_a)[G][NP]) {
-#pragma unroll
-            for (int k = 0; k + 1 < kGroups; ++k)
-                multiply(k, k % 2 ? turn : fa, fb, [&](int t) {
-                    if (t == 0)
-#pragma unroll
-                        for (int n = 0; n < G * NP; ++n) read_a(slot, k + 1, n, k % 2 ? fa : turn);
-                    __builtin_amdgcn_sched_barrier(0);
-                });
-            wait_for_stage<(STAGES - 2) * kInFlight>();
-            const uint32_t to = lds0 + slot * kStageBytes;
-            slot = slot + 1 == STAGES ? 0 : slot + 1;
-            multiply(kGroups - 1, kGroups > 1 ? turn : fa, fb, [&](int t) {
-                // a share of the fetches and of the reads, the latter in the first five turns
-#pragma unroll
-                for (int f = 0; f < kFetches; ++f) {
-                    if (f * kTurns / kFetches != t) continue;
-                    if (f < NP * TA::mine) ta.one(a_at, k_left, to, wave, f / TA::mine, f % TA::mine);
-                    else
-                        tb.one(b_at, k_left, to + NP * TA::bytes, wave, (f - NP * TA::mine) / TB::mine,
-                               (f - NP * TA::mine) % TB::mine);
-                }
-#pragma unroll
-                for (int n = 0; n < kReads; ++n) {
-                    if (n * (kTurns - 1) / kReads != t) continue;
-                    if (n < G * NP) read_a(slot, 0, n, next_a);
-                    else read_b(slot, n - G * NP, next_b);
-                }
-                __builtin_amdgcn_sched_barrier(0);
-            });
-            a_at += a_step, b_at += b_step, k_left -= kStep;
-        };
-#pragma unroll
-        for (int s = 0; s < STAGES; ++s) fetch_stage(s);
-        keep_known();
-        wait_for_stage<(STAGES - 1) * kInFlight>();
-#pragma unroll
-        for (int n = 0; n < G * NP; ++n) read_a(0, 0, n, a0);
-#pragma unroll
-        for (int n = 0; n < NP * NT; ++n) read_b(0, n, b0);
-        if (kGroups > 1)
-#pragma unroll
-            for (int i = 0; i < G; ++i)
-#pragma unroll
-                for (int j = 0; j < NT; ++j) low[(kGroups - 1) % 2][i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-        for (int s = 0; s < steps; s += 2) {
-            step(b0, a0, b1, a1);
-            if (s + 1 < steps) step(b1, a1, b0, a0);
-        }
-        if (kGroups > 1)
-#pragma unroll
-            for (int i = 0; i < G; ++i)
-#pragma unroll
-                for (int j = 0; j < NT; ++j) join(kGroups - 1, i, j);
+        products(std::false_type());
+        if constexpr (RAW)
+            if (__syncthreads_or(top >= TA::kLimit)) products(std::true_type());
     }
     // nothing of this wave is on its way to LDS any more, and nobody reads it
     asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
@@ -682,7 +812,7 @@ __device__ __forceinline__ void product_tile(const Args &g, const int block, cha
     // float32 computation rounded once at its end.
     auto put_prob = [&](int I, float (&p)[4]) {
         typedef Gather<uint16_t, BM * NP> Out;
-        static_assert(KIND == kOut || kRowsOut * BM * NP * 2 <= kStagesBytes<P, BM, BN, STAGES>, "");
+        static_assert(KIND == kOut || kRowsOut * BM * NP * 2 <= kStagesBytes<P, BM, BN, STAGES, RAW>, "");
         const int m = m_in + m_of(I);
         if constexpr (NP > 1 && KIND == kKeep) {
             *(f32x4 *)Out::at(lds, row_out, (m >> 5) * 96 + (m & 31) * 2) = f32x4{p[0], p[1], p[2], p[3]};
@@ -750,8 +880,8 @@ __device__ __forceinline__ void product_tile(const Args &g, const int block, cha
             return sum;
         };
         // a place behind the rows on their way out, where other waves' results wait
-        float2 *const others = (float2 *)(lds + kStagesBytes<P, BM, BN, STAGES>) - WM * BN;
-        static_assert(KIND == kStats || kRowsOut * BM * NP * 2 + WM * BN * 8 <= kStagesBytes<P, BM, BN, STAGES>, "");
+        float2 *const others = (float2 *)(lds + kStagesBytes<P, BM, BN, STAGES, RAW>) - WM * BN;
+        static_assert(KIND == kStats || kRowsOut * BM * NP * 2 + WM * BN * 8 <= kStagesBytes<P, BM, BN, STAGES, RAW>, "");
         if constexpr (KIND == kKeep) {
             // the tile's maximum first: what is kept is relative to it
 #pragma unroll
@@ -846,7 +976,7 @@ __device__ __forceinline__ void product_tile(const Args &g, const int block, cha
     }
     if constexpr (KIND == kOut) {
         typedef typename ElementOf<P>::type E;
-        static_assert(kRowsOut * BM * 4 <= kStagesBytes<P, BM, BN, STAGES>, "");
+        static_assert(kRowsOut * BM * 4 <= kStagesBytes<P, BM, BN, STAGES, RAW>, "");
         const float factor = g.slice ? 1.f : out_factor<P>(g.factor);
 #pragma unroll
         for (int j = 0; j < NT; ++j) {
@@ -880,6 +1010,18 @@ __global__ __launch_bounds__(WM * WN * 64) void product_kernel(Args g)
     product_tile<P, BM, BN, WM, WN, A_ACROSS, B_ACROSS, KIND, STAGES>(g, blockIdx.x, lds);
 }
 
+// Of float32 weights as they are, for few tokens: logits (A along the reduction) and hidden gradients (across it).  Splitting a
+// fragment into planes takes some 70 vector instructions, which run between the products of the one before; two workgroups
+// on a CU cover each other's waits (37 tokens, 50021 words x 2048, the logits: 130 us; with five stages and one workgroup 200,
+// with the split in one piece behind its loads 150; 410 MB of weights take 75).
+template <int KIND>
+__global__ __launch_bounds__(256, 2) void raw_kernel(Args g)
+{
+    constexpr int BM = kRawWords, BN = kRawTokens, STAGES = 2;
+    __shared__ __attribute__((aligned(1024))) char lds[kLdsBytes<Split, BM, BN, STAGES, KIND != kOut, true>];
+    product_tile<Split, BM, BN, 4, 1, KIND == kOut, false, KIND, STAGES, true>(g, blockIdx.x, lds);
+}
+
 // Both gradients' products in one launch, `first` workgroups for the first.
 template <typename P, int BM, int BN, int WM, int WN, int STAGES>
 __global__ __launch_bounds__(WM * WN * 64) void both_kernel(Args hidden, Args weight, int first)
@@ -890,6 +1032,8 @@ __global__ __launch_bounds__(WM * WN * 64) void both_kernel(Args hidden, Args we
     else
         product_tile<P, BM, BN, WM, WN, true, true, kOut, STAGES>(weight, blockIdx.x - first, lds);
 }
+
+int launch_raw(int kind, Args &g, hipStream_t st);
 
 // Which product a launch is.
 enum { kLogitStats = 0, kLogitKeep = 1, kLogitProb = 2, kHidden = 3, kWeight = 4 };

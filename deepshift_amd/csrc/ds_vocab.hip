@@ -488,6 +488,7 @@ struct Plan {
     bool pack_h, pack_w;
     bool keep;            // the last piece's exponentials become its probabilities (run may decide against it)
     bool few;             // ds_vocab_few.hip's kernels
+    bool raw;             // float32 weights as they are, for the matrix cores
     int tile_logits, tile_words, tile_tokens;
     Choice hidden, weight;
     int words;            // of a piece's probabilities, a multiple of 32,
@@ -499,7 +500,14 @@ inline bool in_place(const void *p, int64_t ld, int64_t D) { return (uintptr_t)p
 
 // Up to how many tokens of float32 read the weights as they are.  Small heads give each workgroup too little to read: 16 tokens of
 // 512 features, 1000 words, 44 us a step where planes take 33 (8 tokens: 31 and 34), 16 of 1024, 8000 words, 74 and 78.
-inline int64_t few_tokens(int64_t weights) { return weights < 1 << 23 ? kFewTokens / 2 : kFewTokens; }
+constexpr int64_t kManyWeights = 1 << 23;
+inline int64_t few_tokens(int64_t weights) { return weights < kManyWeights ? kFewTokens / 2 : kFewTokens; }
+
+// Up to how many tokens of float32 the matrix instructions take weights as they are, split into planes by every tile of 64 tokens;
+// for more, planes for all of them to share are worth what writing and reading them takes.  50021 words of 2048 features, the loss
+// and a step, in us: 64 tokens 123 and 465 (by planes 425 and 789), 256 tokens 373 and 1132 (550 and 1266), 512 tokens 672 and
+// 2053 (850 and 2088); 24 tokens of 1024 features, 8200 words, 42 and 91 (41 and 86).
+constexpr int64_t kRawMost = 512;
 
 // What a call does: the loss, the gradients, or both.
 enum { kLoss = 1, kGrad = 2 };
@@ -513,7 +521,9 @@ Plan plan_of(const void *hidden, int64_t ldh, const void *weight, int64_t ldw, i
     p.ldd = row_elements<P>(D);
     p.few = NP > 1 && T > 0 && T <= few_tokens(V * D) && g_tune.vocab_tile == kTuneUnset;
     p.pack_h = !p.few && (NP > 1 || what & kGrad || !in_place(hidden, ldh, D));  // for gradients: without the rows that do not count
-    p.pack_w = !p.few && (NP > 1 || !in_place(weight, ldw, D));
+    p.raw = NP > 1 && !p.few && T > 0 && T <= kRawMost && V * D >= kManyWeights && g_tune.vocab_tile == kTuneUnset && (uintptr_t)weight % 16 == 0 &&
+            ldw % 4 == 0 && D % 4 == 0;
+    p.pack_w = !p.few && !p.raw && (NP > 1 || !in_place(weight, ldw, D));
     const int kb = g_tune.vocab_piece_kb;
     const size_t piece_bytes = kb == kTuneUnset ? kPieceBytes : (size_t)kb << 10;
     int64_t most = V;
@@ -529,9 +539,9 @@ Plan plan_of(const void *hidden, int64_t ldh, const void *weight, int64_t ldw, i
     if (p.piece > V) p.piece = V;
     p.pieces = (V + p.piece - 1) / p.piece;
     p.keep = what == (kLoss | kGrad) && T <= 65535 * 8;
-    p.tile_logits = p.few ? 0 : choose<P>(p.piece, T, D, kShapes, 1, what & kGrad).tile;
-    p.tile_words = p.few ? kFewWords : Shapes<P>::m[p.tile_logits];
-    p.tile_tokens = p.few ? kFewTokens : Shapes<P>::n[p.tile_logits];
+    p.tile_logits = p.few || p.raw ? 0 : choose<P>(p.piece, T, D, kShapes, 1, what & kGrad).tile;
+    p.tile_words = p.few ? kFewWords : p.raw ? kRawWords : Shapes<P>::m[p.tile_logits];
+    p.tile_tokens = p.few ? kFewTokens : p.raw ? kRawTokens : Shapes<P>::n[p.tile_logits];
     size_t at = 0;
     auto take = [&](size_t n) {
         const size_t was = at;
@@ -557,6 +567,11 @@ Plan plan_of(const void *hidden, int64_t ldh, const void *weight, int64_t ldw, i
             p.weight.splits = 1;
         } else {
             p.hidden = choose<P>(D, T, p.piece, kGradShapes<P>, 64, false);
+            if (p.raw) {
+                // two workgroups a CU, with 256 words at least
+                const int64_t tiles = std::max<int64_t>(1, (D + kRawWords - 1) / kRawWords * ((T + kRawTokens - 1) / kRawTokens));
+                p.hidden.splits = (int)std::max<int64_t>(1, std::min({(int64_t)64, 2 * device_cus() / tiles, p.piece / 256}));
+            }
             p.weight = choose<P>(D, p.piece, T, kGradShapes<P>, 64, false);
         }
         p.prob = take((size_t)T * p.ldp * 2);
@@ -635,7 +650,7 @@ Args logit_args(const Call &c, const Plan &p, int64_t v0, int64_t n, const Opera
 {
     Args g{};
     g.a = o.w, g.b = o.h;
-    g.M = (int)n, g.N = (int)c.T, g.K = p.few ? (int)c.D : p.Dp;
+    g.M = (int)n, g.N = (int)c.T, g.K = p.few || p.raw ? (int)c.D : p.Dp;
     g.splits = 1, g.k_split = (p.Dp + P::step - 1) / P::step * P::step;
     g.bias = c.bias, g.bias_type = c.type;
     g.target = c.target, g.target_wide = c.wide;
@@ -651,6 +666,7 @@ inline bool joined_later(const Plan &p, int64_t T, int tiles) { return p.keep &&
 template <typename P>
 int product(const Plan &p, int kind, int tile, Args &g, int64_t T, hipStream_t st)
 {
+    if (p.raw && kind != kWeight) return launch_raw(kind, g, st);
     return p.few ? launch_few(kind, (int)T, g, st) : launch_product<P>(kind, tile, g, nullptr, st);
 }
 
@@ -768,7 +784,7 @@ int loss_grad(const Call &c, const Plan &p, Operands<P> &o, const Rows &of, Grad
         const int tm = Shapes<P>::m[p.weight.tile], tn = Shapes<P>::n[p.weight.tile];
         const int64_t across = (int64_t)ceil_div((int)c.T, tn) * p.hidden.splits + ceil_div((int)n, tn);
         const int64_t blocks = ceil_div((int)c.D, tm) * across;
-        const bool both = !p.few && wanted[0] && wanted[1] && !joined[1] && p.hidden.tile == p.weight.tile && blocks <= 2 * device_cus();
+        const bool both = !p.few && !p.raw && wanted[0] && wanted[1] && !joined[1] && p.hidden.tile == p.weight.tile && blocks <= 2 * device_cus();
         if (both) DS_TRY(launch_product<P>(kHidden, p.weight.tile, g[0], &g[1], c.st));
         for (int which = 0; which < 2; ++which) {
             Args &x = g[which];

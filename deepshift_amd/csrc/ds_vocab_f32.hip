@@ -12,5 +12,18 @@ template <> int launch_product<Split>(int kind, int tile, Args &g, Args *other, 
     return launch_tiled<Split, 32, 32, 1, 2, 6, false>(kind, g, other, st);
 }
 
+int launch_raw(int kind, Args &g, hipStream_t st)
+{
+    g.tiles_m = ceil_div(g.M, kRawWords), g.tiles_n = ceil_div(g.N, kRawTokens);
+    const int64_t blocks = (int64_t)g.tiles_m * g.tiles_n * g.splits;
+    if (blocks > 0x7fffffff) return DS_ETOOLARGE;
+    const dim3 grid((unsigned)blocks), threads(256);
+    if (kind == kLogitStats) hipLaunchKernelGGL((raw_kernel<kStats>), grid, threads, 0, st, g);
+    else if (kind == kLogitKeep) hipLaunchKernelGGL((raw_kernel<kKeep>), grid, threads, 0, st, g);
+    else if (kind == kLogitProb) hipLaunchKernelGGL((raw_kernel<kProb>), grid, threads, 0, st, g);
+    else hipLaunchKernelGGL((raw_kernel<kOut>), grid, threads, 0, st, g);
+    return launch_status();
+}
+
 }  // namespace vocab
 }  // namespace ds

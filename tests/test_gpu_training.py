@@ -296,6 +296,50 @@ def test_cross_entropy_of_a_few_tokens(T):
         _head_check(clean, w, b, y, -100, grads, rows, leaves[0].grad, leaves[1].grad, leaves[2].grad if b is not None else None)
 
 
+@pytest.mark.parametrize("T", [17, 40, 64, 65, 130])
+def test_cross_entropy_of_weights_as_they_are(T):
+    # many weights, few tokens: words around a tile's 128, features around a stage's 32
+    for i, (D, V) in enumerate([(1024, 8193), (4, 2097153), (2052, 4224), (36, 233100), (1056, 7999)]):
+        print(T, D, V, flush=True)
+        g = _gen(T, D, V, 6)
+        h, w, b, y = _head(T, D, V, torch.float32, i % 2 == 0, g)
+        y[0], y[1], y[2] = V - 1, 0, 128
+        y[3::5] = -100
+        h[3::5] = float("nan")
+        kept = int((y != -100).sum())
+        clean = torch.where((y != -100)[:, None], h, torch.zeros_like(h))
+        share = torch.full((T,), 1.0 / kept, device=DEV)
+        for tune in ({}, dict(vocab_piece_kb=3 * 2 * T * (V // 3) // 1024)):
+            with Tune(**tune):
+                rows = training.linear_cross_entropy(h, w, y, b, reduction="none")
+                loss, dh, dw, db = training.linear_cross_entropy_grad(h, w, y, b)
+                again = training.linear_cross_entropy_grad(h, w, y, b)
+            _head_check(clean, w, b, y, -100, share, rows, dh, dw, db)
+            assert all(x is z or torch.equal(x, z) for x, z in zip((loss, dh, dw, db), again))
+        del again, dh, dw, db
+        leaves = [x.detach().requires_grad_() for x in (h, w) + ((b,) if b is not None else ())]
+        training.linear_cross_entropy(leaves[0], leaves[1], y, *leaves[2:], reduction="sum").backward()
+        _head_check(clean, w, b, y, -100, torch.ones(T, device=DEV), rows, leaves[0].grad, leaves[1].grad,
+                    leaves[2].grad if b is not None else None)
+
+
+def test_cross_entropy_of_extreme_weights_as_they_are():
+    # the largest float32, and the smallest, split without loss
+    g = _gen(1, 2, 3)
+    T, D, V = 20, 1024, 8200
+    h, w, b, y = _head(T, D, V, torch.float32, False, g)
+    for small, large in ((2.0 ** -100, 2.0 ** 97), (2.0 ** 60, 2.0 ** -62)):
+        rows = training.linear_cross_entropy(h * small, w * large, y, reduction="none")
+        with Tune(vocab_tile=1):
+            want = training.linear_cross_entropy(h * small, w * large, y, reduction="none")
+        _head_check(h * small, w * large, None, y, -100, torch.ones(T, device=DEV), rows)
+        _head_check(h * small, w * large, None, y, -100, torch.ones(T, device=DEV), want)
+    w[:, 0] = torch.finfo(torch.float32).max
+    h[:, 0] = 2.0 ** -125
+    rows = training.linear_cross_entropy(h, w, y, reduction="none")
+    _head_check(h, w, None, y, -100, torch.ones(T, device=DEV), rows)
+
+
 def test_cross_entropy_of_a_few_tokens_with_words_taken_out():
     g = _gen(8, 8)
     h, w, b, y = _head(6, 20, 200, torch.float32, True, g)
