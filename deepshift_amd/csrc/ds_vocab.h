@@ -198,6 +198,12 @@ __device__ __forceinline__ void fetch(uint32_t offset, i32x4 buffer, uint32_t ld
     asm volatile("s_mov_b32 m0, %2\n\ts_nop 3\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds"
                  :: "v"(offset), "s"(buffer), "s"(lds) : "memory");
 }
+// The same, 4 bytes per lane, at `lds` + 4 l.
+__device__ __forceinline__ void fetch_word(uint32_t offset, i32x4 buffer, uint32_t lds)
+{
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 3\n\tbuffer_load_dword %0, %1, 0 offen lds"
+                 :: "v"(offset), "s"(buffer), "s"(lds) : "memory");
+}
 constexpr uint32_t kNothing = 0x80000000u;
 
 __device__ __forceinline__ i32x4 buffer_at(uint64_t address)
@@ -306,15 +312,21 @@ struct Tile {
 //   along k:  [row][32], rows of 128 bytes, whose 16-byte pieces are exchanged by row;
 //   across:   [k][ROWS], whose 64-byte pieces are exchanged by k / 8, so that the four groups of 16 lanes that read together
 //             meet other banks.
-// Rows and reductions are multiples of four.
-template <int ROWS, bool ACROSS, int WAVES>
+// WIDTH floats a lane and fetch: four, where rows begin at multiples of 16 bytes and end at multiples of four floats, or one
+// (28 tokens, 61003 words x 3405: the loss in 246 us, with planes written first 773).
+template <int ROWS, bool ACROSS, int WAVES, int WIDTH>
 struct RawTile {
     static constexpr int kStep = Split::step, kPlanes = 1;
-    static constexpr int bytes = ROWS * kStep * 4, fetches = bytes / 1024, mine = fetches / WAVES;
+    static constexpr int bytes = ROWS * kStep * 4, fetches = bytes / (256 * WIDTH), mine = fetches / WAVES;
     static_assert(fetches % WAVES == 0 && ROWS >= 64, "");
 
-    uint32_t offset[mine];
-    int k_at[mine];
+    // Fetches that are `kTurn` apart differ in what all lanes share: kShared rows (of 16 bytes along k, single floats across).
+    // Fetch i of a wave has the floats from 64 WIDTH i on: of one float each, two rows, or half of a k.
+    static constexpr int kTurn = WIDTH == 4 ? mine : ACROSS ? 2 : 4;
+    uint32_t offset[kTurn];
+    int k_at[kTurn];
+    int rows_after;  // single floats along k: rows behind this lane's first one
+    int64_t pitch;   // bytes
 
     __device__ static __forceinline__ int swapped(int row) { return row & 7; }
     __device__ static __forceinline__ int swapped_across(int k) { return (k >> 3 & 3) << 2; }
@@ -322,23 +334,37 @@ struct RawTile {
     __device__ void init(const Operand &o, int rows_left, int wave)
     {
         const int lane = threadIdx.x & 63;
+        pitch = o.ld * 4;
+        rows_after = rows_left - wave * mine * 2 - lane / 32;
 #pragma unroll
-        for (int i = 0; i < mine; ++i) {
-            const int p = (wave * mine + i) * 64 + lane;
+        for (int i = 0; i < kTurn; ++i) {
+            const int f = ((wave * mine + i) * 64 + lane) * WIDTH, p = f / 4, e = f % 4;  // float, 16-byte piece
             if constexpr (!ACROSS) {
                 const int row = p / 8, piece = p % 8 ^ swapped(row);
-                k_at[i] = piece * 4;
-                offset[i] = row < rows_left ? (uint32_t)(row * o.ld * 4 + piece * 16) : kNothing;
+                k_at[i] = piece * 4 + e;
+                offset[i] = WIDTH == 1 || row < rows_left ? (uint32_t)(row * pitch + piece * 16 + e * 4) : kNothing;
             } else {
                 const int k = p / (ROWS / 4), piece = p % (ROWS / 4) ^ swapped_across(k);
                 k_at[i] = k;
-                offset[i] = piece * 4 < rows_left ? (uint32_t)(k * o.ld * 4 + piece * 16) : kNothing;
+                offset[i] = piece * 4 + e < rows_left ? (uint32_t)(k * pitch + piece * 16 + e * 4) : kNothing;
             }
         }
     }
     __device__ __forceinline__ void one(uint64_t base, int k_left, uint32_t lds, int wave, int, int i) const
     {
-        fetch(k_at[i] < k_left ? offset[i] : kNothing, buffer_at(base), lds + (wave * mine + i) * 1024);
+        const uint32_t to = lds + (wave * mine + i) * 256 * WIDTH;
+        if constexpr (WIDTH == 4) {
+            fetch(k_at[i] < k_left ? offset[i] : kNothing, buffer_at(base), to);
+        } else if constexpr (ACROSS) {
+            // a wave has mine / 2 whole k, whose pieces are exchanged alike
+            static_assert(ROWS == 128 && mine / 2 == 8, "");
+            const int k = wave * (mine / 2) + i / 2;
+            fetch_word(k < k_left ? offset[i % 2] : kNothing, buffer_at(base + i / 2 * pitch), to);
+        } else {
+            // rows 2 i on: the exchange comes again after eight of them
+            const bool real = 2 * i < rows_after && k_at[i % 4] < k_left;
+            fetch_word(real ? offset[i % 4] : kNothing, buffer_at(base + i / 4 * 8 * pitch), to);
+        }
     }
     __device__ __forceinline__ void stage(uint64_t base, int k_left, uint32_t lds, int wave) const
     {
@@ -508,18 +534,18 @@ __device__ __forceinline__ int spread_sums(float (&v)[ALL], int lane)
 // are read and stages fetched between rows of products, a few each: with all of them behind the barrier the matrix cores were
 // busy 55 % of the cycles instead of 70 to 85 (4.0 instead of 3.2 ms for the scores above).  32 x 32 instructions take half as
 // many issues as 16 x 16 ones at the same rate; float32 keeps the smaller ones, whose partial sums of the planes fit.
-template <typename P, int BM, int BN, int WM, int WN, bool A_ACROSS, bool B_ACROSS, int KIND, int STAGES, bool RAW = false>
+template <typename P, int BM, int BN, int WM, int WN, bool A_ACROSS, bool B_ACROSS, int KIND, int STAGES, int RAW = 0>
 __device__ __forceinline__ void product_tile(const Args &g, const int block, char *lds)
 {
     using U = Unit<P>;
     constexpr int WAVES = WM * WN, MT = BM / WM / U::size, NT = BN / WN / U::size, NP = P::planes;
     constexpr int kStep = P::step;
     static_assert(!RAW || NP == 3, "");
-    using TA = typename std::conditional<RAW, RawTile<BM, A_ACROSS, WAVES>, Tile<P, BM, A_ACROSS, WAVES>>::type;
+    using TA = typename std::conditional<(RAW > 0), RawTile<BM, A_ACROSS, WAVES, RAW ? RAW : 4>, Tile<P, BM, A_ACROSS, WAVES>>::type;
     using TB = Tile<P, BN, B_ACROSS, WAVES>;
     constexpr int kBytesA = TA::kPlanes * TA::bytes, kStageBytes = kBytesA + NP * TB::bytes;
     constexpr int kFetchesA = TA::kPlanes * TA::mine, kInFlight = kFetchesA + NP * TB::mine;  // loads of one stage and wave
-    static_assert(STAGES * kStageBytes == kStagesBytes<P, BM, BN, STAGES, RAW>, "");
+    static_assert(STAGES * kStageBytes == kStagesBytes<P, BM, BN, STAGES, (RAW > 0)>, "");
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
     const int wm = wave % WM, wn = wave / WM;
 
@@ -554,7 +580,7 @@ __device__ __forceinline__ void product_tile(const Args &g, const int block, cha
 #pragma unroll
             for (int r = 0; r < 4 * U::groups; ++r) acc[i][j][r] = 0.f;
 
-    Known<BM, BN> &known = *(Known<BM, BN> *)(lds + kStagesBytes<P, BM, BN, STAGES, RAW>);
+    Known<BM, BN> &known = *(Known<BM, BN> *)(lds + kStagesBytes<P, BM, BN, STAGES, (RAW > 0)>);
     static_assert(BM <= WAVES * 64 && BN <= WAVES * 64, "a thread per word and token");
     constexpr int kNowhere = -(1 << 20);
     float bias = -INFINITY, lse = INFINITY, scale = 0.f;
@@ -812,7 +838,7 @@ __device__ __forceinline__ void product_tile(const Args &g, const int block, cha
     // float32 computation rounded once at its end.
     auto put_prob = [&](int I, float (&p)[4]) {
         typedef Gather<uint16_t, BM * NP> Out;
-        static_assert(KIND == kOut || kRowsOut * BM * NP * 2 <= kStagesBytes<P, BM, BN, STAGES, RAW>, "");
+        static_assert(KIND == kOut || kRowsOut * BM * NP * 2 <= kStagesBytes<P, BM, BN, STAGES, (RAW > 0)>, "");
         const int m = m_in + m_of(I);
         if constexpr (NP > 1 && KIND == kKeep) {
             *(f32x4 *)Out::at(lds, row_out, (m >> 5) * 96 + (m & 31) * 2) = f32x4{p[0], p[1], p[2], p[3]};
@@ -880,8 +906,8 @@ __device__ __forceinline__ void product_tile(const Args &g, const int block, cha
             return sum;
         };
         // a place behind the rows on their way out, where other waves' results wait
-        float2 *const others = (float2 *)(lds + kStagesBytes<P, BM, BN, STAGES, RAW>) - WM * BN;
-        static_assert(KIND == kStats || kRowsOut * BM * NP * 2 + WM * BN * 8 <= kStagesBytes<P, BM, BN, STAGES, RAW>, "");
+        float2 *const others = (float2 *)(lds + kStagesBytes<P, BM, BN, STAGES, (RAW > 0)>) - WM * BN;
+        static_assert(KIND == kStats || kRowsOut * BM * NP * 2 + WM * BN * 8 <= kStagesBytes<P, BM, BN, STAGES, (RAW > 0)>, "");
         if constexpr (KIND == kKeep) {
             // the tile's maximum first: what is kept is relative to it
 #pragma unroll
@@ -976,7 +1002,7 @@ __device__ __forceinline__ void product_tile(const Args &g, const int block, cha
     }
     if constexpr (KIND == kOut) {
         typedef typename ElementOf<P>::type E;
-        static_assert(kRowsOut * BM * 4 <= kStagesBytes<P, BM, BN, STAGES, RAW>, "");
+        static_assert(kRowsOut * BM * 4 <= kStagesBytes<P, BM, BN, STAGES, (RAW > 0)>, "");
         const float factor = g.slice ? 1.f : out_factor<P>(g.factor);
 #pragma unroll
         for (int j = 0; j < NT; ++j) {
@@ -1014,12 +1040,12 @@ __global__ __launch_bounds__(WM * WN * 64) void product_kernel(Args g)
 // fragment into planes takes some 70 vector instructions, which run between the products of the one before; two workgroups
 // on a CU cover each other's waits (37 tokens, 50021 words x 2048, the logits: 130 us; with five stages and one workgroup 200,
 // with the split in one piece behind its loads 150; 410 MB of weights take 75).
-template <int KIND>
+template <int KIND, int WIDTH>
 __global__ __launch_bounds__(256, 2) void raw_kernel(Args g)
 {
     constexpr int BM = kRawWords, BN = kRawTokens, STAGES = 2;
     __shared__ __attribute__((aligned(1024))) char lds[kLdsBytes<Split, BM, BN, STAGES, KIND != kOut, true>];
-    product_tile<Split, BM, BN, 4, 1, KIND == kOut, false, KIND, STAGES, true>(g, blockIdx.x, lds);
+    product_tile<Split, BM, BN, 4, 1, KIND == kOut, false, KIND, STAGES, WIDTH>(g, blockIdx.x, lds);
 }
 
 // Both gradients' products in one launch, `first` workgroups for the first.
@@ -1033,7 +1059,7 @@ __global__ __launch_bounds__(WM * WN * 64) void both_kernel(Args hidden, Args we
         product_tile<P, BM, BN, WM, WN, true, true, kOut, STAGES>(weight, blockIdx.x - first, lds);
 }
 
-int launch_raw(int kind, Args &g, hipStream_t st);
+int launch_raw(int kind, int width, Args &g, hipStream_t st);
 
 // Which product a launch is.
 enum { kLogitStats = 0, kLogitKeep = 1, kLogitProb = 2, kHidden = 3, kWeight = 4 };

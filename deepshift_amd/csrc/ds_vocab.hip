@@ -488,7 +488,7 @@ struct Plan {
     bool pack_h, pack_w;
     bool keep;            // the last piece's exponentials become its probabilities (run may decide against it)
     bool few;             // ds_vocab_few.hip's kernels
-    bool raw;             // float32 weights as they are, for the matrix cores
+    int raw;              // float32 weights as they are for the matrix cores, so many at a time, or 0
     int tile_logits, tile_words, tile_tokens;
     Choice hidden, weight;
     int words;            // of a piece's probabilities, a multiple of 32,
@@ -506,7 +506,8 @@ inline int64_t few_tokens(int64_t weights) { return weights < kManyWeights ? kFe
 // Up to how many tokens of float32 the matrix instructions take weights as they are, split into planes by every tile of 64 tokens;
 // for more, planes for all of them to share are worth what writing and reading them takes.  50021 words of 2048 features, the loss
 // and a step, in us: 64 tokens 123 and 465 (by planes 425 and 789), 256 tokens 373 and 1132 (550 and 1266), 512 tokens 672 and
-// 2053 (850 and 2088); 24 tokens of 1024 features, 8200 words, 42 and 91 (41 and 86).
+// 2053 (850 and 2088); of 2049 features, fetched one by one, 512 tokens 757 and 2452 (887 and 2339); 24 tokens of 1024 features,
+// 8200 words, 42 and 91 (41 and 86).
 constexpr int64_t kRawMost = 512;
 
 // What a call does: the loss, the gradients, or both.
@@ -521,8 +522,8 @@ Plan plan_of(const void *hidden, int64_t ldh, const void *weight, int64_t ldw, i
     p.ldd = row_elements<P>(D);
     p.few = NP > 1 && T > 0 && T <= few_tokens(V * D) && g_tune.vocab_tile == kTuneUnset;
     p.pack_h = !p.few && (NP > 1 || what & kGrad || !in_place(hidden, ldh, D));  // for gradients: without the rows that do not count
-    p.raw = NP > 1 && !p.few && T > 0 && T <= kRawMost && V * D >= kManyWeights && g_tune.vocab_tile == kTuneUnset && (uintptr_t)weight % 16 == 0 &&
-            ldw % 4 == 0 && D % 4 == 0;
+    if (NP > 1 && !p.few && T > 0 && T <= kRawMost && V * D >= kManyWeights && g_tune.vocab_tile == kTuneUnset)
+        p.raw = (uintptr_t)weight % 16 == 0 && ldw % 4 == 0 && D % 4 == 0 ? 4 : 1;
     p.pack_w = !p.few && !p.raw && (NP > 1 || !in_place(weight, ldw, D));
     const int kb = g_tune.vocab_piece_kb;
     const size_t piece_bytes = kb == kTuneUnset ? kPieceBytes : (size_t)kb << 10;
@@ -666,7 +667,7 @@ inline bool joined_later(const Plan &p, int64_t T, int tiles) { return p.keep &&
 template <typename P>
 int product(const Plan &p, int kind, int tile, Args &g, int64_t T, hipStream_t st)
 {
-    if (p.raw && kind != kWeight) return launch_raw(kind, g, st);
+    if (p.raw && kind != kWeight) return launch_raw(kind, p.raw, g, st);
     return p.few ? launch_few(kind, (int)T, g, st) : launch_product<P>(kind, tile, g, nullptr, st);
 }
 

@@ -12,17 +12,23 @@ template <> int launch_product<Split>(int kind, int tile, Args &g, Args *other, 
     return launch_tiled<Split, 32, 32, 1, 2, 6, false>(kind, g, other, st);
 }
 
-int launch_raw(int kind, Args &g, hipStream_t st)
+template <int WIDTH>
+int launch_raw_tiles(int kind, const Args &g, dim3 grid, hipStream_t st)
+{
+    const dim3 threads(256);
+    if (kind == kLogitStats) hipLaunchKernelGGL((raw_kernel<kStats, WIDTH>), grid, threads, 0, st, g);
+    else if (kind == kLogitKeep) hipLaunchKernelGGL((raw_kernel<kKeep, WIDTH>), grid, threads, 0, st, g);
+    else if (kind == kLogitProb) hipLaunchKernelGGL((raw_kernel<kProb, WIDTH>), grid, threads, 0, st, g);
+    else hipLaunchKernelGGL((raw_kernel<kOut, WIDTH>), grid, threads, 0, st, g);
+    return launch_status();
+}
+
+int launch_raw(int kind, int width, Args &g, hipStream_t st)
 {
     g.tiles_m = ceil_div(g.M, kRawWords), g.tiles_n = ceil_div(g.N, kRawTokens);
     const int64_t blocks = (int64_t)g.tiles_m * g.tiles_n * g.splits;
     if (blocks > 0x7fffffff) return DS_ETOOLARGE;
-    const dim3 grid((unsigned)blocks), threads(256);
-    if (kind == kLogitStats) hipLaunchKernelGGL((raw_kernel<kStats>), grid, threads, 0, st, g);
-    else if (kind == kLogitKeep) hipLaunchKernelGGL((raw_kernel<kKeep>), grid, threads, 0, st, g);
-    else if (kind == kLogitProb) hipLaunchKernelGGL((raw_kernel<kProb>), grid, threads, 0, st, g);
-    else hipLaunchKernelGGL((raw_kernel<kOut>), grid, threads, 0, st, g);
-    return launch_status();
+    return width == 4 ? launch_raw_tiles<4>(kind, g, dim3((unsigned)blocks), st) : launch_raw_tiles<1>(kind, g, dim3((unsigned)blocks), st);
 }
 
 }  // namespace vocab

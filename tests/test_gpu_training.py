@@ -323,6 +323,25 @@ def test_cross_entropy_of_weights_as_they_are(T):
                     leaves[2].grad if b is not None else None)
 
 
+@pytest.mark.parametrize("T", [17, 64, 100])
+def test_cross_entropy_of_weights_as_they_are_wherever_rows_begin(T):
+    for D, V, before, behind in [(1021, 8300, 0, 0), (3, 2796203, 0, 0), (1024, 8200, 1, 2), (2050, 4097, 2, 0), (1023, 8201, 0, 1)]:
+        print(T, D, V, before, behind, flush=True)
+        g = _gen(T, D, V, 9)
+        h, w, b, y = _head(T, D, V, torch.float32, True, g)
+        y[0], y[1], y[2] = V - 1, 0, 128
+        y[3::5] = -100
+        wide = torch.full((V, before + D + behind), float("nan"), device=DEV)
+        wide[:, before:before + D] = w
+        wide = wide[:, before:before + D]
+        share = torch.full((T,), 1.0 / int((y != -100).sum()), device=DEV)
+        rows = training.linear_cross_entropy(h, wide, y, b, reduction="none")
+        loss, dh, dw, db = training.linear_cross_entropy_grad(h, wide, y, b)
+        _head_check(h, w, b, y, -100, share, rows, dh, dw, db)
+        again = training.linear_cross_entropy_grad(h, wide, y, b)
+        assert all(torch.equal(x, z) for x, z in zip((loss, dh, dw, db), again))
+
+
 def test_cross_entropy_of_extreme_weights_as_they_are():
     # the largest float32, and the smallest, split without loss
     g = _gen(1, 2, 3)
