@@ -285,7 +285,7 @@ __global__ __launch_bounds__(256) void embed_scatter_kernel(SortPass p)
 // The sorted tokens are cut into chunks; a wave adds up one chunk for 64 * N columns.  A word whose tokens lie in one chunk
 // is finished there.  One that runs on leaves a partial sum: in slot 1 of the chunk that it begins in, in slot 0 of the
 // others; embed_join_kernel joins them in order, so that a word with most of the tokens does not wait for one wave.  Bound by
-// memory: 65536 x 2048 bfloat16 gradients in, 0.27 GB, and 0.21 GB of finished rows out in 90 us.  Eight rows are on their
+// memory: 65536 x 2048 bfloat16 gradients of words drawn evenly in, 0.27 GB, and 0.21 GB of finished rows out in 90 us.  Eight rows are on their
 // way at a time; sixteen take more registers than they hide (151 us where eight took 114).
 template <typename E, int N>
 __global__ __launch_bounds__(64) void embed_sum_kernel(const E *__restrict__ g, int64_t ldg, const uint32_t *__restrict__ keys,
