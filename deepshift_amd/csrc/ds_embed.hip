@@ -17,11 +17,14 @@ constexpr int kLookupUnits = 4;  // accesses a thread has in flight
 // the caches by, which leaves them to the rows that more tokens share: 131072 tokens of 4096 bfloat16 features from 131072
 // words drawn as text has them take 320 us, 4.2 TB/s of what has to move (352 us with ordinary stores; 2 or 8 accesses a thread
 // make no difference; a large copy reaches 4.9 TB/s).  64 tokens of 512: 3.4 us.
-template <typename E, int N>
+// ANY: rows that begin or end elsewhere than at multiples of 16 bytes; their accesses are as wide, the last one of a row but for
+// what there is (65536 x 2047 bfloat16: 122 us, element by element 209, 77 for 2048).
+template <typename E, bool ANY>
 __global__ __launch_bounds__(256) void embed_kernel(const void *__restrict__ ids, int wide, const E *__restrict__ w,
-                                                    E *__restrict__ out, int64_t T, int64_t V, int64_t ldw, float scale,
+                                                    E *__restrict__ out, int64_t T, int64_t V, int64_t D, int64_t ldw, float scale,
                                                     uint32_t per_row, FastDiv by_row)
 {
+    constexpr int N = 16 / sizeof(E);
     const uint64_t first = (uint64_t)blockIdx.x * (256 * kLookupUnits);
     const uint64_t row0 = first / per_row;
     const uint32_t rem0 = (uint32_t)(first - row0 * per_row);
@@ -33,8 +36,11 @@ __global__ __launch_bounds__(256) void embed_kernel(const void *__restrict__ ids
         const uint32_t r = div_by(local, by_row);
         const int64_t t = (int64_t)row0 + r;
         id[j] = t < T ? token_at(ids, wide, t, V) : -1;
-        if (id[j] >= 0)
-            got[j] = ((const Vec<E, N> *)(w + (int64_t)id[j] * ldw))[local - r * per_row];
+        if (id[j] < 0) continue;
+        const E *const row = w + (int64_t)id[j] * ldw;
+        const uint32_t unit = local - r * per_row;
+        if constexpr (ANY) got[j] = load_any<E, N>(row + (int64_t)unit * N, D - (int64_t)unit * N);
+        else got[j] = ((const Vec<E, N> *)row)[unit];
     }
 #pragma unroll
     for (int j = 0; j < kLookupUnits; ++j) {
@@ -43,7 +49,13 @@ __global__ __launch_bounds__(256) void embed_kernel(const void *__restrict__ ids
         Vec<E, N> o;
 #pragma unroll
         for (int e = 0; e < N; ++e) o.v[e] = from_float<E>(id[j] >= 0 ? to_float(got[j].v[e]) * scale : NAN);
-        store_streaming((Vec<E, N> *)out + at, o);
+        if constexpr (ANY) {
+            const uint32_t local = rem0 + j * 256 + threadIdx.x, r = div_by(local, by_row);
+            const int64_t col = (int64_t)(local - r * per_row) * N;
+            store_any<E, N>(out + ((int64_t)row0 + r) * D + col, o, D - col);
+        } else {
+            store_streaming((Vec<E, N> *)out + at, o);
+        }
     }
 }
 
@@ -51,18 +63,14 @@ template <typename E>
 int launch_embed(const void *ids, int wide, const void *w, void *out, int64_t T, int64_t V, int64_t D, int64_t ldw,
                  float scale, hipStream_t st)
 {
-    const int n = vector_elements(sizeof(E), {D, ldw}, {w, out});
-    const uint64_t per_row = (uint64_t)(D / n), blocks = ((uint64_t)T * per_row + 256 * kLookupUnits - 1) / (256 * kLookupUnits);
+    constexpr int N = 16 / sizeof(E);
+    const bool any = vector_elements(sizeof(E), {D, ldw}, {w, out}) < N;
+    const uint64_t per_row = (uint64_t)((D + N - 1) / N), blocks = ((uint64_t)T * per_row + 256 * kLookupUnits - 1) / (256 * kLookupUnits);
     if (per_row > 0x7fffffffull - 256 * kLookupUnits || blocks > 0x7fffffffull) return DS_ETOOLARGE;
     const FastDiv by_row = fast_div((uint32_t)per_row);
-#define DS_LAUNCH(N)                                                                                                    \
-    hipLaunchKernelGGL((embed_kernel<E, N>), dim3((unsigned)blocks), dim3(256), 0, st, ids, wide, (const E *)w, (E *)out, \
-                       T, V, ldw, scale, (uint32_t)per_row, by_row)
-    if (n == 8) { if constexpr (sizeof(E) == 2) DS_LAUNCH(8); }
-    else if (n == 4) DS_LAUNCH(4);
-    else if (n == 2) DS_LAUNCH(2);
-    else DS_LAUNCH(1);
-#undef DS_LAUNCH
+    auto kernel = any ? embed_kernel<E, true> : embed_kernel<E, false>;
+    hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(256), 0, st, ids, wide, (const E *)w, (E *)out, T, V, D, ldw, scale,
+                       (uint32_t)per_row, by_row);
     return launch_status();
 }
 
@@ -285,9 +293,9 @@ __global__ __launch_bounds__(256) void embed_scatter_kernel(SortPass p)
 // The sorted tokens are cut into chunks; a wave adds up one chunk for 64 * N columns.  A word whose tokens lie in one chunk
 // is finished there.  One that runs on leaves a partial sum: in slot 1 of the chunk that it begins in, in slot 0 of the
 // others; embed_join_kernel joins them in order, so that a word with most of the tokens does not wait for one wave.  Bound by
-// memory: 65536 x 2048 bfloat16 gradients of words drawn evenly in, 0.27 GB, and 0.21 GB of finished rows out in 90 us.  Eight rows are on their
-// way at a time; sixteen take more registers than they hide (151 us where eight took 114).
-template <typename E, int N>
+// memory: 65536 x 2048 bfloat16 gradients of words drawn evenly in, 0.27 GB, and 0.21 GB of finished rows out in 90 us.  Eight
+// rows are on their way at a time; sixteen take more registers than they hide (151 us where eight took 114).
+template <typename E, int N, bool ANY>
 __global__ __launch_bounds__(64) void embed_sum_kernel(const E *__restrict__ g, int64_t ldg, const uint32_t *__restrict__ keys,
                                                        const uint32_t *__restrict__ pos, E *__restrict__ dw,
                                                        float *__restrict__ part, int64_t T, int64_t D, int chunk, float scale)
@@ -295,6 +303,7 @@ __global__ __launch_bounds__(64) void embed_sum_kernel(const E *__restrict__ g, 
     const int64_t from = (int64_t)blockIdx.x * chunk, to = min(T, from + chunk);
     const int64_t col = ((int64_t)blockIdx.y * 64 + threadIdx.x) * N;
     const bool in = col < D;
+    const int left = (int)min(D - col, (int64_t)N);
     const uint32_t before = from > 0 ? keys[from - 1] : kNoWord;
     const uint32_t behind = to < T ? keys[to] : kNoWord;
     float acc[N];
@@ -310,7 +319,11 @@ __global__ __launch_bounds__(64) void embed_sum_kernel(const E *__restrict__ g, 
         for (int j = 0; j < kAhead; ++j) {
             const bool real = i + j < to;
             key[j] = real ? keys[i + j] : kNoWord;
-            if (real && key[j] != kNoWord && in) got[j] = *(const Vec<E, N> *)(g + (int64_t)pos[i + j] * ldg + col);
+            if (real && key[j] != kNoWord && in) {
+                const E *const row = g + (int64_t)pos[i + j] * ldg + col;
+                if constexpr (ANY) got[j] = load_any<E, N>(row, left);
+                else got[j] = *(const Vec<E, N> *)row;
+            }
         }
 #pragma unroll
         for (int j = 0; j < kAhead; ++j) {
@@ -320,12 +333,14 @@ __global__ __launch_bounds__(64) void embed_sum_kernel(const E *__restrict__ g, 
                 if (run != kNoWord && in) {
                     if (first && run == before) {
 #pragma unroll
-                        for (int e = 0; e < N; ++e) part[(int64_t)blockIdx.x * 2 * D + col + e] = acc[e];
+                        for (int e = 0; e < N; ++e)
+                            if (!ANY || e < left) part[(int64_t)blockIdx.x * 2 * D + col + e] = acc[e];
                     } else {
                         Vec<E, N> o;
 #pragma unroll
                         for (int e = 0; e < N; ++e) o.v[e] = from_float<E>(acc[e] * scale);
-                        store_streaming((Vec<E, N> *)(dw + (int64_t)run * D + col), o);
+                        if constexpr (ANY) store_any<E, N>(dw + (int64_t)run * D + col, o, left);
+                        else store_streaming((Vec<E, N> *)(dw + (int64_t)run * D + col), o);
                     }
                 }
                 first = false;
@@ -342,12 +357,14 @@ __global__ __launch_bounds__(64) void embed_sum_kernel(const E *__restrict__ g, 
     const bool came = first && run == before, goes = run == behind;
     if (came || goes) {
 #pragma unroll
-        for (int e = 0; e < N; ++e) part[((int64_t)blockIdx.x * 2 + (came ? 0 : 1)) * D + col + e] = acc[e];
+        for (int e = 0; e < N; ++e)
+            if (!ANY || e < left) part[((int64_t)blockIdx.x * 2 + (came ? 0 : 1)) * D + col + e] = acc[e];
     } else {
         Vec<E, N> o;
 #pragma unroll
         for (int e = 0; e < N; ++e) o.v[e] = from_float<E>(acc[e] * scale);
-        store_streaming((Vec<E, N> *)(dw + (int64_t)run * D + col), o);
+        if constexpr (ANY) store_any<E, N>(dw + (int64_t)run * D + col, o, left);
+        else store_streaming((Vec<E, N> *)(dw + (int64_t)run * D + col), o);
     }
 }
 
@@ -369,18 +386,22 @@ __device__ __forceinline__ uint32_t wave_lower_bound(const uint32_t *__restrict_
 }
 
 // The partial sums of a word that begins in chunk c0 and ends in c1, in order; `p` is chunk 0's slot 0, at the columns wanted.
-template <typename E, int N>
-__device__ __forceinline__ Vec<E, N> joined(const float *__restrict__ p, uint32_t c0, uint32_t c1, int64_t D, float scale)
+template <typename E, int N, bool ANY>
+__device__ __forceinline__ Vec<E, N> joined(const float *__restrict__ p, uint32_t c0, uint32_t c1, int64_t D, int left, float scale)
 {
     float acc[N];
 #pragma unroll
-    for (int e = 0; e < N; ++e) acc[e] = p[((int64_t)c0 * 2 + 1) * D + e];
+    for (int e = 0; e < N; ++e) acc[e] = !ANY || e < left ? p[((int64_t)c0 * 2 + 1) * D + e] : 0.f;
     constexpr int kAhead = N <= 2 ? 24 : 8;  // partial sums on their way
     for (uint32_t c = c0 + 1; c <= c1; c += kAhead) {
         Vec<float, N> got[kAhead];
 #pragma unroll
-        for (int j = 0; j < kAhead; ++j)
-            if (c + j <= c1) got[j] = *(const Vec<float, N> *)(p + (int64_t)(c + j) * 2 * D);
+        for (int j = 0; j < kAhead; ++j) {
+            if (c + j > c1) continue;
+            const float *const at = p + (int64_t)(c + j) * 2 * D;
+            if constexpr (ANY) got[j] = load_any<float, N>(at, left);
+            else got[j] = *(const Vec<float, N> *)at;
+        }
 #pragma unroll
         for (int j = 0; j < kAhead; ++j)
 #pragma unroll
@@ -394,7 +415,7 @@ __device__ __forceinline__ Vec<E, N> joined(const float *__restrict__ p, uint32_
 
 // Words in several chunks: their joined sums, by the workgroup of the chunk that such a word begins in.  Bound by latency: 44
 // partial sums of the most frequent of 2065 tokens in 4.4 us.
-template <typename E, int N>
+template <typename E, int N, bool ANY>
 __global__ __launch_bounds__(64) void embed_join_kernel(const uint32_t *__restrict__ keys, const float *__restrict__ part,
                                                         E *__restrict__ dw, int64_t T, int64_t D, int chunk, float scale)
 {
@@ -404,7 +425,11 @@ __global__ __launch_bounds__(64) void embed_join_kernel(const uint32_t *__restri
     if (run == kNoWord || keys[to] != run || (from > 0 && keys[from - 1] == run)) return;
     const uint32_t end = (uint32_t)to + wave_lower_bound(keys + to, (uint32_t)(T - to), run + 1);
     const int64_t col = ((int64_t)blockIdx.y * 64 + threadIdx.x) * N;
-    if (col < D) *(Vec<E, N> *)(dw + (int64_t)run * D + col) = joined<E, N>(part + col, blockIdx.x, (end - 1) / chunk, D, scale);
+    if (col >= D) return;
+    const int left = (int)min(D - col, (int64_t)N);
+    const Vec<E, N> o = joined<E, N, ANY>(part + col, blockIdx.x, (end - 1) / chunk, D, left, scale);
+    if constexpr (ANY) store_any<E, N>(dw + (int64_t)run * D + col, o, left);
+    else *(Vec<E, N> *)(dw + (int64_t)run * D + col) = o;
 }
 
 // Tokens a chunk: long ones leave hot words fewer partial sums to join, short ones more waves (2065 tokens, 700 of them one word:
@@ -434,21 +459,29 @@ template <typename E>
 int launch_embed_grad(const uint32_t *keys, const uint32_t *pos, const void *g, int64_t ldg, void *dw, float *part, int64_t T,
                       int64_t D, float scale, hipStream_t st)
 {
-    const int n = vector_elements(sizeof(E), {D, ldg}, {g, dw});
+    constexpr int kWide = 16 / sizeof(E);
+    int n = vector_elements(sizeof(E), {D, ldg}, {g, dw});
     const int chunk = embed_chunk(T);
-    const int64_t chunks = (T + chunk - 1) / chunk, slices = (D / n + 63) / 64;
+    const int64_t chunks = (T + chunk - 1) / chunk;
+    auto slices_of = [&](int width) { return ((D + width - 1) / width + 63) / 64; };
+    // Rows that allow one element at a time: as wide as others, wherever they begin, where that leaves every CU four waves
+    // (65536 x 2047 bfloat16 282, now 199 us, x 1023 float32 171 and 145; but 2065 x 385 float32 17 us, and 24 that way).
+    const bool any = n == 1 && chunks * slices_of(kWide) >= 4 * device_cus();
+    if (any) n = kWide;
+    const int64_t slices = slices_of(n);
     if (chunks > 0x7fffffff || slices > 65535) return DS_ETOOLARGE;
-#define DS_LAUNCH(N)                                                                                                    \
-    do {                                                                                                                \
-        hipLaunchKernelGGL((embed_sum_kernel<E, N>), dim3((unsigned)chunks, (unsigned)slices), dim3(64), 0, st,         \
-                           (const E *)g, ldg, keys, pos, (E *)dw, part, T, D, chunk, scale);                            \
-        hipLaunchKernelGGL((embed_join_kernel<E, N>), dim3((unsigned)chunks, (unsigned)slices), dim3(64), 0, st, keys,  \
-                           part, (E *)dw, T, D, chunk, scale);                                                          \
+    const dim3 grid((unsigned)chunks, (unsigned)slices);
+#define DS_LAUNCH(N, ANY)                                                                                                 \
+    do {                                                                                                                  \
+        hipLaunchKernelGGL((embed_sum_kernel<E, N, ANY>), grid, dim3(64), 0, st, (const E *)g, ldg, keys, pos, (E *)dw, part, T, \
+                           D, chunk, scale);                                                                              \
+        hipLaunchKernelGGL((embed_join_kernel<E, N, ANY>), grid, dim3(64), 0, st, keys, part, (E *)dw, T, D, chunk, scale); \
     } while (0)
-    if (n == 8) { if constexpr (sizeof(E) == 2) DS_LAUNCH(8); }
-    else if (n == 4) DS_LAUNCH(4);
-    else if (n == 2) DS_LAUNCH(2);
-    else DS_LAUNCH(1);
+    if (any) DS_LAUNCH(kWide, true);
+    else if (n == 8) { if constexpr (sizeof(E) == 2) DS_LAUNCH(8, false); }
+    else if (n == 4) DS_LAUNCH(4, false);
+    else if (n == 2) DS_LAUNCH(2, false);
+    else DS_LAUNCH(1, false);
 #undef DS_LAUNCH
     return launch_status();
 }

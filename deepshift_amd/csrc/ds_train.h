@@ -45,6 +45,37 @@ __device__ __forceinline__ void store_streaming(Vec<E, N> *to, const Vec<E, N> &
     }
 }
 
+// N elements wherever they lie; those from `left` on are not touched (and zeros).
+template <typename E, int N>
+__device__ __forceinline__ Vec<E, N> load_any(const E *p, int64_t left)
+{
+    Vec<E, N> v{};
+    if (left >= N) {
+        __builtin_memcpy(&v, p, sizeof(v));
+    } else {
+#pragma unroll
+        for (int e = 0; e < N - 1; ++e)
+            if (e < left) v.v[e] = p[e];
+    }
+    return v;
+}
+template <typename E, int N>
+__device__ __forceinline__ void store_any(E *p, const Vec<E, N> &v, int64_t left)
+{
+    static_assert(sizeof(v) == 16, "");
+    if (left >= N) {
+        // (the compiler is kept from seeing the same values stored on both paths, for which it finds common pieces)
+        typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+        u32x4 w = __builtin_bit_cast(u32x4, v);
+        asm("" : "+v"(w));
+        __builtin_memcpy(p, &w, 16);
+    } else {
+#pragma unroll
+        for (int e = 0; e < N - 1; ++e)
+            if (e < left) p[e] = v.v[e];
+    }
+}
+
 inline int element_bytes(int type) { return type == DS_F32 ? 4 : type == DS_BF16 || type == DS_F16 ? 2 : 0; }
 
 // The widest access, in elements of `bytes`, that every one of the sizes (in elements) and addresses allows.

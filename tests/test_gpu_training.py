@@ -142,6 +142,27 @@ def test_embedding_offsets_beyond_32_bits():
     assert torch.equal(got[V - 1], last) and (got[V - 2] == 0).all() and (got[V // 2] == 0).all()
 
 
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+def test_embedding_of_rows_that_begin_anywhere(dtype):
+    for T, V, D, before in [(9000, 300, 257, 0), (20000, 3000, 131, 0), (17000, 65, 513, 0), (9000, 50, 384, 1), (100, 40, 385, 3),
+                            (5, 3, 1, 1), (9, 7, 9, 0)]:
+        print(T, V, D, before, flush=True)
+        g = _gen(T, V, D)
+        wide = torch.full((V, D + before), float("nan"), dtype=dtype, device=DEV)
+        wide[:, before:] = _rand(g, V, D, dtype=dtype)
+        ids = torch.randint(0, V, (T,), generator=g).to(DEV)
+        ids[::3] = V - 1
+        assert torch.equal(training.embedding(ids, wide[:, before:], 0.5), (wide[:, before:].float()[ids] * 0.5).to(dtype))
+        flat = torch.full((T, D + before), float("nan"), dtype=dtype, device=DEV)
+        flat[:, before:] = _rand(g, T, D, dtype=dtype)
+        grad = flat[:, before:]
+        got = training.embedding_grad(ids, grad, V, 0.5)
+        want = torch.zeros(V, D, dtype=torch.float64, device=DEV).index_add_(0, ids, grad.double()) * 0.5
+        size = torch.zeros(V, D, dtype=torch.float64, device=DEV).index_add_(0, ids, grad.double().abs()) * 0.5
+        _within(got, want, (T + 2) * E * size + U[dtype] * want.abs() * 1.01 + TINY[dtype], "gradient")
+        assert torch.equal(got, training.embedding_grad(ids, grad, V, 0.5))
+
+
 def test_embedding_module_under_autograd():
     torch.manual_seed(0)
     m = training.ScaledEmbedding(40, 12, scale=3.0, padding_idx=-1).to(DEV)
