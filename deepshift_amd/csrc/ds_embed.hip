@@ -124,9 +124,10 @@ __device__ __forceinline__ uint32_t key_at(const void *ids, int wide, int64_t i,
 
 // Up to kRankMost tokens: the place of a token is the number of tokens with a smaller word, or the same word and an earlier
 // position.  Every workgroup holds all words in LDS and places 64 tokens, its 16 waves each compare them with a sixteenth:
-// T * T comparisons, two instructions each.  One launch: 7 us for 2065 tokens, 9 for 4096, 15 for 8192, where the passes below
-// take 22 (20 against 26 for 16384).
-constexpr int kRankMost = 8192;  // a multiple of 64
+// T * T comparisons, two instructions each.  One launch: 7 us for 2065 tokens, 9 for 4096, 15 for 8192.  Against two of the passes
+// below a whole gradient (of 128 features) takes 27 instead of 35 us for 9000 tokens, 31 and 37 for 12288, 36 and 33 for 16384;
+// against one pass, which fewer than 511 words need, both take 22.7 for 6144 tokens, and that is half as many.
+constexpr int kRankMost = 12288;  // a multiple of 128
 
 // Workgroups behind those that sort fill `zeros` with zeros.
 __global__ __launch_bounds__(1024) void embed_rank_kernel(const void *__restrict__ ids, int wide, int T, int64_t V,
@@ -493,14 +494,14 @@ int sort_tokens(const void *ids, int wide, int64_t T, int64_t V, int64_t padding
     uint32_t *k[2] = {(uint32_t *)(ws + s.keys[0]), (uint32_t *)(ws + s.keys[1])};
     uint32_t *p[2] = {(uint32_t *)(ws + s.pos[0]), (uint32_t *)(ws + s.pos[1])};
     int at = 0;
-    if (T == 0 || (T <= kRankMost && g_tune.embed_radix != 1)) {
+    // the low bits of kNoWord, all set but the last, have to stay above every word
+    int bits = 1;
+    while (((int64_t)1 << bits) <= V + 1) ++bits;
+    if (T == 0 || (T <= (bits > kDigitBits ? kRankMost : kRankMost / 2) && g_tune.embed_radix != 1)) {
         const Zeros z = zeros_of(zeros, bytes, 1024);
         hipLaunchKernelGGL(embed_rank_kernel, dim3((unsigned)((T + 63) / 64 + zero_blocks(z, 1024))), dim3(1024), 0, st, ids, wide,
                            (int)T, V, padding, k[0], p[0], z);
     } else {
-        // the low bits of kNoWord, all set but the last, have to stay above every word
-        int bits = 1;
-        while (((int64_t)1 << bits) <= V + 1) ++bits;
         int64_t blocks = min((int64_t)kSortBlocks, (T + kSortTile - 1) / kSortTile);
         const int64_t stretch = ((T + blocks - 1) / blocks + kSortTile - 1) / kSortTile * kSortTile;
         blocks = (T + stretch - 1) / stretch;
