@@ -142,6 +142,22 @@ def test_embedding_offsets_beyond_32_bits():
     assert torch.equal(got[V - 1], last) and (got[V - 2] == 0).all() and (got[V // 2] == 0).all()
 
 
+@pytest.mark.parametrize("T, V", [(6144, 400), (6145, 400), (8192, 510), (8192, 511), (12288, 1125), (12289, 1125), (12288, 262143)])
+def test_embedding_gradient_where_the_sort_changes(T, V):
+    g = _gen(T, V)
+    ids = torch.randint(0, V, (T,), generator=g).to(DEV)
+    ids[::5] = V // 2
+    ids[1::7] = -1     # no word
+    grad = _rand(g, T, 20)
+    real = ids >= 0
+    got = training.embedding_grad(ids, grad, V, 2.0, padding_idx=3)
+    want, size = (torch.zeros(V, 20, dtype=torch.float64, device=DEV).index_add_(0, ids[real], x[real]) * 2 for x in
+                  (grad.double(), grad.double().abs()))
+    want[3], size[3] = 0, 0
+    _within(got, want, (T + 2) * E * size + TINY[torch.float32], "gradient")
+    assert (got[3] == 0).all() and torch.equal(got, training.embedding_grad(ids.int(), grad, V, 2.0, padding_idx=3))
+
+
 @pytest.mark.parametrize("dtype", TYPES, ids=str)
 def test_embedding_of_rows_that_begin_anywhere(dtype):
     for T, V, D, before in [(9000, 300, 257, 0), (20000, 3000, 131, 0), (17000, 65, 513, 0), (9000, 50, 384, 1), (100, 40, 385, 3),
