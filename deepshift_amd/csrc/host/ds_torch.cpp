@@ -331,6 +331,35 @@ bool look_at(const char *name, PyObject *list, c10::Device device, std::vector<c
     return contiguous;
 }
 
+int64_t bytes_of(int64_t n, int type) { return n * (type == DS_F32 ? 4 : 2); }
+
+// Nothing may be written twice, and what one tensor's elements are read from may not be written for another: workgroups do both at
+// the same time.  A tensor scaled in place, to its own type, is read by whoever writes it.
+void check_overlaps(const std::vector<ds_tensor> &table)
+{
+    struct Range {
+        uintptr_t from, to;
+        bool written;
+        bool operator<(const Range &o) const { return from < o.from; }
+    };
+    std::vector<Range> ranges;
+    ranges.reserve(2 * table.size());
+    for (const ds_tensor &x : table) {
+        if (x.n == 0) continue;
+        ranges.push_back({(uintptr_t)x.dst, (uintptr_t)x.dst + bytes_of(x.n, x.dst_type), true});
+        if (x.src != x.dst || x.src_type != x.dst_type)
+            ranges.push_back({(uintptr_t)x.src, (uintptr_t)x.src + bytes_of(x.n, x.src_type), false});
+    }
+    if (!std::is_sorted(ranges.begin(), ranges.end())) std::sort(ranges.begin(), ranges.end());
+    uintptr_t any = 0, written = 0;  // where the ranges so far end at the latest
+    for (const Range &r : ranges) {
+        if (r.from < (r.written ? any : written))
+            refuse(PyExc_ValueError, "a tensor is given twice, or one that is written shares memory with another one");
+        any = std::max(any, r.to);
+        if (r.written) written = std::max(written, r.to);
+    }
+}
+
 // clip(grads, outs or None, max_norm, scale, any_order, stream): the norm; None, with nothing done, where a tensor is not
 // contiguous and the caller has not said by `any_order` that all elements fill stretches of memory in the same order.
 PyObject *clip(PyObject *, PyObject *const *args, Py_ssize_t count)
@@ -367,17 +396,7 @@ PyObject *clip(PyObject *, PyObject *const *args, Py_ssize_t count)
             x.n = from[i]->numel();
             x.src_type = from_types[i], x.dst_type = elsewhere ? to_types[i] : from_types[i];
         }
-        if (scale) {
-            // nothing may be written twice
-            std::vector<std::pair<uintptr_t, uintptr_t>> written;
-            written.reserve(n);
-            for (Py_ssize_t i = 0; i < n; ++i)
-                if (table[i].n) written.emplace_back((uintptr_t)table[i].dst, (uintptr_t)table[i].dst + to[i]->nbytes());
-            if (!std::is_sorted(written.begin(), written.end())) std::sort(written.begin(), written.end());
-            for (size_t i = 1; i < written.size(); ++i)
-                if (written[i].first < written[i - 1].second)
-                    refuse(PyExc_ValueError, "a tensor is given twice, or shares memory with another one that is written");
-        }
+        if (scale) check_overlaps(table);
         const auto options = at::TensorOptions().device(device);
         at::Tensor norm = at::empty({}, options.dtype(at::kFloat));
         const size_t bytes = ds_clip_workspace_bytes((int)n);

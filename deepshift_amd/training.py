@@ -177,12 +177,55 @@ def _clip(grads, max_norm, out, scale):
         norm = clip(grads, outs, max_norm, scale, False, _stream_of(device))
         if norm is None:
             # not all contiguous; what is written to copies is copied back, on the same stream
+            if scale:
+                _check_apart(grads if outs is None else outs)
             sources, targets, back = _stretches(grads, grads if outs is None else outs)
             norm = clip(sources, None if targets is sources else targets, max_norm, scale, True, _stream_of(device))
             if scale:
                 for o, copy in back:
                     o.copy_(copy)
     return norm
+
+
+def _meet(a, b):
+    """Whether two tensors have a byte of memory in common."""
+    reach = {}   # by how many bytes an index moves: which differences of indices there are
+    for t, other in ((a, False), (b, True)):
+        for n, stride in zip(t.shape, t.stride()):
+            low, high = reach.get(stride * t.element_size(), (0, 0))
+            reach[stride * t.element_size()] = (low - n + 1, high) if other else (low, high + n - 1)
+    reach.pop(0, None)
+    steps = sorted(((step, low, high) for step, (low, high) in reach.items()), reverse=True)
+
+    def found(steps, least, most):
+        """Whether the steps add up to something from ``least`` to ``most``."""
+        if not steps:
+            return least <= 0 <= most
+        (step, low, high), rest = steps[0], steps[1:]
+        below, above = sum(s * x for s, x, _ in rest), sum(s * x for s, _, x in rest)
+        return any(found(rest, least - x * step, most - x * step)
+                   for x in range(max(low, -((above - least) // step)), min(high, (most - below) // step) + 1))
+
+    gap = b.data_ptr() - a.data_ptr()
+    return found(steps, gap - a.element_size() + 1, gap + b.element_size() - 1)
+
+
+def _check_apart(outs):
+    """Refuses tensors whose elements are written twice, however they lie in memory."""
+    spans = []
+    for t in outs:
+        if t.numel():
+            if any(n > 1 and stride == 0 for n, stride in zip(t.shape, t.stride())):
+                raise ValueError("elements of a tensor that is written share their memory")
+            length = sum((n - 1) * stride for n, stride in zip(t.shape, t.stride())) + 1
+            spans.append((t.data_ptr(), t.data_ptr() + length * t.element_size(), t))
+    spans.sort(key=lambda span: span[0])
+    open_ = []
+    for span in spans:
+        open_ = [other for other in open_ if other[1] > span[0]]
+        if any(_meet(other[2], span[2]) for other in open_):
+            raise ValueError("a tensor is given twice, or one that is written shares memory with another one")
+        open_.append(span)
 
 
 def _stretches(grads, outs):
@@ -212,8 +255,8 @@ def gradient_norm(grads):
 def clip_gradients_(grads, max_norm, out=None):
     """Scales ``grads`` by ``min(1, max_norm / (norm + 1e-6))`` and returns ``norm``, their global 2-norm before it (a float32
     scalar on the device; nothing waits for it).  The results go to ``out``, a tensor for each gradient, of any of the three
-    types, or in place.  Types may differ from tensor to tensor.  A norm that is infinite or NaN scales by 0 or NaN.  Tensors
-    that are written may not overlap."""
+    types, or in place.  Types may differ from tensor to tensor.  A norm that is infinite or NaN scales by 0 or NaN.  A tensor
+    that is written may share no memory with another one, of ``grads`` or of ``out`` (but be its own gradient)."""
     max_norm = float(max_norm)
     if not max_norm >= 0:
         raise ValueError("max_norm must not be negative")

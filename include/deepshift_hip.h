@@ -576,7 +576,8 @@ typedef struct {
 } ds_tensor;
 
 /* The global norm of `count` tensors (an array on the host), norm[0] = sqrt(sum of squares) on the device (NULL: not wanted);
- * with scale != 0 also dst = src * min(1, max_norm / (norm + 1e-6)).  Squares are summed in 64 bits.  Bit-reproducible. */
+ * with scale != 0 also dst = src * min(1, max_norm / (norm + 1e-6)).  Squares are summed in 64 bits.  Bit-reproducible.
+ * What is written may share no memory with another tensor of either side; dst may be src, of the same type. */
 size_t ds_clip_workspace_bytes(int count);
 int ds_clip(const ds_tensor *tensors, int count, float max_norm, int scale, float *norm, void *workspace,
             size_t workspace_bytes, ds_stream_t stream);
