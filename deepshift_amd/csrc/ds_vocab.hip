@@ -203,8 +203,8 @@ __global__ __launch_bounds__(1024) void row_kernel(Rows r)
 
 __global__ void no_rows_kernel(int mean, float *total) { write_total(0, 0, mean, total); }
 
-// Gradients of single losses: the largest of them in `factor`, each one's share of that in `scale`, so that what the products
-// take lies in [-1, 1] whatever the gradients' size.
+// Gradients of single losses: the largest finite one in `factor`, each one's share of that in `scale`, so that what the products
+// take lies in [-1, 1] whatever the gradients' size, or is no number where its own gradient is none.
 __global__ __launch_bounds__(1024) void row_scale_kernel(const float *__restrict__ grad, const void *__restrict__ target,
                                                          int wide, int T, int64_t ignore, float *__restrict__ scale,
                                                          float *__restrict__ factor)
@@ -212,20 +212,17 @@ __global__ __launch_bounds__(1024) void row_scale_kernel(const float *__restrict
     __shared__ float lds[16];
     float top = 0.f;
     for (int t = threadIdx.x; t < T; t += 1024) {
-        const int64_t y = wide ? ((const int64_t *)target)[t] : (int64_t)((const int32_t *)target)[t];
-        const float g = y == ignore ? 0.f : fabsf(grad[t]);
-        top = g > top || g != g ? g : top;
+        const float g = fabsf(grad[t]);
+        if (target_of(target, wide, t) != ignore && g < INFINITY) top = fmaxf(top, g);
     }
 #pragma unroll
-    for (int o = 32; o > 0; o >>= 1) {
-        const float other = __shfl_xor(top, o);
-        top = other > top || other != other ? other : top;
-    }
+    for (int o = 32; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
     if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = top;
     __syncthreads();
     top = 0.f;
-    for (int w = 0; w < 16; ++w) top = lds[w] > top || lds[w] != lds[w] ? lds[w] : top;
-    for (int t = threadIdx.x; t < T; t += 1024) scale[t] = top == 0.f ? 0.f : grad[t] / top;
+    for (int w = 0; w < 16; ++w) top = fmaxf(top, lds[w]);
+    if (top == 0.f) top = 1.f;
+    for (int t = threadIdx.x; t < T; t += 1024) scale[t] = grad[t] / top;
     if (threadIdx.x == 0) *factor = top;
 }
 

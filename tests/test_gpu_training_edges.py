@@ -6,9 +6,64 @@ import pytest
 import torch
 
 from deepshift_amd import training
-from tests.test_gpu_training import DEV, E, _gen, _rand
+from tests.test_gpu_training import DEV, E, TINY, TYPES, U, _gen, _head, _rand, _within
 
 pytestmark = pytest.mark.gpu
+
+
+def _softmax(h, w, b):
+    """Logits, probabilities, and how far off float32 may have them, in 64 bits."""
+    H, W = h.double(), w.double()
+    s, size = H @ W.t(), H.abs() @ W.abs().t()
+    if b is not None:
+        s, size = s + b.double(), size + b.double().abs()
+    d = ((h.shape[1] + 8) * E * size).amax(1, keepdim=True)
+    p = s.softmax(1)
+    return p, p * (2 * d + (4 * s.abs().amax(1, keepdim=True) + 16) * E)
+
+
+def _own_rows(h, w, b, y, g, dh, roundings=2):
+    """``dh`` against 64 bits, each row by the size of its own gradient ``g``."""
+    dtype, V, g = h.dtype, w.shape[0], g.double()[:, None]
+    p, off = _softmax(h, w, b)
+    p = p.scatter_add(1, y[:, None], torch.full_like(g, -1.0))
+    off = (off + p.abs() * roundings * U[dtype] + TINY[dtype] * 2.0 ** -14) * g.abs()
+    W = w.double()
+    want, off = (p * g) @ W, off @ W.abs()
+    _within(dh, want, off + (V + 16) * E * ((p * g).abs() @ W.abs()) + (U[dtype] + 4 * E) * (want.abs() + off) + TINY[dtype], "dhidden")
+
+
+def _backward(h, w, b, y, up, **kw):
+    """Gradients of hidden, weight and bias under autograd."""
+    leaves = [x.detach().requires_grad_() for x in (h, w) + (() if b is None else (b,))]
+    loss = training.linear_cross_entropy(leaves[0], leaves[1], y, *leaves[2:], **kw)
+    return torch.autograd.grad(loss, leaves, up)
+
+
+# ---- gradients of rows ------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("bad", [float("inf"), -float("inf"), float("nan")], ids=str)
+def test_a_rows_gradient_that_is_no_number_stays_in_its_row(dtype, bad):
+    for T, D, V in [(6, 40, 200), (70, 48, 300), (20, 1024, 8200), (300, 64, 513)]:
+        print(T, D, V, flush=True)
+        g = _gen(T, D, V, 71)
+        h, w, b, y = _head(T, D, V, dtype, True, g)
+        up = _rand(g, T)
+        up[3] = bad
+        dh, dw, db = _backward(h, w, b, y, up, reduction="none")
+        fine = torch.arange(T, device=DEV) != 3
+        assert not dh[3].isfinite().any() and not dw.isfinite().any() and not db.isfinite().any()
+        _own_rows(h[fine], w, b, y[fine], up[fine], dh[fine])
+        # the only gradient that is not 0
+        up = torch.where(fine, 0.0, up)
+        dh, dw, db = _backward(h, w, b, y, up, reduction="none")
+        assert not dh[3].isfinite().any() and (dh[fine] == 0).all()
+        # of a token that does not count
+        y[3], up[0] = -100, 0.5
+        dh, dw, db = _backward(h, w, b, y, up, reduction="none")
+        assert (dh[1:] == 0).all() and dw.isfinite().all() and db.isfinite().all()
+        _own_rows(h[:1], w, b, y[:1], up[:1], dh[:1])
 
 
 # ---- tensors that overlap -----------------------------------------------------------------------------------------
