@@ -138,6 +138,7 @@ struct Args {
     // kProb (prob also kKeep)
     const float *lse;     // [T], base 2
     const float *row_scale;  // [T], or NULL: 1 for every counted row
+    const float *row_power;  // float16, [T], or NULL: powers of two that rows have left to be multiplied with (kOut: of C)
     void *prob;           // [T] rows of ldp
     int64_t ldp;
     int prob_words;       // words of a row, a multiple of 32; zeros from M on
@@ -462,6 +463,7 @@ struct Known {
     int want[BN];     // the target, counted from the tile's first word, where it lies in the tile; else far below 0
     float lse[BN];    // +inf for rows that do not count: theirs are probabilities of 0
     float scale[BN];
+    float power[BN];
 };
 template <typename P, int BM, int BN, int STAGES, bool LOGITS, bool RAW = false>
 constexpr int kLdsBytes = kStagesBytes<P, BM, BN, STAGES, RAW> + (LOGITS ? (int)sizeof(Known<BM, BN>) : 0);
@@ -583,7 +585,7 @@ __device__ __forceinline__ void product_tile(const Args &g, const int block, cha
     Known<BM, BN> &known = *(Known<BM, BN> *)(lds + kStagesBytes<P, BM, BN, STAGES, (RAW > 0)>);
     static_assert(BM <= WAVES * 64 && BN <= WAVES * 64, "a thread per word and token");
     constexpr int kNowhere = -(1 << 20);
-    float bias = -INFINITY, lse = INFINITY, scale = 0.f;
+    float bias = -INFINITY, lse = INFINITY, scale = 0.f, power = 1.f;
     int want = kNowhere;
     if constexpr (KIND != kOut) {
         const int m = m0 + threadIdx.x, n = n0 + threadIdx.x;
@@ -595,6 +597,7 @@ __device__ __forceinline__ void product_tile(const Args &g, const int block, cha
                 if (y != g.ignore) {
                     lse = g.lse[n];
                     scale = y < 0 || y >= g.V ? NAN : g.row_scale ? g.row_scale[n] : 1.f;
+                    if (P::half && g.row_power) power = g.row_power[n];
                 } else {
                     want = kNowhere;
                 }
@@ -606,7 +609,8 @@ __device__ __forceinline__ void product_tile(const Args &g, const int block, cha
         if constexpr (KIND != kOut) {
             if (threadIdx.x < BM) known.bias[threadIdx.x] = bias;
             if (threadIdx.x < BN)
-                known.want[threadIdx.x] = want, known.lse[threadIdx.x] = lse, known.scale[threadIdx.x] = scale;
+                known.want[threadIdx.x] = want, known.lse[threadIdx.x] = lse, known.scale[threadIdx.x] = scale,
+                known.power[threadIdx.x] = power;
         }
     };
 
@@ -959,6 +963,7 @@ __device__ __forceinline__ void product_tile(const Args &g, const int block, cha
 #pragma unroll
         for (int j = 0; j < NT; ++j) {
             const float lse = known.lse[n_in + j * U::size], scale = known.scale[n_in + j * U::size];
+            const float power = P::half ? known.power[n_in + j * U::size] : 1.f;
             const float least = lse == INFINITY ? -INFINITY : -126.f;
             const int at = known.want[n_in + j * U::size] - m_in;
 #pragma unroll
@@ -973,7 +978,7 @@ __device__ __forceinline__ void product_tile(const Args &g, const int block, cha
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
                     p[r] *= scale;
-                    over_n[I * 4 + r] += p[r];
+                    over_n[I * 4 + r] += p[r] * power;
                 }
                 put_prob(I, p);
             }
@@ -1003,9 +1008,11 @@ __device__ __forceinline__ void product_tile(const Args &g, const int block, cha
     if constexpr (KIND == kOut) {
         typedef typename ElementOf<P>::type E;
         static_assert(kRowsOut * BM * 4 <= kStagesBytes<P, BM, BN, STAGES, (RAW > 0)>, "");
-        const float factor = g.slice ? 1.f : out_factor<P>(g.factor);
+        const float all = g.slice ? 1.f : out_factor<P>(g.factor);
 #pragma unroll
         for (int j = 0; j < NT; ++j) {
+            const int own = n0 + n_in + j * U::size;
+            const float factor = P::half && g.row_power && !g.slice && own < g.n_store ? all * g.row_power[own] : all;
             auto leave = [&](auto kind, int64_t ld, void *base) {
                 typedef decltype(kind) S;
                 typedef Gather<S, BM> Out;

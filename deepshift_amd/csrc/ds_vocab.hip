@@ -204,10 +204,11 @@ __global__ __launch_bounds__(1024) void row_kernel(Rows r)
 __global__ void no_rows_kernel(int mean, float *total) { write_total(0, 0, mean, total); }
 
 // Gradients of single losses: the largest finite one in `factor`, each one's share of that in `scale`, so that what the products
-// take lies in [-1, 1] whatever the gradients' size, or is no number where its own gradient is none.
+// take lies in [-1, 1] whatever the gradients' size, or is no number where its own gradient is none.  With `power` the shares are
+// cut into a part from a half to 1, which stays in `scale`, and a power of two.
 __global__ __launch_bounds__(1024) void row_scale_kernel(const float *__restrict__ grad, const void *__restrict__ target,
                                                          int wide, int T, int64_t ignore, float *__restrict__ scale,
-                                                         float *__restrict__ factor)
+                                                         float *__restrict__ factor, float *__restrict__ power)
 {
     __shared__ float lds[16];
     float top = 0.f;
@@ -222,8 +223,37 @@ __global__ __launch_bounds__(1024) void row_scale_kernel(const float *__restrict
     top = 0.f;
     for (int w = 0; w < 16; ++w) top = fmaxf(top, lds[w]);
     if (top == 0.f) top = 1.f;
-    for (int t = threadIdx.x; t < T; t += 1024) scale[t] = grad[t] / top;
+    for (int t = threadIdx.x; t < T; t += 1024) {
+        float share = grad[t] / top;
+        if (power) {
+            int e = 0;
+            if (fabsf(share) < INFINITY) share = frexpf(share, &e);
+            power[t] = target_of(target, wide, t) == ignore ? 1.f : ldexpf(1.f, e);
+        }
+        scale[t] = share;
+    }
     if (threadIdx.x == 0) *factor = top;
+}
+
+// Rows of float16 probabilities times their powers of two, in place.  A row whose gradient is 2^-20 of the largest keeps all bits of
+// its probabilities until its own hidden gradient is formed; then every row goes to the common scale, on which the weights'
+// gradient sums them and on which float16 holds what is above 2^-39 of the largest.  Bound by memory: 2048 x 32768 in
+// 24 us of 540 (bfloat16, which needs none of it, 450).
+__global__ __launch_bounds__(256) void power_kernel(f16_t *__restrict__ prob, int64_t ldp, int words, int64_t T,
+                                                    const float *__restrict__ power)
+{
+    const int units = words / 8;
+    const int64_t total = T * units;
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
+        const int64_t t = i / units;
+        const float by = power[t];
+        if (by == 1.f) continue;
+        Vec<f16_t, 8> *const at = (Vec<f16_t, 8> *)(prob + t * ldp) + (i - t * units);
+        Vec<f16_t, 8> v = *at;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v.v[e] = from_float<f16_t>(to_float(v.v[e]) * by);
+        *at = v;
+    }
 }
 
 // ---- exponentials to probabilities -----------------------------------------------------------------------------------
@@ -411,8 +441,8 @@ __global__ __launch_bounds__(256) void bias_join_kernel(BiasJoin b, const float 
 // multiplied and rounded.  Workgroups from `blocks` on join a bias.
 template <typename P, typename E>
 __global__ __launch_bounds__(256) void join_kernel(const float *__restrict__ slices, int splits, int64_t n, int M, float *acc,
-                                                   int first, int last, const float *f0, const float *f1, E *__restrict__ out,
-                                                   int64_t ldo, int blocks, BiasJoin bias)
+                                                   int first, int last, const float *f0, const float *f1,
+                                                   const float *row_power, E *__restrict__ out, int64_t ldo, int blocks, BiasJoin bias)
 {
     const float *const f[2] = {f0, f1};
     if ((int)blockIdx.x >= blocks) {
@@ -430,7 +460,7 @@ __global__ __launch_bounds__(256) void join_kernel(const float *__restrict__ sli
 #pragma unroll
             for (int j = 0; j < kAhead; ++j) s += got[j];
         }
-        if (last) out[i / M * ldo + i % M] = from_float<E>(s * factor);
+        if (last) out[i / M * ldo + i % M] = from_float<E>(s * (P::half && row_power ? factor * row_power[i / M] : factor));
         else acc[i] = s;
     }
 }
@@ -490,7 +520,7 @@ struct Plan {
     Choice hidden, weight;
     int words;            // of a piece's probabilities, a multiple of 32,
     int64_t ldp;          // and what a row of them takes
-    size_t h, w, stats, picked, shares, arrived, prob, bias, slices, acc, scale, factor, bytes;
+    size_t h, w, stats, picked, shares, arrived, prob, bias, slices, acc, scale, power, factor, bytes;
 };
 
 inline bool in_place(const void *p, int64_t ld, int64_t D) { return (uintptr_t)p % 16 == 0 && ld % 8 == 0 && D % 8 == 0; }
@@ -585,6 +615,7 @@ Plan plan_of(const void *hidden, int64_t ldh, const void *weight, int64_t ldw, i
         p.slices = take(slices);
         if (p.pieces > 1) p.acc = take((size_t)T * D * 4);
         p.scale = take((size_t)T * 4);
+        if (P::half) p.power = take((size_t)T * 4);
         p.factor = take(4);
     }
     p.bytes = at ? at : 256;
@@ -705,9 +736,11 @@ template <typename P>
 int loss_grad(const Call &c, const Plan &p, Operands<P> &o, const Rows &of, Grads r)
 {
     typedef typename ElementOf<P>::type E;
+    // rows of float16 whose gradients are of different sizes keep scales of their own until their hidden gradients are formed
+    float *const power = P::half && r.row_grad && r.dhidden ? (float *)(c.ws + p.power) : nullptr;
     if (c.T > 0 && r.row_grad) {
         hipLaunchKernelGGL(row_scale_kernel, dim3(1), dim3(1024), 0, c.st, r.row_grad, c.target, c.wide, (int)c.T, c.ignore,
-                           (float *)(c.ws + p.scale), (float *)(c.ws + p.factor));
+                           (float *)(c.ws + p.scale), (float *)(c.ws + p.factor), power);
         r.grad = (const float *)(c.ws + p.factor);
     }
     float *const slices = (float *)(c.ws + p.slices);
@@ -740,6 +773,7 @@ int loss_grad(const Call &c, const Plan &p, Operands<P> &o, const Rows &of, Grad
                 Args g = logit_args<P>(c, p, v0, n, o);
                 g.lse = r.lse;
                 g.row_scale = r.row_grad ? (const float *)(c.ws + p.scale) : nullptr;
+                g.row_power = power;
                 g.prob = c.ws + p.prob, g.ldp = p.ldp, g.prob_words = p.words;
                 g.factor[0] = r.grad, g.factor[1] = r.share;
                 g.bias_out = bias_out, g.bias_part = bias_part;
@@ -777,17 +811,24 @@ int loss_grad(const Call &c, const Plan &p, Operands<P> &o, const Rows &of, Grad
             x.target = c.target, x.target_wide = c.wide, x.ignore = c.ignore;
             joined[which] = x.splits > 1 || (!which && (p.pieces > 1 || p.few));
             x.slice = joined[which] ? slices : nullptr;
+            x.row_power = which ? nullptr : power;
         }
         // few workgroups each, and no slices to share: both in one launch
         const int tm = Shapes<P>::m[p.weight.tile], tn = Shapes<P>::n[p.weight.tile];
         const int64_t across = (int64_t)ceil_div((int)c.T, tn) * p.hidden.splits + ceil_div((int)n, tn);
         const int64_t blocks = ceil_div((int)c.D, tm) * across;
-        const bool both = !p.few && !p.raw && wanted[0] && wanted[1] && !joined[1] && p.hidden.tile == p.weight.tile && blocks <= 2 * device_cus();
+        const bool both = !p.few && !p.raw && !power && wanted[0] && wanted[1] && !joined[1] && p.hidden.tile == p.weight.tile && blocks <= 2 * device_cus();
         if (both) DS_TRY(launch_product<P>(kHidden, p.weight.tile, g[0], &g[1], c.st));
         for (int which = 0; which < 2; ++which) {
             Args &x = g[which];
             if (!wanted[which]) continue;
             const int tile = which ? p.weight.tile : p.hidden.tile;
+            if (which && power && c.T > 0) {
+                const int words = ceil_div((int)n, 32) * 32;
+                const int64_t all = (c.T * (words / 8) + 255) / 256;
+                hipLaunchKernelGGL(power_kernel, dim3((unsigned)(all < 16384 ? all : 16384)), dim3(256), 0, c.st,
+                                   (f16_t *)(c.ws + p.prob), p.ldp, words, c.T, power);
+            }
             if (!both) DS_TRY(product<P>(p, which ? kWeight : kHidden, tile, x, c.T, c.st));
             if (!joined[which]) continue;
             const int64_t count = (int64_t)x.n_store * c.D;
@@ -795,7 +836,7 @@ int loss_grad(const Call &c, const Plan &p, Operands<P> &o, const Rows &of, Grad
             const int join = (int)(all < 16384 ? all : 16384), more = bias_left ? ceil_div((int)n, 256) : 0;
             hipLaunchKernelGGL((join_kernel<P, E>), dim3(join + more), dim3(256), 0, c.st, slices, x.splits, count, (int)c.D,
                                which ? nullptr : (float *)(c.ws + p.acc), which || first, which || last, r.grad, r.share,
-                               (E *)x.out, c.D, join, bias);
+                               x.row_power, (E *)x.out, c.D, join, bias);
             bias_left = false;
         }
         join_bias_alone();

@@ -2,11 +2,14 @@
 
 Bounds are those of test_gpu_training.py, but for what each test says.
 """
+import math
+
 import pytest
 import torch
 
 from deepshift_amd import training
-from tests.test_gpu_training import DEV, E, TINY, TYPES, U, _gen, _head, _rand, _within
+from tests.conftest import Tune
+from tests.test_gpu_training import DEV, E, TINY, TYPES, U, _gen, _head, _head_check, _rand, _within
 
 pytestmark = pytest.mark.gpu
 
@@ -64,6 +67,30 @@ def test_a_rows_gradient_that_is_no_number_stays_in_its_row(dtype, bad):
         dh, dw, db = _backward(h, w, b, y, up, reduction="none")
         assert (dh[1:] == 0).all() and dw.isfinite().all() and db.isfinite().all()
         _own_rows(h[:1], w, b, y[:1], up[:1], dh[:1])
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+def test_gradients_of_rows_far_apart_keep_their_bits(dtype):
+    # many words and large weights: by 2^-26 of the largest gradient most probabilities are below 2^-39, and what a row of 2^-17
+    # gets is inside float16 all the same
+    for T, D, V, kb in [(70, 48, 20000, 1 << 20), (300, 200, 15000, 1 << 20), (40, 64, 20000, 200)]:
+        print(T, D, V, kb, flush=True)
+        g = _gen(T, D, V, 72)
+        h, w = _rand(g, T, D, dtype=dtype, scale=0.125 / math.sqrt(D)), _rand(g, V, D, dtype=dtype, scale=16.0)
+        b, y = _rand(g, V, dtype=dtype, scale=0.3), torch.randint(0, V, (T,), generator=g).to(DEV)
+        up = 2.0 ** (torch.arange(T, device=DEV) * 26.0 / (T - 1) - 17.0) * (1 - 2 * (torch.arange(T, device=DEV) % 2))
+        up[5] = 0
+        for tile in (0, 1, 2, 3):
+            with Tune(vocab_tile=tile, vocab_piece_kb=kb):
+                dh, dw, db = _backward(h, w, b, y, up, reduction="none")
+                again = _backward(h, w, b, y, up, reduction="none")
+                leaf = h.detach().requires_grad_()
+                only, = torch.autograd.grad(training.linear_cross_entropy(leaf, w, y, b, reduction="none"), leaf, up)
+            _own_rows(h, w, b, y, up, dh)
+            _own_rows(h, w, b, y, up, only)
+            rows = training.linear_cross_entropy(h, w, y, b, reduction="none")
+            _head_check(h, w, b, y, -100, up, rows, dh, dw, db)
+            assert all(torch.equal(x, z) for x, z in zip((dh, dw, db), again))
 
 
 # ---- tensors that overlap -----------------------------------------------------------------------------------------
