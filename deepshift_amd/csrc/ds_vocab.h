@@ -115,8 +115,8 @@ constexpr int kRawWords = 128, kRawTokens = 64;
 // What a launch computes with its tiles.
 enum {
     kStats = 0,  // maxima and sums of the logits' exponentials
-    kKeep = 1,   // the same, and the exponentials themselves, relative to their tile's maximum, where P will be (of float32 as
-                 // they are, 32 of them in the first 128 of the 192 bytes that their planes will take)
+    kKeep = 1,   // the same, and the exponentials themselves, relative to their tile's maximum, in 32 bits: of float32 where P will be
+                 // (32 of them in the first 128 of the 192 bytes that their planes will take), of 16-bit types beside it
     kProb = 2,   // P, from finished sums
     kOut = 3     // a gradient
 };
@@ -141,6 +141,8 @@ struct Args {
     const float *row_power;  // float16, [T], or NULL: powers of two that rows have left to be multiplied with (kOut: of C)
     void *prob;           // [T] rows of ldp
     int64_t ldp;
+    float *kept;          // kKeep of 16-bit types: [T] rows of ld_kept
+    int64_t ld_kept;
     int prob_words;       // words of a row, a multiple of 32; zeros from M on
     float *bias_part;     // [tiles_n][ld of the piece]: sums over the rows of a tile, or NULL
     int ld_bias_part;
@@ -465,8 +467,15 @@ struct Known {
     float scale[BN];
     float power[BN];
 };
-template <typename P, int BM, int BN, int STAGES, bool LOGITS, bool RAW = false>
-constexpr int kLdsBytes = kStagesBytes<P, BM, BN, STAGES, RAW> + (LOGITS ? (int)sizeof(Known<BM, BN>) : 0);
+// Rows that leave together, what one of them takes, and whether the waves' maxima and sums find a place behind them in the
+// stages (256 x 256 tiles' exponentials fill those).
+template <typename P, int WN> constexpr int kRowsLeaving = WN * Unit<P>::size;
+template <typename P, int BM, int KIND> constexpr int kRowBytes = KIND == kOut || (KIND == kKeep && P::planes == 1) ? BM * 4 : BM * P::planes * 2;
+template <typename P, int BM, int BN, int WM, int WN, int KIND, int STAGES, bool RAW>
+constexpr bool kRoomBehind = KIND == kStats || kRowsLeaving<P, WN> * kRowBytes<P, BM, KIND> + WM * BN * 8 <= kStagesBytes<P, BM, BN, STAGES, RAW>;
+template <typename P, int BM, int BN, int WM, int WN, int KIND, int STAGES, bool RAW = false>
+constexpr int kLdsBytes = kStagesBytes<P, BM, BN, STAGES, RAW> + (KIND != kOut ? (int)sizeof(Known<BM, BN>) : 0) +
+                          (KIND == kKeep && !kRoomBehind<P, BM, BN, WM, WN, KIND, STAGES, RAW> ? WM * BN * 8 : 0);
 
 // Results on their way out: rows of COLS elements gathered in LDS, whose 16-byte pieces are exchanged by row, so that lanes
 // that each hold a few neighbours of another row do not meet in a bank; from there every row leaves as one stretch.  (Stored
@@ -609,8 +618,8 @@ __device__ __forceinline__ void product_tile(const Args &g, const int block, cha
         if constexpr (KIND != kOut) {
             if (threadIdx.x < BM) known.bias[threadIdx.x] = bias;
             if (threadIdx.x < BN)
-                known.want[threadIdx.x] = want, known.lse[threadIdx.x] = lse, known.scale[threadIdx.x] = scale,
-                known.power[threadIdx.x] = power;
+                known.want[threadIdx.x] = want, known.lse[threadIdx.x] = lse, known.scale[threadIdx.x] = scale;
+            if (P::half && KIND == kProb && threadIdx.x < BN) known.power[threadIdx.x] = power;
         }
     };
 
@@ -833,18 +842,21 @@ __device__ __forceinline__ void product_tile(const Args &g, const int block, cha
     float *fl = (float *)lds;
     // a logit, base 2
     auto logit = [&](int I, int j, int r) -> float { return fmaf(value(I, j, r), kLog2e, known.bias[m_in + m_of(I) + r]); };
-    constexpr int kRowsOut = WN * U::size, kThreads = WAVES * 64;  // rows that leave together: one j of every wave
+    constexpr int kRowsOut = kRowsLeaving<P, WN>, kThreads = WAVES * 64;  // one j of every wave
+    static_assert(KIND == kStats || kRowsOut * kRowBytes<P, BM, KIND> <= kStagesBytes<P, BM, BN, STAGES, (RAW > 0)>, "");
     auto n_of = [](int row, int j) { return (row / U::size * NT + j) * U::size + row % U::size; };
     const int row_out = wn * U::size + lane % U::size;
     // Four neighbouring probabilities to their place among the rows that leave.  Here they are rounded to the operands' type (of
-    // float32 nothing is lost in three planes): the second product's other operand has no more bits either, each rounding is
-    // independent of the others, and against 64 bits the gradients are as far off, 0.0017 of their norm in bfloat16, as a
-    // float32 computation rounded once at its end.
+    // float32 nothing is lost in three planes): the second product's other operand has no more bits either, and each rounding is
+    // independent of the others.  Against 64 bits the gradients of 2048 tokens over 32768 words are 0.0017 of their norm off in
+    // bfloat16, as a float32 computation rounded once at its end is; over 64 words, where more than the targets' probabilities
+    // count, 0.0020 (float16 0.00026 and 0.00021).  Two planes of P would halve the rate of both gradients' products.
     auto put_prob = [&](int I, float (&p)[4]) {
         typedef Gather<uint16_t, BM * NP> Out;
-        static_assert(KIND == kOut || kRowsOut * BM * NP * 2 <= kStagesBytes<P, BM, BN, STAGES, (RAW > 0)>, "");
         const int m = m_in + m_of(I);
-        if constexpr (NP > 1 && KIND == kKeep) {
+        if constexpr (NP == 1 && KIND == kKeep) {
+            *(f32x4 *)Gather<float, BM>::at(lds, row_out, m) = f32x4{p[0], p[1], p[2], p[3]};
+        } else if constexpr (KIND == kKeep) {
             *(f32x4 *)Out::at(lds, row_out, (m >> 5) * 96 + (m & 31) * 2) = f32x4{p[0], p[1], p[2], p[3]};
         } else if constexpr (NP == 1) {
             *(s16x4 *)Out::at(lds, row_out, m) = round4<P>(f32x4{p[0], p[1], p[2], p[3]} * (P::half ? kProbScale : 1.f));
@@ -861,11 +873,18 @@ __device__ __forceinline__ void product_tile(const Args &g, const int block, cha
     };
     auto leave_prob = [&](int j) {
         __syncthreads();
-        constexpr int kFilled = NP > 1 && KIND == kKeep ? 64 : 96;  // of three planes' place
-        Gather<uint16_t, BM * NP>::template leave<kThreads, kFilled, 96>(lds, kRowsOut, (g.prob_words - m0) * NP, [&](int row) -> uint16_t * {
-            const int t = n0 + n_of(row, j);
-            return t < g.N ? (uint16_t *)g.prob + t * g.ldp + m0 * NP : nullptr;
-        });
+        if constexpr (NP == 1 && KIND == kKeep) {
+            Gather<float, BM>::template leave<kThreads>(lds, kRowsOut, g.prob_words - m0, [&](int row) -> float * {
+                const int t = n0 + n_of(row, j);
+                return t < g.N ? g.kept + t * g.ld_kept + m0 : nullptr;
+            });
+        } else {
+            constexpr int kFilled = KIND == kKeep ? 64 : 96;  // of three planes' place
+            Gather<uint16_t, BM * NP>::template leave<kThreads, kFilled, 96>(lds, kRowsOut, (g.prob_words - m0) * NP, [&](int row) -> uint16_t * {
+                const int t = n0 + n_of(row, j);
+                return t < g.N ? (uint16_t *)g.prob + t * g.ldp + m0 * NP : nullptr;
+            });
+        }
         __syncthreads();
     };
     if constexpr (KIND == kStats || KIND == kKeep) {
@@ -910,8 +929,8 @@ __device__ __forceinline__ void product_tile(const Args &g, const int block, cha
             return sum;
         };
         // a place behind the rows on their way out, where other waves' results wait
-        float2 *const others = (float2 *)(lds + kStagesBytes<P, BM, BN, STAGES, (RAW > 0)>) - WM * BN;
-        static_assert(KIND == kStats || kRowsOut * BM * NP * 2 + WM * BN * 8 <= kStagesBytes<P, BM, BN, STAGES, (RAW > 0)>, "");
+        constexpr bool kRoom = kRoomBehind<P, BM, BN, WM, WN, KIND, STAGES, (RAW > 0)>;
+        float2 *const others = kRoom ? (float2 *)(lds + kStagesBytes<P, BM, BN, STAGES, (RAW > 0)>) - WM * BN : (float2 *)(&known + 1);
         if constexpr (KIND == kKeep) {
             // the tile's maximum first: what is kept is relative to it
 #pragma unroll
@@ -1007,7 +1026,6 @@ __device__ __forceinline__ void product_tile(const Args &g, const int block, cha
     }
     if constexpr (KIND == kOut) {
         typedef typename ElementOf<P>::type E;
-        static_assert(kRowsOut * BM * 4 <= kStagesBytes<P, BM, BN, STAGES, (RAW > 0)>, "");
         const float all = g.slice ? 1.f : out_factor<P>(g.factor);
 #pragma unroll
         for (int j = 0; j < NT; ++j) {
@@ -1039,7 +1057,7 @@ __device__ __forceinline__ void product_tile(const Args &g, const int block, cha
 template <typename P, int BM, int BN, int WM, int WN, bool A_ACROSS, bool B_ACROSS, int KIND, int STAGES>
 __global__ __launch_bounds__(WM * WN * 64) void product_kernel(Args g)
 {
-    __shared__ __attribute__((aligned(1024))) char lds[kLdsBytes<P, BM, BN, STAGES, KIND != kOut>];
+    __shared__ __attribute__((aligned(1024))) char lds[kLdsBytes<P, BM, BN, WM, WN, KIND, STAGES>];
     product_tile<P, BM, BN, WM, WN, A_ACROSS, B_ACROSS, KIND, STAGES>(g, blockIdx.x, lds);
 }
 
@@ -1051,7 +1069,7 @@ template <int KIND, int WIDTH>
 __global__ __launch_bounds__(256, 2) void raw_kernel(Args g)
 {
     constexpr int BM = kRawWords, BN = kRawTokens, STAGES = 2;
-    __shared__ __attribute__((aligned(1024))) char lds[kLdsBytes<Split, BM, BN, STAGES, KIND != kOut, true>];
+    __shared__ __attribute__((aligned(1024))) char lds[kLdsBytes<Split, BM, BN, 4, 1, KIND, STAGES, true>];
     product_tile<Split, BM, BN, 4, 1, KIND == kOut, false, KIND, STAGES, WIDTH>(g, blockIdx.x, lds);
 }
 
@@ -1059,7 +1077,7 @@ __global__ __launch_bounds__(256, 2) void raw_kernel(Args g)
 template <typename P, int BM, int BN, int WM, int WN, int STAGES>
 __global__ __launch_bounds__(WM * WN * 64) void both_kernel(Args hidden, Args weight, int first)
 {
-    __shared__ __attribute__((aligned(1024))) char lds[kLdsBytes<P, BM, BN, STAGES, false>];
+    __shared__ __attribute__((aligned(1024))) char lds[kLdsBytes<P, BM, BN, WM, WN, kOut, STAGES>];
     if ((int)blockIdx.x < first)
         product_tile<P, BM, BN, WM, WN, true, false, kOut, STAGES>(hidden, blockIdx.x, lds);
     else

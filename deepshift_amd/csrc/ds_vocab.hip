@@ -7,8 +7,8 @@
 // of them), the backward pass computes the logits of a piece of the vocabulary again, leaves that piece's P in a workspace of
 // a bounded size, and forms both gradients from it: four products of 2 T D V operations for a step, of which three are the
 // formula's own.  Where loss and gradients are asked for in one call, the forward pass leaves the last piece's exponentials,
-// relative to their tiles' maxima, in that workspace, and a pass over them makes them P: three products for that piece, which
-// may be the whole vocabulary.
+// relative to their tiles' maxima, in a workspace, in 32 bits, and a pass over them makes them P: three products for that piece,
+// which may be the whole vocabulary.
 #include "ds_vocab.h"
 #include <algorithm>
 
@@ -258,16 +258,19 @@ __global__ __launch_bounds__(256) void power_kernel(f16_t *__restrict__ prob, in
 
 // ---- exponentials to probabilities -----------------------------------------------------------------------------------
 
-// P[t][v] = scale_t (e[t][v] 2^(top[tile of v][t] - lse[t]) - [v = y_t]), in place; the target's own from its logit, in 32 bits.
-// A workgroup has 256 words of some rows, a thread 8 words of every eighth of them; its rows' sums are the bias's gradient.
-// 16-bit exponentials have been rounded once, and their probabilities are once more: bfloat16 gradients are 0.0021 of their norm
-// off instead of 0.0017, float16 ones 0.00022 instead of 0.00021, for one product less of four (float16 in place of bfloat16 would
-// hold nothing below 2^-39 of a tile's largest).
+// P[t][v] = e[t][v] 2^(top[tile of v][t] - lse[t]) - [v = y_t]; the target's own from its logit.  All in 32 bits until P is rounded to
+// the operands' type, once, as where the logits are formed again.  A workgroup has 256 words of some rows, a thread 8 words of
+// every eighth of them; its rows' sums are the bias's gradient.  float32's exponentials lie where their planes go, those of 16-bit
+// types in a place of their own.
 // Bound by memory: 2048 x 32768 float32 exponentials to three planes in 155 us, 0.67 GB at 4.3 TB/s, where forming the logits
-// again takes 830.
+// again takes 830; 8192 x 65536 bfloat16 probabilities from 32 bits in 590, 3.2 GB at 5.4 TB/s, where forming the logits again
+// takes 3500.  (Kept in 16 bits, and so rounded twice, their pass took 400 and the product before it 3530 instead of 3675, of
+// 23500 a step.)
 struct Finish {
     void *prob;
     int64_t ldp;
+    const float *kept;     // exponentials, rows of ld_kept; of float32 32 of every 48
+    int64_t ld_kept;
     int words, tile;       // words of a row, a multiple of 32; words a tile of the logits had
     int rows;              // of a workgroup, a multiple of 8
     int64_t v0, n;         // the piece: its first word, and how many there are
@@ -343,7 +346,7 @@ __global__ __launch_bounds__(256) void finish_kernel(Finish f)
     for (int e = 0; e < 8; ++e) over_t[e] = 0.f;
     const float2 *tops = r.stats + (int64_t)(f.tile0 + (word < f.words ? word / f.tile : 0)) * r.T;
     uint16_t *const column = (uint16_t *)f.prob + (NP == 1 ? word : (word >> 5) * 96 + (word & 31));
-    const float *const kept = (const float *)((uint16_t *)f.prob + (word >> 5) * 96) + (word & 31);  // of float32
+    const float *const kept = f.kept + (NP == 1 ? word : (word >> 5) * 48 + (word & 31));
 #pragma unroll JOIN ? 1 : 4
     for (int i = 0; i < f.rows; i += 8) {
         const int t = blockIdx.y * f.rows + i + part;
@@ -353,24 +356,14 @@ __global__ __launch_bounds__(256) void finish_kernel(Finish f)
         if (word >= f.words) continue;
         Vec<uint16_t, 8> *const at = (Vec<uint16_t, 8> *)(column + t * f.ldp);
         Vec<uint16_t, 8> v[NP];
-        f32x4 e32[2];
         // four neighbouring lanes' planes take the place of all their exponentials: each lane needs both of its loads for
         // any store, and a wave's loads are one instruction
-        if constexpr (NP == 3) e32[0] = *(const f32x4 *)(kept + t * (f.ldp / 2)), e32[1] = *(const f32x4 *)(kept + t * (f.ldp / 2) + 4);
-        else v[0] = at[0];
+        const f32x4 e32[2] = {*(const f32x4 *)(kept + t * f.ld_kept), *(const f32x4 *)(kept + t * f.ld_kept + 4)};
         // rows that do not count leave nothing; a target that is no word leaves no number
         const float factor = y == r.ignore ? 0.f : y < 0 || y >= r.V ? NAN : exp2f(tops[t].x - lse);
         float p[8];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            if constexpr (NP == 3)
-                p[e] = e32[e / 4][e % 4];
-            else if constexpr (P::half)
-                p[e] = to_float(f16_t{v[0].v[e]}) * (1.f / kProbScale);
-            else
-                p[e] = to_float(bf16_t{v[0].v[e]});
-            p[e] = y == r.ignore ? 0.f : p[e] * factor;
-        }
+        for (int e = 0; e < 8; ++e) p[e] = y == r.ignore ? 0.f : e32[e / 4][e % 4] * factor;
         const int64_t here = y - f.v0 - word;
         if (here >= 0 && here < 8 && word + here < f.n && y != r.ignore) {
             const float hot = exp2f(r.picked[t] - lse) - 1.f;
@@ -468,7 +461,8 @@ __global__ __launch_bounds__(256) void join_kernel(const float *__restrict__ sli
 // ---- plan --------------------------------------------------------------------------------------------------------
 
 // Workspace of a piece's P, and of its repacked weights.  Larger pieces mean fewer slices of the hidden gradient to join (95 us
-// a piece for 8192 tokens of 4096 features), smaller ones less memory; the products do not feel it.
+// a piece for 8192 tokens of 4096 features), smaller ones less memory; the products do not feel it.  The exponentials that a call
+// for loss and gradients keeps of 16-bit types take twice as much besides.
 constexpr size_t kPieceBytes = (size_t)1 << 30;
 
 // The tile shape of a product, and how many stretches its reduction of k is cut into (1 of `most_splits`): the pair with the
@@ -513,14 +507,14 @@ struct Plan {
     int64_t ldd;          // and what their rows take
     int64_t piece, pieces;
     bool pack_h, pack_w;
-    bool keep;            // the last piece's exponentials become its probabilities (run may decide against it)
+    bool keep;            // the last piece's exponentials become its probabilities
     bool few;             // ds_vocab_few.hip's kernels
     int raw;              // float32 weights as they are for the matrix cores, so many at a time, or 0
     int tile_logits, tile_words, tile_tokens;
     Choice hidden, weight;
     int words;            // of a piece's probabilities, a multiple of 32,
     int64_t ldp;          // and what a row of them takes
-    size_t h, w, stats, picked, shares, arrived, prob, bias, slices, acc, scale, power, factor, bytes;
+    size_t h, w, stats, picked, shares, arrived, prob, kept, bias, slices, acc, scale, power, factor, bytes;
 };
 
 inline bool in_place(const void *p, int64_t ld, int64_t D) { return (uintptr_t)p % 16 == 0 && ld % 8 == 0 && D % 8 == 0; }
@@ -612,7 +606,9 @@ Plan plan_of(const void *hidden, int64_t ldh, const void *weight, int64_t ldw, i
             const size_t n = (size_t)p.weight.splits * p.piece * D * 4;
             slices = n > slices ? n : slices;
         }
-        p.slices = take(slices);
+        // exponentials are probabilities before there is anything in the slices
+        const size_t kept = p.keep && NP == 1 ? (size_t)T * p.words * 4 : 0;
+        p.kept = p.slices = take(slices > kept ? slices : kept);
         if (p.pieces > 1) p.acc = take((size_t)T * D * 4);
         p.scale = take((size_t)T * 4);
         if (P::half) p.power = take((size_t)T * 4);
@@ -716,6 +712,7 @@ int loss(const Call &c, const Plan &p, bool counted_only, Operands<P> &o, int re
         g.picked = (float *)(c.ws + p.picked);
         g.arrived = (uint32_t *)(c.ws + p.arrived);
         g.prob = c.ws + p.prob, g.ldp = p.ldp, g.prob_words = p.words;
+        g.kept = (float *)(c.ws + p.kept), g.ld_kept = p.words;
         DS_TRY(product<P>(p, p.keep && v0 + n == c.V ? kLogitKeep : kLogitStats, p.tile_logits, g, c.T, c.st));
         tiles += g.tiles_m;
     }
@@ -761,7 +758,8 @@ int loss_grad(const Call &c, const Plan &p, Operands<P> &o, const Rows &of, Grad
             void *const bias_out = r.dbias && !bias_left ? (E *)r.dbias + v0 : nullptr;
             if (kept) {
                 const int words = ceil_div((int)n, 32) * 32;
-                const Finish f{c.ws + p.prob, p.ldp, words, p.tile_words, rows, v0, n, of.tiles - ceil_div((int)n, p.tile_words),
+                const bool beside = P::planes == 1;
+                const Finish f{c.ws + p.prob, p.ldp, (const float *)(c.ws + (beside ? p.kept : p.prob)), beside ? p.words : p.ldp / 2, words, p.tile_words, rows, v0, n, of.tiles - ceil_div((int)n, p.tile_words),
                                p.words, of, bias_part, bias_out, {r.grad, r.share}};
                 const unsigned along = ceil_div(words, 256), down = ceil_div((int)c.T, rows);
                 if (joined_later(p, c.T, of.tiles))
@@ -853,9 +851,7 @@ struct Outputs {
 template <typename P>
 int run(const Call &c, int what, const Outputs &out)
 {
-    Plan p = plan_of<P>(c.hidden, c.ldh, c.weight, c.ldw, c.T, c.D, c.V, what);
-    // a bias's gradient sums what has not been rounded to 16 bits
-    p.keep = p.keep && (P::planes == 3 || !out.grads.dbias);
+    const Plan p = plan_of<P>(c.hidden, c.ldh, c.weight, c.ldw, c.T, c.D, c.V, what);
     if (!c.ws || c.ws_bytes < p.bytes || (uintptr_t)c.ws % 256) return DS_EWORKSPACE;
     Operands<P> o;
     Rows of{};

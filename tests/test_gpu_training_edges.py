@@ -93,6 +93,23 @@ def test_gradients_of_rows_far_apart_keep_their_bits(dtype):
             assert all(torch.equal(x, z) for x, z in zip((dh, dw, db), again))
 
 
+# ---- roundings --------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("dtype", TYPES[1:], ids=str)
+def test_probabilities_are_rounded_once(dtype):
+    # one token: a weight's gradient is one product, p rounded to the type times h, rounded to the type
+    for D, V in [(64, 8192), (40, 20000)]:
+        g = _gen(D, V, 73)
+        h, w, b, y = _head(1, D, V, dtype, False, g)
+        p, off = _softmax(h, w, None)
+        p = p.scatter_add(1, y[:, None], torch.full((1, 1), -1.0, dtype=torch.float64, device=DEV))
+        want = p.t() @ h.double()
+        bound = (off + p.abs() * U[dtype] + TINY[dtype] * 2.0 ** -14).t() @ h.double().abs()
+        bound = bound + (U[dtype] + 4 * E) * (want.abs() + bound) + TINY[dtype]
+        for dw in (training.linear_cross_entropy_grad(h, w, y, reduction="sum")[2], _backward(h, w, None, y, None, reduction="sum")[1]):
+            _within(dw, want, bound, "dweight")
+
+
 # ---- tensors that overlap -----------------------------------------------------------------------------------------
 
 def test_clipping_refuses_to_write_what_another_tensor_reads():
