@@ -984,6 +984,7 @@ __device__ __forceinline__ void product_tile(const Args &g, const int block, cha
             const float lse = known.lse[n_in + j * U::size], scale = known.scale[n_in + j * U::size];
             const float power = P::half ? known.power[n_in + j * U::size] : 1.f;
             const float least = lse == INFINITY ? -INFINITY : -126.f;
+            const bool counts = !(lse == INFINITY && scale == 0.f);  // else nothing is left, also of infinite weights times 0
             const int at = known.want[n_in + j * U::size] - m_in;
 #pragma unroll
             for (int I = 0; I < MG; ++I) {
@@ -996,7 +997,7 @@ __device__ __forceinline__ void product_tile(const Args &g, const int block, cha
                     for (int r = 0; r < 4; ++r) p[r] -= at == m_of(I) + r ? 1.f : 0.f;
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
-                    p[r] *= scale;
+                    p[r] = counts ? p[r] * scale : 0.f;
                     over_n[I * 4 + r] += p[r] * power;
                 }
                 put_prob(I, p);

@@ -110,6 +110,28 @@ def test_probabilities_are_rounded_once(dtype):
             _within(dw, want, bound, "dweight")
 
 
+# ---- infinities -------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+def test_tokens_that_do_not_count_leave_nothing_whatever_weights_hold(dtype):
+    for T, D, V in [(4, 40, 200), (70, 48, 300), (20, 1024, 8200), (300, 64, 513)]:
+        print(T, D, V, flush=True)
+        g = _gen(T, D, V, 77)
+        h, w, b, y = _head(T, D, V, dtype, True, g)
+        h[:, 1] = h[:, 1].abs() + 0.25
+        y = y % 100
+        y[2::5] = -100
+        h[2::5] = float("nan")
+        other = torch.arange(D, device=DEV) != 1    # there it is 0 times infinity
+        for words in ([150], [100, 150, V - 1]):
+            w[words, 1] = -float("inf")
+            for up in (None, _rand(g, T)):
+                dh, dw, db = _backward(h, w, b, y, up, reduction="mean" if up is None else "none")
+                assert (dh[y == -100][:, other] == 0).all()
+            _, dh, dw, db = training.linear_cross_entropy_grad(h, w, y, b)
+            assert (dh[y == -100][:, other] == 0).all()
+
+
 # ---- tensors that overlap -----------------------------------------------------------------------------------------
 
 def test_clipping_refuses_to_write_what_another_tensor_reads():
