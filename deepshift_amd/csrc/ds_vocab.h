@@ -11,7 +11,8 @@
 // float32 operands come as three bfloat16 planes, x = x0 + 2^-8 x1 + 2^-16 x2, and a product is the sum of the six plane
 // products above 2^-24 of it (x0 y0, x0 y1, x1 y0, x1 y1, x0 y2, x2 y0): six times the bf16 work at a rate of bf16, where the
 // float32 matrix instructions take sixteen times the time of bf16.  The planes' factors keep all 24 bits of the smallest
-// values, which planes without them would lose below 2^-110.
+// values, which planes without them would lose below 2^-110.  Results that infinities make NaN in them are formed again from
+// the largest planes (product_tile).
 //
 // What bounds them: large ones the power of the chip, which holds the clock at 1.5 to 1.6 GHz while the matrix cores are busy 70
 // to 85 % of the cycles (a library's products of the same sizes run at the same rate).  A piece of 8192 tokens x 65536 words x
@@ -475,7 +476,8 @@ template <typename P, int BM, int BN, int WM, int WN, int KIND, int STAGES, bool
 constexpr bool kRoomBehind = KIND == kStats || kRowsLeaving<P, WN> * kRowBytes<P, BM, KIND> + WM * BN * 8 <= kStagesBytes<P, BM, BN, STAGES, RAW>;
 template <typename P, int BM, int BN, int WM, int WN, int KIND, int STAGES, bool RAW = false>
 constexpr int kLdsBytes = kStagesBytes<P, BM, BN, STAGES, RAW> + (KIND != kOut ? (int)sizeof(Known<BM, BN>) : 0) +
-                          (KIND == kKeep && !kRoomBehind<P, BM, BN, WM, WN, KIND, STAGES, RAW> ? WM * BN * 8 : 0);
+                          (KIND == kKeep && !kRoomBehind<P, BM, BN, WM, WN, KIND, STAGES, RAW> ? WM * BN * 8 : 0) +
+                          (P::planes > 1 ? 16 : 0);
 
 // Results on their way out: rows of COLS elements gathered in LDS, whose 16-byte pieces are exchanged by row, so that lanes
 // that each hold a few neighbours of another row do not meet in a bank; from there every row leaves as one stretch.  (Stored
@@ -614,7 +616,9 @@ __device__ __forceinline__ void product_tile(const Args &g, const int block, cha
         }
     }
 
+    int *const met_nan = (int *)(lds + kLdsBytes<P, BM, BN, WM, WN, KIND, STAGES, (RAW > 0)>) - 1;  // of float32: a result is NaN
     auto keep_known = [&] {
+        if (NP > 1 && threadIdx.x == 0) *met_nan = 0;
         if constexpr (KIND != kOut) {
             if (threadIdx.x < BM) known.bias[threadIdx.x] = bias;
             if (threadIdx.x < BN)
@@ -830,9 +834,66 @@ __device__ __forceinline__ void product_tile(const Args &g, const int block, cha
         if constexpr (RAW)
             if (__syncthreads_or(top >= TA::kLimit)) products(std::true_type());
     }
+    if constexpr (NP > 1) {
+        bool odd = false;
+#pragma unroll
+        for (int i = 0; i < MT; ++i)
+#pragma unroll
+            for (int j = 0; j < NT; ++j)
+                odd |= __builtin_isunordered(acc[i][j][0], acc[i][j][1]) || __builtin_isunordered(acc[i][j][2], acc[i][j][3]);
+        if (odd) *met_nan = 1;
+    }
     // nothing of this wave is on its way to LDS any more, and nobody reads it
     asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
     __syncthreads();
+    if constexpr (NP > 1) {
+        // An infinity times a lower plane of 0, or of the other sign than its value, makes a result NaN that may be infinite.
+        // The largest planes have the values' signs, zeros and infinities: their product alone says which it is.  A row of
+        // the wave's tiles at a time, for the whole workgroup where a lane has met one, so that all of it fetches.  Looking for
+        // them takes 0.2 us of a launch of 12 (with this code in the way of what follows 0.4).
+        if (__builtin_expect(*met_nan, 0)) {
+#pragma unroll
+            for (int i = 0; i < MT; ++i) {
+                f32x4 largest[NT];
+#pragma unroll
+                for (int j = 0; j < NT; ++j) largest[j] = f32x4{0.f, 0.f, 0.f, 0.f};
+                a_at = (uint64_t)g.a.at + TA::rows_bytes(g.a, m0) + k_from / kStep * a_step;
+                b_at = (uint64_t)g.b.at + TB::rows_bytes(g.b, n0) + k_from / kStep * b_step;
+                k_left = k_to - k_from;
+#pragma unroll 1
+                for (int s = 0; s < steps; ++s) {
+#pragma unroll
+                    for (int f = 0; f < TA::mine; ++f) ta.one(a_at, k_left, lds0, wave, 0, f);
+#pragma unroll
+                    for (int f = 0; f < TB::mine; ++f) tb.one(b_at, k_left, lds0 + kBytesA, wave, 0, f);
+                    a_at += a_step, b_at += b_step, k_left -= kStep;
+                    wait_for_stage<0>();
+                    s16x8 fa;
+                    if constexpr (RAW) {
+                        float x[8];
+                        TA::load(lds, (wm * MT + i) * U::size, x);
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) {
+                            bf16_t planes[3];
+                            split_planes(x[e], planes);
+                            fa[e] = (short)planes[0].bits;
+                        }
+                    } else {
+                        fa = TA::fragment(lds, (wm * MT + i) * U::size, 0);
+                    }
+#pragma unroll
+                    for (int j = 0; j < NT; ++j)
+                        largest[j] = U::multiply(fa, TB::fragment(lds + kBytesA, (wn * NT + j) * U::size, 0), largest[j]);
+                    wait_for_stage<0>();
+                }
+#pragma unroll
+                for (int j = 0; j < NT; ++j)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r)
+                        if (acc[i][j][r] != acc[i][j][r]) acc[i][j][r] = largest[j][r];
+            }
+        }
+    }
 
     // This lane's results: I counts its groups of four neighbouring m, j its n.
     constexpr int MG = MT * U::groups;

@@ -132,6 +132,68 @@ def test_tokens_that_do_not_count_leave_nothing_whatever_weights_hold(dtype):
             assert (dh[y == -100][:, other] == 0).all()
 
 
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+def test_an_infinite_weight_takes_a_word_out(dtype):
+    for T, D, V, kb in [(4, 40, 200, 0), (20, 40, 200, 0), (70, 48, 300, 0), (150, 33, 700, 1), (300, 256, 515, 0), (20, 1024, 8200, 0),
+                        (20, 1023, 8300, 0), (100, 1024, 8200, 0)]:
+        g = _gen(T, D, V, 74)
+        h, w, b, y = _head(T, D, V, dtype, True, g)
+        h[:, 1] = h[:, 1].abs().clamp(min=0.25)
+        h[::3, 1], h[1::3, 1] = 1.0, 0.3      # with and without bits behind bfloat16's
+        out = torch.tensor([0, V // 2, V - 1], device=DEV)
+        y = 1 + y % (V // 2 - 1)
+        y[2::5] = -100
+        masked, bias = w.clone(), b.clone()
+        masked[out, 1], bias[out] = 0.0, -float("inf")
+        w[out, 1] = -float("inf")
+        w[out[1], 2], masked[out[1], 2] = 0.3, 0.3
+        other = torch.arange(D, device=DEV) != 1
+        share = torch.full((T,), 1.0 / int((y != -100).sum()), device=DEV)
+        for tile in (-1, 0, 1, 2, 3):
+            print(T, D, V, tile, flush=True)
+            tune = dict(vocab_tile=tile) if tile >= 0 else {}
+            if kb:
+                tune["vocab_piece_kb"] = kb
+            with Tune(**tune):
+                rows = training.linear_cross_entropy(h, w, y, b, reduction="none")
+                _, *step = training.linear_cross_entropy_grad(h, w, y, b)
+                auto = _backward(h, w, b, y, None)
+            for dh, dw, db in (step, auto):
+                # 0 times infinity where the weight is, nothing else
+                assert dh[y != -100][:, 1].isnan().all()
+                dh = torch.where(other, dh, _masked_column(h, masked, bias, y, share, dtype))
+                _head_check(h, masked, bias, y, -100, share, rows, dh, dw, db)
+
+
+def _masked_column(h, w, b, y, share, dtype):
+    """The definition's ``dhidden``, in place of a column that is not looked at."""
+    s = torch.where((y != -100)[:, None], h, torch.zeros_like(h)).double() @ w.double().t() + b.double()
+    p = s.softmax(1).scatter_add(1, y.clamp(min=0)[:, None], torch.full((len(y), 1), -1.0, dtype=torch.float64, device=DEV))
+    return ((p * (share * (y != -100)).double()[:, None]) @ w.double()).to(dtype)
+
+
+def test_float32_infinities_do_what_they_do_in_64_bits():
+    # every path of float32, and every kind of product that an infinity may be in
+    for T, D, V in [(5, 8, 20), (17, 8, 20), (40, 2048, 4200), (40, 2047, 4200), (200, 40, 300)]:
+        print(T, D, V, flush=True)
+        g = _gen(T, D, V, 75)
+        h, w, b, y = _head(T, D, V, torch.float32, False, g)
+        y = y % 7
+        h[0, 2], w[:, 2] = -float("inf"), w[:, 2].abs() + 0.1   # every logit of a token -inf
+        h[1, 3] = float("inf")                                  # signs of both kinds
+        w[V - 1, 4], h[:, 4] = float("inf"), -h[:, 4].abs() - 0.1   # a word taken out
+        w[V - 2, 5], h[2, 5] = float("inf"), 0.0                # 0 times infinity
+        h[3:, 5] = -0.5
+        rows = training.linear_cross_entropy(h, w, y, reduction="none")
+        s = h.double() @ w.double().t()
+        assert s[2, V - 2].isnan() and s[0].isneginf().sum() >= V - 2
+        assert rows[:3].isnan().all()
+        s = s[3:, :V - 2]
+        want = s.logsumexp(1) - s.gather(1, y[3:, None])[:, 0]
+        size = (h[3:].abs().double() @ w[:V - 2].abs().double().t()).amax(1)
+        _within(rows[3:], want, 2 * (D + 8) * E * size + (6 * size + 20) * E, "loss")
+
+
 # ---- tensors that overlap -----------------------------------------------------------------------------------------
 
 def test_clipping_refuses_to_write_what_another_tensor_reads():
