@@ -235,6 +235,15 @@ PyObject *tuple_of(std::initializer_list<at::Tensor> tensors)
     return t;
 }
 
+// A scalar of its own on element `i` of `t`'s memory: what a Function returns may be changed in place (loss /= n), unless it is a
+// view, and counts its changes by itself.
+at::Tensor scalar_at(const at::Tensor &t, int64_t i)
+{
+    at::Tensor s = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(t.storage()), t.key_set(), t.dtype());
+    s.unsafeGetTensorImpl()->set_sizes_and_strides(at::IntArrayRef{}, at::IntArrayRef{}, t.storage_offset() + i);
+    return s;
+}
+
 // What a call finds out about the losses of rows.
 struct Losses {
     int reduction;
@@ -246,7 +255,8 @@ struct Losses {
         lse = h.empty({h.T}, at::kFloat);
         if (reduction) total = h.empty({2}, at::kFloat);
     }
-    at::Tensor result() const { return reduction ? total.select(0, 0) : rows; }
+    at::Tensor result() const { return reduction ? scalar_at(total, 0) : rows; }
+    at::Tensor share() const { return reduction ? scalar_at(total, 1) : at::Tensor(); }
 };
 
 // cross_entropy(hidden, weight, target, bias or None, ignore, reduction, stream): the loss, and what its gradients need: the
@@ -262,7 +272,7 @@ PyObject *cross_entropy(PyObject *, PyObject *const *args, Py_ssize_t count)
                              h.target.const_data_ptr(), (int)h.target.element_size(), h.ignore, h.T, h.D, h.V, h.type, l.reduction,
                              at_or_null<float>(l.rows), at_or_null<float>(l.lse), at_or_null<float>(l.total),
                              ws.mutable_data_ptr(), ws.nbytes(), stream(args[6])));
-        return tuple_of({l.result(), l.lse, l.reduction ? l.total.select(0, 1) : at::Tensor()});
+        return tuple_of({l.result(), l.lse, l.share()});
     });
 }
 

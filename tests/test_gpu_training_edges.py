@@ -194,6 +194,30 @@ def test_float32_infinities_do_what_they_do_in_64_bits():
         _within(rows[3:], want, 2 * (D + 8) * E * size + (6 * size + 20) * E, "loss")
 
 
+# ---- losses -----------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("reduction", ["none", "sum", "mean"])
+def test_a_loss_may_be_changed_in_place(reduction):
+    g = _gen(76)
+    h, w, b, y = _head(9, 16, 30, torch.float32, True, g)
+    want = _backward(h, w, b, y, torch.full((9,) if reduction == "none" else (), 0.5, device=DEV), reduction=reduction)
+    leaves = [x.detach().requires_grad_() for x in (h, w, b)]
+    loss = training.linear_cross_entropy(leaves[0], leaves[1], y, leaves[2], reduction=reduction)
+    assert loss._base is None
+    before = loss.detach().clone()
+    loss /= 2
+    loss += 3.0
+    assert torch.equal(loss, before / 2 + 3.0)
+    loss.sum().backward()
+    assert all(torch.equal(x.grad, z) for x, z in zip(leaves, want))
+    for loss in (training.linear_cross_entropy(h, w, y, b, reduction=reduction),
+                 training.linear_cross_entropy_grad(h, w, y, b, reduction=reduction)[0]):
+        assert loss._base is None and loss.shape == before.shape
+        before = loss.clone()
+        loss *= 2
+        assert torch.equal(loss, before * 2)
+
+
 # ---- tensors that overlap -----------------------------------------------------------------------------------------
 
 def test_clipping_refuses_to_write_what_another_tensor_reads():
