@@ -47,7 +47,10 @@ template <typename... T> [[noreturn]] void refuse(PyObject *type, const T &...pa
 const at::Tensor &tensor(const char *name, PyObject *o)
 {
     if (!THPVariable_Check(o)) refuse(PyExc_TypeError, name, " must be a tensor, is ", Py_TYPE(o)->tp_name);
-    return THPVariable_Unpack(o);
+    const at::Tensor &t = THPVariable_Unpack(o);
+    if (t._fw_grad(0).defined())
+        refuse(PyExc_NotImplementedError, name, " has a tangent, and these operators have no forward-mode derivatives");
+    return t;
 }
 
 int checked_type(const char *name, const at::Tensor &t)

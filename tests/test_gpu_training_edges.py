@@ -218,6 +218,23 @@ def test_a_loss_may_be_changed_in_place(reduction):
         assert torch.equal(loss, before * 2)
 
 
+# ---- what is recorded -------------------------------------------------------------------------------------------
+
+def test_forward_mode_is_refused_on_the_gpu():
+    import torch.autograd.forward_ad as forward_ad
+    g = _gen(78)
+    h, w, b, y = _head(9, 16, 30, torch.float32, True, g)
+    leaf = w.clone().requires_grad_()
+    with forward_ad.dual_level():
+        dual = {k: forward_ad.make_dual(t, torch.ones_like(t)) for k, t in dict(h=h, w=w, b=b).items()}
+        for call in (lambda: training.embedding(y, dual["w"]), lambda: training.embedding_grad(y, dual["h"], 30),
+                     lambda: training.linear_cross_entropy(dual["h"], w, y, b), lambda: training.linear_cross_entropy(h, dual["w"], y, b),
+                     lambda: training.linear_cross_entropy(h, leaf, y, dual["b"]), lambda: training.gradient_norm([h, dual["w"]]),
+                     lambda: training.clip_gradients_([h.clone()], 1.0, out=[dual["h"]])):
+            with pytest.raises(NotImplementedError, match="forward"):
+                call()
+
+
 # ---- tensors that overlap -----------------------------------------------------------------------------------------
 
 def test_clipping_refuses_to_write_what_another_tensor_reads():

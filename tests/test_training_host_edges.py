@@ -6,6 +6,8 @@ import torch
 
 from deepshift_amd import training
 
+IDS, X, W = torch.zeros(3, dtype=torch.int64), torch.ones(3, 4), torch.ones(5, 4)
+
 
 def test_whether_tensors_meet_is_told_exactly():
     # against the bytes themselves
@@ -28,3 +30,14 @@ def test_whether_tensors_meet_is_told_exactly():
     with pytest.raises(ValueError, match="share"):
         training._check_apart([base[:, :1].expand(6, 4)])
     training._check_apart([base[:, 2:5], base[:, 5:], base[:, :2].t(), base[:0]])
+
+
+def test_forward_mode_is_refused():
+    import torch.autograd.forward_ad as forward_ad
+    with forward_ad.dual_level():
+        w, x = forward_ad.make_dual(W, torch.ones_like(W)), forward_ad.make_dual(X, torch.ones_like(X))
+        for call in (lambda: training.embedding(IDS, w), lambda: training.embedding_grad(IDS, x, 5),
+                     lambda: training.linear_cross_entropy(x, W, IDS), lambda: training.linear_cross_entropy_grad(X, w, IDS),
+                     lambda: training.gradient_norm([x, X]), lambda: training.clip_gradients_([x], 1.0, out=[X])):
+            with pytest.raises(NotImplementedError, match="forward"):
+                call()
