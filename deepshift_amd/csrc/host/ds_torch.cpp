@@ -4,8 +4,10 @@
 // Bound by the launches themselves (2.7 us each) and torch's allocations (0.8 us).
 #include <Python.h>
 #include <torch/csrc/autograd/python_variable.h>
+#include <ATen/TracerMode.h>
 #include <ATen/core/Tensor.h>
 #include <ATen/ops/empty.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <algorithm>
 #include <string>
 #include <vector>
@@ -85,11 +87,22 @@ void expect(const char *entry, int status)
     if (status != DS_OK) throw Failure{entry, status};
 }
 
+// A trace would hold the allocation of a result, and nothing that writes it.
+void refuse_tracing()
+{
+    namespace modes = c10::impl;
+    if (at::tracer::impl::is_dispatch_enabled() ||
+        (modes::TorchDispatchModeTLS::any_modes_set() &&
+         modes::TorchDispatchModeTLS::get_mode(modes::TorchDispatchModeKey::PROXY).has_value()))
+        refuse(PyExc_NotImplementedError, "these operators cannot be traced");
+}
+
 // Runs an entry point; whatever is thrown in it becomes a Python exception.
 template <typename F> PyObject *guarded(Py_ssize_t got, Py_ssize_t wanted, F &&body)
 {
     try {
         if (got != wanted) refuse(PyExc_TypeError, std::to_string(wanted), " arguments expected");
+        refuse_tracing();
         return body();
     } catch (const Refusal &r) {
         if (r.type) PyErr_SetString(r.type, r.text.c_str());

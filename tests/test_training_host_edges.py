@@ -41,3 +41,18 @@ def test_forward_mode_is_refused():
                      lambda: training.gradient_norm([x, X]), lambda: training.clip_gradients_([x], 1.0, out=[X])):
             with pytest.raises(NotImplementedError, match="forward"):
                 call()
+
+
+def test_tracing_is_refused():
+    from torch.fx.experimental.proxy_tensor import make_fx
+    for call, arg in ((lambda w: training.embedding(IDS, w), W), (lambda x: training.embedding_grad(IDS, x, 5), X),
+                      (lambda x: training.linear_cross_entropy(x, W, IDS), X),
+                      (lambda x: training.linear_cross_entropy_grad(x, W, IDS)[:3], X),
+                      (lambda x: training.linear_cross_entropy(x, W.clone().requires_grad_(), IDS), X),
+                      (lambda x: training.gradient_norm([x]), X), (lambda x: training.clip_gradients_([x], 1.0), X)):
+        with pytest.raises(NotImplementedError, match="trac"):
+            torch.jit.trace(call, (arg,))
+        with pytest.raises(NotImplementedError, match="trac"):
+            make_fx(call)(arg)
+    with pytest.raises(ValueError, match="GPU"):
+        training.embedding(IDS, W)      # and afterwards it is as before
