@@ -52,6 +52,7 @@ const at::Tensor &tensor(const char *name, PyObject *o)
     const at::Tensor &t = THPVariable_Unpack(o);
     if (t._fw_grad(0).defined())
         refuse(PyExc_NotImplementedError, name, " has a tangent, and these operators have no forward-mode derivatives");
+    if (t.is_neg()) refuse(PyExc_ValueError, name, " is a lazily negated view: resolve_neg() gives its values");
     return t;
 }
 

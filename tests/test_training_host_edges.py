@@ -56,3 +56,11 @@ def test_tracing_is_refused():
             make_fx(call)(arg)
     with pytest.raises(ValueError, match="GPU"):
         training.embedding(IDS, W)      # and afterwards it is as before
+
+
+def test_lazily_negated_tensors_are_refused():
+    w = torch._neg_view(W)
+    with pytest.raises(ValueError, match="resolve_neg"):
+        training.embedding(IDS, w)
+    with pytest.raises(ValueError, match="resolve_neg"):
+        training.clip_gradients_([w], 1.0)
