@@ -90,9 +90,9 @@ def embedding(ids, weight, scale=1.0, padding_idx=None):
     scale = float(scale)
     if not math.isfinite(scale):
         raise ValueError("scale must be finite")
+    if padding_idx is not None and weight.dim() == 2:
+        _padding(padding_idx, weight.shape[0])
     if weight.requires_grad and torch.is_grad_enabled():
-        if weight.dim() == 2:
-            _padding(padding_idx, weight.shape[0])
         return _Embedding.apply(ids, weight, scale, padding_idx)
     return _embed(ids, weight, scale)
 

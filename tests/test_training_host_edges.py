@@ -64,3 +64,9 @@ def test_lazily_negated_tensors_are_refused():
         training.embedding(IDS, w)
     with pytest.raises(ValueError, match="resolve_neg"):
         training.clip_gradients_([w], 1.0)
+
+
+def test_a_wrong_padding_idx_is_refused_without_gradients_too():
+    for padding in (5, -6):
+        with pytest.raises(ValueError, match="padding_idx"):
+            training.embedding(IDS, W, padding_idx=padding)
