@@ -10,7 +10,6 @@ Functions whose names end in ``_grad`` return gradients directly; ``embedding`` 
 in autograd.
 """
 import contextlib
-import math
 
 import torch
 import torch.nn as nn
@@ -53,11 +52,21 @@ def embedding_grad(ids, grad, num_embeddings, scale=1.0, padding_idx=None):
     """Gradient of :func:`embedding` with respect to its weight, ``[num_embeddings, D]`` in ``grad``'s type: row ``v`` is
     ``scale`` times the sum of ``grad`` over the tokens ``v``, in ascending order and 32 bits.  Tokens equal to
     ``padding_idx`` add nothing, and neither do numbers outside ``[0, num_embeddings)``."""
-    V = int(num_embeddings)
+    V, scale = int(num_embeddings), _scale(scale)
     padding = _padding(padding_idx, V)
     device = grad.device
     with _on(device):
-        return _lib.native().embed_grad(ids, grad, V, float(scale), padding, _stream_of(device))
+        return _lib.native().embed_grad(ids, grad, V, scale, padding, _stream_of(device))
+
+
+_LARGEST = (2 - 2.0 ** -24) * 2.0 ** 127   # float32 rounds it, and what is beyond, to infinity
+
+
+def _scale(scale):
+    scale = float(scale)
+    if not abs(scale) < _LARGEST:
+        raise ValueError("scale must be finite in float32, is %r" % scale)
+    return scale
 
 
 def _padding(padding_idx, V):
@@ -87,9 +96,7 @@ def embedding(ids, weight, scale=1.0, padding_idx=None):
     """``scale * weight[ids]`` for ``ids`` of any shape (int64 or int32) and ``weight`` ``[V, D]``, multiplied in 32 bits and
     rounded once.  A number outside ``[0, V)`` gives a row of NaN (the GPU cannot raise).  ``padding_idx`` names the word
     whose row gets no gradient."""
-    scale = float(scale)
-    if not math.isfinite(scale):
-        raise ValueError("scale must be finite")
+    scale = _scale(scale)
     if padding_idx is not None and weight.dim() == 2:
         _padding(padding_idx, weight.shape[0])
     if weight.requires_grad and torch.is_grad_enabled():

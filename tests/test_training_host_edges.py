@@ -70,3 +70,11 @@ def test_a_wrong_padding_idx_is_refused_without_gradients_too():
     for padding in (5, -6):
         with pytest.raises(ValueError, match="padding_idx"):
             training.embedding(IDS, W, padding_idx=padding)
+
+
+@pytest.mark.parametrize("scale", [1e39, -1e39, float("inf"), float("nan")])
+def test_scales_beyond_float32_are_refused(scale):
+    with pytest.raises(ValueError, match="scale"):
+        training.embedding(IDS, W, scale)
+    with pytest.raises(ValueError, match="scale"):
+        training.embedding_grad(IDS, X, 5, scale)
