@@ -271,10 +271,12 @@ def clip_gradients_(grads, max_norm, out=None):
         return _clip(grads, max_norm, out, True)
 
 
-def clip_grad_norm_(parameters, max_norm, error_if_nonfinite=False):
+def clip_grad_norm_(parameters, max_norm, norm_type=2.0, error_if_nonfinite=False):
     """Clips the ``.grad`` of ``parameters`` (those that have one) in place by their global 2-norm, which is returned: the
-    counterpart of ``torch.nn.utils.clip_grad_norm_``.  ``error_if_nonfinite`` raises before anything is scaled, and waits
-    for the GPU to know."""
+    counterpart of ``torch.nn.utils.clip_grad_norm_`` for gradients on one device; a ``norm_type`` other than 2 is refused.
+    ``error_if_nonfinite`` raises before anything is scaled, and waits for the GPU to know."""
+    if isinstance(norm_type, (bool, str)) or norm_type != 2:
+        raise ValueError("norm_type must be 2, is %r" % (norm_type,))
     parameters = [parameters] if isinstance(parameters, torch.Tensor) else parameters
     grads = [p.grad for p in parameters if p.grad is not None]
     if not grads:

@@ -78,3 +78,13 @@ def test_scales_beyond_float32_are_refused(scale):
         training.embedding(IDS, W, scale)
     with pytest.raises(ValueError, match="scale"):
         training.embedding_grad(IDS, X, 5, scale)
+
+
+@pytest.mark.parametrize("norm_type", [1, 1.0, float("inf"), 0, "fro"])
+def test_norms_other_than_the_second_are_refused(norm_type):
+    p = torch.nn.Parameter(torch.ones(3))
+    p.grad = torch.ones(3)
+    with pytest.raises(ValueError, match="norm_type"):
+        training.clip_grad_norm_([p], 1.0, norm_type)
+    with pytest.raises(ValueError, match="norm_type"):
+        training.clip_grad_norm_([p], 1.0, norm_type=norm_type)
