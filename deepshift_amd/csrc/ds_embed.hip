@@ -456,22 +456,35 @@ inline EmbedSpace embed_space(int64_t T, int64_t D)
     return s;
 }
 
-template <typename E>
-int launch_embed_grad(const uint32_t *keys, const uint32_t *pos, const void *g, int64_t ldg, void *dw, float *part, int64_t T,
-                      int64_t D, float scale, hipStream_t st)
+// How the sums' launches go over a gradient: `width` columns a lane, `any`: wherever its rows begin.
+struct SumGrid {
+    int width, chunk;
+    bool any;
+    int64_t chunks, slices;
+    bool fits() const { return chunks <= 0x7fffffff && slices <= 65535; }
+};
+inline SumGrid sum_grid(int bytes, const void *g, int64_t ldg, const void *dw, int64_t T, int64_t D)
 {
-    constexpr int kWide = 16 / sizeof(E);
-    int n = vector_elements(sizeof(E), {D, ldg}, {g, dw});
-    const int chunk = embed_chunk(T);
-    const int64_t chunks = (T + chunk - 1) / chunk;
+    const int wide = 16 / bytes;
+    SumGrid s{vector_elements(bytes, {D, ldg}, {g, dw}), embed_chunk(T), false, 0, 0};
+    s.chunks = (T + s.chunk - 1) / s.chunk;
     auto slices_of = [&](int width) { return ((D + width - 1) / width + 63) / 64; };
     // Rows that allow one element at a time: as wide as others, wherever they begin, where that leaves every CU four waves
     // (65536 x 2047 bfloat16 282, now 199 us, x 1023 float32 171 and 145; but 2065 x 385 float32 17 us, and 24 that way).
-    const bool any = n == 1 && chunks * slices_of(kWide) >= 4 * device_cus();
-    if (any) n = kWide;
-    const int64_t slices = slices_of(n);
-    if (chunks > 0x7fffffff || slices > 65535) return DS_ETOOLARGE;
-    const dim3 grid((unsigned)chunks, (unsigned)slices);
+    s.any = s.width == 1 && s.chunks * slices_of(wide) >= 4 * device_cus();
+    if (s.any) s.width = wide;
+    s.slices = slices_of(s.width);
+    return s;
+}
+
+template <typename E>
+int launch_embed_grad(const SumGrid &s, const uint32_t *keys, const uint32_t *pos, const void *g, int64_t ldg, void *dw, float *part,
+                      int64_t T, int64_t D, float scale, hipStream_t st)
+{
+    constexpr int kWide = 16 / sizeof(E);
+    const int n = s.width, chunk = s.chunk;
+    const bool any = s.any;
+    const dim3 grid((unsigned)s.chunks, (unsigned)s.slices);
 #define DS_LAUNCH(N, ANY)                                                                                                 \
     do {                                                                                                                  \
         hipLaunchKernelGGL((embed_sum_kernel<E, N, ANY>), grid, dim3(64), 0, st, (const E *)g, ldg, keys, pos, (E *)dw, part, T, \
@@ -561,6 +574,8 @@ DS_EXPORT int ds_embed_grad(const void *ids, int id_bytes, const void *grad, int
     if (V == 0 || D == 0) return DS_OK;
     if (!dweight || (T > 0 && (!ids || !grad || ldg < D))) return DS_EINVAL;
     if (V > 0x7fffffff || T > 0x7fffffff || D > 0x7fffffff || V * D > (int64_t)1 << 44) return DS_ETOOLARGE;
+    const SumGrid sums = sum_grid(element_bytes(type), grad, ldg, dweight, T, D);
+    if (T > 0 && !sums.fits()) return DS_ETOOLARGE;
     const EmbedSpace s = embed_space(T, D);
     if (workspace_bytes < s.bytes || !workspace || (uintptr_t)workspace % 16) return DS_EWORKSPACE;
     hipStream_t st = (hipStream_t)stream;
@@ -570,7 +585,7 @@ DS_EXPORT int ds_embed_grad(const void *ids, int id_bytes, const void *grad, int
                                    &pos);
     if (status != DS_OK || T == 0) return status;
     float *part = (float *)((char *)workspace + s.part);
-    if (type == DS_F32) return launch_embed_grad<float>(keys, pos, grad, ldg, dweight, part, T, D, scale, st);
-    if (type == DS_BF16) return launch_embed_grad<bf16_t>(keys, pos, grad, ldg, dweight, part, T, D, scale, st);
-    return launch_embed_grad<f16_t>(keys, pos, grad, ldg, dweight, part, T, D, scale, st);
+    if (type == DS_F32) return launch_embed_grad<float>(sums, keys, pos, grad, ldg, dweight, part, T, D, scale, st);
+    if (type == DS_BF16) return launch_embed_grad<bf16_t>(sums, keys, pos, grad, ldg, dweight, part, T, D, scale, st);
+    return launch_embed_grad<f16_t>(sums, keys, pos, grad, ldg, dweight, part, T, D, scale, st);
 }

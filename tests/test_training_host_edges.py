@@ -4,7 +4,7 @@ import itertools
 import pytest
 import torch
 
-from deepshift_amd import training
+from deepshift_amd import _lib, training
 
 IDS, X, W = torch.zeros(3, dtype=torch.int64), torch.ones(3, 4), torch.ones(5, 4)
 
@@ -88,3 +88,9 @@ def test_norms_other_than_the_second_are_refused(norm_type):
         training.clip_grad_norm_([p], 1.0, norm_type)
     with pytest.raises(ValueError, match="norm_type"):
         training.clip_grad_norm_([p], 1.0, norm_type=norm_type)
+
+
+def test_a_size_that_has_no_grid_is_refused_before_anything_is_written():
+    # more slices of columns than a launch has along y
+    assert _lib.lib().ds_embed_grad(4096, 8, 4096, 1 << 25, 4096, 4, 8, 1 << 25, -1, 1.0, 0, 4096, 1 << 62, None) == -5
+    assert _lib.lib().ds_embed_grad(4096, 8, 4096, 1 << 30, 4096, 4, 8, 1 << 30, -1, 1.0, 1, 4096, 1 << 62, None) == -5
