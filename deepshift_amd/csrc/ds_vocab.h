@@ -436,8 +436,19 @@ __device__ __forceinline__ int64_t target_at(const Args &a, int t)
     return a.target_wide ? ((const int64_t *)a.target)[t] : (int64_t)((const int32_t *)a.target)[t];
 }
 
-// What sums of probabilities are multiplied with on their way out.
-__device__ __forceinline__ float factor_of(const float *const *f) { return (f[0] ? *f[0] : 1.f) * (f[1] ? *f[1] : 1.f); }
+// What sums of probabilities are multiplied with on their way out, and what probabilities are: the loss's gradient times a row's
+// share belongs to the former if it is a number, else to the rows that count, so that it makes nothing of the others' zeros.
+__device__ __forceinline__ float both_factors(const float *const *f) { return (f[0] ? *f[0] : 1.f) * (f[1] ? *f[1] : 1.f); }
+__device__ __forceinline__ float factor_of(const float *const *f)
+{
+    const float all = both_factors(f);
+    return fabsf(all) < INFINITY ? all : 1.f;
+}
+__device__ __forceinline__ float prob_factor_of(const float *const *f)
+{
+    const float all = both_factors(f);
+    return fabsf(all) < INFINITY ? 1.f : all;
+}
 template <typename P>
 __device__ __forceinline__ float out_factor(const float *const *f)
 {
@@ -607,7 +618,7 @@ __device__ __forceinline__ void product_tile(const Args &g, const int block, cha
             if constexpr (KIND == kProb) {
                 if (y != g.ignore) {
                     lse = g.lse[n];
-                    scale = y < 0 || y >= g.V ? NAN : g.row_scale ? g.row_scale[n] : 1.f;
+                    scale = y < 0 || y >= g.V ? NAN : g.row_scale ? g.row_scale[n] : prob_factor_of(g.factor);
                     if (P::half && g.row_power) power = g.row_power[n];
                 } else {
                     want = kNowhere;

@@ -88,7 +88,7 @@ __global__ __launch_bounds__(256) void few_logits_kernel(Args g)
         uint16_t *const row = (uint16_t *)g.prob + t * g.ldp + m0 * 3;
         if (KIND == kProb) {
             const float lse = g.lse[t];
-            const float scale = y < 0 || y >= g.V ? NAN : g.row_scale ? g.row_scale[t] : 1.f;
+            const float scale = y < 0 || y >= g.V ? NAN : g.row_scale ? g.row_scale[t] : prob_factor_of(g.factor);
             const float p = y == g.ignore ? 0.f : (exp2f(x - lse) - (hot ? 1.f : 0.f)) * scale;
             over_t += p;
             bf16_t planes[3];

@@ -70,6 +70,24 @@ def test_a_rows_gradient_that_is_no_number_stays_in_its_row(dtype, bad):
 
 
 @pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("bad", [float("inf"), -float("inf"), float("nan")], ids=str)
+def test_a_losss_gradient_that_is_no_number_leaves_tokens_that_do_not_count(dtype, bad):
+    up = torch.tensor(bad, device=DEV)
+    for T, D, V in [(6, 40, 200), (70, 48, 300), (20, 1024, 8200), (300, 64, 513)]:
+        print(T, D, V, flush=True)
+        g = _gen(T, D, V, 79)
+        h, w, b, y = _head(T, D, V, dtype, True, g)
+        y[2::5] = -100
+        for reduction in ("sum", "mean"):
+            dh, dw, db = _backward(h, w, b, y, up, reduction=reduction)
+            assert (dh[2::5] == 0).all() and not dh[y != -100].isfinite().any()
+            assert not dw.isfinite().any() and not db.isfinite().any()
+            # nothing counts
+            for grad in _backward(h, w, b, torch.full_like(y, -100), up, reduction=reduction):
+                assert (grad == 0).all()
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
 def test_gradients_of_rows_far_apart_keep_their_bits(dtype):
     # many words and large weights: by 2^-26 of the largest gradient most probabilities are below 2^-39, and what a row of 2^-17
     # gets is inside float16 all the same
