@@ -524,15 +524,28 @@ inline bool in_place(const void *p, int64_t ld, int64_t D) { return (uintptr_t)p
 constexpr int64_t kManyWeights = 1 << 23;
 inline int64_t few_tokens(int64_t weights) { return weights < kManyWeights ? kFewTokens / 2 : kFewTokens; }
 
-// Up to how many tokens of float32 the matrix instructions take weights as they are, split into planes by every tile of 64 tokens;
-// for more, planes for all of them to share are worth what writing and reading them takes.  50021 words of 2048 features, the loss
-// and a step, in us: 64 tokens 123 and 465 (by planes 425 and 789), 256 tokens 373 and 1132 (550 and 1266), 512 tokens 672 and
-// 2053 (850 and 2088); of 2049 features, fetched one by one, 512 tokens 757 and 2452 (887 and 2339); 24 tokens of 1024 features,
-// 8200 words, 42 and 91 (41 and 86).
-constexpr int64_t kRawMost = 512;
-
 // What a call does: the loss, the gradients, or both.
 enum { kLoss = 1, kGrad = 2 };
+
+// Up to how many tokens of float32 the matrix instructions take weights as they are, `width` floats at a time, split into planes by
+// every tile of 64 tokens; for more, planes for all of them to share are worth what writing and reading them takes, the sooner the
+// fewer weights there are, for gradients (whose hidden states are in planes either way) and for weights that come one by one.
+// Measured as they are and by planes, in us:
+//                                  loss of 24       128         512     a step of 24         128           256           512 tokens
+//   1024 features,  8200 words      46   44     47   62     93   94      93   88    117  121     166  152       260  225
+//   1024,          16400            45   69     61   72    140  153     108  137    163  169     252  265       412  412
+//   1024,          33000            60  126     93  154    243  271     158  242    267  330     424  482       735  753
+//   1023 (one by one), 8300         53   42     55   60    106   94     105   88    131  123     180  155       285  228
+//   1023,          16400            54   70     67   73    158  153     120  138    176  171     276  267       451  415
+//   1023,          33000            66  132    106  159    268  274     174  251    294  338     464  490       805  760
+//   2049,          50021           143  389    242  410    767  796     437  706    737  898    1266 1332      2424 2206
+constexpr int64_t kManyOddWeights = 7 << 21;
+inline int64_t raw_tokens(int64_t weights, int width, int what)
+{
+    const bool odd = width == 1, grad = what & kGrad;
+    if (weights < (odd ? kManyOddWeights : kManyWeights)) return 0;
+    return std::min<int64_t>(odd && grad ? 256 : 512, weights >> (15 + odd + grad));
+}
 
 template <typename P>
 Plan plan_of(const void *hidden, int64_t ldh, const void *weight, int64_t ldw, int64_t T, int64_t D, int64_t V, int what)
@@ -543,8 +556,10 @@ Plan plan_of(const void *hidden, int64_t ldh, const void *weight, int64_t ldw, i
     p.ldd = row_elements<P>(D);
     p.few = NP > 1 && T > 0 && T <= few_tokens(V * D) && g_tune.vocab_tile == kTuneUnset;
     p.pack_h = !p.few && (NP > 1 || what & kGrad || !in_place(hidden, ldh, D));  // for gradients: without the rows that do not count
-    if (NP > 1 && !p.few && T > 0 && T <= kRawMost && V * D >= kManyWeights && g_tune.vocab_tile == kTuneUnset)
-        p.raw = (uintptr_t)weight % 16 == 0 && ldw % 4 == 0 && D % 4 == 0 ? 4 : 1;
+    if (NP > 1 && !p.few && T > 0 && g_tune.vocab_tile == kTuneUnset) {
+        const int width = (uintptr_t)weight % 16 == 0 && ldw % 4 == 0 && D % 4 == 0 ? 4 : 1;
+        if (T <= raw_tokens(V * D, width, what)) p.raw = width;
+    }
     p.pack_w = !p.few && !p.raw && (NP > 1 || !in_place(weight, ldw, D));
     const int kb = g_tune.vocab_piece_kb;
     const size_t piece_bytes = kb == kTuneUnset ? kPieceBytes : (size_t)kb << 10;

@@ -153,7 +153,8 @@ def test_tokens_that_do_not_count_leave_nothing_whatever_weights_hold(dtype):
 @pytest.mark.parametrize("dtype", TYPES, ids=str)
 def test_an_infinite_weight_takes_a_word_out(dtype):
     for T, D, V, kb in [(4, 40, 200, 0), (20, 40, 200, 0), (70, 48, 300, 0), (150, 33, 700, 1), (300, 256, 515, 0), (20, 1024, 8200, 0),
-                        (20, 1023, 8300, 0), (100, 1024, 8200, 0)]:
+                        (20, 1023, 8300, 0), (100, 1024, 8200, 0),
+                        (20, 1023, 14500, 0)]:
         g = _gen(T, D, V, 74)
         h, w, b, y = _head(T, D, V, dtype, True, g)
         h[:, 1] = h[:, 1].abs().clamp(min=0.25)
@@ -192,7 +193,7 @@ def _masked_column(h, w, b, y, share, dtype):
 
 def test_float32_infinities_do_what_they_do_in_64_bits():
     # every path of float32, and every kind of product that an infinity may be in
-    for T, D, V in [(5, 8, 20), (17, 8, 20), (40, 2048, 4200), (40, 2047, 4200), (200, 40, 300)]:
+    for T, D, V in [(5, 8, 20), (17, 8, 20), (40, 2048, 4200), (40, 2047, 4200), (40, 2047, 7200), (200, 40, 300)]:
         print(T, D, V, flush=True)
         g = _gen(T, D, V, 75)
         h, w, b, y = _head(T, D, V, torch.float32, False, g)
@@ -210,6 +211,29 @@ def test_float32_infinities_do_what_they_do_in_64_bits():
         want = s.logsumexp(1) - s.gather(1, y[3:, None])[:, 0]
         size = (h[3:].abs().double() @ w[:V - 2].abs().double().t()).amax(1)
         _within(rows[3:], want, 2 * (D + 8) * E * size + (6 * size + 20) * E, "loss")
+
+
+# ---- weights as they are -----------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("T", [17, 64, 100, 127])
+def test_weights_as_they_are_from_where_rows_that_begin_anywhere_take_them(T):
+    # 7 * 2^21 weights and more, that come one float at a time, and on both sides of where planes take over
+    for D, V, before, behind in [(1021, 14500, 0, 0), (1024, 14400, 1, 2), (2050, 7200, 2, 0), (1023, 14349, 0, 1), (1023, 14351, 0, 0),
+                                 (31, 520000, 0, 0)]:
+        print(T, D, V, before, behind, flush=True)
+        g = _gen(T, D, V, 80)
+        h, w, b, y = _head(T, D, V, torch.float32, True, g)
+        y[0], y[1], y[2] = V - 1, 0, 128
+        y[3::5] = -100
+        wide = torch.full((V, before + D + behind), float("nan"), device=DEV)
+        wide[:, before:before + D] = w
+        wide = wide[:, before:before + D]
+        share = torch.full((T,), 1.0 / int((y != -100).sum()), device=DEV)
+        rows = training.linear_cross_entropy(h, wide, y, b, reduction="none")
+        loss, dh, dw, db = training.linear_cross_entropy_grad(h, wide, y, b)
+        _head_check(h, w, b, y, -100, share, rows, dh, dw, db)
+        again = training.linear_cross_entropy_grad(h, wide, y, b)
+        assert all(torch.equal(x, z) for x, z in zip((loss, dh, dw, db), again))
 
 
 # ---- losses -----------------------------------------------------------------------------------------------------
