@@ -65,7 +65,7 @@ struct Tune {
     std::atomic<int> notail{kTuneUnset};  // int8 kernel: keep the last round of tiles on the tile-per-wave launch
     std::atomic<int> perm{kTuneUnset};    // int32 cooperative launch: 0 = the share space walks the pixel tiles as they lie
     std::atomic<int> wide{kTuneUnset};    // int8 fused launch: 1 = widened tile buffer (eight waves) for every reduction longer than a chunk
-    std::atomic<int> vocab_tile{kTuneUnset};      // cross entropy: tile shape of every product (0, 1, 2)
+    std::atomic<int> vocab_tile{kTuneUnset};      // cross entropy: tile shape of every product (0 to 3)
     std::atomic<int> vocab_piece_kb{kTuneUnset};  // ... workspace of a piece of the vocabulary in KiB
     std::atomic<int> vocab_split{kTuneUnset};     // ... stretches that the gradients' reductions are cut into, at most
     std::atomic<int> embed_radix{kTuneUnset};     // embedding gradient: 1 = the radix sort for any number of tokens

@@ -16,8 +16,8 @@
 //
 // What bounds them: large ones the power of the chip, which holds the clock at 1.5 to 1.6 GHz while the matrix cores are busy 70
 // to 85 % of the cycles (a library's products of the same sizes run at the same rate).  A piece of 8192 tokens x 65536 words x
-// 4096 features, bfloat16, 4.4 TFLOP each: scores 3.2 ms, probabilities 3.5 ms, hidden gradients 3.15 ms, weight gradients 3.2 ms,
-// 1.25 to 1.4 PFLOP/s; plain library products of these operands take 3.24, 3.43 and 3.92 ms.  float32, 2048 tokens x 32768 words x
+// 4096 features, bfloat16, 4.4 TFLOP each: scores 3.2 ms, with their exponentials 3.7 ms, probabilities 3.5 ms, hidden gradients
+// 3.15 ms, weight gradients 3.2 ms, 1.2 to 1.4 PFLOP/s; plain library products of these operands take 3.24, 3.43 and 3.92 ms.  float32, 2048 tokens x 32768 words x
 // 1024 features, 137 GFLOP each: 0.68 to 0.85 ms, 1.0 to 1.2 PFLOP/s of plane products, 160 to 200 TFLOP/s of float32, where the
 // library reaches 154.  Few tokens are bound by reading the weights (37 tokens, 50021 words x 2048, bfloat16: 205 MB in 41 us),
 // small problems by what one CU can fetch at a time, some 50 bytes per ns from other XCDs' results: hence the small tiles.
