@@ -184,9 +184,9 @@ def _clip(grads, max_norm, out, scale):
         norm = clip(grads, outs, max_norm, scale, False, _stream_of(device))
         if norm is None:
             # not all contiguous; what is written to copies is copied back, on the same stream
-            if scale:
-                _check_apart(grads if outs is None else outs)
             sources, targets, back = _stretches(grads, grads if outs is None else outs)
+            if scale and back:
+                _check_apart(grads if outs is None else outs)    # the copies hide what they are copied back to
             norm = clip(sources, None if targets is sources else targets, max_norm, scale, True, _stream_of(device))
             if scale:
                 for o, copy in back:
