@@ -861,7 +861,8 @@ __device__ __forceinline__ void product_tile(const Args &g, const int block, cha
         // An infinity times a lower plane of 0, or of the other sign than its value, makes a result NaN that may be infinite.
         // The largest planes have the values' signs, zeros and infinities: their product alone says which it is.  A row of
         // the wave's tiles at a time, for the whole workgroup where a lane has met one, so that all of it fetches.  Looking for
-        // them takes 0.2 us of a launch of 12 (with this code in the way of what follows 0.4).
+        // them takes 0.2 us of a launch of 12 (with this code in the way of what follows 0.4); a step of 2048 x 1024 over 32768
+        // words takes 4.3 ms instead of 2.6 with a NaN in one token, 5.3 with one in every word.
         if (__builtin_expect(*met_nan, 0)) {
 #pragma unroll
             for (int i = 0; i < MT; ++i) {
