@@ -58,6 +58,7 @@ class Tensor(ctypes.Structure):
 _tp = ctypes.POINTER(Tensor)
 _float = ctypes.c_float
 _matrix = [_ptr, _c_i64]   # an operand and the distance of its rows
+_sequence = [_ptr, _c_i64, _c_i64]   # sequences, the distances of them and of their tokens
 
 # name -> (restype, argtypes); mirrors include/deepshift_hip.h one to one
 SIGNATURES = {
@@ -131,6 +132,10 @@ SIGNATURES = {
     "ds_vocab_loss_grad": (_c_int, _matrix * 2 + [_ptr, _ptr, _c_int] + [_c_i64] * 4 + [_c_int] + [_ptr] * 8 + [_size, _ptr]),
     "ds_vocab_loss_step": (_c_int, _matrix * 2 + [_ptr, _ptr, _c_int] + [_c_i64] * 4 + [_c_int, _c_int] + [_ptr] * 7 +
                            [_size, _ptr]),
+    "ds_recur_blocks": (_c_i64, [_c_i64]),
+    "ds_recur_workspace_bytes": (_size, [_c_i64] * 3 + [_c_int]),
+    "ds_recur_forward": (_c_int, _sequence * 2 + [_ptr, _ptr, _c_int, _ptr, _ptr, _ptr] + [_c_i64] * 3 + [_c_int, _ptr, _size, _ptr]),
+    "ds_recur_backward": (_c_int, _sequence * 3 + [_ptr, _ptr, _c_int] + [_ptr] * 4 + [_c_i64] * 3 + [_c_int, _ptr, _size, _ptr]),
     "ds_clip_workspace_bytes": (_size, [_c_int]),
     "ds_clip": (_c_int, [_tp, _c_int, _float, _c_int, _ptr, _ptr, _size, _ptr]),
     "ds_valu_calibrate": (_c_int, [_ptr, _c_int, _c_int, _ptr]),

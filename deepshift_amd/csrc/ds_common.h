@@ -69,13 +69,14 @@ struct Tune {
     std::atomic<int> vocab_piece_kb{kTuneUnset};  // ... workspace of a piece of the vocabulary in KiB
     std::atomic<int> vocab_split{kTuneUnset};     // ... stretches that the gradients' reductions are cut into, at most
     std::atomic<int> embed_radix{kTuneUnset};     // embedding gradient: 1 = the radix sort for any number of tokens
+    std::atomic<int> recur_segments{kTuneUnset};  // recurrence: segments that a sequence is cut into, at most
     std::atomic<int> chain_spin_us{-1};   // layer-chain launch: bound of a barrier wait in microseconds (-1: default)
     std::atomic<int> chain_extra{-1};     // ... arrivals a barrier waits for beyond the grid (they never come)
     void reset()
     {
         planes = kTuneUnset; split = kTuneUnset; tile = kTuneUnset; cu = kTuneUnset; notail = kTuneUnset;
         wide = kTuneUnset; perm = kTuneUnset;
-        vocab_tile = kTuneUnset; vocab_piece_kb = kTuneUnset; vocab_split = kTuneUnset; embed_radix = kTuneUnset;
+        vocab_tile = kTuneUnset; vocab_piece_kb = kTuneUnset; vocab_split = kTuneUnset; embed_radix = kTuneUnset; recur_segments = kTuneUnset;
         chain_spin_us = -1; chain_extra = -1;
     }
 };

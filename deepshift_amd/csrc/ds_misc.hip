@@ -72,6 +72,7 @@ DS_EXPORT int ds_test_tune(const char *knob, int value)
     else if (k == "wide") g_tune.wide = value;
     else if (k == "perm") g_tune.perm = value;
     else if (k == "vocab_tile") g_tune.vocab_tile = value;
+    else if (k == "recur_segments") g_tune.recur_segments = value;
     else if (k == "vocab_piece_kb") g_tune.vocab_piece_kb = value;
     else if (k == "vocab_split") g_tune.vocab_split = value;
     else if (k == "embed_radix") g_tune.embed_radix = value;

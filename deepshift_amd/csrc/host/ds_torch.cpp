@@ -342,6 +342,110 @@ PyObject *cross_entropy_step(PyObject *, PyObject *const *args, Py_ssize_t count
     });
 }
 
+// Sequences [B, T, D] whose channels lie contiguously.
+struct Sequences {
+    at::Tensor t;
+    Sequences(const at::Tensor &given) : t(given)
+    {
+        if (t.defined() && t.size(2) > 1 && t.stride(2) != 1) t = t.contiguous();
+    }
+    const void *at() const { return t.defined() ? t.const_data_ptr() : nullptr; }
+    int64_t batch() const { return t.defined() && t.size(0) > 1 ? t.stride(0) : 0; }
+    int64_t token() const { return t.defined() && t.size(1) > 1 ? t.stride(1) : 0; }
+};
+
+void check_like(const char *name, const at::Tensor &t, const char *like, at::ScalarType type, c10::Device device, at::IntArrayRef sizes)
+{
+    if (t.scalar_type() != type || t.device() != device)
+        refuse(PyExc_TypeError, name, " must be ", c10::toString(type), " on ", device.str(), like, ", is ",
+               c10::toString(t.scalar_type()), " on ", t.device().str());
+    if (t.sizes() != sizes) refuse(PyExc_ValueError, name, " must be ", sizes, ", is ", t.sizes());
+}
+
+// The operands of a gated recurrence: x and gate [B, T, D], lengths [B] or None.
+struct Recurrence {
+    at::Tensor x, gate, lengths;
+    int64_t B, T, D;
+    int type;
+
+    Recurrence(PyObject *x_, PyObject *gate_, PyObject *lengths_) : x(tensor("x", x_)), gate(tensor("gate", gate_))
+    {
+        type = checked_type("x", x);
+        if (x.dim() != 3) refuse(PyExc_ValueError, "x must be [B, T, D], is ", x.sizes());
+        check_like("gate", gate, " like x", x.scalar_type(), x.device(), x.sizes());
+        B = x.size(0), T = x.size(1), D = x.size(2);
+        if (lengths_ != Py_None) {
+            lengths = tokens("lengths", lengths_, x.device());
+            if (lengths.dim() != 1 || lengths.size(0) != B)
+                refuse(PyExc_ValueError, "lengths must be [", std::to_string(B), "], is ", lengths.sizes());
+        }
+    }
+    at::Tensor empty(at::IntArrayRef sizes, at::ScalarType as) const
+    {
+        return at::empty(sizes, at::TensorOptions().device(x.device()).dtype(as));
+    }
+    // float32 [B, D] or None
+    at::Tensor state(const char *name, PyObject *o) const
+    {
+        if (o == Py_None) return at::Tensor();
+        const at::Tensor &t = tensor(name, o);
+        check_like(name, t, "", at::kFloat, x.device(), {B, D});
+        return t.contiguous();
+    }
+    const void *lengths_at() const { return lengths.defined() ? lengths.const_data_ptr() : nullptr; }
+    int length_bytes() const { return lengths.defined() ? (int)lengths.element_size() : 0; }
+    at::Tensor workspace() const { return empty({(int64_t)ds_recur_workspace_bytes(B, T, D, type)}, at::kByte); }
+};
+
+// recurrence(x, gate, state or None, lengths or None, keep, stream): all states, the last ones, and, if they are to be kept for
+// gradients, those before every block
+PyObject *recurrence(PyObject *, PyObject *const *args, Py_ssize_t count)
+{
+    return guarded(count, 6, [&] {
+        const Recurrence r(args[0], args[1], args[3]);
+        const at::Tensor state = r.state("state", args[2]);
+        const Sequences x(r.x), gate(r.gate);
+        const at::Tensor out = r.empty({r.B, r.T, r.D}, r.x.scalar_type()), last = r.empty({r.B, r.D}, at::kFloat);
+        at::Tensor kept;
+        if (integer(args[4])) kept = r.empty({r.B, ds_recur_blocks(r.T), r.D}, at::kFloat);
+        const at::Tensor ws = r.workspace();
+        expect("ds_recur_forward",
+               ds_recur_forward(x.at(), x.batch(), x.token(), gate.at(), gate.batch(), gate.token(),
+                                state.defined() ? (const float *)state.const_data_ptr() : nullptr, r.lengths_at(), r.length_bytes(),
+                                at_or_null(out), at_or_null<float>(last), at_or_null<float>(kept), r.B, r.T, r.D, r.type,
+                                ws.mutable_data_ptr(), ws.nbytes(), stream(args[5])));
+        return tuple_of({out, last, kept});
+    });
+}
+
+// recurrence_grad(x, gate, grad or None, grad_last or None, lengths or None, kept, wanted, stream): gradients of x, gate and the
+// first state; bits 0 to 2 of `wanted` say which
+PyObject *recurrence_grad(PyObject *, PyObject *const *args, Py_ssize_t count)
+{
+    return guarded(count, 8, [&] {
+        const Recurrence r(args[0], args[1], args[4]);
+        const at::Tensor grad_last = r.state("grad_last", args[3]);
+        const at::Tensor given = args[2] == Py_None ? at::Tensor() : tensor("grad", args[2]);
+        if (given.defined()) check_like("grad", given, " like x", r.x.scalar_type(), r.x.device(), r.x.sizes());
+        const at::Tensor &kept = tensor("kept", args[5]);
+        check_like("kept", kept, "", at::kFloat, r.x.device(), {r.B, ds_recur_blocks(r.T), r.D});
+        const Sequences x(r.x), gate(r.gate), grad(given);
+        const int64_t wanted = integer(args[6]);
+        at::Tensor dx, dgate, dstate;
+        if (wanted & 1) dx = r.empty(r.x.sizes(), r.x.scalar_type());
+        if (wanted & 2) dgate = r.empty(r.x.sizes(), r.x.scalar_type());
+        if (wanted & 4) dstate = r.empty({r.B, r.D}, at::kFloat);
+        const at::Tensor ws = r.workspace();
+        expect("ds_recur_backward",
+               ds_recur_backward(x.at(), x.batch(), x.token(), gate.at(), gate.batch(), gate.token(), grad.at(), grad.batch(),
+                                 grad.token(), grad_last.defined() ? (const float *)grad_last.const_data_ptr() : nullptr,
+                                 r.lengths_at(), r.length_bytes(), (const float *)kept.contiguous().const_data_ptr(), at_or_null(dx),
+                                 at_or_null(dgate), at_or_null<float>(dstate), r.B, r.T, r.D, r.type, ws.mutable_data_ptr(),
+                                 ws.nbytes(), stream(args[7])));
+        return tuple_of({dx, dgate, dstate});
+    });
+}
+
 // The tensors of a list: types, one device; false where one is not contiguous.
 bool look_at(const char *name, PyObject *list, c10::Device device, std::vector<const at::Tensor *> &tensors, std::vector<int> &types)
 {
@@ -448,6 +552,10 @@ PyMethodDef methods[] = {
      "cross_entropy_grad(hidden, weight, target, bias or None, ignore, lse, share or None, grad, wanted, stream) -> gradients"},
     {"cross_entropy_step", (PyCFunction)(void (*)(void))cross_entropy_step, METH_FASTCALL,
      "cross_entropy_step(hidden, weight, target, bias or None, ignore, reduction, stream) -> loss, gradients"},
+    {"recurrence", (PyCFunction)(void (*)(void))recurrence, METH_FASTCALL,
+     "recurrence(x, gate, state or None, lengths or None, keep, stream) -> states, last ones, kept ones or None"},
+    {"recurrence_grad", (PyCFunction)(void (*)(void))recurrence_grad, METH_FASTCALL,
+     "recurrence_grad(x, gate, grad or None, grad_last or None, lengths or None, kept, wanted, stream) -> gradients"},
     {"clip", (PyCFunction)(void (*)(void))clip, METH_FASTCALL,
      "clip(grads, outs or None, max_norm, scale, any_order, stream) -> norm, or None"},
     {nullptr, nullptr, 0, nullptr},

@@ -19,7 +19,7 @@ from torch.autograd.function import once_differentiable
 from . import _lib
 
 __all__ = ["embedding", "embedding_grad", "linear_cross_entropy", "linear_cross_entropy_grad", "gradient_norm",
-           "clip_gradients_", "clip_grad_norm_", "ScaledEmbedding", "LinearCrossEntropy"]
+           "clip_gradients_", "clip_grad_norm_", "gated_recurrence", "ScaledEmbedding", "LinearCrossEntropy"]
 
 _REDUCTIONS = {"none": _lib.DS_NONE, "sum": _lib.DS_SUM, "mean": _lib.DS_MEAN}
 
@@ -164,6 +164,51 @@ def linear_cross_entropy_grad(hidden, weight, target, bias=None, ignore_index=-1
     device = hidden.device
     with _on(device):
         return _lib.native().cross_entropy_step(hidden, weight, target, bias, ignore_index, reduction, _stream_of(device))
+
+
+# ---------------------------------------------------------------------------------------------
+# recurrence
+# ---------------------------------------------------------------------------------------------
+
+def _recur(x, gate, state, lengths, keep):
+    device = x.device
+    with _on(device):
+        return _lib.native().recurrence(x, gate, state, lengths, keep, _stream_of(device))
+
+
+class _GatedRecurrence(Function):
+    @staticmethod
+    def forward(ctx, x, gate, state, lengths):
+        out, last, kept = _recur(x, gate, state, lengths, True)
+        ctx.save_for_backward(x, gate, lengths, kept)
+        ctx.set_materialize_grads(False)
+        return out, last
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad, grad_last):
+        x, gate, lengths, kept = ctx.saved_tensors
+        device, needed = x.device, ctx.needs_input_grad
+        if grad is None and grad_last is None:
+            return None, None, None, None
+        with _on(device):
+            dx, dgate, dstate = _lib.native().recurrence_grad(x, gate, grad, grad_last, lengths, kept,
+                                                              needed[0] | needed[1] << 1 | needed[2] << 2, _stream_of(device))
+        return dx, dgate, dstate, None
+
+
+def gated_recurrence(x, gate, state=None, lengths=None):
+    """``(out, last)`` of the recurrence ``h[t] = a[t] * h[t - 1] + (1 - a[t]) * x[t]`` with ``a = sigmoid(gate)``, channel by
+    channel along sequences.
+
+    ``x`` and ``gate`` ``[B, T, D]`` are of one type; they may be pieces of one tensor (``chunk`` of a projection's result).
+    ``state`` ``[B, D]`` in float32 is what the sequences begin with, zeros if there is none; ``out`` ``[B, T, D]`` holds every
+    ``h``, ``last`` ``[B, D]`` the last ones in float32, to go on from: token by token with ``T`` = 1, or piece by piece.
+    ``lengths`` ``[B]`` (int64 or int32, held to ``[0, T]``) ends a sequence early: what ``x`` and ``gate`` hold behind it is not
+    looked at, ``out`` and the gradients are 0 there, and ``last`` is the state at its end."""
+    if torch.is_grad_enabled() and (x.requires_grad or gate.requires_grad or (state is not None and state.requires_grad)):
+        return _GatedRecurrence.apply(x, gate, state, lengths)
+    return _recur(x, gate, state, lengths, False)[:2]
 
 
 # ---------------------------------------------------------------------------------------------

@@ -567,6 +567,26 @@ int ds_vocab_loss_step(const void *hidden, int64_t ldh, const void *weight, int6
                        float *lse, float *total, void *dhidden, void *dweight, void *dbias, void *workspace,
                        size_t workspace_bytes, ds_stream_t stream);
 
+/* Gated linear recurrence along sequences, channel by channel: with a = 1 / (1 + exp(-gate)),
+ *   h[t] = a[t] h[t - 1] + (1 - a[t]) x[t],
+ * from state[b][:] (zeros where state is NULL).  x and gate hold [B][T][D] elements of `type`, channels next to each other,
+ * tokens *_token and sequences *_batch elements apart; state and last are float32 [B][D], out is [B][T][D].  With lengths
+ * (int32 or int64, length_bytes 4 or 8, held to [0, T]) a sequence ends there: what x and gate hold behind it is not looked at,
+ * out is 0 there, and last is the state at its end.  kept [B][ds_recur_blocks(T)][D], or NULL, is what ds_recur_backward needs.
+ * workspace: 256-byte aligned, ds_recur_workspace_bytes() bytes. */
+int64_t ds_recur_blocks(int64_t T);
+size_t ds_recur_workspace_bytes(int64_t B, int64_t T, int64_t D, int type);
+int ds_recur_forward(const void *x, int64_t x_batch, int64_t x_token, const void *gate, int64_t gate_batch, int64_t gate_token,
+                     const float *state, const void *lengths, int length_bytes, void *out, float *last, float *kept, int64_t B,
+                     int64_t T, int64_t D, int type, void *workspace, size_t workspace_bytes, ds_stream_t stream);
+
+/* Its gradients for grad (of out, or NULL) and grad_last (of last, or NULL): dx and dgate [B][T][D], dstate float32 [B][D],
+ * each NULL where it is not asked for; 0 behind a sequence's end. */
+int ds_recur_backward(const void *x, int64_t x_batch, int64_t x_token, const void *gate, int64_t gate_batch, int64_t gate_token,
+                      const void *grad, int64_t grad_batch, int64_t grad_token, const float *grad_last, const void *lengths,
+                      int length_bytes, const float *kept, void *dx, void *dgate, float *dstate, int64_t B, int64_t T, int64_t D,
+                      int type, void *workspace, size_t workspace_bytes, ds_stream_t stream);
+
 /* One tensor of ds_clip: n elements at src, and where their clipped values go (src itself for a clip in place). */
 typedef struct {
     const void *src;

@@ -20,8 +20,8 @@ extern "C" {
  * a small bound every workgroup gives up and exits, which is how the tests reach that path without
  * hanging anything); "vocab_tile" (0 to 3: tile shape of the products of ds_vocab_*), "vocab_piece_kb"
  * (workspace of a piece of the vocabulary there, in KiB), "vocab_split" (stretches that its gradients'
- * reductions are cut into, at most) and "embed_radix" (1: ds_embed_grad sorts any number of tokens as it
- * sorts many).  knob == NULL clears every override.  Each knob is an atomic integer that an
+ * reductions are cut into, at most), "embed_radix" (1: ds_embed_grad sorts any number of tokens as it
+ * sorts many) and "recur_segments" (segments that ds_recur_* cut a sequence into, at most).  knob == NULL clears every override.  Each knob is an atomic integer that an
  * entry point reads once per call, so a call sees either the old or the new value of a knob, never a
  * torn one; a thread that changes a knob changes the dispatch of every thread of the process, which
  * is why this header is not the production one.  The dispatch's own choice is the measured best. */
