@@ -25,6 +25,7 @@ DS_CHAIN_CONTROL_BYTES = 12288
 DS_CHAIN_STATUS_AT = 1536
 DS_F32, DS_BF16, DS_F16 = 0, 1, 2
 DS_NONE, DS_SUM, DS_MEAN = 0, 1, 2
+DS_SILU, DS_GELU, DS_RELU, DS_SIGMOID = 0, 1, 2, 3
 
 _c_int = ctypes.c_int
 _c_i64 = ctypes.c_int64
@@ -132,6 +133,9 @@ SIGNATURES = {
     "ds_vocab_loss_grad": (_c_int, _matrix * 2 + [_ptr, _ptr, _c_int] + [_c_i64] * 4 + [_c_int] + [_ptr] * 8 + [_size, _ptr]),
     "ds_vocab_loss_step": (_c_int, _matrix * 2 + [_ptr, _ptr, _c_int] + [_c_i64] * 4 + [_c_int, _c_int] + [_ptr] * 7 +
                            [_size, _ptr]),
+    "ds_gated_workspace_bytes": (_size, _matrix * 2 + [_c_i64] * 3 + [_c_int, _c_int]),
+    "ds_gated_forward": (_c_int, _matrix * 2 + [_ptr, _c_int] + [_c_i64] * 3 + [_c_int, _ptr, _ptr, _ptr, _size, _ptr]),
+    "ds_gated_backward": (_c_int, _matrix * 2 + [_ptr] + _matrix + [_c_int] + [_c_i64] * 3 + [_c_int] + [_ptr] * 4 + [_size, _ptr]),
     "ds_recur_blocks": (_c_i64, [_c_i64]),
     "ds_recur_workspace_bytes": (_size, [_c_i64] * 3 + [_c_int]),
     "ds_recur_forward": (_c_int, _sequence * 2 + [_ptr, _ptr, _c_int, _ptr, _ptr, _ptr] + [_c_i64] * 3 + [_c_int, _ptr, _size, _ptr]),

@@ -119,7 +119,8 @@ enum {
     kKeep = 1,   // the same, and the exponentials themselves, relative to their tile's maximum, in 32 bits: of float32 where P will be
                  // (32 of them in the first 128 of the 192 bytes that their planes will take), of 16-bit types beside it
     kProb = 2,   // P, from finished sums
-    kOut = 3     // a gradient
+    kOut = 3,    // a gradient
+    kGate = 4    // act(gate) up, of the two halves of the rows of A (ds_gated*.hip)
 };
 
 struct Args {
@@ -155,6 +156,11 @@ struct Args {
     int64_t ldo;
     const float *factor[2];  // what results are multiplied with, 1 value each, or NULL
     int n_store;          // rows of C that exist (N may be rounded up for the loads)
+    // kGate (bias, out and ldo too): M is half of A's rows
+    int64_t half_bytes;   // from the first half to the second
+    int activation;
+    void *halves;         // [N][2][ldz] both halves of the products, or NULL
+    int64_t ldz;
 };
 
 constexpr float kLog2e = 1.4426950408889634f;
@@ -225,7 +231,9 @@ __device__ __forceinline__ i32x4 buffer_at(uint64_t address)
 //             (0-3, 12-15, 20-23 and 24-27, and so on) meet all banks;
 //   across:   [k][ROWS], its 32-byte pieces exchanged by k, so that the transposing reads that 32 lanes make together, of
 //             k .. k + 3 and k + 8 .. k + 11 or of two neighbouring pieces of k .. k + 3, meet all banks.
-template <typename P, int ROWS, bool ACROSS, int WAVES>
+//   PAIRED, along k: rows come by turns of a unit from two places, the same rows of both halves of a matrix, so that one lane's
+//             results of two neighbouring units belong together.
+template <typename P, int ROWS, bool ACROSS, int WAVES, bool PAIRED = false>
 struct Tile {
     static constexpr int kStep = P::step, kPlanes = P::planes;
     static constexpr int bytes = ROWS * kStep * 2;           // of a plane
@@ -236,6 +244,9 @@ struct Tile {
 
     uint32_t offset[mine];  // of this lane within the tile's first stage, or kNothing
     int k_at[mine];         // along: first k of this lane's piece; across: its k
+    int64_t half_bytes = 0; // PAIRED
+    static constexpr int kFetchRows = 512 / kStep;  // along
+    static_assert(!PAIRED || (!ACROSS && ROWS % (2 * P::unit) == 0 && P::unit % kFetchRows == 0), "a fetch has rows of one half");
 
     __device__ static __forceinline__ int swapped(int row) { return kPieces == 8 ? (row & 7) ^ (row >> 4 & 1) : row >> 1 & 3; }
     __device__ static __forceinline__ int swapped_across(int k)
@@ -251,7 +262,8 @@ struct Tile {
         for (int i = 0; i < mine; ++i) {
             const int p = (wave * mine + i) * 64 + lane;  // 16-byte piece of the stage
             if constexpr (!ACROSS) {
-                const int row = p / kPieces, piece = (p % kPieces) ^ swapped(row);
+                const int slot = p / kPieces, piece = (p % kPieces) ^ swapped(slot);
+                const int row = PAIRED ? slot / (2 * P::unit) * P::unit + slot % P::unit : slot;
                 k_at[i] = piece * 8;
                 offset[i] = row < rows_left ? (uint32_t)(row * o.ld * 2 + piece * 16) : kNothing;
             } else {
@@ -267,6 +279,7 @@ struct Tile {
     // `base`.
     __device__ __forceinline__ void one(uint64_t base, int k_left, uint32_t lds, int wave, int q, int i) const
     {
+        if (PAIRED && (wave * mine + i) * kFetchRows / P::unit % 2) base += half_bytes;
         fetch(k_at[i] < k_left ? offset[i] : kNothing, buffer_at(base + q * 64), lds + q * bytes + (wave * mine + i) * 1024);
     }
     __device__ __forceinline__ void stage(uint64_t base, int k_left, uint32_t lds, int wave) const
@@ -318,7 +331,7 @@ struct Tile {
 //             meet other banks.
 // WIDTH floats a lane and fetch: four, where rows begin at multiples of 16 bytes and end at multiples of four floats, or one
 // (28 tokens, 61003 words x 3405: the loss in 246 us, with planes written first 773).
-template <int ROWS, bool ACROSS, int WAVES, int WIDTH>
+template <int ROWS, bool ACROSS, int WAVES, int WIDTH, bool PAIRED = false>
 struct RawTile {
     static constexpr int kStep = Split::step, kPlanes = 1;
     static constexpr int bytes = ROWS * kStep * 4, fetches = bytes / (256 * WIDTH), mine = fetches / WAVES;
@@ -331,6 +344,8 @@ struct RawTile {
     int k_at[kTurn];
     int rows_after;  // single floats along k: rows behind this lane's first one
     int64_t pitch;   // bytes
+    int64_t half_bytes = 0;  // PAIRED, four floats along k: a fetch has eight rows
+    static_assert(!PAIRED || (!ACROSS && WIDTH == 4 && ROWS % 32 == 0), "");
 
     __device__ static __forceinline__ int swapped(int row) { return row & 7; }
     __device__ static __forceinline__ int swapped_across(int k) { return (k >> 3 & 3) << 2; }
@@ -344,7 +359,8 @@ struct RawTile {
         for (int i = 0; i < kTurn; ++i) {
             const int f = ((wave * mine + i) * 64 + lane) * WIDTH, p = f / 4, e = f % 4;  // float, 16-byte piece
             if constexpr (!ACROSS) {
-                const int row = p / 8, piece = p % 8 ^ swapped(row);
+                const int slot = p / 8, piece = p % 8 ^ swapped(slot);
+                const int row = PAIRED ? slot / 32 * 16 + slot % 16 : slot;
                 k_at[i] = piece * 4 + e;
                 offset[i] = WIDTH == 1 || row < rows_left ? (uint32_t)(row * pitch + piece * 16 + e * 4) : kNothing;
             } else {
@@ -357,6 +373,7 @@ struct RawTile {
     __device__ __forceinline__ void one(uint64_t base, int k_left, uint32_t lds, int wave, int, int i) const
     {
         const uint32_t to = lds + (wave * mine + i) * 256 * WIDTH;
+        if (PAIRED && (wave * mine + i) / 2 % 2) base += half_bytes;
         if constexpr (WIDTH == 4) {
             fetch(k_at[i] < k_left ? offset[i] : kNothing, buffer_at(base), to);
         } else if constexpr (ACROSS) {
@@ -458,6 +475,16 @@ template <typename P> struct ElementOf { typedef bf16_t type; };
 template <> struct ElementOf<F16> { typedef f16_t type; };
 template <> struct ElementOf<Split> { typedef float type; };
 
+// What a gate does to its half, in 32 bits.
+__device__ __forceinline__ float logistic(float x) { return __builtin_amdgcn_rcpf(1.f + exp2_of(x * -kLog2e)); }
+__device__ __forceinline__ float activation_of(int kind, float x)
+{
+    if (kind == DS_SILU) return x * logistic(x);
+    if (kind == DS_GELU) return 0.5f * x * erfcf(x * -0.7071067811865476f);
+    if (kind == DS_RELU) return x < 0.f ? 0.f : x;
+    return logistic(x);
+}
+
 // Until all but `in_flight` of this wave's fetches have arrived and all its reads of LDS, and then until every wave's have.
 template <int in_flight>
 __device__ __forceinline__ void wait_for_stage()
@@ -482,7 +509,7 @@ struct Known {
 // Rows that leave together, what one of them takes, and whether the waves' maxima and sums find a place behind them in the
 // stages (256 x 256 tiles' exponentials fill those).
 template <typename P, int WN> constexpr int kRowsLeaving = WN * Unit<P>::size;
-template <typename P, int BM, int KIND> constexpr int kRowBytes = KIND == kOut || (KIND == kKeep && P::planes == 1) ? BM * 4 : BM * P::planes * 2;
+template <typename P, int BM, int KIND> constexpr int kRowBytes = KIND == kGate ? BM / 2 * 4 : KIND == kOut || (KIND == kKeep && P::planes == 1) ? BM * 4 : BM * P::planes * 2;
 template <typename P, int BM, int BN, int WM, int WN, int KIND, int STAGES, bool RAW>
 constexpr bool kRoomBehind = KIND == kStats || kRowsLeaving<P, WN> * kRowBytes<P, BM, KIND> + WM * BN * 8 <= kStagesBytes<P, BM, BN, STAGES, RAW>;
 template <typename P, int BM, int BN, int WM, int WN, int KIND, int STAGES, bool RAW = false>
@@ -565,7 +592,9 @@ __device__ __forceinline__ void product_tile(const Args &g, const int block, cha
     constexpr int WAVES = WM * WN, MT = BM / WM / U::size, NT = BN / WN / U::size, NP = P::planes;
     constexpr int kStep = P::step;
     static_assert(!RAW || NP == 3, "");
-    using TA = typename std::conditional<(RAW > 0), RawTile<BM, A_ACROSS, WAVES, RAW ? RAW : 4>, Tile<P, BM, A_ACROSS, WAVES>>::type;
+    constexpr bool kPaired = KIND == kGate;
+    using TA = typename std::conditional<(RAW > 0), RawTile<BM, A_ACROSS, WAVES, RAW ? RAW : 4, kPaired>,
+                                         Tile<P, BM, A_ACROSS, WAVES, kPaired>>::type;
     using TB = Tile<P, BN, B_ACROSS, WAVES>;
     constexpr int kBytesA = TA::kPlanes * TA::bytes, kStageBytes = kBytesA + NP * TB::bytes;
     constexpr int kFetchesA = TA::kPlanes * TA::mine, kInFlight = kFetchesA + NP * TB::mine;  // loads of one stage and wave
@@ -575,13 +604,14 @@ __device__ __forceinline__ void product_tile(const Args &g, const int block, cha
 
     int tm, tn, split;
     tile_of(block, g.tiles_m, g.tiles_n, g.splits, &tm, &tn, &split);
-    const int m0 = tm * BM, n0 = tn * BN;
+    const int m0 = tm * (kPaired ? BM / 2 : BM), n0 = tn * BN;
     const int k_from = split * g.k_split, k_to = min(g.K, k_from + g.k_split);
     const int steps = (k_to - k_from + kStep - 1) / kStep;
 
     TA ta;
     TB tb;
     ta.init(g.a, g.M - m0, wave);
+    if constexpr (kPaired) ta.half_bytes = g.half_bytes;
     tb.init(g.b, g.N - n0, wave);
     const int64_t a_step = TA::step_bytes(g.a), b_step = TB::step_bytes(g.b);
     uint64_t a_at = (uint64_t)g.a.at + TA::rows_bytes(g.a, m0) + k_from / kStep * a_step;
@@ -609,7 +639,10 @@ __device__ __forceinline__ void product_tile(const Args &g, const int block, cha
     constexpr int kNowhere = -(1 << 20);
     float bias = -INFINITY, lse = INFINITY, scale = 0.f, power = 1.f;
     int want = kNowhere;
-    if constexpr (KIND != kOut) {
+    if constexpr (KIND == kGate) {
+        const int slot = threadIdx.x, m = m0 + slot / (2 * U::size) * U::size + slot % U::size;
+        bias = slot < BM && m < g.M ? bias_at(g, m + (slot / U::size % 2 ? g.M : 0)) : 0.f;
+    } else if constexpr (KIND != kOut) {
         const int m = m0 + threadIdx.x, n = n0 + threadIdx.x;
         if (threadIdx.x < BM && m < g.M) bias = bias_at(g, g.v0 + m) * kLog2e;
         if (threadIdx.x < BN && n < g.N) {
@@ -632,7 +665,7 @@ __device__ __forceinline__ void product_tile(const Args &g, const int block, cha
         if (NP > 1 && threadIdx.x == 0) *met_nan = 0;
         if constexpr (KIND != kOut) {
             if (threadIdx.x < BM) known.bias[threadIdx.x] = bias;
-            if (threadIdx.x < BN)
+            if (KIND != kGate && threadIdx.x < BN)
                 known.want[threadIdx.x] = want, known.lse[threadIdx.x] = lse, known.scale[threadIdx.x] = scale;
             if (P::half && KIND == kProb && threadIdx.x < BN) known.power[threadIdx.x] = power;
         }
@@ -1096,6 +1129,47 @@ __device__ __forceinline__ void product_tile(const Args &g, const int block, cha
                 if (g.bias_out) ((E *)g.bias_out)[m0 + c] = from_float<E>(s * factor);
                 else g.bias_part[(int64_t)tn * g.ld_bias_part + m0 + c] = s;
             }
+        }
+    }
+    if constexpr (KIND == kGate) {
+        typedef typename ElementOf<P>::type E;
+        typedef Gather<E, BM / 2> Out;
+        static_assert(MT % 2 == 0, "both halves of a result in one wave");
+        // which 0: the gated values, 1 and 2: the halves of the products as they are
+        auto pass = [&](int j, auto which, void *base, int64_t ld) {
+            constexpr int kWhich = decltype(which)::value;
+#pragma unroll
+            for (int i = 0; i < MT / 2; ++i)
+#pragma unroll
+                for (int q = 0; q < U::groups; ++q) {
+                    const int slot = (wm * MT + 2 * i) * U::size + U::lane_m(lane) + U::group_m(q);
+                    const f32x4 zero = f32x4{0.f, 0.f, 0.f, 0.f};
+                    f32x4 gate = kWhich == 2 ? zero : *(const f32x4 *)&known.bias[slot];
+                    f32x4 up = kWhich == 1 ? zero : *(const f32x4 *)&known.bias[slot + U::size];
+                    f32x4 v;
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        if (kWhich != 2) gate[r] += acc[2 * i][j][q * 4 + r];
+                        if (kWhich != 1) up[r] += acc[2 * i + 1][j][q * 4 + r];
+                        v[r] = kWhich == 0 ? activation_of(g.activation, gate[r]) * up[r] : kWhich == 1 ? gate[r] : up[r];
+                    }
+                    char *to = Out::at(lds, row_out, (wm * (MT / 2) + i) * U::size + U::lane_m(lane) + U::group_m(q));
+                    if constexpr (sizeof(E) == 4) *(f32x4 *)to = v;
+                    else *(s16x4 *)to = round4<P>(v);
+                }
+            __syncthreads();
+            Out::template leave<kThreads>(lds, kRowsOut, g.M - m0, [&](int row) -> E * {
+                const int n = n0 + n_of(row, j);
+                return n < g.N ? (E *)base + n * ld + m0 : nullptr;
+            });
+            __syncthreads();
+        };
+#pragma unroll
+        for (int j = 0; j < NT; ++j) {
+            pass(j, std::integral_constant<int, 0>(), g.out, g.ldo);
+            if (!g.halves) continue;
+            pass(j, std::integral_constant<int, 1>(), g.halves, 2 * g.ldz);
+            pass(j, std::integral_constant<int, 2>(), (E *)g.halves + g.ldz, 2 * g.ldz);
         }
     }
     if constexpr (KIND == kOut) {

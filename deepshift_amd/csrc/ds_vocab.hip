@@ -9,8 +9,7 @@
 // formula's own.  Where loss and gradients are asked for in one call, the forward pass leaves the last piece's exponentials,
 // relative to their tiles' maxima, in a workspace, in 32 bits, and a pass over them makes them P: three products for that piece,
 // which may be the whole vocabulary.
-#include "ds_vocab.h"
-#include <algorithm>
+#include "ds_vocab_host.h"
 
 namespace ds {
 namespace vocab {
@@ -21,19 +20,7 @@ namespace vocab {
 // Bound by memory: (2048 + 32768) x 1024 float32 in 64 us, 5.5 TB/s.  Loads are 16 bytes wherever a row begins: 50021 x 2049
 // bfloat16 take 75 us, element by element 176.
 // Rows whose target is `ignore` (where targets are given) become zeros: tokens that do
-// not count leave nothing in the weights' gradient, not even a value that is no number.
-struct Pack {
-    const void *x;
-    int64_t ld, rows;
-    int D, Dp;
-    uint16_t *out;
-    int64_t ldo;
-    const void *target;
-    int wide;
-    int64_t ignore;
-};
-
-// One operand, or two in one launch, the first by `first` workgroups.
+// not count leave nothing in the weights' gradient, not even a value that is no number.  The first operand by `first` workgroups.
 template <typename E>
 __global__ __launch_bounds__(256) void pack_kernel(Pack one, Pack two, int first)
 {
@@ -84,6 +71,10 @@ int launch_pack(const Pack &one, const Pack &two, hipStream_t st)
     hipLaunchKernelGGL((pack_kernel<E>), dim3(all), dim3(256), 0, st, one, two, first);
     return launch_status();
 }
+
+template int launch_pack<float>(const Pack &, const Pack &, hipStream_t);
+template int launch_pack<bf16_t>(const Pack &, const Pack &, hipStream_t);
+template int launch_pack<f16_t>(const Pack &, const Pack &, hipStream_t);
 
 // ---- rows ------------------------------------------------------------------------------------------------------
 
@@ -408,11 +399,6 @@ __global__ __launch_bounds__(256) void finish_kernel(Finish f)
 // ---- joins -------------------------------------------------------------------------------------------------------
 
 // The sums of a bias's tiles, to the gradient of 256 words.
-struct BiasJoin {
-    const float *part;
-    int ld, tiles, n;
-    void *out;
-};
 template <typename E>
 __device__ __forceinline__ void join_bias(const BiasJoin &b, int block, float factor)
 {
@@ -458,49 +444,36 @@ __global__ __launch_bounds__(256) void join_kernel(const float *__restrict__ sli
     }
 }
 
+template <typename E> int launch_bias_join(const BiasJoin &b, const float *f0, const float *f1, hipStream_t st)
+{
+    hipLaunchKernelGGL((bias_join_kernel<E>), dim3(ceil_div(b.n, 256)), dim3(256), 0, st, b, f0, f1);
+    return launch_status();
+}
+template int launch_bias_join<float>(const BiasJoin &, const float *, const float *, hipStream_t);
+template int launch_bias_join<bf16_t>(const BiasJoin &, const float *, const float *, hipStream_t);
+template int launch_bias_join<f16_t>(const BiasJoin &, const float *, const float *, hipStream_t);
+
+template <typename P> int launch_join(const float *slices, int splits, int64_t count, int M, const float *f0, const float *f1, void *out,
+                                      hipStream_t st)
+{
+    typedef typename ElementOf<P>::type E;
+    const int64_t all = (count + 255) / 256;
+    const int blocks = (int)(all < 16384 ? all : 16384);
+    if (blocks == 0) return DS_OK;
+    hipLaunchKernelGGL((join_kernel<P, E>), dim3(blocks), dim3(256), 0, st, slices, splits, count, M, (float *)nullptr, 1, 1, f0, f1,
+                       (const float *)nullptr, (E *)out, (int64_t)M, blocks, BiasJoin{});
+    return launch_status();
+}
+template int launch_join<Split>(const float *, int, int64_t, int, const float *, const float *, void *, hipStream_t);
+template int launch_join<Bf16>(const float *, int, int64_t, int, const float *, const float *, void *, hipStream_t);
+template int launch_join<F16>(const float *, int, int64_t, int, const float *, const float *, void *, hipStream_t);
+
 // ---- plan --------------------------------------------------------------------------------------------------------
 
 // Workspace of a piece's P, and of its repacked weights.  Larger pieces mean fewer slices of the hidden gradient to join (95 us
 // a piece for 8192 tokens of 4096 features), smaller ones less memory; the products do not feel it.  The exponentials that a call
 // for loss and gradients keeps of 16-bit types take twice as much besides.
 constexpr size_t kPieceBytes = (size_t)1 << 30;
-
-// The tile shape of a product, and how many stretches its reduction of k is cut into (1 of `most_splits`): the pair with the
-// shortest estimate, rounds of workgroups times their steps and ends; slices are written and read once more by a launch of
-// their own.  What decides it, measured: hidden gradients of 1543 x 1000 from 20011 words, float16, 157 us on 128 x 128 tiles
-// in two stretches, 76 us on 256 x 256 in eight; 2048 x 1024 from 32768 words, float32, 1113 us (128 x 128, two) and 707 us
-// (256 x 128, four); 64 x 512 from 1000 words, float32, 25 us in one stretch, 13 in four; scores of 512 tokens of 1024 features
-// over 8000 words, bfloat16, 25, 16, 16 and 19 us from the largest tiles to the smallest.
-struct Choice { int tile, splits; };
-template <typename P>
-Choice choose(int64_t m, int64_t n, int64_t k, int shapes, int most_splits, bool prob)
-{
-    typedef Shapes<P> S;
-    const int cus = device_cus(), tile_knob = g_tune.vocab_tile, split_knob = g_tune.vocab_split;
-    const int64_t steps = (k + P::step - 1) / P::step;
-    Choice best{0, 1};
-    if (m < 1 || n < 1) return best;
-    double shortest = 1e300;
-    for (int i = 0; i < shapes; ++i) {
-        if (tile_knob >= 0 && tile_knob < shapes && i != tile_knob) continue;
-        const int64_t tiles = ((m + S::m[i] - 1) / S::m[i]) * ((n + S::n[i] - 1) / S::n[i]);
-        const int64_t fill = (int64_t)cus * S::resident[i];
-        // stretches of 256 at least, and no more workgroups than two rounds of them
-        int most = most_splits;
-        if (most > steps * P::step / 256) most = (int)(steps * P::step / 256);
-        if (split_knob >= 1) most = most < split_knob ? most : split_knob;
-        else if (most > 2 * fill / tiles) most = (int)(2 * fill / tiles);
-        if (most < 1) most = 1;
-        for (int s = split_knob >= 1 ? most : 1; s <= most; s += 1 + s / 4) {
-            const int64_t blocks = tiles * s;
-            const double step = blocks <= cus ? S::alone_us[i] : S::step_us[i];
-            const double round = (double)((steps + s - 1) / s) * step + S::ends_us[i] + (prob ? S::prob_us[i] : 0);
-            const double us = (double)((blocks + fill - 1) / fill) * round + (s > 1 ? 4 + (double)s * m * n * 4 / 3e6 : 0);
-            if (us < shortest) shortest = us, best = Choice{i, s};
-        }
-    }
-    return best;
-}
 
 struct Plan {
     int Dp;               // features of repacked operands,
@@ -516,36 +489,6 @@ struct Plan {
     int64_t ldp;          // and what a row of them takes
     size_t h, w, stats, picked, shares, arrived, prob, kept, bias, slices, acc, scale, power, factor, bytes;
 };
-
-inline bool in_place(const void *p, int64_t ld, int64_t D) { return (uintptr_t)p % 16 == 0 && ld % 8 == 0 && D % 8 == 0; }
-
-// Up to how many tokens of float32 read the weights as they are.  Small heads give each workgroup too little to read: 16 tokens of
-// 512 features, 1000 words, 44 us a step where planes take 33 (8 tokens: 31 and 34), 16 of 1024, 8000 words, 74 and 78.
-constexpr int64_t kManyWeights = 1 << 23;
-inline int64_t few_tokens(int64_t weights) { return weights < kManyWeights ? kFewTokens / 2 : kFewTokens; }
-
-// What a call does: the loss, the gradients, or both.
-enum { kLoss = 1, kGrad = 2 };
-
-// Up to how many tokens of float32 the matrix instructions take weights as they are, `width` floats at a time, split into planes by
-// every tile of 64 tokens; for more, planes for all of them to share are worth what writing and reading them takes, the sooner the
-// fewer weights there are, for gradients (whose hidden states are in planes either way) and for weights that come one by one.
-// Measured as they are and by planes, in us:
-//                                  loss of 24       128         512     a step of 24         128           256           512 tokens
-//   1024 features,  8200 words      46   44     47   62     93   94      93   88    117  121     166  152       260  225
-//   1024,          16400            45   69     61   72    140  153     108  137    163  169     252  265       412  412
-//   1024,          33000            60  126     93  154    243  271     158  242    267  330     424  482       735  753
-//   1023 (one by one), 8300         53   42     55   60    106   94     105   88    131  123     180  155       285  228
-//   1023,          16400            54   70     67   73    158  153     120  138    176  171     276  267       451  415
-//   1023,          33000            66  132    106  159    268  274     174  251    294  338     464  490       805  760
-//   2049,          50021           143  389    242  410    767  796     437  706    737  898    1266 1332      2424 2206
-constexpr int64_t kManyOddWeights = 7 << 21;
-inline int64_t raw_tokens(int64_t weights, int width, int what)
-{
-    const bool odd = width == 1, grad = what & kGrad;
-    if (weights < (odd ? kManyOddWeights : kManyWeights)) return 0;
-    return std::min<int64_t>(odd && grad ? 256 : 512, weights >> (15 + odd + grad));
-}
 
 template <typename P>
 Plan plan_of(const void *hidden, int64_t ldh, const void *weight, int64_t ldw, int64_t T, int64_t D, int64_t V, int what)
@@ -650,12 +593,6 @@ inline int check(const Call &c)
     if (c.T > most || c.V > most || c.D > 1000000 || c.ldh > 2000000 || c.ldw > 2000000) return DS_ETOOLARGE;
     return DS_OK;
 }
-
-#define DS_TRY(what)                    \
-    do {                                \
-        const int s_ = (what);          \
-        if (s_ != DS_OK) return s_;     \
-    } while (0)
 
 // The operands as the products take them: hidden states once, weights piece by piece.
 template <typename P>

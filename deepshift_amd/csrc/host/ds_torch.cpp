@@ -394,7 +394,12 @@ struct Recurrence {
     }
     const void *lengths_at() const { return lengths.defined() ? lengths.const_data_ptr() : nullptr; }
     int length_bytes() const { return lengths.defined() ? (int)lengths.element_size() : 0; }
-    at::Tensor workspace() const { return empty({(int64_t)ds_recur_workspace_bytes(B, T, D, type)}, at::kByte); }
+    // not defined where none is needed
+    at::Tensor workspace() const
+    {
+        const size_t bytes = ds_recur_workspace_bytes(B, T, D, type);
+        return bytes ? empty({(int64_t)bytes}, at::kByte) : at::Tensor();
+    }
 };
 
 // recurrence(x, gate, state or None, lengths or None, keep, stream): all states, the last ones, and, if they are to be kept for
@@ -413,7 +418,7 @@ PyObject *recurrence(PyObject *, PyObject *const *args, Py_ssize_t count)
                ds_recur_forward(x.at(), x.batch(), x.token(), gate.at(), gate.batch(), gate.token(),
                                 state.defined() ? (const float *)state.const_data_ptr() : nullptr, r.lengths_at(), r.length_bytes(),
                                 at_or_null(out), at_or_null<float>(last), at_or_null<float>(kept), r.B, r.T, r.D, r.type,
-                                ws.mutable_data_ptr(), ws.nbytes(), stream(args[5])));
+                                at_or_null(ws), ws.defined() ? ws.nbytes() : 0, stream(args[5])));
         return tuple_of({out, last, kept});
     });
 }
@@ -440,9 +445,99 @@ PyObject *recurrence_grad(PyObject *, PyObject *const *args, Py_ssize_t count)
                ds_recur_backward(x.at(), x.batch(), x.token(), gate.at(), gate.batch(), gate.token(), grad.at(), grad.batch(),
                                  grad.token(), grad_last.defined() ? (const float *)grad_last.const_data_ptr() : nullptr,
                                  r.lengths_at(), r.length_bytes(), (const float *)kept.contiguous().const_data_ptr(), at_or_null(dx),
-                                 at_or_null(dgate), at_or_null<float>(dstate), r.B, r.T, r.D, r.type, ws.mutable_data_ptr(),
-                                 ws.nbytes(), stream(args[7])));
+                                 at_or_null(dgate), at_or_null<float>(dstate), r.B, r.T, r.D, r.type, at_or_null(ws),
+                                 ws.defined() ? ws.nbytes() : 0, stream(args[7])));
         return tuple_of({dx, dgate, dstate});
+    });
+}
+
+// The operands of a gated block: x [..., D], weight [2 F, D], bias [2 F] or None.
+struct Gated {
+    at::Tensor x, weight, bias;
+    std::vector<int64_t> shape;  // of x
+    int64_t ldx, ldw, T, D, F, activation;
+    int type;
+
+    Gated(PyObject *x_, PyObject *weight_, PyObject *bias_, PyObject *activation_) : x(tensor("x", x_)), weight(tensor("weight", weight_))
+    {
+        constexpr int64_t kLongestRow = 2000000;
+        type = checked_type("x", x);
+        if (x.dim() < 1) refuse(PyExc_ValueError, "x must have the features as its last axis, is ", x.sizes());
+        shape = x.sizes().vec();
+        D = shape.back();
+        if (weight.dim() != 2 || weight.size(1) != D || weight.size(0) % 2)
+            refuse(PyExc_ValueError, "weight must be [2 F, ", std::to_string(D), "], is ", weight.sizes());
+        F = weight.size(0) / 2;
+        check_like("weight", weight, " like x", x.scalar_type(), x.device(), weight.sizes());
+        if (bias_ != Py_None) {
+            bias = tensor("bias", bias_);
+            check_like("bias", bias, " like x", x.scalar_type(), x.device(), {2 * F});
+            bias = bias.contiguous();
+        }
+        activation = integer(activation_);
+        T = 1;
+        for (size_t i = 0; i + 1 < shape.size(); ++i) T *= shape[i];
+        if (x.dim() != 2) x = x.reshape({T, D});
+        ldx = rows(x, kLongestRow);
+        ldw = rows(weight, kLongestRow);
+    }
+    at::Tensor empty(at::IntArrayRef sizes, at::ScalarType as) const
+    {
+        return at::empty(sizes, at::TensorOptions().device(x.device()).dtype(as));
+    }
+    at::Tensor empty(at::IntArrayRef sizes) const { return empty(sizes, x.scalar_type()); }
+    at::Tensor workspace(int what) const
+    {
+        return empty({(int64_t)ds_gated_workspace_bytes(x.const_data_ptr(), ldx, weight.const_data_ptr(), ldw, T, D, F, type, what)},
+                     at::kByte);
+    }
+    std::vector<int64_t> kept() const { return {T, 2, (F + 7) / 8 * 8}; }
+};
+
+// gated(x, weight, bias or None, activation, keep, stream): the block's result, and both halves of its product if they are to be
+// kept for gradients
+PyObject *gated(PyObject *, PyObject *const *args, Py_ssize_t count)
+{
+    return guarded(count, 6, [&] {
+        const Gated g(args[0], args[1], args[2], args[3]);
+        std::vector<int64_t> shape = g.shape;
+        shape.back() = g.F;
+        const at::Tensor out = g.empty(shape);
+        at::Tensor halves;
+        if (integer(args[4])) halves = g.empty(g.kept());
+        const at::Tensor ws = g.workspace(1);
+        expect("ds_gated_forward",
+               ds_gated_forward(g.x.const_data_ptr(), g.ldx, g.weight.const_data_ptr(), g.ldw,
+                                g.bias.defined() ? g.bias.const_data_ptr() : nullptr, (int)g.activation, g.T, g.D, g.F, g.type,
+                                at_or_null(out), at_or_null(halves), ws.mutable_data_ptr(), ws.nbytes(), stream(args[5])));
+        return tuple_of({out, halves});
+    });
+}
+
+// gated_grad(x, weight, halves, grad, activation, wanted, stream): gradients of x, weight and bias; bits 0 to 2 of `wanted` say
+// which
+PyObject *gated_grad(PyObject *, PyObject *const *args, Py_ssize_t count)
+{
+    return guarded(count, 7, [&] {
+        const Gated g(args[0], args[1], Py_None, args[4]);
+        const at::Tensor &halves = tensor("halves", args[2]);
+        check_like("halves", halves, " like x", g.x.scalar_type(), g.x.device(), g.kept());
+        at::Tensor grad = tensor("grad", args[3]);
+        std::vector<int64_t> shape = g.shape;
+        shape.back() = g.F;
+        check_like("grad", grad, " like x", g.x.scalar_type(), g.x.device(), shape);
+        if (grad.dim() != 2) grad = grad.reshape({g.T, g.F});
+        const int64_t ldg = rows(grad), wanted = integer(args[5]);
+        at::Tensor dx, dweight, dbias;
+        if (wanted & 1) dx = g.empty(g.shape);
+        if (wanted & 2) dweight = g.empty({2 * g.F, g.D});
+        if (wanted & 4) dbias = g.empty({2 * g.F});
+        const at::Tensor ws = g.workspace(2);
+        expect("ds_gated_backward",
+               ds_gated_backward(g.x.const_data_ptr(), g.ldx, g.weight.const_data_ptr(), g.ldw, halves.const_data_ptr(),
+                                 grad.const_data_ptr(), ldg, (int)g.activation, g.T, g.D, g.F, g.type, at_or_null(dx),
+                                 at_or_null(dweight), at_or_null(dbias), ws.mutable_data_ptr(), ws.nbytes(), stream(args[6])));
+        return tuple_of({dx, dweight, dbias});
     });
 }
 
@@ -556,6 +651,10 @@ PyMethodDef methods[] = {
      "recurrence(x, gate, state or None, lengths or None, keep, stream) -> states, last ones, kept ones or None"},
     {"recurrence_grad", (PyCFunction)(void (*)(void))recurrence_grad, METH_FASTCALL,
      "recurrence_grad(x, gate, grad or None, grad_last or None, lengths or None, kept, wanted, stream) -> gradients"},
+    {"gated", (PyCFunction)(void (*)(void))gated, METH_FASTCALL,
+     "gated(x, weight, bias or None, activation, keep, stream) -> result, halves of the product or None"},
+    {"gated_grad", (PyCFunction)(void (*)(void))gated_grad, METH_FASTCALL,
+     "gated_grad(x, weight, halves, grad, activation, wanted, stream) -> gradients"},
     {"clip", (PyCFunction)(void (*)(void))clip, METH_FASTCALL,
      "clip(grads, outs or None, max_norm, scale, any_order, stream) -> norm, or None"},
     {nullptr, nullptr, 0, nullptr},

@@ -179,11 +179,18 @@ class LinearShift(_PackedWeightsMixin, nn.Module):
             # the packed weights already hold the clamped, rounded codes (pack_module_weights), so
             # the per-call clamp of the float parameter (modules.py:125) would change nothing here
             return self._kernel_forward(input)
+        return F.linear(input, self.float_weight(), self.bias)
+
+    def float_weight(self):
+        """The weights of the float path, +-2^shift, with straight-through gradients."""
         self.shift.data = ste.clamp(self.shift.data, *self.shift_range)
         shift_rounded = ste.round(self.shift, rounding=self.rounding)
         sign_rounded_signed = ste.sign(ste.round(self.sign, rounding=self.rounding))
-        weight_ps = ste.unsym_grad_mul(2 ** shift_rounded, sign_rounded_signed)
-        return F.linear(input, weight_ps, self.bias)
+        return ste.unsym_grad_mul(2 ** shift_rounded, sign_rounded_signed)
+
+    def float_input(self, input):
+        """What the float path multiplies with them."""
+        return input
 
     def extra_repr(self):
         return 'in_features={}, out_features={}, bias={}'.format(

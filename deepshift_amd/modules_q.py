@@ -104,16 +104,22 @@ class LinearShiftQ(_PackedQMixin, nn.Module):
         if self.use_kernel:
             # packed from the clamped weight (pack_module_weights_q): nothing left to clamp per call
             return self._kernel_forward(input)
-        self.weight.data = ste.clampabs(self.weight.data, 2 ** self.shift_range[0],
-                                        2 ** self.shift_range[1])
-        weight_q = ste.round_power_of_2(self.weight, self.rounding)
-        input_fixed_point = ste.round_fixed_point(input, self.act_integer_bits,
-                                                  self.act_fraction_bits)
-        out = input_fixed_point.mm(weight_q.t())
+        weight_q = self.float_weight()
+        out = self.float_input(input).mm(weight_q.t())
         if self.bias is not None:
             # modules_q.py:129: the un-rounded bias is added on this path
             out = out + self.bias.unsqueeze(0).expand_as(out)
         return out
+
+    def float_weight(self):
+        """The weights of the float path, rounded to powers of two, with straight-through gradients."""
+        self.weight.data = ste.clampabs(self.weight.data, 2 ** self.shift_range[0],
+                                        2 ** self.shift_range[1])
+        return ste.round_power_of_2(self.weight, self.rounding)
+
+    def float_input(self, input):
+        """What the float path multiplies with them: the activations in fixed point."""
+        return ste.round_fixed_point(input, self.act_integer_bits, self.act_fraction_bits)
 
     def extra_repr(self):
         return 'in_features={}, out_features={}, bias={}'.format(

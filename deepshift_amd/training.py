@@ -16,10 +16,10 @@ import torch.nn as nn
 from torch.autograd import Function
 from torch.autograd.function import once_differentiable
 
-from . import _lib
+from . import _lib, modules, modules_q
 
-__all__ = ["embedding", "embedding_grad", "linear_cross_entropy", "linear_cross_entropy_grad", "gradient_norm",
-           "clip_gradients_", "clip_grad_norm_", "gated_recurrence", "ScaledEmbedding", "LinearCrossEntropy"]
+__all__ = ["embedding", "embedding_grad", "linear_cross_entropy", "linear_cross_entropy_grad", "gated_linear", "gated_recurrence",
+           "gradient_norm", "clip_gradients_", "clip_grad_norm_", "ScaledEmbedding", "LinearCrossEntropy", "GatedLinear", "GatedShift"]
 
 _REDUCTIONS = {"none": _lib.DS_NONE, "sum": _lib.DS_SUM, "mean": _lib.DS_MEAN}
 
@@ -212,6 +212,56 @@ def gated_recurrence(x, gate, state=None, lengths=None):
 
 
 # ---------------------------------------------------------------------------------------------
+# gated block
+# ---------------------------------------------------------------------------------------------
+
+_ACTIVATIONS = {"silu": _lib.DS_SILU, "gelu": _lib.DS_GELU, "relu": _lib.DS_RELU, "sigmoid": _lib.DS_SIGMOID}
+
+
+def _activation(activation):
+    if activation not in _ACTIVATIONS:
+        raise ValueError("activation must be 'silu', 'gelu', 'relu' or 'sigmoid', is %r" % (activation,))
+    return _ACTIVATIONS[activation]
+
+
+def _gate(x, weight, bias, activation, keep):
+    device = x.device
+    with _on(device):
+        return _lib.native().gated(x, weight, bias, activation, keep, _stream_of(device))
+
+
+class _GatedLinear(Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, activation):
+        out, halves = _gate(x, weight, bias, activation, True)
+        ctx.save_for_backward(x, weight, halves)
+        ctx.activation = activation
+        return out
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad):
+        x, weight, halves = ctx.saved_tensors
+        device, needed = x.device, ctx.needs_input_grad
+        with _on(device):
+            dx, dweight, dbias = _lib.native().gated_grad(x, weight, halves, grad, ctx.activation,
+                                                          needed[0] | needed[1] << 1 | needed[2] << 2, _stream_of(device))
+        return dx, dweight, dbias, None
+
+
+def gated_linear(x, weight, bias=None, activation="silu"):
+    """``act(x @ gate.T + b) * (x @ up.T + c)``, the gated block of a feed-forward layer, both projections, the activation and the
+    product in one kernel: ``weight`` ``[2 F, D]`` is ``gate`` above ``up`` and ``bias`` ``[2 F]`` ``b`` before ``c`` -- what one
+    linear layer, or one ``LinearShift``, of ``2 F`` features holds.  ``x`` ``[..., D]``, all of one type; ``activation`` is
+    ``'silu'``, ``'gelu'`` (by the error function), ``'relu'`` or ``'sigmoid'``.  For gradients both projections are kept in that
+    type."""
+    activation = _activation(activation)
+    if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or (bias is not None and bias.requires_grad)):
+        return _GatedLinear.apply(x, weight, bias, activation)
+    return _gate(x, weight, bias, activation, False)[0]
+
+
+# ---------------------------------------------------------------------------------------------
 # clipping
 # ---------------------------------------------------------------------------------------------
 
@@ -382,3 +432,45 @@ class LinearCrossEntropy(nn.Module):
     def extra_repr(self):
         return "{}, {}, bias={}, ignore_index={}, reduction={}".format(
             self.in_features, self.num_classes, self.bias is not None, self.ignore_index, self.reduction)
+
+
+class GatedLinear(nn.Module):
+    """:func:`gated_linear` with a weight and a bias of its own, drawn as an ``nn.Linear`` of ``2 * out_features`` draws them."""
+
+    def __init__(self, in_features, out_features, bias=True, activation="silu"):
+        super().__init__()
+        _activation(activation)
+        self.in_features, self.out_features, self.activation = in_features, out_features, activation
+        both = nn.Linear(in_features, 2 * out_features, bias=bias)
+        self.weight, self.bias = both.weight, both.bias
+
+    def forward(self, x):
+        return gated_linear(x, self.weight, self.bias, self.activation)
+
+    def extra_repr(self):
+        return "{}, {}, bias={}, activation={!r}".format(self.in_features, self.out_features, self.bias is not None, self.activation)
+
+
+class GatedShift(nn.Module):
+    """The gated block with weights of powers of two: ``layer`` is one ``LinearShift`` (``shift_type`` ``'PS'``) or ``LinearShiftQ``
+    (``'Q'``) of twice the width, whose float path's weights go into :func:`gated_linear`; straight-through gradients reach its
+    parameters.  With ``use_kernel`` (no gradients) the layer runs on the shift kernels, and the gate behind it."""
+
+    def __init__(self, in_features, out_features, bias=True, activation="silu", shift_type="PS", **options):
+        super().__init__()
+        if shift_type not in ("PS", "Q"):
+            raise ValueError("shift_type must be 'PS' or 'Q', is %r" % (shift_type,))
+        _activation(activation)
+        self.in_features, self.out_features, self.activation = in_features, out_features, activation
+        kind = modules.LinearShift if shift_type == "PS" else modules_q.LinearShiftQ
+        self.layer = kind(in_features, 2 * out_features, bias=bias, **options)
+
+    def forward(self, x):
+        layer = self.layer
+        if layer.use_kernel:
+            gate, up = layer(x).chunk(2, -1)
+            return getattr(nn.functional if self.activation in ("silu", "gelu") else torch, self.activation)(gate) * up
+        return gated_linear(layer.float_input(x), layer.float_weight(), layer.bias, self.activation)
+
+    def extra_repr(self):
+        return "{}, {}, activation={!r}".format(self.in_features, self.out_features, self.activation)

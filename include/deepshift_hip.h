@@ -567,13 +567,29 @@ int ds_vocab_loss_step(const void *hidden, int64_t ldh, const void *weight, int6
                        float *lse, float *total, void *dhidden, void *dweight, void *dbias, void *workspace,
                        size_t workspace_bytes, ds_stream_t stream);
 
+/* Gated block of a feed-forward layer: out[t][f] = act(x[t] . weight[f] + bias[f]) * (x[t] . weight[F + f] + bias[F + f]), x [T][D],
+ * weight [2 F][D], bias [2 F] or NULL, out [T][F], all of `type`.  halves, or NULL, is [T][2][F rounded up to a multiple of 8] and
+ * gets both products, which ds_gated_backward takes.  workspace: 256-byte aligned, ds_gated_workspace_bytes(..., what) bytes with
+ * what = 1 here and 2 there. */
+enum { DS_SILU = 0, DS_GELU = 1, DS_RELU = 2, DS_SIGMOID = 3 };
+size_t ds_gated_workspace_bytes(const void *x, int64_t ldx, const void *weight, int64_t ldw, int64_t T, int64_t D, int64_t F, int type,
+                                int what);
+int ds_gated_forward(const void *x, int64_t ldx, const void *weight, int64_t ldw, const void *bias, int activation, int64_t T,
+                     int64_t D, int64_t F, int type, void *out, void *halves, void *workspace, size_t workspace_bytes,
+                     ds_stream_t stream);
+
+/* Its gradients for grad [T][F], rows ldg apart: dx [T][D], dweight [2 F][D], dbias [2 F], each NULL where it is not asked for. */
+int ds_gated_backward(const void *x, int64_t ldx, const void *weight, int64_t ldw, const void *halves, const void *grad, int64_t ldg,
+                      int activation, int64_t T, int64_t D, int64_t F, int type, void *dx, void *dweight, void *dbias,
+                      void *workspace, size_t workspace_bytes, ds_stream_t stream);
+
 /* Gated linear recurrence along sequences, channel by channel: with a = 1 / (1 + exp(-gate)),
  *   h[t] = a[t] h[t - 1] + (1 - a[t]) x[t],
  * from state[b][:] (zeros where state is NULL).  x and gate hold [B][T][D] elements of `type`, channels next to each other,
  * tokens *_token and sequences *_batch elements apart; state and last are float32 [B][D], out is [B][T][D].  With lengths
  * (int32 or int64, length_bytes 4 or 8, held to [0, T]) a sequence ends there: what x and gate hold behind it is not looked at,
  * out is 0 there, and last is the state at its end.  kept [B][ds_recur_blocks(T)][D], or NULL, is what ds_recur_backward needs.
- * workspace: 256-byte aligned, ds_recur_workspace_bytes() bytes. */
+ * workspace: 256-byte aligned, ds_recur_workspace_bytes() bytes (0 for many sizes: then it may be NULL). */
 int64_t ds_recur_blocks(int64_t T);
 size_t ds_recur_workspace_bytes(int64_t B, int64_t T, int64_t D, int type);
 int ds_recur_forward(const void *x, int64_t x_batch, int64_t x_token, const void *gate, int64_t gate_batch, int64_t gate_token,

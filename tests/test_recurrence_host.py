@@ -34,7 +34,7 @@ def test_forward_mode_and_tracing_are_refused():
 
 def test_the_library_checks_sizes_and_pointers():
     L = _lib.lib()
-    assert [L.ds_recur_blocks(T) for T in (0, 1, 8, 9, 64, 65, 128, 129)] == [0, 1, 1, 1, 2, 1, 1, 2]
+    assert [L.ds_recur_blocks(T) for T in (0, 1, 8, 9, 32, 33, 64, 65, 129)] == [0, 1, 1, 1, 1, 1, 1, 2, 3]
     assert L.ds_recur_workspace_bytes(2, 3, 4, 7) == 0 and L.ds_recur_workspace_bytes(-1, 3, 4, 0) == 0
     at = X.data_ptr()
 
