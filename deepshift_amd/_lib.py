@@ -59,6 +59,7 @@ class Tensor(ctypes.Structure):
 _tp = ctypes.POINTER(Tensor)
 _float = ctypes.c_float
 _matrix = [_ptr, _c_i64]   # an operand and the distance of its rows
+_taught = [_ptr, _ptr, _c_int, _ptr, _c_int, _c_int, _float]   # a bias, and a teacher's words
 _sequence = [_ptr, _c_i64, _c_i64]   # sequences, the distances of them and of their tokens
 
 # name -> (restype, argtypes); mirrors include/deepshift_hip.h one to one
@@ -133,6 +134,10 @@ SIGNATURES = {
     "ds_vocab_loss_grad": (_c_int, _matrix * 2 + [_ptr, _ptr, _c_int] + [_c_i64] * 4 + [_c_int] + [_ptr] * 8 + [_size, _ptr]),
     "ds_vocab_loss_step": (_c_int, _matrix * 2 + [_ptr, _ptr, _c_int] + [_c_i64] * 4 + [_c_int, _c_int] + [_ptr] * 7 +
                            [_size, _ptr]),
+    "ds_distill_workspace_bytes": (_size, _matrix * 2 + [_c_i64] * 3 + [_c_int] * 3),
+    "ds_distill_loss": (_c_int, _matrix * 2 + _taught + [_c_i64] * 3 + [_c_int, _c_int] + [_ptr] * 4 + [_size, _ptr]),
+    "ds_distill_loss_grad": (_c_int, _matrix * 2 + _taught + [_c_i64] * 3 + [_c_int] + [_ptr] * 8 + [_size, _ptr]),
+    "ds_distill_loss_step": (_c_int, _matrix * 2 + _taught + [_c_i64] * 3 + [_c_int, _c_int] + [_ptr] * 7 + [_size, _ptr]),
     "ds_gated_workspace_bytes": (_size, _matrix * 2 + [_c_i64] * 3 + [_c_int, _c_int]),
     "ds_gated_forward": (_c_int, _matrix * 2 + [_ptr, _c_int] + [_c_i64] * 3 + [_c_int, _ptr, _ptr, _ptr, _size, _ptr]),
     "ds_gated_backward": (_c_int, _matrix * 2 + [_ptr] + _matrix + [_c_int] + [_c_i64] * 3 + [_c_int] + [_ptr] * 4 + [_size, _ptr]),

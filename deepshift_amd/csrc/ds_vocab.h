@@ -156,6 +156,13 @@ struct Args {
     int64_t ldo;
     const float *factor[2];  // what results are multiplied with, 1 value each, or NULL
     int n_store;          // rows of C that exist (N may be rounded up for the loads)
+    // TAUGHT: instead of one target a token has up to `taught_words` of them, each with a probability: their numbers in ascending
+    // order, 0x7fffffff behind the last, and the probabilities; picked has as many values a token.  `target` only says which
+    // tokens count.  Logits are multiplied by `warmth`.
+    const int *taught_ids;
+    const float *taught;
+    int taught_words;
+    float warmth;
     // kGate (bias, out and ldo too): M is half of A's rows
     int64_t half_bytes;   // from the first half to the second
     int activation;
@@ -506,14 +513,20 @@ struct Known {
     float scale[BN];
     float power[BN];
 };
+template <int BM, int BN>
+struct TaughtKnown : Known<BM, BN> {
+    int first[BN], last[BN];  // which of the token's words lie in the tile
+};
+template <int BM, int BN, bool TAUGHT>
+using KnownOf = typename std::conditional<TAUGHT, TaughtKnown<BM, BN>, Known<BM, BN>>::type;
 // Rows that leave together, what one of them takes, and whether the waves' maxima and sums find a place behind them in the
 // stages (256 x 256 tiles' exponentials fill those).
 template <typename P, int WN> constexpr int kRowsLeaving = WN * Unit<P>::size;
 template <typename P, int BM, int KIND> constexpr int kRowBytes = KIND == kGate ? BM / 2 * 4 : KIND == kOut || (KIND == kKeep && P::planes == 1) ? BM * 4 : BM * P::planes * 2;
 template <typename P, int BM, int BN, int WM, int WN, int KIND, int STAGES, bool RAW>
 constexpr bool kRoomBehind = KIND == kStats || kRowsLeaving<P, WN> * kRowBytes<P, BM, KIND> + WM * BN * 8 <= kStagesBytes<P, BM, BN, STAGES, RAW>;
-template <typename P, int BM, int BN, int WM, int WN, int KIND, int STAGES, bool RAW = false>
-constexpr int kLdsBytes = kStagesBytes<P, BM, BN, STAGES, RAW> + (KIND != kOut ? (int)sizeof(Known<BM, BN>) : 0) +
+template <typename P, int BM, int BN, int WM, int WN, int KIND, int STAGES, bool RAW = false, bool TAUGHT = false>
+constexpr int kLdsBytes = kStagesBytes<P, BM, BN, STAGES, RAW> + (KIND != kOut ? (int)sizeof(KnownOf<BM, BN, TAUGHT>) : 0) +
                           (KIND == kKeep && !kRoomBehind<P, BM, BN, WM, WN, KIND, STAGES, RAW> ? WM * BN * 8 : 0) +
                           (P::planes > 1 ? 16 : 0);
 
@@ -585,7 +598,7 @@ __device__ __forceinline__ int spread_sums(float (&v)[ALL], int lane)
 // are read and stages fetched between rows of products, a few each: with all of them behind the barrier the matrix cores were
 // busy 55 % of the cycles instead of 70 to 85 (4.0 instead of 3.2 ms for the scores above).  32 x 32 instructions take half as
 // many issues as 16 x 16 ones at the same rate; float32 keeps the smaller ones, whose partial sums of the planes fit.
-template <typename P, int BM, int BN, int WM, int WN, bool A_ACROSS, bool B_ACROSS, int KIND, int STAGES, int RAW = 0>
+template <typename P, int BM, int BN, int WM, int WN, bool A_ACROSS, bool B_ACROSS, int KIND, int STAGES, int RAW = 0, bool TAUGHT = false>
 __device__ __forceinline__ void product_tile(const Args &g, const int block, char *lds)
 {
     using U = Unit<P>;
@@ -634,20 +647,37 @@ __device__ __forceinline__ void product_tile(const Args &g, const int block, cha
 #pragma unroll
             for (int r = 0; r < 4 * U::groups; ++r) acc[i][j][r] = 0.f;
 
-    Known<BM, BN> &known = *(Known<BM, BN> *)(lds + kStagesBytes<P, BM, BN, STAGES, (RAW > 0)>);
+    typedef KnownOf<BM, BN, TAUGHT> Here;
+    Here &known = *(Here *)(lds + kStagesBytes<P, BM, BN, STAGES, (RAW > 0)>);
     static_assert(BM <= WAVES * 64 && BN <= WAVES * 64, "a thread per word and token");
     constexpr int kNowhere = -(1 << 20);
     float bias = -INFINITY, lse = INFINITY, scale = 0.f, power = 1.f;
-    int want = kNowhere;
+    int want = kNowhere, first = 0, last = 0;
+    // base 2
+    const float to_logit = TAUGHT ? kLog2e * g.warmth : kLog2e;
     if constexpr (KIND == kGate) {
         const int slot = threadIdx.x, m = m0 + slot / (2 * U::size) * U::size + slot % U::size;
         bias = slot < BM && m < g.M ? bias_at(g, m + (slot / U::size % 2 ? g.M : 0)) : 0.f;
     } else if constexpr (KIND != kOut) {
         const int m = m0 + threadIdx.x, n = n0 + threadIdx.x;
-        if (threadIdx.x < BM && m < g.M) bias = bias_at(g, g.v0 + m) * kLog2e;
+        if (threadIdx.x < BM && m < g.M) bias = bias_at(g, g.v0 + m) * to_logit;
         if (threadIdx.x < BN && n < g.N) {
             const int64_t y = target_at(g, n), here = y - g.v0 - m0;
-            if (here >= 0 && here < BM && m0 + here < g.M) want = (int)here;
+            if (!TAUGHT && here >= 0 && here < BM && m0 + here < g.M) want = (int)here;
+            if constexpr (TAUGHT) {
+                // the first of the token's words that is not below `word`
+                const int *const ids = g.taught_ids + (int64_t)n * g.taught_words;
+                auto behind = [&](int word) {
+                    int low = 0, high = g.taught_words;
+                    while (low < high) {
+                        const int middle = (low + high) / 2;
+                        if (ids[middle] < word) low = middle + 1;
+                        else high = middle;
+                    }
+                    return low;
+                };
+                first = behind(g.v0 + m0), last = behind(g.v0 + min(g.M, m0 + BM));
+            }
             if constexpr (KIND == kProb) {
                 if (y != g.ignore) {
                     lse = g.lse[n];
@@ -660,11 +690,13 @@ __device__ __forceinline__ void product_tile(const Args &g, const int block, cha
         }
     }
 
-    int *const met_nan = (int *)(lds + kLdsBytes<P, BM, BN, WM, WN, KIND, STAGES, (RAW > 0)>) - 1;  // of float32: a result is NaN
+    int *const met_nan = (int *)(lds + kLdsBytes<P, BM, BN, WM, WN, KIND, STAGES, (RAW > 0), TAUGHT>) - 1;  // of float32: a result is NaN
     auto keep_known = [&] {
         if (NP > 1 && threadIdx.x == 0) *met_nan = 0;
         if constexpr (KIND != kOut) {
             if (threadIdx.x < BM) known.bias[threadIdx.x] = bias;
+            if constexpr (TAUGHT)
+                if (threadIdx.x < BN) known.first[threadIdx.x] = first, known.last[threadIdx.x] = last;
             if (KIND != kGate && threadIdx.x < BN)
                 known.want[threadIdx.x] = want, known.lse[threadIdx.x] = lse, known.scale[threadIdx.x] = scale;
             if (P::half && KIND == kProb && threadIdx.x < BN) known.power[threadIdx.x] = power;
@@ -947,7 +979,31 @@ __device__ __forceinline__ void product_tile(const Args &g, const int block, cha
     auto value = [&](int I, int j, int r) -> float { return acc[I / U::groups][j][I % U::groups * 4 + r]; };
     float *fl = (float *)lds;
     // a logit, base 2
-    auto logit = [&](int I, int j, int r) -> float { return fmaf(value(I, j, r), kLog2e, known.bias[m_in + m_of(I) + r]); };
+    auto logit = [&](int I, int j, int r) -> float { return fmaf(value(I, j, r), to_logit, known.bias[m_in + m_of(I) + r]); };
+    // TAUGHT: walks over the taught words of column j that lie in the tile, along with its words: `found(e, r)` for those among
+    // the four of I.  Both are in ascending order; lanes that share a column skip each other's.
+    int taught_at = 0, taught_last = 0, taught_word = 0;
+    const int *taught_ids = nullptr;
+    auto look_at_taught = [&] {
+        taught_word = taught_at < taught_last ? taught_ids[taught_at] - g.v0 - m0 - m_in : 0x7fffffff;
+    };
+    auto begin_taught = [&](int j) {
+        if constexpr (TAUGHT) {
+            const int c = n_in + j * U::size;
+            taught_at = known.first[c], taught_last = known.last[c];
+            taught_ids = g.taught_ids + (int64_t)(n0 + c) * g.taught_words;
+            look_at_taught();
+        }
+    };
+    auto walk_taught = [&](int I, auto found) {
+        if constexpr (TAUGHT)
+            while (__any(taught_word < m_of(I) + 4)) {
+                if (taught_word >= m_of(I) + 4) continue;
+                if (taught_word >= m_of(I)) found(taught_at, taught_word - m_of(I));
+                ++taught_at;
+                look_at_taught();
+            }
+    };
     constexpr int kRowsOut = kRowsLeaving<P, WN>, kThreads = WAVES * 64;  // one j of every wave
     static_assert(KIND == kStats || kRowsOut * kRowBytes<P, BM, KIND> <= kStagesBytes<P, BM, BN, STAGES, (RAW > 0)>, "");
     auto n_of = [](int row, int j) { return (row / U::size * NT + j) * U::size + row % U::size; };
@@ -999,6 +1055,7 @@ __device__ __forceinline__ void product_tile(const Args &g, const int block, cha
         auto tops_of = [&](int j) {
             const int at = known.want[n_in + j * U::size] - m_in;  // where the target lies behind this lane's first word
             float top = -INFINITY;
+            begin_taught(j);
 #pragma unroll
             for (int I = 0; I < MG; ++I) {
                 float s[4];
@@ -1011,6 +1068,10 @@ __device__ __forceinline__ void product_tile(const Args &g, const int block, cha
 #pragma unroll
                     for (int r = 0; r < 4; ++r)
                         if (at == m_of(I) + r) g.picked[n0 + n_in + j * U::size] = s[r];
+                walk_taught(I, [&](int e, int which) {
+                    g.picked[(int64_t)(n0 + n_in + j * U::size) * g.taught_words + e] =
+                        which < 2 ? which == 0 ? s[0] : s[1] : which == 2 ? s[2] : s[3];
+                });
             }
             return top;
         };
@@ -1092,6 +1153,7 @@ __device__ __forceinline__ void product_tile(const Args &g, const int block, cha
             const float least = lse == INFINITY ? -INFINITY : -126.f;
             const bool counts = !(lse == INFINITY && scale == 0.f);  // else nothing is left, also of infinite weights times 0
             const int at = known.want[n_in + j * U::size] - m_in;
+            begin_taught(j);
 #pragma unroll
             for (int I = 0; I < MG; ++I) {
                 float x[4], p[4];
@@ -1101,6 +1163,11 @@ __device__ __forceinline__ void product_tile(const Args &g, const int block, cha
                 if ((unsigned)(at - m_of(I)) < 4u)
 #pragma unroll
                     for (int r = 0; r < 4; ++r) p[r] -= at == m_of(I) + r ? 1.f : 0.f;
+                walk_taught(I, [&](int e, int which) {
+                    const float q = g.taught[(int64_t)(n0 + n_in + j * U::size) * g.taught_words + e];
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) p[r] -= which == r ? q : 0.f;
+                });
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
                     p[r] = counts ? p[r] * scale : 0.f;
@@ -1221,6 +1288,21 @@ __global__ __launch_bounds__(256, 2) void raw_kernel(Args g)
     product_tile<Split, BM, BN, 4, 1, KIND == kOut, false, KIND, STAGES, WIDTH>(g, blockIdx.x, lds);
 }
 
+// The logits where every token has words of a teacher's (ds_taught*.hip).
+template <typename P, int BM, int BN, int WM, int WN, int KIND, int STAGES>
+__global__ __launch_bounds__(WM * WN * 64) void taught_kernel(Args g)
+{
+    __shared__ __attribute__((aligned(1024))) char lds[kLdsBytes<P, BM, BN, WM, WN, KIND, STAGES, false, true>];
+    product_tile<P, BM, BN, WM, WN, false, false, KIND, STAGES, 0, true>(g, blockIdx.x, lds);
+}
+template <int KIND, int WIDTH>
+__global__ __launch_bounds__(256, 2) void taught_raw_kernel(Args g)
+{
+    constexpr int BM = kRawWords, BN = kRawTokens, STAGES = 2;
+    __shared__ __attribute__((aligned(1024))) char lds[kLdsBytes<Split, BM, BN, 4, 1, KIND, STAGES, true, true>];
+    product_tile<Split, BM, BN, 4, 1, false, false, KIND, STAGES, WIDTH, true>(g, blockIdx.x, lds);
+}
+
 // Both gradients' products in one launch, `first` workgroups for the first.
 template <typename P, int BM, int BN, int WM, int WN, int STAGES>
 __global__ __launch_bounds__(WM * WN * 64) void both_kernel(Args hidden, Args weight, int first)
@@ -1258,10 +1340,35 @@ template <typename P> constexpr int kGradShapes = P::planes == 1 ? 4 : 3;
 // one launch, both with that shape (g is kHidden, *other kWeight).  A translation unit per P.
 template <typename P> int launch_product(int kind, int tile, Args &g, Args *other, hipStream_t st);
 
+// The logits' products (kinds up to kLogitProb) where the words are a teacher's; or, as they are, float32 weights `width` at a time.
+template <typename P> int launch_taught(int kind, int tile, Args &g, hipStream_t st);
+int launch_taught_raw(int kind, int width, Args &g, hipStream_t st);
+
 // The same for up to kFewTokens tokens of float32, with operands that lie as the caller's do (P excepted); the logits' tiles are
 // kFewWords words of all tokens, hidden gradients always go to slices.
 constexpr int kFewTokens = 16, kFewWords = 32;
 int launch_few(int kind, int tokens, Args &g, hipStream_t st);
+
+template <typename P, int BM, int BN, int WM, int WN, int STAGES>
+int launch_taught_tiled(int kind, Args &g, hipStream_t st)
+{
+    g.tiles_m = ceil_div(g.M, BM), g.tiles_n = ceil_div(g.N, BN);
+    const int64_t blocks = (int64_t)g.tiles_m * g.tiles_n;
+    if (blocks > 0x7fffffff) return DS_ETOOLARGE;
+    const dim3 grid((unsigned)blocks), threads(WM * WN * 64);
+    if (kind == kLogitStats) hipLaunchKernelGGL((taught_kernel<P, BM, BN, WM, WN, kStats, STAGES>), grid, threads, 0, st, g);
+    else if (kind == kLogitKeep) hipLaunchKernelGGL((taught_kernel<P, BM, BN, WM, WN, kKeep, STAGES>), grid, threads, 0, st, g);
+    else hipLaunchKernelGGL((taught_kernel<P, BM, BN, WM, WN, kProb, STAGES>), grid, threads, 0, st, g);
+    return launch_status();
+}
+template <typename P>
+int launch_taught_16(int kind, int tile, Args &g, hipStream_t st)
+{
+    if (tile == 0) return launch_taught_tiled<P, 256, 256, 2, 4, 2>(kind, g, st);
+    if (tile == 1) return launch_taught_tiled<P, 128, 128, 2, 2, 2>(kind, g, st);
+    if (tile == 2) return launch_taught_tiled<P, 128, 64, 4, 1, 3>(kind, g, st);
+    return launch_taught_tiled<P, 64, 64, 2, 2, 3>(kind, g, st);
+}
 
 template <typename P, int BM, int BN, int WM, int WN, int STAGES, bool GRADS = true>
 int launch_tiled(int kind, Args &g, Args *other, hipStream_t st)

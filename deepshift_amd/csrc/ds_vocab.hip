@@ -9,6 +9,11 @@
 // formula's own.  Where loss and gradients are asked for in one call, the forward pass leaves the last piece's exponentials,
 // relative to their tiles' maxima, in a workspace, in 32 bits, and a pass over them makes them P: three products for that piece,
 // which may be the whole vocabulary.
+//
+// Distillation from a teacher's best K words is the same with many targets a token, q the softmax of their logits by the
+// temperature c:  p = softmax(s / c)      loss[t] = c^2 sum_k q_k (log q_k - log p_k)      P = c g_t (p - q).
+// One launch makes q of the teacher's logits and puts the words in ascending order; the tiles find the words that lie in them by
+// a binary search while their operands arrive, and walk over them along with their logits.
 #include "ds_vocab_host.h"
 
 namespace ds {
@@ -90,11 +95,11 @@ struct Share { double loss, rows; };
 
 // total[0]: the sum or the mean of the counted rows' losses, total[1]: one row's share in it.  Without a counted row both the
 // loss and the gradients are 0.
-__device__ __forceinline__ void write_total(double loss, double rows, int mean, float *total)
+__device__ __forceinline__ void write_total(double loss, double rows, int mean, float *total, float temperature = 1.f)
 {
     const double share = mean && rows > 0 ? 1.0 / rows : 1.0;
     total[0] = (float)(loss * share);
-    total[1] = (float)share;
+    total[1] = (float)(share * temperature);  // (the gradient of a teacher's words is the temperature times P)
 }
 
 // A maximum and a sum of exponentials relative to it, joined with another such pair.
@@ -118,6 +123,10 @@ struct Rows {
     Share *shares;
     uint32_t *arrived;
     float *total;
+    // of a teacher: its probabilities of the picked words, so many of each, and its temperature; else NULL, 0 and 1
+    const float *taught;
+    int words;
+    float temperature;
 };
 
 __device__ __forceinline__ float log_of_sum(float top, float sum) { return sum == 0.f ? -INFINITY : top + log2f(sum); }
@@ -125,6 +134,19 @@ __device__ __forceinline__ float log_of_sum(float top, float sum) { return sum =
 __device__ __forceinline__ float loss_of(const Rows &r, int t, int64_t y, float lse)
 {
     return y == r.ignore ? 0.f : y < 0 || y >= r.V ? NAN : (lse - r.picked[t]) * kLn2;
+}
+
+// A share of a row's distance from its teacher: every `step`-th of its words from `from` on.
+__device__ __forceinline__ float taught_loss(const Rows &r, int t, float lse, int from, int step)
+{
+    float sum = 0.f;
+    const float *const q = r.taught + (int64_t)t * r.words, *const s = r.picked + (int64_t)t * r.words;
+#pragma unroll 4
+    for (int k = from; k < r.words; k += step) {
+        const float p = q[k];
+        if (p > 0.f) sum += p * (log2f(p) - (s[k] - lse));  // (places behind the last word hold 0, and their logits nothing)
+    }
+    return sum;
 }
 
 // A workgroup's part in the total: its wave's sums of losses and of counted rows, `group` of `groups`.  The one that ends last
@@ -135,7 +157,7 @@ __device__ __forceinline__ void add_to_total(const Rows &r, double loss, double 
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) loss += __shfl_xor(loss, o), counted += __shfl_xor(counted, o);
     if (groups == 1) {
-        if (lane == 0) write_total(loss, counted, r.reduction == DS_MEAN, r.total);
+        if (lane == 0) write_total(loss, counted, r.reduction == DS_MEAN, r.total, r.temperature);
         return;
     }
     uint32_t before = 0;
@@ -149,7 +171,7 @@ __device__ __forceinline__ void add_to_total(const Rows &r, double loss, double 
     for (int i = lane; i < groups; i += 64) loss += r.shares[i].loss, counted += r.shares[i].rows;
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) loss += __shfl_xor(loss, o), counted += __shfl_xor(counted, o);
-    if (lane == 0) write_total(loss, counted, r.reduction == DS_MEAN, r.total);
+    if (lane == 0) write_total(loss, counted, r.reduction == DS_MEAN, r.total, r.temperature);
 }
 
 // Joins the tiles' maxima and sums: a workgroup has kRowsJoined rows, each of its waves a sixteenth of the tiles and each
@@ -181,11 +203,18 @@ __global__ __launch_bounds__(1024) void row_kernel(Rows r)
 #pragma unroll
     for (int o = 16; o < 64; o <<= 1) join_pair(top, sum, __shfl_xor(top, o), __shfl_xor(sum, o));
     double mine = 0, counts = 0;
+    float away = 0.f;
+    if (r.taught) {
+        if (t < r.T) away = taught_loss(r, t, log_of_sum(top, sum), part, 4);
+#pragma unroll
+        for (int o = 16; o < 64; o <<= 1) away += __shfl_xor(away, o);
+        away *= kLn2 * r.temperature * r.temperature;
+    }
     if (t < r.T && part == 0) {
         const float lse = log_of_sum(top, sum);
         const int64_t y = target_of(r.target, r.wide, t);
         r.lse[t] = lse;
-        const float l = loss_of(r, t, y, lse);
+        const float l = !r.taught ? loss_of(r, t, y, lse) : y == r.ignore ? 0.f : y >= r.V ? NAN : away;
         r.loss[t] = l;
         mine = l, counts = y != r.ignore;
     }
@@ -271,6 +300,7 @@ struct Finish {
     float *bias_part;      // [workgroups along T][ld_bias_part], or NULL
     void *bias_out;        // one workgroup has all rows: the gradient itself, of V words, or NULL
     const float *factor[2];
+    const int *taught_ids; // TAUGHT: [T][words of a teacher], as Args has them
 };
 // 64 rows, or 8 where that would leave CUs without work.
 inline int finish_rows(int64_t T, int64_t words) { return (T + 63) / 64 * ((words + 255) / 256) >= 2 * device_cus() ? 64 : 8; }
@@ -290,7 +320,9 @@ __device__ __forceinline__ float lse_of_row(const Rows &r, int t, int lane)
 
 // JOIN: every workgroup joins its rows' sums for itself, and one more (the last along the rows) all of them, for the losses;
 // else they are in of.lse.
-template <typename P, bool JOIN>
+// TAUGHT: of the words that a teacher has for the row, those among the workgroup's 256 are found by the half wave that has the
+// row, 32 at a time, and each is handed to the lane that has its word.
+template <typename P, bool JOIN, bool TAUGHT = false>
 __global__ __launch_bounds__(256) void finish_kernel(Finish f)
 {
     typedef typename ElementOf<P>::type E;
@@ -338,12 +370,34 @@ __global__ __launch_bounds__(256) void finish_kernel(Finish f)
     const float2 *tops = r.stats + (int64_t)(f.tile0 + (word < f.words ? word / f.tile : 0)) * r.T;
     uint16_t *const column = (uint16_t *)f.prob + (NP == 1 ? word : (word >> 5) * 96 + (word & 31));
     const float *const kept = f.kept + (NP == 1 ? word : (word >> 5) * 48 + (word & 31));
-#pragma unroll JOIN ? 1 : 4
+#pragma unroll JOIN || TAUGHT ? 1 : 4
     for (int i = 0; i < f.rows; i += 8) {
         const int t = blockIdx.y * f.rows + i + part;
         if (t >= r.T) break;
         const int64_t y = target_of(r.target, r.wide, t);
         const float lse = JOIN ? lse_of_row(r, t, lane) : r.lse[t];
+        float taught[8];
+        if constexpr (TAUGHT) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) taught[e] = 0.f;
+            const int64_t row = (int64_t)t * r.words;
+            const int from = (int)f.v0 + blockIdx.x * 256, to = (int)f.v0 + min((int)f.n, (int)blockIdx.x * 256 + 256), half = threadIdx.x & 32;
+            for (int k = 0; k < r.words; k += 32) {
+                const int id = k + lane < r.words ? f.taught_ids[row + k + lane] : 0x7fffffff;
+                const bool inside = id >= from && id < to;
+                const float q = inside ? r.taught[row + k + lane] : 0.f;
+                uint32_t left = (uint32_t)(__ballot(inside) >> half);
+                while (__any(left != 0)) {
+                    const int of = half + (left ? __ffs(left) - 1 : 0);
+                    const int here = __shfl(id, of) - from - lane * 8;
+                    const float probability = __shfl(q, of);
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) taught[e] += left && here == e ? probability : 0.f;
+                    left &= left - 1;
+                }
+                if (__all(id >= to)) break;  // they are in ascending order
+            }
+        }
         if (word >= f.words) continue;
         Vec<uint16_t, 8> *const at = (Vec<uint16_t, 8> *)(column + t * f.ldp);
         Vec<uint16_t, 8> v[NP];
@@ -356,7 +410,10 @@ __global__ __launch_bounds__(256) void finish_kernel(Finish f)
 #pragma unroll
         for (int e = 0; e < 8; ++e) p[e] = y == r.ignore ? 0.f : e32[e / 4][e % 4] * factor;
         const int64_t here = y - f.v0 - word;
-        if (here >= 0 && here < 8 && word + here < f.n && y != r.ignore) {
+        if constexpr (TAUGHT) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) p[e] = y == r.ignore ? 0.f : p[e] - taught[e];
+        } else if (here >= 0 && here < 8 && word + here < f.n && y != r.ignore) {
             const float hot = exp2f(r.picked[t] - lse) - 1.f;
 #pragma unroll
             for (int e = 0; e < 8; ++e) p[e] = here == e ? hot : p[e];
@@ -394,6 +451,64 @@ __global__ __launch_bounds__(256) void finish_kernel(Finish f)
     for (int w = 0; w < 8; ++w) s += sums[w][threadIdx.x];
     if (f.bias_out) ((E *)f.bias_out)[v] = from_float<E>(s * factor_of(f.factor));
     else f.bias_part[(int64_t)blockIdx.y * f.ld_bias_part + v] = s;
+}
+
+// ---- a teacher's words -------------------------------------------------------------------------------------------------
+
+// What a teacher says of every token: its best words' numbers and logits, K of each.
+struct Teacher {
+    const void *ids;
+    int wide;
+    const void *logits;
+    int type, K;
+    int64_t T, V;
+    float temperature;
+    int *sorted;       // [T][K] numbers in ascending order, 0x7fffffff behind the last
+    float *taught;     // [T][K] their probabilities
+    int *target;       // [T] 0, -1 where there is no word, V where the probabilities are no numbers or a word is none
+    float *factor;     // the temperature
+};
+constexpr int kMostTaught = 1024;
+
+// Probabilities of a token's words, in the order of their numbers: a workgroup has a token, a thread a word, whose place is how
+// many come before it (the comparisons of 64 words take less time than their loads: 8192 tokens in 12 us).
+__global__ __launch_bounds__(kMostTaught) void teacher_kernel(Teacher f)
+{
+    __shared__ int ids[kMostTaught];
+    __shared__ float tops[16], sums[16];
+    __shared__ int found[16];
+    const int k = threadIdx.x, wave = k >> 6, lane = k & 63, waves = blockDim.x >> 6;
+    const int64_t t = blockIdx.x, at = t * f.K + k;
+    int id = 0x7fffffff, seen = 0;  // 1: a word, 2: something that is none, or no number
+    float logit = -INFINITY;
+    if (k < f.K) {
+        const int64_t word = f.wide ? ((const int64_t *)f.ids)[at] : (int64_t)((const int32_t *)f.ids)[at];
+        logit = f.type == DS_F32 ? ((const float *)f.logits)[at]
+                : f.type == DS_BF16 ? to_float(((const bf16_t *)f.logits)[at]) : to_float(((const f16_t *)f.logits)[at]);
+        if (word < 0 || logit == -INFINITY) logit = -INFINITY;
+        else if (word >= f.V || !(logit < INFINITY)) logit = -INFINITY, seen = 3;
+        else id = (int)word, seen = 1;
+    }
+    float top = logit;
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o)), seen |= __shfl_xor(seen, o);
+    ids[k] = id;
+    if (lane == 0) tops[wave] = top, found[wave] = seen;
+    __syncthreads();
+    for (int w = 0; w < waves; ++w) top = fmaxf(top, tops[w]), seen |= found[w];
+    const float warmth = kLog2e / f.temperature;
+    float e = id == 0x7fffffff ? 0.f : exp2f((logit - top) * warmth), sum = e;
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o);
+    if (lane == 0) sums[wave] = sum;
+    int place = 0;
+    for (int i = 0; i < f.K; ++i) place += ids[i] < id || (ids[i] == id && i < k);
+    __syncthreads();
+    sum = 0.f;
+    for (int w = 0; w < waves; ++w) sum += sums[w];
+    if (k < f.K) f.sorted[t * f.K + place] = id, f.taught[t * f.K + place] = id == 0x7fffffff ? 0.f : e / sum;
+    if (k == 0) f.target[t] = seen == 0 ? -1 : seen & 2 ? (int)f.V : 0;
+    if (k == 0 && t == 0) *f.factor = f.temperature;
 }
 
 // ---- joins -------------------------------------------------------------------------------------------------------
@@ -488,16 +603,17 @@ struct Plan {
     int words;            // of a piece's probabilities, a multiple of 32,
     int64_t ldp;          // and what a row of them takes
     size_t h, w, stats, picked, shares, arrived, prob, kept, bias, slices, acc, scale, power, factor, bytes;
+    size_t sorted, taught, target, temperature;  // a teacher's words
 };
 
 template <typename P>
-Plan plan_of(const void *hidden, int64_t ldh, const void *weight, int64_t ldw, int64_t T, int64_t D, int64_t V, int what)
+Plan plan_of(const void *hidden, int64_t ldh, const void *weight, int64_t ldw, int64_t T, int64_t D, int64_t V, int what, int words = 0)
 {
     constexpr size_t NP = P::planes;
     Plan p{};
     p.Dp = (int)(NP > 1 ? (D + 31) / 32 * 32 : (D + 7) / 8 * 8);
     p.ldd = row_elements<P>(D);
-    p.few = NP > 1 && T > 0 && T <= few_tokens(V * D) && g_tune.vocab_tile == kTuneUnset;
+    p.few = NP > 1 && !words && T > 0 && T <= few_tokens(V * D) && g_tune.vocab_tile == kTuneUnset;
     p.pack_h = !p.few && (NP > 1 || what & kGrad || !in_place(hidden, ldh, D));  // for gradients: without the rows that do not count
     if (NP > 1 && !p.few && T > 0 && g_tune.vocab_tile == kTuneUnset) {
         const int width = (uintptr_t)weight % 16 == 0 && ldw % 4 == 0 && D % 4 == 0 ? 4 : 1;
@@ -528,12 +644,16 @@ Plan plan_of(const void *hidden, int64_t ldh, const void *weight, int64_t ldw, i
         at = align_up(at + n, 256);
         return was;
     };
+    if (words) {
+        p.sorted = take((size_t)T * words * 4), p.taught = take((size_t)T * words * 4);
+        p.target = take((size_t)T * 4), p.temperature = take(4);
+    }
     if (p.pack_h) p.h = take((size_t)T * p.ldd * 2);
     if (p.pack_w) p.w = take((size_t)p.piece * p.ldd * 2);
     if (what & kLoss) {
         const int64_t tiles = (p.piece + p.tile_words - 1) / p.tile_words;
         p.stats = take((size_t)(tiles * p.pieces) * T * 8);
-        p.picked = take((size_t)T * 4);
+        p.picked = take((size_t)T * (words ? words : 1) * 4);
         p.shares = take((size_t)((T + kRowsJoined - 1) / kRowsJoined) * sizeof(Share));
         p.arrived = take(4);
     }
@@ -583,6 +703,7 @@ struct Call {
     char *ws;
     size_t ws_bytes;
     hipStream_t st;
+    Teacher teacher;   // K 0: none, target has the words
 };
 
 inline int check(const Call &c)
@@ -632,17 +753,27 @@ Args logit_args(const Call &c, const Plan &p, int64_t v0, int64_t n, const Opera
     g.bias = c.bias, g.bias_type = c.type;
     g.target = c.target, g.target_wide = c.wide;
     g.V = c.V, g.ignore = c.ignore, g.v0 = (int)v0;
+    g.taught_ids = c.teacher.sorted, g.taught = c.teacher.taught, g.taught_words = c.teacher.K;
+    g.warmth = c.teacher.K ? 1.f / c.teacher.temperature : 1.f;
     return g;
 }
 
 // Whether finish_kernel joins the rows' sums: each of its workgroups does it for its own rows, and one for all, which pays
 // while there are few of both (64 tokens, 1000 words, float32: 3 us of a step).
-inline bool joined_later(const Plan &p, int64_t T, int tiles) { return p.keep && p.pieces == 1 && T <= 128 && tiles <= 64; }
+inline bool joined_later(const Call &c, const Plan &p, int tiles)
+{
+    return p.keep && p.pieces == 1 && c.T <= 128 && tiles <= 64 && !c.teacher.K;
+}
 
 // One product, of `kind`, by the kernels of the plan; fills in the tile counts.
 template <typename P>
 int product(const Plan &p, int kind, int tile, Args &g, int64_t T, hipStream_t st)
 {
+    if (g.taught_words && kind <= kLogitProb) {
+        if constexpr (P::planes > 1)
+            if (p.raw) return launch_taught_raw(kind, p.raw, g, st);
+        return launch_taught<P>(kind, tile, g, st);
+    }
     if (p.raw && kind != kWeight) return launch_raw(kind, p.raw, g, st);
     return p.few ? launch_few(kind, (int)T, g, st) : launch_product<P>(kind, tile, g, nullptr, st);
 }
@@ -671,8 +802,9 @@ int loss(const Call &c, const Plan &p, bool counted_only, Operands<P> &o, int re
         tiles += g.tiles_m;
     }
     *of = Rows{(const float2 *)(c.ws + p.stats), (const float *)(c.ws + p.picked), tiles, (int)c.T, c.target, c.wide, c.V, c.ignore,
-               lse, rows, reduction, (Share *)(c.ws + p.shares), (uint32_t *)(c.ws + p.arrived), total};
-    if (!joined_later(p, c.T, tiles))
+               lse, rows, reduction, (Share *)(c.ws + p.shares), (uint32_t *)(c.ws + p.arrived), total, c.teacher.taught, c.teacher.K,
+               c.teacher.K ? c.teacher.temperature : 1.f};
+    if (!joined_later(c, p, tiles))
         hipLaunchKernelGGL(row_kernel, dim3((unsigned)((c.T + kRowsJoined - 1) / kRowsJoined)), dim3(1024), 0, c.st, *of);
     return launch_status();
 }
@@ -694,6 +826,8 @@ int loss_grad(const Call &c, const Plan &p, Operands<P> &o, const Rows &of, Grad
                            (float *)(c.ws + p.scale), (float *)(c.ws + p.factor), power);
         r.grad = (const float *)(c.ws + p.factor);
     }
+    // the temperature, where no row's share has it
+    if (c.teacher.K && c.T > 0 && !r.share) r.share = c.teacher.factor;
     float *const slices = (float *)(c.ws + p.slices);
     // the last piece first: its exponentials may be there, and its weights are
     for (int64_t i = 0; i < p.pieces; ++i) {
@@ -707,17 +841,19 @@ int loss_grad(const Call &c, const Plan &p, Operands<P> &o, const Rows &of, Grad
             const int rows = kept ? finish_rows(c.T, p.words) : p.tile_tokens;
             bias_tiles = (int)((c.T + rows - 1) / rows);
             // the sums of one workgroup are the gradient, but for the share that a launch which joins the rows only finds
-            bias_left = r.dbias && (bias_tiles > 1 || joined_later(p, c.T, of.tiles));
+            bias_left = r.dbias && (bias_tiles > 1 || joined_later(c, p, of.tiles));
             float *const bias_part = bias_left ? (float *)(c.ws + p.bias) : nullptr;
             void *const bias_out = r.dbias && !bias_left ? (E *)r.dbias + v0 : nullptr;
             if (kept) {
                 const int words = ceil_div((int)n, 32) * 32;
                 const bool beside = P::planes == 1;
                 const Finish f{c.ws + p.prob, p.ldp, (const float *)(c.ws + (beside ? p.kept : p.prob)), beside ? p.words : p.ldp / 2, words, p.tile_words, rows, v0, n, of.tiles - ceil_div((int)n, p.tile_words),
-                               p.words, of, bias_part, bias_out, {r.grad, r.share}};
+                               p.words, of, bias_part, bias_out, {r.grad, r.share}, c.teacher.sorted};
                 const unsigned along = ceil_div(words, 256), down = ceil_div((int)c.T, rows);
-                if (joined_later(p, c.T, of.tiles))
+                if (joined_later(c, p, of.tiles))
                     hipLaunchKernelGGL((finish_kernel<P, true>), dim3(along, down + 1), dim3(256), 0, c.st, f);
+                else if (c.teacher.K)
+                    hipLaunchKernelGGL((finish_kernel<P, false, true>), dim3(along, down), dim3(256), 0, c.st, f);
                 else
                     hipLaunchKernelGGL((finish_kernel<P, false>), dim3(along, down), dim3(256), 0, c.st, f);
             } else {
@@ -803,10 +939,18 @@ struct Outputs {
 };
 
 template <typename P>
-int run(const Call &c, int what, const Outputs &out)
+int run(Call c, int what, const Outputs &out)
 {
-    const Plan p = plan_of<P>(c.hidden, c.ldh, c.weight, c.ldw, c.T, c.D, c.V, what);
+    const Plan p = plan_of<P>(c.hidden, c.ldh, c.weight, c.ldw, c.T, c.D, c.V, what, c.teacher.K);
     if (!c.ws || c.ws_bytes < p.bytes || (uintptr_t)c.ws % 256) return DS_EWORKSPACE;
+    if (c.teacher.K) {
+        Teacher &t = c.teacher;
+        t.sorted = (int *)(c.ws + p.sorted), t.taught = (float *)(c.ws + p.taught);
+        t.target = (int *)(c.ws + p.target), t.factor = (float *)(c.ws + p.temperature);
+        // from here on tokens without a word are those that do not count
+        c.target = t.target, c.wide = 0, c.ignore = -1;
+        if (c.T > 0) hipLaunchKernelGGL(teacher_kernel, dim3((unsigned)c.T), dim3(ceil_div(t.K, 64) * 64), 0, c.st, t);
+    }
     Operands<P> o;
     Rows of{};
     if (what & kLoss) DS_TRY(loss<P>(c, p, what & kGrad, o, out.reduction, out.rows, out.lse, out.total, &of));
@@ -828,6 +972,67 @@ int run(const Call &c, int what, const Outputs &out)
 using namespace ds;
 using namespace ds::vocab;
 
+DS_EXPORT size_t ds_distill_workspace_bytes(const void *hidden, int64_t ldh, const void *weight, int64_t ldw, int64_t T, int64_t D,
+                                            int64_t V, int type, int words, int what)
+{
+    if (T < 0 || D < 0 || V < 1 || !element_bytes(type) || words < 1 || words > kMostTaught || what < kLoss || what > (kLoss | kGrad))
+        return 0;
+    if (type == DS_F32) return plan_of<Split>(hidden, ldh, weight, ldw, T, D, V, what, words).bytes;
+    if (type == DS_BF16) return plan_of<Bf16>(hidden, ldh, weight, ldw, T, D, V, what, words).bytes;
+    return plan_of<F16>(hidden, ldh, weight, ldw, T, D, V, what, words).bytes;
+}
+
+// `what` and where its results go, of a teacher's words.
+static int run_taught(const Teacher &teacher, int id_bytes, Call c, int what, const Outputs &out)
+{
+    if (id_bytes != 4 && id_bytes != 8) return DS_EINVAL;
+    if (teacher.K < 1 || teacher.K > kMostTaught || !element_bytes(teacher.type)) return DS_EINVAL;
+    if (!(teacher.temperature >= 0x1p-20f && teacher.temperature <= 0x1p20f)) return DS_EINVAL;
+    if (c.T > 0 && (!teacher.ids || !teacher.logits)) return DS_EINVAL;
+    if (c.T > 0xffffffff / (ceil_div(teacher.K, 64) * 64)) return DS_ETOOLARGE;  // threads of teacher_kernel
+    c.teacher = teacher;
+    c.target = teacher.ids;
+    return run(c, what, out);
+}
+
+DS_EXPORT int ds_distill_loss(const void *hidden, int64_t ldh, const void *weight, int64_t ldw, const void *bias, const void *ids,
+                              int id_bytes, const void *logits, int logits_type, int words, float temperature, int64_t T, int64_t D,
+                              int64_t V, int type, int reduction, float *rows, float *lse, float *total, void *workspace,
+                              size_t workspace_bytes, ds_stream_t stream)
+{
+    if (reduction < 0 || reduction > DS_MEAN || (T > 0 && (!rows || !lse)) || (reduction && !total)) return DS_EINVAL;
+    const Teacher teacher{ids, id_bytes == 8, logits, logits_type, words, T, V, temperature, nullptr, nullptr, nullptr, nullptr};
+    return run_taught(teacher, id_bytes, Call{hidden, weight, bias, nullptr, ldh, ldw, T, D, V, -1, 0, type, (char *)workspace,
+                                              workspace_bytes, (hipStream_t)stream, Teacher{}},
+                      kLoss, Outputs{reduction, rows, lse, total, Grads{}});
+}
+
+DS_EXPORT int ds_distill_loss_grad(const void *hidden, int64_t ldh, const void *weight, int64_t ldw, const void *bias, const void *ids,
+                                   int id_bytes, const void *logits, int logits_type, int words, float temperature, int64_t T,
+                                   int64_t D, int64_t V, int type, const float *lse, const float *row_grad, const float *grad,
+                                   const float *share, void *dhidden, void *dweight, void *dbias, void *workspace,
+                                   size_t workspace_bytes, ds_stream_t stream)
+{
+    if ((row_grad && (grad || share)) || (T > 0 && !lse)) return DS_EINVAL;
+    const Teacher teacher{ids, id_bytes == 8, logits, logits_type, words, T, V, temperature, nullptr, nullptr, nullptr, nullptr};
+    return run_taught(teacher, id_bytes, Call{hidden, weight, bias, nullptr, ldh, ldw, T, D, V, -1, 0, type, (char *)workspace,
+                                              workspace_bytes, (hipStream_t)stream, Teacher{}},
+                      kGrad, Outputs{0, nullptr, nullptr, nullptr, Grads{lse, row_grad, grad, share, dhidden, dweight, dbias}});
+}
+
+DS_EXPORT int ds_distill_loss_step(const void *hidden, int64_t ldh, const void *weight, int64_t ldw, const void *bias, const void *ids,
+                                   int id_bytes, const void *logits, int logits_type, int words, float temperature, int64_t T,
+                                   int64_t D, int64_t V, int type, int reduction, float *rows, float *lse, float *total, void *dhidden,
+                                   void *dweight, void *dbias, void *workspace, size_t workspace_bytes, ds_stream_t stream)
+{
+    if (reduction < 0 || reduction > DS_MEAN || (T > 0 && (!rows || !lse)) || (reduction && !total)) return DS_EINVAL;
+    const Teacher teacher{ids, id_bytes == 8, logits, logits_type, words, T, V, temperature, nullptr, nullptr, nullptr, nullptr};
+    return run_taught(teacher, id_bytes, Call{hidden, weight, bias, nullptr, ldh, ldw, T, D, V, -1, 0, type, (char *)workspace,
+                                              workspace_bytes, (hipStream_t)stream, Teacher{}},
+                      kLoss | kGrad, Outputs{reduction, rows, lse, total,
+                                             Grads{lse, nullptr, nullptr, reduction ? total + 1 : nullptr, dhidden, dweight, dbias}});
+}
+
 DS_EXPORT size_t ds_vocab_workspace_bytes(const void *hidden, int64_t ldh, const void *weight, int64_t ldw, int64_t T, int64_t D,
                                           int64_t V, int type, int what)
 {
@@ -845,7 +1050,7 @@ DS_EXPORT int ds_vocab_loss(const void *hidden, int64_t ldh, const void *weight,
     if ((target_bytes != 4 && target_bytes != 8) || reduction < 0 || reduction > DS_MEAN) return DS_EINVAL;
     if ((T > 0 && (!rows || !lse)) || (reduction && !total)) return DS_EINVAL;
     return run(Call{hidden, weight, bias, target, ldh, ldw, T, D, V, ignore, target_bytes == 8, type, (char *)workspace,
-                    workspace_bytes, (hipStream_t)stream},
+                    workspace_bytes, (hipStream_t)stream, Teacher{}},
                kLoss, Outputs{reduction, rows, lse, total, Grads{}});
 }
 
@@ -856,7 +1061,7 @@ DS_EXPORT int ds_vocab_loss_grad(const void *hidden, int64_t ldh, const void *we
 {
     if ((target_bytes != 4 && target_bytes != 8) || (row_grad && (grad || share)) || (T > 0 && !lse)) return DS_EINVAL;
     return run(Call{hidden, weight, bias, target, ldh, ldw, T, D, V, ignore, target_bytes == 8, type, (char *)workspace,
-                    workspace_bytes, (hipStream_t)stream},
+                    workspace_bytes, (hipStream_t)stream, Teacher{}},
                kGrad, Outputs{0, nullptr, nullptr, nullptr, Grads{lse, row_grad, grad, share, dhidden, dweight, dbias}});
 }
 
@@ -868,7 +1073,7 @@ DS_EXPORT int ds_vocab_loss_step(const void *hidden, int64_t ldh, const void *we
     if ((target_bytes != 4 && target_bytes != 8) || reduction < 0 || reduction > DS_MEAN) return DS_EINVAL;
     if ((T > 0 && (!rows || !lse)) || (reduction && !total)) return DS_EINVAL;
     return run(Call{hidden, weight, bias, target, ldh, ldw, T, D, V, ignore, target_bytes == 8, type, (char *)workspace,
-                    workspace_bytes, (hipStream_t)stream},
+                    workspace_bytes, (hipStream_t)stream, Teacher{}},
                kLoss | kGrad, Outputs{reduction, rows, lse, total,
                                       Grads{lse, nullptr, nullptr, reduction ? total + 1 : nullptr, dhidden, dweight, dbias}});
 }

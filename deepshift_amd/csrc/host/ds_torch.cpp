@@ -181,16 +181,15 @@ PyObject *embed_grad(PyObject *, PyObject *const *args, Py_ssize_t count)
     });
 }
 
-// The operands of a head's cross entropy: hidden [..., D], weight [V, D], target [...], bias [V] or None.
-struct Head {
-    at::Tensor hidden, weight, target, bias;
+// A linear head: hidden [..., D], weight [V, D], bias [V] or None.
+struct LinearHead {
+    at::Tensor hidden, weight, bias;
     std::vector<int64_t> shape;  // of hidden
-    int64_t ldh, ldw, T, D, V, ignore;
+    int64_t ldh, ldw, T, D, V;
     int type;
 
-    explicit Head(PyObject *const *args) : hidden(tensor("hidden", args[0])), weight(tensor("weight", args[1]))
+    LinearHead(PyObject *hidden_, PyObject *weight_) : hidden(tensor("hidden", hidden_)), weight(tensor("weight", weight_))
     {
-        constexpr int64_t kLongestRow = 2000000;  // elements between rows that the products' 32-bit offsets reach
         type = checked_type("hidden", hidden);
         if (hidden.dim() < 1) refuse(PyExc_ValueError, "hidden must have the features as its last axis, is ", hidden.sizes());
         shape = hidden.sizes().vec();
@@ -200,18 +199,20 @@ struct Head {
         V = weight.size(0);
         if (V < 1) refuse(PyExc_ValueError, "weight must have at least one row");
         alike("weight", weight);
-        target = tokens("target", args[2], hidden.device());
-        if (target.sizes() != hidden.sizes().slice(0, shape.size() - 1))
-            refuse(PyExc_ValueError, "target must be ", hidden.sizes().slice(0, shape.size() - 1), ", is ", target.sizes());
-        if (args[3] != Py_None) {
-            bias = tensor("bias", args[3]);
+    }
+    at::IntArrayRef tokens_of() const { return at::IntArrayRef(shape).slice(0, shape.size() - 1); }
+    // the bias, and rows of the operands, of T tokens
+    void settle(PyObject *bias_, int64_t tokens)
+    {
+        constexpr int64_t kLongestRow = 2000000;  // elements between rows that the products' 32-bit offsets reach
+        if (bias_ != Py_None) {
+            bias = tensor("bias", bias_);
             alike("bias", bias);
             if (bias.dim() != 1 || bias.size(0) != V)
                 refuse(PyExc_ValueError, "bias must be [", std::to_string(V), "], is ", bias.sizes());
             bias = bias.contiguous();
         }
-        ignore = integer(args[4]);
-        T = target.numel();
+        T = tokens;
         if (hidden.dim() != 2) hidden = hidden.reshape({T, D});
         ldh = rows(hidden, kLongestRow);
         ldw = rows(weight, kLongestRow);
@@ -229,6 +230,21 @@ struct Head {
         return at::empty(sizes, at::TensorOptions().device(hidden.device()).dtype(as));
     }
     at::Tensor empty(at::IntArrayRef sizes) const { return empty(sizes, hidden.scalar_type()); }
+    const void *bias_at() const { return bias.defined() ? bias.const_data_ptr() : nullptr; }
+};
+
+// The operands of a head's cross entropy: target [...], and the number that does not count.
+struct Head : LinearHead {
+    at::Tensor target;
+    int64_t ignore;
+
+    explicit Head(PyObject *const *args) : LinearHead(args[0], args[1])
+    {
+        target = tokens("target", args[2], hidden.device());
+        if (target.sizes() != tokens_of()) refuse(PyExc_ValueError, "target must be ", tokens_of(), ", is ", target.sizes());
+        settle(args[3], target.numel());
+        ignore = integer(args[4]);
+    }
 
     // loss 1, gradients 2, both 3
     at::Tensor workspace(int what) const
@@ -237,7 +253,42 @@ struct Head {
             ds_vocab_workspace_bytes(hidden.const_data_ptr(), ldh, weight.const_data_ptr(), ldw, T, D, V, type, what);
         return empty({(int64_t)bytes}, at::kByte);
     }
-    const void *bias_at() const { return bias.defined() ? bias.const_data_ptr() : nullptr; }
+};
+
+// The operands of a head's distillation: a teacher's ids and logits [..., K], and the temperature.
+struct Pupil : LinearHead {
+    at::Tensor ids, logits;
+    int64_t K;
+    int logits_type;
+    float temperature;
+
+    explicit Pupil(PyObject *const *args) : LinearHead(args[0], args[1])
+    {
+        ids = tokens("teacher_ids", args[2], hidden.device());
+        if (ids.dim() < 1 || ids.sizes().slice(0, ids.dim() - 1) != tokens_of())
+            refuse(PyExc_ValueError, "teacher_ids must be ", tokens_of(), " and one more axis, is ", ids.sizes());
+        K = ids.size(-1);
+        if (K < 1 || K > 1024) refuse(PyExc_ValueError, "a teacher must have 1 to 1024 words for a token, has ", std::to_string(K));
+        logits = tensor("teacher_logits", args[3]);
+        logits_type = type_code(logits);
+        if (logits_type < 0)
+            refuse(PyExc_TypeError, "teacher_logits must be float32, bfloat16 or float16, is ", c10::toString(logits.scalar_type()));
+        if (logits.device() != hidden.device())
+            refuse(PyExc_ValueError, "teacher_logits must be on ", hidden.device().str(), ", is on ", logits.device().str());
+        if (logits.sizes() != ids.sizes())
+            refuse(PyExc_ValueError, "teacher_logits must be ", ids.sizes(), " like teacher_ids, is ", logits.sizes());
+        logits = logits.contiguous();
+        int64_t tokens = 1;
+        for (int64_t n : tokens_of()) tokens *= n;
+        settle(args[4], tokens);
+        temperature = (float)number(args[5]);
+    }
+    at::Tensor workspace(int what) const
+    {
+        return empty({(int64_t)ds_distill_workspace_bytes(hidden.const_data_ptr(), ldh, weight.const_data_ptr(), ldw, T, D, V, type,
+                                                          (int)K, what)},
+                     at::kByte);
+    }
 };
 
 template <typename E = void> E *at_or_null(const at::Tensor &t) { return t.defined() ? (E *)t.mutable_data_ptr() : nullptr; }
@@ -266,9 +317,9 @@ struct Losses {
     int reduction;
     at::Tensor rows, lse, total;
 
-    Losses(const Head &h, PyObject *red) : reduction((int)integer(red))
+    Losses(const LinearHead &h, PyObject *red) : reduction((int)integer(red))
     {
-        rows = h.empty(h.target.sizes(), at::kFloat);
+        rows = h.empty(h.tokens_of(), at::kFloat);
         lse = h.empty({h.T}, at::kFloat);
         if (reduction) total = h.empty({2}, at::kFloat);
     }
@@ -293,6 +344,14 @@ PyObject *cross_entropy(PyObject *, PyObject *const *args, Py_ssize_t count)
     });
 }
 
+void check_losses(const LinearHead &h, const at::Tensor &lse, const at::Tensor &grad, const at::Tensor &share)
+{
+    for (const at::Tensor *t : {&lse, &grad, &share})
+        if (t->defined() && (t->scalar_type() != at::kFloat || !t->is_contiguous() || t->device() != h.hidden.device() ||
+                             t->numel() != (t == &lse || (t == &grad && !share.defined()) ? h.T : 1)))
+            refuse(PyExc_ValueError, "lse, share and grad must be float32 and fit the tokens");
+}
+
 // cross_entropy_grad(hidden, weight, target, bias or None, ignore, lse, share or None, grad, wanted, stream): gradients of
 // hidden, weight and bias for `grad`, of the loss or (where there is no share) of the rows; bits 0 to 2 of `wanted` say which
 PyObject *cross_entropy_grad(PyObject *, PyObject *const *args, Py_ssize_t count)
@@ -301,10 +360,7 @@ PyObject *cross_entropy_grad(PyObject *, PyObject *const *args, Py_ssize_t count
         const Head h(args);
         const at::Tensor &lse = tensor("lse", args[5]), &grad = tensor("grad", args[7]);
         const at::Tensor share = args[6] == Py_None ? at::Tensor() : tensor("share", args[6]);
-        for (const at::Tensor *t : {&lse, &grad, &share})
-            if (t->defined() && (t->scalar_type() != at::kFloat || !t->is_contiguous() || t->device() != h.hidden.device() ||
-                                 t->numel() != (t == &lse || (t == &grad && !share.defined()) ? h.T : 1)))
-                refuse(PyExc_ValueError, "lse, share and grad must be float32 and fit the tokens");
+        check_losses(h, lse, grad, share);
         const int64_t wanted = integer(args[8]);
         at::Tensor dhidden, dweight, dbias;
         if (wanted & 1) dhidden = h.empty(h.shape);
@@ -338,6 +394,69 @@ PyObject *cross_entropy_step(PyObject *, PyObject *const *args, Py_ssize_t count
                                   l.reduction, at_or_null<float>(l.rows), at_or_null<float>(l.lse), at_or_null<float>(l.total),
                                   at_or_null(dhidden), at_or_null(dweight), at_or_null(dbias), ws.mutable_data_ptr(), ws.nbytes(),
                                   stream(args[6])));
+        return tuple_of({l.result(), dhidden, dweight, dbias});
+    });
+}
+
+// distill(hidden, weight, teacher_ids, teacher_logits, bias or None, temperature, reduction, stream): as cross_entropy
+PyObject *distill(PyObject *, PyObject *const *args, Py_ssize_t count)
+{
+    return guarded(count, 8, [&] {
+        const Pupil h(args);
+        const Losses l(h, args[6]);
+        const at::Tensor ws = h.workspace(1);
+        expect("ds_distill_loss",
+               ds_distill_loss(h.hidden.const_data_ptr(), h.ldh, h.weight.const_data_ptr(), h.ldw, h.bias_at(),
+                               h.ids.const_data_ptr(), (int)h.ids.element_size(), h.logits.const_data_ptr(), h.logits_type, (int)h.K,
+                               h.temperature, h.T, h.D, h.V, h.type, l.reduction, at_or_null<float>(l.rows),
+                               at_or_null<float>(l.lse), at_or_null<float>(l.total), ws.mutable_data_ptr(), ws.nbytes(),
+                               stream(args[7])));
+        return tuple_of({l.result(), l.lse, l.share()});
+    });
+}
+
+// distill_grad(hidden, weight, teacher_ids, teacher_logits, bias or None, temperature, lse, share or None, grad, wanted, stream): as
+// cross_entropy_grad
+PyObject *distill_grad(PyObject *, PyObject *const *args, Py_ssize_t count)
+{
+    return guarded(count, 11, [&] {
+        const Pupil h(args);
+        const at::Tensor &lse = tensor("lse", args[6]), &grad = tensor("grad", args[8]);
+        const at::Tensor share = args[7] == Py_None ? at::Tensor() : tensor("share", args[7]);
+        check_losses(h, lse, grad, share);
+        const int64_t wanted = integer(args[9]);
+        at::Tensor dhidden, dweight, dbias;
+        if (wanted & 1) dhidden = h.empty(h.shape);
+        if (wanted & 2) dweight = h.empty({h.V, h.D});
+        if (wanted & 4 && h.bias.defined()) dbias = h.empty({h.V});
+        const at::Tensor ws = h.workspace(2);
+        const float *g = (const float *)grad.const_data_ptr();
+        expect("ds_distill_loss_grad",
+               ds_distill_loss_grad(h.hidden.const_data_ptr(), h.ldh, h.weight.const_data_ptr(), h.ldw, h.bias_at(),
+                                    h.ids.const_data_ptr(), (int)h.ids.element_size(), h.logits.const_data_ptr(), h.logits_type,
+                                    (int)h.K, h.temperature, h.T, h.D, h.V, h.type, (const float *)lse.const_data_ptr(),
+                                    share.defined() ? nullptr : g, share.defined() ? g : nullptr,
+                                    share.defined() ? (const float *)share.const_data_ptr() : nullptr, at_or_null(dhidden),
+                                    at_or_null(dweight), at_or_null(dbias), ws.mutable_data_ptr(), ws.nbytes(), stream(args[10])));
+        return tuple_of({dhidden, dweight, dbias});
+    });
+}
+
+// distill_step(hidden, weight, teacher_ids, teacher_logits, bias or None, temperature, reduction, stream): as cross_entropy_step
+PyObject *distill_step(PyObject *, PyObject *const *args, Py_ssize_t count)
+{
+    return guarded(count, 8, [&] {
+        const Pupil h(args);
+        const Losses l(h, args[6]);
+        const at::Tensor dhidden = h.empty(h.shape), dweight = h.empty({h.V, h.D});
+        const at::Tensor dbias = h.bias.defined() ? h.empty({h.V}) : at::Tensor();
+        const at::Tensor ws = h.workspace(3);
+        expect("ds_distill_loss_step",
+               ds_distill_loss_step(h.hidden.const_data_ptr(), h.ldh, h.weight.const_data_ptr(), h.ldw, h.bias_at(),
+                                    h.ids.const_data_ptr(), (int)h.ids.element_size(), h.logits.const_data_ptr(), h.logits_type,
+                                    (int)h.K, h.temperature, h.T, h.D, h.V, h.type, l.reduction, at_or_null<float>(l.rows),
+                                    at_or_null<float>(l.lse), at_or_null<float>(l.total), at_or_null(dhidden), at_or_null(dweight),
+                                    at_or_null(dbias), ws.mutable_data_ptr(), ws.nbytes(), stream(args[7])));
         return tuple_of({l.result(), dhidden, dweight, dbias});
     });
 }
@@ -647,6 +766,13 @@ PyMethodDef methods[] = {
      "cross_entropy_grad(hidden, weight, target, bias or None, ignore, lse, share or None, grad, wanted, stream) -> gradients"},
     {"cross_entropy_step", (PyCFunction)(void (*)(void))cross_entropy_step, METH_FASTCALL,
      "cross_entropy_step(hidden, weight, target, bias or None, ignore, reduction, stream) -> loss, gradients"},
+    {"distill", (PyCFunction)(void (*)(void))distill, METH_FASTCALL,
+     "distill(hidden, weight, teacher_ids, teacher_logits, bias or None, temperature, reduction, stream) -> loss, lse, share or None"},
+    {"distill_grad", (PyCFunction)(void (*)(void))distill_grad, METH_FASTCALL,
+     "distill_grad(hidden, weight, teacher_ids, teacher_logits, bias or None, temperature, lse, share or None, grad, wanted, stream) "
+     "-> gradients"},
+    {"distill_step", (PyCFunction)(void (*)(void))distill_step, METH_FASTCALL,
+     "distill_step(hidden, weight, teacher_ids, teacher_logits, bias or None, temperature, reduction, stream) -> loss, gradients"},
     {"recurrence", (PyCFunction)(void (*)(void))recurrence, METH_FASTCALL,
      "recurrence(x, gate, state or None, lengths or None, keep, stream) -> states, last ones, kept ones or None"},
     {"recurrence_grad", (PyCFunction)(void (*)(void))recurrence_grad, METH_FASTCALL,

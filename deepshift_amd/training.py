@@ -18,8 +18,9 @@ from torch.autograd.function import once_differentiable
 
 from . import _lib, modules, modules_q
 
-__all__ = ["embedding", "embedding_grad", "linear_cross_entropy", "linear_cross_entropy_grad", "gated_linear", "gated_recurrence",
-           "gradient_norm", "clip_gradients_", "clip_grad_norm_", "ScaledEmbedding", "LinearCrossEntropy", "GatedLinear", "GatedShift"]
+__all__ = ["embedding", "embedding_grad", "linear_cross_entropy", "linear_cross_entropy_grad", "linear_distillation",
+           "linear_distillation_grad", "gated_linear", "gated_recurrence", "gradient_norm", "clip_gradients_", "clip_grad_norm_",
+           "ScaledEmbedding", "LinearCrossEntropy", "GatedLinear", "GatedShift"]
 
 _REDUCTIONS = {"none": _lib.DS_NONE, "sum": _lib.DS_SUM, "mean": _lib.DS_MEAN}
 
@@ -209,6 +210,70 @@ def gated_recurrence(x, gate, state=None, lengths=None):
     if torch.is_grad_enabled() and (x.requires_grad or gate.requires_grad or (state is not None and state.requires_grad)):
         return _GatedRecurrence.apply(x, gate, state, lengths)
     return _recur(x, gate, state, lengths, False)[:2]
+
+
+# ---------------------------------------------------------------------------------------------
+# distillation of a linear head
+# ---------------------------------------------------------------------------------------------
+
+def _warmth(temperature, reduction):
+    """``temperature`` and ``reduction`` as the library takes them."""
+    if reduction not in _REDUCTIONS:
+        raise ValueError("reduction must be 'none', 'sum' or 'mean', is %r" % (reduction,))
+    temperature = float(temperature)
+    if not 2.0 ** -20 <= temperature <= 2.0 ** 20:
+        raise ValueError("temperature must be from 2^-20 to 2^20, is %r" % temperature)
+    return temperature, _REDUCTIONS[reduction]
+
+
+class _LinearDistillation(Function):
+    @staticmethod
+    def forward(ctx, hidden, weight, ids, logits, bias, temperature, reduction):
+        device = hidden.device
+        with _on(device):
+            loss, lse, share = _lib.native().distill(hidden, weight, ids, logits, bias, temperature, reduction, _stream_of(device))
+        ctx.save_for_backward(hidden, weight, ids, logits, bias, lse, share)
+        ctx.temperature = temperature
+        return loss
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad):
+        hidden, weight, ids, logits, bias, lse, share = ctx.saved_tensors
+        device, needed = hidden.device, ctx.needs_input_grad
+        with _on(device):
+            dhidden, dweight, dbias = _lib.native().distill_grad(
+                hidden, weight, ids, logits, bias, ctx.temperature, lse, share, grad.float().contiguous(),
+                needed[0] | needed[1] << 1 | needed[4] << 2, _stream_of(device))
+        return dhidden, dweight, None, None, dbias, None, None
+
+
+def linear_distillation(hidden, weight, teacher_ids, teacher_logits, bias=None, temperature=1.0, reduction="mean"):
+    """How far ``softmax((hidden @ weight.T + bias) / temperature)`` is from a teacher that is known by its best words, without ever
+    storing the logits: ``temperature ** 2`` times the Kullback-Leibler divergence of ``q``, the softmax of
+    ``teacher_logits / temperature`` over those words.
+
+    ``hidden`` ``[..., D]``, ``weight`` ``[V, D]`` and ``bias`` ``[V]`` are of one type; ``teacher_ids`` ``[..., K]`` (int64 or int32)
+    and ``teacher_logits`` ``[..., K]`` (float32, bfloat16 or float16) name 1 to 1024 words for every token, in any order; they get no
+    gradient.  A place with a negative number or a logit of ``-inf`` holds none, and a word in two places has both shares.  The
+    loss is float32: per token with ``reduction='none'``, else their sum, or their mean over the tokens that have a word; tokens
+    without one have loss 0 and leave nothing in any gradient.  A number of ``V`` or more, or a logit that is NaN or ``inf``, gives
+    NaN."""
+    temperature, reduction = _warmth(temperature, reduction)
+    if torch.is_grad_enabled() and (hidden.requires_grad or weight.requires_grad or (bias is not None and bias.requires_grad)):
+        return _LinearDistillation.apply(hidden, weight, teacher_ids, teacher_logits.detach(), bias, temperature, reduction)
+    device = hidden.device
+    with _on(device):
+        return _lib.native().distill(hidden, weight, teacher_ids, teacher_logits, bias, temperature, reduction, _stream_of(device))[0]
+
+
+def linear_distillation_grad(hidden, weight, teacher_ids, teacher_logits, bias=None, temperature=1.0, reduction="mean"):
+    """``(loss, dhidden, dweight, dbias)`` of :func:`linear_distillation` for a gradient of 1 (of ones, with
+    ``reduction='none'``), without autograd; ``dbias`` is ``None`` where there is no bias."""
+    temperature, reduction = _warmth(temperature, reduction)
+    device = hidden.device
+    with _on(device):
+        return _lib.native().distill_step(hidden, weight, teacher_ids, teacher_logits, bias, temperature, reduction, _stream_of(device))
 
 
 # ---------------------------------------------------------------------------------------------
@@ -425,6 +490,10 @@ class LinearCrossEntropy(nn.Module):
 
     def forward(self, hidden, target):
         return linear_cross_entropy(hidden, self.weight, target, self.bias, self.ignore_index, self.reduction)
+
+    def distill(self, hidden, teacher_ids, teacher_logits, temperature=1.0):
+        """:func:`linear_distillation` of this head, reduced as its loss is."""
+        return linear_distillation(hidden, self.weight, teacher_ids, teacher_logits, self.bias, temperature, self.reduction)
 
     def logits(self, hidden):
         return nn.functional.linear(hidden, self.weight, self.bias)

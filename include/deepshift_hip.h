@@ -567,6 +567,30 @@ int ds_vocab_loss_step(const void *hidden, int64_t ldh, const void *weight, int6
                        float *lse, float *total, void *dhidden, void *dweight, void *dbias, void *workspace,
                        size_t workspace_bytes, ds_stream_t stream);
 
+/* Distillation of a linear head from a teacher's best words: with p = softmax((hidden weight^T + bias) / temperature) and q the
+ * softmax of logits[t][:] / temperature over the words ids[t][:] (K = `words` of each token, 1 to 1024, in any order, a word's
+ * share being the sum of its places'),
+ *   rows[t] = temperature^2 sum_k q_k (log q_k - log p_k).
+ * A place with a negative number or a logit of -inf holds no word; a token without words does not count: its loss is 0 and it
+ * leaves nothing in the gradients.  A number of V or more, or a logit that is NaN or +inf, makes the token's loss and gradients NaN.
+ * ids are int32 or int64 (id_bytes 4 or 8), logits of type logits_type, temperature from 2^-20 to 2^20; everything else as
+ * ds_vocab_loss and its gradients have it, but that total[1] is a row's share times the temperature.  The workspace takes
+ * ds_distill_workspace_bytes(). */
+size_t ds_distill_workspace_bytes(const void *hidden, int64_t ldh, const void *weight, int64_t ldw, int64_t T, int64_t D, int64_t V,
+                                  int type, int words, int what);
+int ds_distill_loss(const void *hidden, int64_t ldh, const void *weight, int64_t ldw, const void *bias, const void *ids, int id_bytes,
+                    const void *logits, int logits_type, int words, float temperature, int64_t T, int64_t D, int64_t V, int type,
+                    int reduction, float *rows, float *lse, float *total, void *workspace, size_t workspace_bytes,
+                    ds_stream_t stream);
+int ds_distill_loss_grad(const void *hidden, int64_t ldh, const void *weight, int64_t ldw, const void *bias, const void *ids,
+                         int id_bytes, const void *logits, int logits_type, int words, float temperature, int64_t T, int64_t D,
+                         int64_t V, int type, const float *lse, const float *row_grad, const float *grad, const float *share,
+                         void *dhidden, void *dweight, void *dbias, void *workspace, size_t workspace_bytes, ds_stream_t stream);
+int ds_distill_loss_step(const void *hidden, int64_t ldh, const void *weight, int64_t ldw, const void *bias, const void *ids,
+                         int id_bytes, const void *logits, int logits_type, int words, float temperature, int64_t T, int64_t D,
+                         int64_t V, int type, int reduction, float *rows, float *lse, float *total, void *dhidden, void *dweight,
+                         void *dbias, void *workspace, size_t workspace_bytes, ds_stream_t stream);
+
 /* Gated block of a feed-forward layer: out[t][f] = act(x[t] . weight[f] + bias[f]) * (x[t] . weight[F + f] + bias[F + f]), x [T][D],
  * weight [2 F][D], bias [2 F] or NULL, out [T][F], all of `type`.  halves, or NULL, is [T][2][F rounded up to a multiple of 8] and
  * gets both products, which ds_gated_backward takes.  workspace: 256-byte aligned, ds_gated_workspace_bytes(..., what) bytes with
