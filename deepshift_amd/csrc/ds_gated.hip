@@ -3,8 +3,8 @@
 //   g = x Wg^T + bg      u = x Wu^T + bu      y = act(g) u                W = [Wg; Wu], 2 F rows
 //   dz = [dy u act'(g), dy act(g)]            dx = dz W      dW = dz^T x      db = sum_t dz[t]
 //
-// One product with both halves forms y in its epilogue; for gradients it leaves g and u too, in the operands' type, each rounded
-// once from 32 bits (in the gradients they meet dz, which is rounded to that type for its products anyway).  Going back, one pass
+// One product with both halves forms y in its epilogue; for gradients it leaves g and u too, in 32 bits (rounded to bfloat16 they
+// moved dx and dW by as much again as the rounding of dz, which its products need, and of the results).  Going back, one pass
 // makes dz of them, in the layout that the products of the vocabulary's cross entropy take, whose two gradient products do the
 // rest: 4 T D F operations forward and 8 T D F back, as the formulas have them.
 #include "ds_gated.h"
@@ -28,7 +28,7 @@ __device__ __forceinline__ void slope_of(int kind, float g, float &act, float &s
 }
 
 struct Back {
-    const void *halves;   // [T][2][ldz]
+    const float *halves;  // [T][2][ldz]
     const void *grad;     // [T] rows of ldg
     int64_t ldz, ldg, T;
     int F, activation;
@@ -39,7 +39,8 @@ struct Back {
     float *bias_part;     // [workgroups along T][2 F], or NULL
     // float16: dz is held times a power of two that brings the largest to the upper end of its range (loss gradients are small:
     // those below 2^-14 would lose bits, those below 2^-24 everything)
-    uint32_t *top;        // the largest finite |dz|
+    float *tops;          // the largest finite |dz| of each workgroup of top_kernel, `top_groups` of them
+    int top_groups;
     float *factor;        // what the results are multiplied with, but for kProbScale
 };
 
@@ -48,8 +49,8 @@ template <typename E>
 __device__ __forceinline__ void gradients_of(const Back &f, int64_t t, int c, float (&dg)[8], float (&du)[8])
 {
     constexpr int N = 16 / sizeof(E);
-    const Vec<E, 8> g = *(const Vec<E, 8> *)((const E *)f.halves + t * 2 * f.ldz + c);
-    const Vec<E, 8> u = *(const Vec<E, 8> *)((const E *)f.halves + (t * 2 + 1) * f.ldz + c);
+    const Vec<float, 8> g = *(const Vec<float, 8> *)(f.halves + t * 2 * f.ldz + c);
+    const Vec<float, 8> u = *(const Vec<float, 8> *)(f.halves + (t * 2 + 1) * f.ldz + c);
     float dy[8];
 #pragma unroll
     for (int k = 0; k < 8; k += N) {
@@ -60,17 +61,28 @@ __device__ __forceinline__ void gradients_of(const Back &f, int64_t t, int c, fl
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
         float act, slope;
-        slope_of(f.activation, to_float(g.v[e]), act, slope);
-        dg[e] = c + e < f.F ? dy[e] * (to_float(u.v[e]) * slope) : 0.f;
+        slope_of(f.activation, g.v[e], act, slope);
+        dg[e] = c + e < f.F ? dy[e] * (u.v[e] * slope) : 0.f;
         du[e] = c + e < f.F ? dy[e] * act : 0.f;
     }
 }
 
-__device__ __forceinline__ int power_above(uint32_t top)
+__device__ __forceinline__ int power_above(float top)
 {
     int e = 0;
-    frexpf(__uint_as_float(top), &e);
-    return top == 0 ? 0 : e < -100 ? -100 : e > 120 ? 120 : e;
+    frexpf(top, &e);
+    return top == 0.f ? 0 : e < -100 ? -100 : e > 120 ? 120 : e;
+}
+
+// The largest of a workgroup of 256 threads.
+__device__ __forceinline__ float largest(float top)
+{
+    __shared__ float of_wave[4];
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
+    if ((threadIdx.x & 63) == 0) of_wave[threadIdx.x >> 6] = top;
+    __syncthreads();
+    return fmaxf(fmaxf(of_wave[0], of_wave[1]), fmaxf(of_wave[2], of_wave[3]));
 }
 
 // Eight values to their place in a row of dz; `left` of them exist.
@@ -117,7 +129,9 @@ __global__ __launch_bounds__(256) void back_kernel(Back f)
     const int lane = threadIdx.x % 32, part = threadIdx.x / 32, c = blockIdx.x * 256 + lane * 8;
     float scale = 1.f;
     if constexpr (P::half) {
-        const int e = power_above(*f.top);
+        float top = 0.f;
+        for (int i = threadIdx.x; i < f.top_groups; i += 256) top = fmaxf(top, f.tops[i]);
+        const int e = power_above(largest(top));
         scale = ldexpf(kProbScale, -e);
         if (blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0) *f.factor = ldexpf(1.f, e);
     }
@@ -161,28 +175,28 @@ __global__ __launch_bounds__(256) void back_kernel(Back f)
     }
 }
 
-__global__ void no_top_kernel(uint32_t *top) { *top = 0; }
-
-// The largest finite |dz|; a maximum does not mind the order of the atomics.
+// The largest finite |dz|, of every workgroup's eighths of rows (one atomic maximum for all waves took 100 us where 1543 rows of
+// 2731 columns take 12).
+constexpr int kTopGroups = 1024;
 __global__ __launch_bounds__(256) void top_kernel(Back f)
 {
-    const int lane = threadIdx.x % 32, part = threadIdx.x / 32, c = blockIdx.x * 256 + lane * 8;
+    const int lane = threadIdx.x % 32, part = threadIdx.x / 32, across = (f.F + 255) / 256;
+    const int64_t units = (f.T + 7) / 8 * across;
     float top = 0.f;
-    if (c < f.F)
-        for (int i = 0; i < f.rows; i += 8) {
-            const int64_t t = (int64_t)blockIdx.y * f.rows + i + part;
-            if (t >= f.T) break;
-            float dg[8], du[8];
-            gradients_of<f16_t>(f, t, c, dg, du);
+    for (int64_t i = blockIdx.x; i < units; i += gridDim.x) {
+        const int64_t t = i / across * 8 + part;
+        const int c = (int)(i % across) * 256 + lane * 8;
+        if (t >= f.T || c >= f.F) continue;
+        float dg[8], du[8];
+        gradients_of<f16_t>(f, t, c, dg, du);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                if (fabsf(dg[e]) < INFINITY) top = fmaxf(top, fabsf(dg[e]));
-                if (fabsf(du[e]) < INFINITY) top = fmaxf(top, fabsf(du[e]));
-            }
+        for (int e = 0; e < 8; ++e) {
+            if (fabsf(dg[e]) < INFINITY) top = fmaxf(top, fabsf(dg[e]));
+            if (fabsf(du[e]) < INFINITY) top = fmaxf(top, fabsf(du[e]));
         }
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
-    if ((threadIdx.x & 63) == 0 && top > 0.f) atomicMax(f.top, __float_as_uint(top));
+    }
+    top = largest(top);
+    if (threadIdx.x == 0) f.tops[blockIdx.x] = top;
 }
 
 struct Call {
@@ -201,7 +215,7 @@ struct Plan {
     int64_t ldd, ldp;
     bool pack_x, pack_w, raw;
     Choice hidden, weight;
-    size_t x, w, dz, bias, slices, top, factor, bytes;
+    size_t x, w, dz, bias, slices, tops, factor, bytes;
 };
 
 template <typename P>
@@ -229,7 +243,9 @@ Plan plan_of(const void *x, int64_t ldx, const void *weight, int64_t ldw, int64_
     } else {
         p.words = (int)(kSplit ? (2 * F + 31) / 32 * 32 : (2 * F + 7) / 8 * 8);
         p.ldp = (int64_t)p.words * P::planes;
-        p.rows = (T + 63) / 64 * ((F + 255) / 256) >= 2 * device_cus() ? 64 : 8;
+        // as many as leave every CU two workgroups: a bias's gradient is a sum over the workgroups along T
+        p.rows = 64;
+        while (p.rows > 8 && (T + p.rows - 1) / p.rows * ((F + 255) / 256) < 2 * device_cus()) p.rows /= 2;
         p.rows = std::max(p.rows, (int)((T + 65534) / 65535 + 7) / 8 * 8);  // the grid's second axis has 65535 workgroups
         p.dz = take((size_t)T * p.ldp * 2);
         p.bias = take((size_t)((T + p.rows - 1) / p.rows) * 2 * F * 4);
@@ -239,7 +255,7 @@ Plan plan_of(const void *x, int64_t ldx, const void *weight, int64_t ldw, int64_
         if (p.hidden.splits > 1) slices = (size_t)p.hidden.splits * T * D * 4;
         if (p.weight.splits > 1) slices = std::max(slices, (size_t)p.weight.splits * 2 * F * D * 4);
         p.slices = take(slices);
-        p.top = take(4), p.factor = take(4);
+        if (P::half) p.tops = take(kTopGroups * 4), p.factor = take(4);
     }
     p.bytes = at ? at : 256;
     return p;
@@ -269,7 +285,7 @@ int operands(const Call &c, const Plan &p, Operand &x, Operand &w)
 }
 
 template <typename P>
-int forward(const Call &c, const void *bias, int activation, void *out, void *halves)
+int forward(const Call &c, const void *bias, int activation, void *out, float *halves)
 {
     const Plan p = plan_of<P>(c.x, c.ldx, c.weight, c.ldw, c.T, c.D, c.F, kForward);
     if (!c.ws || c.ws_bytes < p.bytes || (uintptr_t)c.ws % 256) return DS_EWORKSPACE;
@@ -292,7 +308,7 @@ struct Results {
 };
 
 template <typename P>
-int backward(const Call &c, const void *halves, const void *grad, int64_t ldg, int activation, const Results &r)
+int backward(const Call &c, const float *halves, const void *grad, int64_t ldg, int activation, const Results &r)
 {
     typedef typename ElementOf<P>::type E;
     const Plan p = plan_of<P>(c.x, c.ldx, c.weight, c.ldw, c.T, c.D, c.F, kBackward);
@@ -303,11 +319,13 @@ int backward(const Call &c, const void *halves, const void *grad, int64_t ldg, i
     float *const factor = P::half ? (float *)(c.ws + p.factor) : nullptr;
     const int tiles = ceil_div(T, p.rows);
     Back f{halves, grad, (c.F + 7) / 8 * 8, ldg, c.T, (int)c.F, activation, p.rows, c.ws + p.dz, p.ldp, p.words,
-           r.dbias ? (float *)(c.ws + p.bias) : nullptr, (uint32_t *)(c.ws + p.top), factor};
+           r.dbias ? (float *)(c.ws + p.bias) : nullptr, (float *)(c.ws + p.tops), 0, factor};
     const dim3 grid(ceil_div((int)c.F, 256), tiles);
-    if (P::half) hipLaunchKernelGGL(no_top_kernel, dim3(1), dim3(1), 0, c.st, f.top);
     if (T > 0 && n > 0) {
-        if (P::half) hipLaunchKernelGGL(top_kernel, grid, dim3(256), 0, c.st, f);
+        if (P::half) {
+            f.top_groups = (int)std::min<int64_t>(kTopGroups, (int64_t)ceil_div(T, 8) * grid.x);
+            hipLaunchKernelGGL(top_kernel, dim3(f.top_groups), dim3(256), 0, c.st, f);
+        }
         hipLaunchKernelGGL((back_kernel<P>), grid, dim3(256), 0, c.st, f);
     }
     const bool made = T > 0 && n > 0;  // dz, and with it the factor
@@ -363,7 +381,7 @@ DS_EXPORT size_t ds_gated_workspace_bytes(const void *x, int64_t ldx, const void
 }
 
 DS_EXPORT int ds_gated_forward(const void *x, int64_t ldx, const void *weight, int64_t ldw, const void *bias, int activation,
-                               int64_t T, int64_t D, int64_t F, int type, void *out, void *halves, void *workspace,
+                               int64_t T, int64_t D, int64_t F, int type, void *out, float *halves, void *workspace,
                                size_t workspace_bytes, ds_stream_t stream)
 {
     const gated::Call c{x, weight, ldx, ldw, T, D, F, type, (char *)workspace, workspace_bytes, (hipStream_t)stream};
@@ -375,7 +393,7 @@ DS_EXPORT int ds_gated_forward(const void *x, int64_t ldx, const void *weight, i
     return forward<F16>(c, bias, activation, out, halves);
 }
 
-DS_EXPORT int ds_gated_backward(const void *x, int64_t ldx, const void *weight, int64_t ldw, const void *halves, const void *grad,
+DS_EXPORT int ds_gated_backward(const void *x, int64_t ldx, const void *weight, int64_t ldw, const float *halves, const void *grad,
                                 int64_t ldg, int activation, int64_t T, int64_t D, int64_t F, int type, void *dx, void *dweight,
                                 void *dbias, void *workspace, size_t workspace_bytes, ds_stream_t stream)
 {

@@ -166,7 +166,7 @@ struct Args {
     // kGate (bias, out and ldo too): M is half of A's rows
     int64_t half_bytes;   // from the first half to the second
     int activation;
-    void *halves;         // [N][2][ldz] both halves of the products, or NULL
+    float *halves;        // [N][2][ldz] both halves of the products, or NULL
     int64_t ldz;
 };
 
@@ -1200,11 +1200,12 @@ __device__ __forceinline__ void product_tile(const Args &g, const int block, cha
     }
     if constexpr (KIND == kGate) {
         typedef typename ElementOf<P>::type E;
-        typedef Gather<E, BM / 2> Out;
         static_assert(MT % 2 == 0, "both halves of a result in one wave");
-        // which 0: the gated values, 1 and 2: the halves of the products as they are
-        auto pass = [&](int j, auto which, void *base, int64_t ld) {
+        // which 0: the gated values, 1 and 2: the halves of the products as they are, in 32 bits
+        auto pass = [&](int j, auto which, auto *base, int64_t ld) {
             constexpr int kWhich = decltype(which)::value;
+            typedef typename std::remove_pointer<decltype(base)>::type S;
+            typedef Gather<S, BM / 2> Out;
 #pragma unroll
             for (int i = 0; i < MT / 2; ++i)
 #pragma unroll
@@ -1221,22 +1222,22 @@ __device__ __forceinline__ void product_tile(const Args &g, const int block, cha
                         v[r] = kWhich == 0 ? activation_of(g.activation, gate[r]) * up[r] : kWhich == 1 ? gate[r] : up[r];
                     }
                     char *to = Out::at(lds, row_out, (wm * (MT / 2) + i) * U::size + U::lane_m(lane) + U::group_m(q));
-                    if constexpr (sizeof(E) == 4) *(f32x4 *)to = v;
+                    if constexpr (sizeof(S) == 4) *(f32x4 *)to = v;
                     else *(s16x4 *)to = round4<P>(v);
                 }
             __syncthreads();
-            Out::template leave<kThreads>(lds, kRowsOut, g.M - m0, [&](int row) -> E * {
+            Out::template leave<kThreads>(lds, kRowsOut, g.M - m0, [&](int row) -> S * {
                 const int n = n0 + n_of(row, j);
-                return n < g.N ? (E *)base + n * ld + m0 : nullptr;
+                return n < g.N ? base + n * ld + m0 : nullptr;
             });
             __syncthreads();
         };
 #pragma unroll
         for (int j = 0; j < NT; ++j) {
-            pass(j, std::integral_constant<int, 0>(), g.out, g.ldo);
+            pass(j, std::integral_constant<int, 0>(), (E *)g.out, g.ldo);
             if (!g.halves) continue;
             pass(j, std::integral_constant<int, 1>(), g.halves, 2 * g.ldz);
-            pass(j, std::integral_constant<int, 2>(), (E *)g.halves + g.ldz, 2 * g.ldz);
+            pass(j, std::integral_constant<int, 2>(), g.halves + g.ldz, 2 * g.ldz);
         }
     }
     if constexpr (KIND == kOut) {

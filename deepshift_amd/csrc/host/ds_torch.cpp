@@ -623,12 +623,12 @@ PyObject *gated(PyObject *, PyObject *const *args, Py_ssize_t count)
         shape.back() = g.F;
         const at::Tensor out = g.empty(shape);
         at::Tensor halves;
-        if (integer(args[4])) halves = g.empty(g.kept());
+        if (integer(args[4])) halves = g.empty(g.kept(), at::kFloat);
         const at::Tensor ws = g.workspace(1);
         expect("ds_gated_forward",
                ds_gated_forward(g.x.const_data_ptr(), g.ldx, g.weight.const_data_ptr(), g.ldw,
                                 g.bias.defined() ? g.bias.const_data_ptr() : nullptr, (int)g.activation, g.T, g.D, g.F, g.type,
-                                at_or_null(out), at_or_null(halves), ws.mutable_data_ptr(), ws.nbytes(), stream(args[5])));
+                                at_or_null(out), at_or_null<float>(halves), ws.mutable_data_ptr(), ws.nbytes(), stream(args[5])));
         return tuple_of({out, halves});
     });
 }
@@ -640,7 +640,7 @@ PyObject *gated_grad(PyObject *, PyObject *const *args, Py_ssize_t count)
     return guarded(count, 7, [&] {
         const Gated g(args[0], args[1], Py_None, args[4]);
         const at::Tensor &halves = tensor("halves", args[2]);
-        check_like("halves", halves, " like x", g.x.scalar_type(), g.x.device(), g.kept());
+        check_like("halves", halves, "", at::kFloat, g.x.device(), g.kept());
         at::Tensor grad = tensor("grad", args[3]);
         std::vector<int64_t> shape = g.shape;
         shape.back() = g.F;
@@ -653,7 +653,7 @@ PyObject *gated_grad(PyObject *, PyObject *const *args, Py_ssize_t count)
         if (wanted & 4) dbias = g.empty({2 * g.F});
         const at::Tensor ws = g.workspace(2);
         expect("ds_gated_backward",
-               ds_gated_backward(g.x.const_data_ptr(), g.ldx, g.weight.const_data_ptr(), g.ldw, halves.const_data_ptr(),
+               ds_gated_backward(g.x.const_data_ptr(), g.ldx, g.weight.const_data_ptr(), g.ldw, (const float *)halves.const_data_ptr(),
                                  grad.const_data_ptr(), ldg, (int)g.activation, g.T, g.D, g.F, g.type, at_or_null(dx),
                                  at_or_null(dweight), at_or_null(dbias), ws.mutable_data_ptr(), ws.nbytes(), stream(args[6])));
         return tuple_of({dx, dweight, dbias});

@@ -318,8 +318,8 @@ def gated_linear(x, weight, bias=None, activation="silu"):
     """``act(x @ gate.T + b) * (x @ up.T + c)``, the gated block of a feed-forward layer, both projections, the activation and the
     product in one kernel: ``weight`` ``[2 F, D]`` is ``gate`` above ``up`` and ``bias`` ``[2 F]`` ``b`` before ``c`` -- what one
     linear layer, or one ``LinearShift``, of ``2 F`` features holds.  ``x`` ``[..., D]``, all of one type; ``activation`` is
-    ``'silu'``, ``'gelu'`` (by the error function), ``'relu'`` or ``'sigmoid'``.  For gradients both projections are kept in that
-    type."""
+    ``'silu'``, ``'gelu'`` (by the error function), ``'relu'`` or ``'sigmoid'``.  For gradients both projections are kept, in
+    32 bits."""
     activation = _activation(activation)
     if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or (bias is not None and bias.requires_grad)):
         return _GatedLinear.apply(x, weight, bias, activation)

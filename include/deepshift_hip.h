@@ -592,18 +592,18 @@ int ds_distill_loss_step(const void *hidden, int64_t ldh, const void *weight, in
                          void *dbias, void *workspace, size_t workspace_bytes, ds_stream_t stream);
 
 /* Gated block of a feed-forward layer: out[t][f] = act(x[t] . weight[f] + bias[f]) * (x[t] . weight[F + f] + bias[F + f]), x [T][D],
- * weight [2 F][D], bias [2 F] or NULL, out [T][F], all of `type`.  halves, or NULL, is [T][2][F rounded up to a multiple of 8] and
- * gets both products, which ds_gated_backward takes.  workspace: 256-byte aligned, ds_gated_workspace_bytes(..., what) bytes with
+ * weight [2 F][D], bias [2 F] or NULL, out [T][F], all of `type`.  halves, or NULL, is float32 [T][2][F rounded up to a multiple of
+ * 8] and gets both products, which ds_gated_backward takes.  workspace: 256-byte aligned, ds_gated_workspace_bytes(..., what) bytes with
  * what = 1 here and 2 there. */
 enum { DS_SILU = 0, DS_GELU = 1, DS_RELU = 2, DS_SIGMOID = 3 };
 size_t ds_gated_workspace_bytes(const void *x, int64_t ldx, const void *weight, int64_t ldw, int64_t T, int64_t D, int64_t F, int type,
                                 int what);
 int ds_gated_forward(const void *x, int64_t ldx, const void *weight, int64_t ldw, const void *bias, int activation, int64_t T,
-                     int64_t D, int64_t F, int type, void *out, void *halves, void *workspace, size_t workspace_bytes,
+                     int64_t D, int64_t F, int type, void *out, float *halves, void *workspace, size_t workspace_bytes,
                      ds_stream_t stream);
 
 /* Its gradients for grad [T][F], rows ldg apart: dx [T][D], dweight [2 F][D], dbias [2 F], each NULL where it is not asked for. */
-int ds_gated_backward(const void *x, int64_t ldx, const void *weight, int64_t ldw, const void *halves, const void *grad, int64_t ldg,
+int ds_gated_backward(const void *x, int64_t ldx, const void *weight, int64_t ldw, const float *halves, const void *grad, int64_t ldg,
                       int activation, int64_t T, int64_t D, int64_t F, int type, void *dx, void *dweight, void *dbias,
                       void *workspace, size_t workspace_bytes, ds_stream_t stream);
 
