@@ -513,12 +513,17 @@ struct Known {
     float scale[BN];
     float power[BN];
 };
-template <int BM, int BN>
+// Of a teacher's words: which of the token's lie in the tile, and of the first four of them (there are hardly ever more) where, counted
+// from the tile's first word, and the probabilities; so the epilogue waits for memory where there are more only.
+constexpr int kTaughtKnown = 4;
+template <int BM, int BN, int KIND>
 struct TaughtKnown : Known<BM, BN> {
-    int first[BN], last[BN];  // which of the token's words lie in the tile
+    uint64_t words[BN];  // 16 bits each
+    int first[BN], count[BN];
+    float taught[KIND == kProb ? BN : 1][kTaughtKnown];
 };
-template <int BM, int BN, bool TAUGHT>
-using KnownOf = typename std::conditional<TAUGHT, TaughtKnown<BM, BN>, Known<BM, BN>>::type;
+template <int BM, int BN, int KIND, bool TAUGHT>
+using KnownOf = typename std::conditional<TAUGHT, TaughtKnown<BM, BN, KIND>, Known<BM, BN>>::type;
 // Rows that leave together, what one of them takes, and whether the waves' maxima and sums find a place behind them in the
 // stages (256 x 256 tiles' exponentials fill those).
 template <typename P, int WN> constexpr int kRowsLeaving = WN * Unit<P>::size;
@@ -526,7 +531,7 @@ template <typename P, int BM, int KIND> constexpr int kRowBytes = KIND == kGate 
 template <typename P, int BM, int BN, int WM, int WN, int KIND, int STAGES, bool RAW>
 constexpr bool kRoomBehind = KIND == kStats || kRowsLeaving<P, WN> * kRowBytes<P, BM, KIND> + WM * BN * 8 <= kStagesBytes<P, BM, BN, STAGES, RAW>;
 template <typename P, int BM, int BN, int WM, int WN, int KIND, int STAGES, bool RAW = false, bool TAUGHT = false>
-constexpr int kLdsBytes = kStagesBytes<P, BM, BN, STAGES, RAW> + (KIND != kOut ? (int)sizeof(KnownOf<BM, BN, TAUGHT>) : 0) +
+constexpr int kLdsBytes = kStagesBytes<P, BM, BN, STAGES, RAW> + (KIND != kOut ? (int)sizeof(KnownOf<BM, BN, KIND, TAUGHT>) : 0) +
                           (KIND == kKeep && !kRoomBehind<P, BM, BN, WM, WN, KIND, STAGES, RAW> ? WM * BN * 8 : 0) +
                           (P::planes > 1 ? 16 : 0);
 
@@ -647,12 +652,12 @@ __device__ __forceinline__ void product_tile(const Args &g, const int block, cha
 #pragma unroll
             for (int r = 0; r < 4 * U::groups; ++r) acc[i][j][r] = 0.f;
 
-    typedef KnownOf<BM, BN, TAUGHT> Here;
+    typedef KnownOf<BM, BN, KIND, TAUGHT> Here;
     Here &known = *(Here *)(lds + kStagesBytes<P, BM, BN, STAGES, (RAW > 0)>);
     static_assert(BM <= WAVES * 64 && BN <= WAVES * 64, "a thread per word and token");
     constexpr int kNowhere = -(1 << 20);
     float bias = -INFINITY, lse = INFINITY, scale = 0.f, power = 1.f;
-    int want = kNowhere, first = 0, last = 0;
+    int want = kNowhere;
     // base 2
     const float to_logit = TAUGHT ? kLog2e * g.warmth : kLog2e;
     if constexpr (KIND == kGate) {
@@ -664,20 +669,6 @@ __device__ __forceinline__ void product_tile(const Args &g, const int block, cha
         if (threadIdx.x < BN && n < g.N) {
             const int64_t y = target_at(g, n), here = y - g.v0 - m0;
             if (!TAUGHT && here >= 0 && here < BM && m0 + here < g.M) want = (int)here;
-            if constexpr (TAUGHT) {
-                // the first of the token's words that is not below `word`
-                const int *const ids = g.taught_ids + (int64_t)n * g.taught_words;
-                auto behind = [&](int word) {
-                    int low = 0, high = g.taught_words;
-                    while (low < high) {
-                        const int middle = (low + high) / 2;
-                        if (ids[middle] < word) low = middle + 1;
-                        else high = middle;
-                    }
-                    return low;
-                };
-                first = behind(g.v0 + m0), last = behind(g.v0 + min(g.M, m0 + BM));
-            }
             if constexpr (KIND == kProb) {
                 if (y != g.ignore) {
                     lse = g.lse[n];
@@ -691,12 +682,56 @@ __device__ __forceinline__ void product_tile(const Args &g, const int block, cha
     }
 
     int *const met_nan = (int *)(lds + kLdsBytes<P, BM, BN, WM, WN, KIND, STAGES, (RAW > 0), TAUGHT>) - 1;  // of float32: a result is NaN
+    // A token's words in the tile, searched for while the first stages are on their way: both ends at once, among seven words a
+    // round.
+    auto keep_taught = [&] {
+        if constexpr (TAUGHT) {
+            const int n = n0 + threadIdx.x;
+            int low[2] = {0, 0};
+            uint64_t words = 0;
+            if (n < g.N) {
+                const int *const ids = g.taught_ids + (int64_t)n * g.taught_words;
+                const int ends[2] = {g.v0 + m0, g.v0 + min(g.M, m0 + BM)};
+                int high[2] = {g.taught_words, g.taught_words};  // those before low lie before the end, those from high on do not
+                while (low[0] < high[0] || low[1] < high[1]) {
+                    int id[2][7];
+    #pragma unroll
+                    for (int e = 0; e < 2; ++e)
+    #pragma unroll
+                        for (int i = 0; i < 7; ++i) {
+                            const int at = low[e] + (i + 1) * ((high[e] - low[e] + 7) / 8) - 1;
+                            id[e][i] = at >= 0 && at < high[e] ? ids[at] : 0x7fffffff;
+                        }
+    #pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        const int step = (high[e] - low[e] + 7) / 8;
+                        int before = 0;
+    #pragma unroll
+                        for (int i = 0; i < 7; ++i) before += id[e][i] < ends[e];
+                        if (before < 7) high[e] = max(low[e], min(high[e], low[e] + (before + 1) * step - 1));
+                        low[e] += before * step;
+                    }
+                }
+                int id[kTaughtKnown];
+    #pragma unroll
+                for (int i = 0; i < kTaughtKnown; ++i) {
+                    const bool there = low[0] + i < low[1];
+                    id[i] = there ? ids[low[0] + i] - ends[0] : 0;
+                    if (KIND == kProb)
+                        known.taught[threadIdx.x][i] = there ? g.taught[(int64_t)n * g.taught_words + low[0] + i] : 0.f;
+                }
+    #pragma unroll
+                for (int i = 0; i < kTaughtKnown; ++i) words |= (uint64_t)(uint32_t)id[i] << 16 * i;
+            }
+            known.words[threadIdx.x] = words, known.first[threadIdx.x] = low[0], known.count[threadIdx.x] = low[1] - low[0];
+        }
+    };
     auto keep_known = [&] {
         if (NP > 1 && threadIdx.x == 0) *met_nan = 0;
         if constexpr (KIND != kOut) {
             if (threadIdx.x < BM) known.bias[threadIdx.x] = bias;
             if constexpr (TAUGHT)
-                if (threadIdx.x < BN) known.first[threadIdx.x] = first, known.last[threadIdx.x] = last;
+                if (threadIdx.x < BN) keep_taught();
             if (KIND != kGate && threadIdx.x < BN)
                 known.want[threadIdx.x] = want, known.lse[threadIdx.x] = lse, known.scale[threadIdx.x] = scale;
             if (P::half && KIND == kProb && threadIdx.x < BN) known.power[threadIdx.x] = power;
@@ -980,29 +1015,37 @@ __device__ __forceinline__ void product_tile(const Args &g, const int block, cha
     float *fl = (float *)lds;
     // a logit, base 2
     auto logit = [&](int I, int j, int r) -> float { return fmaf(value(I, j, r), to_logit, known.bias[m_in + m_of(I) + r]); };
-    // TAUGHT: walks over the taught words of column j that lie in the tile, along with its words: `found(e, r)` for those among
-    // the four of I.  Both are in ascending order; lanes that share a column skip each other's.
-    int taught_at = 0, taught_last = 0, taught_word = 0;
-    const int *taught_ids = nullptr;
-    auto look_at_taught = [&] {
-        taught_word = taught_at < taught_last ? taught_ids[taught_at] - g.v0 - m0 - m_in : 0x7fffffff;
-    };
-    auto begin_taught = [&](int j) {
+    // TAUGHT: over the taught words of column j that lie in the tile, in ascending order; `found(k, word)` for those among this lane's,
+    // k counted from the first, word from m_in.  The registers that hold a word are found by comparing it with all of them, in one
+    // loop over the words: a loop in every four of its logits' code, along with them, took 62 us for scores of 130 tokens of 2048
+    // features over 50021 words, bfloat16, where this takes 50 and a single target 48 (8192 x 4096 x 65536: 4.01, 3.90, 3.72 ms).
+    int64_t taught_first = 0;  // in the whole list
+    auto walk_taught = [&](int j, auto found) {
         if constexpr (TAUGHT) {
             const int c = n_in + j * U::size;
-            taught_at = known.first[c], taught_last = known.last[c];
-            taught_ids = g.taught_ids + (int64_t)(n0 + c) * g.taught_words;
-            look_at_taught();
+            const int count = known.count[c];
+            taught_first = (int64_t)(n0 + c) * g.taught_words + known.first[c];
+            uint64_t words = known.words[c];
+            for (int k = 0; __any(k < count); ++k, words >>= 16) {
+                if (k >= count) continue;
+                found(k, (k < kTaughtKnown ? (int)(words & 0xffff) : g.taught_ids[taught_first + k] - g.v0 - m0) - m_in);
+            }
         }
     };
-    auto walk_taught = [&](int I, auto found) {
-        if constexpr (TAUGHT)
-            while (__any(taught_word < m_of(I) + 4)) {
-                if (taught_word >= m_of(I) + 4) continue;
-                if (taught_word >= m_of(I)) found(taught_at, taught_word - m_of(I));
-                ++taught_at;
-                look_at_taught();
+    auto pick_taught = [&](int j) {
+        walk_taught(j, [&](int k, int word) {
+            float v[4];
+            bool mine = false;
+#pragma unroll
+            for (int I = 0; I < MG; ++I) {
+                const bool here = (word & ~3) == m_of(I);
+                mine |= here;
+#pragma unroll
+                for (int r = 0; r < 4; ++r) v[r] = here || I == 0 ? value(I, j, r) : v[r];
             }
+            const int r = word & 3;
+            if (mine) g.picked[taught_first + k] = fmaf(r < 2 ? r == 0 ? v[0] : v[1] : r == 2 ? v[2] : v[3], to_logit, known.bias[m_in + word]);
+        });
     };
     constexpr int kRowsOut = kRowsLeaving<P, WN>, kThreads = WAVES * 64;  // one j of every wave
     static_assert(KIND == kStats || kRowsOut * kRowBytes<P, BM, KIND> <= kStagesBytes<P, BM, BN, STAGES, (RAW > 0)>, "");
@@ -1055,7 +1098,6 @@ __device__ __forceinline__ void product_tile(const Args &g, const int block, cha
         auto tops_of = [&](int j) {
             const int at = known.want[n_in + j * U::size] - m_in;  // where the target lies behind this lane's first word
             float top = -INFINITY;
-            begin_taught(j);
 #pragma unroll
             for (int I = 0; I < MG; ++I) {
                 float s[4];
@@ -1064,15 +1106,12 @@ __device__ __forceinline__ void product_tile(const Args &g, const int block, cha
                     s[r] = logit(I, j, r);
                     top = fmaxf(top, s[r]);  // what is no number shows in the sum
                 }
-                if ((unsigned)(at - m_of(I)) < 4u)
+                if (!TAUGHT && (unsigned)(at - m_of(I)) < 4u)
 #pragma unroll
                     for (int r = 0; r < 4; ++r)
                         if (at == m_of(I) + r) g.picked[n0 + n_in + j * U::size] = s[r];
-                walk_taught(I, [&](int e, int which) {
-                    g.picked[(int64_t)(n0 + n_in + j * U::size) * g.taught_words + e] =
-                        which < 2 ? which == 0 ? s[0] : s[1] : which == 2 ? s[2] : s[3];
-                });
             }
+            if constexpr (TAUGHT) pick_taught(j);
             return top;
         };
         // exponentials relative to `top`, and their sum over this lane's words; a column of nothing but -inf keeps a sum of 0
@@ -1153,21 +1192,39 @@ __device__ __forceinline__ void product_tile(const Args &g, const int block, cha
             const float least = lse == INFINITY ? -INFINITY : -126.f;
             const bool counts = !(lse == INFINITY && scale == 0.f);  // else nothing is left, also of infinite weights times 0
             const int at = known.want[n_in + j * U::size] - m_in;
-            begin_taught(j);
+            if constexpr (TAUGHT) {
+                // the probabilities take the products' places, and the teacher's leave them
+#pragma unroll
+                for (int I = 0; I < MG; ++I) {
+                    float x[4], p[4];
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) x[r] = logit(I, j, r) - lse;
+                    exp2_of_four(x, p, least);
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) acc[I / U::groups][j][I % U::groups * 4 + r] = p[r];
+                }
+                walk_taught(j, [&](int k, int word) {
+                    const float q = k < kTaughtKnown ? known.taught[n_in + j * U::size][k] : g.taught[taught_first + k];
+#pragma unroll
+                    for (int I = 0; I < MG; ++I)
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) acc[I / U::groups][j][I % U::groups * 4 + r] -= word == m_of(I) + r ? q : 0.f;
+                });
+            }
 #pragma unroll
             for (int I = 0; I < MG; ++I) {
                 float x[4], p[4];
+                if constexpr (TAUGHT) {
 #pragma unroll
-                for (int r = 0; r < 4; ++r) x[r] = logit(I, j, r) - lse;
-                exp2_of_four(x, p, least);
-                if ((unsigned)(at - m_of(I)) < 4u)
+                    for (int r = 0; r < 4; ++r) p[r] = value(I, j, r);
+                } else {
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) p[r] -= at == m_of(I) + r ? 1.f : 0.f;
-                walk_taught(I, [&](int e, int which) {
-                    const float q = g.taught[(int64_t)(n0 + n_in + j * U::size) * g.taught_words + e];
+                    for (int r = 0; r < 4; ++r) x[r] = logit(I, j, r) - lse;
+                    exp2_of_four(x, p, least);
+                    if ((unsigned)(at - m_of(I)) < 4u)
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) p[r] -= which == r ? q : 0.f;
-                });
+                        for (int r = 0; r < 4; ++r) p[r] -= at == m_of(I) + r ? 1.f : 0.f;
+                }
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
                     p[r] = counts ? p[r] * scale : 0.f;

@@ -13,7 +13,7 @@
 // Distillation from a teacher's best K words is the same with many targets a token, q the softmax of their logits by the
 // temperature c:  p = softmax(s / c)      loss[t] = c^2 sum_k q_k (log q_k - log p_k)      P = c g_t (p - q).
 // One launch makes q of the teacher's logits and puts the words in ascending order; the tiles find the words that lie in them by
-// a binary search while their operands arrive, and walk over them along with their logits.
+// a search while their operands arrive.
 #include "ds_vocab_host.h"
 
 namespace ds {
@@ -350,12 +350,22 @@ __global__ __launch_bounds__(256) void finish_kernel(Finish f)
             }
             parts[wave * 64 + row] = float2{top, sum};
             __syncthreads();
-            if (wave == 0 && t < r.T) {
+            float lse = 0.f, away = 0.f;
+            if (t < r.T && (TAUGHT || wave == 0)) {
+                top = -INFINITY, sum = 0.f;
 #pragma unroll
-                for (int w = 1; w < 4; ++w) join_pair(top, sum, parts[w * 64 + row].x, parts[w * 64 + row].y);
-                const float lse = log_of_sum(top, sum);
+                for (int w = 0; w < 4; ++w) join_pair(top, sum, parts[w * 64 + row].x, parts[w * 64 + row].y);
+                lse = log_of_sum(top, sum);
+            }
+            if constexpr (TAUGHT) {
+                float *const shares = sums[2];  // [4][64], behind the parts
+                if (t < r.T) shares[wave * 64 + row] = taught_loss(r, t, lse, wave, 4);
+                __syncthreads();
+                away = (shares[row] + shares[64 + row] + shares[128 + row] + shares[192 + row]) * (kLn2 * r.temperature * r.temperature);
+            }
+            if (wave == 0 && t < r.T) {
                 const int64_t y = target_of(r.target, r.wide, t);
-                const float l = loss_of(r, t, y, lse);
+                const float l = !TAUGHT ? loss_of(r, t, y, lse) : y == r.ignore ? 0.f : y >= r.V ? NAN : away;
                 r.lse[t] = lse, r.loss[t] = l;
                 loss += l, counted += y != r.ignore;
             }
@@ -759,10 +769,10 @@ Args logit_args(const Call &c, const Plan &p, int64_t v0, int64_t n, const Opera
 }
 
 // Whether finish_kernel joins the rows' sums: each of its workgroups does it for its own rows, and one for all, which pays
-// while there are few of both (64 tokens, 1000 words, float32: 3 us of a step).
+// while there are few of both (64 tokens, 1000 words, float32: 3 us of a step) and of a teacher's words.
 inline bool joined_later(const Call &c, const Plan &p, int tiles)
 {
-    return p.keep && p.pieces == 1 && c.T <= 128 && tiles <= 64 && !c.teacher.K;
+    return p.keep && p.pieces == 1 && c.T <= 128 && tiles <= 64 && c.teacher.K <= 64;
 }
 
 // One product, of `kind`, by the kernels of the plan; fills in the tile counts.
@@ -850,7 +860,9 @@ int loss_grad(const Call &c, const Plan &p, Operands<P> &o, const Rows &of, Grad
                 const Finish f{c.ws + p.prob, p.ldp, (const float *)(c.ws + (beside ? p.kept : p.prob)), beside ? p.words : p.ldp / 2, words, p.tile_words, rows, v0, n, of.tiles - ceil_div((int)n, p.tile_words),
                                p.words, of, bias_part, bias_out, {r.grad, r.share}, c.teacher.sorted};
                 const unsigned along = ceil_div(words, 256), down = ceil_div((int)c.T, rows);
-                if (joined_later(c, p, of.tiles))
+                if (joined_later(c, p, of.tiles) && c.teacher.K)
+                    hipLaunchKernelGGL((finish_kernel<P, true, true>), dim3(along, down + 1), dim3(256), 0, c.st, f);
+                else if (joined_later(c, p, of.tiles))
                     hipLaunchKernelGGL((finish_kernel<P, true>), dim3(along, down + 1), dim3(256), 0, c.st, f);
                 else if (c.teacher.K)
                     hipLaunchKernelGGL((finish_kernel<P, false, true>), dim3(along, down), dim3(256), 0, c.st, f);
