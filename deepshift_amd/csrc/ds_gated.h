@@ -13,6 +13,17 @@ template <typename P> int launch_gate(int tile, Args &g, hipStream_t st);
 // float32 weights as they are
 int launch_gate_raw(Args &g, hipStream_t st);
 
+// A few tokens, whose operands lie as the caller's do (ds_gated_few.hip).
+struct Few {
+    const void *x, *weight, *bias;
+    int64_t ldx, ldw, F;
+    int T, D, activation;
+    void *out;            // [T][F]
+    float *halves;        // as Args has them
+    int64_t ldz;
+};
+template <typename E> int launch_few(const Few &f, hipStream_t st);
+
 template <typename P, int BM, int BN, int WM, int WN, int STAGES>
 int launch_gate_tiled(Args &g, hipStream_t st)
 {

@@ -213,10 +213,25 @@ enum { kForward = 1, kBackward = 2 };
 struct Plan {
     int Dp, tile, rows, words;
     int64_t ldd, ldp;
-    bool pack_x, pack_w, raw;
+    bool pack_x, pack_w, raw, few;
     Choice hidden, weight;
     size_t x, w, dz, bias, slices, tops, factor, bytes;
 };
+
+// Up to how many tokens a wave multiplies its weights as they lie, in vector registers: of float32 as long as that is bound by memory
+// (then weights are split for the matrix instructions), of 16-bit types as long as the tiles, which are too few to read as fast, take
+// longer, the more so where they need operands repacked.  As they lie and by tiles, in us, 8192 results, weights from memory:
+//                                  1 token       2         3         4         5         8 tokens
+//   4096 features, bfloat16       26   35    31   35   38   35   40   36   58   35   70   36
+//   4096, float16                 26   35    27   35   31   36   32   35   37   36   38   36
+//   4095, bfloat16                36   74    53   74   44   74   45   75   75   74   78   74
+//   4096, float32                 48  215    52  215   53  215   54  215   62  216   64  217     (9: 132 split by the tiles)
+//   1024, 2731 results, float32    9   34     8   33   10   33   10   33   14   33   14   34
+template <typename P>
+int64_t most_few(const void *x, int64_t ldx, const void *weight, int64_t ldw, int64_t D)
+{
+    return P::planes > 1 ? 8 : in_place(x, ldx, D) && in_place(weight, ldw, D) ? 2 : 4;
+}
 
 template <typename P>
 Plan plan_of(const void *x, int64_t ldx, const void *weight, int64_t ldw, int64_t T, int64_t D, int64_t F, int what)
@@ -225,11 +240,12 @@ Plan plan_of(const void *x, int64_t ldx, const void *weight, int64_t ldw, int64_
     Plan p{};
     p.Dp = (int)(kSplit ? (D + 31) / 32 * 32 : (D + 7) / 8 * 8);
     p.ldd = row_elements<P>(D);
-    // few tokens of float32: weights that are split where they are needed, as the cross entropy's
-    p.raw = kSplit && what == kForward && (uintptr_t)weight % 16 == 0 && ldw % 4 == 0 && D % 4 == 0 &&
+    p.few = what == kForward && T <= most_few<P>(x, ldx, weight, ldw, D) && g_tune.vocab_tile == kTuneUnset;
+    // not many tokens of float32: weights that are split where they are needed, as the cross entropy's
+    p.raw = !p.few && kSplit && what == kForward && (uintptr_t)weight % 16 == 0 && ldw % 4 == 0 && D % 4 == 0 &&
             T <= raw_tokens(2 * F * D, 4, kLoss) && g_tune.vocab_tile == kTuneUnset;
-    p.pack_x = kSplit || !in_place(x, ldx, D);
-    p.pack_w = !p.raw && (kSplit || !in_place(weight, ldw, D));
+    p.pack_x = !p.few && (kSplit || !in_place(x, ldx, D));
+    p.pack_w = !p.few && !p.raw && (kSplit || !in_place(weight, ldw, D));
     size_t at = 0;
     auto take = [&](size_t n) {
         const size_t was = at;
@@ -290,6 +306,10 @@ int forward(const Call &c, const void *bias, int activation, void *out, float *h
     const Plan p = plan_of<P>(c.x, c.ldx, c.weight, c.ldw, c.T, c.D, c.F, kForward);
     if (!c.ws || c.ws_bytes < p.bytes || (uintptr_t)c.ws % 256) return DS_EWORKSPACE;
     if (c.T == 0 || c.F == 0) return DS_OK;
+    const int64_t ldz = (c.F + 7) / 8 * 8;
+    if (p.few)
+        return launch_few<typename ElementOf<P>::type>(
+            Few{c.x, c.weight, bias, c.ldx, c.ldw, c.F, (int)c.T, (int)c.D, activation, out, halves, ldz}, c.st);
     Args g{};
     DS_TRY(operands<P>(c, p, g.b, g.a));
     g.M = (int)c.F, g.N = (int)c.T, g.K = p.raw ? (int)c.D : p.Dp;
@@ -297,7 +317,7 @@ int forward(const Call &c, const void *bias, int activation, void *out, float *h
     g.half_bytes = c.F * g.a.ld * (p.raw ? 4 : 2);
     g.bias = bias, g.bias_type = c.type, g.activation = activation;
     g.out = out, g.ldo = c.F;
-    g.halves = halves, g.ldz = (c.F + 7) / 8 * 8;
+    g.halves = halves, g.ldz = ldz;
     if constexpr (P::planes > 1)
         if (p.raw) return launch_gate_raw(g, c.st);
     return launch_gate<P>(p.tile, g, c.st);
