@@ -6,6 +6,12 @@ The model predicts the next token of a synthetic stream (every token is a fixed 
 the embeddings of the last two: ``training.ScaledEmbedding``, a stack of ``LinearShift`` layers on their float path (or
 ``LinearShiftQ``), and ``training.LinearCrossEntropy``; the gradients, which straight-through estimators pass to shifts and
 signs unscaled, are clipped by their global norm.  Prints the loss and the norm as it goes, then tokens per second.
+
+    python -m deepshift_amd.train_tokens --sequence 128 --teach 16
+
+trains on ragged sequences instead, with a model whose layers mix their tokens (``training.gated_recurrence``) and whose
+feed-forward layers are gated (``training.GatedShift``), and lets it learn from a teacher of twice the width too, which is trained
+along, by that one's best words (``training.linear_distillation``).
 """
 import argparse
 import time
@@ -38,6 +44,64 @@ class TokenModel(nn.Module):
         return self.head(self.hidden(tokens), target)
 
 
+def _rows(layer, x):
+    """A layer over rows (``LinearShiftQ`` takes matrices) of all axes but the last."""
+    return layer(x.flatten(0, -2)).unflatten(0, x.shape[:-1])
+
+
+class SequenceLayer(nn.Module):
+    """A shift layer to values and gates, their recurrence along the sequence and a shift layer back, then a gated block of shift
+    layers; each behind a norm, and added to what came in."""
+
+    def __init__(self, width, shift_type="PS", weight_bits=5):
+        super().__init__()
+        layer = modules.LinearShift if shift_type == "PS" else modules_q.LinearShiftQ
+        self.norms = nn.ModuleList([nn.LayerNorm(width) for _ in range(2)])
+        self.enter = layer(width, 2 * width, weight_bits=weight_bits)
+        self.leave = layer(width, width, weight_bits=weight_bits)
+        self.gated = training.GatedShift(width, 2 * width, shift_type=shift_type, weight_bits=weight_bits)
+        self.down = layer(2 * width, width, weight_bits=weight_bits)
+
+    def forward(self, x, state=None, lengths=None):
+        """``x`` [B, T, width], and what :func:`training.gated_recurrence` begins with and ends at."""
+        value, gate = _rows(self.enter, self.norms[0](x)).chunk(2, -1)
+        mixed, state = training.gated_recurrence(value, gate, state, lengths)
+        x = x + _rows(self.leave, mixed)
+        return x + _rows(self.down, self.gated(self.norms[1](x))), state
+
+
+class SequenceModel(nn.Module):
+    """Embeddings, ``depth`` layers that mix the tokens of a sequence, a linear head with its loss."""
+
+    def __init__(self, vocabulary, width, depth, shift_type="PS", weight_bits=5):
+        super().__init__()
+        self.embedding = training.ScaledEmbedding(vocabulary, width, scale=width ** 0.5)
+        self.layers = nn.ModuleList([SequenceLayer(width, shift_type, weight_bits) for _ in range(depth)])
+        self.norm = nn.LayerNorm(width)
+        self.head = training.LinearCrossEntropy(width, vocabulary)
+
+    def hidden(self, tokens, states=None, lengths=None):
+        """``tokens`` [B, T] -> [B, T, width], and the layers' states behind them, to go on from."""
+        x, ends = self.embedding(tokens), []
+        for i, layer in enumerate(self.layers):
+            x, end = layer(x, None if states is None else states[i], lengths)
+            ends.append(end)
+        return self.norm(x), ends
+
+    def forward(self, tokens, target, lengths=None):
+        return self.head(self.hidden(tokens, None, lengths)[0], target)
+
+    @torch.no_grad()
+    def generate(self, tokens, count):
+        """The likeliest ``count`` tokens behind ``tokens`` [B, T], one at a time."""
+        hidden, states = self.hidden(tokens)
+        made = []
+        for _ in range(count):
+            made.append(self.head.logits(hidden[:, -1:]).argmax(-1))
+            hidden, states = self.hidden(made[-1], states)
+        return torch.cat(made, 1) if made else tokens[:, :0]
+
+
 def batch(tokens, vocabulary, device, generator, noise=0.1, ignored=0.05):
     """Pairs of tokens and what follows them; a few targets are not to be counted."""
     pair = torch.randint(0, vocabulary, (tokens, 2), generator=generator, device=device)
@@ -47,6 +111,42 @@ def batch(tokens, vocabulary, device, generator, noise=0.1, ignored=0.05):
     draw = torch.rand(tokens, generator=generator, device=device)
     target = torch.where(draw < noise, shuffled, target)
     return pair, torch.where(draw > 1 - ignored, torch.full_like(target, -100), target)
+
+
+def sequences(count, length, vocabulary, device, generator, noise=0.1):
+    """Ragged sequences, what follows each token (by itself and the one before it), and the lengths; targets behind a sequence's end
+    are not to be counted."""
+    tokens, target = batch(count * length, vocabulary, device, generator, noise, ignored=0.0)
+    tokens = tokens[:, 0].view(count, length)
+    before = torch.nn.functional.pad(tokens, (1, 0))[:, :-1]
+    true = (tokens // 3 + before // 5) % vocabulary
+    shuffled = torch.rand(count, length, generator=generator, device=device) < noise
+    target = torch.where(shuffled, target.view(count, length), true)
+    lengths = torch.randint((length + 1) // 2, length + 1, (count,), generator=generator, device=device)
+    inside = torch.arange(length, device=device) < lengths[:, None]
+    return tokens, torch.where(inside, target, -100), lengths
+
+
+def best_words(teacher, tokens, target, lengths, words):
+    """Numbers and logits [B, T, words] of a teacher's best words, none for tokens whose target does not count."""
+    with torch.no_grad():
+        best = teacher.head.logits(teacher.hidden(tokens, None, lengths)[0]).topk(words, -1)
+        return torch.where((target == -100)[..., None], -1, best.indices), best.values
+
+
+def sequence_step(model, optimizer, tokens, target, lengths, max_norm, teacher=None, words=0, temperature=2.0):
+    """One step, half of whose loss is the distance from a teacher where there is one; returns the targets' loss and the gradients'
+    norm before clipping, both on the device."""
+    optimizer.zero_grad(set_to_none=True)
+    hidden, _ = model.hidden(tokens, None, lengths)
+    loss = total = model.head(hidden, target)
+    if teacher is not None:
+        ids, logits = best_words(teacher, tokens, target, lengths, words)
+        total = 0.5 * loss + 0.5 * model.head.distill(hidden, ids, logits, temperature)
+    total.backward()
+    norm = training.clip_grad_norm_(model.parameters(), max_norm)
+    optimizer.step()
+    return loss.detach(), norm
 
 
 def train_step(model, optimizer, pair, target, max_norm):
@@ -70,29 +170,48 @@ def main(argv=None):
     parser.add_argument("--weight-bits", type=int, default=5)
     parser.add_argument("--lr", type=float, default=2e-3)
     parser.add_argument("--max-norm", type=float, default=1.0)
+    parser.add_argument("--sequence", type=int, default=0, help="train on sequences of up to so many tokens")
+    parser.add_argument("--teach", type=int, default=0, help="how many words of a teacher's to learn from (with --sequence)")
+    parser.add_argument("--temperature", type=float, default=2.0, help="of the teacher")
     parser.add_argument("--seed", type=int, default=0)
     args = parser.parse_args(argv)
     if args.width % 2 or min(args.steps, args.tokens, args.vocabulary, args.width) < 1:
         parser.error("width has to be even, and all sizes positive")
+    if not 0 <= args.sequence <= args.tokens:
+        parser.error("a sequence has at most as many tokens as a step")
+    if not 0 <= args.teach <= min(args.vocabulary, 1024) or (args.teach and not args.sequence):
+        parser.error("a teacher needs sequences, and has at most 1024 words, and the vocabulary's")
     if not torch.cuda.is_available():
         parser.error("training needs a GPU")
     device = torch.device("cuda", torch.cuda.current_device())
     torch.manual_seed(args.seed)
     generator = torch.Generator(device=device).manual_seed(args.seed)
+    kind = SequenceModel if args.sequence else TokenModel
+    teacher = None
     with device:
-        model = TokenModel(args.vocabulary, args.width, args.depth, args.shift_type, args.weight_bits)
+        model = kind(args.vocabulary, args.width, args.depth, args.shift_type, args.weight_bits)
+        if args.teach:
+            teacher = kind(args.vocabulary, 2 * args.width, args.depth, args.shift_type, args.weight_bits)
+            its_optimizer = torch.optim.Adam(teacher.parameters(), lr=args.lr)
     optimizer = torch.optim.Adam(model.parameters(), lr=args.lr)
     first = loss = None
     start = time.perf_counter()
     for step in range(args.steps):
-        pair, target = batch(args.tokens, args.vocabulary, device, generator)
-        loss, norm = train_step(model, optimizer, pair, target, args.max_norm)
+        if args.sequence:
+            data = sequences(args.tokens // args.sequence, args.sequence, args.vocabulary, device, generator)
+            if teacher is not None:
+                sequence_step(teacher, its_optimizer, *data, args.max_norm)
+            loss, norm = sequence_step(model, optimizer, *data, args.max_norm, teacher, args.teach, args.temperature)
+        else:
+            pair, target = batch(args.tokens, args.vocabulary, device, generator)
+            loss, norm = train_step(model, optimizer, pair, target, args.max_norm)
         first = loss if first is None else first
         if step % 10 == 0 or step == args.steps - 1:
             print("step %4d  loss %.4f  norm %.3f" % (step, loss.item(), norm.item()), flush=True)
     torch.cuda.synchronize()
     took = time.perf_counter() - start
-    print("%.0f tokens/s" % (args.steps * args.tokens / took))
+    tokens = args.tokens // args.sequence * args.sequence if args.sequence else args.tokens
+    print("%.0f tokens/s" % (args.steps * tokens / took))
     return first.item(), loss.item()
 
 

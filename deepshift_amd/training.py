@@ -1,13 +1,14 @@
-"""Operators of a token model's training step around shift layers: the scaled embedding lookup at its entrance, the cross
-entropy of a linear head over a large vocabulary at its exit, and the clipping of gradients by their global norm.
+"""Operators of a token model's training step around shift layers: the scaled embedding lookup at its entrance, the gated
+recurrence that mixes a sequence's tokens and the gated block of a feed-forward layer between, the cross entropy of a linear head
+over a large vocabulary, and its distance from a teacher's best words, at its exit, and the clipping of gradients by their global
+norm.
 
 The layers between are ``LinearShift`` / ``LinearShiftQ`` on their float path, whose straight-through gradients
 (``ste.py``) reach shifts and signs unscaled -- the reason to clip them.  Everything here runs in the gfx950 library, on the
 current stream of the tensors' device, on float32, bfloat16 and float16; sums are held in 32 bits or more and rounded once,
 and a call repeats bit for bit.  There is no CPU path: a CPU tensor raises.
 
-Functions whose names end in ``_grad`` return gradients directly; ``embedding`` and ``linear_cross_entropy`` also take part
-in autograd.
+Functions whose names end in ``_grad`` return gradients directly; the others, but for the clipping, take part in autograd.
 """
 import contextlib
 

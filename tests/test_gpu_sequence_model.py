@@ -1,0 +1,128 @@
+"""GPU: the recurrence, the gated block and the distillation together, as deepshift_amd.train_tokens uses them."""
+import pytest
+import torch
+import torch.nn.functional as F
+
+from deepshift_amd import train_tokens, training
+
+pytestmark = pytest.mark.gpu
+DEV = torch.device("cuda:0")
+
+
+def _plain_layer(layer, x, inside):
+    """The layer's own weights, everything else in 64 bits, token by token."""
+    def linear(part, v):
+        return F.linear(v, part.float_weight().double(), part.bias.double())
+
+    def norm(part, v):
+        return F.layer_norm(v, part.normalized_shape, part.weight.double(), part.bias.double(), part.eps)
+
+    value, gate = linear(layer.enter, norm(layer.norms[0], x)).chunk(2, -1)
+    h, steps = torch.zeros_like(value[:, 0]), []
+    for t in range(x.shape[1]):
+        a = gate[:, t].sigmoid()
+        h = torch.where(inside[:, t, None], a * h + (1 - a) * value[:, t], h)
+        steps.append(torch.where(inside[:, t, None], h, 0.0))
+    x = x + linear(layer.leave, torch.stack(steps, 1))
+    g, u = linear(layer.gated.layer, norm(layer.norms[1], x)).chunk(2, -1)
+    return x + linear(layer.down, F.silu(g) * u), h
+
+
+def _plain_loss(model, tokens, target, lengths, ids, logits, c):
+    inside = torch.arange(tokens.shape[1], device=DEV) < lengths[:, None]
+    x = model.embedding.weight.double()[tokens] * model.embedding.scale
+    for layer in model.layers:
+        x, _ = _plain_layer(layer, x, inside)
+    x = F.layer_norm(x, model.norm.normalized_shape, model.norm.weight.double(), model.norm.bias.double(), model.norm.eps)
+    z = F.linear(x, model.head.weight.double(), model.head.bias.double())
+    hard = F.cross_entropy(z.flatten(0, 1), target.flatten())
+    there = ids >= 0
+    kept = there.any(-1)
+    q = torch.where(there, logits.double() / c, -1e300).softmax(-1) * there
+    logp = (z / c).log_softmax(-1).gather(-1, ids.clamp(min=0))
+    soft = c * c * torch.where(there, q * (q.clamp(min=1e-300).log() - logp), 0.0).sum() / kept.sum()
+    return 0.5 * hard + 0.5 * soft
+
+
+def test_a_step_has_the_gradients_of_its_formula():
+    torch.manual_seed(0)
+    generator = torch.Generator(device=DEV).manual_seed(1)
+    V, c = 90, 2.0
+    with DEV:
+        model, teacher = train_tokens.SequenceModel(V, 32, 2), train_tokens.SequenceModel(V, 64, 1)
+    tokens, target, lengths = train_tokens.sequences(5, 33, V, DEV, generator)
+    assert ((target == -100).sum(1) == 33 - lengths).all() and (lengths < 33).any()
+    ids, logits = train_tokens.best_words(teacher, tokens, target, lengths, 7)
+    assert ids.shape == (5, 33, 7) and ((ids < 0).all(-1) == (target == -100)).all()
+    hidden, _ = model.hidden(tokens, None, lengths)
+    loss = 0.5 * model.head(hidden, target) + 0.5 * model.head.distill(hidden, ids, logits, c)
+    got = torch.autograd.grad(loss, list(model.parameters()))
+    # the same weights, in 64 bits
+    want_loss = _plain_loss(model, tokens, target, lengths, ids, logits, c)
+    want = torch.autograd.grad(want_loss, list(model.parameters()))
+    assert abs(loss.double() - want_loss) <= 1e-5 * abs(want_loss)
+    for (name, _), p, q in zip(model.named_parameters(), got, want):
+        # float32 through some thirty operations with conditions of some hundreds: 2^-24 * 30 * 500 of the gradient's norm
+        assert (p.double() - q.double()).norm() <= 1e-3 * q.double().norm() + 1e-9, name
+
+
+def test_tokens_one_by_one_are_the_sequence():
+    torch.manual_seed(1)
+    with DEV:
+        model = train_tokens.SequenceModel(70, 48, 2)
+    tokens = torch.randint(0, 70, (3, 20), device=DEV)
+    with torch.no_grad():
+        whole, ends = model.hidden(tokens)
+        states, steps = None, []
+        for t in range(20):
+            hidden, states = model.hidden(tokens[:, t:t + 1], states)
+            steps.append(hidden)
+        # two orders of the same float32 sums, behind norms of size 1
+        assert torch.allclose(torch.cat(steps, 1), whole, rtol=0, atol=1e-3)
+        for p, q in zip(states, ends):
+            assert p.dtype == torch.float32 and torch.allclose(p, q, rtol=1e-3, atol=1e-3)
+    made = model.generate(tokens, 5)
+    assert made.shape == (3, 5) and model.generate(tokens, 0).shape == (3, 0)
+    logits = model.head.logits(whole[:, -1])
+    assert (logits.gather(1, made[:, :1])[:, 0] >= logits.amax(1) - 1e-2).all()
+
+
+@pytest.mark.parametrize("shift_type", ["PS", "Q"])
+def test_the_command_runs(shift_type):
+    losses = train_tokens.main(["--steps", "3", "--tokens", "600", "--sequence", "50", "--teach", "5", "--vocabulary", "64", "--width", "32",
+                                "--depth", "1", "--shift-type", shift_type])
+    assert all(0 < loss < 20 for loss in losses)
+    assert all(0 < loss < 20 for loss in train_tokens.main(["--steps", "2", "--tokens", "300", "--sequence", "30", "--vocabulary", "64",
+                                                            "--width", "32"]))
+
+
+def test_a_step_can_be_captured():
+    torch.manual_seed(2)
+    generator = torch.Generator(device=DEV).manual_seed(3)
+    with DEV:
+        model, teacher = train_tokens.SequenceModel(80, 32, 1), train_tokens.SequenceModel(80, 32, 1)
+    data = train_tokens.sequences(4, 24, 80, DEV, generator)
+
+    def step():
+        tokens, target, lengths = data
+        hidden, _ = model.hidden(tokens, None, lengths)
+        ids, logits = train_tokens.best_words(teacher, tokens, target, lengths, 6)
+        loss = model.head(hidden, target) + model.head.distill(hidden, ids, logits)
+        return [loss.detach()] + list(torch.autograd.grad(loss, list(model.head.parameters()) + list(model.layers[0].gated.parameters())))
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured = step()
+    for i in range(3):
+        for kept, new in zip(data, train_tokens.sequences(4, 24, 80, DEV, generator)):
+            kept.copy_(new)
+        graph.replay()
+        torch.cuda.synchronize()
+        for p, q in zip(captured, step()):
+            # the library's part repeats bit for bit; torch's own products may take other kernels under capture
+            assert (p - q).norm() <= 1e-4 * q.norm() + 1e-6, "replay %d" % i
