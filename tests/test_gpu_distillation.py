@@ -330,6 +330,50 @@ def test_layouts(dtype):
     assert one.shape == () and torch.equal(one, training.linear_distillation(h[:1], w, ids[:1], logits[:1], b, reduction="none")[0])
 
 
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+def test_many_words_of_one_tile(dtype):
+    # more of them than a tile keeps at hand, neighbours and the same ones again, and more than there are
+    T, D, V = 40, 48, 700
+    for K, low, high in ((40, 100, 160), (9, 250, 262), (64, 640, 700), (50, 0, 7)):
+        h, w, b, _, logits = _case(T, D, V, K, dtype, True, 20)
+        ids = torch.randint(low, high, (T, K), generator=_gen(21, K)).to(DEV)
+        ids[5] = -1
+        ones = torch.ones(T, device=DEV)
+        for tune in (dict(), dict(vocab_piece_kb=1)):
+            for tile in (None, 0, 1, 2, 3):
+                with Tune(vocab_tile=tile, **tune):
+                    rows = training.linear_distillation(h, w, ids, logits, b, 1.3, "none")
+                    step = training.linear_distillation_grad(h, w, ids, logits, b, 1.3, "sum")
+                    got = _autograd(h, w, ids, logits, b, 1.3, "sum")
+                _check(h, w, b, ids, logits, 1.3, ones, rows, *step[1:])
+                _check(h, w, b, ids, logits, 1.3, ones, rows, *got[1:])
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+def test_temperatures_at_both_ends(dtype):
+    T, D, V, K = 30, 40, 300, 8
+    h, w, b, ids, logits = _case(T, D, V, K, dtype, True, 22)
+    ones = torch.ones(T, device=DEV)
+    for c in (2.0 ** 20, 1000.0, 0.03, 2.0 ** -20):
+        rows = training.linear_distillation(h, w, ids, logits, b, c, "none")
+        step = training.linear_distillation_grad(h, w, ids, logits, b, c, "sum")
+        # float16 ends at 65504, and gradients are 2^20 (p - q) w there
+        beyond = c > 1e6 and dtype == torch.float16
+        assert not any(t.isnan().any() for t in step) and (beyond or all(t.isfinite().all() for t in step))
+        _check(h, w, b, ids, logits, c, ones, rows, *(() if beyond else step[1:]))
+
+
+def test_many_tokens():
+    for dtype in TYPES:
+        T, D, V, K = 70001, 16, 50, 3
+        h, w, b, ids, logits = _case(T, D, V, K, dtype, True, 23)
+        n = int((ids >= 0).any(1).sum())
+        rows = training.linear_distillation(h, w, ids, logits, b, 2.0, "none")
+        step = training.linear_distillation_grad(h, w, ids, logits, b, 2.0)
+        want, bound = _check(h, w, b, ids, logits, 2.0, torch.full((T,), 1.0 / n, device=DEV), rows, *step[1:])
+        assert abs(step[0].double() - want.sum() / n) <= (bound.sum() + 4 * E * want.abs().sum()) / n
+
+
 def test_gradients_against_differences():
     T, D, V, K, c = 20, 16, 50, 6, 1.7
     h, w, b, ids, logits = _case(T, D, V, K, torch.float32, True, 15)

@@ -268,6 +268,20 @@ def test_gradients_against_differences():
             assert abs(along - slope) <= 1000 * E * (got[1 + i].double().abs() * way.abs()).sum() + 1e-6 * abs(slope) + 1e-6
 
 
+def test_many_tokens():
+    for dtype in TYPES:
+        T, D, F = 70001, 16, 24
+        x, w, b, grad = _case(T, D, F, dtype, True, 12)
+        _check(x, w, b, "silu", grad, *_step(x, w, b, "silu", grad))
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+def test_a_few_tokens_of_shared_memory(dtype):
+    x, w, b, grad = _case(3, 64, 40, dtype, True, 13)
+    for x2, w2 in ((x[:1].expand(3, 64), w), (x, w[:1].expand(80, 64)), (x.t().contiguous().t(), w.t().contiguous().t())):
+        _check(x2, w2, b, "gelu", grad, *_step(x2, w2, b, "gelu", grad))
+
+
 def test_empty_sizes():
     for T, D, F in ((0, 8, 4), (5, 0, 4), (5, 8, 0), (0, 0, 0)):
         x, w, b = [torch.randn(*s, device=DEV, requires_grad=True) for s in ((T, D), (2 * F, D), (2 * F,))]
