@@ -26,13 +26,10 @@ namespace vocab {
 // bfloat16 take 75 us, element by element 176.
 // Rows whose target is `ignore` (where targets are given) become zeros: tokens that do
 // not count leave nothing in the weights' gradient, not even a value that is no number.  The first operand by `first` workgroups.
-template <typename E>
-__global__ __launch_bounds__(256) void pack_kernel(Pack one, Pack two, int first)
+template <typename E, typename COUNTS>
+__device__ __forceinline__ void pack_rows(const Pack &p, int block, int blocks, const COUNTS &counts)
 {
     constexpr int N = 16 / sizeof(E);
-    const bool is_one = (int)blockIdx.x < first;
-    const Pack &p = is_one ? one : two;
-    const int block = is_one ? blockIdx.x : blockIdx.x - first, blocks = is_one ? first : gridDim.x - first;
     const int units = p.Dp / N;
     const int64_t total = p.rows * units;
     for (int64_t i = (int64_t)block * 256 + threadIdx.x; i < total; i += (int64_t)blocks * 256) {
@@ -40,7 +37,7 @@ __global__ __launch_bounds__(256) void pack_kernel(Pack one, Pack two, int first
         const int c = (int)(i - r * units) * N;
         const E *x = (const E *)p.x + r * p.ld;
         Vec<E, N> v{};
-        if (p.target && (p.wide ? ((const int64_t *)p.target)[r] : (int64_t)((const int32_t *)p.target)[r]) == p.ignore) {
+        if (!counts(r)) {
         } else if (c + N <= p.D) __builtin_memcpy(&v, x + c, sizeof(v));  // wherever it lies
         else
 #pragma unroll
@@ -65,13 +62,27 @@ __global__ __launch_bounds__(256) void pack_kernel(Pack one, Pack two, int first
 }
 
 template <typename E>
+__global__ __launch_bounds__(256) void pack_kernel(Pack one, Pack two, int first)
+{
+    const bool is_one = (int)blockIdx.x < first;
+    const Pack &p = is_one ? one : two;
+    const void *const target = p.target;
+    const int wide = p.wide;
+    const int64_t ignore = p.ignore;
+    pack_rows<E>(p, is_one ? blockIdx.x : blockIdx.x - first, is_one ? first : gridDim.x - first, [=](int64_t r) {
+        return !target || (wide ? ((const int64_t *)target)[r] : (int64_t)((const int32_t *)target)[r]) != ignore;
+    });
+}
+
+template <typename E> int pack_blocks(const Pack &p)
+{
+    const int64_t b = (p.rows * (p.Dp / (16 / (int)sizeof(E))) + 255) / 256;
+    return (int)(b < 8192 ? b : 8192);
+}
+template <typename E>
 int launch_pack(const Pack &one, const Pack &two, hipStream_t st)
 {
-    auto blocks = [](const Pack &p) {
-        const int64_t b = (p.rows * (p.Dp / (16 / (int)sizeof(E))) + 255) / 256;
-        return (int)(b < 8192 ? b : 8192);
-    };
-    const int first = blocks(one), all = first + blocks(two);
+    const int first = pack_blocks<E>(one), all = first + pack_blocks<E>(two);
     if (all == 0) return DS_OK;
     hipLaunchKernelGGL((pack_kernel<E>), dim3(all), dim3(256), 0, st, one, two, first);
     return launch_status();
@@ -480,22 +491,29 @@ struct Teacher {
 };
 constexpr int kMostTaught = 1024;
 
+// What stands at a place: a word's number, below 0 where there is none, and its logit.
+__device__ __forceinline__ int64_t word_at(const Teacher &f, int64_t at, float &logit)
+{
+    const int64_t word = f.wide ? ((const int64_t *)f.ids)[at] : (int64_t)((const int32_t *)f.ids)[at];
+    logit = f.type == DS_F32 ? ((const float *)f.logits)[at]
+            : f.type == DS_BF16 ? to_float(((const bf16_t *)f.logits)[at]) : to_float(((const f16_t *)f.logits)[at]);
+    return logit == -INFINITY ? -1 : word;
+}
+
 // Probabilities of a token's words, in the order of their numbers: a workgroup has a token, a thread a word, whose place is how
 // many come before it (the comparisons of 64 words take less time than their loads: 8192 tokens in 12 us).
-__global__ __launch_bounds__(kMostTaught) void teacher_kernel(Teacher f)
+template <int MOST>
+__device__ __forceinline__ void teach(const Teacher &f, int64_t t)
 {
-    __shared__ int ids[kMostTaught];
-    __shared__ float tops[16], sums[16];
-    __shared__ int found[16];
+    __shared__ int ids[MOST];
+    __shared__ float tops[MOST / 64], sums[MOST / 64];
+    __shared__ int found[MOST / 64];
     const int k = threadIdx.x, wave = k >> 6, lane = k & 63, waves = blockDim.x >> 6;
-    const int64_t t = blockIdx.x, at = t * f.K + k;
     int id = 0x7fffffff, seen = 0;  // 1: a word, 2: something that is none, or no number
     float logit = -INFINITY;
     if (k < f.K) {
-        const int64_t word = f.wide ? ((const int64_t *)f.ids)[at] : (int64_t)((const int32_t *)f.ids)[at];
-        logit = f.type == DS_F32 ? ((const float *)f.logits)[at]
-                : f.type == DS_BF16 ? to_float(((const bf16_t *)f.logits)[at]) : to_float(((const f16_t *)f.logits)[at]);
-        if (word < 0 || logit == -INFINITY) logit = -INFINITY;
+        const int64_t word = word_at(f, t * f.K + k, logit);
+        if (word < 0) logit = -INFINITY;
         else if (word >= f.V || !(logit < INFINITY)) logit = -INFINITY, seen = 3;
         else id = (int)word, seen = 1;
     }
@@ -519,6 +537,28 @@ __global__ __launch_bounds__(kMostTaught) void teacher_kernel(Teacher f)
     if (k < f.K) f.sorted[t * f.K + place] = id, f.taught[t * f.K + place] = id == 0x7fffffff ? 0.f : e / sum;
     if (k == 0) f.target[t] = seen == 0 ? -1 : seen & 2 ? (int)f.V : 0;
     if (k == 0 && t == 0) *f.factor = f.temperature;
+}
+__global__ __launch_bounds__(kMostTaught) void teacher_kernel(Teacher f) { teach<kMostTaught>(f, blockIdx.x); }
+
+// Operands too, in one launch, up to kTaughtBeside tokens of 256 words (one of five to eight that a small call takes; of many tokens
+// waves without words would cost more): hidden states look for themselves whether a token has any.
+constexpr int kTaughtBeside = 1024;
+template <typename E>
+__global__ __launch_bounds__(256) void teacher_pack_kernel(Teacher f, Pack one, Pack two, int first)
+{
+    const int block = blockIdx.x - (int)f.T;
+    if (block < 0) {
+        teach<256>(f, blockIdx.x);
+    } else if (block < first) {
+        pack_rows<E>(one, block, first, [&](int64_t r) {
+            bool any = !one.target;
+            float logit;
+            for (int k = 0; k < f.K && !any; ++k) any = word_at(f, r * f.K + k, logit) >= 0;
+            return any;
+        });
+    } else {
+        pack_rows<E>(two, block - first, gridDim.x - (int)f.T - first, [](int64_t) { return true; });
+    }
 }
 
 // ---- joins -------------------------------------------------------------------------------------------------------
@@ -725,12 +765,18 @@ inline int check(const Call &c)
     return DS_OK;
 }
 
+inline void launch_teacher(const Teacher &t, hipStream_t st)
+{
+    hipLaunchKernelGGL(teacher_kernel, dim3((unsigned)t.T), dim3(ceil_div(t.K, 64) * 64), 0, st, t);
+}
+
 // The operands as the products take them: hidden states once, weights piece by piece.
 template <typename P>
 struct Operands {
     Operand h, w;
     int64_t w_at = -1;
     bool h_there = false;
+    bool untaught = false;   // the teacher's words are still to be put in order
 
     int prepare(const Call &c, const Plan &p, bool counted_only, int64_t v0, int64_t n)
     {
@@ -748,6 +794,16 @@ struct Operands {
             w = p.pack_w ? Operand{c.ws + p.w, p.ldd} : Operand{from, c.ldw};
             if (p.pack_w) pw = Pack{from, c.ldw, n, (int)c.D, p.Dp, (uint16_t *)(c.ws + p.w), p.ldd, nullptr, 0, 0};
             w_at = v0;
+        }
+        if (untaught) {
+            untaught = false;
+            const Teacher &t = c.teacher;
+            const int first = pack_blocks<E>(ph), all = first + pack_blocks<E>(pw);
+            if (all > 0 && t.K <= 256 && t.T <= kTaughtBeside) {
+                hipLaunchKernelGGL((teacher_pack_kernel<E>), dim3((unsigned)t.T + all), dim3(256), 0, c.st, t, ph, pw, first);
+                return launch_status();
+            }
+            launch_teacher(t, c.st);
         }
         return launch_pack<E>(ph, pw, c.st);
     }
@@ -961,9 +1017,12 @@ int run(Call c, int what, const Outputs &out)
         t.target = (int *)(c.ws + p.target), t.factor = (float *)(c.ws + p.temperature);
         // from here on tokens without a word are those that do not count
         c.target = t.target, c.wide = 0, c.ignore = -1;
-        if (c.T > 0) hipLaunchKernelGGL(teacher_kernel, dim3((unsigned)c.T), dim3(ceil_div(t.K, 64) * 64), 0, c.st, t);
     }
     Operands<P> o;
+    if (c.teacher.K && c.T > 0) {
+        if (what & kLoss) o.untaught = true;
+        else launch_teacher(c.teacher, c.st);
+    }
     Rows of{};
     if (what & kLoss) DS_TRY(loss<P>(c, p, what & kGrad, o, out.reduction, out.rows, out.lse, out.total, &of));
     if (what & kGrad) DS_TRY(loss_grad<P>(c, p, o, of, out.grads));

@@ -262,6 +262,20 @@ def test_places_without_words_and_tokens_that_do_not_count(dtype):
 
 
 @pytest.mark.parametrize("dtype", TYPES, ids=str)
+def test_empty_places_in_front(dtype):
+    for T, K in ((60, 9), (60, 300), (1100, 9)):
+        h, w, b, ids, logits = _case(T, 40, 400, K, dtype, True, 24)
+        ids = torch.randint(0, 400, (T, K), generator=_gen(25, K)).to(DEV)
+        ids[::2, :K - 1], logits[1::4, :K - 2] = -1, -float("inf")
+        ids[3::8] = -1
+        n = int(((ids >= 0) & (logits > -float("inf"))).any(1).sum())
+        rows = training.linear_distillation(h, w, ids, logits, b, 2.0, "none")
+        step = training.linear_distillation_grad(h, w, ids, logits, b, 2.0)
+        assert n < T
+        _check(h, w, b, ids, logits, 2.0, torch.full((T,), 1.0 / n, device=DEV), rows, *step[1:])
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
 def test_what_is_no_number_or_no_word_stays_in_its_token(dtype):
     T, D, V, K = 30, 40, 300, 6
     h, w, b, ids, logits = _case(T, D, V, K, dtype, True, 10)
