@@ -295,8 +295,8 @@ int operands(const Call &c, const Plan &p, Operand &x, Operand &w)
     x = p.pack_x ? Operand{c.ws + p.x, p.ldd} : Operand{c.x, c.ldx};
     w = p.pack_w ? Operand{c.ws + p.w, p.ldd} : Operand{c.weight, c.ldw};
     if (c.D == 0) return DS_OK;
-    if (p.pack_x) px = Pack{c.x, c.ldx, c.T, (int)c.D, p.Dp, (uint16_t *)(c.ws + p.x), p.ldd, nullptr, 0, 0};
-    if (p.pack_w) pw = Pack{c.weight, c.ldw, 2 * c.F, (int)c.D, p.Dp, (uint16_t *)(c.ws + p.w), p.ldd, nullptr, 0, 0};
+    if (p.pack_x) px = Pack{c.x, c.ldx, c.T, (int)c.D, p.Dp, (uint16_t *)(c.ws + p.x), p.ldd, nullptr, 0, 0, 0};
+    if (p.pack_w) pw = Pack{c.weight, c.ldw, 2 * c.F, (int)c.D, p.Dp, (uint16_t *)(c.ws + p.w), p.ldd, nullptr, 0, 0, 0};
     return launch_pack<E>(px, pw, c.st);
 }
 

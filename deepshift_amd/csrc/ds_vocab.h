@@ -163,6 +163,10 @@ struct Args {
     const float *taught;
     int taught_words;
     float warmth;
+    // bfloat16: for groups of 256 words that `twice` marks (all, where it is NULL) what P loses by its rounding stands `again` rows
+    // behind it.  In the weights' gradient (kOut) those groups have both in a reduction twice as long.
+    const uint8_t *twice;
+    int64_t again;
     // kGate (bias, out and ldo too): M is half of A's rows
     int64_t half_bytes;   // from the first half to the second
     int activation;
@@ -597,6 +601,13 @@ __device__ __forceinline__ int spread_sums(float (&v)[ALL], int lane)
     }
 }
 
+// What a value loses when it is rounded to bfloat16; nothing of what is no number.
+__device__ __forceinline__ float rounding_of(float v)
+{
+    const float off = v - to_float(from_float<bf16_t>(v));
+    return fabsf(off) < INFINITY ? off : 0.f;
+}
+
 // One tile of a product, by a whole workgroup; `block` counts the product's workgroups.
 //
 // Operands go from memory to LDS without registers, two stages and more ahead; a wave holds up to 128 x 64 results.  Fragments
@@ -623,7 +634,10 @@ __device__ __forceinline__ void product_tile(const Args &g, const int block, cha
     int tm, tn, split;
     tile_of(block, g.tiles_m, g.tiles_n, g.splits, &tm, &tn, &split);
     const int m0 = tm * (kPaired ? BM / 2 : BM), n0 = tn * BN;
-    const int k_from = split * g.k_split, k_to = min(g.K, k_from + g.k_split);
+    int K = g.K, k_split = g.k_split;
+    if constexpr (NP == 1 && KIND == kOut)
+        if (g.twice && g.twice[(g.v0 + n0) / 256]) K *= 2, k_split *= 2;
+    const int k_from = split * k_split, k_to = min(K, k_from + k_split);
     const int steps = (k_to - k_from + kStep - 1) / kStep;
 
     TA ta;
@@ -1076,7 +1090,7 @@ __device__ __forceinline__ void product_tile(const Args &g, const int block, cha
             }
         }
     };
-    auto leave_prob = [&](int j) {
+    auto leave_prob = [&](int j, int64_t later = 0) {
         __syncthreads();
         if constexpr (NP == 1 && KIND == kKeep) {
             Gather<float, BM>::template leave<kThreads>(lds, kRowsOut, g.prob_words - m0, [&](int row) -> float * {
@@ -1087,7 +1101,7 @@ __device__ __forceinline__ void product_tile(const Args &g, const int block, cha
             constexpr int kFilled = KIND == kKeep ? 64 : 96;  // of three planes' place
             Gather<uint16_t, BM * NP>::template leave<kThreads, kFilled, 96>(lds, kRowsOut, (g.prob_words - m0) * NP, [&](int row) -> uint16_t * {
                 const int t = n0 + n_of(row, j);
-                return t < g.N ? (uint16_t *)g.prob + t * g.ldp + m0 * NP : nullptr;
+                return t < g.N ? (uint16_t *)g.prob + (t + later) * g.ldp + m0 * NP : nullptr;
             });
         }
         __syncthreads();
@@ -1229,10 +1243,22 @@ __device__ __forceinline__ void product_tile(const Args &g, const int block, cha
                 for (int r = 0; r < 4; ++r) {
                     p[r] = counts ? p[r] * scale : 0.f;
                     over_n[I * 4 + r] += p[r] * power;
+                    if constexpr (TAUGHT && NP == 1) acc[I / U::groups][j][I % U::groups * 4 + r] = p[r];
                 }
                 put_prob(I, p);
             }
             leave_prob(j);
+            if constexpr (TAUGHT && NP == 1 && !P::half)
+                if (g.again && (!g.twice || g.twice[(g.v0 + m0) / 256])) {
+#pragma unroll
+                    for (int I = 0; I < MG; ++I) {
+                        float rest[4];
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) rest[r] = rounding_of(value(I, j, r));
+                        put_prob(I, rest);
+                    }
+                    leave_prob(j, g.again);
+                }
         }
         if (g.bias_part || g.bias_out) {
             typedef typename ElementOf<P>::type E;

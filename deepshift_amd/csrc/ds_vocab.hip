@@ -46,6 +46,7 @@ __device__ __forceinline__ void pack_rows(const Pack &p, int block, int blocks, 
         uint16_t *row = p.out + r * p.ldo;
         if constexpr (sizeof(E) == 2) {
             *(Vec<E, N> *)(row + c) = v;
+            if (p.again) *(Vec<E, N> *)(row + p.again * p.ldo + c) = v;
         } else {
             Vec<bf16_t, N> q[3];
 #pragma unroll
@@ -185,13 +186,73 @@ __device__ __forceinline__ void add_to_total(const Rows &r, double loss, double 
     if (lane == 0) write_total(loss, counted, r.reduction == DS_MEAN, r.total, r.temperature);
 }
 
+// ---- a teacher's heavy words ----------------------------------------------------------------------------------------
+//
+// P is rounded to the operands' type for the gradients' products.  Its own column's size is what a row of the weights' gradient is
+// off by then, and words that most tokens teach have columns hundreds of times larger than others: of bfloat16 single values were
+// off by half of the whole gradient's root mean square (8192 tokens, 64 of 65536 words, as often as text has them).  So P keeps its
+// rounding's remainder for groups of 256 words that hold such a word, and the weights' gradient takes both (0.03 of it then): a
+// handful of 256 groups, and a step of 10.9 ms takes 11.2.  Up to kTwiceAll tokens all groups have it, which costs nothing beside the weights; words
+// of a vocabulary up to kNoneHeavy move too little, and a single word's P is near -1, which rounds to itself.
+constexpr int64_t kTwiceAll = 64, kNoneHeavy = 4096;
+
+struct Marks {
+    const int *sorted;
+    const float *taught;
+    int64_t T, V;
+    int K;
+    uint8_t *twice;      // [groups of 256 words]
+};
+
+// By one workgroup, while others join the rows: of up to 512 tokens and 16384 words, evenly spread, the words' sums of squared probabilities, whole numbers of 2^-20 by a hash
+// of the word; a sum that is a hundred-and-twenty-eighth of all marks the group of its likeliest word.
+__device__ __forceinline__ void mark_heavy(const Marks &m)
+{
+    constexpr int kBuckets = 4096;
+    __shared__ uint32_t sums[kBuckets];
+    __shared__ unsigned long long likeliest[kBuckets];
+    __shared__ unsigned long long all;
+    for (int i = threadIdx.x; i < kBuckets; i += blockDim.x) sums[i] = 0, likeliest[i] = 0;
+    if (threadIdx.x == 0) all = 0;
+    const int64_t groups = (m.V + 255) / 256;
+    for (int64_t i = threadIdx.x; i < groups; i += blockDim.x) m.twice[i] = 0;
+    __threadfence();
+    __syncthreads();
+    const int64_t most = min((int64_t)512, (int64_t)16384 / m.K), step = (m.T + most - 1) / most, places = (m.T + step - 1) / step * m.K;
+    unsigned long long mine = 0;
+#pragma unroll 4
+    for (int64_t i = threadIdx.x; i < places; i += blockDim.x) {
+        const int64_t at = i / m.K * step * m.K + i % m.K;
+        const float q = m.taught[at];
+        const uint32_t id = (uint32_t)m.sorted[at], sum = (uint32_t)(q * q * 0x1p20f);
+        if (sum == 0) continue;
+        const uint32_t bucket = id * 2654435761u >> 20;
+        atomicAdd(&sums[bucket], sum);
+        atomicMax(&likeliest[bucket], (unsigned long long)__float_as_uint(q) << 32 | id);
+        mine += sum;
+    }
+    atomicAdd(&all, mine);
+    __syncthreads();
+    for (int i = threadIdx.x; i < kBuckets; i += blockDim.x)
+        if (sums[i] && sums[i] * 128ull >= all) m.twice[(uint32_t)likeliest[i] / 256] = 1;
+}
+__global__ __launch_bounds__(1024) void mark_kernel(Marks m) { mark_heavy(m); }
+
 // Joins the tiles' maxima and sums: a workgroup has kRowsJoined rows, each of its waves a sixteenth of the tiles and each
 // quarter of a wave a quarter of those.  Bound by latency: 37 rows of 391 tiles in 4.4 us (18 with 64 rows a workgroup and a
 // wave's tiles one after the other), 8192 rows of 512 tiles, 34 MB, in 20.
 constexpr int kRowsJoined = 16;
 
-__global__ __launch_bounds__(1024) void row_kernel(Rows r)
+// MARK: the last workgroup marks a teacher's heavy words meanwhile.
+template <bool MARK>
+__global__ __launch_bounds__(1024) void row_kernel(Rows r, Marks m)
 {
+    const int groups = MARK ? gridDim.x - 1 : gridDim.x;
+    if constexpr (MARK)
+        if ((int)blockIdx.x == groups) {
+            mark_heavy(m);
+            return;
+        }
     __shared__ float tops[64][kRowsJoined], sums[64][kRowsJoined];
     const int row = threadIdx.x % kRowsJoined, part = threadIdx.x / kRowsJoined, t = blockIdx.x * kRowsJoined + row;
     float top = -INFINITY, sum = 0.f;
@@ -229,7 +290,7 @@ __global__ __launch_bounds__(1024) void row_kernel(Rows r)
         r.loss[t] = l;
         mine = l, counts = y != r.ignore;
     }
-    if (r.reduction) add_to_total(r, mine, counts, blockIdx.x, gridDim.x);
+    if (r.reduction) add_to_total(r, mine, counts, blockIdx.x, groups);
 }
 
 __global__ void no_rows_kernel(int mean, float *total) { write_total(0, 0, mean, total); }
@@ -312,6 +373,8 @@ struct Finish {
     void *bias_out;        // one workgroup has all rows: the gradient itself, of V words, or NULL
     const float *factor[2];
     const int *taught_ids; // TAUGHT: [T][words of a teacher], as Args has them
+    const uint8_t *twice;  // and these two
+    int64_t again;
 };
 // 64 rows, or 8 where that would leave CUs without work.
 inline int finish_rows(int64_t T, int64_t words) { return (T + 63) / 64 * ((words + 255) / 256) >= 2 * device_cus() ? 64 : 8; }
@@ -391,6 +454,7 @@ __global__ __launch_bounds__(256) void finish_kernel(Finish f)
     const float2 *tops = r.stats + (int64_t)(f.tile0 + (word < f.words ? word / f.tile : 0)) * r.T;
     uint16_t *const column = (uint16_t *)f.prob + (NP == 1 ? word : (word >> 5) * 96 + (word & 31));
     const float *const kept = f.kept + (NP == 1 ? word : (word >> 5) * 48 + (word & 31));
+    const bool both = f.again && (!f.twice || f.twice[f.v0 / 256 + blockIdx.x]);
 #pragma unroll JOIN || TAUGHT ? 1 : 4
     for (int i = 0; i < f.rows; i += 8) {
         const int t = blockIdx.y * f.rows + i + part;
@@ -460,6 +524,12 @@ __global__ __launch_bounds__(256) void finish_kernel(Finish f)
         }
 #pragma unroll
         for (int q = 0; q < NP; ++q) at[q * 4] = v[q];
+        if constexpr (TAUGHT && NP == 1 && !P::half)
+            if (both) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) v[0].v[e] = from_float<bf16_t>(rounding_of(p[e])).bits;
+                *(Vec<uint16_t, 8> *)(column + (t + f.again) * f.ldp) = v[0];
+            }
     }
     if (!f.bias_part && !f.bias_out) return;
 #pragma unroll
@@ -653,7 +723,8 @@ struct Plan {
     int words;            // of a piece's probabilities, a multiple of 32,
     int64_t ldp;          // and what a row of them takes
     size_t h, w, stats, picked, shares, arrived, prob, kept, bias, slices, acc, scale, power, factor, bytes;
-    size_t sorted, taught, target, temperature;  // a teacher's words
+    size_t sorted, taught, target, temperature, twice;  // a teacher's words
+    int again;            // the remainders of P are there: 1 for marked groups, 2 for all
 };
 
 template <typename P>
@@ -697,8 +768,11 @@ Plan plan_of(const void *hidden, int64_t ldh, const void *weight, int64_t ldw, i
     if (words) {
         p.sorted = take((size_t)T * words * 4), p.taught = take((size_t)T * words * 4);
         p.target = take((size_t)T * 4), p.temperature = take(4);
+        if (NP == 1 && !P::half && what & kGrad && words > 1 && V > kNoneHeavy) p.again = T <= kTwiceAll ? 2 : 1;
+        if (p.again == 1) p.twice = take((size_t)((V + 255) / 256));
     }
-    if (p.pack_h) p.h = take((size_t)T * p.ldd * 2);
+    const size_t copies = p.again ? 2 : 1;
+    if (p.pack_h) p.h = take(copies * T * p.ldd * 2);
     if (p.pack_w) p.w = take((size_t)p.piece * p.ldd * 2);
     if (what & kLoss) {
         const int64_t tiles = (p.piece + p.tile_words - 1) / p.tile_words;
@@ -724,7 +798,7 @@ Plan plan_of(const void *hidden, int64_t ldh, const void *weight, int64_t ldw, i
             }
             p.weight = choose<P>(D, p.piece, T, kGradShapes<P>, 64, false);
         }
-        p.prob = take((size_t)T * p.ldp * 2);
+        p.prob = take(copies * T * p.ldp * 2);
         // what a workgroup of either pass leaves of its rows
         const int kept_rows = finish_rows(T, p.words), rows = p.keep && kept_rows < p.tile_tokens ? kept_rows : p.tile_tokens;
         p.bias = take((size_t)((T + rows - 1) / rows) * p.words * 4);
@@ -787,12 +861,12 @@ struct Operands {
             h = p.pack_h ? Operand{c.ws + p.h, p.ldd} : Operand{c.hidden, c.ldh};
             if (p.pack_h)
                 ph = Pack{c.hidden, c.ldh, c.T, (int)c.D, p.Dp, (uint16_t *)(c.ws + p.h), p.ldd,
-                          counted_only ? c.target : nullptr, c.wide, c.ignore};
+                          counted_only ? c.target : nullptr, c.wide, c.ignore, p.again ? c.T : 0};
             h_there = true;
         }
         if (w_at != v0) {
             w = p.pack_w ? Operand{c.ws + p.w, p.ldd} : Operand{from, c.ldw};
-            if (p.pack_w) pw = Pack{from, c.ldw, n, (int)c.D, p.Dp, (uint16_t *)(c.ws + p.w), p.ldd, nullptr, 0, 0};
+            if (p.pack_w) pw = Pack{from, c.ldw, n, (int)c.D, p.Dp, (uint16_t *)(c.ws + p.w), p.ldd, nullptr, 0, 0, 0};
             w_at = v0;
         }
         if (untaught) {
@@ -828,7 +902,12 @@ Args logit_args(const Call &c, const Plan &p, int64_t v0, int64_t n, const Opera
 // while there are few of both (64 tokens, 1000 words, float32: 3 us of a step) and of a teacher's words.
 inline bool joined_later(const Call &c, const Plan &p, int tiles)
 {
-    return p.keep && p.pieces == 1 && c.T <= 128 && tiles <= 64 && c.teacher.K <= 64;
+    return p.keep && p.pieces == 1 && c.T <= 128 && tiles <= 64 && c.teacher.K <= 64 && p.again != 1;
+}
+
+inline Marks marks_of(const Call &c, const Plan &p)
+{
+    return Marks{c.teacher.sorted, c.teacher.taught, c.T, c.V, c.teacher.K, (uint8_t *)(c.ws + p.twice)};
 }
 
 // One product, of `kind`, by the kernels of the plan; fills in the tile counts.
@@ -870,8 +949,9 @@ int loss(const Call &c, const Plan &p, bool counted_only, Operands<P> &o, int re
     *of = Rows{(const float2 *)(c.ws + p.stats), (const float *)(c.ws + p.picked), tiles, (int)c.T, c.target, c.wide, c.V, c.ignore,
                lse, rows, reduction, (Share *)(c.ws + p.shares), (uint32_t *)(c.ws + p.arrived), total, c.teacher.taught, c.teacher.K,
                c.teacher.K ? c.teacher.temperature : 1.f};
-    if (!joined_later(c, p, tiles))
-        hipLaunchKernelGGL(row_kernel, dim3((unsigned)((c.T + kRowsJoined - 1) / kRowsJoined)), dim3(1024), 0, c.st, *of);
+    const unsigned groups = (unsigned)((c.T + kRowsJoined - 1) / kRowsJoined);
+    if (p.again == 1) hipLaunchKernelGGL(row_kernel<true>, dim3(groups + 1), dim3(1024), 0, c.st, *of, marks_of(c, p));
+    else if (!joined_later(c, p, tiles)) hipLaunchKernelGGL(row_kernel<false>, dim3(groups), dim3(1024), 0, c.st, *of, Marks{});
     return launch_status();
 }
 
@@ -895,6 +975,7 @@ int loss_grad(const Call &c, const Plan &p, Operands<P> &o, const Rows &of, Grad
     // the temperature, where no row's share has it
     if (c.teacher.K && c.T > 0 && !r.share) r.share = c.teacher.factor;
     float *const slices = (float *)(c.ws + p.slices);
+    const uint8_t *const twice = p.again == 1 ? (const uint8_t *)(c.ws + p.twice) : nullptr;
     // the last piece first: its exponentials may be there, and its weights are
     for (int64_t i = 0; i < p.pieces; ++i) {
         const int64_t v0 = (i == 0 ? p.pieces - 1 : i - 1) * p.piece;
@@ -914,7 +995,7 @@ int loss_grad(const Call &c, const Plan &p, Operands<P> &o, const Rows &of, Grad
                 const int words = ceil_div((int)n, 32) * 32;
                 const bool beside = P::planes == 1;
                 const Finish f{c.ws + p.prob, p.ldp, (const float *)(c.ws + (beside ? p.kept : p.prob)), beside ? p.words : p.ldp / 2, words, p.tile_words, rows, v0, n, of.tiles - ceil_div((int)n, p.tile_words),
-                               p.words, of, bias_part, bias_out, {r.grad, r.share}, c.teacher.sorted};
+                               p.words, of, bias_part, bias_out, {r.grad, r.share}, c.teacher.sorted, twice, p.again ? c.T : 0};
                 const unsigned along = ceil_div(words, 256), down = ceil_div((int)c.T, rows);
                 if (joined_later(c, p, of.tiles) && c.teacher.K)
                     hipLaunchKernelGGL((finish_kernel<P, true, true>), dim3(along, down + 1), dim3(256), 0, c.st, f);
@@ -932,6 +1013,7 @@ int loss_grad(const Call &c, const Plan &p, Operands<P> &o, const Rows &of, Grad
                 g.row_power = power;
                 g.prob = c.ws + p.prob, g.ldp = p.ldp, g.prob_words = p.words;
                 g.factor[0] = r.grad, g.factor[1] = r.share;
+                g.twice = twice, g.again = p.again ? c.T : 0;
                 g.bias_out = bias_out, g.bias_part = bias_part;
                 g.ld_bias_part = p.words;
                 DS_TRY(product<P>(p, kLogitProb, p.tile_logits, g, c.T, c.st));
@@ -957,7 +1039,8 @@ int loss_grad(const Call &c, const Plan &p, Operands<P> &o, const Rows &of, Grad
             x.M = (int)c.D;
             x.N = which ? (int)((n + 7) / 8 * 8) : (int)c.T;
             x.n_store = which ? (int)n : (int)c.T;
-            x.K = which ? (int)c.T : (int)n;
+            x.K = which ? (int)c.T * (p.again == 2 ? 2 : 1) : (int)n;
+            if (which) x.twice = twice, x.v0 = (int)v0;
             x.factor[0] = r.grad, x.factor[1] = r.share;
             x.out = which ? (void *)((E *)r.dweight + v0 * c.D) : r.dhidden;
             x.ldo = c.D;
@@ -1022,6 +1105,7 @@ int run(Call c, int what, const Outputs &out)
     if (c.teacher.K && c.T > 0) {
         if (what & kLoss) o.untaught = true;
         else launch_teacher(c.teacher, c.st);
+        if (!(what & kLoss) && p.again == 1) hipLaunchKernelGGL(mark_kernel, dim3(1), dim3(1024), 0, c.st, marks_of(c, p));
     }
     Rows of{};
     if (what & kLoss) DS_TRY(loss<P>(c, p, what & kGrad, o, out.reduction, out.rows, out.lse, out.total, &of));

@@ -23,6 +23,7 @@ struct Pack {
     const void *target;
     int wide;
     int64_t ignore;
+    int64_t again;   // of 16 bits: rows are written once more, so many rows behind; or 0
 };
 // One operand, or two in one launch.  For float, bf16_t and f16_t.
 template <typename E> int launch_pack(const Pack &one, const Pack &two, hipStream_t st);

@@ -377,6 +377,39 @@ def test_temperatures_at_both_ends(dtype):
         _check(h, w, b, ids, logits, c, ones, rows, *(() if beyond else step[1:]))
 
 
+@pytest.mark.parametrize("T", [3, 64, 65, 500, 1300])
+def test_words_that_most_tokens_teach(T):
+    # bfloat16: what P loses by its rounding is kept for them, 2^-16 of it is left
+    dtype, D, V, K, c = torch.bfloat16, 72, 9001, 12, 1.4
+    h, w, b, ids, logits = _case(T, D, V, K, dtype, True, 26)
+    ids = torch.randint(0, V, (T, K), generator=_gen(27)).to(DEV)
+    often = torch.tensor([8999, 4321, 300], device=DEV)
+    ids[:, :3], logits[:, :3] = often, logits[:, :3] + torch.tensor([6.0, 5.5, 5.0], device=DEV)
+    ones = torch.ones(T, device=DEV)
+    for tune in (dict(), dict(vocab_piece_kb=max(1, T * 4)), dict(vocab_split=3)):
+        for tile in (None, 0, 1, 2, 3):
+            with Tune(vocab_tile=tile, **tune):
+                rows = training.linear_distillation(h, w, ids, logits, b, c, "none")
+                step = training.linear_distillation_grad(h, w, ids, logits, b, c, "sum")
+                got = _autograd(h, w, ids, logits, b, c, "sum")
+            for dh, dw, db in (step[1:], got[1:]):
+                _check(h, w, b, ids, logits, c, ones, rows, dh, dw, db)
+                _, _, _, _, _, whole, whole_off = _teacher(ids, logits, V, c)
+                H = h.double()
+                s = (H @ w.double().t().contiguous() + b.double()) / c
+                size = (H.abs() @ w.double().abs().t().contiguous() + b.double().abs()) / c
+                d = ((D + 8) * E * size + 2 * E * s.abs()).amax(1, keepdim=True)
+                p = s.softmax(1)
+                P = ((p - whole) * c)[:, often].t().contiguous()
+                soft = (p * (2 * d + (4 * s.abs().amax(1, keepdim=True) + 16) * E) + whole_off + E * (p + whole)) * c
+                off = soft[:, often].t().contiguous() + P.abs() * 2.0 ** -15
+                exact = P @ H
+                bound = off @ H.abs() + (2 * T + 16) * E * (P.abs() @ H.abs()) + 1.01 * U[dtype] * exact.abs()
+                _within(dw[often], exact, bound, "dweight of frequent words")
+            again = training.linear_distillation_grad(h, w, ids, logits, b, c, "sum") if not tune and tile is None else step
+            assert all(torch.equal(x, y) for x, y in zip(again, step))
+
+
 def test_many_tokens():
     for dtype in TYPES:
         T, D, V, K = 70001, 16, 50, 3
