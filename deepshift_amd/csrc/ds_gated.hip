@@ -230,7 +230,7 @@ struct Plan {
 template <typename P>
 int64_t most_few(const void *x, int64_t ldx, const void *weight, int64_t ldw, int64_t D)
 {
-    return P::planes > 1 ? 8 : in_place(x, ldx, D) && in_place(weight, ldw, D) ? 2 : 4;
+    return P::planes > 1 ? 16 : in_place(x, ldx, D) && in_place(weight, ldw, D) ? 2 : 4;
 }
 
 template <typename P>

@@ -86,8 +86,12 @@ int launch_few(const Few &f, hipStream_t st)
     if (f.T == 1) hipLaunchKernelGGL((few_kernel<E, 1, 1, 4>), blocks(1), dim3(256), 0, st, f);
     else if (f.T == 2) hipLaunchKernelGGL((few_kernel<E, 2, 1, 4>), blocks(1), dim3(256), 0, st, f);
     else if (f.T <= 4) hipLaunchKernelGGL((few_kernel<E, 4, 2, 2>), blocks(2), dim3(256), 0, st, f);
-    else if constexpr (sizeof(E) == 4) hipLaunchKernelGGL((few_kernel<E, 8, 2, 2>), blocks(2), dim3(256), 0, st, f);
-    else return DS_EINVAL;
+    else if constexpr (sizeof(E) == 4) {
+        if (f.T <= 8) hipLaunchKernelGGL((few_kernel<E, 8, 2, 2>), blocks(2), dim3(256), 0, st, f);
+        else hipLaunchKernelGGL((few_kernel<E, 16, 2, 1>), blocks(2), dim3(256), 0, st, f);
+    } else {
+        return DS_EINVAL;
+    }
     return launch_status();
 }
 template int launch_few<float>(const Few &, hipStream_t);
