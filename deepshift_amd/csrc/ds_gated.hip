@@ -225,8 +225,9 @@ struct Plan {
 //   4096 features, bfloat16       26   35    31   35   38   35   40   36   58   35   70   36
 //   4096, float16                 26   35    27   35   31   36   32   35   37   36   38   36
 //   4095, bfloat16                36   74    53   74   44   74   45   75   75   74   78   74
-//   4096, float32                 48  215    52  215   53  215   54  215   62  216   64  217     (9: 132 split by the tiles)
-//   1024, 2731 results, float32    9   34     8   33   10   33   10   33   14   33   14   34
+//   4096, float32                 48  215    52  215   53  215   54  215   62  216   64  217   16: 85  132 (split by the tiles)
+//   1024, 2731 results, float32    9   34     8   33   10   33   10   33   14   33   14   34    16: 20   36
+//   4096, 512 results, float32                                                      27   85    16: 24   85
 template <typename P>
 int64_t most_few(const void *x, int64_t ldx, const void *weight, int64_t ldw, int64_t D)
 {
