@@ -8,7 +8,9 @@ The layers between are ``LinearShift`` / ``LinearShiftQ`` on their float path, w
 current stream of the tensors' device, on float32, bfloat16 and float16; sums are held in 32 bits or more and rounded once,
 and a call repeats bit for bit.  There is no CPU path: a CPU tensor raises.
 
-Functions whose names end in ``_grad`` return gradients directly; the others, but for the clipping, take part in autograd.
+Functions whose names end in ``_grad`` return gradients directly; the others, but for the clipping, take part in autograd.  All
+can be captured into a graph; where ``backward()`` is, no graph recorded eagerly from the same parameters may be alive (PyTorch
+adds gradients up on the stream that recorded them first).
 """
 import contextlib
 

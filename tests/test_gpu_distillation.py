@@ -411,8 +411,9 @@ def test_words_that_most_tokens_teach(T):
 
 
 def test_many_tokens():
-    for dtype in TYPES:
-        T, D, V, K = 70001, 16, 50, 3
+    # more of them than a launch's second axis has workgroups for, too
+    for dtype, T in [(dtype, 70001) for dtype in TYPES] + [(torch.bfloat16, 530001), (torch.float32, 530001)]:
+        D, V, K = 16, 50, 3
         h, w, b, ids, logits = _case(T, D, V, K, dtype, True, 23)
         n = int((ids >= 0).any(1).sum())
         rows = training.linear_distillation(h, w, ids, logits, b, 2.0, "none")
@@ -508,6 +509,22 @@ def test_another_stream_and_captured_replays():
                 replay.replay()
                 torch.cuda.synchronize()
                 assert all(torch.equal(p, q) for p, q in zip(results, call())), "replay %d" % i
+
+
+def test_two_streams_at_once():
+    for dtype in TYPES:
+        cases = [_case(90, 64, 5000, 12, dtype, True, 28, i) for i in range(2)]
+        want = [training.linear_distillation_grad(h, w, ids, logits, b, 2.0) for h, w, b, ids, logits in cases]
+        streams = [torch.cuda.Stream() for _ in cases]
+        for s in streams:
+            s.wait_stream(torch.cuda.current_stream())
+        got = [[], []]
+        for _ in range(10):
+            for (h, w, b, ids, logits), s, results in zip(cases, streams, got):
+                with torch.cuda.stream(s):
+                    results.append(training.linear_distillation_grad(h, w, ids, logits, b, 2.0))
+        torch.cuda.synchronize()
+        assert all(torch.equal(p, q) for results, first in zip(got, want) for one in results for p, q in zip(one, first))
 
 
 def test_the_heads_module():

@@ -269,10 +269,27 @@ def test_gradients_against_differences():
 
 
 def test_many_tokens():
+    # more of them than a launch's second axis has workgroups of 64 for, too
     for dtype in TYPES:
-        T, D, F = 70001, 16, 24
-        x, w, b, grad = _case(T, D, F, dtype, True, 12)
-        _check(x, w, b, "silu", grad, *_step(x, w, b, "silu", grad))
+        for T, D, F in ((70001, 16, 24), (4300001, 8, 8)):
+            x, w, b, grad = _case(T, D, F, dtype, True, 12)
+            _check(x, w, b, "silu", grad, *_step(x, w, b, "silu", grad))
+
+
+def test_two_streams_at_once():
+    for dtype in TYPES:
+        cases = [_case(90, 64, 200, dtype, True, 14, i) for i in range(2)]
+        want = [_step(x, w, b, "gelu", grad) for x, w, b, grad in cases]
+        streams = [torch.cuda.Stream() for _ in cases]
+        for s in streams:
+            s.wait_stream(torch.cuda.current_stream())
+        got = [[], []]
+        for _ in range(10):
+            for (x, w, b, grad), s, results in zip(cases, streams, got):
+                with torch.cuda.stream(s):
+                    results.append(_step(x, w, b, "gelu", grad))
+        torch.cuda.synchronize()
+        assert all(torch.equal(p, q) for results, first in zip(got, want) for one in results for p, q in zip(one, first))
 
 
 @pytest.mark.parametrize("dtype", TYPES, ids=str)
