@@ -192,8 +192,8 @@ __device__ __forceinline__ void add_to_total(const Rows &r, double loss, double 
 // off by then, and words that most tokens teach have columns hundreds of times larger than others: of bfloat16 single values were
 // off by half of the whole gradient's root mean square (8192 tokens, 64 of 65536 words, as often as text has them).  So P keeps its
 // rounding's remainder for groups of 256 words that hold such a word, and the weights' gradient takes both (0.03 of it then): a
-// handful of 256 groups, and a step of 10.9 ms takes 11.2.  Up to kTwiceAll tokens all groups have it, which costs nothing beside the weights; words
-// of a vocabulary up to kNoneHeavy move too little, and a single word's P is near -1, which rounds to itself.
+// handful of 256 groups, and a step of 10.9 ms takes 11.2.  Up to kTwiceAll tokens all groups have it, which costs nothing beside the weights; with
+// more of them, words of a vocabulary up to kNoneHeavy move too little.  A single word's P is near -1, which rounds to itself.
 constexpr int64_t kTwiceAll = 64, kNoneHeavy = 4096;
 
 struct Marks {
@@ -768,7 +768,7 @@ Plan plan_of(const void *hidden, int64_t ldh, const void *weight, int64_t ldw, i
     if (words) {
         p.sorted = take((size_t)T * words * 4), p.taught = take((size_t)T * words * 4);
         p.target = take((size_t)T * 4), p.temperature = take(4);
-        if (NP == 1 && !P::half && what & kGrad && words > 1 && V > kNoneHeavy) p.again = T <= kTwiceAll ? 2 : 1;
+        if (NP == 1 && !P::half && what & kGrad && words > 1 && (T <= kTwiceAll || V > kNoneHeavy)) p.again = T <= kTwiceAll ? 2 : 1;
         if (p.again == 1) p.twice = take((size_t)((V + 255) / 256));
     }
     const size_t copies = p.again ? 2 : 1;
