@@ -80,6 +80,14 @@ class _PackedWeightsMixin:
         state.pop("_handoff_buffers", None)
         return state
 
+    def _clamp_shift(self):
+        """Holds the shifts of the float path to their range where they are: a captured graph that runs the layer reads and writes
+        the parameter's own memory at every replay.  Packed words are built again behind it, as behind any change."""
+        with torch.inference_mode():   # (also a parameter that was made there)
+            self.shift.data.clamp_(*self.shift_range)
+        if self._packed_from is not None:
+            object.__setattr__(self, "_packed_from", ())
+
     def packed_weights(self):
         """The layer's ConcWeight, (re)built if it is missing or older than the parameters."""
         if self._conc_weight is None or (self._packed_from is not None and
@@ -183,7 +191,7 @@ class LinearShift(_PackedWeightsMixin, nn.Module):
 
     def float_weight(self):
         """The weights of the float path, +-2^shift, with straight-through gradients."""
-        self.shift.data = ste.clamp(self.shift.data, *self.shift_range)
+        self._clamp_shift()
         shift_rounded = ste.round(self.shift, rounding=self.rounding)
         sign_rounded_signed = ste.sign(ste.round(self.sign, rounding=self.rounding))
         return ste.unsym_grad_mul(2 ** shift_rounded, sign_rounded_signed)
@@ -517,7 +525,7 @@ class Conv2dShift(_ConvNdShift):
             if not self.use_cuda:
                 return conv_cpu_forward(self, input, *module_codes(self))
             return conv_kernel_forward(self, input, self.packed_weights())
-        self.shift.data = ste.clamp(self.shift.data, *self.shift_range)
+        self._clamp_shift()
 
         shift_rounded = ste.round(self.shift, self.rounding)
         sign_rounded_signed = ste.sign(ste.round(self.sign, self.rounding))

@@ -1,9 +1,11 @@
 """GPU: the recurrence, the gated block and the distillation together, as deepshift_amd.train_tokens uses them."""
+import copy
+
 import pytest
 import torch
 import torch.nn.functional as F
 
-from deepshift_amd import train_tokens, training
+from deepshift_amd import modules, train_tokens, training
 
 pytestmark = pytest.mark.gpu
 DEV = torch.device("cuda:0")
@@ -126,3 +128,68 @@ def test_a_step_can_be_captured():
         for p, q in zip(captured, step()):
             # the library's part repeats bit for bit; torch's own products may take other kernels under capture
             assert (p - q).norm() <= 1e-4 * q.norm() + 1e-6, "replay %d" % i
+
+
+@pytest.mark.parametrize("shift_type", ["PS", "Q"])
+def test_a_captured_step_reads_the_parameters_that_are_there(shift_type):
+    # updates between replays, by an optimizer and through .data, out of the range that the float path holds them to
+    torch.manual_seed(4)
+    generator = torch.Generator(device=DEV).manual_seed(5)
+    with DEV:
+        model = train_tokens.SequenceModel(60, 32, 1, shift_type)
+    tokens, target, lengths = train_tokens.sequences(4, 16, 60, DEV, generator)
+    parameters = list(model.parameters())
+
+    def step(model):
+        return torch.autograd.grad(model(tokens, target, lengths), list(model.parameters()))
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step(model)
+    torch.cuda.current_stream().wait_stream(side)
+    places = [p.data_ptr() for p in parameters]
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured = step(model)
+    assert [p.data_ptr() for p in parameters] == places
+    optimizer = torch.optim.SGD(parameters, lr=2.0)
+    for i in range(4):
+        twin = copy.deepcopy(model)
+        graph.replay()
+        torch.cuda.synchronize()
+        for (name, p), g, want in zip(model.named_parameters(), captured, step(twin)):
+            # torch's own products may take other kernels under capture
+            assert (g - want).norm() <= 1e-4 * want.norm() + 1e-6, (i, name)
+            p.grad = g.clone()
+        for (name, p), q in zip(model.named_parameters(), twin.parameters()):
+            assert torch.equal(p, q), (i, name)
+        torch.nn.utils.clip_grad_norm_(parameters, 1.0)
+        before = [p.detach().clone() for p in parameters]
+        optimizer.step()
+        for layer in (model.layers[0].enter, model.layers[0].gated.layer):
+            (layer.shift if shift_type == "PS" else layer.weight).data.mul_(1.5)
+        after = [p.detach().clone() for p in parameters]
+        assert any(not torch.equal(p, q) for p, q in zip(before, after))
+        fill = [torch.full_like(p, 7.0) for p in parameters for _ in range(4)]   # memory that a pass may have left is used again
+        del fill
+
+
+@pytest.mark.parametrize("kind", ["linear", "conv"])
+def test_words_are_packed_again_behind_a_float_pass(kind):
+    # an update through .data leaves no trace in the parameter's version; a pass over the float parameters behind it does
+    torch.manual_seed(0)
+    make = (lambda: modules.LinearShift(6, 4)) if kind == "linear" else (lambda: modules.Conv2dShift(3, 4, 3))
+    x = torch.randn(*((2, 6) if kind == "linear" else (2, 3, 8, 8)), device=DEV)
+    layer, fresh = make().to(DEV), make().to(DEV)
+    first = layer.packed_weights().data.clone()
+    layer.shift.data.sub_(5.0).round_()
+    layer(x)
+    assert not torch.equal(layer.packed_weights().data, first)
+    fresh.load_state_dict(layer.state_dict())
+    assert torch.equal(layer.packed_weights().data, fresh.packed_weights().data)
+    assert layer.packed_weights() is layer.packed_weights()
+    # words given from outside stay
+    layer.conc_weight = given = fresh.packed_weights()
+    layer(x)
+    assert layer.packed_weights() is given
