@@ -204,37 +204,42 @@ struct Marks {
     uint8_t *twice;      // [groups of 256 words]
 };
 
-// By one workgroup, while others join the rows: of up to 512 tokens and 16384 words, evenly spread, the words' sums of squared probabilities, whole numbers of 2^-20 by a hash
-// of the word; a sum that is a hundred-and-twenty-eighth of all marks the group of its likeliest word.
+// By one workgroup, while others join the rows: of up to 512 tokens and 16384 words, evenly spread, the words' sums of squared
+// probabilities, whole numbers of 2^-20, in two tables by a hash of the word each.  A word whose sums are a hundred-and-twenty-eighth of
+// all in both of them marks its group: all that have as much themselves, and one of some 10000 others that share their places with
+// such words in both.
 __device__ __forceinline__ void mark_heavy(const Marks &m)
 {
     constexpr int kBuckets = 4096;
-    __shared__ uint32_t sums[kBuckets];
-    __shared__ unsigned long long likeliest[kBuckets];
+    __shared__ uint32_t sums[2][kBuckets];
     __shared__ unsigned long long all;
-    for (int i = threadIdx.x; i < kBuckets; i += blockDim.x) sums[i] = 0, likeliest[i] = 0;
+    for (int i = threadIdx.x; i < kBuckets; i += blockDim.x) sums[0][i] = 0, sums[1][i] = 0;
     if (threadIdx.x == 0) all = 0;
     const int64_t groups = (m.V + 255) / 256;
     for (int64_t i = threadIdx.x; i < groups; i += blockDim.x) m.twice[i] = 0;
     __threadfence();
     __syncthreads();
     const int64_t most = min((int64_t)512, (int64_t)16384 / m.K), step = (m.T + most - 1) / most, places = (m.T + step - 1) / step * m.K;
-    unsigned long long mine = 0;
+    auto over_sample = [&](auto found) {
 #pragma unroll 4
-    for (int64_t i = threadIdx.x; i < places; i += blockDim.x) {
-        const int64_t at = i / m.K * step * m.K + i % m.K;
-        const float q = m.taught[at];
-        const uint32_t id = (uint32_t)m.sorted[at], sum = (uint32_t)(q * q * 0x1p20f);
-        if (sum == 0) continue;
-        const uint32_t bucket = id * 2654435761u >> 20;
-        atomicAdd(&sums[bucket], sum);
-        atomicMax(&likeliest[bucket], (unsigned long long)__float_as_uint(q) << 32 | id);
+        for (int64_t i = threadIdx.x; i < places; i += blockDim.x) {
+            const int64_t at = i / m.K * step * m.K + i % m.K;
+            const float q = m.taught[at];
+            const uint32_t id = (uint32_t)m.sorted[at], sum = (uint32_t)(q * q * 0x1p20f);
+            if (sum > 0) found(id, sums[0][id * 2654435769u >> 20], sums[1][id * 3242174889u >> 20], sum);
+        }
+    };
+    unsigned long long mine = 0;
+    over_sample([&](uint32_t, uint32_t &one, uint32_t &two, uint32_t sum) {
+        atomicAdd(&one, sum);
+        atomicAdd(&two, sum);
         mine += sum;
-    }
+    });
     atomicAdd(&all, mine);
     __syncthreads();
-    for (int i = threadIdx.x; i < kBuckets; i += blockDim.x)
-        if (sums[i] && sums[i] * 128ull >= all) m.twice[(uint32_t)likeliest[i] / 256] = 1;
+    over_sample([&](uint32_t id, uint32_t &one, uint32_t &two, uint32_t) {
+        if (min(one, two) * 128ull >= all) m.twice[id / 256] = 1;
+    });
 }
 __global__ __launch_bounds__(1024) void mark_kernel(Marks m) { mark_heavy(m); }
 

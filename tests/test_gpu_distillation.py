@@ -556,3 +556,51 @@ def test_refusals_on_the_gpu():
     dh, = torch.autograd.grad(f(h, w, ids, logits, b), h, create_graph=True)
     with pytest.raises(RuntimeError):
         dh.sum().backward()
+
+
+def _check_frequent(h, w, b, ids, logits, c, often, dw):
+    """``dw`` of a step with reduction 'sum', at words whose P keeps what it loses by its rounding to bfloat16: 2^-16 of it is left."""
+    (T, D), V = h.shape, w.shape[0]
+    kept, _, _, _, _, whole, whole_off = _teacher(ids, logits, V, c)
+    H = torch.where(kept[:, None], h.double(), 0.0)
+    s = H @ w.double().t().contiguous()
+    size = H.abs() @ w.double().abs().t().contiguous()
+    if b is not None:
+        s, size = s + b.double(), size + b.double().abs()
+    s, size = s / c, size / c
+    d = ((D + 8) * E * size + 2 * E * s.abs()).amax(1, keepdim=True)
+    p = s.softmax(1)
+    P = ((p - whole) * c * kept[:, None])[:, often].t().contiguous()
+    soft = (p * (2 * d + (4 * s.abs().amax(1, keepdim=True) + 16) * E) + whole_off + E * (p + whole)) * c * kept[:, None]
+    off = soft[:, often].t().contiguous() + P.abs() * 2.0 ** -15
+    exact = P @ H
+    bound = off @ H.abs() + (2 * T + 16) * E * (P.abs() @ H.abs()) + 1.01 * U[h.dtype] * exact.abs()
+    _within(dw[often], exact, bound, "dweight of frequent words")
+
+
+def _frequent(T, D, V, K, often, strength, *key):
+    """A case whose first words are the same for all tokens, the others anywhere."""
+    h, w, b, _, logits = _case(T, D, V, K, torch.bfloat16, True, *key)
+    ids = torch.randint(0, V, (T, K), generator=_gen(*key, 1)).to(DEV)
+    ids[:, :len(often)] = torch.tensor(often, device=DEV)
+    logits[:, :len(often)] = logits[:, :len(often)] * 0.3 + strength
+    return h, w, b, ids, logits
+
+
+def test_frequent_words_beside_rare_ones_of_more_weight():
+    # words of other groups that one token teaches, with nearly all of its probability, and that lie in the frequent words' places of
+    # a table of 4096, as a multiplication by the golden ratio finds them
+    T, D, V, K, c, often = 500, 1000, 60001, 12, 1.3, [8999, 4321, 300, 55000]
+    h, w, b, ids, logits = _frequent(T, D, V, K, often, 4.0, 41)
+    places = (torch.arange(V) * 2654435761) % 2 ** 32 >> 20
+    for i, word in enumerate(often):
+        rare = [int(r) for r in (places == places[word]).nonzero() if int(r) // 256 != word // 256]
+        assert len(rare) >= 3
+        for j, r in enumerate(rare):
+            ids[40 * i + j, 5], logits[40 * i + j, 5] = r, 16.0
+    rows = training.linear_distillation(h, w, ids, logits, b, c, "none")
+    step = training.linear_distillation_grad(h, w, ids, logits, b, c, "sum")
+    got = _autograd(h, w, ids, logits, b, c, "sum")
+    _check(h, w, b, ids, logits, c, torch.ones(T, device=DEV), rows, *step[1:])
+    for dw in (step[2], got[2]):
+        _check_frequent(h, w, b, ids, logits, c, often, dw)
