@@ -199,31 +199,55 @@ constexpr int64_t kTwiceAll = 64, kNoneHeavy = 4096;
 struct Marks {
     const int *sorted;
     const float *taught;
+    const int *target;   // [T] 0: the token counts
     int64_t T, V;
     int K;
     uint8_t *twice;      // [groups of 256 words]
 };
 
-// By one workgroup, while others join the rows: of up to 512 tokens and 16384 words, evenly spread, the words' sums of squared
-// probabilities, whole numbers of 2^-20, in two tables by a hash of the word each.  A word whose sums are a hundred-and-twenty-eighth of
+// By one workgroup, while others join the rows: of up to 512 tokens and 16384 words, one of every stretch of tokens, the words' sums of
+// squared probabilities, whole numbers of 2^-20, in two tables by a hash of the word each.  A word whose sums are a hundred-and-twenty-eighth of
 // all in both of them marks its group: all that have as much themselves, and one of some 10000 others that share their places with
-// such words in both.
+// such words in both.  A stretch's token is its first that counts, looked for from a place that moves by the golden ratio from stretch
+// to stretch: at the same place of each, tokens of equal sequences would all stand at one place of theirs.
 __device__ __forceinline__ void mark_heavy(const Marks &m)
 {
-    constexpr int kBuckets = 4096;
+    constexpr int kBuckets = 4096, kSample = 512;
     __shared__ uint32_t sums[2][kBuckets];
+    __shared__ int sample[kSample];  // tokens, -1 where none of a stretch counts
     __shared__ unsigned long long all;
     for (int i = threadIdx.x; i < kBuckets; i += blockDim.x) sums[0][i] = 0, sums[1][i] = 0;
     if (threadIdx.x == 0) all = 0;
     const int64_t groups = (m.V + 255) / 256;
     for (int64_t i = threadIdx.x; i < groups; i += blockDim.x) m.twice[i] = 0;
     __threadfence();
+    const int most = min(kSample, 16384 / m.K), step = (int)((m.T + most - 1) / most), stretches = (int)((m.T + step - 1) / step);
+    const int places = stretches * m.K;
+    for (int i = threadIdx.x; i < stretches; i += blockDim.x) {
+        const int first = i * step, count = (int)min((int64_t)step, m.T - first);
+        const int from = (int)((uint64_t)(uint32_t)(i * 2654435769u) * count >> 32);
+        int found = -1;
+        constexpr int kAhead = 8;
+        for (int j = 0; j < count && found < 0; j += kAhead) {
+            int at[kAhead], target[kAhead];
+#pragma unroll
+            for (int k = 0; k < kAhead; ++k) {
+                at[k] = from + min(j + k, count - 1);
+                at[k] = first + (at[k] < count ? at[k] : at[k] - count);
+                target[k] = m.target[at[k]];
+            }
+#pragma unroll
+            for (int k = kAhead - 1; k >= 0; --k) found = target[k] == 0 ? at[k] : found;
+        }
+        sample[i] = found;
+    }
     __syncthreads();
-    const int64_t most = min((int64_t)512, (int64_t)16384 / m.K), step = (m.T + most - 1) / most, places = (m.T + step - 1) / step * m.K;
     auto over_sample = [&](auto found) {
 #pragma unroll 4
-        for (int64_t i = threadIdx.x; i < places; i += blockDim.x) {
-            const int64_t at = i / m.K * step * m.K + i % m.K;
+        for (int i = threadIdx.x; i < places; i += blockDim.x) {
+            const int t = sample[i / m.K];
+            if (t < 0) continue;
+            const int64_t at = (int64_t)t * m.K + i % m.K;
             const float q = m.taught[at];
             const uint32_t id = (uint32_t)m.sorted[at], sum = (uint32_t)(q * q * 0x1p20f);
             if (sum > 0) found(id, sums[0][id * 2654435769u >> 20], sums[1][id * 3242174889u >> 20], sum);
@@ -912,7 +936,7 @@ inline bool joined_later(const Call &c, const Plan &p, int tiles)
 
 inline Marks marks_of(const Call &c, const Plan &p)
 {
-    return Marks{c.teacher.sorted, c.teacher.taught, c.T, c.V, c.teacher.K, (uint8_t *)(c.ws + p.twice)};
+    return Marks{c.teacher.sorted, c.teacher.taught, c.teacher.target, c.T, c.V, c.teacher.K, (uint8_t *)(c.ws + p.twice)};
 }
 
 // One product, of `kind`, by the kernels of the plan; fills in the tile counts.

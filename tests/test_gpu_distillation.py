@@ -604,3 +604,38 @@ def test_frequent_words_beside_rare_ones_of_more_weight():
     _check(h, w, b, ids, logits, c, torch.ones(T, device=DEV), rows, *step[1:])
     for dw in (step[2], got[2]):
         _check_frequent(h, w, b, ids, logits, c, often, dw)
+
+
+@pytest.mark.parametrize("first", ["none", "others"])
+def test_frequent_words_of_sequences(first):
+    # tokens of equal sequences in a row, whose first ones (prompts, what begins a text) have no words, or words of their own
+    T, D, V, K, c, often = 512, 1000, 5003, 256, 1.3, [4999, 2321, 300]
+    h, w, b, ids, logits = _frequent(T, D, V, K, often, 4.0, 42)
+    logits[:, 3:] = logits[:, 3:] / 3 - 2
+    starts = torch.arange(T, device=DEV) % 8 < 2
+    if first == "none":
+        ids[starts] = -1
+    else:
+        ids[starts] = torch.randint(600, 1800, (int(starts.sum()), K), generator=_gen(43)).to(DEV)
+        logits[starts] = 0.0
+    rows = training.linear_distillation(h, w, ids, logits, b, c, "none")
+    step = training.linear_distillation_grad(h, w, ids, logits, b, c, "sum")
+    got = _autograd(h, w, ids, logits, b, c, "sum")
+    _check(h, w, b, ids, logits, c, torch.ones(T, device=DEV), rows, *step[1:])
+    for dw in (step[2], got[2]):
+        _check_frequent(h, w, b, ids, logits, c, often, dw)
+
+
+@pytest.mark.parametrize("K", [12, 256, 1024])
+def test_frequent_words_of_a_few_tokens_among_many_that_do_not_count(K):
+    D, V, c, often = 1000, 5003, 1.3, [4999, 2321, 300]
+    for T in (513, 5000, 40000):
+        h, w, b, ids, logits = _frequent(T, D, V, K, often, 4.0, 44)
+        logits[:, 3:] = logits[:, 3:] / 3 - 2
+        ids[torch.arange(T, device=DEV) % (T // 20) != T // 20 - 1] = -1
+        step = training.linear_distillation_grad(h, w, ids, logits, b, c, "sum")
+        # (sums over the tokens that count: the others are zeros)
+        kept = (ids[:, 0] >= 0)
+        _check_frequent(h[kept], w, b, ids[kept], logits[kept], c, often, step[2])
+    ids[:] = -1
+    assert all((t == 0).all() for t in training.linear_distillation_grad(h, w, ids, logits, b, c, "sum"))
