@@ -189,12 +189,21 @@ __device__ __forceinline__ void add_to_total(const Rows &r, double loss, double 
 // ---- a teacher's heavy words ----------------------------------------------------------------------------------------
 //
 // P is rounded to the operands' type for the gradients' products.  Its own column's size is what a row of the weights' gradient is
-// off by then, and words that most tokens teach have columns hundreds of times larger than others: of bfloat16 single values were
-// off by half of the whole gradient's root mean square (8192 tokens, 64 of 65536 words, as often as text has them).  So P keeps its
-// rounding's remainder for groups of 256 words that hold such a word, and the weights' gradient takes both (0.03 of it then): a
-// handful of 256 groups, and a step of 10.9 ms takes 11.2.  Up to kTwiceAll tokens all groups have it, which costs nothing beside the weights; with
-// more of them, words of a vocabulary up to kNoneHeavy move too little.  A single word's P is near -1, which rounds to itself.
-constexpr int64_t kTwiceAll = 64, kNoneHeavy = 4096;
+// off by then, and words that most tokens teach have columns hundreds of times larger than others.  Of bfloat16 single values were
+// off by half of the whole gradient's root mean square, beyond their own rounding (8192 tokens, 64 of 65536 words, as often as text
+// has them; of 65 to 8192 tokens over 1000 words by 0.16, over 2000 by 0.21, over 4096 by 0.32).  So P keeps its rounding's remainder
+// for groups of 256 words that hold such a word, and the weights' gradient takes both: 0.03 to 0.1 of it then over 65536 words,
+// whose step of 8192 x 4096 takes 11.2 ms instead of 10.9; the workspace holds P and the hidden states twice.  A single word's P is
+// near -1, which rounds to itself.
+//
+// Up to kTwiceAll tokens, which costs nothing beside the weights, and up to kTwiceWords words all groups have it: less than 0.001 of
+// the root mean square there.  A step in us without it, with groups that are looked for, and with all:
+//      tokens, features, words           none  marked   all         tokens, features, words           none  marked   all
+//         65      512     1000             30      38    30            512     1024     4096            68      88    74
+//        128      512     1000             31      41    31           2048     1024     4096           136     174   158
+//       1024      512     1000             50      63    54           4096     1024     2000           151     184   182
+//       8192      512     1000            130     155   145           8192     4096     4096           804    1000  1031
+constexpr int64_t kTwiceAll = 64, kTwiceWords = 4096;
 
 struct Marks {
     const int *sorted;
@@ -797,7 +806,7 @@ Plan plan_of(const void *hidden, int64_t ldh, const void *weight, int64_t ldw, i
     if (words) {
         p.sorted = take((size_t)T * words * 4), p.taught = take((size_t)T * words * 4);
         p.target = take((size_t)T * 4), p.temperature = take(4);
-        if (NP == 1 && !P::half && what & kGrad && words > 1 && (T <= kTwiceAll || V > kNoneHeavy)) p.again = T <= kTwiceAll ? 2 : 1;
+        if (NP == 1 && !P::half && what & kGrad && words > 1) p.again = T <= kTwiceAll || V <= kTwiceWords ? 2 : 1;
         if (p.again == 1) p.twice = take((size_t)((V + 255) / 256));
     }
     const size_t copies = p.again ? 2 : 1;

@@ -639,3 +639,19 @@ def test_frequent_words_of_a_few_tokens_among_many_that_do_not_count(K):
         _check_frequent(h[kept], w, b, ids[kept], logits[kept], c, often, step[2])
     ids[:] = -1
     assert all((t == 0).all() for t in training.linear_distillation_grad(h, w, ids, logits, b, c, "sum"))
+
+
+@pytest.mark.parametrize("T", [2, 64, 65, 128, 129, 1500])
+def test_frequent_words_of_small_vocabularies(T):
+    D, c = 264, 1.3
+    for V, often in ((40, [7, 3]), (300, [299, 5]), (1000, [999, 300, 5]), (4096, [4095, 2000, 0]), (4097, [4096, 2000, 0])):
+        h, w, b, ids, logits = _frequent(T, D, V, 8, often, 3.0, 45)
+        rows = training.linear_distillation(h, w, ids, logits, b, c, "none")
+        step = training.linear_distillation_grad(h, w, ids, logits, b, c, "sum")
+        got = _autograd(h, w, ids, logits, b, c, "sum")
+        again = training.linear_distillation_grad(h, w, ids, logits, b, c, "sum")
+        assert all(torch.equal(p, q) for p, q in zip(step, again))
+        for dh, dw, db in (step[1:], got[1:]):
+            print(T, V, flush=True)
+            _check(h, w, b, ids, logits, c, torch.ones(T, device=DEV), rows, dh, dw, db)
+            _check_frequent(h, w, b, ids, logits, c, often, dw)
