@@ -93,9 +93,9 @@ class SequenceModel(nn.Module):
 
     @torch.no_grad()
     def generate(self, tokens, count):
-        """The likeliest ``count`` tokens behind ``tokens`` [B, T], one at a time; ``T`` is 1 at least."""
-        if tokens.dim() != 2 or tokens.shape[1] < 1 or count < 0:
-            raise ValueError("tokens must be [B, T] with a token at least, is %s, and count must not be negative" % list(tokens.shape))
+        """The likeliest ``count`` tokens behind ``tokens`` [B, T], one at a time; they need one at least to go on from."""
+        if count > 0 and tokens.shape[-1] < 1:
+            raise ValueError("tokens must be [B, T] with a token at least, is %s" % list(tokens.shape))
         hidden, states = self.hidden(tokens)
         made = []
         for _ in range(count):
