@@ -9,12 +9,15 @@ One deliberate difference: packed kernel weights are built from the shifts AFTER
 the layer's ``shift_range`` (the reference packs first and clamps later in ``forward``,
 modules.py:125,313), so the kernel path and the float path of a converted model always use the
 same power-of-two weights.
+
+``training.GatedLinear``, which holds the weights of two linear layers, becomes ``training.GatedShift``
+as one ``nn.Linear``; the head of ``training.LinearCrossEntropy`` stays as it is.
 """
 import copy
 
 import torch.nn as nn
 
-from . import modules, modules_q, utils
+from . import modules, modules_q, training, utils
 
 __all__ = ["convert_to_shift", "round_shift_weights", "count_layer_type"]
 
@@ -46,6 +49,13 @@ def _convert_linear(linear, shift_type, convert_weights, freeze_sign, kw):
     return layer.to(linear.weight.device)
 
 
+def _convert_gated(gated, shift_type, convert_weights, freeze_sign, kw):
+    both = nn.Linear(gated.in_features, 2 * gated.out_features, gated.bias is not None, device='meta')
+    both.weight, both.bias = gated.weight, gated.bias
+    layer = _convert_linear(both, shift_type, convert_weights, freeze_sign, kw)
+    return training.GatedShift(gated.in_features, gated.out_features, activation=gated.activation, layer=layer)
+
+
 def _convert_conv2d(conv, shift_type, convert_weights, freeze_sign, kw):
     has_bias = conv.bias is not None
     args = (conv.in_channels, conv.out_channels, conv.kernel_size, conv.stride, conv.padding,
@@ -74,10 +84,14 @@ def _convert_conv2d(conv, shift_type, convert_weights, freeze_sign, kw):
     return layer.to(conv.weight.device)
 
 
+_LINEAR = {nn.Linear: _convert_linear, training.GatedLinear: _convert_gated}
+
+
 def convert_to_shift(model, shift_depth, shift_type, convert_all_linear=True, convert_weights=False,
                      freeze_sign=False, use_kernel=False, use_cuda=True, rounding='deterministic',
                      weight_bits=5, act_integer_bits=16, act_fraction_bits=16):
-    """Replace Linear/Conv2d layers by shift layers, last layer first; returns (model, count)."""
+    """Replace Linear/Conv2d layers (and GatedLinear blocks, each like one Linear) by shift layers, last
+    layer first; returns (model, count)."""
     kw = dict(use_kernel=use_kernel, use_cuda=use_cuda, rounding=rounding, weight_bits=weight_bits,
               act_integer_bits=act_integer_bits, act_fraction_bits=act_fraction_bits)
     conversion_count = 0
@@ -88,10 +102,10 @@ def convert_to_shift(model, shift_depth, shift_type, convert_all_linear=True, co
                 convert_all_linear=convert_all_linear, convert_weights=convert_weights,
                 freeze_sign=freeze_sign, **kw)
             conversion_count += num_converted
-        if type(module) == nn.Linear and (convert_all_linear == True  # noqa: E712
-                                          or conversion_count < shift_depth):
-            model._modules[name] = _convert_linear(module, shift_type, convert_weights, freeze_sign,
-                                                   kw)
+        if type(module) in _LINEAR and (convert_all_linear == True  # noqa: E712
+                                        or conversion_count < shift_depth):
+            model._modules[name] = _LINEAR[type(module)](module, shift_type, convert_weights,
+                                                         freeze_sign, kw)
             if convert_all_linear == False:  # noqa: E712
                 conversion_count += 1
         if type(module) == nn.Conv2d and conversion_count < shift_depth:

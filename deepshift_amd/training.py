@@ -526,16 +526,22 @@ class GatedLinear(nn.Module):
 class GatedShift(nn.Module):
     """The gated block with weights of powers of two: ``layer`` is one ``LinearShift`` (``shift_type`` ``'PS'``) or ``LinearShiftQ``
     (``'Q'``) of twice the width, whose float path's weights go into :func:`gated_linear`; straight-through gradients reach its
-    parameters.  With ``use_kernel`` (no gradients) the layer runs on the shift kernels, and the gate behind it."""
+    parameters.  With ``use_kernel`` (no gradients) the layer runs on the shift kernels, and the gate behind it.  A ``layer`` that
+    is there already is taken as it is."""
 
-    def __init__(self, in_features, out_features, bias=True, activation="silu", shift_type="PS", **options):
+    def __init__(self, in_features, out_features, bias=True, activation="silu", shift_type="PS", layer=None, **options):
         super().__init__()
         if shift_type not in ("PS", "Q"):
             raise ValueError("shift_type must be 'PS' or 'Q', is %r" % (shift_type,))
         _activation(activation)
         self.in_features, self.out_features, self.activation = in_features, out_features, activation
-        kind = modules.LinearShift if shift_type == "PS" else modules_q.LinearShiftQ
-        self.layer = kind(in_features, 2 * out_features, bias=bias, **options)
+        if layer is None:
+            kind = modules.LinearShift if shift_type == "PS" else modules_q.LinearShiftQ
+            layer = kind(in_features, 2 * out_features, bias=bias, **options)
+        elif (layer.in_features, layer.out_features) != (in_features, 2 * out_features):
+            raise ValueError("layer must have %d features and give %d, has %d and gives %d" % (
+                in_features, 2 * out_features, layer.in_features, layer.out_features))
+        self.layer = layer
 
     def forward(self, x):
         layer = self.layer
