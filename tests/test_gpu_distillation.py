@@ -655,3 +655,23 @@ def test_frequent_words_of_small_vocabularies(T):
             print(T, V, flush=True)
             _check(h, w, b, ids, logits, c, torch.ones(T, device=DEV), rows, dh, dw, db)
             _check_frequent(h, w, b, ids, logits, c, often, dw)
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+def test_gradients_that_lie_in_other_ways(dtype):
+    # of single losses: what a sum, a mean, a part of them or a repeated one hands back
+    h, w, b, ids, logits = _case(4 * 15, 40, 300, 6, dtype, True, 46)
+    for make in (lambda loss: loss.sum(), lambda loss: loss.mean(), lambda loss: loss.t()[::2].sum(),
+                 lambda loss: loss[:1].expand(5, 15).sum(), lambda loss: (loss.t() @ torch.ones(4, 2, device=DEV)).sum()):
+        leaves = [t.detach().requires_grad_() for t in (h, w, b)]
+        loss = training.linear_distillation(leaves[0].view(4, 15, 40), leaves[1], ids.view(4, 15, 6), logits.view(4, 15, 6), leaves[2],
+                                            reduction="none")
+        given, = torch.autograd.grad(make(loss), loss, retain_graph=True)
+        got = torch.autograd.grad(make(loss), leaves)
+        _check(h, w, b, ids, logits, 1.0, given.reshape(-1), loss.detach().reshape(-1), *got)
+    # a single token without an axis of its own
+    leaves = [t.detach().requires_grad_() for t in (h[3], w, b)]
+    loss = training.linear_distillation(leaves[0], leaves[1], ids[3], logits[3], leaves[2], 2.0)
+    assert loss.shape == ()
+    got = torch.autograd.grad(loss, leaves)
+    _check(h[3:4], w, b, ids[3:4], logits[3:4], 2.0, torch.ones(1, device=DEV), loss.detach()[None], got[0][None], got[1], got[2])

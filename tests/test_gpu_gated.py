@@ -404,3 +404,50 @@ def test_refusals_on_the_gpu():
     dx, = torch.autograd.grad(training.gated_linear(x, w).sum(), x, create_graph=True)
     with pytest.raises(RuntimeError):
         dx.sum().backward()
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("kind", KINDS)
+def test_activations_on_the_same_inputs_every_time(dtype, kind):
+    # (strings hash to other numbers in every process: seeds are numbers)
+    x, w, b, grad = _case(200, 96, 160, dtype, True, KINDS.index(kind), 61)
+    _check(x, w, b, kind, grad, *_step(x, w, b, kind, grad))
+    x, w, b, grad = _case(40, 64, 64, dtype, True, KINDS.index(kind), 62)
+    x = x * 12
+    _check(x, w, b, kind, grad, *_step(x, w, b, kind, grad))
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("kind", KINDS)
+def test_infinite_operands(dtype, kind):
+    # infinities of x, of either half's weights, of both and of a bias: results as the formula has them, the others as ever
+    for T, D, F, tiles in ((90, 72, 40, (None, 0, 1, 2, 3)), (3, 200, 50, (None,)), (40, 1024, 4096, (None,)), (300, 257, 129, (None,))):
+        x, w, b, _ = _case(T, D, F, dtype, True, KINDS.index(kind), 63)
+        inf = float("inf")
+        x[T // 2, 5], x[1, D - 1] = inf, -inf
+        w[6, 7], w[F + 9, 5], w[F - 1, D - 1], b[F + 11], b[3] = -inf, inf, inf, inf, -inf
+        z = x.double() @ w.double().t().contiguous() + b.double()
+        want = FUNCTIONS[kind](z[:, :F]) * z[:, F:]
+        for tile in tiles:
+            print(T, D, F, tile, flush=True)
+            with Tune(vocab_tile=tile):
+                out = training.gated_linear(x, w, b, kind)
+            assert torch.equal(out.isnan(), want.isnan())
+            assert torch.equal(out.isposinf(), want.isposinf()) and torch.equal(out.isneginf(), want.isneginf())
+            rows = [t for t in range(T) if t not in (T // 2, 1)]
+            units = [f for f in range(F) if f not in (6, 9, F - 1, 11, 3)]
+            both = units + [F + f for f in units]
+            _check(x[rows], w[both], b[both], kind, None, out[rows][:, units])
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+def test_gradients_that_lie_in_other_ways(dtype):
+    # what a sum, a mean, a transposed or a repeated result hands back
+    x, w, b, grad = _case(60, 40, 24, dtype, True, 64)
+    for make in (lambda out: out.sum(), lambda out: (out.t() * grad.t()).sum(), lambda out: out[:, :1].sum(),
+                 lambda out: (out.unsqueeze(0) * grad).sum() + out.mean()):
+        leaves = [t.detach().requires_grad_() for t in (x, w, b)]
+        out = training.gated_linear(*leaves)
+        given, = torch.autograd.grad(make(out), out, retain_graph=True)
+        got = torch.autograd.grad(make(out), leaves)
+        _check(x, w, b, "silu", given, out.detach(), *got)

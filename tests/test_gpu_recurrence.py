@@ -344,3 +344,20 @@ def test_second_derivatives_are_refused():
     dx, = torch.autograd.grad(training.gated_recurrence(x, gate)[0].sum(), x, create_graph=True)
     with pytest.raises(RuntimeError):
         dx.sum().backward()
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+def test_gradients_that_lie_in_other_ways(dtype):
+    # what a sum, a mean, a transposed or a repeated result hands back, of even and odd channels
+    for B, T, D in ((3, 70, 66), (2, 9, 5), (1, 300, 1), (4, 1, 130)):
+        g = _gen(B, T, D, 71)
+        x, gate, state = _rand(g, B, T, D, dtype=dtype), _rand(g, B, T, D, dtype=dtype, shift=1.0), _rand(g, B, D)
+        weight = _rand(g, B, T, D, dtype=dtype)
+        for make in (lambda out, last: out.sum() + last.sum(), lambda out, last: (out.transpose(0, 1) * weight.transpose(0, 1)).sum(),
+                     lambda out, last: out.mean(1).sum() + last[:, :1].sum(), lambda out, last: out[:, -1:].expand(B, 3, D).sum(),
+                     lambda out, last: (out.transpose(1, 2) @ weight.float().to(dtype)).sum() if dtype == torch.float32 else last.t().sum()):
+            leaves = [t.detach().requires_grad_() for t in (x, gate, state)]
+            out, last = training.gated_recurrence(*leaves)
+            given = torch.autograd.grad(make(out, last), (out, last), retain_graph=True, allow_unused=True)
+            got = torch.autograd.grad(make(out, last), leaves)
+            _check(x, gate, state, None, given[0], given[1], [out.detach(), last.detach()] + list(got))

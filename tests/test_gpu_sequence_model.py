@@ -5,7 +5,7 @@ import pytest
 import torch
 import torch.nn.functional as F
 
-from deepshift_amd import modules, train_tokens, training
+from deepshift_amd import convert, modules, train_tokens, training
 
 pytestmark = pytest.mark.gpu
 DEV = torch.device("cuda:0")
@@ -193,3 +193,24 @@ def test_words_are_packed_again_behind_a_float_pass(kind):
     layer.conc_weight = given = fresh.packed_weights()
     layer(x)
     assert layer.packed_weights() is given
+
+
+@pytest.mark.parametrize("shift_type", ["PS", "Q"])
+def test_converted_gated_blocks(shift_type):
+    # a float block, converted: its float path is the block with rounded weights, its kernels give the same in fixed point
+    torch.manual_seed(6)
+    with DEV:
+        block = training.GatedLinear(48, 40, activation="gelu")
+    x = torch.randn(5, 9, 48, device=DEV)
+    plain, _ = convert.convert_to_shift(torch.nn.Sequential(copy.deepcopy(block)), 9, shift_type, convert_weights=True)
+    fixed, _ = convert.convert_to_shift(torch.nn.Sequential(copy.deepcopy(block)), 9, shift_type, convert_weights=True, use_kernel=True)
+    layer = plain[0].layer
+    z = F.linear(layer.float_input(x).double(), layer.float_weight().double(), layer.bias.double())
+    want = F.gelu(z[..., :40]) * z[..., 40:]
+    with torch.no_grad():
+        # 48 products and a bias in 32 bits, an activation's slope of 1.13, sizes of up to 20
+        assert (plain(x).double() - want).abs().max() <= 1e-4
+        # inputs and biases off by 2^-16, times 48 weights of 1/4 at most, slopes and factors of up to 20
+        assert (fixed(x).double() - want).abs().max() <= 2.0 ** -16 * 13 * 2 * 20
+    grads = torch.autograd.grad(plain(x).sum(), list(plain.parameters()))
+    assert all(g.isfinite().all() for g in grads) and any((g != 0).any() for g in grads)
