@@ -38,7 +38,9 @@ struct Back {
     int words;
     float *bias_part;     // [workgroups along T][2 F], or NULL
     // float16: dz is held times a power of two that brings the largest to the upper end of its range (loss gradients are small:
-    // those below 2^-14 would lose bits, those below 2^-24 everything)
+    // those below 2^-14 would lose bits, those below 2^-24 everything).  One for all rows: a row whose largest is r times that of all
+    // is off by up to 2^-39 / r of its own, which is more than its rounding, 2^-11, below r = 2^-28; dx itself, from the same
+    // weights, has 30 powers of two from float16's largest to the least with all bits.
     float *tops;          // the largest finite |dz| of each workgroup of top_kernel, `top_groups` of them
     int top_groups;
     float *factor;        // what the results are multiplied with, but for kProbScale

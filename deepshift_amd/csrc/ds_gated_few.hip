@@ -2,7 +2,7 @@
 //
 // Reading the weights is what counts then.  A wave has both halves' rows of one or two results, its lanes share the features, and
 // every weight is loaded once, as it lies, and multiplied in vector registers in 32 bits; the tokens come from the caches.  One token
-// of 4096 features, 8192 results: bfloat16 26 us, 5.2 TB/s, float32 48 us, 5.6 TB/s (a copy of 2 GiB runs at 5.0).  Which numbers of
+// of 4096 features, 8192 results: bfloat16 26 us, 5.2 TB/s, float32 48 us, 5.6 TB/s (a copy of 2 GiB runs at 4.9).  Which numbers of
 // tokens come here, and what they take otherwise, is measured at most_few (ds_gated.hip).
 #include "ds_gated.h"
 

@@ -11,8 +11,10 @@
 // states, which are formed again from those that the forward pass leaves of every workgroup's first tokens.
 // States, products and sums are float32; results are rounded once.
 //
-// Bound by memory: 8 sequences of 8192 tokens and 4096 channels, bfloat16, forward in 410 us, 3.9 TB/s, backward in 654, 4.1 TB/s,
-// where a copy of 0.5 GB runs at 4.3.  What that took: loads that are as many in every turn and stores that leave through a
+// Bound by memory: 8 sequences of 8192 tokens and 4096 channels, bfloat16, forward in 350 to 410 us (cards differ), 3.9 to 4.6 TB/s,
+// backward in 570 to 654, 4.1 to 4.7 TB/s, where a copy of 2 GiB runs at 4.9; 2048 channels of float32 in 336 and 530.  Sequences that
+// end early take hardly less, since the longest one's workgroups are waited for (half of the tokens: 352 and 568, float32 312 and
+// 458, on one card).  What that took: loads that are as many in every turn and stores that leave through a
 // descriptor, so that nothing but the loads of a turn is waited for (with conditions around both, and 16 waves a workgroup,
 // whose registers spilled, the two took 2.9 ms together).
 //
@@ -383,6 +385,8 @@ inline Plan plan_of(int64_t B, int64_t T, int64_t D, int type, bool pairs)
     //   2 x 4096 x 4096          110, 184  (4: 89, 123)     153, 257        (4: 82, 120, 8: 67, 112, 16: 70, 117)
     //   1 x 65536 x 2048        1856, 2662 (16: 342, 448)  2404, 3925       (16: 329, 439, 32: 294, 429, 64: 292, 462)
     //   1 x 1024 x 1024           30, -    (8: 11)           41, -          (8: 12)
+    //   3 x 4096 x 4096          132, 191  (4: 117, 168, 8: 114, 165, 16: 121, 178), where one channel a lane leaves a quarter of
+    // the CUs without work, and the rule cuts nothing.
     const bool two = workgroups(2) >= cus || (2 * workgroups(1) <= cus && workgroups(2) * (p.blocks / 2) >= 2 * cus);
     p.V = type != DS_F32 && pairs && two ? 2 : 1;
     p.groups = (int)((D + 64 * p.V - 1) / (64 * p.V));

@@ -6,7 +6,9 @@ norm.
 The layers between are ``LinearShift`` / ``LinearShiftQ`` on their float path, whose straight-through gradients
 (``ste.py``) reach shifts and signs unscaled -- the reason to clip them.  Everything here runs in the gfx950 library, on the
 current stream of the tensors' device, on float32, bfloat16 and float16; sums are held in 32 bits or more and rounded once,
-and a call repeats bit for bit.  There is no CPU path: a CPU tensor raises.
+and a call repeats bit for bit.  In 16-bit types the matrix instructions take gradients in that type too: probabilities of a
+vocabulary, and the gradient of a gated block's projections, are rounded to it before the products that they go into (but for
+:func:`linear_distillation`'s frequent words in bfloat16, which keep what that loses).  There is no CPU path: a CPU tensor raises.
 
 Functions whose names end in ``_grad`` return gradients directly; the others, but for the clipping, take part in autograd.  All
 can be captured into a graph; where ``backward()`` is, no graph recorded eagerly from the same parameters may be alive (PyTorch
@@ -258,7 +260,8 @@ def linear_distillation(hidden, weight, teacher_ids, teacher_logits, bias=None, 
 
     ``hidden`` ``[..., D]``, ``weight`` ``[V, D]`` and ``bias`` ``[V]`` are of one type; ``teacher_ids`` ``[..., K]`` (int64 or int32)
     and ``teacher_logits`` ``[..., K]`` (float32, bfloat16 or float16) name 1 to 1024 words for every token, in any order; they get no
-    gradient.  A place with a negative number or a logit of ``-inf`` holds none, and a word in two places has both shares.  The
+    gradient.  A place with a negative number or a logit of ``-inf`` holds none.  A word in two places has both shares, and each
+    place its own ``q log q`` in the loss, which is no longer the words' divergence then.  The
     loss is float32: per token with ``reduction='none'``, else their sum, or their mean over the tokens that have a word; tokens
     without one have loss 0 and leave nothing in any gradient.  A number of ``V`` or more, or a logit that is NaN or ``inf``, gives
     NaN."""
@@ -322,7 +325,7 @@ def gated_linear(x, weight, bias=None, activation="silu"):
     product in one kernel: ``weight`` ``[2 F, D]`` is ``gate`` above ``up`` and ``bias`` ``[2 F]`` ``b`` before ``c`` -- what one
     linear layer, or one ``LinearShift``, of ``2 F`` features holds.  ``x`` ``[..., D]``, all of one type; ``activation`` is
     ``'silu'``, ``'gelu'`` (by the error function), ``'relu'`` or ``'sigmoid'``.  For gradients both projections are kept, in
-    32 bits."""
+    32 bits; their own gradient is rounded to the type once, for the products that make those of ``x`` and ``weight`` of it."""
     activation = _activation(activation)
     if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or (bias is not None and bias.requires_grad)):
         return _GatedLinear.apply(x, weight, bias, activation)

@@ -568,9 +568,9 @@ int ds_vocab_loss_step(const void *hidden, int64_t ldh, const void *weight, int6
                        size_t workspace_bytes, ds_stream_t stream);
 
 /* Distillation of a linear head from a teacher's best words: with p = softmax((hidden weight^T + bias) / temperature) and q the
- * softmax of logits[t][:] / temperature over the words ids[t][:] (K = `words` of each token, 1 to 1024, in any order, a word's
- * share being the sum of its places'),
- *   rows[t] = temperature^2 sum_k q_k (log q_k - log p_k).
+ * softmax of logits[t][:] / temperature over the words ids[t][:] (K = `words` of each token, 1 to 1024, in any order),
+ *   rows[t] = temperature^2 sum_k q_k (log q_k - log p_k),
+ * the sum going over places: a word in two of them has both shares in the gradients, and a term for each in rows.
  * A place with a negative number or a logit of -inf holds no word; a token without words does not count: its loss is 0 and it
  * leaves nothing in the gradients.  A number of V or more, or a logit that is NaN or +inf, makes the token's loss and gradients NaN.
  * ids are int32 or int64 (id_bytes 4 or 8), logits of type logits_type, temperature from 2^-20 to 2^20; everything else as
