@@ -83,8 +83,12 @@ class _PackedWeightsMixin:
     def _clamp_shift(self):
         """Holds the shifts of the float path to their range where they are: a captured graph that runs the layer reads and writes
         the parameter's own memory at every replay.  Packed words are built again behind it, as behind any change."""
-        with torch.inference_mode():   # (also a parameter that was made there)
-            self.shift.data.clamp_(*self.shift_range)
+        shift = self.shift.data
+        if shift.is_contiguous() or all(n < 2 or stride for n, stride in zip(shift.shape, shift.stride())):
+            with torch.inference_mode():   # (also a parameter that was made there)
+                shift.clamp_(*self.shift_range)
+        else:   # an expanded one has no memory for each of its elements
+            self.shift.data = shift.clamp(*self.shift_range)
         if self._packed_from is not None:
             object.__setattr__(self, "_packed_from", ())
 

@@ -44,3 +44,16 @@ def test_parameters_made_without_gradients_and_passes_without_them(make):
         layer(_input(layer))
     layer(_input(layer)).sum().backward()
     assert _parameter(layer).grad is not None
+
+
+def test_an_expanded_parameter_is_taken_as_it_was():
+    layer = modules.LinearShift(6, 4)
+    layer.shift = torch.nn.Parameter(torch.full((1, 6), -90.0).expand(4, 6))
+    same = modules.LinearShift(6, 4)
+    same.load_state_dict(layer.state_dict())
+    x = torch.randn(3, 6)
+    assert torch.equal(layer(x), same(x)) and (layer.shift == layer.shift_range[0]).all()
+    # rows of another order have memory of their own
+    layer.shift = torch.nn.Parameter(torch.full((6, 4), -90.0).t())
+    at = layer.shift.data_ptr()
+    assert torch.equal(layer(x), same(x)) and layer.shift.data_ptr() == at
