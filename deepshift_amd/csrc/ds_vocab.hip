@@ -194,7 +194,7 @@ __device__ __forceinline__ void add_to_total(const Rows &r, double loss, double 
 // has them; of 65 to 8192 tokens over 1000 words by 0.16, over 2000 by 0.21, over 4096 by 0.32).  So P keeps its rounding's remainder
 // for groups of 256 words that hold such a word, and the weights' gradient takes both: 0.03 to 0.1 of it then over 65536 words,
 // whose step of 8192 x 4096 takes 11.2 ms instead of 10.9; the workspace holds P and the hidden states twice.  A single word's P is
-// near -1, which rounds to itself.
+// near -1, which rounds to itself.  Words that only the student finds likely, token for token, are rounded as the cross entropy's are.
 //
 // Up to kTwiceAll tokens, which costs nothing beside the weights, and up to kTwiceWords words all groups have it: less than 0.001 of
 // the root mean square there.  A step in us without it, with groups that are looked for, and with all:
@@ -208,7 +208,8 @@ constexpr int64_t kTwiceAll = 64, kTwiceWords = 4096;
 struct Marks {
     const int *sorted;
     const float *taught;
-    const int *target;   // [T] 0: the token counts
+    const int *target;   // [T] 0: the token counts,
+    const float *grad;   // [T] unless this is 0; or NULL
     int64_t T, V;
     int K;
     uint8_t *twice;      // [groups of 256 words]
@@ -217,7 +218,7 @@ struct Marks {
 // By one workgroup, while others join the rows: of up to 512 tokens and 16384 words, one of every stretch of tokens, the words' sums of
 // squared probabilities, whole numbers of 2^-20, in two tables by a hash of the word each.  A word whose sums are a hundred-and-twenty-eighth of
 // all in both of them marks its group: all that have as much themselves, and one of some 10000 others that share their places with
-// such words in both.  A stretch's token is its first that counts, looked for from a place that moves by the golden ratio from stretch
+// such words in both.  A stretch's token is its first that counts and has a gradient, looked for from a place that moves by the golden ratio from stretch
 // to stretch: at the same place of each, tokens of equal sequences would all stand at one place of theirs.
 __device__ __forceinline__ void mark_heavy(const Marks &m)
 {
@@ -243,7 +244,7 @@ __device__ __forceinline__ void mark_heavy(const Marks &m)
             for (int k = 0; k < kAhead; ++k) {
                 at[k] = from + min(j + k, count - 1);
                 at[k] = first + (at[k] < count ? at[k] : at[k] - count);
-                target[k] = m.target[at[k]];
+                target[k] = m.grad && m.grad[at[k]] == 0.f ? -1 : m.target[at[k]];
             }
 #pragma unroll
             for (int k = kAhead - 1; k >= 0; --k) found = target[k] == 0 ? at[k] : found;
@@ -943,9 +944,9 @@ inline bool joined_later(const Call &c, const Plan &p, int tiles)
     return p.keep && p.pieces == 1 && c.T <= 128 && tiles <= 64 && c.teacher.K <= 64 && p.again != 1;
 }
 
-inline Marks marks_of(const Call &c, const Plan &p)
+inline Marks marks_of(const Call &c, const Plan &p, const float *row_grad)
 {
-    return Marks{c.teacher.sorted, c.teacher.taught, c.teacher.target, c.T, c.V, c.teacher.K, (uint8_t *)(c.ws + p.twice)};
+    return Marks{c.teacher.sorted, c.teacher.taught, c.teacher.target, row_grad, c.T, c.V, c.teacher.K, (uint8_t *)(c.ws + p.twice)};
 }
 
 // One product, of `kind`, by the kernels of the plan; fills in the tile counts.
@@ -988,7 +989,7 @@ int loss(const Call &c, const Plan &p, bool counted_only, Operands<P> &o, int re
                lse, rows, reduction, (Share *)(c.ws + p.shares), (uint32_t *)(c.ws + p.arrived), total, c.teacher.taught, c.teacher.K,
                c.teacher.K ? c.teacher.temperature : 1.f};
     const unsigned groups = (unsigned)((c.T + kRowsJoined - 1) / kRowsJoined);
-    if (p.again == 1) hipLaunchKernelGGL(row_kernel<true>, dim3(groups + 1), dim3(1024), 0, c.st, *of, marks_of(c, p));
+    if (p.again == 1) hipLaunchKernelGGL(row_kernel<true>, dim3(groups + 1), dim3(1024), 0, c.st, *of, marks_of(c, p, nullptr));
     else if (!joined_later(c, p, tiles)) hipLaunchKernelGGL(row_kernel<false>, dim3(groups), dim3(1024), 0, c.st, *of, Marks{});
     return launch_status();
 }
@@ -1143,7 +1144,7 @@ int run(Call c, int what, const Outputs &out)
     if (c.teacher.K && c.T > 0) {
         if (what & kLoss) o.untaught = true;
         else launch_teacher(c.teacher, c.st);
-        if (!(what & kLoss) && p.again == 1) hipLaunchKernelGGL(mark_kernel, dim3(1), dim3(1024), 0, c.st, marks_of(c, p));
+        if (!(what & kLoss) && p.again == 1) hipLaunchKernelGGL(mark_kernel, dim3(1), dim3(1024), 0, c.st, marks_of(c, p, out.grads.row_grad));
     }
     Rows of{};
     if (what & kLoss) DS_TRY(loss<P>(c, p, what & kGrad, o, out.reduction, out.rows, out.lse, out.total, &of));

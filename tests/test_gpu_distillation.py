@@ -675,3 +675,17 @@ def test_gradients_that_lie_in_other_ways(dtype):
     assert loss.shape == ()
     got = torch.autograd.grad(loss, leaves)
     _check(h[3:4], w, b, ids[3:4], logits[3:4], 2.0, torch.ones(1, device=DEV), loss.detach()[None], got[0][None], got[1], got[2])
+
+
+def test_frequent_words_of_tokens_whose_loss_is_used():
+    # single losses times a mask of zeros and ones, as a program forms their mean over answers without their prompts
+    T, D, V, K, c, often = 512, 1000, 5003, 256, 1.3, [4999, 2321, 300]
+    h, w, b, ids, logits = _frequent(T, D, V, K, often, 4.0, 47)
+    logits[:, 3:] = logits[:, 3:] / 3 - 2
+    mask = (torch.arange(T, device=DEV) % 64 == 63).float()
+    ids[mask == 0] = torch.randint(600, 1800, (int((mask == 0).sum()), K), generator=_gen(48)).to(DEV)
+    rows = training.linear_distillation(h, w, ids, logits, b, c, "none")
+    _, dh, dw, db = _autograd(h, w, ids, logits, b, c, "none", mask)
+    _check(h, w, b, ids, logits, c, mask, rows, dh, dw, db)
+    kept = mask == 1
+    _check_frequent(h[kept], w, b, ids[kept], logits[kept], c, often, dw)
