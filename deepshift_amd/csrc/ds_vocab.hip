@@ -215,11 +215,12 @@ struct Marks {
     uint8_t *twice;      // [groups of 256 words]
 };
 
-// By one workgroup, while others join the rows: of up to 512 tokens and 16384 words, one of every stretch of tokens, the words' sums of
-// squared probabilities, whole numbers of 2^-20, in two tables by a hash of the word each.  A word whose sums are a hundred-and-twenty-eighth of
-// all in both of them marks its group: all that have as much themselves, and one of some 10000 others that share their places with
-// such words in both.  A stretch's token is its first that counts and has a gradient, looked for from a place that moves by the golden ratio from stretch
-// to stretch: at the same place of each, tokens of equal sequences would all stand at one place of theirs.
+// By one workgroup, while others join the rows (8192 tokens of 64 words: 55 us instead of 22, by itself 30): of up to 512 tokens and
+// 16384 words, one token of every stretch, the words' sums of squared probabilities, whole numbers of 2^-20, in two tables by a hash
+// of the word each.  A word whose sums are a hundred-and-twenty-eighth of all in both of them marks its group: all that have as much
+// themselves, and one of some 10000 others that share their places with such words in both.  A stretch's token is its first that
+// counts and has a gradient, looked for from a place that moves by the golden ratio from stretch to stretch: at the same place of
+// each, tokens of equal sequences would all stand at one place of theirs.
 __device__ __forceinline__ void mark_heavy(const Marks &m)
 {
     constexpr int kBuckets = 4096, kSample = 512;
